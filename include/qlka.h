@@ -224,6 +224,69 @@ int qlka_layer_fwd_masked(int kind, const float* q, const float* k, const float*
                           int P, int D, int N, int M, int C, void* ws, size_t ws_bytes, void* stream);
 
 /*
+ * Softmax attention to a sequence of another length, and the learned relative position bias by buckets. No counterpart in
+ * the reference's operators: its "softmax" baseline is torch's scaled_dot_product_attention
+ * (Experiments/kernel_attention/attention.py:99-102), for which it has no position bias.
+ *
+ *   S[b,h,m,n] = scale <q[b,h,m], k[b,h/(H/G),n]> + table[bucket(n - (m + start))][h]      (table may be NULL: no bias)
+ *   out[b,h,m] = sum_n P[m,n] v[b,h/(H/G),n],  P = softmax of S over the keys that the query sees
+ * A query sees key n if keep[b][n] is nonzero (keep may be NULL) and, with causal, n <= m + start. A row that sees no key
+ * (or only scores of -inf) gives zeros, here and in every gradient. Masked keys' rows are not read. Sums, the softmax's
+ * statistics and every sum of the gradients are fp32; with QLKA_BF16 the probabilities and dS are rounded to bf16 for their
+ * matrix products, and each result once at its end.
+ *
+ * q (B, H, M, D), k and v (B, G, N, D) with H a multiple of G; D up to 128, its elements contiguous; *_stride are the
+ * distances in elements between batches, heads and rows (a dimension of size 1: any value). keep is rows of N bytes,
+ * keep_stride bytes apart. M and N may be 0.
+ *
+ * Buckets: a side's bucket i holds the distances from border[i - 1] up to below border[i] (bucket 0 from 0 on, the last one
+ * without end); border is non-decreasing and positive, on the host. bidirectional: distance |d| for d = n - (m + start),
+ * keys after the query (d > 0) in buckets num_borders + 1 on, 2 (num_borders + 1) buckets in all. Else distance max(-d, 0)
+ * and num_borders + 1 buckets. table and g_table are (buckets, H) fp32, contiguous.
+ *
+ * Forward: writes out and, where not NULL, lse (B, H, M) (log2 of each row's sum, +inf for a row without keys) and out_lo
+ * (with QLKA_BF16 and a table: what rounding out cut off, same strides as out; the probabilities are then taken to 16 bits).
+ * Backward: reads q, k, v, out, lse, g_out and, where not NULL, out_lo, writes g_q (may be NULL), g_k and g_v (both or neither
+ * NULL) and g_table (may be NULL; with QLKA_BF16 it needs out_lo). No atomics: results do not change from run to run.
+ */
+#define QLKA_F32  0
+#define QLKA_BF16 1
+#define QLKA_MAX_BUCKETS 256
+typedef struct qlka_softmax_args {
+    int dtype, B, H, G, M, N, D;
+    int causal, start;
+    float scale;
+    const void *q, *k, *v;
+    int64_t q_stride[3], k_stride[3], v_stride[3];
+    const uint8_t* keep;
+    int64_t keep_stride;
+    const float* table;
+    const int* border;
+    int num_borders, bidirectional;
+    void *out, *out_lo;
+    int64_t out_stride[3];
+    float* lse;
+    const void* g_out;
+    int64_t g_out_stride[3];
+    void *g_q, *g_k, *g_v;
+    int64_t g_q_stride[3], g_k_stride[3], g_v_stride[3];
+    float* g_table;
+} qlka_softmax_args;
+size_t qlka_softmax_fwd_ws_bytes(const qlka_softmax_args* args);
+int qlka_softmax_fwd(const qlka_softmax_args* args, void* ws, size_t ws_bytes, void* stream);
+size_t qlka_softmax_bwd_ws_bytes(const qlka_softmax_args* args);
+int qlka_softmax_bwd(const qlka_softmax_args* args, void* ws, size_t ws_bytes, void* stream);
+/*
+ * The bias as a map, out (H, M, N) fp32 with out[h,m,n] = table[bucket(n - (m + start))][h], and its gradient, g_table
+ * (buckets, H) = the sums of g (H, M, N) over each bucket.
+ */
+int qlka_bias_map_fwd(const float* table, const int* border, int num_borders, int bidirectional, float* out, int H, int M,
+                      int N, int start, void* stream);
+size_t qlka_bias_map_bwd_ws_bytes(int num_borders, int bidirectional, int H, int M, int N);
+int qlka_bias_map_bwd(const float* g, const int* border, int num_borders, int bidirectional, float* g_table, int H, int M,
+                      int N, int start, void* ws, size_t ws_bytes, void* stream);
+
+/*
  * Test entry: stable ascending sort of num_segs contiguous segments of seg_len fp32 keys; perm[i] is the in-segment
  * index of the i-th smallest key (np.argsort(kind="stable"); -0.0 ties +0.0 and is written as +0.0).
  * Replaces launch_iota + launch_cub_sort (Weighted_Abs_Sum/csrc/sort_utils.cu:85-117).

@@ -1,0 +1,97 @@
+// The relative position bias by buckets as a map: out[h, m, n] = table[bucket(n - (m + start))][h], and its gradient, the sums
+// of the map's gradient over each bucket. Both are bound by the map's bytes. The map is constant along its diagonals: a
+// workgroup finds the bucket of each diagonal of its tile once, and writes rows as windows of one array in LDS.
+#include "softmax_tile.h"
+
+namespace qlka {
+namespace sm {
+
+constexpr int MAP_ROWS = 64, MAP_COLS = 1024, MAP_T = 256;
+
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));   // rows start at any float
+
+__global__ __launch_bounds__(MAP_T) void map_fwd(const float* table, const SmBuckets bk, float* out, int H, int M, int N,
+                                                 int start) {
+    __shared__ float along[MAP_ROWS + MAP_COLS];
+    __shared__ int border[QLKA_MAX_BUCKETS];
+    const int n0 = blockIdx.x * MAP_COLS, m0 = blockIdx.y * MAP_ROWS, h = blockIdx.z, tid = threadIdx.x;
+    const int rows = min(MAP_ROWS, M - m0), cols = min(MAP_COLS, N - n0);
+    for (int i = tid; i < bk.n; i += MAP_T) border[i] = bk.border[i];
+    __syncthreads();
+    const int lo = n0 - (m0 + rows - 1) - start;
+    for (int i = tid; i < rows + cols - 1; i += MAP_T)
+        along[i] = table[(int64_t)bucket_of(border, bk.n, bk.both, lo + i) * H + h];
+    __syncthreads();
+    float* to = out + ((int64_t)h * M + m0) * N + n0;
+    const int c = 4 * tid;
+    for (int r = 0; r < rows; ++r, to += N) {
+        const float* a = &along[rows - 1 - r + c];
+        if (c + 3 < cols) {
+            *reinterpret_cast<f32x4u*>(to + c) = f32x4u{a[0], a[1], a[2], a[3]};
+        } else {
+            for (int i = 0; c + i < cols; ++i) to[c + i] = a[i];
+        }
+    }
+}
+
+// A workgroup sums its rows along 1024 diagonals, four a thread, then the diagonals of a bucket.
+__global__ __launch_bounds__(MAP_T) void map_bwd(const float* g, const SmBuckets bk, float* part, int M, int N, int start) {
+    constexpr int PER = MAP_COLS / MAP_T, NW = MAP_T / 64;
+    __shared__ int border[QLKA_MAX_BUCKETS];
+    __shared__ float sums[NW][QLKA_MAX_BUCKETS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m0 = blockIdx.y * MAP_ROWS, h = blockIdx.z;
+    const int rows = min(MAP_ROWS, M - m0), buckets = (bk.n + 1) * (bk.both ? 2 : 1);
+    for (int i = tid; i < bk.n; i += MAP_T) border[i] = bk.border[i];
+    for (int i = lane; i < buckets; i += 64) sums[wave][i] = 0.f;
+    __syncthreads();
+    // diagonal c of row m0 + r is column c + r; columns from -(rows - 1) on
+    const int c0 = blockIdx.x * MAP_COLS - (MAP_ROWS - 1) + tid;
+    const float* from = g + ((int64_t)h * M + m0) * N;
+    float x[PER] = {};
+#pragma unroll 4
+    for (int r = 0; r < rows; ++r, from += N)
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int n = c0 + j * MAP_T + r;
+            if (n >= 0 && n < N) x[j] += from[n];
+        }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        float y = x[j];
+        const int bucket = bucket_of(border, bk.n, bk.both, c0 + j * MAP_T - m0 - start);
+#pragma unroll
+        for (int k = 1; k < 64; k *= 2) {                  // lanes of one bucket are neighbours
+            const float z = __shfl_up(y, k);
+            const int c = __shfl_up(bucket, k);
+            if (lane >= k && c == bucket) y += z;
+        }
+        const int after = __shfl_down(bucket, 1);
+        if (lane == 63 || after != bucket) sums[wave][bucket] += y;
+    }
+    __syncthreads();
+    part += (((int64_t)h * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * buckets;
+    for (int i = tid; i < buckets; i += MAP_T) part[i] = sums[0][i] + sums[1][i] + sums[2][i] + sums[3][i];
+}
+
+static dim3 map_grid(int M, int cols, int H) {
+    return dim3((unsigned)((cols + MAP_COLS - 1) / MAP_COLS), (unsigned)((M + MAP_ROWS - 1) / MAP_ROWS), (unsigned)H);
+}
+
+}  // namespace sm
+
+int bias_map_fwd(const float* table, const SmBuckets& bk, float* out, int H, int M, int N, int start, hipStream_t st) {
+    sm::map_fwd<<<sm::map_grid(M, N, H), sm::MAP_T, 0, st>>>(table, bk, out, H, M, N, start);
+    return (int)hipGetLastError();
+}
+
+int bias_map_blocks(int M, int N) {
+    const dim3 g = sm::map_grid(M, N + sm::MAP_ROWS - 1, 1);
+    return (int)(g.x * g.y);
+}
+
+int bias_map_bwd(const float* g, const SmBuckets& bk, float* part, int H, int M, int N, int start, hipStream_t st) {
+    sm::map_bwd<<<sm::map_grid(M, N + sm::MAP_ROWS - 1, H), sm::MAP_T, 0, st>>>(g, bk, part, M, N, start);
+    return (int)hipGetLastError();
+}
+
+}  // namespace qlka

@@ -701,6 +701,15 @@ int run_bwd_columns(const float* v, const float* g_w, const float* g_u, float sc
 
 }  // namespace
 
+namespace qlka {
+
+int api_error(int code, const char* message) {
+    g_err = message;
+    return code;
+}
+
+}  // namespace qlka
+
 extern "C" {
 
 const char* qlka_last_error(void) { return g_err.c_str(); }

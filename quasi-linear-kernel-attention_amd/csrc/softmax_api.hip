@@ -1,0 +1,326 @@
+// The C ABI of softmax attention and of the bias map (include/qlka.h): validation, the choice of kernel and split, the
+// workspace and the launches.
+#include "qlka.h"
+#include "qlka_internal.h"
+#include "softmax.h"
+
+#include <algorithm>
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+
+using namespace qlka;
+
+namespace {
+
+constexpr int64_t LONGEST = 1 << 28;      // rows, keys, positions: sums of a few stay in 32 bits
+constexpr int64_t MOST_ROWS = INT32_MAX;
+
+int refuse(const char* fmt, ...) {
+    char buf[256];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    return api_error(QLKA_EINVAL, buf);
+}
+
+int status(int e, const char* where) {
+    if (e == 0) return QLKA_OK;
+    char buf[256];
+    snprintf(buf, sizeof(buf), "%s: %s", where, hipGetErrorString((hipError_t)e));
+    return api_error(QLKA_EHIP, buf);
+}
+
+size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+int check_buckets(const int* border, int n, int both, SmBuckets* bk) {
+    const int most = both ? QLKA_MAX_BUCKETS / 2 : QLKA_MAX_BUCKETS;
+    if (n < 0 || n >= most) return refuse("at most %d buckets", QLKA_MAX_BUCKETS);
+    if (n > 0 && !border) return refuse("border must be non-null");
+    bk->n = n;
+    bk->both = both ? 1 : 0;
+    bk->far = 0;
+    for (int i = 0; i < n; ++i) {
+        if (border[i] < 1 || border[i] > LONGEST || border[i] < bk->far)
+            return refuse("border must be positive, non-decreasing and at most 2^28");
+        bk->border[i] = bk->far = border[i];
+    }
+    return QLKA_OK;
+}
+
+int check_sizes(const qlka_softmax_args* a) {
+    if (!a) return refuse("args must be non-null");
+    if (a->dtype != QLKA_F32 && a->dtype != QLKA_BF16) return refuse("dtype must be QLKA_F32 or QLKA_BF16");
+    if (a->B < 0 || a->M < 0 || a->N < 0 || a->H < 1 || a->G < 1) return refuse("B, M and N must be >= 0, H and G >= 1");
+    if (a->H % a->G) return refuse("H must be a multiple of G");
+    if (a->D < 1 || a->D > 128) return refuse("D must be in [1, 128]");
+    if (a->M > LONGEST || a->N > LONGEST || a->start > LONGEST || a->start < -LONGEST)
+        return refuse("M, N and |start| must be <= 2^28");
+    if ((double)a->B * a->H * a->M > (double)MOST_ROWS || (double)a->B * a->G * a->N > (double)MOST_ROWS)
+        return refuse("B * H * M and B * G * N must fit int32");
+    if (!std::isfinite(a->scale)) return refuse("scale must be finite");
+    return QLKA_OK;
+}
+
+// ---- how a call runs
+
+// Splits of an axis of `tiles` tiles so that `groups` workgroups become about `want`, each with `least` tiles or more.
+int splits_for(int64_t groups, int64_t tiles, int64_t want, int64_t least) {
+    if (groups >= want / 2) return 1;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(want, std::max<int64_t>(groups, 1)), tiles / least, 256}));
+}
+
+int tile_rows(const qlka_softmax_args* a) { return a->dtype == QLKA_F32 && a->D > 64 ? 32 : 64; }
+
+struct RowPlan { int waves, blocks, splits; };
+// kernels that own `len` rows of each of `heads` heads and go over `tiles` tiles of the other side
+RowPlan row_plan(int B, int heads, int len, int64_t tiles) {
+    RowPlan r;
+    r.waves = len <= 32 ? 1 : len <= 64 ? 2 : 4;
+    r.blocks = (int)ceil_div(len, 32 * r.waves);
+    r.splits = splits_for((int64_t)B * heads * r.blocks, tiles, 1024, 4);
+    return r;
+}
+
+// Few query rows per key head: the kernel without matrix tiles (softmax_step.hip).
+bool steps(const qlka_softmax_args* a) { return (int64_t)a->H / a->G * a->M <= 8; }
+
+struct FwdPlan { bool step; RowPlan rows; size_t part, part2; };
+FwdPlan fwd_plan(const qlka_softmax_args* a) {
+    FwdPlan f{};
+    f.step = steps(a);
+    if (f.step) f.rows = {0, 0, splits_for((int64_t)a->B * a->G, ceil_div(a->N, 64), 2048, 4)};
+    else f.rows = row_plan(a->B, a->H, a->M, ceil_div(a->N, tile_rows(a)));
+    if (f.rows.splits > 1) {
+        const size_t rows = (size_t)f.rows.splits * a->B * a->H * a->M;
+        f.part = align256(rows * sm_padded(a->D) * 4);
+        f.part2 = align256(rows * 8);
+    }
+    return f;
+}
+
+struct BwdPlan { RowPlan dq, dkv; size_t delta, part, part2, table; };
+BwdPlan bwd_plan(const qlka_softmax_args* a, bool dq, bool dkv, bool table) {
+    BwdPlan w{};
+    const int t = tile_rows(a), DP = sm_padded(a->D);
+    w.delta = align256((size_t)a->B * a->H * a->M * 4);
+    if (dq || table) {
+        w.dq = row_plan(a->B, a->H, a->M, ceil_div(a->N, t));
+        if (w.dq.splits > 1) w.part = align256((size_t)w.dq.splits * a->B * a->H * a->M * DP * 4);
+    }
+    if (table)
+        w.table = align256((size_t)a->H * a->B * w.dq.blocks * w.dq.splits * (a->num_borders + 1) *
+                           (a->bidirectional ? 2 : 1) * 4);
+    if (dkv) {
+        w.dkv = row_plan(a->B, a->G, a->N, ceil_div(a->M, t) * (a->H / a->G));
+        if (w.dkv.splits > 1) {
+            w.part2 = align256((size_t)w.dkv.splits * a->B * a->G * a->N * DP * 4);
+            w.part = std::max(w.part, w.part2);
+        }
+    }
+    return w;
+}
+
+// ---- arguments to kernel parameters
+
+SmStrides strides(const int64_t* s) { return {s[0], s[1], s[2]}; }
+
+bool in_pieces(const qlka_softmax_args* a, const void* x, const int64_t* s, int heads, int rows) {
+    const int64_t piece = a->dtype == QLKA_F32 ? 4 : 8;
+    return a->D % 8 == 0 && (uintptr_t)x % 16 == 0 && (a->B <= 1 || s[0] % piece == 0) &&
+           (heads <= 1 || s[1] % piece == 0) && (rows <= 1 || s[2] % piece == 0);
+}
+
+int params(const qlka_softmax_args* a, SmParams* p) {
+    *p = SmParams{};
+    p->q = a->q; p->k = a->k; p->v = a->v; p->g_out = a->g_out;
+    p->out = a->out; p->out_lo = a->out_lo;
+    p->g_q = a->g_q; p->g_k = a->g_k; p->g_v = a->g_v;
+    p->sq = strides(a->q_stride); p->sk = strides(a->k_stride); p->sv = strides(a->v_stride);
+    p->so = strides(a->out_stride); p->sg = strides(a->g_out_stride);
+    p->sgq = strides(a->g_q_stride); p->sgk = strides(a->g_k_stride); p->sgv = strides(a->g_v_stride);
+    p->keep = a->keep; p->keep_stride = a->keep_stride;
+    p->table = a->table;
+    p->lse = a->lse;
+    p->B = a->B; p->H = a->H; p->G = a->G; p->M = a->M; p->N = a->N; p->D = a->D;
+    p->causal = a->causal ? 1 : 0;
+    p->start = a->start;
+    p->splits = p->blocks = 1;
+    p->scale = std::fabs(a->scale);
+    p->q_sign = std::signbit(a->scale) ? -1.f : 1.f;
+    const auto bit = [&](int v, const void* x, const int64_t* s, int heads, int rows) {
+        return in_pieces(a, x, s, heads, rows) ? v : 0; };
+    p->vec = bit(VEC_Q, a->q, a->q_stride, a->H, a->M) | bit(VEC_K, a->k, a->k_stride, a->G, a->N) |
+             bit(VEC_V, a->v, a->v_stride, a->G, a->N) | bit(VEC_G, a->g_out, a->g_out_stride, a->H, a->M) |
+             bit(VEC_GQ, a->g_q, a->g_q_stride, a->H, a->M) | bit(VEC_GK, a->g_k, a->g_k_stride, a->G, a->N) |
+             bit(VEC_GV, a->g_v, a->g_v_stride, a->G, a->N);
+    if (bit(1, a->out, a->out_stride, a->H, a->M) && (uintptr_t)a->out_lo % 16 == 0) p->vec |= VEC_O;
+    if ((uintptr_t)a->keep % 16 == 0 && (a->B <= 1 || a->keep_stride % 16 == 0)) p->vec |= VEC_KEEP;
+    return a->table ? check_buckets(a->border, a->num_borders, a->bidirectional, &p->bk) : QLKA_OK;
+}
+
+int need_ws(const void* ws, size_t have, size_t need) {
+    if (need == 0) return QLKA_OK;
+    if (!ws || have < need || (uintptr_t)ws % 16) return api_error(QLKA_EWORKSPACE, "workspace too small, null or not aligned to 16 bytes");
+    return QLKA_OK;
+}
+
+int fits_grid(int64_t groups) {
+    return groups <= INT32_MAX ? QLKA_OK : refuse("too many workgroups: B * heads * blocks of rows must fit int32");
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t qlka_softmax_fwd_ws_bytes(const qlka_softmax_args* a) {
+    if (check_sizes(a)) return 0;
+    const FwdPlan f = fwd_plan(a);
+    return f.part + f.part2;
+}
+
+int qlka_softmax_fwd(const qlka_softmax_args* a, void* ws, size_t ws_bytes, void* stream) {
+    api_error(QLKA_OK, "");
+    if (int e = check_sizes(a)) return e;
+    SmParams p;
+    if (int e = params(a, &p)) return e;
+    if (a->B == 0 || a->M == 0) return QLKA_OK;
+    if (!a->q || !a->out || (a->N > 0 && (!a->k || !a->v))) return refuse("q, k, v and out must be non-null");
+    if (a->out_lo && (a->dtype == QLKA_F32 || !a->table)) return refuse("out_lo goes with QLKA_BF16 and a table");
+    const FwdPlan f = fwd_plan(a);
+    if (int e = need_ws(ws, ws_bytes, f.part + f.part2)) return e;
+    if (int e = fits_grid((int64_t)a->B * (f.step ? a->G : a->H) * std::max(f.rows.blocks, 1) * f.rows.splits)) return e;
+    hipStream_t st = (hipStream_t)stream;
+    p.splits = f.rows.splits;
+    p.blocks = f.rows.blocks;
+    p.part = (float*)ws;
+    p.part2 = (float*)((char*)ws + f.part);
+    int e;
+    if (f.step) {
+        StageTimer timer("softmax_step", st);
+        e = sm_step(a->dtype, p, st);
+    } else {
+        StageTimer timer("softmax_fwd", st);
+        e = sm_fwd(a->dtype, p, f.rows.waves, st);
+    }
+    if (e || p.splits == 1) return status(e, "softmax attention");
+    StageTimer timer("softmax_combine", st);
+    return status(sm_combine(a->dtype, p, st), "softmax attention, joining of splits");
+}
+
+size_t qlka_softmax_bwd_ws_bytes(const qlka_softmax_args* a) {
+    if (check_sizes(a)) return 0;
+    const BwdPlan w = bwd_plan(a, a->g_q, a->g_k, a->g_table);
+    return w.delta + w.part + w.part2 + w.table;
+}
+
+int qlka_softmax_bwd(const qlka_softmax_args* a, void* ws, size_t ws_bytes, void* stream) {
+    api_error(QLKA_OK, "");
+    if (int e = check_sizes(a)) return e;
+    SmParams p;
+    if (int e = params(a, &p)) return e;
+    if (!a->g_k != !a->g_v) return refuse("g_k and g_v: both or neither");
+    if (a->g_table && !a->table) return refuse("g_table needs the table");
+    const bool rows = (int64_t)a->B * a->M > 0, keys = (int64_t)a->B * a->N > 0;
+    if (rows && (!a->q || !a->out || !a->lse || !a->g_out)) return refuse("q, out, lse and g_out must be non-null");
+    if (keys && (!a->k || !a->v)) return refuse("k and v must be non-null");
+    if (a->out_lo && (a->dtype == QLKA_F32 || !a->table)) return refuse("out_lo goes with QLKA_BF16 and a table");
+    if (rows && a->g_table && a->dtype == QLKA_BF16 && !a->out_lo) return refuse("g_table needs out_lo with QLKA_BF16");
+    const BwdPlan w = bwd_plan(a, a->g_q, a->g_k, a->g_table);
+    if (int e = need_ws(ws, ws_bytes, w.delta + w.part + w.part2 + w.table)) return e;
+    if (int e = fits_grid((int64_t)a->B * a->H * w.dq.blocks * w.dq.splits)) return e;
+    if (int e = fits_grid((int64_t)a->B * a->G * w.dkv.blocks * w.dkv.splits)) return e;
+    hipStream_t st = (hipStream_t)stream;
+    char* at = (char*)ws;
+    p.delta = (float*)at; at += w.delta;
+    p.part = (float*)at; at += w.part;
+    p.part2 = (float*)at; at += w.part2;
+    p.part_table = (float*)at;
+    if (rows) {
+        StageTimer timer("softmax_delta", st);
+        if (int e = sm_delta(a->dtype, p, st)) return status(e, "softmax attention backward, row sums");
+    }
+    if (!a->g_table) p.part_table = nullptr;
+    if (rows && (a->g_q || a->g_table)) {
+        p.splits = w.dq.splits;
+        p.blocks = w.dq.blocks;
+        {
+            StageTimer timer("softmax_dq", st);
+            if (int e = sm_dq(a->dtype, p, w.dq.waves, st)) return status(e, "softmax attention backward, queries");
+        }
+        if (p.splits > 1 && a->g_q) {
+            StageTimer timer("softmax_sum", st);
+            if (int e = sm_sum_parts(a->dtype, p.part, a->g_q, p.sgq, p.vec & VEC_GQ, a->scale, p.splits, a->B, a->H, a->M,
+                                     a->D, st))
+                return status(e, "softmax attention backward, joining of splits");
+        }
+    }
+    if (a->g_table) {
+        StageTimer timer("softmax_table", st);
+        const int count = rows ? a->B * w.dq.blocks * w.dq.splits : 0;
+        if (int e = sm_sum_table(p.part_table, a->g_table, a->H, count, sm_buckets(p.bk), st))
+            return status(e, "softmax attention backward, table");
+    }
+    if (keys && a->g_k) {
+        p.splits = w.dkv.splits;
+        p.blocks = w.dkv.blocks;
+        {
+            StageTimer timer("softmax_dkv", st);
+            if (int e = sm_dkv(a->dtype, p, w.dkv.waves, st)) return status(e, "softmax attention backward, keys");
+        }
+        if (p.splits > 1) {
+            StageTimer timer("softmax_sum", st);
+            int e = sm_sum_parts(a->dtype, p.part, a->g_k, p.sgk, p.vec & VEC_GK, a->scale, p.splits, a->B, a->G, a->N, a->D, st);
+            if (!e) e = sm_sum_parts(a->dtype, p.part2, a->g_v, p.sgv, p.vec & VEC_GV, 1.f, p.splits, a->B, a->G, a->N, a->D, st);
+            if (e) return status(e, "softmax attention backward, joining of splits");
+        }
+    }
+    return QLKA_OK;
+}
+
+static int check_map(int H, int M, int N, int start) {
+    if (H < 1 || H > 65535) return refuse("H must be in [1, 65535]");
+    if (M < 0 || N < 0 || M > 1 << 21 || N > 1 << 21) return refuse("M and N must be in [0, 2^21]");
+    if (start > LONGEST || start < -LONGEST) return refuse("|start| must be <= 2^28");
+    return QLKA_OK;
+}
+
+int qlka_bias_map_fwd(const float* table, const int* border, int num_borders, int bidirectional, float* out, int H, int M,
+                      int N, int start, void* stream) {
+    api_error(QLKA_OK, "");
+    if (int e = check_map(H, M, N, start)) return e;
+    SmBuckets bk;
+    if (int e = check_buckets(border, num_borders, bidirectional, &bk)) return e;
+    if (M == 0 || N == 0) return QLKA_OK;
+    if (!table || !out) return refuse("table and out must be non-null");
+    StageTimer timer("bias_map", (hipStream_t)stream);
+    return status(bias_map_fwd(table, bk, out, H, M, N, start, (hipStream_t)stream), "bias map");
+}
+
+size_t qlka_bias_map_bwd_ws_bytes(int num_borders, int bidirectional, int H, int M, int N) {
+    if (check_map(H, M, N, 0) || num_borders < 0 || M == 0 || N == 0) return 0;
+    return (size_t)H * bias_map_blocks(M, N) * (num_borders + 1) * (bidirectional ? 2 : 1) * 4;
+}
+
+int qlka_bias_map_bwd(const float* g, const int* border, int num_borders, int bidirectional, float* g_table, int H, int M,
+                      int N, int start, void* ws, size_t ws_bytes, void* stream) {
+    api_error(QLKA_OK, "");
+    if (int e = check_map(H, M, N, start)) return e;
+    SmBuckets bk;
+    if (int e = check_buckets(border, num_borders, bidirectional, &bk)) return e;
+    const bool any = M > 0 && N > 0;
+    if (!g_table || (any && !g)) return refuse("g and g_table must be non-null");
+    if (int e = need_ws(ws, ws_bytes, qlka_bias_map_bwd_ws_bytes(num_borders, bidirectional, H, M, N))) return e;
+    hipStream_t st = (hipStream_t)stream;
+    if (any) {
+        StageTimer timer("bias_map_bwd", st);
+        if (int e = bias_map_bwd(g, bk, (float*)ws, H, M, N, start, st)) return status(e, "bias map backward");
+    }
+    StageTimer timer("softmax_table", st);
+    return status(sm_sum_table((const float*)ws, g_table, H, any ? bias_map_blocks(M, N) : 0, sm_buckets(bk), st),
+                  "bias map backward, table");
+}
+
+}  // extern "C"

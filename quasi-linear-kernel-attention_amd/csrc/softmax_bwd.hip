@@ -1,0 +1,464 @@
+// Softmax attention, backward. With P the probabilities of the forward (formed again from its row statistics),
+//   dV = P^T dO,  dP = dO V^T,  delta = rowsum(dO * O),  dS = P * (dP - delta),  dQ = scale dS K,  dK = scale dS^T Q,
+// and the gradient of a bias bucket is the sum of dS over its scores.
+//
+// Two kernels, each forming P and dP for itself: softmax_dq goes over the keys for 32 queries a wave, softmax_dkv over the
+// queries (of all the heads that share a key head) for 32 keys a wave. That is 7 products instead of the 5 of one pass, and no
+// sum between workgroups: no atomics, results that do not change from run to run. Scores stay in registers as in the
+// forward. Rounding P and dS to bf16 for the products with bf16 operands costs what rounding the results does. For the
+// table's gradient, which is fp32, dS is taken as it is, and delta formed from O to 16 bits (softmax_fwd.hip, FINE).
+#include "softmax_tile.h"
+
+#include <limits>
+
+namespace qlka {
+namespace sm {
+
+constexpr float HIGH = std::numeric_limits<float>::infinity();
+
+// delta: DP / 8 lanes a row
+template <class T, int DP>
+__global__ __launch_bounds__(256) void softmax_delta(const SmParams p) {
+    constexpr int LANES = DP / 8;
+    const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES, rows = (int64_t)p.B * p.H * p.M;
+    const int d = threadIdx.x % LANES * 8;
+    float x = 0.f;
+    if (row < rows) {
+        const int m = (int)(row % p.M), head = (int)(row / p.M % p.H), b = (int)(row / p.M / p.H);
+        const T* out = (const T*)p.out + b * p.so.b + head * p.so.h + m * p.so.r;
+        const auto g = load_seg((const T*)p.g_out + b * p.sg.b + head * p.sg.h + m * p.sg.r, d, p.D, p.vec & VEC_G);
+        const auto o = load_seg(out, d, p.D, p.vec & VEC_O);
+        typename Elem<T>::seg lo = {};
+        if (p.out_lo) lo = load_seg((const T*)p.out_lo + (out - (const T*)p.out), d, p.D, p.vec & VEC_O);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x = __builtin_fmaf((float)g[i], (float)o[i] + (float)lo[i], x);
+    }
+#pragma unroll
+    for (int far = 1; far < LANES; far *= 2) x += __shfl_xor(x, far);
+    if (row < rows && d == 0) p.delta[row] = x;
+}
+
+// Adds a wave's 32 x 32 scores' gradients to the buckets of their distances. A lane holds one query (lane % 32) and 16 keys;
+// for each register the values of 32 queries are turned in the wave until lane t holds the diagonal (key - query) = t or
+// t - 32, so a diagonal's sum gathers in one lane; lanes of one bucket, which are neighbours, are then summed by a segmented
+// scan. base: the distance of the tile's first key and first query. acc: this wave's own, in LDS.
+__device__ __forceinline__ void add_band(f32x16 ds, int base, float* acc, const int* border, const SmBuckets& bk, int lane) {
+    const int t = lane & 31, half = lane >> 5;
+    float pos = 0.f, neg = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int n = reg_row(r) + 4 * half, from = ((n - t) & 31) | (lane & 32);
+        const float x = __int_as_float(__builtin_amdgcn_ds_bpermute(4 * from, __float_as_int(ds[r])));
+        pos += t <= n ? x : 0.f;
+        neg += t <= n ? 0.f : x;
+    }
+    pos += other_half(pos);
+    neg += other_half(neg);
+    float x = half ? pos : neg;
+    const int bucket = bucket_of(border, bk.n, bk.both, base + lane - 32);
+#pragma unroll
+    for (int k = 1; k < 64; k *= 2) {
+        const float y = __shfl_up(x, k);
+        const int c = __shfl_up(bucket, k);
+        if (lane >= k && c == bucket) x += y;
+    }
+    const int after = __shfl_down(bucket, 1);
+    if (lane == 63 || after != bucket) acc[bucket] += x;
+}
+
+template <class T, int DP, int NW, bool BIAS>
+__global__ __launch_bounds__(64 * NW) void softmax_dq(const SmParams p) {
+    constexpr int NP = Elem<T>::PARTS, BN = Shape<T, DP>::BN, NT = 64 * NW, ROWS = 32 * NW, NS = BN / 32, ND = DP / 32;
+    __shared__ Tile<NP, BN, DP> kt, vt;
+    __shared__ BiasLds table;
+    __shared__ float near_bias[BIAS ? ROWS + BN : 1], sums[BIAS ? NW : 1][QLKA_MAX_BUCKETS];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+    int w = xcd_work(blockIdx.x, gridDim.x);
+    const int block = w % p.blocks; w /= p.blocks;
+    const int split_i = w % p.splits; w /= p.splits;
+    const int head = w % p.H, b = w / p.H, kvh = head / (p.H / p.G);
+    const int m0 = block * ROWS, mw = m0 + wave * 32, m = mw + col;
+    const T* k = (const T*)p.k + b * p.sk.b + kvh * p.sk.h;
+    const T* v = (const T*)p.v + b * p.sv.b + kvh * p.sv.h;
+    const bool vk = p.vec & VEC_K, vv = p.vec & VEC_V;
+    const int64_t row = ((int64_t)b * p.H + head) * p.M + m;
+
+    Frag<NP> qf[DP / 16], gf[DP / 16];
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+        typename Elem<T>::seg s = {}, g = {};
+        if (m < p.M) {
+            s = load_seg((const T*)p.q + b * p.sq.b + head * p.sq.h + m * p.sq.r, 16 * c + 8 * half, p.D, p.vec & VEC_Q);
+            g = load_seg((const T*)p.g_out + b * p.sg.b + head * p.sg.h + m * p.sg.r, 16 * c + 8 * half, p.D, p.vec & VEC_G);
+        }
+        if (p.q_sign < 0) s = -s;
+        qf[c] = frag_of(s);
+        gf[c] = frag_of(g);
+    }
+    const float lse = m < p.M ? p.lse[row] : HIGH, delta = m < p.M ? p.delta[row] : 0.f;
+    const int buckets = (p.bk.n + 1) * (p.bk.both ? 2 : 1);
+    float left = 0.f, right = 0.f;                     // this lane's sums far below and far above the diagonal
+    const bool to_table = BIAS && p.part_table;
+    if constexpr (BIAS) {
+        table.fill(p, head, tid, NT);
+        for (int i = lane; i < buckets; i += 64) sums[wave][i] = 0.f;
+        __syncthreads();
+    }
+
+    const int tiles = (p.N + BN - 1) / BN;
+    int t0 = (int)((int64_t)tiles * split_i / p.splits), t1 = (int)((int64_t)tiles * (split_i + 1) / p.splits);
+    if (p.causal) {
+        const int last = min(m0 + ROWS, p.M) - 1 + p.start;
+        t1 = min(t1, last < 0 ? 0 : last / BN + 1);
+    }
+    KeyBits<BN> seen(p, b);
+    Staged<T, DP, BN, NT> ks, vs;
+    const float c2 = p.scale * LOG2E;
+    f32x16 dq[ND] = {};
+
+    int t = seen.next(t0, t1);
+    if (t < t1) {
+        const uint64_t bits = seen.of(t);
+        ks.load(k, p.sk.r, t * BN, bits, p.D, vk, tid);
+        vs.load(v, p.sv.r, t * BN, bits, p.D, vv, tid);
+    }
+    while (t < t1) {
+        const int n0 = t * BN;
+        const uint64_t bits = seen.of(t);
+        float far = 0.f;
+        int fb = -1;
+        __syncthreads();
+        ks.store(kt, tid);
+        vs.store(vt, tid);
+        if constexpr (BIAS) {
+            const int lo = n0 - (m0 + ROWS - 1) - p.start;
+            fb = far_bucket(p.bk, lo, n0 + BN - 1 - m0 - p.start);
+            if (fb < 0) {
+                for (int i = tid; i < ROWS + BN - 1; i += NT)
+                    near_bias[i] = table.value[bucket_of(table.border, p.bk.n, p.bk.both, lo + i)];
+            } else {
+                far = table.value[fb];
+            }
+        }
+        const int tn = seen.next(t + 1, t1);
+        __syncthreads();
+        if (tn < t1) {
+            const uint64_t nb = seen.of(tn);
+            ks.load(k, p.sk.r, tn * BN, nb, p.D, vk, tid);
+            vs.load(v, p.sv.r, tn * BN, nb, p.D, vv, tid);
+        }
+        t = tn;
+        if (mw >= p.M || (p.causal && n0 > mw + 31 + p.start)) continue;
+
+        const bool edge = p.causal && n0 + BN - 1 > mw + p.start;
+        const bool all = bits == (BN == 64 ? ~0ull : 0xffffffffull) && !edge;
+        const uint64_t mine = bits >> (4 * half);
+        const int lim = edge ? m + p.start - n0 - 4 * half : BN;
+        const float* nb = &near_bias[BIAS ? ROWS - 1 - wave * 32 - col + 4 * half : 0];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            f32x16 s = {}, dp = {};
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) s = mma(kt.row(32 * i + col, 16 * c + 8 * half), qf[c], s);
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) dp = mma(vt.row(32 * i + col, 16 * c + 8 * half), gf[c], dp);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int n = 32 * i + reg_row(r);
+                const float e = fexp2(__builtin_fmaf(s[r], c2, (BIAS && fb < 0 ? nb[n] : far) - lse));
+                float ds = e * (dp[r] - delta);
+                if (!all && !((mine >> n & 1) && n <= lim)) ds = 0.f;
+                s[r] = ds;
+            }
+            if (to_table) {
+                if (fb < 0) {
+                    add_band(s, n0 + 32 * i - mw - p.start, sums[wave], table.border, p.bk, lane);
+                } else {
+                    float a = 0.f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) a += s[r];
+                    if (fb == p.bk.n) left += a; else right += a;
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                f32x8 x;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = s[8 * c + j];
+                const Frag<NP> df = split<NP>(x);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) dq[d] = mma(kt.column(32 * i + 16 * c, 32 * d, lane), df, dq[d]);
+            }
+        }
+    }
+    if (to_table) {
+#pragma unroll
+        for (int x = 1; x < 64; x *= 2) {
+            left += __shfl_xor(left, x);
+            right += __shfl_xor(right, x);
+        }
+        if (lane == 0) {
+            sums[wave][p.bk.n] += left;
+            sums[wave][p.bk.both ? 2 * p.bk.n + 1 : 0] += right;
+        }
+        __syncthreads();
+        const int64_t count = (int64_t)p.B * p.splits * p.blocks;
+        float* part = p.part_table + (head * count + ((int64_t)b * p.splits + split_i) * p.blocks + block) * buckets;
+        for (int i = tid; i < buckets; i += NT) {
+            float a = 0.f;
+            for (int j = 0; j < NW; ++j) a += sums[j][i];
+            part[i] = a;
+        }
+    }
+    if (m >= p.M || !p.g_q) return;
+    const float f = p.scale * p.q_sign;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int at = 32 * d + 8 * r + 4 * half;
+            f32x4 x = {dq[d][4 * r], dq[d][4 * r + 1], dq[d][4 * r + 2], dq[d][4 * r + 3]};
+            if (p.splits > 1)
+                *reinterpret_cast<f32x4*>(p.part + ((int64_t)split_i * p.B * p.H * p.M + row) * DP + at) = x;
+            else
+                store4((T*)p.g_q + b * p.sgq.b + head * p.sgq.h + m * p.sgq.r, at, p.D, p.vec & VEC_GQ, x * f);
+        }
+}
+
+template <class T, int DP, int NW, bool BIAS>
+__global__ __launch_bounds__(64 * NW) void softmax_dkv(const SmParams p) {
+    constexpr int NP = Elem<T>::PARTS, BM = Shape<T, DP>::BN, NT = 64 * NW, KEYS = 32 * NW, NS = BM / 32, ND = DP / 32;
+    __shared__ Tile<NP, BM, DP> qt, gt;
+    __shared__ __attribute__((aligned(16))) float lse[BM], delta[BM];
+    __shared__ BiasLds table;
+    __shared__ float near_bias[BIAS ? KEYS + BM : 1];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+    int w = xcd_work(blockIdx.x, gridDim.x);
+    const int block = w % p.blocks; w /= p.blocks;
+    const int split_i = w % p.splits; w /= p.splits;
+    const int kvh = w % p.G, b = w / p.G, share = p.H / p.G;
+    const int n0 = block * KEYS, nw = n0 + wave * 32, n = nw + col;
+    const bool shown = n < p.N && (!p.keep || p.keep[b * p.keep_stride + n]);
+    const bool idle = !__any(shown);
+
+    Frag<NP> kf[DP / 16], vf[DP / 16];
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+        typename Elem<T>::seg s = {}, x = {};
+        if (shown) {
+            s = load_seg((const T*)p.k + b * p.sk.b + kvh * p.sk.h + n * p.sk.r, 16 * c + 8 * half, p.D, p.vec & VEC_K);
+            x = load_seg((const T*)p.v + b * p.sv.b + kvh * p.sv.h + n * p.sv.r, 16 * c + 8 * half, p.D, p.vec & VEC_V);
+        }
+        if (p.q_sign < 0) s = -s;
+        kf[c] = frag_of(s);
+        vf[c] = frag_of(x);
+    }
+
+    // the tiles of queries of all heads that share these keys, one after the other
+    const int tiles = (p.M + BM - 1) / BM;
+    const int64_t work = (int64_t)tiles * share;
+    const int t1 = (int)(work * (split_i + 1) / p.splits);
+    const auto next = [&](int t) {                     // the first tile from t on with a query that sees a key here
+        if (p.causal)
+            while (t < t1 && t % tiles * BM + BM - 1 + p.start < n0) ++t;
+        return t;
+    };
+    Staged<T, DP, BM, NT> qs, gs;
+    float ls = HIGH, des = 0.f;
+    const auto load = [&](int t) {
+        const int head = kvh * share + t / tiles, m0 = t % tiles * BM, left = p.M - m0;
+        const uint64_t bits = left >= 64 ? ~0ull : (1ull << left) - 1;
+        qs.load((const T*)p.q + b * p.sq.b + head * p.sq.h, p.sq.r, m0, bits, p.D, p.vec & VEC_Q, tid);
+        gs.load((const T*)p.g_out + b * p.sg.b + head * p.sg.h, p.sg.r, m0, bits, p.D, p.vec & VEC_G, tid);
+        ls = HIGH;
+        des = 0.f;
+        if (tid < BM && tid < left) {
+            const int64_t row = ((int64_t)b * p.H + head) * p.M + m0 + tid;
+            ls = p.lse[row];
+            des = p.delta[row];
+        }
+    };
+    const float c2 = p.scale * LOG2E;
+    f32x16 dk[ND] = {}, dv[ND] = {};
+    int filled = -1;                                   // the head whose bias stands in LDS
+
+    int t = next((int)(work * split_i / p.splits));
+    if (t < t1) load(t);
+    while (t < t1) {
+        const int m0 = t % tiles * BM, head = kvh * share + t / tiles;
+        float far = 0.f;
+        bool near = false;
+        __syncthreads();
+        qs.store(qt, tid);
+        gs.store(gt, tid);
+        if (tid < BM) {
+            lse[tid] = ls;
+            delta[tid] = des;
+        }
+        if constexpr (BIAS) {
+            if (head != filled) {
+                table.fill(p, head, tid, NT);
+                filled = head;
+                __syncthreads();
+            }
+            const int lo = n0 - (m0 + BM - 1) - p.start;
+            const int fb = far_bucket(p.bk, lo, n0 + KEYS - 1 - m0 - p.start);
+            near = fb < 0;
+            if (near) {
+                for (int i = tid; i < KEYS + BM - 1; i += NT)
+                    near_bias[i] = table.value[bucket_of(table.border, p.bk.n, p.bk.both, lo + i)];
+            } else {
+                far = table.value[fb];
+            }
+        }
+        __syncthreads();
+        t = next(t + 1);
+        if (t < t1) load(t);
+        if (idle || (p.causal && m0 + BM - 1 + p.start < nw)) continue;
+
+        const bool edge = p.causal && m0 + p.start < nw + 31;
+        const int lim = edge ? n - p.start - m0 - 4 * half : -1;         // the first query that sees the key
+        const float* nb = &near_bias[BIAS ? wave * 32 + col + BM - 1 - 4 * half : 0];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            f32x16 s = {}, dp = {};
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) s = mma(qt.row(32 * i + col, 16 * c + 8 * half), kf[c], s);
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) dp = mma(gt.row(32 * i + col, 16 * c + 8 * half), vf[c], dp);
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) {
+                const f32x4 l4 = *reinterpret_cast<const f32x4*>(&lse[32 * i + 8 * r4 + 4 * half]);
+                const f32x4 d4 = *reinterpret_cast<const f32x4*>(&delta[32 * i + 8 * r4 + 4 * half]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int r = 4 * r4 + j, mr = 32 * i + 8 * r4 + j;
+                    float e = fexp2(__builtin_fmaf(s[r], c2, (BIAS && near ? nb[-mr] : far) - l4[j]));
+                    if (!shown || mr < lim) e = 0.f;
+                    float ds = e * (dp[r] - d4[j]);
+                    if (!shown || mr < lim) ds = 0.f;
+                    s[r] = e;
+                    dp[r] = ds;
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                f32x8 x, y;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    x[j] = s[8 * c + j];
+                    y[j] = dp[8 * c + j];
+                }
+                const Frag<NP> pf = split<NP>(x), df = split<NP>(y);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    dv[d] = mma(gt.column(32 * i + 16 * c, 32 * d, lane), pf, dv[d]);
+                    dk[d] = mma(qt.column(32 * i + 16 * c, 32 * d, lane), df, dk[d]);
+                }
+            }
+        }
+    }
+    if (n >= p.N) return;
+    const float f = p.scale * p.q_sign;
+    const int64_t row = ((int64_t)b * p.G + kvh) * p.N + n, all = (int64_t)p.B * p.G * p.N;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int at = 32 * d + 8 * r + 4 * half;
+            f32x4 x = {dk[d][4 * r], dk[d][4 * r + 1], dk[d][4 * r + 2], dk[d][4 * r + 3]};
+            f32x4 y = {dv[d][4 * r], dv[d][4 * r + 1], dv[d][4 * r + 2], dv[d][4 * r + 3]};
+            if (p.splits > 1) {
+                *reinterpret_cast<f32x4*>(p.part + (split_i * all + row) * DP + at) = x;
+                *reinterpret_cast<f32x4*>(p.part2 + (split_i * all + row) * DP + at) = y;
+            } else {
+                store4((T*)p.g_k + b * p.sgk.b + kvh * p.sgk.h + n * p.sgk.r, at, p.D, p.vec & VEC_GK, x * f);
+                store4((T*)p.g_v + b * p.sgv.b + kvh * p.sgv.h + n * p.sgv.r, at, p.D, p.vec & VEC_GV, y);
+            }
+        }
+}
+
+// Sum of the splits' partial rows: DP / 4 lanes a row.
+template <class T, int DP>
+__global__ __launch_bounds__(256) void softmax_sum(const float* part, T* out, SmStrides so, bool vec, float scale,
+                                                   int splits, int64_t rows, int heads, int len, int D) {
+    constexpr int LANES = DP / 4;
+    const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES;
+    const int d = threadIdx.x % LANES * 4;
+    if (row >= rows) return;
+    f32x4 x = {};
+    for (int s = 0; s < splits; ++s) x = x + *reinterpret_cast<const f32x4*>(part + (s * rows + row) * DP + d);
+    const int i = (int)(row % len), h = (int)(row / len % heads), b = (int)(row / len / heads);
+    store4(out + b * so.b + h * so.h + i * so.r, d, D, vec, x * scale);
+}
+
+// One workgroup for each (head, bucket).
+__global__ __launch_bounds__(256) void softmax_table(const float* part, float* g_table, int H, int count, int buckets) {
+    __shared__ float s[4];
+    const int h = blockIdx.x, k = blockIdx.y;
+    float x = 0.f;
+    for (int i = threadIdx.x; i < count; i += 256) x += part[((int64_t)h * count + i) * buckets + k];
+#pragma unroll
+    for (int far = 1; far < 64; far *= 2) x += __shfl_xor(x, far);
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = x;
+    __syncthreads();
+    if (threadIdx.x == 0) g_table[(int64_t)k * H + h] = s[0] + s[1] + s[2] + s[3];
+}
+
+template <class T, int DP> int run_delta(const SmParams& p, hipStream_t st) {
+    const int64_t threads = (int64_t)p.B * p.H * p.M * (DP / 8);
+    softmax_delta<T, DP><<<dim3((unsigned)((threads + 255) / 256)), 256, 0, st>>>(p);
+    return (int)hipGetLastError();
+}
+template <class T, int DP, int NW> int run_dq(const SmParams& p, hipStream_t st) {
+    const dim3 grid((unsigned)((int64_t)p.B * p.H * p.blocks * p.splits));
+    if (p.table) softmax_dq<T, DP, NW, true><<<grid, 64 * NW, 0, st>>>(p);
+    else softmax_dq<T, DP, NW, false><<<grid, 64 * NW, 0, st>>>(p);
+    return (int)hipGetLastError();
+}
+template <class T, int DP, int NW> int run_dkv(const SmParams& p, hipStream_t st) {
+    const dim3 grid((unsigned)((int64_t)p.B * p.G * p.blocks * p.splits));
+    if (p.table) softmax_dkv<T, DP, NW, true><<<grid, 64 * NW, 0, st>>>(p);
+    else softmax_dkv<T, DP, NW, false><<<grid, 64 * NW, 0, st>>>(p);
+    return (int)hipGetLastError();
+}
+template <class T, int DP> int run_sum(const float* part, void* out, SmStrides so, bool vec, float scale, int splits, int B,
+                                       int heads, int len, int D, hipStream_t st) {
+    const int64_t rows = (int64_t)B * heads * len, threads = rows * (DP / 4);
+    softmax_sum<T, DP><<<dim3((unsigned)((threads + 255) / 256)), 256, 0, st>>>(part, (T*)out, so, vec, scale, splits, rows,
+                                                                               heads, len, D);
+    return (int)hipGetLastError();
+}
+
+}  // namespace sm
+
+int sm_delta(int dtype, const SmParams& p, hipStream_t st) {
+    return sm::dispatch(dtype, p.D, [&](auto t, auto dp) { return sm::run_delta<decltype(t), dp.value>(p, st); });
+}
+
+int sm_dq(int dtype, const SmParams& p, int waves, hipStream_t st) {
+    return sm::dispatch(dtype, p.D, [&](auto t, auto dp) {
+        return waves == 1 ? sm::run_dq<decltype(t), dp.value, 1>(p, st)
+             : waves == 2 ? sm::run_dq<decltype(t), dp.value, 2>(p, st) : sm::run_dq<decltype(t), dp.value, 4>(p, st); });
+}
+
+int sm_dkv(int dtype, const SmParams& p, int waves, hipStream_t st) {
+    return sm::dispatch(dtype, p.D, [&](auto t, auto dp) {
+        return waves == 1 ? sm::run_dkv<decltype(t), dp.value, 1>(p, st)
+             : waves == 2 ? sm::run_dkv<decltype(t), dp.value, 2>(p, st) : sm::run_dkv<decltype(t), dp.value, 4>(p, st); });
+}
+
+int sm_sum_parts(int dtype, const float* part, void* out, SmStrides so, bool vec, float scale, int splits, int B, int heads,
+                 int len, int D, hipStream_t st) {
+    return sm::dispatch(dtype, D, [&](auto t, auto dp) {
+        return sm::run_sum<decltype(t), dp.value>(part, out, so, vec, scale, splits, B, heads, len, D, st); });
+}
+
+int sm_sum_table(const float* part, float* g_table, int H, int count, int buckets, hipStream_t st) {
+    sm::softmax_table<<<dim3((unsigned)H, (unsigned)buckets), 256, 0, st>>>(part, g_table, H, count, buckets);
+    return (int)hipGetLastError();
+}
+
+}  // namespace qlka

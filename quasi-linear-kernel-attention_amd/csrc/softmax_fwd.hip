@@ -1,0 +1,269 @@
+// Softmax attention, forward: O = softmax(scale q k^T + bias) v over the visible keys, one pass over the keys with the
+// running maximum and sum.
+//
+// A wave owns 32 queries and keeps S^T = k q^T tiles in registers (a lane holds one query's scores, softmax_tile.h), so
+// the row maximum and sum need one exchange between the halves of the wave, and O^T += v^T P^T takes the probabilities
+// from the registers they are in. A workgroup of `waves` waves shares the tiles of k and v in LDS; the next tile's loads are
+// issued before the current tile's products. The running maximum is moved only when it grows by more than 2^8, so
+// that the output is hardly ever scaled; probabilities are then at most 2^8. Rounding them to bf16 for the product with bf16
+// values (not for fp32) costs what rounding the result does; their sum is of the unrounded ones. Where the table's
+// gradient will be wanted (FINE) they are taken in two parts of 8 bits: that gradient is fp32 and a sum over whole rows of
+// dS = P (dP - delta), in which an error of delta, the row sum of dO * O, does not average out.
+//
+// Masked keys are read as zeros (what stands there may be anything) and their tiles, where none is left, are skipped.
+// When a call has too few queries to fill the GPU, the keys are split: each split leaves its unscaled O with its maximum
+// and sum, and softmax_combine joins them.
+#include "softmax_tile.h"
+
+#include <limits>
+
+namespace qlka {
+namespace sm {
+
+constexpr float GROW = 8.f;
+
+template <class T, int DP, int NW, bool BIAS, bool FINE>
+__global__ __launch_bounds__(64 * NW) void softmax_fwd(const SmParams p) {
+    constexpr int NP = Elem<T>::PARTS, BN = Shape<T, DP>::BN, NT = 64 * NW, ROWS = 32 * NW, NS = BN / 32, ND = DP / 32;
+    __shared__ Tile<NP, BN, DP> kt, vt;
+    __shared__ BiasLds table;
+    __shared__ float near_bias[BIAS ? ROWS + BN : 1];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+    int w = xcd_work(blockIdx.x, gridDim.x);
+    const int block = w % p.blocks; w /= p.blocks;
+    const int split_i = w % p.splits; w /= p.splits;
+    const int head = w % p.H, b = w / p.H, kvh = head / (p.H / p.G);
+    const int m0 = block * ROWS, mw = m0 + wave * 32, m = mw + col;
+    const T* q = (const T*)p.q + b * p.sq.b + head * p.sq.h;
+    const T* k = (const T*)p.k + b * p.sk.b + kvh * p.sk.h;
+    const T* v = (const T*)p.v + b * p.sv.b + kvh * p.sv.h;
+    const bool vk = p.vec & VEC_K, vv = p.vec & VEC_V;
+
+    Frag<NP> qf[DP / 16];
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+        typename Elem<T>::seg s = {};
+        if (m < p.M) s = load_seg(q + m * p.sq.r, 16 * c + 8 * half, p.D, p.vec & VEC_Q);
+        if (p.q_sign < 0) s = -s;
+        qf[c] = frag_of(s);
+    }
+    if constexpr (BIAS) {
+        table.fill(p, head, tid, NT);
+        __syncthreads();
+    }
+
+    const int tiles = (p.N + BN - 1) / BN;
+    int t0 = (int)((int64_t)tiles * split_i / p.splits), t1 = (int)((int64_t)tiles * (split_i + 1) / p.splits);
+    if (p.causal) {
+        const int last = min(m0 + ROWS, p.M) - 1 + p.start;          // the last key that a row here sees
+        t1 = min(t1, last < 0 ? 0 : last / BN + 1);
+    }
+    KeyBits<BN> seen(p, b);
+    Staged<T, DP, BN, NT> ks, vs;
+    const float c2 = p.scale * LOG2E;
+    f32x16 o[ND] = {};
+    float top = -std::numeric_limits<float>::infinity(), ref = 0.f, sum = 0.f;
+
+    int t = seen.next(t0, t1);
+    if (t < t1) {
+        const uint64_t bits = seen.of(t);
+        ks.load(k, p.sk.r, t * BN, bits, p.D, vk, tid);
+        vs.load(v, p.sv.r, t * BN, bits, p.D, vv, tid);
+    }
+    while (t < t1) {
+        const int n0 = t * BN;
+        const uint64_t bits = seen.of(t);
+        float far = 0.f;
+        bool near = false;
+        __syncthreads();
+        ks.store(kt, tid);
+        vs.store(vt, tid);
+        if constexpr (BIAS) {
+            const int lo = n0 - (m0 + ROWS - 1) - p.start;
+            const int fb = far_bucket(p.bk, lo, n0 + BN - 1 - m0 - p.start);
+            near = fb < 0;
+            if (near) {
+                for (int i = tid; i < ROWS + BN - 1; i += NT)
+                    near_bias[i] = table.value[bucket_of(table.border, p.bk.n, p.bk.both, lo + i)];
+            } else {
+                far = table.value[fb];
+            }
+        }
+        const int tn = seen.next(t + 1, t1);
+        __syncthreads();
+        if (tn < t1) {
+            const uint64_t nb = seen.of(tn);
+            ks.load(k, p.sk.r, tn * BN, nb, p.D, vk, tid);
+            vs.load(v, p.sv.r, tn * BN, nb, p.D, vv, tid);
+        }
+        t = tn;
+        if (mw >= p.M || (p.causal && n0 > mw + 31 + p.start)) continue;
+
+        f32x16 s[NS] = {};
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) s[i] = mma(kt.row(32 * i + col, 16 * c + 8 * half), qf[c], s[i]);
+
+        // scores in log2 units are fma(s, mul, add) from here on
+        float mul = c2, add = far;
+        const bool edge = p.causal && n0 + BN - 1 > mw + p.start;
+        const bool all = bits == (BN == 64 ? ~0ull : 0xffffffffull) && !edge;
+        if (near || !all) {
+            const uint64_t mine = bits >> (4 * half);
+            const int lim = edge ? m + p.start - n0 - 4 * half : BN;     // the last key seen
+            const float* nb = &near_bias[BIAS ? ROWS - 1 - wave * 32 - col + 4 * half : 0];
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int n = 32 * i + reg_row(r);
+                    float x = __builtin_fmaf(s[i][r], c2, BIAS && near ? nb[n] : far);
+                    if (!all && !((mine >> n & 1) && n <= lim)) x = -std::numeric_limits<float>::infinity();
+                    s[i][r] = x;
+                }
+            mul = 1.f;
+            add = 0.f;
+        }
+        float hi = s[0][0];
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) hi = fmaxf(hi, s[i][r]);
+        hi = fmaxf(hi, other_half(hi));
+        hi = __builtin_fmaf(hi, mul, add);
+        if (__any(hi > top + GROW)) {                                     // top -inf: any score at all
+            const bool first = top == -std::numeric_limits<float>::infinity();
+            const float was = ref;
+            top = fmaxf(top, hi);
+            ref = top == -std::numeric_limits<float>::infinity() ? 0.f : top;
+            const float f = first ? 1.f : fexp2(was - ref);               // the first time there is nothing to scale
+            sum *= f;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[d] *= f;
+        }
+        add -= ref;
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                f32x8 e;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    e[j] = fexp2(__builtin_fmaf(s[i][8 * c + j], mul, add));
+                    sum += e[j];
+                }
+                const Frag<NP> pf = split<NP>(e);
+                Frag<NP> rest;
+                if constexpr (FINE) rest = split<NP>(e - __builtin_convertvector(pf.p[0], f32x8));
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    const Frag<NP> vf = vt.column(32 * i + 16 * c, 32 * d, lane);
+                    if constexpr (FINE) o[d] = mma(vf, rest, o[d]);
+                    o[d] = mma(vf, pf, o[d]);
+                }
+            }
+    }
+    if (m >= p.M) return;
+    sum += other_half(sum);
+    const int64_t row = ((int64_t)b * p.H + head) * p.M + m;
+    if (p.splits > 1) {
+        const int64_t at = (int64_t)split_i * p.B * p.H * p.M + row;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                *reinterpret_cast<f32x4*>(p.part + at * DP + 32 * d + 8 * r + 4 * half) =
+                    f32x4{o[d][4 * r], o[d][4 * r + 1], o[d][4 * r + 2], o[d][4 * r + 3]};
+        if (half == 0) {
+            p.part2[2 * at] = ref;
+            p.part2[2 * at + 1] = sum;
+        }
+        return;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    T* out = (T*)p.out + b * p.so.b + head * p.so.h + m * p.so.r;
+    T* lo = p.out_lo ? (T*)p.out_lo + b * p.so.b + head * p.so.h + m * p.so.r : nullptr;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            f32x4 x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = o[d][4 * r + i] * inv;
+            store4(out, 32 * d + 8 * r + 4 * half, p.D, p.vec & VEC_O, x);
+            if constexpr (FINE) {
+                if (lo) {
+                    x = x - __builtin_convertvector(__builtin_convertvector(x, bf16x4), f32x4);
+                    store4(lo, 32 * d + 8 * r + 4 * half, p.D, p.vec & VEC_O, x);
+                }
+            }
+        }
+    if (p.lse && half == 0)
+        p.lse[row] = sum == 0.f ? std::numeric_limits<float>::infinity() : ref + __log2f(sum);
+}
+
+template <class T, int DP, int NW> int launch_fwd(const SmParams& p, hipStream_t st) {
+    const dim3 grid((unsigned)((int64_t)p.B * p.H * p.blocks * p.splits));
+    if (sizeof(T) == 2 && p.out_lo) softmax_fwd<T, DP, NW, true, sizeof(T) == 2><<<grid, 64 * NW, 0, st>>>(p);
+    else if (p.table) softmax_fwd<T, DP, NW, true, false><<<grid, 64 * NW, 0, st>>>(p);
+    else softmax_fwd<T, DP, NW, false, false><<<grid, 64 * NW, 0, st>>>(p);
+    return (int)hipGetLastError();
+}
+// Joins the splits of a row: a group of DP / 4 lanes a row, four elements a lane.
+template <class T, int DP>
+__global__ __launch_bounds__(256) void softmax_combine(const SmParams p) {
+    constexpr int LANES = DP / 4;
+    const int64_t rows = (int64_t)p.B * p.H * p.M;
+    const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES;
+    const int d = threadIdx.x % LANES * 4;
+    if (row >= rows) return;
+    float ref = -std::numeric_limits<float>::infinity(), sum = 0.f;
+    for (int s = 0; s < p.splits; ++s) {
+        const float2 a = *reinterpret_cast<const float2*>(p.part2 + 2 * (s * rows + row));
+        if (a.y == 0.f) continue;                                         // no key here
+        const float to = fmaxf(ref, a.x);
+        sum = sum * fexp2(ref - to) + a.y * fexp2(a.x - to);
+        ref = to;
+    }
+    f32x4 x = {};
+    for (int s = 0; s < p.splits; ++s) {
+        const float2 a = *reinterpret_cast<const float2*>(p.part2 + 2 * (s * rows + row));
+        if (a.y == 0.f) continue;
+        const f32x4 y = *reinterpret_cast<const f32x4*>(p.part + (s * rows + row) * DP + d);
+        x = x + y * fexp2(a.x - ref);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    x = x * inv;
+    const int m = (int)(row % p.M), head = (int)(row / p.M % p.H), b = (int)(row / p.M / p.H);
+    const int64_t at = b * p.so.b + head * p.so.h + m * p.so.r;
+    store4((T*)p.out + at, d, p.D, p.vec & VEC_O, x);
+    if constexpr (sizeof(T) == 2) {
+        if (p.out_lo) {
+            x = x - __builtin_convertvector(__builtin_convertvector(x, bf16x4), f32x4);
+            store4((T*)p.out_lo + at, d, p.D, p.vec & VEC_O, x);
+        }
+    }
+    if (p.lse && d == 0) p.lse[row] = sum == 0.f ? std::numeric_limits<float>::infinity() : ref + __log2f(sum);
+}
+
+template <class T, int DP> int launch_combine(const SmParams& p, hipStream_t st) {
+    const int64_t threads = (int64_t)p.B * p.H * p.M * (DP / 4);
+    softmax_combine<T, DP><<<dim3((unsigned)((threads + 255) / 256)), 256, 0, st>>>(p);
+    return (int)hipGetLastError();
+}
+
+}  // namespace sm
+
+int sm_fwd(int dtype, const SmParams& p, int waves, hipStream_t st) {
+    return sm::dispatch(dtype, p.D, [&](auto t, auto dp) {
+        return waves == 1 ? sm::launch_fwd<decltype(t), dp.value, 1>(p, st)
+             : waves == 2 ? sm::launch_fwd<decltype(t), dp.value, 2>(p, st) : sm::launch_fwd<decltype(t), dp.value, 4>(p, st); });
+}
+
+int sm_combine(int dtype, const SmParams& p, hipStream_t st) {
+    return sm::dispatch(dtype, p.D, [&](auto t, auto dp) { return sm::launch_combine<decltype(t), dp.value>(p, st); });
+}
+
+}  // namespace qlka

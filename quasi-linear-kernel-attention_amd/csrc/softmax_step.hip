@@ -1,0 +1,211 @@
+// Softmax attention for a few query rows per key head (a decoder's single tokens; with shared heads all their queries):
+// bound by reading k and v once.
+//
+// A key row is read by DP / 8 lanes of a wave, 8 elements each, so a wave reads 512 / DP keys with one 16-byte load a lane (two
+// for float) and keeps four such loads of k and four of v in flight. Scores are formed with fp32 multiply-adds and summed
+// over a row's lanes by DPP; every group of lanes runs its own softmax over the keys that pass it, and the groups, then the
+// waves, are joined at the end. The keys are split over workgroups until the GPU is full (softmax_combine joins the
+// splits). A matrix tile would use one of its 32 rows here.
+#include "softmax_tile.h"
+
+#include <limits>
+
+namespace qlka {
+namespace sm {
+
+constexpr int STEP_WAVES = 4, STEP_LOADS = 4;
+
+template <int CTRL> __device__ __forceinline__ float dpp(float x) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+// sum over groups of 4, 8 or 16 successive lanes, in every lane
+template <int LANES> __device__ __forceinline__ float row_sum(float x) {
+    x += dpp<0xB1>(x);                       // quad: 1 0 3 2
+    x += dpp<0x4E>(x);                       // quad: 2 3 0 1
+    if constexpr (LANES >= 8) x += dpp<0x141>(x);    // half row mirrored: the other quad
+    if constexpr (LANES >= 16) x += dpp<0x140>(x);   // row mirrored: the other half
+    return x;
+}
+
+__device__ __forceinline__ f32x8 floats(bf16x8 x) { return __builtin_convertvector(x, f32x8); }
+__device__ __forceinline__ f32x8 floats(f32x8 x) { return x; }
+
+template <class T, int DP, int R, bool BIAS>
+__global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p) {
+    constexpr int LANES = DP / 8, KEYS = 64 / LANES, U = STEP_LOADS, NW = STEP_WAVES, NT = 64 * NW;
+    constexpr float LOW = -std::numeric_limits<float>::infinity();
+    __shared__ float join_o[NW][R][DP], join_m[NW][R], join_s[NW][R];
+    __shared__ float table[BIAS ? R : 1][QLKA_MAX_BUCKETS];
+    __shared__ int border[BIAS ? QLKA_MAX_BUCKETS : 1];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, group = lane / LANES, d = lane % LANES * 8;
+    int w = xcd_work(blockIdx.x, gridDim.x);
+    const int split_i = w % p.splits; w /= p.splits;
+    const int kvh = w % p.G, b = w / p.G, share = p.H / p.G, rows = share * p.M;
+    const T* k = (const T*)p.k + b * p.sk.b + kvh * p.sk.h;
+    const T* v = (const T*)p.v + b * p.sv.b + kvh * p.sv.h;
+    const bool vk = p.vec & VEC_K, vv = p.vec & VEC_V;
+
+    f32x8 q[R], o[R];
+    float top[R], sum[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        o[r] = f32x8{};
+        q[r] = f32x8{};
+        top[r] = LOW;
+        sum[r] = 0.f;
+        if (r < rows) {
+            const int head = kvh * share + r / p.M, m = r % p.M;
+            q[r] = floats(load_seg((const T*)p.q + b * p.sq.b + head * p.sq.h + m * p.sq.r, d, p.D, p.vec & VEC_Q)) *
+                   (p.q_sign * p.scale * LOG2E);
+            if constexpr (BIAS)
+                for (int i = tid; i < (p.bk.n + 1) * (p.bk.both ? 2 : 1); i += NT)
+                    table[r][i] = p.table[(int64_t)i * p.H + head] * LOG2E;
+        }
+    }
+    if constexpr (BIAS) {
+        for (int i = tid; i < p.bk.n; i += NT) border[i] = p.bk.border[i];
+        __syncthreads();
+    }
+
+    const int tiles = (p.N + 63) / 64;
+    const int t0 = (int)((int64_t)tiles * split_i / p.splits);
+    int t1 = (int)((int64_t)tiles * (split_i + 1) / p.splits);
+    const int last = p.causal ? p.M - 1 + p.start : p.N - 1;          // the last key that any row sees
+    t1 = min(t1, last < 0 ? 0 : last / 64 + 1);
+    KeyBits<64> seen(p, b);
+    for (int t = t0 + wave; t < t1; t += NW) {
+        const int n0 = t * 64;
+        uint64_t bits = seen.of(t);
+        if (last - n0 < 63) bits &= (1ull << (last - n0 + 1)) - 1;
+        int fb = -1;
+        if constexpr (BIAS) fb = far_bucket(p.bk, n0 - (p.M - 1) - p.start, n0 + 63 - p.start);
+#pragma unroll 1
+        for (int u0 = 0; u0 < 64; u0 += U * KEYS) {
+            if (!(bits >> u0 & (U * KEYS == 64 ? ~0ull : (1ull << (U * KEYS % 64)) - 1))) continue;
+            typename Elem<T>::seg ks[U], vs[U];
+            bool in[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int n = u0 + u * KEYS + group;
+                in[u] = bits >> n & 1;
+                ks[u] = {};
+                if (in[u]) ks[u] = load_seg(k + (n0 + n) * p.sk.r, d, p.D, vk);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                vs[u] = {};
+                if (in[u]) vs[u] = load_seg(v + (n0 + u0 + u * KEYS + group) * p.sv.r, d, p.D, vv);
+            }
+            float x[R][U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const f32x8 kf = floats(ks[u]);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    float a = q[r][0] * kf[0];
+#pragma unroll
+                    for (int i = 1; i < 8; ++i) a = __builtin_fmaf(q[r][i], kf[i], a);
+                    x[r][u] = row_sum<LANES>(a);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                if (r >= rows) continue;
+                const int seat = r % p.M + p.start;                    // the query's position
+                float hi = LOW;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int n = n0 + u0 + u * KEYS + group;
+                    if constexpr (BIAS)
+                        x[r][u] += table[r][fb >= 0 ? fb : bucket_of(border, p.bk.n, p.bk.both, n - seat)];
+                    if (!in[u] || (p.causal && n > seat)) x[r][u] = LOW;
+                    hi = fmaxf(hi, x[r][u]);
+                }
+                const float to = fmaxf(top[r], hi), ref = to == LOW ? 0.f : to, f = fexp2(top[r] - ref);
+                top[r] = to;
+                sum[r] *= f;
+                o[r] *= f;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const float e = fexp2(x[r][u] - ref);
+                    sum[r] += e;
+                    o[r] += floats(vs[u]) * e;
+                }
+            }
+        }
+    }
+
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int far = LANES; far < 64; far *= 2) {
+            const float top2 = __shfl_xor(top[r], far), to = fmaxf(top[r], top2), ref = to == LOW ? 0.f : to;
+            const float f = fexp2(top[r] - ref), f2 = fexp2(top2 - ref);
+            sum[r] = sum[r] * f + __shfl_xor(sum[r], far) * f2;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[r][i] = o[r][i] * f + __shfl_xor(o[r][i], far) * f2;
+            top[r] = to;
+        }
+        if (group == 0) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) join_o[wave][r][d + i] = o[r][i];
+            if (d == 0) {
+                join_m[wave][r] = top[r];
+                join_s[wave][r] = sum[r];
+            }
+        }
+    }
+    __syncthreads();
+    const int64_t all = (int64_t)p.B * p.H * p.M;
+    for (int e = tid; e < rows * DP; e += NT) {
+        const int r = e / DP, c = e % DP, head = kvh * share + r / p.M, m = r % p.M;
+        float to = LOW;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) to = fmaxf(to, join_m[i][r]);
+        const float ref = to == LOW ? 0.f : to;
+        float s = 0.f, x = 0.f;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            const float f = fexp2(join_m[i][r] - ref);
+            s += join_s[i][r] * f;
+            x += join_o[i][r][c] * f;
+        }
+        const int64_t row = ((int64_t)b * p.H + head) * p.M + m;
+        if (p.splits > 1) {
+            p.part[(split_i * all + row) * DP + c] = x;
+            if (c == 0) {
+                p.part2[2 * (split_i * all + row)] = ref;
+                p.part2[2 * (split_i * all + row) + 1] = s;
+            }
+            continue;
+        }
+        x = s == 0.f ? 0.f : x / s;
+        if (c < p.D) {
+            const int64_t at = b * p.so.b + head * p.so.h + m * p.so.r + c;
+            const T y = (T)x;
+            ((T*)p.out)[at] = y;
+            if (sizeof(T) == 2 && p.out_lo) ((T*)p.out_lo)[at] = (T)(x - (float)y);
+        }
+        if (p.lse && c == 0) p.lse[row] = s == 0.f ? std::numeric_limits<float>::infinity() : ref + __log2f(s);
+    }
+}
+
+template <class T, int DP, int R> int launch_step(const SmParams& p, hipStream_t st) {
+    const dim3 grid((unsigned)((int64_t)p.B * p.G * p.splits));
+    if (p.table) softmax_step<T, DP, R, true><<<grid, 64 * STEP_WAVES, 0, st>>>(p);
+    else softmax_step<T, DP, R, false><<<grid, 64 * STEP_WAVES, 0, st>>>(p);
+    return (int)hipGetLastError();
+}
+template <class T, int DP> int pick_step(const SmParams& p, hipStream_t st) {
+    const int rows = p.H / p.G * p.M;
+    return rows == 1 ? launch_step<T, DP, 1>(p, st) : rows == 2 ? launch_step<T, DP, 2>(p, st)
+         : rows <= 4 ? launch_step<T, DP, 4>(p, st) : launch_step<T, DP, 8>(p, st);
+}
+}  // namespace sm
+
+int sm_step(int dtype, const SmParams& p, hipStream_t st) {
+    return sm::dispatch(dtype, p.D, [&](auto t, auto dp) { return sm::pick_step<decltype(t), dp.value>(p, st); });
+}
+
+}  // namespace qlka

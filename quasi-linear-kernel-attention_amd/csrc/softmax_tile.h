@@ -1,0 +1,269 @@
+// Device pieces of the softmax attention kernels (gfx950, wave64): matrix fragments, tiles in LDS, masks, buckets.
+//
+// Products run on v_mfma_f32_32x32x16_bf16 (lane l: row or column l % 32, elements 8 (l / 32) + 0..7 of a 16-element
+// chunk; result: column l % 32, rows 8 (r / 4) + 4 (l / 32) + r % 4 for register r). The scores are formed with the
+// other side's rows in the registers, so a lane holds scores of one row (or one key), and eight successive result registers
+// are, as they are, the second operand of the next product: its 16-element chunk is taken in the order
+//   slot (half, j) <- element 8 (j / 4) + 4 half + j % 4,
+// and the first operand is read from LDS in that order, transposed, by ds_read_b64_tr_b16 (four successive rows of one
+// column a lane). No score crosses lanes or goes through LDS.
+//
+// float inputs are split into three bf16 parts of 8 bits each (24 in all), and a product is the six products of parts
+// whose sizes add up to 2^-16 of the largest or more; what is left out is below 2^-26 of it. At 6 bf16 products that is 2.7
+// times the rate of the fp32 matrix instruction. An infinity among the inputs gives NaN this way.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <cstdint>
+#include <type_traits>
+
+#include "softmax.h"
+
+namespace qlka {
+namespace sm {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(8))) float f32x8;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+template <class T> struct Elem;
+template <> struct Elem<__bf16> { static constexpr int PARTS = 1; typedef bf16x8 seg; };
+template <> struct Elem<float> { static constexpr int PARTS = 3; typedef f32x8 seg; };
+
+template <int NP> struct Frag { bf16x8 p[NP]; };
+
+template <int NP> __device__ __forceinline__ Frag<NP> split(f32x8 x) {
+    Frag<NP> f;
+    f.p[0] = __builtin_convertvector(x, bf16x8);
+    if constexpr (NP == 3) {
+        x = x - __builtin_convertvector(f.p[0], f32x8);
+        f.p[1] = __builtin_convertvector(x, bf16x8);
+        x = x - __builtin_convertvector(f.p[1], f32x8);
+        f.p[2] = __builtin_convertvector(x, bf16x8);
+    }
+    return f;
+}
+__device__ __forceinline__ Frag<1> frag_of(bf16x8 x) { return Frag<1>{{x}}; }
+__device__ __forceinline__ Frag<3> frag_of(f32x8 x) { return split<3>(x); }
+
+__device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+template <int NP> __device__ __forceinline__ f32x16 mma(const Frag<NP>& a, const Frag<NP>& b, f32x16 c) {
+    if constexpr (NP == 3) {
+        c = mfma(a.p[0], b.p[2], c);
+        c = mfma(a.p[2], b.p[0], c);
+        c = mfma(a.p[1], b.p[1], c);
+        c = mfma(a.p[0], b.p[1], c);
+        c = mfma(a.p[1], b.p[0], c);
+    }
+    return mfma(a.p[0], b.p[0], c);
+}
+
+__device__ __forceinline__ float fexp2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+__device__ __forceinline__ int reg_row(int r) { return (r >> 2) * 8 + (r & 3); }   // + 4 (lane / 32)
+
+// Eight elements d .. d + 7 of a row of D; zeros past D. vec: the row is 16-byte aligned and D a multiple of 8.
+template <class T> __device__ __forceinline__ typename Elem<T>::seg load_seg(const T* row, int d, int D, bool vec) {
+    typename Elem<T>::seg x = {};
+    if (vec) {
+        if (d < D) x = *reinterpret_cast<const typename Elem<T>::seg*>(row + d);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (d + i < D) x[i] = row[d + i];
+    }
+    return x;
+}
+
+// A tile of ROWS rows of DP elements in LDS, one plane for each part; rows are 16 bytes further apart than their length,
+// which spreads both the row reads and the transposing reads over the banks.
+template <int NP, int ROWS, int DP> struct Tile {
+    static constexpr int LD = DP + 8, PLANE = ROWS * LD;
+    __bf16 x[NP * PLANE];
+
+    template <class Seg> __device__ __forceinline__ void put(int row, int d, Seg s) {
+        const Frag<NP> f = frag_of(s);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) *reinterpret_cast<bf16x8*>(&x[i * PLANE + row * LD + d]) = f.p[i];
+    }
+    // elements d .. d + 7 of a row
+    __device__ __forceinline__ Frag<NP> row(int row, int d) const {
+        Frag<NP> f;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) f.p[i] = *reinterpret_cast<const bf16x8*>(&x[i * PLANE + row * LD + d]);
+        return f;
+    }
+    // column d0 + lane % 32 over rows row0 .. row0 + 15, in the slots' order
+    __device__ __forceinline__ Frag<NP> column(int row0, int d0, int lane) const {
+        const int at = (row0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * LD + d0 + (lane & 16) + (lane & 3) * 4;
+        Frag<NP> f;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            union { s16x4 s[2]; bf16x8 b; } u;
+            typedef __attribute__((address_space(3))) s16x4 lds4;
+            u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)&x[i * PLANE + at]);
+            u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)&x[i * PLANE + at + 8 * LD]);
+            f.p[i] = u.b;
+        }
+        return f;
+    }
+};
+
+// Rows of the tiles that a workgroup goes through.
+template <class T, int DP> struct Shape {
+    static constexpr int NP = Elem<T>::PARTS;
+    static constexpr int BN = NP == 3 && DP == 128 ? 32 : 64;
+};
+
+// This thread's share of a tile of BN rows, between its global loads and its LDS stores.
+template <class T, int DP, int BN, int NT> struct Staged {
+    static constexpr int SEGS = DP / 8, PER = BN * SEGS / NT;
+    typename Elem<T>::seg s[PER];
+    static_assert(PER * NT == BN * SEGS, "every thread takes the same number of pieces");
+
+    __device__ __forceinline__ void load(const T* base, int64_t stride, int n0, uint64_t bits, int D, bool vec, int tid) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int e = tid + i * NT, row = e / SEGS, d = e % SEGS * 8;
+            s[i] = {};
+            if (bits >> row & 1) s[i] = load_seg(base + (n0 + row) * stride, d, D, vec);
+        }
+    }
+    template <class TileT> __device__ __forceinline__ void store(TileT& t, int tid) const {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int e = tid + i * NT;
+            t.put(e / SEGS, e % SEGS * 8, s[i]);
+        }
+    }
+};
+
+// 4 bytes' truth as 4 bits
+__device__ __forceinline__ uint32_t truth4(uint32_t w) {
+    const uint32_t y = ((((w & 0x7f7f7f7fu) + 0x7f7f7f7fu) | w) >> 7) & 0x01010101u;
+    return (y * 0x10204080u) >> 28;
+}
+
+__device__ __forceinline__ uint64_t lane_u64(uint64_t x, int lane) {
+    return (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, lane) |
+           (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), lane) << 32;
+}
+
+// The keys of each tile of BN that a batch's mask keeps, one bit a key; 64 tiles are looked at together, one a lane.
+template <int BN> struct KeyBits {
+    const uint8_t* keep;       // the batch's row, or null
+    int N, window;
+    bool vec;
+    uint64_t bits;             // of tile 64 * window + lane
+
+    __device__ __forceinline__ KeyBits(const SmParams& p, int b)
+        : keep(p.keep ? p.keep + b * p.keep_stride : nullptr), N(p.N), window(-1), vec(p.vec & VEC_KEEP), bits(0) {}
+
+    __device__ __forceinline__ void look(int w) {
+        if (w == window) return;
+        window = w;
+        const int64_t n0 = ((int64_t)w * 64 + (threadIdx.x & 63)) * BN;
+        const int64_t left = N - n0;
+        bits = left <= 0 ? 0 : left >= 64 ? ~0ull : (1ull << left) - 1;
+        if (BN < 64) bits &= (1ull << BN) - 1;
+        if (!keep || left <= 0) return;
+        uint64_t seen = 0;
+        if (vec && left >= BN) {
+#pragma unroll
+            for (int j = 0; j < BN / 16; ++j) {
+                const uint4 w4 = *reinterpret_cast<const uint4*>(keep + n0 + 16 * j);
+                const uint64_t t = truth4(w4.x) | truth4(w4.y) << 4 | truth4(w4.z) << 8 | truth4(w4.w) << 12;
+                seen |= t << (16 * j);
+            }
+        } else {
+            const int n = left < BN ? (int)left : BN;
+            for (int j = 0; j < n; ++j) seen |= (uint64_t)(keep[n0 + j] != 0) << j;
+        }
+        bits &= seen;
+    }
+    __device__ __forceinline__ uint64_t of(int t) { look(t >> 6); return lane_u64(bits, t & 63); }
+    // the first tile from t on that has a key, or end
+    __device__ __forceinline__ int next(int t, int end) {
+        if (!keep) return t < end ? t : end;
+        while (t < end) {
+            look(t >> 6);
+            const uint64_t any = __ballot(bits != 0) >> (t & 63);
+            if (any) { const int f = t + __builtin_ctzll(any); return f < end ? f : end; }
+            t = (t | 63) + 1;
+        }
+        return end;
+    }
+};
+
+// The bias of one head in LDS: its column of the table in log2 units, and the borders.
+struct BiasLds {
+    float value[QLKA_MAX_BUCKETS];
+    int border[QLKA_MAX_BUCKETS];
+    __device__ __forceinline__ void fill(const SmParams& p, int head, int tid, int nt) {
+        const int nb = (p.bk.n + 1) * (p.bk.both ? 2 : 1);
+        for (int i = tid; i < nb; i += nt) value[i] = p.table[(int64_t)i * p.H + head] * LOG2E;
+        for (int i = tid; i < p.bk.n; i += nt) border[i] = p.bk.border[i];
+    }
+};
+
+// number of borders <= dist
+__device__ __forceinline__ int count_borders(const int* border, int n, int dist) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (border[mid] <= dist) lo = mid + 1; else hi = mid;
+    }
+    return lo;
+}
+// bucket of the distance diff = key - query
+__device__ __forceinline__ int bucket_of(const int* border, int n, int both, int diff) {
+    const int dist = diff <= 0 ? -diff : both ? diff : 0;
+    return count_borders(border, n, dist) + (both && diff > 0 ? n + 1 : 0);
+}
+
+// Where all distances from lo to hi are in one bucket far from the diagonal: that bucket, else -1.
+__device__ __forceinline__ int far_bucket(const SmBuckets& bk, int lo, int hi) {
+    if (hi <= -bk.far) return bk.n;
+    if (bk.both) return lo >= bk.far && lo > 0 ? 2 * bk.n + 1 : -1;
+    return lo >= 0 ? 0 : -1;
+}
+
+// A linear workgroup index -> work index: workgroups go round the 8 XCDs, so successive work goes to one XCD, whose L2
+// then serves all blocks of a head.
+__device__ __forceinline__ int xcd_work(int wg, int total) {
+    const int x = wg & 7, per = total >> 3, more = total & 7;
+    return x * per + (x < more ? x : more) + (wg >> 3);
+}
+
+// f(element, padded row length) for a call's type and row length.
+template <class F> int dispatch(int dtype, int D, F f) {
+    const int DP = sm_padded(D);
+    const auto at = [&](auto t) {
+        return DP == 32 ? f(t, std::integral_constant<int, 32>()) : DP == 64 ? f(t, std::integral_constant<int, 64>())
+                                                                            : f(t, std::integral_constant<int, 128>()); };
+    return dtype == QLKA_BF16 ? at(__bf16()) : at(float());
+}
+
+// Stores four successive elements d .. d + 3 of a row.
+template <class T> __device__ __forceinline__ void store4(T* row, int d, int D, bool vec, f32x4 x) {
+    if (vec) {
+        if (d < D) {
+            if constexpr (sizeof(T) == 2) *reinterpret_cast<bf16x4*>(row + d) = __builtin_convertvector(x, bf16x4);
+            else *reinterpret_cast<f32x4*>(row + d) = x;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (d + i < D) row[d + i] = (T)x[i];
+    }
+}
+
+}  // namespace sm
+}  // namespace qlka

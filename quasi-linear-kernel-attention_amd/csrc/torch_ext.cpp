@@ -358,6 +358,236 @@ std::vector<Tensor> abs_sum_autograd(const Tensor& q, const Tensor& k, const Ten
     return AbsSumFn::apply(q, k, v, path, full, keep);
 }
 
+// ---- softmax attention to a sequence of another length, and the bucketed position bias (qlka_softmax_*, qlka_bias_map_*)
+
+struct SoftmaxCall {
+    Tensor q, k, v, table, keep;      // table and keep may be undefined
+    double scale;
+    bool causal;
+    int64_t start;
+    std::vector<int64_t> border;
+    bool both;
+};
+
+int64_t bucket_count(const std::vector<int64_t>& border, bool both) { return ((int64_t)border.size() + 1) * (both ? 2 : 1); }
+
+void check_table(const Tensor& table, int64_t heads, const std::vector<int64_t>& border, bool both) {
+    TORCH_CHECK(table.scalar_type() == at::kFloat, "table must be float32");
+    TORCH_CHECK(table.dim() == 2 && table.size(0) == bucket_count(border, both) && table.size(1) == heads,
+                "table must be (num_buckets, H) = (", bucket_count(border, both), ", ", heads, "), got ", table.sizes());
+}
+
+void check_start(int64_t start) { TORCH_CHECK(std::abs(start) <= (1 << 28), "|start| must be <= 2^28"); }
+
+void check_softmax(const SoftmaxCall& c) {
+    const Tensor &q = c.q, &k = c.k, &v = c.v;
+    TORCH_CHECK(q.is_cuda() && k.is_cuda() && v.is_cuda(), "q, k and v must be CUDA tensors");
+    TORCH_CHECK(q.device() == k.device() && q.device() == v.device(), "q, k and v must be on one device");
+    TORCH_CHECK(q.scalar_type() == at::kFloat || q.scalar_type() == at::kBFloat16, "q must be float32 or bfloat16");
+    TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(),
+                "q, k and v must have the same dtype");
+    TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "q, k and v must be 4D: (B, heads, length, D)");
+    TORCH_CHECK(k.sizes() == v.sizes(), "k and v must have the same shape");
+    TORCH_CHECK(q.size(0) == k.size(0), "batch size must match");
+    TORCH_CHECK(q.size(3) == k.size(3), "q and k must have the same head dimension");
+    TORCH_CHECK(q.size(1) >= 1 && k.size(1) >= 1 && q.size(1) % k.size(1) == 0,
+                "the heads of q must be a multiple of those of k and v");
+    TORCH_CHECK(1 <= q.size(3) && q.size(3) <= 128, "the head dimension must be in [1, 128]");
+    TORCH_CHECK(q.size(2) <= (1 << 28) && k.size(2) <= (1 << 28), "lengths must be <= 2^28");
+    TORCH_CHECK(q.size(0) <= INT32_MAX && q.size(1) <= INT32_MAX &&
+                    (double)q.size(0) * q.size(1) * q.size(2) <= INT32_MAX &&
+                    (double)k.size(0) * k.size(1) * k.size(2) <= INT32_MAX,
+                "batch * heads * length must fit int32");
+    check_start(c.start);
+    if (c.table.defined()) {
+        TORCH_CHECK(c.table.device() == q.device(), "table must be on q's device");
+        check_table(c.table, q.size(1), c.border, c.both);
+        TORCH_CHECK(c.table.is_contiguous(), "table must be contiguous");
+    }
+    if (c.keep.defined()) {
+        TORCH_CHECK(c.keep.device() == q.device(), "keep must be on q's device");
+        TORCH_CHECK(c.keep.scalar_type() == at::kBool || c.keep.scalar_type() == at::kByte, "keep must be bool or uint8");
+        TORCH_CHECK(c.keep.dim() == 2 && c.keep.size(0) == q.size(0) && c.keep.size(1) == k.size(2),
+                    "keep must be (B, N) = (", q.size(0), ", ", k.size(2), "), got ", c.keep.sizes());
+    }
+}
+
+// rows whose elements are next to each other
+Tensor packed_rows(const Tensor& t) { return t.size(3) == 1 || t.stride(3) == 1 ? t : t.contiguous(); }
+// an output laid out as t is
+Tensor empty_rows(const Tensor& t) {
+    Tensor r = at::empty_like(t);
+    return t.size(3) == 1 || r.stride(3) == 1 ? r : at::empty(t.sizes(), t.options());
+}
+void set_strides(int64_t* to, const Tensor& t) {
+    for (int i = 0; i < 3; ++i) to[i] = t.stride(i);
+}
+
+// Sizes, inputs and the bias of a call; border has to outlive the arguments.
+qlka_softmax_args softmax_args(const SoftmaxCall& c, const std::vector<int>& border) {
+    qlka_softmax_args a{};
+    a.dtype = c.q.scalar_type() == at::kFloat ? QLKA_F32 : QLKA_BF16;
+    a.B = (int)c.q.size(0); a.H = (int)c.q.size(1); a.G = (int)c.k.size(1);
+    a.M = (int)c.q.size(2); a.N = (int)c.k.size(2); a.D = (int)c.q.size(3);
+    a.causal = c.causal;
+    a.start = (int)c.start;
+    a.scale = (float)c.scale;
+    a.q = c.q.data_ptr(); a.k = c.k.data_ptr(); a.v = c.v.data_ptr();
+    set_strides(a.q_stride, c.q); set_strides(a.k_stride, c.k); set_strides(a.v_stride, c.v);
+    if (c.keep.defined()) {
+        a.keep = (const uint8_t*)c.keep.data_ptr();
+        a.keep_stride = c.keep.stride(0);
+    }
+    if (c.table.defined()) {
+        a.table = c.table.data_ptr<float>();
+        a.border = border.data();
+        a.num_borders = (int)border.size();
+        a.bidirectional = c.both;
+    }
+    return a;
+}
+
+// (out, what rounding it to bfloat16 cut off, the rows' log sums); the last where a gradient will be wanted, the second where
+// the table's will
+std::tuple<Tensor, Tensor, Tensor> softmax_forward(SoftmaxCall& c, bool train, bool train_table) {
+    check_softmax(c);
+    c10::DeviceGuard guard(c.q.device());
+    c.q = packed_rows(c.q);
+    c.k = packed_rows(c.k);
+    c.v = packed_rows(c.v);
+    if (c.keep.defined() && c.keep.size(1) > 1 && c.keep.stride(1) != 1) c.keep = c.keep.contiguous();
+    Tensor out = empty_rows(c.q), lo, lse;
+    const std::vector<int> border(c.border.begin(), c.border.end());
+    qlka_softmax_args a = softmax_args(c, border);
+    a.out = out.data_ptr();
+    set_strides(a.out_stride, out);
+    if (train) {
+        lse = at::empty({a.B, a.H, a.M}, c.q.options().dtype(at::kFloat));
+        a.lse = lse.data_ptr<float>();
+        if (a.dtype == QLKA_BF16 && train_table) {
+            lo = at::empty_strided(out.sizes(), out.strides(), out.options());
+            a.out_lo = lo.data_ptr();
+        }
+    }
+    const size_t bytes = qlka_softmax_fwd_ws_bytes(&a);
+    Tensor ws;
+    if (bytes) ws = workspace(bytes, c.q);
+    check_rc(qlka_softmax_fwd(&a, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(c.q)));
+    return {out, lo, lse};
+}
+
+struct SoftmaxFn : public torch::autograd::Function<SoftmaxFn> {
+    static Tensor forward(AutogradContext* ctx, Tensor q, Tensor k, Tensor v, OptTensor table_, OptTensor keep_,
+                          double scale, bool causal, int64_t start, std::vector<int64_t> border, bool both) {
+        ctx->set_materialize_grads(false);
+        const Tensor table = table_.value_or(Tensor()), keep = keep_.value_or(Tensor());
+        SoftmaxCall c{q, k, v, table, keep, scale, causal, start, border, both};
+        Tensor out, lo, lse;
+        std::tie(out, lo, lse) = softmax_forward(c, true, table.defined() && table.requires_grad());
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["causal"] = causal;
+        ctx->saved_data["start"] = start;
+        ctx->saved_data["border"] = border;
+        ctx->saved_data["both"] = both;
+        ctx->save_for_backward({c.q, c.k, c.v, c.table, c.keep, out, lo, lse});
+        return out;
+    }
+
+    static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "softmax_attention has no second derivative");
+        tensor_list r(10);
+        if (!grads[0].defined()) return r;
+        const auto s = ctx->get_saved_variables();
+        const SoftmaxCall c{s[0], s[1], s[2], s[3], s[4], ctx->saved_data["scale"].toDouble(),
+                            ctx->saved_data["causal"].toBool(), ctx->saved_data["start"].toInt(),
+                            ctx->saved_data["border"].toIntVector(), ctx->saved_data["both"].toBool()};
+        const Tensor &out = s[5], &lo = s[6], &lse = s[7];
+        c10::DeviceGuard guard(c.q.device());
+        const std::vector<int> border(c.border.begin(), c.border.end());
+        qlka_softmax_args a = softmax_args(c, border);
+        const Tensor g = packed_rows(grads[0]);
+        a.out = out.data_ptr();
+        set_strides(a.out_stride, out);
+        if (lo.defined()) a.out_lo = lo.data_ptr();
+        a.lse = lse.data_ptr<float>();
+        a.g_out = g.data_ptr();
+        set_strides(a.g_out_stride, g);
+        if (ctx->needs_input_grad(0)) {
+            r[0] = empty_rows(c.q);
+            a.g_q = r[0].data_ptr();
+            set_strides(a.g_q_stride, r[0]);
+        }
+        if (ctx->needs_input_grad(1) || ctx->needs_input_grad(2)) {
+            r[1] = empty_rows(c.k);
+            r[2] = empty_rows(c.v);
+            a.g_k = r[1].data_ptr();
+            a.g_v = r[2].data_ptr();
+            set_strides(a.g_k_stride, r[1]);
+            set_strides(a.g_v_stride, r[2]);
+        }
+        if (c.table.defined() && ctx->needs_input_grad(3)) {
+            r[3] = at::empty_like(c.table);
+            a.g_table = r[3].data_ptr<float>();
+        }
+        const size_t bytes = qlka_softmax_bwd_ws_bytes(&a);
+        Tensor ws;
+        if (bytes) ws = workspace(bytes, c.q);
+        check_rc(qlka_softmax_bwd(&a, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(c.q)));
+        return r;
+    }
+};
+
+Tensor softmax_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& table, const OptTensor& keep,
+                         double scale, bool causal, int64_t start, const std::vector<int64_t>& border, bool both) {
+    const Tensor t = table.value_or(Tensor()), m = keep.value_or(Tensor());
+    if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() ||
+                                       (t.defined() && t.requires_grad())))
+        return SoftmaxFn::apply(q, k, v, table, keep, scale, causal, start, border, both);
+    SoftmaxCall c{q, k, v, t, m, scale, causal, start, border, both};
+    return std::get<0>(softmax_forward(c, false, false));
+}
+
+struct BiasMapFn : public torch::autograd::Function<BiasMapFn> {
+    static Tensor forward(AutogradContext* ctx, Tensor table, int64_t M, int64_t N, int64_t start,
+                          std::vector<int64_t> border, bool both) {
+        TORCH_CHECK(table.is_cuda(), "table must be a CUDA tensor");
+        TORCH_CHECK(table.dim() == 2 && table.size(1) >= 1, "table must be (num_buckets, H)");
+        check_table(table, table.size(1), border, both);
+        TORCH_CHECK(M >= 0 && N >= 0 && M <= (1 << 21) && N <= (1 << 21), "lengths must be in [0, 2^21]");
+        check_start(start);
+        c10::DeviceGuard guard(table.device());
+        const Tensor t = table.contiguous();
+        const std::vector<int> b(border.begin(), border.end());
+        Tensor out = at::empty({t.size(1), M, N}, t.options());
+        check_rc(qlka_bias_map_fwd(t.data_ptr<float>(), b.data(), (int)b.size(), both, out.data_ptr<float>(),
+                                   (int)t.size(1), (int)M, (int)N, (int)start, stream_of(t)));
+        ctx->saved_data["start"] = start;
+        ctx->saved_data["border"] = border;
+        ctx->saved_data["both"] = both;
+        return out;
+    }
+
+    static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "relative_bias has no second derivative");
+        const Tensor g = grads[0].contiguous();
+        const std::vector<int64_t> border = ctx->saved_data["border"].toIntVector();
+        const bool both = ctx->saved_data["both"].toBool();
+        const std::vector<int> b(border.begin(), border.end());
+        const int H = (int)g.size(0), M = (int)g.size(1), N = (int)g.size(2);
+        c10::DeviceGuard guard(g.device());
+        Tensor gt = at::empty({bucket_count(border, both), H}, g.options());
+        const size_t bytes = qlka_bias_map_bwd_ws_bytes((int)b.size(), both, H, M, N);
+        Tensor ws = workspace(bytes, g);
+        check_rc(qlka_bias_map_bwd(g.data_ptr<float>(), b.data(), (int)b.size(), both, gt.data_ptr<float>(), H, M, N,
+                                   (int)ctx->saved_data["start"].toInt(), ws.data_ptr(), bytes, stream_of(g)));
+        return {gt, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+Tensor relative_bias(const Tensor& table, int64_t M, int64_t N, int64_t start, const std::vector<int64_t>& border, bool both) {
+    return BiasMapFn::apply(table, M, N, start, border, both);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -394,5 +624,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("full"), py::arg("keep"),
           "differentiable weighted_abs_sum (full=False: [out]) / weighted_abs_sum_full ([out_w, out_u]); path "
           "-1/0/1, or 2 for the dense route with sign(0) = 0 in the backward");
+    m.def("softmax_attention", &softmax_attention, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("table"),
+          py::arg("keep"), py::arg("scale"), py::arg("causal"), py::arg("start"), py::arg("border"), py::arg("both"),
+          "differentiable softmax attention (qlka_softmax_fwd / qlka_softmax_bwd)");
+    m.def("relative_bias", &relative_bias, py::arg("table"), py::arg("M"), py::arg("N"), py::arg("start"),
+          py::arg("border"), py::arg("both"), "differentiable bias map (qlka_bias_map_fwd / qlka_bias_map_bwd)");
     m.attr("DIRECT") = DIRECT;
 }

@@ -19,6 +19,25 @@ EXT_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_qlka_torch
 _c_int = ctypes.c_int
 _c_size = ctypes.c_size_t
 _c_ptr = ctypes.c_void_p
+_c_i64x3 = ctypes.c_int64 * 3
+
+
+class SoftmaxArgs(ctypes.Structure):
+    """qlka_softmax_args of include/qlka.h."""
+    _fields_ = ([(n, _c_int) for n in ("dtype", "B", "H", "G", "M", "N", "D", "causal", "start")]
+                + [("scale", ctypes.c_float)]
+                + [(n, _c_ptr) for n in ("q", "k", "v")]
+                + [(n, _c_i64x3) for n in ("q_stride", "k_stride", "v_stride")]
+                + [("keep", _c_ptr), ("keep_stride", ctypes.c_int64), ("table", _c_ptr),
+                   ("border", ctypes.POINTER(_c_int)), ("num_borders", _c_int), ("bidirectional", _c_int),
+                   ("out", _c_ptr), ("out_lo", _c_ptr), ("out_stride", _c_i64x3), ("lse", _c_ptr),
+                   ("g_out", _c_ptr), ("g_out_stride", _c_i64x3), ("g_q", _c_ptr), ("g_k", _c_ptr), ("g_v", _c_ptr)]
+                + [(n, _c_i64x3) for n in ("g_q_stride", "g_k_stride", "g_v_stride")]
+                + [("g_table", _c_ptr)])
+
+
+_c_softmax = ctypes.POINTER(SoftmaxArgs)
+_c_border = [ctypes.POINTER(_c_int), _c_int, _c_int]       # border, num_borders, bidirectional
 
 # name -> (restype, argtypes)
 _SIGNATURES = {
@@ -46,6 +65,13 @@ _SIGNATURES = {
     "qlka_layer_fwd_ws_bytes": (_c_size, [_c_int] * 6),
     "qlka_layer_fwd": (_c_int, [_c_int] + [_c_ptr] * 5 + [_c_int] * 5 + [_c_ptr, _c_size, _c_ptr]),
     "qlka_layer_fwd_masked": (_c_int, [_c_int] + [_c_ptr] * 5 + [_c_int] * 5 + [_c_ptr, _c_size, _c_ptr]),
+    "qlka_softmax_fwd_ws_bytes": (_c_size, [_c_softmax]),
+    "qlka_softmax_fwd": (_c_int, [_c_softmax, _c_ptr, _c_size, _c_ptr]),
+    "qlka_softmax_bwd_ws_bytes": (_c_size, [_c_softmax]),
+    "qlka_softmax_bwd": (_c_int, [_c_softmax, _c_ptr, _c_size, _c_ptr]),
+    "qlka_bias_map_fwd": (_c_int, [_c_ptr] + _c_border + [_c_ptr] + [_c_int] * 4 + [_c_ptr]),
+    "qlka_bias_map_bwd_ws_bytes": (_c_size, [_c_int] * 5),
+    "qlka_bias_map_bwd": (_c_int, [_c_ptr] + _c_border + [_c_ptr] + [_c_int] * 4 + [_c_ptr, _c_size, _c_ptr]),
     "qlka_seg_sort_ws_bytes": (_c_size, [_c_int] * 2),
     "qlka_seg_sort": (_c_int, [_c_ptr] * 3 + [_c_int] * 2 + [_c_ptr, _c_size, _c_ptr]),
     "qlka_merge_rank_ws_bytes": (_c_size, [_c_int] * 3),
