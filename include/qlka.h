@@ -244,10 +244,10 @@ int qlka_layer_fwd_masked(int kind, const float* q, const float* k, const float*
  * keys after the query (d > 0) in buckets num_borders + 1 on, 2 (num_borders + 1) buckets in all. Else distance max(-d, 0)
  * and num_borders + 1 buckets. table and g_table are (buckets, H) fp32, contiguous.
  *
- * Forward: writes out and, where not NULL, lse (B, H, M) (log2 of each row's sum, +inf for a row without keys) and out_lo
- * (with QLKA_BF16 and a table: what rounding out cut off, same strides as out; the probabilities are then taken to 16 bits).
- * Backward: reads q, k, v, out, lse, g_out and, where not NULL, out_lo, writes g_q (may be NULL), g_k and g_v (both or neither
- * NULL) and g_table (may be NULL; with QLKA_BF16 it needs out_lo). No atomics: results do not change from run to run.
+ * Forward: writes out and, where not NULL, lse (B, H, M) (log2 of each row's sum, +inf for a row without keys) and out_full
+ * (with QLKA_BF16 and a table: (B, H, M, D) fp32, out before it is rounded; the probabilities are then taken to 16 bits).
+ * Backward: reads q, k, v, out, lse, g_out and, where not NULL, out_full, writes g_q (may be NULL), g_k and g_v (both or
+ * neither NULL) and g_table (may be NULL; with QLKA_BF16 it needs out_full). No atomics: results do not change from run to run.
  */
 #define QLKA_F32  0
 #define QLKA_BF16 1
@@ -263,8 +263,9 @@ typedef struct qlka_softmax_args {
     const float* table;
     const int* border;
     int num_borders, bidirectional;
-    void *out, *out_lo;
+    void* out;
     int64_t out_stride[3];
+    float* out_full;
     float* lse;
     const void* g_out;
     int64_t g_out_stride[3];

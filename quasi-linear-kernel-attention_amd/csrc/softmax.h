@@ -26,7 +26,8 @@ struct SmBuckets {
 
 struct SmParams {
     const void *q, *k, *v, *g_out;
-    void *out, *out_lo, *g_q, *g_k, *g_v;
+    void *out, *g_q, *g_k, *g_v;
+    float* out_full;                         // [B][H][M][D], or null
     SmStrides sq, sk, sv, so, sg, sgq, sgk, sgv;
     const uint8_t* keep;                     // [B] rows of N bytes, keep_stride apart, or null
     int64_t keep_stride;
@@ -45,7 +46,8 @@ struct SmParams {
     SmBuckets bk;
 };
 
-enum SmVec : int { VEC_Q = 1, VEC_K = 2, VEC_V = 4, VEC_G = 8, VEC_O = 16, VEC_GQ = 32, VEC_GK = 64, VEC_GV = 128, VEC_KEEP = 256 };
+enum SmVec : int { VEC_Q = 1, VEC_K = 2, VEC_V = 4, VEC_G = 8, VEC_O = 16, VEC_GQ = 32, VEC_GK = 64, VEC_GV = 128, VEC_KEEP = 256,
+                   VEC_FULL = 512 };
 
 // Elements of a row in LDS and in the partial rows.
 inline int sm_padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }

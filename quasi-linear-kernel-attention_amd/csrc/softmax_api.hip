@@ -136,7 +136,7 @@ bool in_pieces(const qlka_softmax_args* a, const void* x, const int64_t* s, int 
 int params(const qlka_softmax_args* a, SmParams* p) {
     *p = SmParams{};
     p->q = a->q; p->k = a->k; p->v = a->v; p->g_out = a->g_out;
-    p->out = a->out; p->out_lo = a->out_lo;
+    p->out = a->out; p->out_full = a->out_full;
     p->g_q = a->g_q; p->g_k = a->g_k; p->g_v = a->g_v;
     p->sq = strides(a->q_stride); p->sk = strides(a->k_stride); p->sv = strides(a->v_stride);
     p->so = strides(a->out_stride); p->sg = strides(a->g_out_stride);
@@ -156,7 +156,8 @@ int params(const qlka_softmax_args* a, SmParams* p) {
              bit(VEC_V, a->v, a->v_stride, a->G, a->N) | bit(VEC_G, a->g_out, a->g_out_stride, a->H, a->M) |
              bit(VEC_GQ, a->g_q, a->g_q_stride, a->H, a->M) | bit(VEC_GK, a->g_k, a->g_k_stride, a->G, a->N) |
              bit(VEC_GV, a->g_v, a->g_v_stride, a->G, a->N);
-    if (bit(1, a->out, a->out_stride, a->H, a->M) && (uintptr_t)a->out_lo % 16 == 0) p->vec |= VEC_O;
+    p->vec |= bit(VEC_O, a->out, a->out_stride, a->H, a->M);
+    if (a->D % 8 == 0 && (uintptr_t)a->out_full % 16 == 0) p->vec |= VEC_FULL;
     if ((uintptr_t)a->keep % 16 == 0 && (a->B <= 1 || a->keep_stride % 16 == 0)) p->vec |= VEC_KEEP;
     return a->table ? check_buckets(a->border, a->num_borders, a->bidirectional, &p->bk) : QLKA_OK;
 }
@@ -188,7 +189,7 @@ int qlka_softmax_fwd(const qlka_softmax_args* a, void* ws, size_t ws_bytes, void
     if (int e = params(a, &p)) return e;
     if (a->B == 0 || a->M == 0) return QLKA_OK;
     if (!a->q || !a->out || (a->N > 0 && (!a->k || !a->v))) return refuse("q, k, v and out must be non-null");
-    if (a->out_lo && (a->dtype == QLKA_F32 || !a->table)) return refuse("out_lo goes with QLKA_BF16 and a table");
+    if (a->out_full && (a->dtype == QLKA_F32 || !a->table)) return refuse("out_full goes with QLKA_BF16 and a table");
     const FwdPlan f = fwd_plan(a);
     if (int e = need_ws(ws, ws_bytes, f.part + f.part2)) return e;
     if (int e = fits_grid((int64_t)a->B * (f.step ? a->G : a->H) * std::max(f.rows.blocks, 1) * f.rows.splits)) return e;
@@ -226,8 +227,8 @@ int qlka_softmax_bwd(const qlka_softmax_args* a, void* ws, size_t ws_bytes, void
     const bool rows = (int64_t)a->B * a->M > 0, keys = (int64_t)a->B * a->N > 0;
     if (rows && (!a->q || !a->out || !a->lse || !a->g_out)) return refuse("q, out, lse and g_out must be non-null");
     if (keys && (!a->k || !a->v)) return refuse("k and v must be non-null");
-    if (a->out_lo && (a->dtype == QLKA_F32 || !a->table)) return refuse("out_lo goes with QLKA_BF16 and a table");
-    if (rows && a->g_table && a->dtype == QLKA_BF16 && !a->out_lo) return refuse("g_table needs out_lo with QLKA_BF16");
+    if (a->out_full && (a->dtype == QLKA_F32 || !a->table)) return refuse("out_full goes with QLKA_BF16 and a table");
+    if (rows && a->g_table && a->dtype == QLKA_BF16 && !a->out_full) return refuse("g_table needs out_full with QLKA_BF16");
     const BwdPlan w = bwd_plan(a, a->g_q, a->g_k, a->g_table);
     if (int e = need_ws(ws, ws_bytes, w.delta + w.part + w.part2 + w.table)) return e;
     if (int e = fits_grid((int64_t)a->B * a->H * w.dq.blocks * w.dq.splits)) return e;

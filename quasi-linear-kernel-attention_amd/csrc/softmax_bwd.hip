@@ -27,11 +27,10 @@ __global__ __launch_bounds__(256) void softmax_delta(const SmParams p) {
         const int m = (int)(row % p.M), head = (int)(row / p.M % p.H), b = (int)(row / p.M / p.H);
         const T* out = (const T*)p.out + b * p.so.b + head * p.so.h + m * p.so.r;
         const auto g = load_seg((const T*)p.g_out + b * p.sg.b + head * p.sg.h + m * p.sg.r, d, p.D, p.vec & VEC_G);
-        const auto o = load_seg(out, d, p.D, p.vec & VEC_O);
-        typename Elem<T>::seg lo = {};
-        if (p.out_lo) lo = load_seg((const T*)p.out_lo + (out - (const T*)p.out), d, p.D, p.vec & VEC_O);
+        const f32x8 o = p.out_full ? load_seg(p.out_full + row * p.D, d, p.D, p.vec & VEC_FULL)
+                                   : floats(load_seg(out, d, p.D, p.vec & VEC_O));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x = __builtin_fmaf((float)g[i], (float)o[i] + (float)lo[i], x);
+        for (int i = 0; i < 8; ++i) x = __builtin_fmaf((float)g[i], o[i], x);
     }
 #pragma unroll
     for (int far = 1; far < LANES; far *= 2) x += __shfl_xor(x, far);
@@ -115,7 +114,7 @@ __global__ __launch_bounds__(64 * NW) void softmax_dq(const SmParams p) {
     KeyBits<BN> seen(p, b);
     Staged<T, DP, BN, NT> ks, vs;
     const float c2 = p.scale * LOG2E;
-    f32x16 dq[ND] = {};
+    Acc<NP, NP == 3 && DP < 128> dq[ND];
 
     int t = seen.next(t0, t1);
     if (t < t1) {
@@ -158,11 +157,13 @@ __global__ __launch_bounds__(64 * NW) void softmax_dq(const SmParams p) {
         const float* nb = &near_bias[BIAS ? ROWS - 1 - wave * 32 - col + 4 * half : 0];
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            f32x16 s = {}, dp = {};
+            Acc<NP> sa, dpa;
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) s = mma(kt.row(32 * i + col, 16 * c + 8 * half), qf[c], s);
+            for (int c = 0; c < DP / 16; ++c) sa.add(kt.row(32 * i + col, 16 * c + 8 * half), qf[c]);
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) dp = mma(vt.row(32 * i + col, 16 * c + 8 * half), gf[c], dp);
+            for (int c = 0; c < DP / 16; ++c) dpa.add(vt.row(32 * i + col, 16 * c + 8 * half), gf[c]);
+            f32x16 s = sa.sum();
+            const f32x16 dp = dpa.sum();
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int n = 32 * i + reg_row(r);
@@ -188,7 +189,7 @@ __global__ __launch_bounds__(64 * NW) void softmax_dq(const SmParams p) {
                 for (int j = 0; j < 8; ++j) x[j] = s[8 * c + j];
                 const Frag<NP> df = split<NP>(x);
 #pragma unroll
-                for (int d = 0; d < ND; ++d) dq[d] = mma(kt.column(32 * i + 16 * c, 32 * d, lane), df, dq[d]);
+                for (int d = 0; d < ND; ++d) dq[d].add(kt.column(32 * i + 16 * c, 32 * d, lane), df);
             }
         }
     }
@@ -218,7 +219,7 @@ __global__ __launch_bounds__(64 * NW) void softmax_dq(const SmParams p) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int at = 32 * d + 8 * r + 4 * half;
-            f32x4 x = {dq[d][4 * r], dq[d][4 * r + 1], dq[d][4 * r + 2], dq[d][4 * r + 3]};
+            const f32x4 x = quad(dq[d].sum(), r);
             if (p.splits > 1)
                 *reinterpret_cast<f32x4*>(p.part + ((int64_t)split_i * p.B * p.H * p.M + row) * DP + at) = x;
             else
@@ -281,7 +282,7 @@ __global__ __launch_bounds__(64 * NW) void softmax_dkv(const SmParams p) {
         }
     };
     const float c2 = p.scale * LOG2E;
-    f32x16 dk[ND] = {}, dv[ND] = {};
+    Acc<NP, NP == 3 && DP < 128> dk[ND], dv[ND];
     int filled = -1;                                   // the head whose bias stands in LDS
 
     int t = next((int)(work * split_i / p.splits));
@@ -323,11 +324,12 @@ __global__ __launch_bounds__(64 * NW) void softmax_dkv(const SmParams p) {
         const float* nb = &near_bias[BIAS ? wave * 32 + col + BM - 1 - 4 * half : 0];
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            f32x16 s = {}, dp = {};
+            Acc<NP> sa, dpa;
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) s = mma(qt.row(32 * i + col, 16 * c + 8 * half), kf[c], s);
+            for (int c = 0; c < DP / 16; ++c) sa.add(qt.row(32 * i + col, 16 * c + 8 * half), kf[c]);
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) dp = mma(gt.row(32 * i + col, 16 * c + 8 * half), vf[c], dp);
+            for (int c = 0; c < DP / 16; ++c) dpa.add(gt.row(32 * i + col, 16 * c + 8 * half), vf[c]);
+            f32x16 s = sa.sum(), dp = dpa.sum();
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
                 const f32x4 l4 = *reinterpret_cast<const f32x4*>(&lse[32 * i + 8 * r4 + 4 * half]);
@@ -354,8 +356,8 @@ __global__ __launch_bounds__(64 * NW) void softmax_dkv(const SmParams p) {
                 const Frag<NP> pf = split<NP>(x), df = split<NP>(y);
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
-                    dv[d] = mma(gt.column(32 * i + 16 * c, 32 * d, lane), pf, dv[d]);
-                    dk[d] = mma(qt.column(32 * i + 16 * c, 32 * d, lane), df, dk[d]);
+                    dv[d].add(gt.column(32 * i + 16 * c, 32 * d, lane), pf);
+                    dk[d].add(qt.column(32 * i + 16 * c, 32 * d, lane), df);
                 }
             }
         }
@@ -368,8 +370,8 @@ __global__ __launch_bounds__(64 * NW) void softmax_dkv(const SmParams p) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int at = 32 * d + 8 * r + 4 * half;
-            f32x4 x = {dk[d][4 * r], dk[d][4 * r + 1], dk[d][4 * r + 2], dk[d][4 * r + 3]};
-            f32x4 y = {dv[d][4 * r], dv[d][4 * r + 1], dv[d][4 * r + 2], dv[d][4 * r + 3]};
+            const f32x4 x = quad(dk[d].sum(), r);
+            const f32x4 y = quad(dv[d].sum(), r);
             if (p.splits > 1) {
                 *reinterpret_cast<f32x4*>(p.part + (split_i * all + row) * DP + at) = x;
                 *reinterpret_cast<f32x4*>(p.part2 + (split_i * all + row) * DP + at) = y;

@@ -62,7 +62,7 @@ __global__ __launch_bounds__(64 * NW) void softmax_fwd(const SmParams p) {
     KeyBits<BN> seen(p, b);
     Staged<T, DP, BN, NT> ks, vs;
     const float c2 = p.scale * LOG2E;
-    f32x16 o[ND] = {};
+    Acc<NP> o[ND];
     float top = -std::numeric_limits<float>::infinity(), ref = 0.f, sum = 0.f;
 
     int t = seen.next(t0, t1);
@@ -100,11 +100,14 @@ __global__ __launch_bounds__(64 * NW) void softmax_fwd(const SmParams p) {
         t = tn;
         if (mw >= p.M || (p.causal && n0 > mw + 31 + p.start)) continue;
 
-        f32x16 s[NS] = {};
+        f32x16 s[NS];
 #pragma unroll
-        for (int i = 0; i < NS; ++i)
+        for (int i = 0; i < NS; ++i) {
+            Acc<NP> a;
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) s[i] = mma(kt.row(32 * i + col, 16 * c + 8 * half), qf[c], s[i]);
+            for (int c = 0; c < DP / 16; ++c) a.add(kt.row(32 * i + col, 16 * c + 8 * half), qf[c]);
+            s[i] = a.sum();
+        }
 
         // scores in log2 units are fma(s, mul, add) from here on
         float mul = c2, add = far;
@@ -141,7 +144,7 @@ __global__ __launch_bounds__(64 * NW) void softmax_fwd(const SmParams p) {
             const float f = first ? 1.f : fexp2(was - ref);               // the first time there is nothing to scale
             sum *= f;
 #pragma unroll
-            for (int d = 0; d < ND; ++d) o[d] *= f;
+            for (int d = 0; d < ND; ++d) o[d].scale(f);
         }
         add -= ref;
 #pragma unroll
@@ -160,13 +163,16 @@ __global__ __launch_bounds__(64 * NW) void softmax_fwd(const SmParams p) {
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
                     const Frag<NP> vf = vt.column(32 * i + 16 * c, 32 * d, lane);
-                    if constexpr (FINE) o[d] = mma(vf, rest, o[d]);
-                    o[d] = mma(vf, pf, o[d]);
+                    if constexpr (FINE) o[d].add(vf, rest);
+                    o[d].add(vf, pf);
                 }
             }
     }
     if (m >= p.M) return;
     sum += other_half(sum);
+    f32x16 os[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) os[d] = o[d].sum();
     const int64_t row = ((int64_t)b * p.H + head) * p.M + m;
     if (p.splits > 1) {
         const int64_t at = (int64_t)split_i * p.B * p.H * p.M + row;
@@ -175,7 +181,7 @@ __global__ __launch_bounds__(64 * NW) void softmax_fwd(const SmParams p) {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 *reinterpret_cast<f32x4*>(p.part + at * DP + 32 * d + 8 * r + 4 * half) =
-                    f32x4{o[d][4 * r], o[d][4 * r + 1], o[d][4 * r + 2], o[d][4 * r + 3]};
+                    quad(os[d], r);
         if (half == 0) {
             p.part2[2 * at] = ref;
             p.part2[2 * at + 1] = sum;
@@ -184,21 +190,13 @@ __global__ __launch_bounds__(64 * NW) void softmax_fwd(const SmParams p) {
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     T* out = (T*)p.out + b * p.so.b + head * p.so.h + m * p.so.r;
-    T* lo = p.out_lo ? (T*)p.out_lo + b * p.so.b + head * p.so.h + m * p.so.r : nullptr;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            f32x4 x;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = o[d][4 * r + i] * inv;
+            const f32x4 x = quad(os[d], r) * inv;
             store4(out, 32 * d + 8 * r + 4 * half, p.D, p.vec & VEC_O, x);
-            if constexpr (FINE) {
-                if (lo) {
-                    x = x - __builtin_convertvector(__builtin_convertvector(x, bf16x4), f32x4);
-                    store4(lo, 32 * d + 8 * r + 4 * half, p.D, p.vec & VEC_O, x);
-                }
-            }
+            if constexpr (FINE) store4(p.out_full + row * p.D, 32 * d + 8 * r + 4 * half, p.D, p.vec & VEC_FULL, x);
         }
     if (p.lse && half == 0)
         p.lse[row] = sum == 0.f ? std::numeric_limits<float>::infinity() : ref + __log2f(sum);
@@ -206,7 +204,7 @@ __global__ __launch_bounds__(64 * NW) void softmax_fwd(const SmParams p) {
 
 template <class T, int DP, int NW> int launch_fwd(const SmParams& p, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)p.B * p.H * p.blocks * p.splits));
-    if (sizeof(T) == 2 && p.out_lo) softmax_fwd<T, DP, NW, true, sizeof(T) == 2><<<grid, 64 * NW, 0, st>>>(p);
+    if (sizeof(T) == 2 && p.out_full) softmax_fwd<T, DP, NW, true, sizeof(T) == 2><<<grid, 64 * NW, 0, st>>>(p);
     else if (p.table) softmax_fwd<T, DP, NW, true, false><<<grid, 64 * NW, 0, st>>>(p);
     else softmax_fwd<T, DP, NW, false, false><<<grid, 64 * NW, 0, st>>>(p);
     return (int)hipGetLastError();
@@ -239,12 +237,7 @@ __global__ __launch_bounds__(256) void softmax_combine(const SmParams p) {
     const int m = (int)(row % p.M), head = (int)(row / p.M % p.H), b = (int)(row / p.M / p.H);
     const int64_t at = b * p.so.b + head * p.so.h + m * p.so.r;
     store4((T*)p.out + at, d, p.D, p.vec & VEC_O, x);
-    if constexpr (sizeof(T) == 2) {
-        if (p.out_lo) {
-            x = x - __builtin_convertvector(__builtin_convertvector(x, bf16x4), f32x4);
-            store4((T*)p.out_lo + at, d, p.D, p.vec & VEC_O, x);
-        }
-    }
+    if (p.out_full) store4(p.out_full + row * p.D, d, p.D, p.vec & VEC_FULL, x);
     if (p.lse && d == 0) p.lse[row] = sum == 0.f ? std::numeric_limits<float>::infinity() : ref + __log2f(sum);
 }
 

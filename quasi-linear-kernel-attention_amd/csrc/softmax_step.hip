@@ -27,9 +27,6 @@ template <int LANES> __device__ __forceinline__ float row_sum(float x) {
     return x;
 }
 
-__device__ __forceinline__ f32x8 floats(bf16x8 x) { return __builtin_convertvector(x, f32x8); }
-__device__ __forceinline__ f32x8 floats(f32x8 x) { return x; }
-
 template <class T, int DP, int R, bool BIAS>
 __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p) {
     constexpr int LANES = DP / 8, KEYS = 64 / LANES, U = STEP_LOADS, NW = STEP_WAVES, NT = 64 * NW;
@@ -183,9 +180,8 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p
         x = s == 0.f ? 0.f : x / s;
         if (c < p.D) {
             const int64_t at = b * p.so.b + head * p.so.h + m * p.so.r + c;
-            const T y = (T)x;
-            ((T*)p.out)[at] = y;
-            if (sizeof(T) == 2 && p.out_lo) ((T*)p.out_lo)[at] = (T)(x - (float)y);
+            ((T*)p.out)[at] = (T)x;
+            if (p.out_full) p.out_full[row * p.D + c] = x;
         }
         if (p.lse && c == 0) p.lse[row] = s == 0.f ? std::numeric_limits<float>::infinity() : ref + __log2f(s);
     }

@@ -54,17 +54,37 @@ __device__ __forceinline__ Frag<3> frag_of(f32x8 x) { return split<3>(x); }
 __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
-template <int NP> __device__ __forceinline__ f32x16 mma(const Frag<NP>& a, const Frag<NP>& b, f32x16 c) {
-    if constexpr (NP == 3) {
-        c = mfma(a.p[0], b.p[2], c);
-        c = mfma(a.p[2], b.p[0], c);
-        c = mfma(a.p[1], b.p[1], c);
-        c = mfma(a.p[0], b.p[1], c);
-        c = mfma(a.p[1], b.p[0], c);
+// A sum of products. The matrix instruction drops what of a product lies a few bits below the sum's last one, always
+// downwards: 0.007 of a last place an instruction, measured, which a long sum of few signs would show. So the five
+// products of the smaller parts gather in a sum of their own (APART), 2^-8 as large; where registers do not reach for it (rows
+// of 128 in the backward) they do not.
+template <int NP, bool APART = NP == 3> struct Acc {
+    f32x16 main = {}, rest = {};
+    __device__ __forceinline__ void add(const Frag<NP>& a, const Frag<NP>& b) {
+        if constexpr (NP == 3) {
+            f32x16& r = APART ? rest : main;
+            r = mfma(a.p[0], b.p[2], r);
+            r = mfma(a.p[2], b.p[0], r);
+            r = mfma(a.p[1], b.p[1], r);
+            r = mfma(a.p[0], b.p[1], r);
+            r = mfma(a.p[1], b.p[0], r);
+        }
+        main = mfma(a.p[0], b.p[0], main);
     }
-    return mfma(a.p[0], b.p[0], c);
-}
+    __device__ __forceinline__ void scale(float f) {
+        main *= f;
+        if constexpr (APART) rest *= f;
+    }
+    __device__ __forceinline__ f32x16 sum() const {
+        if constexpr (APART) return main + rest;
+        else return main;
+    }
+};
 
+__device__ __forceinline__ f32x8 floats(bf16x8 x) { return __builtin_convertvector(x, f32x8); }
+__device__ __forceinline__ f32x8 floats(f32x8 x) { return x; }
+// registers 4 r .. 4 r + 3: four successive rows of a result
+__device__ __forceinline__ f32x4 quad(f32x16 x, int r) { return f32x4{x[4 * r], x[4 * r + 1], x[4 * r + 2], x[4 * r + 3]}; }
 __device__ __forceinline__ float fexp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
 __device__ __forceinline__ int reg_row(int r) { return (r >> 2) * 8 + (r & 3); }   // + 4 (lane / 32)

@@ -447,7 +447,7 @@ qlka_softmax_args softmax_args(const SoftmaxCall& c, const std::vector<int>& bor
     return a;
 }
 
-// (out, what rounding it to bfloat16 cut off, the rows' log sums); the last where a gradient will be wanted, the second where
+// (out, out before its rounding to bfloat16, the rows' log sums); the last where a gradient will be wanted, the second where
 // the table's will
 std::tuple<Tensor, Tensor, Tensor> softmax_forward(SoftmaxCall& c, bool train, bool train_table) {
     check_softmax(c);
@@ -456,7 +456,7 @@ std::tuple<Tensor, Tensor, Tensor> softmax_forward(SoftmaxCall& c, bool train, b
     c.k = packed_rows(c.k);
     c.v = packed_rows(c.v);
     if (c.keep.defined() && c.keep.size(1) > 1 && c.keep.stride(1) != 1) c.keep = c.keep.contiguous();
-    Tensor out = empty_rows(c.q), lo, lse;
+    Tensor out = empty_rows(c.q), full, lse;
     const std::vector<int> border(c.border.begin(), c.border.end());
     qlka_softmax_args a = softmax_args(c, border);
     a.out = out.data_ptr();
@@ -465,15 +465,15 @@ std::tuple<Tensor, Tensor, Tensor> softmax_forward(SoftmaxCall& c, bool train, b
         lse = at::empty({a.B, a.H, a.M}, c.q.options().dtype(at::kFloat));
         a.lse = lse.data_ptr<float>();
         if (a.dtype == QLKA_BF16 && train_table) {
-            lo = at::empty_strided(out.sizes(), out.strides(), out.options());
-            a.out_lo = lo.data_ptr();
+            full = at::empty({a.B, a.H, a.M, a.D}, lse.options());
+            a.out_full = full.data_ptr<float>();
         }
     }
     const size_t bytes = qlka_softmax_fwd_ws_bytes(&a);
     Tensor ws;
     if (bytes) ws = workspace(bytes, c.q);
     check_rc(qlka_softmax_fwd(&a, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(c.q)));
-    return {out, lo, lse};
+    return {out, full, lse};
 }
 
 struct SoftmaxFn : public torch::autograd::Function<SoftmaxFn> {
@@ -482,14 +482,14 @@ struct SoftmaxFn : public torch::autograd::Function<SoftmaxFn> {
         ctx->set_materialize_grads(false);
         const Tensor table = table_.value_or(Tensor()), keep = keep_.value_or(Tensor());
         SoftmaxCall c{q, k, v, table, keep, scale, causal, start, border, both};
-        Tensor out, lo, lse;
-        std::tie(out, lo, lse) = softmax_forward(c, true, table.defined() && table.requires_grad());
+        Tensor out, full, lse;
+        std::tie(out, full, lse) = softmax_forward(c, true, table.defined() && table.requires_grad());
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["causal"] = causal;
         ctx->saved_data["start"] = start;
         ctx->saved_data["border"] = border;
         ctx->saved_data["both"] = both;
-        ctx->save_for_backward({c.q, c.k, c.v, c.table, c.keep, out, lo, lse});
+        ctx->save_for_backward({c.q, c.k, c.v, c.table, c.keep, out, full, lse});
         return out;
     }
 
@@ -501,14 +501,14 @@ struct SoftmaxFn : public torch::autograd::Function<SoftmaxFn> {
         const SoftmaxCall c{s[0], s[1], s[2], s[3], s[4], ctx->saved_data["scale"].toDouble(),
                             ctx->saved_data["causal"].toBool(), ctx->saved_data["start"].toInt(),
                             ctx->saved_data["border"].toIntVector(), ctx->saved_data["both"].toBool()};
-        const Tensor &out = s[5], &lo = s[6], &lse = s[7];
+        const Tensor &out = s[5], &full = s[6], &lse = s[7];
         c10::DeviceGuard guard(c.q.device());
         const std::vector<int> border(c.border.begin(), c.border.end());
         qlka_softmax_args a = softmax_args(c, border);
         const Tensor g = packed_rows(grads[0]);
         a.out = out.data_ptr();
         set_strides(a.out_stride, out);
-        if (lo.defined()) a.out_lo = lo.data_ptr();
+        if (full.defined()) a.out_full = full.data_ptr<float>();
         a.lse = lse.data_ptr<float>();
         a.g_out = g.data_ptr();
         set_strides(a.g_out_stride, g);

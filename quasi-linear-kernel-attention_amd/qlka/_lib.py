@@ -30,7 +30,7 @@ class SoftmaxArgs(ctypes.Structure):
                 + [(n, _c_i64x3) for n in ("q_stride", "k_stride", "v_stride")]
                 + [("keep", _c_ptr), ("keep_stride", ctypes.c_int64), ("table", _c_ptr),
                    ("border", ctypes.POINTER(_c_int)), ("num_borders", _c_int), ("bidirectional", _c_int),
-                   ("out", _c_ptr), ("out_lo", _c_ptr), ("out_stride", _c_i64x3), ("lse", _c_ptr),
+                   ("out", _c_ptr), ("out_stride", _c_i64x3), ("out_full", _c_ptr), ("lse", _c_ptr),
                    ("g_out", _c_ptr), ("g_out_stride", _c_i64x3), ("g_q", _c_ptr), ("g_k", _c_ptr), ("g_v", _c_ptr)]
                 + [(n, _c_i64x3) for n in ("g_q_stride", "g_k_stride", "g_v_stride")]
                 + [("g_table", _c_ptr)])
