@@ -66,7 +66,7 @@ __device__ __forceinline__ void add_band(f32x16 ds, int base, float* acc, const 
 }
 
 template <class T, int DP, int NW, bool BIAS>
-__global__ __launch_bounds__(64 * NW) void softmax_dq(const SmParams p) {
+__global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(const SmParams p) {
     constexpr int NP = Elem<T>::PARTS, BN = Shape<T, DP>::BN, NT = 64 * NW, ROWS = 32 * NW, NS = BN / 32, ND = DP / 32;
     __shared__ Tile<NP, BN, DP> kt, vt;
     __shared__ BiasLds table;
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(64 * NW) void softmax_dq(const SmParams p) {
 }
 
 template <class T, int DP, int NW, bool BIAS>
-__global__ __launch_bounds__(64 * NW) void softmax_dkv(const SmParams p) {
+__global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(const SmParams p) {
     constexpr int NP = Elem<T>::PARTS, BM = Shape<T, DP>::BN, NT = 64 * NW, KEYS = 32 * NW, NS = BM / 32, ND = DP / 32;
     __shared__ Tile<NP, BM, DP> qt, gt;
     __shared__ __attribute__((aligned(16))) float lse[BM], delta[BM];

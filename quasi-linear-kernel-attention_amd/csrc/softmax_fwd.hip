@@ -23,7 +23,7 @@ namespace sm {
 constexpr float GROW = 8.f;
 
 template <class T, int DP, int NW, bool BIAS, bool FINE>
-__global__ __launch_bounds__(64 * NW) void softmax_fwd(const SmParams p) {
+__global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(const SmParams p) {
     constexpr int NP = Elem<T>::PARTS, BN = Shape<T, DP>::BN, NT = 64 * NW, ROWS = 32 * NW, NS = BN / 32, ND = DP / 32;
     __shared__ Tile<NP, BN, DP> kt, vt;
     __shared__ BiasLds table;
@@ -209,41 +209,60 @@ template <class T, int DP, int NW> int launch_fwd(const SmParams& p, hipStream_t
     else softmax_fwd<T, DP, NW, false, false><<<grid, 64 * NW, 0, st>>>(p);
     return (int)hipGetLastError();
 }
-// Joins the splits of a row: a group of DP / 4 lanes a row, four elements a lane.
+// Joins the splits of a row, a wave a row: first a lane for each split's maximum and sum, then DP / 4 lanes for each of
+// several splits at a time, four elements a lane. Both steps' loads are issued together: a row costs two memory latencies.
+constexpr int COMBINE_ROWS = 4, MOST_SPLITS = 256;
+
 template <class T, int DP>
-__global__ __launch_bounds__(256) void softmax_combine(const SmParams p) {
-    constexpr int LANES = DP / 4;
-    const int64_t rows = (int64_t)p.B * p.H * p.M;
-    const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES;
-    const int d = threadIdx.x % LANES * 4;
+__global__ __launch_bounds__(64 * COMBINE_ROWS) void softmax_combine(const SmParams p) {
+    constexpr int LANES = DP / 4, AT_ONCE = 64 / LANES, LOOK = MOST_SPLITS / 64;
+    constexpr float LOW = -std::numeric_limits<float>::infinity();
+    __shared__ float weight[COMBINE_ROWS][MOST_SPLITS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t rows = (int64_t)p.B * p.H * p.M, row = (int64_t)blockIdx.x * COMBINE_ROWS + wave;
     if (row >= rows) return;
-    float ref = -std::numeric_limits<float>::infinity(), sum = 0.f;
-    for (int s = 0; s < p.splits; ++s) {
-        const float2 a = *reinterpret_cast<const float2*>(p.part2 + 2 * (s * rows + row));
-        if (a.y == 0.f) continue;                                         // no key here
-        const float to = fmaxf(ref, a.x);
-        sum = sum * fexp2(ref - to) + a.y * fexp2(a.x - to);
-        ref = to;
+    float2 a[LOOK];
+    float ref = LOW;
+#pragma unroll
+    for (int i = 0; i < LOOK; ++i) {
+        const int s = lane + 64 * i;
+        a[i] = float2{LOW, 0.f};
+        if (s < p.splits) a[i] = *reinterpret_cast<const float2*>(p.part2 + 2 * (s * rows + row));
+        if (a[i].y == 0.f) a[i].x = LOW;                                  // no key there
+        ref = fmaxf(ref, a[i].x);
     }
+#pragma unroll
+    for (int far = 1; far < 64; far *= 2) ref = fmaxf(ref, __shfl_xor(ref, far));
+    if (ref == LOW) ref = 0.f;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < LOOK; ++i) {
+        const float f = fexp2(a[i].x - ref);
+        if (lane + 64 * i < p.splits) weight[wave][lane + 64 * i] = f;
+        sum += a[i].y * f;
+    }
+#pragma unroll
+    for (int far = 1; far < 64; far *= 2) sum += __shfl_xor(sum, far);
+    const int d = lane % LANES * 4, first = lane / LANES;
     f32x4 x = {};
-    for (int s = 0; s < p.splits; ++s) {
-        const float2 a = *reinterpret_cast<const float2*>(p.part2 + 2 * (s * rows + row));
-        if (a.y == 0.f) continue;
-        const f32x4 y = *reinterpret_cast<const f32x4*>(p.part + (s * rows + row) * DP + d);
-        x = x + y * fexp2(a.x - ref);
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    x = x * inv;
+#pragma unroll 4
+    for (int s = first; s < p.splits; s += AT_ONCE)
+        x = x + *reinterpret_cast<const f32x4*>(p.part + (s * rows + row) * DP + d) * weight[wave][s];
+#pragma unroll
+    for (int far = LANES; far < 64; far *= 2)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] += __shfl_xor(x[i], far);
+    x = x * (sum == 0.f ? 0.f : 1.f / sum);
+    if (first) return;
     const int m = (int)(row % p.M), head = (int)(row / p.M % p.H), b = (int)(row / p.M / p.H);
-    const int64_t at = b * p.so.b + head * p.so.h + m * p.so.r;
-    store4((T*)p.out + at, d, p.D, p.vec & VEC_O, x);
+    store4((T*)p.out + b * p.so.b + head * p.so.h + m * p.so.r, d, p.D, p.vec & VEC_O, x);
     if (p.out_full) store4(p.out_full + row * p.D, d, p.D, p.vec & VEC_FULL, x);
     if (p.lse && d == 0) p.lse[row] = sum == 0.f ? std::numeric_limits<float>::infinity() : ref + __log2f(sum);
 }
 
 template <class T, int DP> int launch_combine(const SmParams& p, hipStream_t st) {
-    const int64_t threads = (int64_t)p.B * p.H * p.M * (DP / 4);
-    softmax_combine<T, DP><<<dim3((unsigned)((threads + 255) / 256)), 256, 0, st>>>(p);
+    const int64_t rows = (int64_t)p.B * p.H * p.M;
+    softmax_combine<T, DP><<<dim3((unsigned)((rows + COMBINE_ROWS - 1) / COMBINE_ROWS)), 64 * COMBINE_ROWS, 0, st>>>(p);
     return (int)hipGetLastError();
 }
 

@@ -5,7 +5,8 @@
 // for float) and keeps four such loads of k and four of v in flight. Scores are formed with fp32 multiply-adds and summed
 // over a row's lanes by DPP; every group of lanes runs its own softmax over the keys that pass it, and the groups, then the
 // waves, are joined at the end. The keys are split over workgroups until the GPU is full (softmax_combine joins the
-// splits). A matrix tile would use one of its 32 rows here.
+// splits). A matrix tile would use one of its 32 rows here. Near the diagonal a lane finds the bias of one key of the tile for
+// every row, which the keys' groups then read from LDS.
 #include "softmax_tile.h"
 
 #include <limits>
@@ -13,7 +14,7 @@
 namespace qlka {
 namespace sm {
 
-constexpr int STEP_WAVES = 4, STEP_LOADS = 4;
+constexpr int STEP_WAVES = 4;
 
 template <int CTRL> __device__ __forceinline__ float dpp(float x) {
     return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, true));
@@ -29,11 +30,12 @@ template <int LANES> __device__ __forceinline__ float row_sum(float x) {
 
 template <class T, int DP, int R, bool BIAS>
 __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p) {
-    constexpr int LANES = DP / 8, KEYS = 64 / LANES, U = STEP_LOADS, NW = STEP_WAVES, NT = 64 * NW;
+    constexpr int LANES = DP / 8, KEYS = 64 / LANES, U = 4, NW = STEP_WAVES, NT = 64 * NW;
     constexpr float LOW = -std::numeric_limits<float>::infinity();
     __shared__ float join_o[NW][R][DP], join_m[NW][R], join_s[NW][R];
     __shared__ float table[BIAS ? R : 1][QLKA_MAX_BUCKETS];
     __shared__ int border[BIAS ? QLKA_MAX_BUCKETS : 1];
+    __shared__ float near_bias[BIAS ? NW : 1][R][64];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, group = lane / LANES, d = lane % LANES * 8;
     int w = xcd_work(blockIdx.x, gridDim.x);
@@ -76,7 +78,14 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p
         uint64_t bits = seen.of(t);
         if (last - n0 < 63) bits &= (1ull << (last - n0 + 1)) - 1;
         int fb = -1;
-        if constexpr (BIAS) fb = far_bucket(p.bk, n0 - (p.M - 1) - p.start, n0 + 63 - p.start);
+        if constexpr (BIAS) {
+            fb = far_bucket(p.bk, n0 - (p.M - 1) - p.start, n0 + 63 - p.start);
+            if (fb < 0)
+                for (int m = 0; m < p.M; ++m) {
+                    const int bucket = bucket_of(border, p.bk.n, p.bk.both, n0 + lane - m - p.start);
+                    for (int r = m; r < rows; r += p.M) near_bias[wave][r][lane] = table[r][bucket];
+                }
+        }
 #pragma unroll 1
         for (int u0 = 0; u0 < 64; u0 += U * KEYS) {
             if (!(bits >> u0 & (U * KEYS == 64 ? ~0ull : (1ull << (U * KEYS % 64)) - 1))) continue;
@@ -114,8 +123,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     const int n = n0 + u0 + u * KEYS + group;
-                    if constexpr (BIAS)
-                        x[r][u] += table[r][fb >= 0 ? fb : bucket_of(border, p.bk.n, p.bk.both, n - seat)];
+                    if constexpr (BIAS) x[r][u] += fb >= 0 ? table[r][fb] : near_bias[wave][r][n - n0];
                     if (!in[u] || (p.causal && n > seat)) x[r][u] = LOW;
                     hi = fmaxf(hi, x[r][u]);
                 }

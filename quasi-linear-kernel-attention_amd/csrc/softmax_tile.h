@@ -140,6 +140,9 @@ template <int NP, int ROWS, int DP> struct Tile {
 template <class T, int DP> struct Shape {
     static constexpr int NP = Elem<T>::PARTS;
     static constexpr int BN = NP == 3 && DP == 128 ? 32 : 64;
+    // Waves a SIMD has room for. From 2 on a wave has 256 registers at most, and the compiler keeps sums in those that vector
+    // instructions can reach; with 1 it puts them in the others and copies every score.
+    static constexpr int WAVES = NP == 3 && DP == 128 ? 1 : 2;
 };
 
 // This thread's share of a tile of BN rows, between its global loads and its LDS stores.
