@@ -72,7 +72,7 @@ int splits_for(int64_t groups, int64_t tiles, int64_t want, int64_t least) {
     return (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(want, std::max<int64_t>(groups, 1)), tiles / least, 256}));
 }
 
-int tile_rows(const qlka_softmax_args* a) { return a->dtype == QLKA_F32 && a->D > 64 ? 32 : 64; }
+int tile_rows(const qlka_softmax_args* a) { return sm_tile_rows(a->dtype == QLKA_F32 ? 3 : 1, sm_padded(a->D)); }
 
 struct RowPlan { int waves, blocks, splits; };
 // kernels that own `len` rows of each of `heads` heads and go over `tiles` tiles of the other side

@@ -112,15 +112,15 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
         t1 = min(t1, last < 0 ? 0 : last / BN + 1);
     }
     KeyBits<BN> seen(p, b);
-    Staged<T, DP, BN, NT> ks, vs;
+    Staged<T, DP, BN, NT> ks(p.sk.r, p.D, vk, tid), vs(p.sv.r, p.D, vv, tid);
     const float c2 = p.scale * LOG2E;
-    Acc<NP, NP == 3 && DP < 128> dq[ND];
+    Acc<NP> dq[ND];
 
     int t = seen.next(t0, t1);
     if (t < t1) {
         const uint64_t bits = seen.of(t);
-        ks.load(k, p.sk.r, t * BN, bits, p.D, vk, tid);
-        vs.load(v, p.sv.r, t * BN, bits, p.D, vv, tid);
+        ks.load(k + (int64_t)t * BN * p.sk.r, p.sk.r, bits, p.D, vk, tid);
+        vs.load(v + (int64_t)t * BN * p.sv.r, p.sv.r, bits, p.D, vv, tid);
     }
     while (t < t1) {
         const int n0 = t * BN;
@@ -144,26 +144,30 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
         __syncthreads();
         if (tn < t1) {
             const uint64_t nb = seen.of(tn);
-            ks.load(k, p.sk.r, tn * BN, nb, p.D, vk, tid);
-            vs.load(v, p.sv.r, tn * BN, nb, p.D, vv, tid);
+            ks.load(k + (int64_t)tn * BN * p.sk.r, p.sk.r, nb, p.D, vk, tid);
+            vs.load(v + (int64_t)tn * BN * p.sv.r, p.sv.r, nb, p.D, vv, tid);
         }
         t = tn;
         if (mw >= p.M || (p.causal && n0 > mw + 31 + p.start)) continue;
 
         const bool edge = p.causal && n0 + BN - 1 > mw + p.start;
-        const bool all = bits == (BN == 64 ? ~0ull : 0xffffffffull) && !edge;
+        const bool all = bits == Staged<T, DP, BN, NT>::ALL && !edge;
         const uint64_t mine = bits >> (4 * half);
         const int lim = edge ? m + p.start - n0 - 4 * half : BN;
         const float* nb = &near_bias[BIAS ? ROWS - 1 - wave * 32 - col + 4 * half : 0];
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             Acc<NP> sa, dpa;
+            sa.start();
 #pragma unroll
             for (int c = 0; c < DP / 16; ++c) sa.add(kt.row(32 * i + col, 16 * c + 8 * half), qf[c]);
+            sa.join();
+            dpa.start();
 #pragma unroll
             for (int c = 0; c < DP / 16; ++c) dpa.add(vt.row(32 * i + col, 16 * c + 8 * half), gf[c]);
-            f32x16 s = sa.sum();
-            const f32x16 dp = dpa.sum();
+            dpa.join();
+            f32x16 s = sa.main;
+            const f32x16 dp = dpa.main;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int n = 32 * i + reg_row(r);
@@ -182,14 +186,15 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
                     if (fb == p.bk.n) left += a; else right += a;
                 }
             }
+            Frag<NP> df[2];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                f32x8 x;
+            for (int c = 0; c < 2; ++c) df[c] = split<NP>(eight(s, c));
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = s[8 * c + j];
-                const Frag<NP> df = split<NP>(x);
+            for (int d = 0; d < ND; ++d) {
+                dq[d].start();
 #pragma unroll
-                for (int d = 0; d < ND; ++d) dq[d].add(kt.column(32 * i + 16 * c, 32 * d, lane), df);
+                for (int c = 0; c < 2; ++c) dq[d].add(kt.column(32 * i + 16 * c, 32 * d, lane), df[c]);
+                dq[d].join();
             }
         }
     }
@@ -219,7 +224,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int at = 32 * d + 8 * r + 4 * half;
-            const f32x4 x = quad(dq[d].sum(), r);
+            const f32x4 x = quad(dq[d].main, r);
             if (p.splits > 1)
                 *reinterpret_cast<f32x4*>(p.part + ((int64_t)split_i * p.B * p.H * p.M + row) * DP + at) = x;
             else
@@ -266,13 +271,13 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
             while (t < t1 && t % tiles * BM + BM - 1 + p.start < n0) ++t;
         return t;
     };
-    Staged<T, DP, BM, NT> qs, gs;
+    Staged<T, DP, BM, NT> qs(p.sq.r, p.D, p.vec & VEC_Q, tid), gs(p.sg.r, p.D, p.vec & VEC_G, tid);
     float ls = HIGH, des = 0.f;
     const auto load = [&](int t) {
         const int head = kvh * share + t / tiles, m0 = t % tiles * BM, left = p.M - m0;
-        const uint64_t bits = left >= 64 ? ~0ull : (1ull << left) - 1;
-        qs.load((const T*)p.q + b * p.sq.b + head * p.sq.h, p.sq.r, m0, bits, p.D, p.vec & VEC_Q, tid);
-        gs.load((const T*)p.g_out + b * p.sg.b + head * p.sg.h, p.sg.r, m0, bits, p.D, p.vec & VEC_G, tid);
+        const uint64_t bits = left >= BM ? Staged<T, DP, BM, NT>::ALL : (1ull << left) - 1;
+        qs.load((const T*)p.q + b * p.sq.b + head * p.sq.h + m0 * p.sq.r, p.sq.r, bits, p.D, p.vec & VEC_Q, tid);
+        gs.load((const T*)p.g_out + b * p.sg.b + head * p.sg.h + m0 * p.sg.r, p.sg.r, bits, p.D, p.vec & VEC_G, tid);
         ls = HIGH;
         des = 0.f;
         if (tid < BM && tid < left) {
@@ -282,7 +287,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
         }
     };
     const float c2 = p.scale * LOG2E;
-    Acc<NP, NP == 3 && DP < 128> dk[ND], dv[ND];
+    Acc<NP> dk[ND], dv[ND];
     int filled = -1;                                   // the head whose bias stands in LDS
 
     int t = next((int)(work * split_i / p.splits));
@@ -325,11 +330,15 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             Acc<NP> sa, dpa;
+            sa.start();
 #pragma unroll
             for (int c = 0; c < DP / 16; ++c) sa.add(qt.row(32 * i + col, 16 * c + 8 * half), kf[c]);
+            sa.join();
+            dpa.start();
 #pragma unroll
             for (int c = 0; c < DP / 16; ++c) dpa.add(gt.row(32 * i + col, 16 * c + 8 * half), vf[c]);
-            f32x16 s = sa.sum(), dp = dpa.sum();
+            dpa.join();
+            f32x16 s = sa.main, dp = dpa.main;
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
                 const f32x4 l4 = *reinterpret_cast<const f32x4*>(&lse[32 * i + 8 * r4 + 4 * half]);
@@ -345,20 +354,24 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
                     dp[r] = ds;
                 }
             }
+            Frag<NP> f[2];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                f32x8 x, y;
+            for (int c = 0; c < 2; ++c) f[c] = split<NP>(eight(s, c));
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    x[j] = s[8 * c + j];
-                    y[j] = dp[8 * c + j];
-                }
-                const Frag<NP> pf = split<NP>(x), df = split<NP>(y);
+            for (int d = 0; d < ND; ++d) {
+                dv[d].start();
 #pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    dv[d].add(gt.column(32 * i + 16 * c, 32 * d, lane), pf);
-                    dk[d].add(qt.column(32 * i + 16 * c, 32 * d, lane), df);
-                }
+                for (int c = 0; c < 2; ++c) dv[d].add(gt.column(32 * i + 16 * c, 32 * d, lane), f[c]);
+                dv[d].join();
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) f[c] = split<NP>(eight(dp, c));
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                dk[d].start();
+#pragma unroll
+                for (int c = 0; c < 2; ++c) dk[d].add(qt.column(32 * i + 16 * c, 32 * d, lane), f[c]);
+                dk[d].join();
             }
         }
     }
@@ -370,8 +383,8 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int at = 32 * d + 8 * r + 4 * half;
-            const f32x4 x = quad(dk[d].sum(), r);
-            const f32x4 y = quad(dv[d].sum(), r);
+            const f32x4 x = quad(dk[d].main, r);
+            const f32x4 y = quad(dv[d].main, r);
             if (p.splits > 1) {
                 *reinterpret_cast<f32x4*>(p.part + (split_i * all + row) * DP + at) = x;
                 *reinterpret_cast<f32x4*>(p.part2 + (split_i * all + row) * DP + at) = y;

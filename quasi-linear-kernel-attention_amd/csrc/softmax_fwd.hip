@@ -6,8 +6,8 @@
 // from the registers they are in. A workgroup of `waves` waves shares the tiles of k and v in LDS; the next tile's loads are
 // issued before the current tile's products. The running maximum is moved only when it grows by more than 2^8, so
 // that the output is hardly ever scaled; probabilities are then at most 2^8. Rounding them to bf16 for the product with bf16
-// values (not for fp32) costs what rounding the result does; their sum is of the unrounded ones. Where the table's
-// gradient will be wanted (FINE) they are taken in two parts of 8 bits: that gradient is fp32 and a sum over whole rows of
+// values (not for fp32) costs what rounding the result does; the sum they are divided by is then that of the rounded ones. Where
+// the table's gradient will be wanted (FINE) they are taken in two parts of 8 bits: that gradient is fp32 and a sum over rows of
 // dS = P (dP - delta), in which an error of delta, the row sum of dO * O, does not average out.
 //
 // Masked keys are read as zeros (what stands there may be anything) and their tiles, where none is left, are skipped.
@@ -60,7 +60,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
         t1 = min(t1, last < 0 ? 0 : last / BN + 1);
     }
     KeyBits<BN> seen(p, b);
-    Staged<T, DP, BN, NT> ks, vs;
+    Staged<T, DP, BN, NT> ks(p.sk.r, p.D, vk, tid), vs(p.sv.r, p.D, vv, tid);
     const float c2 = p.scale * LOG2E;
     Acc<NP> o[ND];
     float top = -std::numeric_limits<float>::infinity(), ref = 0.f, sum = 0.f;
@@ -68,8 +68,8 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
     int t = seen.next(t0, t1);
     if (t < t1) {
         const uint64_t bits = seen.of(t);
-        ks.load(k, p.sk.r, t * BN, bits, p.D, vk, tid);
-        vs.load(v, p.sv.r, t * BN, bits, p.D, vv, tid);
+        ks.load(k + (int64_t)t * BN * p.sk.r, p.sk.r, bits, p.D, vk, tid);
+        vs.load(v + (int64_t)t * BN * p.sv.r, p.sv.r, bits, p.D, vv, tid);
     }
     while (t < t1) {
         const int n0 = t * BN;
@@ -94,8 +94,8 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
         __syncthreads();
         if (tn < t1) {
             const uint64_t nb = seen.of(tn);
-            ks.load(k, p.sk.r, tn * BN, nb, p.D, vk, tid);
-            vs.load(v, p.sv.r, tn * BN, nb, p.D, vv, tid);
+            ks.load(k + (int64_t)tn * BN * p.sk.r, p.sk.r, nb, p.D, vk, tid);
+            vs.load(v + (int64_t)tn * BN * p.sv.r, p.sv.r, nb, p.D, vv, tid);
         }
         t = tn;
         if (mw >= p.M || (p.causal && n0 > mw + 31 + p.start)) continue;
@@ -104,15 +104,17 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             Acc<NP> a;
+            a.start();
 #pragma unroll
             for (int c = 0; c < DP / 16; ++c) a.add(kt.row(32 * i + col, 16 * c + 8 * half), qf[c]);
-            s[i] = a.sum();
+            a.join();
+            s[i] = a.main;
         }
 
         // scores in log2 units are fma(s, mul, add) from here on
         float mul = c2, add = far;
         const bool edge = p.causal && n0 + BN - 1 > mw + p.start;
-        const bool all = bits == (BN == 64 ? ~0ull : 0xffffffffull) && !edge;
+        const bool all = bits == Staged<T, DP, BN, NT>::ALL && !edge;
         if (near || !all) {
             const uint64_t mine = bits >> (4 * half);
             const int lim = edge ? m + p.start - n0 - 4 * half : BN;     // the last key seen
@@ -144,22 +146,27 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
             const float f = first ? 1.f : fexp2(was - ref);               // the first time there is nothing to scale
             sum *= f;
 #pragma unroll
-            for (int d = 0; d < ND; ++d) o[d].scale(f);
+            for (int d = 0; d < ND; ++d) o[d].main *= f;
         }
         add -= ref;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[d].start();
 #pragma unroll
         for (int i = 0; i < NS; ++i)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                f32x8 e;
+                f32x8 e = eight(s[i], c);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    e[j] = fexp2(__builtin_fmaf(s[i][8 * c + j], mul, add));
-                    sum += e[j];
-                }
+                for (int j = 0; j < 8; ++j) e[j] = fexp2(__builtin_fmaf(e[j], mul, add));
                 const Frag<NP> pf = split<NP>(e);
                 Frag<NP> rest;
-                if constexpr (FINE) rest = split<NP>(e - __builtin_convertvector(pf.p[0], f32x8));
+                if constexpr (FINE) rest = split<NP>(e - floats(pf.p[0]));
+                if constexpr (NP == 1 && !FINE) {
+                    sum = add_all(pf.p[0], sum);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) sum += e[j];
+                }
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
                     const Frag<NP> vf = vt.column(32 * i + 16 * c, 32 * d, lane);
@@ -167,12 +174,11 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
                     o[d].add(vf, pf);
                 }
             }
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[d].join();
     }
     if (m >= p.M) return;
     sum += other_half(sum);
-    f32x16 os[ND];
-#pragma unroll
-    for (int d = 0; d < ND; ++d) os[d] = o[d].sum();
     const int64_t row = ((int64_t)b * p.H + head) * p.M + m;
     if (p.splits > 1) {
         const int64_t at = (int64_t)split_i * p.B * p.H * p.M + row;
@@ -181,7 +187,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 *reinterpret_cast<f32x4*>(p.part + at * DP + 32 * d + 8 * r + 4 * half) =
-                    quad(os[d], r);
+                    quad(o[d].main, r);
         if (half == 0) {
             p.part2[2 * at] = ref;
             p.part2[2 * at + 1] = sum;
@@ -194,7 +200,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const f32x4 x = quad(os[d], r) * inv;
+            const f32x4 x = quad(o[d].main, r) * inv;
             store4(out, 32 * d + 8 * r + 4 * half, p.D, p.vec & VEC_O, x);
             if constexpr (FINE) store4(p.out_full + row * p.D, 32 * d + 8 * r + 4 * half, p.D, p.vec & VEC_FULL, x);
         }

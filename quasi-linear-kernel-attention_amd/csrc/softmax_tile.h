@@ -24,6 +24,7 @@ namespace sm {
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((ext_vector_type(8))) float f32x8;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
@@ -56,28 +57,24 @@ __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
 }
 // A sum of products. The matrix instruction drops what of a product lies a few bits below the sum's last one, always
 // downwards: 0.007 of a last place an instruction, measured, which a long sum of few signs would show. So the five
-// products of the smaller parts gather in a sum of their own (APART), 2^-8 as large; where registers do not reach for it (rows
-// of 128 in the backward) they do not.
-template <int NP, bool APART = NP == 3> struct Acc {
-    f32x16 main = {}, rest = {};
+// products of the smaller parts gather in a sum of their own, 2^-8 as large, until join().
+template <int NP> struct Acc {
+    f32x16 main = {}, rest;
+    __device__ __forceinline__ void start() {
+        if constexpr (NP == 3) rest = f32x16{};
+    }
     __device__ __forceinline__ void add(const Frag<NP>& a, const Frag<NP>& b) {
         if constexpr (NP == 3) {
-            f32x16& r = APART ? rest : main;
-            r = mfma(a.p[0], b.p[2], r);
-            r = mfma(a.p[2], b.p[0], r);
-            r = mfma(a.p[1], b.p[1], r);
-            r = mfma(a.p[0], b.p[1], r);
-            r = mfma(a.p[1], b.p[0], r);
+            rest = mfma(a.p[0], b.p[2], rest);
+            rest = mfma(a.p[2], b.p[0], rest);
+            rest = mfma(a.p[1], b.p[1], rest);
+            rest = mfma(a.p[0], b.p[1], rest);
+            rest = mfma(a.p[1], b.p[0], rest);
         }
         main = mfma(a.p[0], b.p[0], main);
     }
-    __device__ __forceinline__ void scale(float f) {
-        main *= f;
-        if constexpr (APART) rest *= f;
-    }
-    __device__ __forceinline__ f32x16 sum() const {
-        if constexpr (APART) return main + rest;
-        else return main;
+    __device__ __forceinline__ void join() {
+        if constexpr (NP == 3) main = main + rest;
     }
 };
 
@@ -85,6 +82,20 @@ __device__ __forceinline__ f32x8 floats(bf16x8 x) { return __builtin_convertvect
 __device__ __forceinline__ f32x8 floats(f32x8 x) { return x; }
 // registers 4 r .. 4 r + 3: four successive rows of a result
 __device__ __forceinline__ f32x4 quad(f32x16 x, int r) { return f32x4{x[4 * r], x[4 * r + 1], x[4 * r + 2], x[4 * r + 3]}; }
+// registers 8 c .. 8 c + 7: the second operand's chunk c
+__device__ __forceinline__ f32x8 eight(f32x16 x, int c) {
+    f32x8 y;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = x[8 * c + j];
+    return y;
+}
+// x[0] + x[1] + ... of eight bf16
+__device__ __forceinline__ float add_all(bf16x8 x, float to) {
+    const bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) to = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{x[2 * i], x[2 * i + 1]}, one, to, false);
+    return to;
+}
 __device__ __forceinline__ float fexp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
 __device__ __forceinline__ int reg_row(int r) { return (r >> 2) * 8 + (r & 3); }   // + 4 (lane / 32)
@@ -139,7 +150,7 @@ template <int NP, int ROWS, int DP> struct Tile {
 // Rows of the tiles that a workgroup goes through.
 template <class T, int DP> struct Shape {
     static constexpr int NP = Elem<T>::PARTS;
-    static constexpr int BN = NP == 3 && DP == 128 ? 32 : 64;
+    static constexpr int BN = sm_tile_rows(NP, DP);
     // Waves a SIMD has room for. From 2 on a wave has 256 registers at most, and the compiler keeps sums in those that vector
     // instructions can reach; with 1 it puts them in the others and copies every score.
     static constexpr int WAVES = NP == 3 && DP == 128 ? 1 : 2;
@@ -148,23 +159,32 @@ template <class T, int DP> struct Shape {
 // This thread's share of a tile of BN rows, between its global loads and its LDS stores.
 template <class T, int DP, int BN, int NT> struct Staged {
     static constexpr int SEGS = DP / 8, PER = BN * SEGS / NT;
+    static constexpr uint64_t ALL = BN == 64 ? ~0ull : (1ull << BN % 64) - 1;
     typename Elem<T>::seg s[PER];
-    static_assert(PER * NT == BN * SEGS, "every thread takes the same number of pieces");
+    uint32_t at;                           // of this thread's first piece from the tile's first row; the others are STEP rows apart
+    bool whole;                            // a tile without gaps is read without any test
+    static constexpr int STEP = NT / SEGS;
+    static_assert(PER * NT == BN * SEGS && STEP * SEGS == NT, "every thread takes the same column of PER rows");
 
-    __device__ __forceinline__ void load(const T* base, int64_t stride, int n0, uint64_t bits, int D, bool vec, int tid) {
+    __device__ __forceinline__ Staged(int64_t stride, int D, bool vec, int tid)
+        : at((uint32_t)(tid / SEGS * stride) + tid % SEGS * 8), whole(vec && D == DP && stride < 1 << 24) {}
+    // tile: its first row; bits: the rows to read, zeros for the others
+    __device__ __forceinline__ void load(const T* tile, int64_t stride, uint64_t bits, int D, bool vec, int tid) {
+        if (whole && bits == ALL) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) s[i] = *reinterpret_cast<const typename Elem<T>::seg*>(tile + i * STEP * stride + at);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int e = tid + i * NT, row = e / SEGS, d = e % SEGS * 8;
+            const int row = tid / SEGS + i * STEP, d = tid % SEGS * 8;
             s[i] = {};
-            if (bits >> row & 1) s[i] = load_seg(base + (n0 + row) * stride, d, D, vec);
+            if (bits >> row & 1) s[i] = load_seg(tile + row * stride, d, D, vec);
         }
     }
     template <class TileT> __device__ __forceinline__ void store(TileT& t, int tid) const {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int e = tid + i * NT;
-            t.put(e / SEGS, e % SEGS * 8, s[i]);
-        }
+        for (int i = 0; i < PER; ++i) t.put((tid + i * NT) / SEGS, (tid + i * NT) % SEGS * 8, s[i]);
     }
 };
 
@@ -211,7 +231,14 @@ template <int BN> struct KeyBits {
         }
         bits &= seen;
     }
-    __device__ __forceinline__ uint64_t of(int t) { look(t >> 6); return lane_u64(bits, t & 63); }
+    __device__ __forceinline__ uint64_t of(int t) {
+        if (!keep) {
+            const int left = N - t * BN;
+            return left >= BN ? (BN == 64 ? ~0ull : (1ull << BN % 64) - 1) : (1ull << left) - 1;
+        }
+        look(t >> 6);
+        return lane_u64(bits, t & 63);
+    }
     // the first tile from t on that has a key, or end
     __device__ __forceinline__ int next(int t, int end) {
         if (!keep) return t < end ? t : end;
