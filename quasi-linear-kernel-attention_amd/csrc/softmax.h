@@ -41,7 +41,7 @@ struct SmParams {
     int causal, start;
     int splits, blocks;                      // splits of the long axis; blocks of rows (or keys) per head
     int vec;                                 // bit per operand: its rows are read / written in 16-byte pieces
-    float scale;                             // |scale|; its sign is in q_sign
+    float scale;                             // |scale|; its sign (or 0) is in q_sign
     float q_sign;
     SmBuckets bk;
 };

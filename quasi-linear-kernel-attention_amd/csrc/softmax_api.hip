@@ -66,21 +66,42 @@ int check_sizes(const qlka_softmax_args* a) {
 
 // ---- how a call runs
 
-// Splits of an axis of `tiles` tiles so that `groups` workgroups become about `want`, each with `least` tiles or more.
-int splits_for(int64_t groups, int64_t tiles, int64_t want, int64_t least) {
-    if (groups >= want / 2) return 1;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(want, std::max<int64_t>(groups, 1)), tiles / least, 256}));
+constexpr int CUS = 256;
+
+// Splits of an axis of `tiles` tiles for `groups` workgroups over the other axes, by an estimate of the time: rounds of
+// workgroups on a CU (one alone on a CU is not twice as fast as two, waits not being filled), each its tiles and what it costs by
+// itself, and the joining of `join` bytes a split. In microseconds, fitted to prompts and gradients of 65 to 8192 keys.
+int splits_for(int64_t groups, int64_t tiles, double tile_us, double join_bytes) {
+    int best = 1;
+    double least = 0;
+    for (int s = 1; s <= 64 && (s == 1 || 2 * s <= tiles); ++s) {
+        const double rounds = std::max<double>(1.7, (double)ceil_div(groups * s, CUS));
+        double t = rounds * (2.0 + tile_us * ceil_div(tiles, s));
+        if (s > 1) t += 4.0 + s * join_bytes / 2e6;
+        if (s == 1 || t < 0.95 * least) {
+            best = s;
+            least = t;
+        }
+    }
+    return best;
+}
+// The same for the kernel of few rows, which is bound by memory: enough workgroups to fill the GPU, four tiles each or more.
+int step_splits(int64_t groups, int64_t tiles) {
+    if (groups >= 1024) return 1;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(2048, std::max<int64_t>(groups, 1)), tiles / 4, 256}));
 }
 
 int tile_rows(const qlka_softmax_args* a) { return sm_tile_rows(a->dtype == QLKA_F32 ? 3 : 1, sm_padded(a->D)); }
 
 struct RowPlan { int waves, blocks, splits; };
 // kernels that own `len` rows of each of `heads` heads and go over `tiles` tiles of the other side
-RowPlan row_plan(int B, int heads, int len, int64_t tiles) {
+RowPlan row_plan(const qlka_softmax_args* a, int heads, int len, int64_t tiles, double products) {
     RowPlan r;
     r.waves = len <= 32 ? 1 : len <= 64 ? 2 : 4;
     r.blocks = (int)ceil_div(len, 32 * r.waves);
-    r.splits = splits_for((int64_t)B * heads * r.blocks, tiles, 1024, 4);
+    const int DP = sm_padded(a->D);
+    const double tile_us = products * 0.3 * DP / 64 * (a->dtype == QLKA_F32 ? 2 : 1);
+    r.splits = splits_for((int64_t)a->B * heads * r.blocks, tiles, tile_us, (double)a->B * heads * len * DP * 8);
     return r;
 }
 
@@ -91,8 +112,8 @@ struct FwdPlan { bool step; RowPlan rows; size_t part, part2; };
 FwdPlan fwd_plan(const qlka_softmax_args* a) {
     FwdPlan f{};
     f.step = steps(a);
-    if (f.step) f.rows = {0, 0, splits_for((int64_t)a->B * a->G, ceil_div(a->N, 64), 2048, 4)};
-    else f.rows = row_plan(a->B, a->H, a->M, ceil_div(a->N, tile_rows(a)));
+    if (f.step) f.rows = {0, 0, step_splits((int64_t)a->B * a->G, ceil_div(a->N, 64))};
+    else f.rows = row_plan(a, a->H, a->M, ceil_div(a->N, tile_rows(a)), 2);
     if (f.rows.splits > 1) {
         const size_t rows = (size_t)f.rows.splits * a->B * a->H * a->M;
         f.part = align256(rows * sm_padded(a->D) * 4);
@@ -107,14 +128,14 @@ BwdPlan bwd_plan(const qlka_softmax_args* a, bool dq, bool dkv, bool table) {
     const int t = tile_rows(a), DP = sm_padded(a->D);
     w.delta = align256((size_t)a->B * a->H * a->M * 4);
     if (dq || table) {
-        w.dq = row_plan(a->B, a->H, a->M, ceil_div(a->N, t));
+        w.dq = row_plan(a, a->H, a->M, ceil_div(a->N, t), 3);
         if (w.dq.splits > 1) w.part = align256((size_t)w.dq.splits * a->B * a->H * a->M * DP * 4);
     }
     if (table)
         w.table = align256((size_t)a->H * a->B * w.dq.blocks * w.dq.splits * (a->num_borders + 1) *
                            (a->bidirectional ? 2 : 1) * 4);
     if (dkv) {
-        w.dkv = row_plan(a->B, a->G, a->N, ceil_div(a->M, t) * (a->H / a->G));
+        w.dkv = row_plan(a, a->G, a->N, ceil_div(a->M, t) * (a->H / a->G), 5);
         if (w.dkv.splits > 1) {
             w.part2 = align256((size_t)w.dkv.splits * a->B * a->G * a->N * DP * 4);
             w.part = std::max(w.part, w.part2);
@@ -148,8 +169,9 @@ int params(const qlka_softmax_args* a, SmParams* p) {
     p->causal = a->causal ? 1 : 0;
     p->start = a->start;
     p->splits = p->blocks = 1;
-    p->scale = std::fabs(a->scale);
-    p->q_sign = std::signbit(a->scale) ? -1.f : 1.f;
+    // scores are held in units of the scale, so a scale of 0 goes into the sign
+    p->scale = a->scale == 0.f ? 1.f : std::fabs(a->scale);
+    p->q_sign = a->scale == 0.f ? 0.f : a->scale < 0.f ? -1.f : 1.f;
     const auto bit = [&](int v, const void* x, const int64_t* s, int heads, int rows) {
         return in_pieces(a, x, s, heads, rows) ? v : 0; };
     p->vec = bit(VEC_Q, a->q, a->q_stride, a->H, a->M) | bit(VEC_K, a->k, a->k_stride, a->G, a->N) |
@@ -239,7 +261,7 @@ int qlka_softmax_bwd(const qlka_softmax_args* a, void* ws, size_t ws_bytes, void
     p.part = (float*)at; at += w.part;
     p.part2 = (float*)at; at += w.part2;
     p.part_table = (float*)at;
-    if (rows) {
+    if (rows && !a->g_q && !a->g_table) {               // else softmax_dq leaves them
         StageTimer timer("softmax_delta", st);
         if (int e = sm_delta(a->dtype, p, st)) return status(e, "softmax attention backward, row sums");
     }

@@ -73,37 +73,14 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
     __shared__ float near_bias[BIAS ? ROWS + BN : 1], sums[BIAS ? NW : 1][QLKA_MAX_BUCKETS];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
-    int w = xcd_work(blockIdx.x, gridDim.x);
-    const int block = w % p.blocks; w /= p.blocks;
-    const int split_i = w % p.splits; w /= p.splits;
-    const int head = w % p.H, b = w / p.H, kvh = head / (p.H / p.G);
+    const Work w = xcd_work(blockIdx.x, p.B * p.H, p.blocks * p.splits);
+    const int block = w.block % p.blocks, split_i = w.block / p.blocks;
+    const int head = w.pair % p.H, b = w.pair / p.H, kvh = head / (p.H / p.G);
     const int m0 = block * ROWS, mw = m0 + wave * 32, m = mw + col;
     const T* k = (const T*)p.k + b * p.sk.b + kvh * p.sk.h;
     const T* v = (const T*)p.v + b * p.sv.b + kvh * p.sv.h;
     const bool vk = p.vec & VEC_K, vv = p.vec & VEC_V;
     const int64_t row = ((int64_t)b * p.H + head) * p.M + m;
-
-    Frag<NP> qf[DP / 16], gf[DP / 16];
-#pragma unroll
-    for (int c = 0; c < DP / 16; ++c) {
-        typename Elem<T>::seg s = {}, g = {};
-        if (m < p.M) {
-            s = load_seg((const T*)p.q + b * p.sq.b + head * p.sq.h + m * p.sq.r, 16 * c + 8 * half, p.D, p.vec & VEC_Q);
-            g = load_seg((const T*)p.g_out + b * p.sg.b + head * p.sg.h + m * p.sg.r, 16 * c + 8 * half, p.D, p.vec & VEC_G);
-        }
-        if (p.q_sign < 0) s = -s;
-        qf[c] = frag_of(s);
-        gf[c] = frag_of(g);
-    }
-    const float lse = m < p.M ? p.lse[row] : HIGH, delta = m < p.M ? p.delta[row] : 0.f;
-    const int buckets = (p.bk.n + 1) * (p.bk.both ? 2 : 1);
-    float left = 0.f, right = 0.f;                     // this lane's sums far below and far above the diagonal
-    const bool to_table = BIAS && p.part_table;
-    if constexpr (BIAS) {
-        table.fill(p, head, tid, NT);
-        for (int i = lane; i < buckets; i += 64) sums[wave][i] = 0.f;
-        __syncthreads();
-    }
 
     const int tiles = (p.N + BN - 1) / BN;
     int t0 = (int)((int64_t)tiles * split_i / p.splits), t1 = (int)((int64_t)tiles * (split_i + 1) / p.splits);
@@ -113,15 +90,46 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
     }
     KeyBits<BN> seen(p, b);
     Staged<T, DP, BN, NT> ks(p.sk.r, p.D, vk, tid), vs(p.sv.r, p.D, vv, tid);
-    const float c2 = p.scale * LOG2E;
-    Acc<NP> dq[ND];
-
     int t = seen.next(t0, t1);
     if (t < t1) {
         const uint64_t bits = seen.of(t);
         ks.load(k + (int64_t)t * BN * p.sk.r, p.sk.r, bits, p.D, vk, tid);
         vs.load(v + (int64_t)t * BN * p.sv.r, p.sv.r, bits, p.D, vv, tid);
     }
+    Frag<NP> qf[DP / 16], gf[DP / 16];
+    float delta = 0.f;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+        const int d = 16 * c + 8 * half;
+        typename Elem<T>::seg s = {}, g = {};
+        f32x8 o = {};
+        if (m < p.M) {
+            s = load_seg((const T*)p.q + b * p.sq.b + head * p.sq.h + m * p.sq.r, d, p.D, p.vec & VEC_Q);
+            g = load_seg((const T*)p.g_out + b * p.sg.b + head * p.sg.h + m * p.sg.r, d, p.D, p.vec & VEC_G);
+            o = p.out_full ? load_seg(p.out_full + row * p.D, d, p.D, p.vec & VEC_FULL)
+                           : floats(load_seg((const T*)p.out + b * p.so.b + head * p.so.h + m * p.so.r, d, p.D, p.vec & VEC_O));
+        }
+        s = s * (T)p.q_sign;
+        qf[c] = frag_of(s);
+        gf[c] = frag_of(g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) delta = __builtin_fmaf((float)g[i], o[i], delta);
+    }
+    delta += other_half(delta);
+    const float lse = m < p.M ? p.lse[row] : HIGH;
+    if (m < p.M && half == 0 && split_i == 0) p.delta[row] = delta;        // softmax_dkv reads it
+    const int buckets = (p.bk.n + 1) * (p.bk.both ? 2 : 1);
+    float left = 0.f, right = 0.f;                     // this lane's sums far below and far above the diagonal
+    const bool to_table = BIAS && p.part_table;
+    if constexpr (BIAS) {
+        table.fill(p, head, tid, NT);
+        for (int i = lane; i < buckets; i += 64) sums[wave][i] = 0.f;
+        __syncthreads();
+    }
+
+    const float c2 = p.scale * LOG2E;
+    Acc<NP> dq[ND];
+
     while (t < t1) {
         const int n0 = t * BN;
         const uint64_t bits = seen.of(t);
@@ -157,6 +165,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
         const float* nb = &near_bias[BIAS ? ROWS - 1 - wave * 32 - col + 4 * half : 0];
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
+            if (!(uint32_t)(bits >> (32 * i))) continue;               // no key among these 32
             Acc<NP> sa, dpa;
             sa.start();
 #pragma unroll
@@ -241,26 +250,12 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
     __shared__ float near_bias[BIAS ? KEYS + BM : 1];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
-    int w = xcd_work(blockIdx.x, gridDim.x);
-    const int block = w % p.blocks; w /= p.blocks;
-    const int split_i = w % p.splits; w /= p.splits;
-    const int kvh = w % p.G, b = w / p.G, share = p.H / p.G;
+    const Work w = xcd_work(blockIdx.x, p.B * p.G, p.blocks * p.splits);
+    const int block = w.block % p.blocks, split_i = w.block / p.blocks;
+    const int kvh = w.pair % p.G, b = w.pair / p.G, share = p.H / p.G;
     const int n0 = block * KEYS, nw = n0 + wave * 32, n = nw + col;
     const bool shown = n < p.N && (!p.keep || p.keep[b * p.keep_stride + n]);
     const bool idle = !__any(shown);
-
-    Frag<NP> kf[DP / 16], vf[DP / 16];
-#pragma unroll
-    for (int c = 0; c < DP / 16; ++c) {
-        typename Elem<T>::seg s = {}, x = {};
-        if (shown) {
-            s = load_seg((const T*)p.k + b * p.sk.b + kvh * p.sk.h + n * p.sk.r, 16 * c + 8 * half, p.D, p.vec & VEC_K);
-            x = load_seg((const T*)p.v + b * p.sv.b + kvh * p.sv.h + n * p.sv.r, 16 * c + 8 * half, p.D, p.vec & VEC_V);
-        }
-        if (p.q_sign < 0) s = -s;
-        kf[c] = frag_of(s);
-        vf[c] = frag_of(x);
-    }
 
     // the tiles of queries of all heads that share these keys, one after the other
     const int tiles = (p.M + BM - 1) / BM;
@@ -286,12 +281,25 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
             des = p.delta[row];
         }
     };
+    int t = next((int)(work * split_i / p.splits));
+    if (t < t1) load(t);
+    Frag<NP> kf[DP / 16], vf[DP / 16];
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+        typename Elem<T>::seg s = {}, x = {};
+        if (shown) {
+            s = load_seg((const T*)p.k + b * p.sk.b + kvh * p.sk.h + n * p.sk.r, 16 * c + 8 * half, p.D, p.vec & VEC_K);
+            x = load_seg((const T*)p.v + b * p.sv.b + kvh * p.sv.h + n * p.sv.r, 16 * c + 8 * half, p.D, p.vec & VEC_V);
+        }
+        s = s * (T)p.q_sign;
+        kf[c] = frag_of(s);
+        vf[c] = frag_of(x);
+    }
+
     const float c2 = p.scale * LOG2E;
     Acc<NP> dk[ND], dv[ND];
     int filled = -1;                                   // the head whose bias stands in LDS
 
-    int t = next((int)(work * split_i / p.splits));
-    if (t < t1) load(t);
     while (t < t1) {
         const int m0 = t % tiles * BM, head = kvh * share + t / tiles;
         float far = 0.f;
@@ -300,8 +308,8 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
         qs.store(qt, tid);
         gs.store(gt, tid);
         if (tid < BM) {
-            lse[tid] = ls;
-            delta[tid] = des;
+            lse[tid] = -ls / c2;
+            delta[tid] = -des;
         }
         if constexpr (BIAS) {
             if (head != filled) {
@@ -329,7 +337,9 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
         const float* nb = &near_bias[BIAS ? wave * 32 + col + BM - 1 - 4 * half : 0];
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            Acc<NP> sa, dpa;
+            if (m0 + 32 * i >= p.M) continue;
+            // scores less the row's log sum (in units of the scores), and dP less delta
+            Acc<NP> sa(rows_of(lse, 32 * i + 4 * half)), dpa(rows_of(delta, 32 * i + 4 * half));
             sa.start();
 #pragma unroll
             for (int c = 0; c < DP / 16; ++c) sa.add(qt.row(32 * i + col, 16 * c + 8 * half), kf[c]);
@@ -340,19 +350,12 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
             dpa.join();
             f32x16 s = sa.main, dp = dpa.main;
 #pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) {
-                const f32x4 l4 = *reinterpret_cast<const f32x4*>(&lse[32 * i + 8 * r4 + 4 * half]);
-                const f32x4 d4 = *reinterpret_cast<const f32x4*>(&delta[32 * i + 8 * r4 + 4 * half]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int r = 4 * r4 + j, mr = 32 * i + 8 * r4 + j;
-                    float e = fexp2(__builtin_fmaf(s[r], c2, (BIAS && near ? nb[-mr] : far) - l4[j]));
-                    if (!shown || mr < lim) e = 0.f;
-                    float ds = e * (dp[r] - d4[j]);
-                    if (!shown || mr < lim) ds = 0.f;
-                    s[r] = e;
-                    dp[r] = ds;
-                }
+            for (int r = 0; r < 16; ++r) {
+                const int mr = 32 * i + reg_row(r);
+                float e = fexp2(__builtin_fmaf(s[r], c2, BIAS && near ? nb[-mr] : far));
+                if (edge && mr < lim) e = 0.f;
+                s[r] = e;
+                dp[r] = edge && mr < lim ? 0.f : e * dp[r];
             }
             Frag<NP> f[2];
 #pragma unroll
@@ -383,8 +386,8 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int at = 32 * d + 8 * r + 4 * half;
-            const f32x4 x = quad(dk[d].main, r);
-            const f32x4 y = quad(dv[d].main, r);
+            f32x4 x = quad(dk[d].main, r), y = quad(dv[d].main, r);
+            if (!shown) x = y = f32x4{};                    // what was computed for a key that nothing sees
             if (p.splits > 1) {
                 *reinterpret_cast<f32x4*>(p.part + (split_i * all + row) * DP + at) = x;
                 *reinterpret_cast<f32x4*>(p.part2 + (split_i * all + row) * DP + at) = y;

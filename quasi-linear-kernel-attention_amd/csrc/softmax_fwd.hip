@@ -30,28 +30,14 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
     __shared__ float near_bias[BIAS ? ROWS + BN : 1];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
-    int w = xcd_work(blockIdx.x, gridDim.x);
-    const int block = w % p.blocks; w /= p.blocks;
-    const int split_i = w % p.splits; w /= p.splits;
-    const int head = w % p.H, b = w / p.H, kvh = head / (p.H / p.G);
+    const Work w = xcd_work(blockIdx.x, p.B * p.H, p.blocks * p.splits);
+    const int block = w.block % p.blocks, split_i = w.block / p.blocks;
+    const int head = w.pair % p.H, b = w.pair / p.H, kvh = head / (p.H / p.G);
     const int m0 = block * ROWS, mw = m0 + wave * 32, m = mw + col;
     const T* q = (const T*)p.q + b * p.sq.b + head * p.sq.h;
     const T* k = (const T*)p.k + b * p.sk.b + kvh * p.sk.h;
     const T* v = (const T*)p.v + b * p.sv.b + kvh * p.sv.h;
     const bool vk = p.vec & VEC_K, vv = p.vec & VEC_V;
-
-    Frag<NP> qf[DP / 16];
-#pragma unroll
-    for (int c = 0; c < DP / 16; ++c) {
-        typename Elem<T>::seg s = {};
-        if (m < p.M) s = load_seg(q + m * p.sq.r, 16 * c + 8 * half, p.D, p.vec & VEC_Q);
-        if (p.q_sign < 0) s = -s;
-        qf[c] = frag_of(s);
-    }
-    if constexpr (BIAS) {
-        table.fill(p, head, tid, NT);
-        __syncthreads();
-    }
 
     const int tiles = (p.N + BN - 1) / BN;
     int t0 = (int)((int64_t)tiles * split_i / p.splits), t1 = (int)((int64_t)tiles * (split_i + 1) / p.splits);
@@ -61,16 +47,29 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
     }
     KeyBits<BN> seen(p, b);
     Staged<T, DP, BN, NT> ks(p.sk.r, p.D, vk, tid), vs(p.sv.r, p.D, vv, tid);
-    const float c2 = p.scale * LOG2E;
-    Acc<NP> o[ND];
-    float top = -std::numeric_limits<float>::infinity(), ref = 0.f, sum = 0.f;
-
     int t = seen.next(t0, t1);
     if (t < t1) {
         const uint64_t bits = seen.of(t);
         ks.load(k + (int64_t)t * BN * p.sk.r, p.sk.r, bits, p.D, vk, tid);
         vs.load(v + (int64_t)t * BN * p.sv.r, p.sv.r, bits, p.D, vv, tid);
     }
+    Frag<NP> qf[DP / 16];
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+        typename Elem<T>::seg s = {};
+        if (m < p.M) s = load_seg(q + m * p.sq.r, 16 * c + 8 * half, p.D, p.vec & VEC_Q);
+        s = s * (T)p.q_sign;
+        qf[c] = frag_of(s);
+    }
+    if constexpr (BIAS) {
+        table.fill(p, head, tid, NT);
+        __syncthreads();
+    }
+
+    const float c2 = p.scale * LOG2E;
+    Acc<NP> o[ND];
+    float top = -std::numeric_limits<float>::infinity(), ref = 0.f, sum = 0.f;
+
     while (t < t1) {
         const int n0 = t * BN;
         const uint64_t bits = seen.of(t);
@@ -103,10 +102,14 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
         f32x16 s[NS];
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
+            s[i] = f32x16{};
+            if (!(uint32_t)(bits >> (32 * i))) continue;               // no key among these 32
             Acc<NP> a;
             a.start();
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int c = 0; c < DP / 16; ++c) a.add(kt.row(32 * i + col, 16 * c + 8 * half), qf[c]);
+            __builtin_amdgcn_s_setprio(0);
             a.join();
             s[i] = a.main;
         }
@@ -152,7 +155,8 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[d].start();
 #pragma unroll
-        for (int i = 0; i < NS; ++i)
+        for (int i = 0; i < NS; ++i) {
+            if (!(uint32_t)(bits >> (32 * i))) continue;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 f32x8 e = eight(s[i], c);
@@ -174,6 +178,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
                     o[d].add(vf, pf);
                 }
             }
+        }
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[d].join();
     }

@@ -38,7 +38,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p
     __shared__ float near_bias[BIAS ? NW : 1][R][64];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, group = lane / LANES, d = lane % LANES * 8;
-    int w = xcd_work(blockIdx.x, gridDim.x);
+    int w = blockIdx.x;                      // nothing is read twice, so any order does
     const int split_i = w % p.splits; w /= p.splits;
     const int kvh = w % p.G, b = w / p.G, share = p.H / p.G, rows = share * p.M;
     const T* k = (const T*)p.k + b * p.sk.b + kvh * p.sk.h;

@@ -60,6 +60,8 @@ __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
 // products of the smaller parts gather in a sum of their own, 2^-8 as large, until join().
 template <int NP> struct Acc {
     f32x16 main = {}, rest;
+    __device__ __forceinline__ Acc() {}
+    __device__ __forceinline__ explicit Acc(f32x16 from) : main(from) {}
     __device__ __forceinline__ void start() {
         if constexpr (NP == 3) rest = f32x16{};
     }
@@ -82,6 +84,17 @@ __device__ __forceinline__ f32x8 floats(bf16x8 x) { return __builtin_convertvect
 __device__ __forceinline__ f32x8 floats(f32x8 x) { return x; }
 // registers 4 r .. 4 r + 3: four successive rows of a result
 __device__ __forceinline__ f32x4 quad(f32x16 x, int r) { return f32x4{x[4 * r], x[4 * r + 1], x[4 * r + 2], x[4 * r + 3]}; }
+// a result's 16 rows of x from x[first] on (first includes 4 (lane / 32))
+__device__ __forceinline__ f32x16 rows_of(const float* x, int first) {
+    f32x16 y;
+#pragma unroll
+    for (int r4 = 0; r4 < 4; ++r4) {
+        const f32x4 z = *reinterpret_cast<const f32x4*>(x + first + 8 * r4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[4 * r4 + j] = z[j];
+    }
+    return y;
+}
 // registers 8 c .. 8 c + 7: the second operand's chunk c
 __device__ __forceinline__ f32x8 eight(f32x16 x, int c) {
     f32x8 y;
@@ -285,11 +298,15 @@ __device__ __forceinline__ int far_bucket(const SmBuckets& bk, int lo, int hi) {
     return lo >= 0 ? 0 : -1;
 }
 
-// A linear workgroup index -> work index: workgroups go round the 8 XCDs, so successive work goes to one XCD, whose L2
-// then serves all blocks of a head.
-__device__ __forceinline__ int xcd_work(int wg, int total) {
-    const int x = wg & 7, per = total >> 3, more = total & 7;
-    return x * per + (x < more ? x : more) + (wg >> 3);
+// The work of a workgroup: `blocks` blocks of each of `pairs` (batch, head) pairs. Workgroups go round the 8 XCDs; all blocks
+// of a pair go to one of them, whose L2 then serves its keys, and successive pairs to different ones, since the heads of a
+// batch with more keys are next to each other. The pairs that are left over are spread over all.
+struct Work { int pair, block; };
+__device__ __forceinline__ Work xcd_work(int wg, int pairs, int blocks) {
+    const int full = (pairs >> 3) * blocks, slot = wg >> 3;
+    if (slot < full) return {slot / blocks * 8 + (wg & 7), slot % blocks};
+    const int rest = wg - 8 * full;
+    return {(pairs & ~7) + rest / blocks, rest % blocks};
 }
 
 // f(element, padded row length) for a call's type and row length.
