@@ -52,7 +52,7 @@ enum SmVec : int { VEC_Q = 1, VEC_K = 2, VEC_V = 4, VEC_G = 8, VEC_O = 16, VEC_G
 // Elements of a row in LDS and in the partial rows.
 inline int sm_padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 // Rows of the tiles that a workgroup goes through, for a number of parts an element and a padded row length.
-constexpr int sm_tile_rows(int parts, int DP) { return parts == 3 && DP >= 64 ? 32 : 64; }
+constexpr int sm_tile_rows(int parts, int DP) { return DP == 128 || (parts == 3 && DP == 64) ? 32 : 64; }
 inline int sm_buckets(const SmBuckets& b) { return (b.n + 1) * (b.both ? 2 : 1); }
 
 // Launchers; each returns a hipError_t value. The dtype is QLKA_F32 or QLKA_BF16.

@@ -68,9 +68,11 @@ __device__ __forceinline__ void add_band(f32x16 ds, int base, float* acc, const 
 template <class T, int DP, int NW, bool BIAS>
 __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(const SmParams p) {
     constexpr int NP = Elem<T>::PARTS, BN = Shape<T, DP>::BN, NT = 64 * NW, ROWS = 32 * NW, NS = BN / 32, ND = DP / 32;
-    __shared__ Tile<NP, BN, DP> kt, vt;
+    typedef Pair<T, DP, BN, NW> PairT;
+    constexpr int BUFFERS = PairT::BUFFERS;
+    __shared__ typename PairT::Lds lds;
     __shared__ BiasLds table;
-    __shared__ float near_bias[BIAS ? ROWS + BN : 1], sums[BIAS ? NW : 1][QLKA_MAX_BUCKETS];
+    __shared__ float near_bias[BUFFERS][BIAS ? ROWS + BN : 1], sums[BIAS ? NW : 1][QLKA_MAX_BUCKETS];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
     const Work w = xcd_work(blockIdx.x, p.B * p.H, p.blocks * p.splits);
@@ -79,7 +81,6 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
     const int m0 = block * ROWS, mw = m0 + wave * 32, m = mw + col;
     const T* k = (const T*)p.k + b * p.sk.b + kvh * p.sk.h;
     const T* v = (const T*)p.v + b * p.sv.b + kvh * p.sv.h;
-    const bool vk = p.vec & VEC_K, vv = p.vec & VEC_V;
     const int64_t row = ((int64_t)b * p.H + head) * p.M + m;
 
     const int tiles = (p.N + BN - 1) / BN;
@@ -89,13 +90,14 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
         t1 = min(t1, last < 0 ? 0 : last / BN + 1);
     }
     KeyBits<BN> seen(p, b);
-    Staged<T, DP, BN, NT> ks(p.sk.r, p.D, vk, tid), vs(p.sv.r, p.D, vv, tid);
-    int t = seen.next(t0, t1);
-    if (t < t1) {
-        const uint64_t bits = seen.of(t);
-        ks.load(k + (int64_t)t * BN * p.sk.r, p.sk.r, bits, p.D, vk, tid);
-        vs.load(v + (int64_t)t * BN * p.sv.r, p.sv.r, bits, p.D, vv, tid);
-    }
+    PairT tile(p.sk.r, p.vec & VEC_K, p.sv.r, p.vec & VEC_V, p.D, tid);
+    const auto fetch = [&](int t, int buffer) {
+        tile.fetch(lds, buffer, k + (int64_t)t * BN * p.sk.r, v + (int64_t)t * BN * p.sv.r, seen.of(t), tid);
+    };
+    if (p.keep || p.N % BN || p.D < DP) PairT::clear(lds, tid);
+    int t = seen.next(t0, t1), buffer = 0;
+    if (t < t1) fetch(t, 0);
+
     Frag<NP> qf[DP / 16], gf[DP / 16];
     float delta = 0.f;
 #pragma unroll
@@ -135,34 +137,31 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
         const uint64_t bits = seen.of(t);
         float far = 0.f;
         int fb = -1;
-        __syncthreads();
-        ks.store(kt, tid);
-        vs.store(vt, tid);
-        if constexpr (BIAS) {
-            const int lo = n0 - (m0 + ROWS - 1) - p.start;
-            fb = far_bucket(p.bk, lo, n0 + BN - 1 - m0 - p.start);
-            if (fb < 0) {
-                for (int i = tid; i < ROWS + BN - 1; i += NT)
-                    near_bias[i] = table.value[bucket_of(table.border, p.bk.n, p.bk.both, lo + i)];
-            } else {
-                far = table.value[fb];
+        float* near_here = near_bias[buffer];
+        tile.arrive(lds, tid, [&] {
+            if constexpr (BIAS) {
+                const int lo = n0 - (m0 + ROWS - 1) - p.start;
+                fb = far_bucket(p.bk, lo, n0 + BN - 1 - m0 - p.start);
+                if (fb < 0) {
+                    for (int i = tid; i < ROWS + BN - 1; i += NT)
+                        near_here[i] = table.value[bucket_of(table.border, p.bk.n, p.bk.both, lo + i)];
+                } else {
+                    far = table.value[fb];
+                }
             }
-        }
-        const int tn = seen.next(t + 1, t1);
-        __syncthreads();
-        if (tn < t1) {
-            const uint64_t nb = seen.of(tn);
-            ks.load(k + (int64_t)tn * BN * p.sk.r, p.sk.r, nb, p.D, vk, tid);
-            vs.load(v + (int64_t)tn * BN * p.sv.r, p.sv.r, nb, p.D, vv, tid);
-        }
-        t = tn;
+        });
+        const auto& kt = lds.a[buffer];
+        const auto& vt = lds.b[buffer];
+        buffer ^= BUFFERS - 1;
+        t = seen.next(t + 1, t1);
+        if (t < t1) fetch(t, buffer);
         if (mw >= p.M || (p.causal && n0 > mw + 31 + p.start)) continue;
 
         const bool edge = p.causal && n0 + BN - 1 > mw + p.start;
-        const bool all = bits == Staged<T, DP, BN, NT>::ALL && !edge;
+        const bool all = bits == PairT::ALL && !edge;
         const uint64_t mine = bits >> (4 * half);
         const int lim = edge ? m + p.start - n0 - 4 * half : BN;
-        const float* nb = &near_bias[BIAS ? ROWS - 1 - wave * 32 - col + 4 * half : 0];
+        const float* nb = &near_here[BIAS ? ROWS - 1 - wave * 32 - col + 4 * half : 0];
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             if (!(uint32_t)(bits >> (32 * i))) continue;               // no key among these 32
@@ -244,10 +243,12 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
 template <class T, int DP, int NW, bool BIAS>
 __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(const SmParams p) {
     constexpr int NP = Elem<T>::PARTS, BM = Shape<T, DP>::BN, NT = 64 * NW, KEYS = 32 * NW, NS = BM / 32, ND = DP / 32;
-    __shared__ Tile<NP, BM, DP> qt, gt;
-    __shared__ __attribute__((aligned(16))) float lse[BM], delta[BM];
+    typedef Pair<T, DP, BM, NW> PairT;
+    constexpr int BUFFERS = PairT::BUFFERS;
+    __shared__ typename PairT::Lds lds;
+    __shared__ __attribute__((aligned(16))) float lse_of[BUFFERS][BM], delta_of[BUFFERS][BM];
     __shared__ BiasLds table;
-    __shared__ float near_bias[BIAS ? KEYS + BM : 1];
+    __shared__ float near_bias[BUFFERS][BIAS ? KEYS + BM : 1];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
     const Work w = xcd_work(blockIdx.x, p.B * p.G, p.blocks * p.splits);
@@ -266,13 +267,12 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
             while (t < t1 && t % tiles * BM + BM - 1 + p.start < n0) ++t;
         return t;
     };
-    Staged<T, DP, BM, NT> qs(p.sq.r, p.D, p.vec & VEC_Q, tid), gs(p.sg.r, p.D, p.vec & VEC_G, tid);
+    PairT tile(p.sq.r, p.vec & VEC_Q, p.sg.r, p.vec & VEC_G, p.D, tid);
     float ls = HIGH, des = 0.f;
-    const auto load = [&](int t) {
+    const auto fetch = [&](int t, int buffer) {
         const int head = kvh * share + t / tiles, m0 = t % tiles * BM, left = p.M - m0;
-        const uint64_t bits = left >= BM ? Staged<T, DP, BM, NT>::ALL : (1ull << left) - 1;
-        qs.load((const T*)p.q + b * p.sq.b + head * p.sq.h + m0 * p.sq.r, p.sq.r, bits, p.D, p.vec & VEC_Q, tid);
-        gs.load((const T*)p.g_out + b * p.sg.b + head * p.sg.h + m0 * p.sg.r, p.sg.r, bits, p.D, p.vec & VEC_G, tid);
+        tile.fetch(lds, buffer, (const T*)p.q + b * p.sq.b + head * p.sq.h + m0 * p.sq.r,
+                   (const T*)p.g_out + b * p.sg.b + head * p.sg.h + m0 * p.sg.r, left >= BM ? PairT::ALL : (1ull << left) - 1, tid);
         ls = HIGH;
         des = 0.f;
         if (tid < BM && tid < left) {
@@ -281,8 +281,9 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
             des = p.delta[row];
         }
     };
-    int t = next((int)(work * split_i / p.splits));
-    if (t < t1) load(t);
+    if (p.M % BM || p.D < DP) PairT::clear(lds, tid);
+    int t = next((int)(work * split_i / p.splits)), buffer = 0;
+    if (t < t1) fetch(t, 0);
     Frag<NP> kf[DP / 16], vf[DP / 16];
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
@@ -304,37 +305,40 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
         const int m0 = t % tiles * BM, head = kvh * share + t / tiles;
         float far = 0.f;
         bool near = false;
-        __syncthreads();
-        qs.store(qt, tid);
-        gs.store(gt, tid);
-        if (tid < BM) {
-            lse[tid] = -ls / c2;
-            delta[tid] = -des;
+        float *near_here = near_bias[buffer], *lse = lse_of[buffer], *delta = delta_of[buffer];
+        if (BIAS && head != filled) {
+            __syncthreads();
+            table.fill(p, head, tid, NT);
+            filled = head;
+            __syncthreads();
         }
-        if constexpr (BIAS) {
-            if (head != filled) {
-                table.fill(p, head, tid, NT);
-                filled = head;
-                __syncthreads();
+        tile.arrive(lds, tid, [&] {
+            if (tid < BM) {
+                lse[tid] = -ls / c2;
+                delta[tid] = -des;
             }
-            const int lo = n0 - (m0 + BM - 1) - p.start;
-            const int fb = far_bucket(p.bk, lo, n0 + KEYS - 1 - m0 - p.start);
-            near = fb < 0;
-            if (near) {
-                for (int i = tid; i < KEYS + BM - 1; i += NT)
-                    near_bias[i] = table.value[bucket_of(table.border, p.bk.n, p.bk.both, lo + i)];
-            } else {
-                far = table.value[fb];
+            if constexpr (BIAS) {
+                const int lo = n0 - (m0 + BM - 1) - p.start;
+                const int fb = far_bucket(p.bk, lo, n0 + KEYS - 1 - m0 - p.start);
+                near = fb < 0;
+                if (near) {
+                    for (int i = tid; i < KEYS + BM - 1; i += NT)
+                        near_here[i] = table.value[bucket_of(table.border, p.bk.n, p.bk.both, lo + i)];
+                } else {
+                    far = table.value[fb];
+                }
             }
-        }
-        __syncthreads();
+        });
+        const auto& qt = lds.a[buffer];
+        const auto& gt = lds.b[buffer];
+        buffer ^= BUFFERS - 1;
         t = next(t + 1);
-        if (t < t1) load(t);
+        if (t < t1) fetch(t, buffer);
         if (idle || (p.causal && m0 + BM - 1 + p.start < nw)) continue;
 
         const bool edge = p.causal && m0 + p.start < nw + 31;
         const int lim = edge ? n - p.start - m0 - 4 * half : -1;         // the first query that sees the key
-        const float* nb = &near_bias[BIAS ? wave * 32 + col + BM - 1 - 4 * half : 0];
+        const float* nb = &near_here[BIAS ? wave * 32 + col + BM - 1 - 4 * half : 0];
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             if (m0 + 32 * i >= p.M) continue;

@@ -25,9 +25,11 @@ constexpr float GROW = 8.f;
 template <class T, int DP, int NW, bool BIAS, bool FINE>
 __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(const SmParams p) {
     constexpr int NP = Elem<T>::PARTS, BN = Shape<T, DP>::BN, NT = 64 * NW, ROWS = 32 * NW, NS = BN / 32, ND = DP / 32;
-    __shared__ Tile<NP, BN, DP> kt, vt;
+    typedef Pair<T, DP, BN, NW> PairT;
+    constexpr int BUFFERS = PairT::BUFFERS;
+    __shared__ typename PairT::Lds lds;
     __shared__ BiasLds table;
-    __shared__ float near_bias[BIAS ? ROWS + BN : 1];
+    __shared__ float near_bias[BUFFERS][BIAS ? ROWS + BN : 1];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
     const Work w = xcd_work(blockIdx.x, p.B * p.H, p.blocks * p.splits);
@@ -37,7 +39,6 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
     const T* q = (const T*)p.q + b * p.sq.b + head * p.sq.h;
     const T* k = (const T*)p.k + b * p.sk.b + kvh * p.sk.h;
     const T* v = (const T*)p.v + b * p.sv.b + kvh * p.sv.h;
-    const bool vk = p.vec & VEC_K, vv = p.vec & VEC_V;
 
     const int tiles = (p.N + BN - 1) / BN;
     int t0 = (int)((int64_t)tiles * split_i / p.splits), t1 = (int)((int64_t)tiles * (split_i + 1) / p.splits);
@@ -46,13 +47,14 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
         t1 = min(t1, last < 0 ? 0 : last / BN + 1);
     }
     KeyBits<BN> seen(p, b);
-    Staged<T, DP, BN, NT> ks(p.sk.r, p.D, vk, tid), vs(p.sv.r, p.D, vv, tid);
-    int t = seen.next(t0, t1);
-    if (t < t1) {
-        const uint64_t bits = seen.of(t);
-        ks.load(k + (int64_t)t * BN * p.sk.r, p.sk.r, bits, p.D, vk, tid);
-        vs.load(v + (int64_t)t * BN * p.sv.r, p.sv.r, bits, p.D, vv, tid);
-    }
+    PairT tile(p.sk.r, p.vec & VEC_K, p.sv.r, p.vec & VEC_V, p.D, tid);
+    const auto fetch = [&](int t, int buffer) {
+        tile.fetch(lds, buffer, k + (int64_t)t * BN * p.sk.r, v + (int64_t)t * BN * p.sv.r, seen.of(t), tid);
+    };
+    if (p.keep || p.N % BN || p.D < DP) PairT::clear(lds, tid);
+    int t = seen.next(t0, t1), buffer = 0;
+    if (t < t1) fetch(t, 0);
+
     Frag<NP> qf[DP / 16];
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
@@ -75,28 +77,25 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
         const uint64_t bits = seen.of(t);
         float far = 0.f;
         bool near = false;
-        __syncthreads();
-        ks.store(kt, tid);
-        vs.store(vt, tid);
-        if constexpr (BIAS) {
-            const int lo = n0 - (m0 + ROWS - 1) - p.start;
-            const int fb = far_bucket(p.bk, lo, n0 + BN - 1 - m0 - p.start);
-            near = fb < 0;
-            if (near) {
-                for (int i = tid; i < ROWS + BN - 1; i += NT)
-                    near_bias[i] = table.value[bucket_of(table.border, p.bk.n, p.bk.both, lo + i)];
-            } else {
-                far = table.value[fb];
+        float* near_here = near_bias[buffer];
+        tile.arrive(lds, tid, [&] {
+            if constexpr (BIAS) {
+                const int lo = n0 - (m0 + ROWS - 1) - p.start;
+                const int fb = far_bucket(p.bk, lo, n0 + BN - 1 - m0 - p.start);
+                near = fb < 0;
+                if (near) {
+                    for (int i = tid; i < ROWS + BN - 1; i += NT)
+                        near_here[i] = table.value[bucket_of(table.border, p.bk.n, p.bk.both, lo + i)];
+                } else {
+                    far = table.value[fb];
+                }
             }
-        }
-        const int tn = seen.next(t + 1, t1);
-        __syncthreads();
-        if (tn < t1) {
-            const uint64_t nb = seen.of(tn);
-            ks.load(k + (int64_t)tn * BN * p.sk.r, p.sk.r, nb, p.D, vk, tid);
-            vs.load(v + (int64_t)tn * BN * p.sv.r, p.sv.r, nb, p.D, vv, tid);
-        }
-        t = tn;
+        });
+        const auto& kt = lds.a[buffer];
+        const auto& vt = lds.b[buffer];
+        buffer ^= BUFFERS - 1;
+        t = seen.next(t + 1, t1);
+        if (t < t1) fetch(t, buffer);
         if (mw >= p.M || (p.causal && n0 > mw + 31 + p.start)) continue;
 
         f32x16 s[NS];
@@ -117,11 +116,11 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
         // scores in log2 units are fma(s, mul, add) from here on
         float mul = c2, add = far;
         const bool edge = p.causal && n0 + BN - 1 > mw + p.start;
-        const bool all = bits == Staged<T, DP, BN, NT>::ALL && !edge;
+        const bool all = bits == PairT::ALL && !edge;
         if (near || !all) {
             const uint64_t mine = bits >> (4 * half);
             const int lim = edge ? m + p.start - n0 - 4 * half : BN;     // the last key seen
-            const float* nb = &near_bias[BIAS ? ROWS - 1 - wave * 32 - col + 4 * half : 0];
+            const float* nb = &near_here[BIAS ? ROWS - 1 - wave * 32 - col + 4 * half : 0];
 #pragma unroll
             for (int i = 0; i < NS; ++i)
 #pragma unroll

@@ -126,34 +126,41 @@ template <class T> __device__ __forceinline__ typename Elem<T>::seg load_seg(con
     return x;
 }
 
-// A tile of ROWS rows of DP elements in LDS, one plane for each part; rows are 16 bytes further apart than their length,
-// which spreads both the row reads and the transposing reads over the banks.
+// A tile of ROWS rows of DP elements in LDS, one plane for each part, without gaps. A row's 16-byte pieces are turned
+// (exclusive or) by bits of the row's number so that the 128 bytes that LDS gives in a cycle, one piece of 8 rows or the two
+// pieces of 4 rows that a transposing read takes, are on different banks.
 template <int NP, int ROWS, int DP> struct Tile {
-    static constexpr int LD = DP + 8, PLANE = ROWS * LD;
+    static constexpr int PLANE = ROWS * DP, PIECES = DP / 8;
     __bf16 x[NP * PLANE];
 
-    template <class Seg> __device__ __forceinline__ void put(int row, int d, Seg s) {
+    static __device__ __forceinline__ int turn(int row) {
+        return DP == 32 ? (row & 2) | (row >> 2 & 1) : (row & 3) << 1 | (row >> 2 & 1);
+    }
+    static __device__ __forceinline__ int at(int row, int piece) { return row * DP + ((piece ^ turn(row)) << 3); }
+
+    template <class Seg> __device__ __forceinline__ void put(int row, int piece, Seg s) {
         const Frag<NP> f = frag_of(s);
 #pragma unroll
-        for (int i = 0; i < NP; ++i) *reinterpret_cast<bf16x8*>(&x[i * PLANE + row * LD + d]) = f.p[i];
+        for (int i = 0; i < NP; ++i) *reinterpret_cast<bf16x8*>(&x[i * PLANE + at(row, piece)]) = f.p[i];
     }
     // elements d .. d + 7 of a row
     __device__ __forceinline__ Frag<NP> row(int row, int d) const {
         Frag<NP> f;
 #pragma unroll
-        for (int i = 0; i < NP; ++i) f.p[i] = *reinterpret_cast<const bf16x8*>(&x[i * PLANE + row * LD + d]);
+        for (int i = 0; i < NP; ++i) f.p[i] = *reinterpret_cast<const bf16x8*>(&x[i * PLANE + at(row, d >> 3)]);
         return f;
     }
     // column d0 + lane % 32 over rows row0 .. row0 + 15, in the slots' order
     __device__ __forceinline__ Frag<NP> column(int row0, int d0, int lane) const {
-        const int at = (row0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * LD + d0 + (lane & 16) + (lane & 3) * 4;
+        const int row = row0 + 4 * (lane >> 5) + ((lane & 15) >> 2);
+        const int from = at(row, (d0 >> 3) + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) + (lane & 1) * 4;
         Frag<NP> f;
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
             union { s16x4 s[2]; bf16x8 b; } u;
             typedef __attribute__((address_space(3))) s16x4 lds4;
-            u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)&x[i * PLANE + at]);
-            u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)&x[i * PLANE + at + 8 * LD]);
+            u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)&x[i * PLANE + from]);
+            u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)&x[i * PLANE + from + 8 * DP]);   // turned alike
             f.p[i] = u.b;
         }
         return f;
@@ -169,35 +176,126 @@ template <class T, int DP> struct Shape {
     static constexpr int WAVES = NP == 3 && DP == 128 ? 1 : 2;
 };
 
-// This thread's share of a tile of BN rows, between its global loads and its LDS stores.
-template <class T, int DP, int BN, int NT> struct Staged {
-    static constexpr int SEGS = DP / 8, PER = BN * SEGS / NT;
-    static constexpr uint64_t ALL = BN == 64 ? ~0ull : (1ull << BN % 64) - 1;
-    typename Elem<T>::seg s[PER];
-    uint32_t at;                           // of this thread's first piece from the tile's first row; the others are STEP rows apart
-    bool whole;                            // a tile without gaps is read without any test
-    static constexpr int STEP = NT / SEGS;
-    static_assert(PER * NT == BN * SEGS && STEP * SEGS == NT, "every thread takes the same column of PER rows");
+// 16 bytes a lane from memory to LDS, lane l's to `to` + 16 l bytes. Written out because of the waits: before every transposing
+// read the compiler would wait for its own form of this, though that goes to the other buffer. Pair::arrive() waits.
+// The low half of a generic pointer into LDS is the place in LDS.
+__device__ __forceinline__ uint32_t lds_place(const void* to) {
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)to);
+}
+__device__ __forceinline__ void load_to_lds(const void* from, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(to), "v"(from) : "memory", "m0");
+}
+__device__ __forceinline__ void load_to_lds(const void* from, uint32_t bytes, uint32_t to) {      // from is the same for all lanes
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :: "s"(to), "v"(bytes), "s"(from) : "memory", "m0");
+}
 
-    __device__ __forceinline__ Staged(int64_t stride, int D, bool vec, int tid)
-        : at((uint32_t)(tid / SEGS * stride) + tid % SEGS * 8), whole(vec && D == DP && stride < 1 << 24) {}
-    // tile: its first row; bits: the rows to read, zeros for the others
-    __device__ __forceinline__ void load(const T* tile, int64_t stride, uint64_t bits, int D, bool vec, int tid) {
-        if (whole && bits == ALL) {
-#pragma unroll
-            for (int i = 0; i < PER; ++i) s[i] = *reinterpret_cast<const typename Elem<T>::seg*>(tile + i * STEP * stride + at);
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int row = tid / SEGS + i * STEP, d = tid % SEGS * 8;
-            s[i] = {};
-            if (bits >> row & 1) s[i] = load_seg(tile + row * stride, d, D, vec);
+// Two tiles (k and v, or q and dO) of ROWS rows on their way into LDS, where a workgroup of NW waves then reads them.
+//
+// bf16 goes there directly (global_load_lds, 16 bytes a lane, 1 KB an instruction; the pieces are turned by reading from turned
+// places), into the other one of two buffers while the current one is read: no registers hold a tile, and one barrier a tile is
+// enough. Rows that are not to be read, and pieces past D, are left out: they hold zeros, or a row of an earlier tile, whose
+// products are multiplied by a probability of zero. float goes through registers, where it is split into parts, and
+// has one buffer and two barriers.
+template <class T, int DP, int ROWS, int NW> struct Pair {
+    static constexpr int NP = Elem<T>::PARTS, NT = 64 * NW, PIECES = DP / 8, BUFFERS = NP == 1 ? 2 : 1;
+    static constexpr uint64_t ALL = ROWS == 64 ? ~0ull : (1ull << ROWS % 64) - 1;
+    typedef Tile<NP, ROWS, DP> TileT;
+    struct Lds { TileT a[BUFFERS], b[BUFFERS]; };
+    static constexpr int HELD = NP == 1 ? 1 : ROWS * PIECES / NT, STEP = NT / PIECES;
+    static_assert(NP == 1 || (HELD * NT == ROWS * PIECES && STEP * PIECES == NT), "a thread takes one column of HELD rows");
+
+    // Rows whose pieces a lane takes: the first one, and every APART-th after it.
+    static constexpr int RPI = 64 / PIECES, EACH = ROWS / RPI / NW, APART = RPI * NW;
+    static constexpr bool ALIKE = APART % 8 == 0 || EACH == 1;       // they are turned alike
+
+    int64_t stride_a, stride_b;
+    int D;
+    bool vec_a, vec_b, whole;
+    uint32_t at_a, at_b;                   // bytes from a tile's first row to this lane's piece
+    typename Elem<T>::seg a[HELD], b[HELD];
+
+    __device__ __forceinline__ Pair(int64_t stride_a, bool vec_a, int64_t stride_b, bool vec_b, int D, int tid)
+        : stride_a(stride_a), stride_b(stride_b), D(D), vec_a(vec_a), vec_b(vec_b) {
+        whole = vec_a && vec_b && D == DP && stride_a < 1 << 22 && stride_b < 1 << 22 && (NP != 1 || ALIKE);
+        int row = tid / PIECES, piece = tid % PIECES;
+        if constexpr (NP == 1) piece ^= TileT::turn(row);
+        at_a = (uint32_t)(row * stride_a + piece * 8) * sizeof(T);
+        at_b = (uint32_t)(row * stride_b + piece * 8) * sizeof(T);
+    }
+    // before the first tile, when some rows or pieces will be left out
+    __device__ __forceinline__ static void clear(Lds& lds, int tid) {
+        if constexpr (NP == 1) {
+            bf16x8* x = reinterpret_cast<bf16x8*>(&lds);
+            for (int i = tid; i < (int)(sizeof(Lds) / 16); i += NT) x[i] = bf16x8{};
+            __syncthreads();
         }
     }
-    template <class TileT> __device__ __forceinline__ void store(TileT& t, int tid) const {
+    // tile_a, tile_b: first rows; bits: the rows to read
+    __device__ __forceinline__ void fetch(Lds& lds, int buffer, const T* tile_a, const T* tile_b, uint64_t bits, int tid) {
+        if (whole && bits == ALL) {                        // without any test
+            if constexpr (NP == 1) {
+                const uint32_t to_a = lds_place(&lds.a[buffer].x[(tid >> 6) * RPI * DP]);
+                const uint32_t to_b = lds_place(&lds.b[buffer].x[(tid >> 6) * RPI * DP]);
 #pragma unroll
-        for (int i = 0; i < PER; ++i) t.put((tid + i * NT) / SEGS, (tid + i * NT) % SEGS * 8, s[i]);
+                for (int j = 0; j < EACH; ++j) load_to_lds(tile_a + j * APART * stride_a, at_a, to_a + j * APART * DP * 2);
+#pragma unroll
+                for (int j = 0; j < EACH; ++j) load_to_lds(tile_b + j * APART * stride_b, at_b, to_b + j * APART * DP * 2);
+            } else {
+                typedef const typename Elem<T>::seg* segs;
+#pragma unroll
+                for (int i = 0; i < HELD; ++i) {
+                    a[i] = *(segs)((const char*)(tile_a + i * STEP * stride_a) + at_a);
+                    b[i] = *(segs)((const char*)(tile_b + i * STEP * stride_b) + at_b);
+                }
+            }
+        } else if constexpr (NP == 1) {
+            direct(lds.a[buffer], tile_a, stride_a, vec_a, bits, tid);
+            direct(lds.b[buffer], tile_b, stride_b, vec_b, bits, tid);
+        } else {
+            hold(a, tile_a, stride_a, vec_a, bits, tid);
+            hold(b, tile_b, stride_b, vec_b, bits, tid);
+        }
+    }
+    // until here the fetched tile has arrived and nobody reads the buffer that the next fetch goes to; between two calls of it
+    // what `more` writes is read
+    template <class F> __device__ __forceinline__ void arrive(Lds& lds, int tid, F more) {
+        if constexpr (NP == 1) {
+            more();
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+        } else {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) {
+                lds.a[0].put(tid / PIECES + i * STEP, tid % PIECES, a[i]);
+                lds.b[0].put(tid / PIECES + i * STEP, tid % PIECES, b[i]);
+            }
+            more();
+            __syncthreads();
+        }
+    }
+
+private:
+    __device__ __forceinline__ void direct(TileT& t, const T* from, int64_t stride, bool vec, uint64_t bits, int tid) {
+        const int lane = tid & 63;
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) {
+            const int first = (tid >> 6) * RPI + j * APART, row = first + lane / PIECES;
+            const int piece = lane % PIECES ^ TileT::turn(row);
+            const uint32_t to = lds_place(&t.x[first * DP]);
+            if (!(bits >> row & 1) || piece * 8 >= D) continue;
+            if (vec) load_to_lds(from + row * stride + piece * 8, to);
+            else *reinterpret_cast<bf16x8*>(&t.x[row * DP + lane % PIECES * 8]) = load_seg(from + row * stride, piece * 8, D, false);
+        }
+    }
+    __device__ __forceinline__ void hold(typename Elem<T>::seg* s, const T* from, int64_t stride, bool vec, uint64_t bits, int tid) {
+        const int row = tid / PIECES, d = tid % PIECES * 8;
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            s[i] = {};
+            if (bits >> (row + i * STEP) & 1) s[i] = load_seg(from + (row + i * STEP) * stride, d, D, vec);
+        }
     }
 };
 
