@@ -65,6 +65,20 @@ __device__ __forceinline__ void add_band(f32x16 ds, int base, float* acc, const 
     if (lane == 63 || after != bucket) acc[bucket] += x;
 }
 
+// f(first half, halves together): both halves of a tile together where registers reach for it, the second only where it has
+// something to do
+template <int NP, int NS, class F> __device__ __forceinline__ void by_halves(bool one, F f) {
+    typedef std::integral_constant<int, 0> zero;
+    typedef std::integral_constant<int, 1> single;
+    if constexpr (NP == 1 && NS == 2) {
+        if (!one) return f(zero(), std::integral_constant<int, 2>());
+    }
+    f(zero(), single());
+    if constexpr (NP != 1 && NS == 2) {
+        if (!one) f(single(), single());
+    }
+}
+
 template <class T, int DP, int NW, bool BIAS>
 __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(const SmParams p) {
     constexpr int NP = Elem<T>::PARTS, BN = Shape<T, DP>::BN, NT = 64 * NW, ROWS = 32 * NW, NS = BN / 32, ND = DP / 32;
@@ -162,49 +176,67 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
         const uint64_t mine = bits >> (4 * half);
         const int lim = edge ? m + p.start - n0 - 4 * half : BN;
         const float* nb = &near_here[BIAS ? ROWS - 1 - wave * 32 - col + 4 * half : 0];
+        const float add = far - lse;
+        // `count` halves of the tile together: the products of one are under way while the other's scores are worked on
+        const auto halves = [&](auto first, auto count) {
+            f32x16 s[count], dp[count];
 #pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            if (!(uint32_t)(bits >> (32 * i))) continue;               // no key among these 32
-            Acc<NP> sa, dpa;
-            sa.start();
+            for (int i = 0; i < count; ++i) {
+                Acc<NP> a;
+                a.start();
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) sa.add(kt.row(32 * i + col, 16 * c + 8 * half), qf[c]);
-            sa.join();
-            dpa.start();
-#pragma unroll
-            for (int c = 0; c < DP / 16; ++c) dpa.add(vt.row(32 * i + col, 16 * c + 8 * half), gf[c]);
-            dpa.join();
-            f32x16 s = sa.main;
-            const f32x16 dp = dpa.main;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int n = 32 * i + reg_row(r);
-                const float e = fexp2(__builtin_fmaf(s[r], c2, (BIAS && fb < 0 ? nb[n] : far) - lse));
-                float ds = e * (dp[r] - delta);
-                if (!all && !((mine >> n & 1) && n <= lim)) ds = 0.f;
-                s[r] = ds;
+                for (int c = 0; c < DP / 16; ++c) a.add(kt.row(32 * (first + i) + col, 16 * c + 8 * half), qf[c]);
+                a.join();
+                s[i] = a.main;
             }
-            if (to_table) {
-                if (fb < 0) {
-                    add_band(s, n0 + 32 * i - mw - p.start, sums[wave], table.border, p.bk, lane);
-                } else {
-                    float a = 0.f;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) a += s[r];
-                    if (fb == p.bk.n) left += a; else right += a;
+            for (int i = 0; i < count; ++i) {
+                Acc<NP> a;
+                a.start();
+#pragma unroll
+                for (int c = 0; c < DP / 16; ++c) a.add(vt.row(32 * (first + i) + col, 16 * c + 8 * half), gf[c]);
+                a.join();
+                dp[i] = a.main;
+            }
+#pragma unroll
+            for (int i = 0; i < count; ++i) {
+                if (BIAS && fb < 0) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c2, nb[32 * (first + i) + reg_row(r)] - lse);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c2, add);
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[i][r] = fexp2(s[i][r]) * (dp[i][r] - delta);
+                if (!all) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (!(mine >> (32 * (first + i) + reg_row(r)) & 1) || 32 * (first + i) + reg_row(r) > lim) s[i][r] = 0.f;
+                }
+                if (to_table) {
+                    if (fb < 0) {
+                        add_band(s[i], n0 + 32 * (first + i) - mw - p.start, sums[wave], table.border, p.bk, lane);
+                    } else {
+                        float a = 0.f;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) a += s[i][r];
+                        if (fb == p.bk.n) left += a; else right += a;
+                    }
+                }
+                Frag<NP> df[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) df[c] = split<NP>(eight(s[i], c));
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    dq[d].start();
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) dq[d].add(kt.column(32 * (first + i) + 16 * c, 32 * d, lane), df[c]);
+                    dq[d].join();
                 }
             }
-            Frag<NP> df[2];
-#pragma unroll
-            for (int c = 0; c < 2; ++c) df[c] = split<NP>(eight(s, c));
-#pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                dq[d].start();
-#pragma unroll
-                for (int c = 0; c < 2; ++c) dq[d].add(kt.column(32 * i + 16 * c, 32 * d, lane), df[c]);
-                dq[d].join();
-            }
-        }
+        };
+        by_halves<NP, NS>(NS == 1 || !(bits >> 32), halves);
     }
     if (to_table) {
 #pragma unroll
@@ -299,6 +331,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
 
     const float c2 = p.scale * LOG2E;
     Acc<NP> dk[ND], dv[ND];
+    const float per_c2 = 1.f / c2;
     int filled = -1;                                   // the head whose bias stands in LDS
 
     while (t < t1) {
@@ -314,7 +347,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
         }
         tile.arrive(lds, tid, [&] {
             if (tid < BM) {
-                lse[tid] = -ls / c2;
+                lse[tid] = -ls * per_c2;
                 delta[tid] = -des;
             }
             if constexpr (BIAS) {
@@ -339,48 +372,68 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
         const bool edge = p.causal && m0 + p.start < nw + 31;
         const int lim = edge ? n - p.start - m0 - 4 * half : -1;         // the first query that sees the key
         const float* nb = &near_here[BIAS ? wave * 32 + col + BM - 1 - 4 * half : 0];
-#pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            if (m0 + 32 * i >= p.M) continue;
+        const auto halves = [&](auto first, auto count) {
             // scores less the row's log sum (in units of the scores), and dP less delta
-            Acc<NP> sa(rows_of(lse, 32 * i + 4 * half)), dpa(rows_of(delta, 32 * i + 4 * half));
-            sa.start();
+            f32x16 s[count], dp[count];
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) sa.add(qt.row(32 * i + col, 16 * c + 8 * half), kf[c]);
-            sa.join();
-            dpa.start();
+            for (int i = 0; i < count; ++i) {
+                Acc<NP> a(rows_of(lse, 32 * (first + i) + 4 * half));
+                a.start();
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) dpa.add(gt.row(32 * i + col, 16 * c + 8 * half), vf[c]);
-            dpa.join();
-            f32x16 s = sa.main, dp = dpa.main;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int mr = 32 * i + reg_row(r);
-                float e = fexp2(__builtin_fmaf(s[r], c2, BIAS && near ? nb[-mr] : far));
-                if (edge && mr < lim) e = 0.f;
-                s[r] = e;
-                dp[r] = edge && mr < lim ? 0.f : e * dp[r];
-            }
-            Frag<NP> f[2];
-#pragma unroll
-            for (int c = 0; c < 2; ++c) f[c] = split<NP>(eight(s, c));
-#pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                dv[d].start();
-#pragma unroll
-                for (int c = 0; c < 2; ++c) dv[d].add(gt.column(32 * i + 16 * c, 32 * d, lane), f[c]);
-                dv[d].join();
+                for (int c = 0; c < DP / 16; ++c) a.add(qt.row(32 * (first + i) + col, 16 * c + 8 * half), kf[c]);
+                a.join();
+                s[i] = a.main;
             }
 #pragma unroll
-            for (int c = 0; c < 2; ++c) f[c] = split<NP>(eight(dp, c));
+            for (int i = 0; i < count; ++i) {
+                Acc<NP> a(rows_of(delta, 32 * (first + i) + 4 * half));
+                a.start();
 #pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                dk[d].start();
-#pragma unroll
-                for (int c = 0; c < 2; ++c) dk[d].add(qt.column(32 * i + 16 * c, 32 * d, lane), f[c]);
-                dk[d].join();
+                for (int c = 0; c < DP / 16; ++c) a.add(gt.row(32 * (first + i) + col, 16 * c + 8 * half), vf[c]);
+                a.join();
+                dp[i] = a.main;
             }
-        }
+#pragma unroll
+            for (int i = 0; i < count; ++i) {
+                if (BIAS && near) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c2, nb[-32 * (first + i) - reg_row(r)]);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c2, far);
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s[i][r] = fexp2(s[i][r]);
+                    dp[i][r] *= s[i][r];
+                }
+                if (edge) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (32 * (first + i) + reg_row(r) < lim) s[i][r] = dp[i][r] = 0.f;
+                }
+                Frag<NP> f[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) f[c] = split<NP>(eight(s[i], c));
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    dv[d].start();
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) dv[d].add(gt.column(32 * (first + i) + 16 * c, 32 * d, lane), f[c]);
+                    dv[d].join();
+                }
+#pragma unroll
+                for (int c = 0; c < 2; ++c) f[c] = split<NP>(eight(dp[i], c));
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    dk[d].start();
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) dk[d].add(qt.column(32 * (first + i) + 16 * c, 32 * d, lane), f[c]);
+                    dk[d].join();
+                }
+            }
+        };
+        by_halves<NP, NS>(m0 + 32 >= p.M, halves);
     }
     if (n >= p.N) return;
     const float f = p.scale * p.q_sign;
