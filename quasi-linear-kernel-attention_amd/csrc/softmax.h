@@ -40,14 +40,10 @@ struct SmParams {
     int B, H, G, M, N, D;
     int causal, start;
     int splits, blocks;                      // splits of the long axis; blocks of rows (or keys) per head
-    int vec;                                 // bit per operand: its rows are read / written in 16-byte pieces
     float scale;                             // |scale|; its sign (or 0) is in q_sign
     float q_sign;
     SmBuckets bk;
 };
-
-enum SmVec : int { VEC_Q = 1, VEC_K = 2, VEC_V = 4, VEC_G = 8, VEC_O = 16, VEC_GQ = 32, VEC_GK = 64, VEC_GV = 128, VEC_KEEP = 256,
-                   VEC_FULL = 512 };
 
 // Elements of a row in LDS and in the partial rows.
 inline int sm_padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
@@ -63,7 +59,7 @@ int sm_delta(int dtype, const SmParams& p, hipStream_t st);
 int sm_dq(int dtype, const SmParams& p, int waves, hipStream_t st);
 int sm_dkv(int dtype, const SmParams& p, int waves, hipStream_t st);
 // out[row] = scale * sum over the splits of part's rows; rows of heads x len per batch
-int sm_sum_parts(int dtype, const float* part, void* out, SmStrides so, bool vec, float scale, int splits, int B, int heads,
+int sm_sum_parts(int dtype, const float* part, void* out, SmStrides so, float scale, int splits, int B, int heads,
                  int len, int D, hipStream_t st);
 // g_table[bucket][h] = sum of part_table over its count rows
 int sm_sum_table(const float* part, float* g_table, int H, int count, int buckets, hipStream_t st);

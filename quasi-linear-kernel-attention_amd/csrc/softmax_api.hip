@@ -55,7 +55,7 @@ int check_sizes(const qlka_softmax_args* a) {
     if (a->dtype != QLKA_F32 && a->dtype != QLKA_BF16) return refuse("dtype must be QLKA_F32 or QLKA_BF16");
     if (a->B < 0 || a->M < 0 || a->N < 0 || a->H < 1 || a->G < 1) return refuse("B, M and N must be >= 0, H and G >= 1");
     if (a->H % a->G) return refuse("H must be a multiple of G");
-    if (a->D < 1 || a->D > 128) return refuse("D must be in [1, 128]");
+    if (a->D < 8 || a->D > 128 || a->D % 8) return refuse("D must be a multiple of 8 in [8, 128]");
     if (a->M > LONGEST || a->N > LONGEST || a->start > LONGEST || a->start < -LONGEST)
         return refuse("M, N and |start| must be <= 2^28");
     if ((double)a->B * a->H * a->M > (double)MOST_ROWS || (double)a->B * a->G * a->N > (double)MOST_ROWS)
@@ -148,10 +148,13 @@ BwdPlan bwd_plan(const qlka_softmax_args* a, bool dq, bool dkv, bool table) {
 
 SmStrides strides(const int64_t* s) { return {s[0], s[1], s[2]}; }
 
-bool in_pieces(const qlka_softmax_args* a, const void* x, const int64_t* s, int heads, int rows) {
+// Rows are read and written in pieces of 16 bytes.
+int check_rows(const qlka_softmax_args* a, const char* name, const void* x, const int64_t* s, int heads, int rows) {
     const int64_t piece = a->dtype == QLKA_F32 ? 4 : 8;
-    return a->D % 8 == 0 && (uintptr_t)x % 16 == 0 && (a->B <= 1 || s[0] % piece == 0) &&
-           (heads <= 1 || s[1] % piece == 0) && (rows <= 1 || s[2] % piece == 0);
+    if (!x || ((uintptr_t)x % 16 == 0 && (a->B <= 1 || s[0] % piece == 0) && (heads <= 1 || s[1] % piece == 0) &&
+               (rows <= 1 || s[2] % piece == 0)))
+        return QLKA_OK;
+    return refuse("the rows of %s must be aligned to 16 bytes", name);
 }
 
 int params(const qlka_softmax_args* a, SmParams* p) {
@@ -172,15 +175,14 @@ int params(const qlka_softmax_args* a, SmParams* p) {
     // scores are held in units of the scale, so a scale of 0 goes into the sign
     p->scale = a->scale == 0.f ? 1.f : std::fabs(a->scale);
     p->q_sign = a->scale == 0.f ? 0.f : a->scale < 0.f ? -1.f : 1.f;
-    const auto bit = [&](int v, const void* x, const int64_t* s, int heads, int rows) {
-        return in_pieces(a, x, s, heads, rows) ? v : 0; };
-    p->vec = bit(VEC_Q, a->q, a->q_stride, a->H, a->M) | bit(VEC_K, a->k, a->k_stride, a->G, a->N) |
-             bit(VEC_V, a->v, a->v_stride, a->G, a->N) | bit(VEC_G, a->g_out, a->g_out_stride, a->H, a->M) |
-             bit(VEC_GQ, a->g_q, a->g_q_stride, a->H, a->M) | bit(VEC_GK, a->g_k, a->g_k_stride, a->G, a->N) |
-             bit(VEC_GV, a->g_v, a->g_v_stride, a->G, a->N);
-    p->vec |= bit(VEC_O, a->out, a->out_stride, a->H, a->M);
-    if (a->D % 8 == 0 && (uintptr_t)a->out_full % 16 == 0) p->vec |= VEC_FULL;
-    if ((uintptr_t)a->keep % 16 == 0 && (a->B <= 1 || a->keep_stride % 16 == 0)) p->vec |= VEC_KEEP;
+    const struct { const char* name; const void* x; const int64_t* s; int heads, rows; } all[] = {
+        {"q", a->q, a->q_stride, a->H, a->M},          {"k", a->k, a->k_stride, a->G, a->N},
+        {"v", a->v, a->v_stride, a->G, a->N},          {"out", a->out, a->out_stride, a->H, a->M},
+        {"g_out", a->g_out, a->g_out_stride, a->H, a->M}, {"g_q", a->g_q, a->g_q_stride, a->H, a->M},
+        {"g_k", a->g_k, a->g_k_stride, a->G, a->N},    {"g_v", a->g_v, a->g_v_stride, a->G, a->N}};
+    for (const auto& o : all)
+        if (int e = check_rows(a, o.name, o.x, o.s, o.heads, o.rows)) return e;
+    if ((uintptr_t)a->out_full % 16) return refuse("out_full must be aligned to 16 bytes");
     return a->table ? check_buckets(a->border, a->num_borders, a->bidirectional, &p->bk) : QLKA_OK;
 }
 
@@ -275,7 +277,7 @@ int qlka_softmax_bwd(const qlka_softmax_args* a, void* ws, size_t ws_bytes, void
         }
         if (p.splits > 1 && a->g_q) {
             StageTimer timer("softmax_sum", st);
-            if (int e = sm_sum_parts(a->dtype, p.part, a->g_q, p.sgq, p.vec & VEC_GQ, a->scale, p.splits, a->B, a->H, a->M,
+            if (int e = sm_sum_parts(a->dtype, p.part, a->g_q, p.sgq, a->scale, p.splits, a->B, a->H, a->M,
                                      a->D, st))
                 return status(e, "softmax attention backward, joining of splits");
         }
@@ -295,8 +297,8 @@ int qlka_softmax_bwd(const qlka_softmax_args* a, void* ws, size_t ws_bytes, void
         }
         if (p.splits > 1) {
             StageTimer timer("softmax_sum", st);
-            int e = sm_sum_parts(a->dtype, p.part, a->g_k, p.sgk, p.vec & VEC_GK, a->scale, p.splits, a->B, a->G, a->N, a->D, st);
-            if (!e) e = sm_sum_parts(a->dtype, p.part2, a->g_v, p.sgv, p.vec & VEC_GV, 1.f, p.splits, a->B, a->G, a->N, a->D, st);
+            int e = sm_sum_parts(a->dtype, p.part, a->g_k, p.sgk, a->scale, p.splits, a->B, a->G, a->N, a->D, st);
+            if (!e) e = sm_sum_parts(a->dtype, p.part2, a->g_v, p.sgv, 1.f, p.splits, a->B, a->G, a->N, a->D, st);
             if (e) return status(e, "softmax attention backward, joining of splits");
         }
     }

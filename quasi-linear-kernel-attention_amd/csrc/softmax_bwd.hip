@@ -26,9 +26,9 @@ __global__ __launch_bounds__(256) void softmax_delta(const SmParams p) {
     if (row < rows) {
         const int m = (int)(row % p.M), head = (int)(row / p.M % p.H), b = (int)(row / p.M / p.H);
         const T* out = (const T*)p.out + b * p.so.b + head * p.so.h + m * p.so.r;
-        const auto g = load_seg((const T*)p.g_out + b * p.sg.b + head * p.sg.h + m * p.sg.r, d, p.D, p.vec & VEC_G);
-        const f32x8 o = p.out_full ? load_seg(p.out_full + row * p.D, d, p.D, p.vec & VEC_FULL)
-                                   : floats(load_seg(out, d, p.D, p.vec & VEC_O));
+        const auto g = load_seg((const T*)p.g_out + b * p.sg.b + head * p.sg.h + m * p.sg.r, d, p.D);
+        const f32x8 o = p.out_full ? load_seg(p.out_full + row * p.D, d, p.D)
+                                   : floats(load_seg(out, d, p.D));
 #pragma unroll
         for (int i = 0; i < 8; ++i) x = __builtin_fmaf((float)g[i], o[i], x);
     }
@@ -65,17 +65,14 @@ __device__ __forceinline__ void add_band(f32x16 ds, int base, float* acc, const 
     if (lane == 63 || after != bucket) acc[bucket] += x;
 }
 
-// f(first half, halves together): both halves of a tile together where registers reach for it, the second only where it has
-// something to do
+// f(first half, halves together): both halves of a tile together where registers reach for it, else one after the other, and
+// the second only where it has something to do
 template <int NP, int NS, class F> __device__ __forceinline__ void by_halves(bool one, F f) {
-    typedef std::integral_constant<int, 0> zero;
-    typedef std::integral_constant<int, 1> single;
-    if constexpr (NP == 1 && NS == 2) {
-        if (!one) return f(zero(), std::integral_constant<int, 2>());
-    }
-    f(zero(), single());
-    if constexpr (NP != 1 && NS == 2) {
-        if (!one) f(single(), single());
+    if constexpr (NP == 1) {
+        f(0, std::integral_constant<int, NS>());
+    } else {
+#pragma unroll 1
+        for (int i = 0; i < (one ? 1 : NS); ++i) f(i, std::integral_constant<int, 1>());
     }
 }
 
@@ -86,6 +83,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
     constexpr int BUFFERS = PairT::BUFFERS;
     __shared__ typename PairT::Lds lds;
     __shared__ BiasLds table;
+    __shared__ __attribute__((aligned(16))) float mask_of[BUFFERS][BN];
     __shared__ float near_bias[BUFFERS][BIAS ? ROWS + BN : 1], sums[BIAS ? NW : 1][QLKA_MAX_BUCKETS];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
@@ -104,11 +102,10 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
         t1 = min(t1, last < 0 ? 0 : last / BN + 1);
     }
     KeyBits<BN> seen(p, b);
-    PairT tile(p.sk.r, p.vec & VEC_K, p.sv.r, p.vec & VEC_V, p.D, tid);
+    PairT tile(lds, p.sk.r, p.sv.r, p.D, tid);
     const auto fetch = [&](int t, int buffer) {
-        tile.fetch(lds, buffer, k + (int64_t)t * BN * p.sk.r, v + (int64_t)t * BN * p.sv.r, seen.of(t), tid);
+        tile.fetch(lds, buffer, k + (int64_t)t * BN * p.sk.r, v + (int64_t)t * BN * p.sv.r, seen.of(t), p.D, tid);
     };
-    if (p.keep || p.N % BN || p.D < DP) PairT::clear(lds, tid);
     int t = seen.next(t0, t1), buffer = 0;
     if (t < t1) fetch(t, 0);
 
@@ -120,10 +117,10 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
         typename Elem<T>::seg s = {}, g = {};
         f32x8 o = {};
         if (m < p.M) {
-            s = load_seg((const T*)p.q + b * p.sq.b + head * p.sq.h + m * p.sq.r, d, p.D, p.vec & VEC_Q);
-            g = load_seg((const T*)p.g_out + b * p.sg.b + head * p.sg.h + m * p.sg.r, d, p.D, p.vec & VEC_G);
-            o = p.out_full ? load_seg(p.out_full + row * p.D, d, p.D, p.vec & VEC_FULL)
-                           : floats(load_seg((const T*)p.out + b * p.so.b + head * p.so.h + m * p.so.r, d, p.D, p.vec & VEC_O));
+            s = load_seg((const T*)p.q + b * p.sq.b + head * p.sq.h + m * p.sq.r, d, p.D);
+            g = load_seg((const T*)p.g_out + b * p.sg.b + head * p.sg.h + m * p.sg.r, d, p.D);
+            o = p.out_full ? load_seg(p.out_full + row * p.D, d, p.D)
+                           : floats(load_seg((const T*)p.out + b * p.so.b + head * p.so.h + m * p.so.r, d, p.D));
         }
         s = s * (T)p.q_sign;
         qf[c] = frag_of(s);
@@ -151,8 +148,9 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
         const uint64_t bits = seen.of(t);
         float far = 0.f;
         int fb = -1;
-        float* near_here = near_bias[buffer];
+        float *near_here = near_bias[buffer], *mask = mask_of[buffer];
         tile.arrive(lds, tid, [&] {
+            if (bits != PairT::ALL) put_mask<BN>(mask, bits, tid);
             if constexpr (BIAS) {
                 const int lo = n0 - (m0 + ROWS - 1) - p.start;
                 fb = far_bucket(p.bk, lo, n0 + BN - 1 - m0 - p.start);
@@ -172,9 +170,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
         if (mw >= p.M || (p.causal && n0 > mw + 31 + p.start)) continue;
 
         const bool edge = p.causal && n0 + BN - 1 > mw + p.start;
-        const bool all = bits == PairT::ALL && !edge;
-        const uint64_t mine = bits >> (4 * half);
-        const int lim = edge ? m + p.start - n0 - 4 * half : BN;
+        const int lim = m + p.start - n0 - 4 * half;                     // at an edge, the last key seen
         const float* nb = &near_here[BIAS ? ROWS - 1 - wave * 32 - col + 4 * half : 0];
         const float add = far - lse;
         // `count` halves of the tile together: the products of one are under way while the other's scores are worked on
@@ -207,12 +203,13 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c2, add);
                 }
+                if (bits != PairT::ALL) s[i] += rows_of(mask, 32 * (first + i) + 4 * half);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[i][r] = fexp2(s[i][r]) * (dp[i][r] - delta);
-                if (!all) {
+                if (edge) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
-                        if (!(mine >> (32 * (first + i) + reg_row(r)) & 1) || 32 * (first + i) + reg_row(r) > lim) s[i][r] = 0.f;
+                        if (32 * (first + i) + reg_row(r) > lim) s[i][r] = 0.f;
                 }
                 if (to_table) {
                     if (fb < 0) {
@@ -268,7 +265,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
             if (p.splits > 1)
                 *reinterpret_cast<f32x4*>(p.part + ((int64_t)split_i * p.B * p.H * p.M + row) * DP + at) = x;
             else
-                store4((T*)p.g_q + b * p.sgq.b + head * p.sgq.h + m * p.sgq.r, at, p.D, p.vec & VEC_GQ, x * f);
+                store4((T*)p.g_q + b * p.sgq.b + head * p.sgq.h + m * p.sgq.r, at, p.D, x * f);
         }
 }
 
@@ -299,12 +296,13 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
             while (t < t1 && t % tiles * BM + BM - 1 + p.start < n0) ++t;
         return t;
     };
-    PairT tile(p.sq.r, p.vec & VEC_Q, p.sg.r, p.vec & VEC_G, p.D, tid);
+    PairT tile(lds, p.sq.r, p.sg.r, p.D, tid);
     float ls = HIGH, des = 0.f;
     const auto fetch = [&](int t, int buffer) {
         const int head = kvh * share + t / tiles, m0 = t % tiles * BM, left = p.M - m0;
         tile.fetch(lds, buffer, (const T*)p.q + b * p.sq.b + head * p.sq.h + m0 * p.sq.r,
-                   (const T*)p.g_out + b * p.sg.b + head * p.sg.h + m0 * p.sg.r, left >= BM ? PairT::ALL : (1ull << left) - 1, tid);
+                   (const T*)p.g_out + b * p.sg.b + head * p.sg.h + m0 * p.sg.r, left >= BM ? PairT::ALL : (1ull << left) - 1, p.D,
+                   tid);
         ls = HIGH;
         des = 0.f;
         if (tid < BM && tid < left) {
@@ -313,7 +311,6 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
             des = p.delta[row];
         }
     };
-    if (p.M % BM || p.D < DP) PairT::clear(lds, tid);
     int t = next((int)(work * split_i / p.splits)), buffer = 0;
     if (t < t1) fetch(t, 0);
     Frag<NP> kf[DP / 16], vf[DP / 16];
@@ -321,8 +318,8 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
     for (int c = 0; c < DP / 16; ++c) {
         typename Elem<T>::seg s = {}, x = {};
         if (shown) {
-            s = load_seg((const T*)p.k + b * p.sk.b + kvh * p.sk.h + n * p.sk.r, 16 * c + 8 * half, p.D, p.vec & VEC_K);
-            x = load_seg((const T*)p.v + b * p.sv.b + kvh * p.sv.h + n * p.sv.r, 16 * c + 8 * half, p.D, p.vec & VEC_V);
+            s = load_seg((const T*)p.k + b * p.sk.b + kvh * p.sk.h + n * p.sk.r, 16 * c + 8 * half, p.D);
+            x = load_seg((const T*)p.v + b * p.sv.b + kvh * p.sv.h + n * p.sv.r, 16 * c + 8 * half, p.D);
         }
         s = s * (T)p.q_sign;
         kf[c] = frag_of(s);
@@ -449,15 +446,15 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
                 *reinterpret_cast<f32x4*>(p.part + (split_i * all + row) * DP + at) = x;
                 *reinterpret_cast<f32x4*>(p.part2 + (split_i * all + row) * DP + at) = y;
             } else {
-                store4((T*)p.g_k + b * p.sgk.b + kvh * p.sgk.h + n * p.sgk.r, at, p.D, p.vec & VEC_GK, x * f);
-                store4((T*)p.g_v + b * p.sgv.b + kvh * p.sgv.h + n * p.sgv.r, at, p.D, p.vec & VEC_GV, y);
+                store4((T*)p.g_k + b * p.sgk.b + kvh * p.sgk.h + n * p.sgk.r, at, p.D, x * f);
+                store4((T*)p.g_v + b * p.sgv.b + kvh * p.sgv.h + n * p.sgv.r, at, p.D, y);
             }
         }
 }
 
 // Sum of the splits' partial rows: DP / 4 lanes a row.
 template <class T, int DP>
-__global__ __launch_bounds__(256) void softmax_sum(const float* part, T* out, SmStrides so, bool vec, float scale,
+__global__ __launch_bounds__(256) void softmax_sum(const float* part, T* out, SmStrides so, float scale,
                                                    int splits, int64_t rows, int heads, int len, int D) {
     constexpr int LANES = DP / 4;
     const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES;
@@ -466,7 +463,7 @@ __global__ __launch_bounds__(256) void softmax_sum(const float* part, T* out, Sm
     f32x4 x = {};
     for (int s = 0; s < splits; ++s) x = x + *reinterpret_cast<const f32x4*>(part + (s * rows + row) * DP + d);
     const int i = (int)(row % len), h = (int)(row / len % heads), b = (int)(row / len / heads);
-    store4(out + b * so.b + h * so.h + i * so.r, d, D, vec, x * scale);
+    store4(out + b * so.b + h * so.h + i * so.r, d, D, x * scale);
 }
 
 // One workgroup for each (head, bucket).
@@ -499,10 +496,10 @@ template <class T, int DP, int NW> int run_dkv(const SmParams& p, hipStream_t st
     else softmax_dkv<T, DP, NW, false><<<grid, 64 * NW, 0, st>>>(p);
     return (int)hipGetLastError();
 }
-template <class T, int DP> int run_sum(const float* part, void* out, SmStrides so, bool vec, float scale, int splits, int B,
+template <class T, int DP> int run_sum(const float* part, void* out, SmStrides so, float scale, int splits, int B,
                                        int heads, int len, int D, hipStream_t st) {
     const int64_t rows = (int64_t)B * heads * len, threads = rows * (DP / 4);
-    softmax_sum<T, DP><<<dim3((unsigned)((threads + 255) / 256)), 256, 0, st>>>(part, (T*)out, so, vec, scale, splits, rows,
+    softmax_sum<T, DP><<<dim3((unsigned)((threads + 255) / 256)), 256, 0, st>>>(part, (T*)out, so, scale, splits, rows,
                                                                                heads, len, D);
     return (int)hipGetLastError();
 }
@@ -525,10 +522,10 @@ int sm_dkv(int dtype, const SmParams& p, int waves, hipStream_t st) {
              : waves == 2 ? sm::run_dkv<decltype(t), dp.value, 2>(p, st) : sm::run_dkv<decltype(t), dp.value, 4>(p, st); });
 }
 
-int sm_sum_parts(int dtype, const float* part, void* out, SmStrides so, bool vec, float scale, int splits, int B, int heads,
+int sm_sum_parts(int dtype, const float* part, void* out, SmStrides so, float scale, int splits, int B, int heads,
                  int len, int D, hipStream_t st) {
     return sm::dispatch(dtype, D, [&](auto t, auto dp) {
-        return sm::run_sum<decltype(t), dp.value>(part, out, so, vec, scale, splits, B, heads, len, D, st); });
+        return sm::run_sum<decltype(t), dp.value>(part, out, so, scale, splits, B, heads, len, D, st); });
 }
 
 int sm_sum_table(const float* part, float* g_table, int H, int count, int buckets, hipStream_t st) {

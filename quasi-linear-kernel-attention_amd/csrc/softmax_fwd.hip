@@ -30,6 +30,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
     __shared__ typename PairT::Lds lds;
     __shared__ BiasLds table;
     __shared__ float near_bias[BUFFERS][BIAS ? ROWS + BN : 1];
+    __shared__ __attribute__((aligned(16))) float mask_of[BUFFERS][BN];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
     const Work w = xcd_work(blockIdx.x, p.B * p.H, p.blocks * p.splits);
@@ -47,11 +48,10 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
         t1 = min(t1, last < 0 ? 0 : last / BN + 1);
     }
     KeyBits<BN> seen(p, b);
-    PairT tile(p.sk.r, p.vec & VEC_K, p.sv.r, p.vec & VEC_V, p.D, tid);
+    PairT tile(lds, p.sk.r, p.sv.r, p.D, tid);
     const auto fetch = [&](int t, int buffer) {
-        tile.fetch(lds, buffer, k + (int64_t)t * BN * p.sk.r, v + (int64_t)t * BN * p.sv.r, seen.of(t), tid);
+        tile.fetch(lds, buffer, k + (int64_t)t * BN * p.sk.r, v + (int64_t)t * BN * p.sv.r, seen.of(t), p.D, tid);
     };
-    if (p.keep || p.N % BN || p.D < DP) PairT::clear(lds, tid);
     int t = seen.next(t0, t1), buffer = 0;
     if (t < t1) fetch(t, 0);
 
@@ -59,7 +59,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
         typename Elem<T>::seg s = {};
-        if (m < p.M) s = load_seg(q + m * p.sq.r, 16 * c + 8 * half, p.D, p.vec & VEC_Q);
+        if (m < p.M) s = load_seg(q + m * p.sq.r, 16 * c + 8 * half, p.D);
         s = s * (T)p.q_sign;
         qf[c] = frag_of(s);
     }
@@ -77,8 +77,9 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
         const uint64_t bits = seen.of(t);
         float far = 0.f;
         bool near = false;
-        float* near_here = near_bias[buffer];
+        float *near_here = near_bias[buffer], *mask = mask_of[buffer];
         tile.arrive(lds, tid, [&] {
+            if (bits != PairT::ALL) put_mask<BN>(mask, bits, tid);
             if constexpr (BIAS) {
                 const int lo = n0 - (m0 + ROWS - 1) - p.start;
                 const int fb = far_bucket(p.bk, lo, n0 + BN - 1 - m0 - p.start);
@@ -101,8 +102,6 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
         f32x16 s[NS];
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            s[i] = f32x16{};
-            if (!(uint32_t)(bits >> (32 * i))) continue;               // no key among these 32
             Acc<NP> a;
             a.start();
             __builtin_amdgcn_s_setprio(1);
@@ -115,21 +114,32 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
 
         // scores in log2 units are fma(s, mul, add) from here on
         float mul = c2, add = far;
-        const bool edge = p.causal && n0 + BN - 1 > mw + p.start;
-        const bool all = bits == PairT::ALL && !edge;
-        if (near || !all) {
-            const uint64_t mine = bits >> (4 * half);
-            const int lim = edge ? m + p.start - n0 - 4 * half : BN;     // the last key seen
+        const bool edge = p.causal && n0 + BN - 1 > mw + p.start, all = bits == PairT::ALL;
+        if (near || edge || !all) {
             const float* nb = &near_here[BIAS ? ROWS - 1 - wave * 32 - col + 4 * half : 0];
+            if (BIAS && near) {
 #pragma unroll
-            for (int i = 0; i < NS; ++i)
+                for (int i = 0; i < NS; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int n = 32 * i + reg_row(r);
-                    float x = __builtin_fmaf(s[i][r], c2, BIAS && near ? nb[n] : far);
-                    if (!all && !((mine >> n & 1) && n <= lim)) x = -std::numeric_limits<float>::infinity();
-                    s[i][r] = x;
-                }
+                    for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c2, nb[32 * i + reg_row(r)]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < NS; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c2, far);
+            }
+            if (!all) {
+#pragma unroll
+                for (int i = 0; i < NS; ++i) s[i] += rows_of(mask, 32 * i + 4 * half);
+            }
+            if (edge) {
+                const int lim = m + p.start - n0 - 4 * half;             // the last key seen
+#pragma unroll
+                for (int i = 0; i < NS; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (32 * i + reg_row(r) > lim) s[i][r] = -std::numeric_limits<float>::infinity();
+            }
             mul = 1.f;
             add = 0.f;
         }
@@ -155,7 +165,6 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
         for (int d = 0; d < ND; ++d) o[d].start();
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            if (!(uint32_t)(bits >> (32 * i))) continue;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 f32x8 e = eight(s[i], c);
@@ -205,8 +214,8 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const f32x4 x = quad(o[d].main, r) * inv;
-            store4(out, 32 * d + 8 * r + 4 * half, p.D, p.vec & VEC_O, x);
-            if constexpr (FINE) store4(p.out_full + row * p.D, 32 * d + 8 * r + 4 * half, p.D, p.vec & VEC_FULL, x);
+            store4(out, 32 * d + 8 * r + 4 * half, p.D, x);
+            if constexpr (FINE) store4(p.out_full + row * p.D, 32 * d + 8 * r + 4 * half, p.D, x);
         }
     if (p.lse && half == 0)
         p.lse[row] = sum == 0.f ? std::numeric_limits<float>::infinity() : ref + __log2f(sum);
@@ -265,8 +274,8 @@ __global__ __launch_bounds__(64 * COMBINE_ROWS) void softmax_combine(const SmPar
     x = x * (sum == 0.f ? 0.f : 1.f / sum);
     if (first) return;
     const int m = (int)(row % p.M), head = (int)(row / p.M % p.H), b = (int)(row / p.M / p.H);
-    store4((T*)p.out + b * p.so.b + head * p.so.h + m * p.so.r, d, p.D, p.vec & VEC_O, x);
-    if (p.out_full) store4(p.out_full + row * p.D, d, p.D, p.vec & VEC_FULL, x);
+    store4((T*)p.out + b * p.so.b + head * p.so.h + m * p.so.r, d, p.D, x);
+    if (p.out_full) store4(p.out_full + row * p.D, d, p.D, x);
     if (p.lse && d == 0) p.lse[row] = sum == 0.f ? std::numeric_limits<float>::infinity() : ref + __log2f(sum);
 }
 

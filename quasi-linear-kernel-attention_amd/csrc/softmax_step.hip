@@ -43,7 +43,6 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p
     const int kvh = w % p.G, b = w / p.G, share = p.H / p.G, rows = share * p.M;
     const T* k = (const T*)p.k + b * p.sk.b + kvh * p.sk.h;
     const T* v = (const T*)p.v + b * p.sv.b + kvh * p.sv.h;
-    const bool vk = p.vec & VEC_K, vv = p.vec & VEC_V;
 
     f32x8 q[R], o[R];
     float top[R], sum[R];
@@ -55,7 +54,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p
         sum[r] = 0.f;
         if (r < rows) {
             const int head = kvh * share + r / p.M, m = r % p.M;
-            q[r] = floats(load_seg((const T*)p.q + b * p.sq.b + head * p.sq.h + m * p.sq.r, d, p.D, p.vec & VEC_Q)) *
+            q[r] = floats(load_seg((const T*)p.q + b * p.sq.b + head * p.sq.h + m * p.sq.r, d, p.D)) *
                    (p.q_sign * p.scale * LOG2E);
             if constexpr (BIAS)
                 for (int i = tid; i < (p.bk.n + 1) * (p.bk.both ? 2 : 1); i += NT)
@@ -96,12 +95,12 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p
                 const int n = u0 + u * KEYS + group;
                 in[u] = bits >> n & 1;
                 ks[u] = {};
-                if (in[u]) ks[u] = load_seg(k + (n0 + n) * p.sk.r, d, p.D, vk);
+                if (in[u]) ks[u] = load_seg(k + (n0 + n) * p.sk.r, d, p.D);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 vs[u] = {};
-                if (in[u]) vs[u] = load_seg(v + (n0 + u0 + u * KEYS + group) * p.sv.r, d, p.D, vv);
+                if (in[u]) vs[u] = load_seg(v + (n0 + u0 + u * KEYS + group) * p.sv.r, d, p.D);
             }
             float x[R][U];
 #pragma unroll

@@ -113,16 +113,10 @@ __device__ __forceinline__ float fexp2(float x) { return __builtin_amdgcn_exp2f(
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
 __device__ __forceinline__ int reg_row(int r) { return (r >> 2) * 8 + (r & 3); }   // + 4 (lane / 32)
 
-// Eight elements d .. d + 7 of a row of D; zeros past D. vec: the row is 16-byte aligned and D a multiple of 8.
-template <class T> __device__ __forceinline__ typename Elem<T>::seg load_seg(const T* row, int d, int D, bool vec) {
+// Eight elements d .. d + 7 of a row of D, a multiple of 8; zeros past D.
+template <class T> __device__ __forceinline__ typename Elem<T>::seg load_seg(const T* row, int d, int D) {
     typename Elem<T>::seg x = {};
-    if (vec) {
-        if (d < D) x = *reinterpret_cast<const typename Elem<T>::seg*>(row + d);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (d + i < D) x[i] = row[d + i];
-    }
+    if (d < D) x = *reinterpret_cast<const typename Elem<T>::seg*>(row + d);
     return x;
 }
 
@@ -194,9 +188,8 @@ __device__ __forceinline__ void load_to_lds(const void* from, uint32_t bytes, ui
 //
 // bf16 goes there directly (global_load_lds, 16 bytes a lane, 1 KB an instruction; the pieces are turned by reading from turned
 // places), into the other one of two buffers while the current one is read: no registers hold a tile, and one barrier a tile is
-// enough. Rows that are not to be read, and pieces past D, are left out: they hold zeros, or a row of an earlier tile, whose
-// products are multiplied by a probability of zero. float goes through registers, where it is split into parts, and
-// has one buffer and two barriers.
+// enough. float goes through registers, where it is split into parts, and has one buffer and two barriers. Rows that are not
+// to be read become zeros.
 template <class T, int DP, int ROWS, int NW> struct Pair {
     static constexpr int NP = Elem<T>::PARTS, NT = 64 * NW, PIECES = DP / 8, BUFFERS = NP == 1 ? 2 : 1;
     static constexpr uint64_t ALL = ROWS == 64 ? ~0ull : (1ull << ROWS % 64) - 1;
@@ -210,51 +203,70 @@ template <class T, int DP, int ROWS, int NW> struct Pair {
     static constexpr bool ALIKE = APART % 8 == 0 || EACH == 1;       // they are turned alike
 
     int64_t stride_a, stride_b;
-    int D;
-    bool vec_a, vec_b, whole;
+    bool near, has;                        // rows within 32 bits of their tile; this lane's piece is not past D
     uint32_t at_a, at_b;                   // bytes from a tile's first row to this lane's piece
     typename Elem<T>::seg a[HELD], b[HELD];
 
-    __device__ __forceinline__ Pair(int64_t stride_a, bool vec_a, int64_t stride_b, bool vec_b, int D, int tid)
-        : stride_a(stride_a), stride_b(stride_b), D(D), vec_a(vec_a), vec_b(vec_b) {
-        whole = vec_a && vec_b && D == DP && stride_a < 1 << 22 && stride_b < 1 << 22 && (NP != 1 || ALIKE);
+    __device__ __forceinline__ Pair(Lds& lds, int64_t stride_a, int64_t stride_b, int D, int tid)
+        : stride_a(stride_a), stride_b(stride_b) {
+        near = stride_a < 1 << 22 && stride_b < 1 << 22 && (NP != 1 || ALIKE);
         int row = tid / PIECES, piece = tid % PIECES;
         if constexpr (NP == 1) piece ^= TileT::turn(row);
+        has = piece * 8 < D;
         at_a = (uint32_t)(row * stride_a + piece * 8) * sizeof(T);
         at_b = (uint32_t)(row * stride_b + piece * 8) * sizeof(T);
-    }
-    // before the first tile, when some rows or pieces will be left out
-    __device__ __forceinline__ static void clear(Lds& lds, int tid) {
-        if constexpr (NP == 1) {
+        if (NP == 1 && D < DP) {           // pieces past D stay as they are
             bf16x8* x = reinterpret_cast<bf16x8*>(&lds);
             for (int i = tid; i < (int)(sizeof(Lds) / 16); i += NT) x[i] = bf16x8{};
             __syncthreads();
         }
     }
     // tile_a, tile_b: first rows; bits: the rows to read
-    __device__ __forceinline__ void fetch(Lds& lds, int buffer, const T* tile_a, const T* tile_b, uint64_t bits, int tid) {
-        if (whole && bits == ALL) {                        // without any test
+    __device__ __forceinline__ void fetch(Lds& lds, int buffer, const T* tile_a, const T* tile_b, uint64_t bits, int D, int tid) {
+        if (near && bits == ALL) {                         // without a test for each row
             if constexpr (NP == 1) {
                 const uint32_t to_a = lds_place(&lds.a[buffer].x[(tid >> 6) * RPI * DP]);
                 const uint32_t to_b = lds_place(&lds.b[buffer].x[(tid >> 6) * RPI * DP]);
+                if (has) {
 #pragma unroll
-                for (int j = 0; j < EACH; ++j) load_to_lds(tile_a + j * APART * stride_a, at_a, to_a + j * APART * DP * 2);
+                    for (int j = 0; j < EACH; ++j) load_to_lds(tile_a + j * APART * stride_a, at_a, to_a + j * APART * DP * 2);
 #pragma unroll
-                for (int j = 0; j < EACH; ++j) load_to_lds(tile_b + j * APART * stride_b, at_b, to_b + j * APART * DP * 2);
+                    for (int j = 0; j < EACH; ++j) load_to_lds(tile_b + j * APART * stride_b, at_b, to_b + j * APART * DP * 2);
+                }
             } else {
                 typedef const typename Elem<T>::seg* segs;
 #pragma unroll
                 for (int i = 0; i < HELD; ++i) {
+                    a[i] = b[i] = {};
+                    if (!has) continue;
                     a[i] = *(segs)((const char*)(tile_a + i * STEP * stride_a) + at_a);
                     b[i] = *(segs)((const char*)(tile_b + i * STEP * stride_b) + at_b);
                 }
             }
         } else if constexpr (NP == 1) {
-            direct(lds.a[buffer], tile_a, stride_a, vec_a, bits, tid);
-            direct(lds.b[buffer], tile_b, stride_b, vec_b, bits, tid);
+#pragma unroll 1
+            for (int j = 0; j < EACH; ++j) {
+                const int first = (tid >> 6) * RPI + j * APART, row = first + (tid & 63) / PIECES;
+                const int slot = tid % PIECES, piece = slot ^ TileT::turn(row);
+                const uint32_t to_a = lds_place(&lds.a[buffer].x[first * DP]), to_b = lds_place(&lds.b[buffer].x[first * DP]);
+                if (piece * 8 >= D) continue;
+                if (bits >> row & 1) {
+                    load_to_lds(tile_a + row * stride_a + piece * 8, to_a);
+                    load_to_lds(tile_b + row * stride_b + piece * 8, to_b);
+                } else {
+                    *reinterpret_cast<bf16x8*>(&lds.a[buffer].x[row * DP + slot * 8]) = bf16x8{};
+                    *reinterpret_cast<bf16x8*>(&lds.b[buffer].x[row * DP + slot * 8]) = bf16x8{};
+                }
+            }
         } else {
-            hold(a, tile_a, stride_a, vec_a, bits, tid);
-            hold(b, tile_b, stride_b, vec_b, bits, tid);
+            const int row = tid / PIECES, d = tid % PIECES * 8;
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) {
+                a[i] = b[i] = {};
+                if (!has || !(bits >> (row + i * STEP) & 1)) continue;
+                a[i] = load_seg(tile_a + (row + i * STEP) * stride_a, d, D);
+                b[i] = load_seg(tile_b + (row + i * STEP) * stride_b, d, D);
+            }
         }
     }
     // until here the fetched tile has arrived and nobody reads the buffer that the next fetch goes to; between two calls of it
@@ -275,28 +287,6 @@ template <class T, int DP, int ROWS, int NW> struct Pair {
             __syncthreads();
         }
     }
-
-private:
-    __device__ __forceinline__ void direct(TileT& t, const T* from, int64_t stride, bool vec, uint64_t bits, int tid) {
-        const int lane = tid & 63;
-#pragma unroll
-        for (int j = 0; j < EACH; ++j) {
-            const int first = (tid >> 6) * RPI + j * APART, row = first + lane / PIECES;
-            const int piece = lane % PIECES ^ TileT::turn(row);
-            const uint32_t to = lds_place(&t.x[first * DP]);
-            if (!(bits >> row & 1) || piece * 8 >= D) continue;
-            if (vec) load_to_lds(from + row * stride + piece * 8, to);
-            else *reinterpret_cast<bf16x8*>(&t.x[row * DP + lane % PIECES * 8]) = load_seg(from + row * stride, piece * 8, D, false);
-        }
-    }
-    __device__ __forceinline__ void hold(typename Elem<T>::seg* s, const T* from, int64_t stride, bool vec, uint64_t bits, int tid) {
-        const int row = tid / PIECES, d = tid % PIECES * 8;
-#pragma unroll
-        for (int i = 0; i < HELD; ++i) {
-            s[i] = {};
-            if (bits >> (row + i * STEP) & 1) s[i] = load_seg(from + (row + i * STEP) * stride, d, D, vec);
-        }
-    }
 };
 
 // 4 bytes' truth as 4 bits
@@ -314,33 +304,28 @@ __device__ __forceinline__ uint64_t lane_u64(uint64_t x, int lane) {
 template <int BN> struct KeyBits {
     const uint8_t* keep;       // the batch's row, or null
     int N, window;
-    bool vec;
     uint64_t bits;             // of tile 64 * window + lane
 
     __device__ __forceinline__ KeyBits(const SmParams& p, int b)
-        : keep(p.keep ? p.keep + b * p.keep_stride : nullptr), N(p.N), window(-1), vec(p.vec & VEC_KEEP), bits(0) {}
+        : keep(p.keep ? p.keep + b * p.keep_stride : nullptr), N(p.N), window(-1), bits(0) {}
 
     __device__ __forceinline__ void look(int w) {
         if (w == window) return;
         window = w;
-        const int64_t n0 = ((int64_t)w * 64 + (threadIdx.x & 63)) * BN;
-        const int64_t left = N - n0;
-        bits = left <= 0 ? 0 : left >= 64 ? ~0ull : (1ull << left) - 1;
-        if (BN < 64) bits &= (1ull << BN) - 1;
-        if (!keep || left <= 0) return;
-        uint64_t seen = 0;
-        if (vec && left >= BN) {
-#pragma unroll
-            for (int j = 0; j < BN / 16; ++j) {
-                const uint4 w4 = *reinterpret_cast<const uint4*>(keep + n0 + 16 * j);
-                const uint64_t t = truth4(w4.x) | truth4(w4.y) << 4 | truth4(w4.z) << 8 | truth4(w4.w) << 12;
-                seen |= t << (16 * j);
+        const int64_t n0 = ((int64_t)w * 64 + (threadIdx.x & 63)) * BN, left = N - n0;
+        bits = 0;
+#pragma unroll 1
+        for (int j = 0; j < BN && j < left; j += 16) {
+            uint64_t t = 0;
+            if (left - j >= 16) {
+                typedef uint32_t u32x4 __attribute__((ext_vector_type(4), aligned(1)));
+                const u32x4 x = *reinterpret_cast<const u32x4*>(keep + n0 + j);
+                t = truth4(x.x) | truth4(x.y) << 4 | truth4(x.z) << 8 | truth4(x.w) << 12;
+            } else {
+                for (int i = 0; i < left - j; ++i) t |= (uint64_t)(keep[n0 + j + i] != 0) << i;
             }
-        } else {
-            const int n = left < BN ? (int)left : BN;
-            for (int j = 0; j < n; ++j) seen |= (uint64_t)(keep[n0 + j] != 0) << j;
+            bits |= t << j;
         }
-        bits &= seen;
     }
     __device__ __forceinline__ uint64_t of(int t) {
         if (!keep) {
@@ -373,6 +358,11 @@ struct BiasLds {
         for (int i = tid; i < p.bk.n; i += nt) border[i] = p.bk.border[i];
     }
 };
+
+// The masked keys of a tile as scores to add: 0 or -inf for each.
+template <int BN> __device__ __forceinline__ void put_mask(float* mask, uint64_t bits, int tid) {
+    if (tid < BN) mask[tid] = bits >> tid & 1 ? 0.f : -__builtin_inff();
+}
 
 // number of borders <= dist
 __device__ __forceinline__ int count_borders(const int* border, int n, int dist) {
@@ -416,18 +406,11 @@ template <class F> int dispatch(int dtype, int D, F f) {
     return dtype == QLKA_BF16 ? at(__bf16()) : at(float());
 }
 
-// Stores four successive elements d .. d + 3 of a row.
-template <class T> __device__ __forceinline__ void store4(T* row, int d, int D, bool vec, f32x4 x) {
-    if (vec) {
-        if (d < D) {
-            if constexpr (sizeof(T) == 2) *reinterpret_cast<bf16x4*>(row + d) = __builtin_convertvector(x, bf16x4);
-            else *reinterpret_cast<f32x4*>(row + d) = x;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (d + i < D) row[d + i] = (T)x[i];
-    }
+// Stores four successive elements d .. d + 3 of a row of D.
+template <class T> __device__ __forceinline__ void store4(T* row, int d, int D, f32x4 x) {
+    if (d >= D) return;
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<bf16x4*>(row + d) = __builtin_convertvector(x, bf16x4);
+    else *reinterpret_cast<f32x4*>(row + d) = x;
 }
 
 }  // namespace sm

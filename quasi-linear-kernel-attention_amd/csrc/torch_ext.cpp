@@ -412,12 +412,21 @@ void check_softmax(const SoftmaxCall& c) {
     }
 }
 
-// rows whose elements are next to each other
-Tensor packed_rows(const Tensor& t) { return t.size(3) == 1 || t.stride(3) == 1 ? t : t.contiguous(); }
+// whether the kernels can read t's rows: their elements next to each other, each row at a multiple of 16 bytes
+bool readable(const Tensor& t) {
+    const int64_t piece = 16 / t.element_size();
+    if (t.stride(3) != 1 || (uintptr_t)t.data_ptr() % 16) return false;
+    for (int i = 0; i < 3; ++i)
+        if (t.size(i) > 1 && t.stride(i) % piece) return false;
+    return true;
+}
+Tensor packed_rows(const Tensor& t) {
+    return t.numel() == 0 || readable(t) ? t : t.clone(at::MemoryFormat::Contiguous);
+}
 // an output laid out as t is
 Tensor empty_rows(const Tensor& t) {
     Tensor r = at::empty_like(t);
-    return t.size(3) == 1 || r.stride(3) == 1 ? r : at::empty(t.sizes(), t.options());
+    return r.numel() == 0 || readable(r) ? r : at::empty(t.sizes(), t.options());
 }
 void set_strides(int64_t* to, const Tensor& t) {
     for (int i = 0; i < 3; ++i) to[i] = t.stride(i);
@@ -539,6 +548,12 @@ struct SoftmaxFn : public torch::autograd::Function<SoftmaxFn> {
 
 Tensor softmax_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& table, const OptTensor& keep,
                          double scale, bool causal, int64_t start, const std::vector<int64_t>& border, bool both) {
+    if (q.dim() == 4 && k.dim() == 4 && v.dim() == 4 && q.size(3) % 8 && q.size(3) == k.size(3) && q.size(3) == v.size(3)) {
+        // zeros up to a multiple of 8 change no product
+        const auto padded = [&](const Tensor& t) { return at::constant_pad_nd(t, {0, 8 - t.size(3) % 8}); };
+        return softmax_attention(padded(q), padded(k), padded(v), table, keep, scale, causal, start, border, both)
+            .narrow(3, 0, q.size(3));
+    }
     const Tensor t = table.value_or(Tensor()), m = keep.value_or(Tensor());
     if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() ||
                                        (t.defined() && t.requires_grad())))
