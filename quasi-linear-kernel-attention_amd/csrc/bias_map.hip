@@ -53,7 +53,9 @@ __global__ __launch_bounds__(MAP_T) void map_bwd(const float* g, const SmBuckets
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[3 + j - i] += y[j];
     };
-    if (first >= 0 && first + MAP_COLS + rows <= N && rows % 4 == 0) {
+    // a wave inside the map; one at an edge, or past it
+    const int lo = first + 256 * wave, hi = lo + 255 + rows - 1;                   // its columns
+    if (lo >= 0 && hi < N && rows % 4 == 0) {
 #pragma unroll 4
         for (int r = 0; r < rows; r += 4) {
             f32x4u y[4];
@@ -62,8 +64,8 @@ __global__ __launch_bounds__(MAP_T) void map_bwd(const float* g, const SmBuckets
 #pragma unroll
             for (int i = 0; i < 4; ++i) add(y[i], i);
         }
-    } else {
-        // at an edge every thread loads, from the nearest value where it has none, so that the loads stay under way together
+    } else if (hi >= 0 && lo < N) {
+        // every lane loads, from the nearest value where it has none, so that the loads stay under way together
 #pragma unroll 2
         for (int r = 0; r < rows; r += 4)
 #pragma unroll

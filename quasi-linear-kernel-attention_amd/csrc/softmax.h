@@ -52,7 +52,9 @@ constexpr int sm_tile_rows(int parts, int DP) { return DP == 128 || (parts == 3 
 inline int sm_buckets(const SmBuckets& b) { return (b.n + 1) * (b.both ? 2 : 1); }
 
 // Launchers; each returns a hipError_t value. The dtype is QLKA_F32 or QLKA_BF16.
-int sm_fwd(int dtype, const SmParams& p, int waves, hipStream_t st);
+constexpr int FWD_WAVES = 4;
+int sm_fwd(int dtype, const SmParams& p, hipStream_t st);
+// waves (of 32 rows) a workgroup: 2 or 4
 int sm_step(int dtype, const SmParams& p, hipStream_t st);
 int sm_combine(int dtype, const SmParams& p, hipStream_t st);
 int sm_delta(int dtype, const SmParams& p, hipStream_t st);

@@ -37,30 +37,38 @@ __global__ __launch_bounds__(256) void softmax_delta(const SmParams p) {
     if (row < rows && d == 0) p.delta[row] = x;
 }
 
+// y of a lane added to x where both lanes' buckets are the same: one step of a segmented scan over a wave (CTRL: a DPP
+// shift within 16 lanes, or the broadcast of a row's last lane to the next)
+template <int CTRL, int ROWS> __device__ __forceinline__ void scan_step(float& x, int bucket) {
+    const int c = __builtin_amdgcn_update_dpp(-1, bucket, CTRL, ROWS, 0xf, false);
+    const int y = __builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, ROWS, 0xf, false);
+    if (c == bucket) x += __int_as_float(y);
+}
+
 // Adds a wave's 32 x 32 scores' gradients to the buckets of their distances. A lane holds one query (lane % 32) and 16 keys;
 // for each register the values of 32 queries are turned in the wave until lane t holds the diagonal (key - query) = t or
 // t - 32, so a diagonal's sum gathers in one lane; lanes of one bucket, which are neighbours, are then summed by a segmented
-// scan. base: the distance of the tile's first key and first query. acc: this wave's own, in LDS.
-__device__ __forceinline__ void add_band(f32x16 ds, int base, float* acc, const int* border, const SmBuckets& bk, int lane) {
-    const int t = lane & 31, half = lane >> 5;
+// scan. buckets: those of the distances from the tile's first key and first query less 32 on. acc: this wave's own, in LDS.
+__device__ __forceinline__ void add_band(f32x16 ds, const uint8_t* buckets, float* acc, int lane) {
+    const int t = lane & 31, half = lane >> 5, from = 4 * (4 * half - t);
     float pos = 0.f, neg = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-        const int n = reg_row(r) + 4 * half, from = ((n - t) & 31) | (lane & 32);
-        const float x = __int_as_float(__builtin_amdgcn_ds_bpermute(4 * from, __float_as_int(ds[r])));
-        pos += t <= n ? x : 0.f;
-        neg += t <= n ? 0.f : x;
+        const int x = __builtin_amdgcn_ds_bpermute(((from + 4 * reg_row(r)) & 124) | (lane & 32) << 2, __float_as_int(ds[r]));
+        const bool after = t <= reg_row(r) + 4 * half;
+        pos += after ? __int_as_float(x) : 0.f;
+        neg += after ? 0.f : __int_as_float(x);
     }
     pos += other_half(pos);
     neg += other_half(neg);
     float x = half ? pos : neg;
-    const int bucket = bucket_of(border, bk.n, bk.both, base + lane - 32);
-#pragma unroll
-    for (int k = 1; k < 64; k *= 2) {
-        const float y = __shfl_up(x, k);
-        const int c = __shfl_up(bucket, k);
-        if (lane >= k && c == bucket) x += y;
-    }
+    const int bucket = buckets[lane];
+    scan_step<0x111, 0xf>(x, bucket);        // row_shr 1, 2, 4, 8
+    scan_step<0x112, 0xf>(x, bucket);
+    scan_step<0x114, 0xf>(x, bucket);
+    scan_step<0x118, 0xf>(x, bucket);
+    scan_step<0x142, 0xa>(x, bucket);        // row_bcast 15 into rows 1 and 3
+    scan_step<0x143, 0xc>(x, bucket);        // row_bcast 31 into rows 2 and 3
     const int after = __shfl_down(bucket, 1);
     if (lane == 63 || after != bucket) acc[bucket] += x;
 }
@@ -85,6 +93,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
     __shared__ BiasLds table;
     __shared__ __attribute__((aligned(16))) float mask_of[BUFFERS][BN];
     __shared__ float near_bias[BUFFERS][BIAS ? ROWS + BN : 1], sums[BIAS ? NW : 1][QLKA_MAX_BUCKETS];
+    __shared__ uint8_t near_bucket[BUFFERS][BIAS ? ROWS + BN : 1];        // from the distance before near_bias's first on
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
     const Work w = xcd_work(blockIdx.x, p.B * p.H, p.blocks * p.splits);
@@ -149,14 +158,18 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
         float far = 0.f;
         int fb = -1;
         float *near_here = near_bias[buffer], *mask = mask_of[buffer];
+        uint8_t* bucket_here = near_bucket[buffer];
         tile.arrive(lds, tid, [&] {
             if (bits != PairT::ALL) put_mask<BN>(mask, bits, tid);
             if constexpr (BIAS) {
                 const int lo = n0 - (m0 + ROWS - 1) - p.start;
                 fb = far_bucket(p.bk, lo, n0 + BN - 1 - m0 - p.start);
                 if (fb < 0) {
-                    for (int i = tid; i < ROWS + BN - 1; i += NT)
-                        near_here[i] = table.value[bucket_of(table.border, p.bk.n, p.bk.both, lo + i)];
+                    for (int i = tid; i < ROWS + BN; i += NT) {
+                        const int bucket = bucket_of(table.border, p.bk.n, p.bk.both, lo + i - 1);
+                        bucket_here[i] = (uint8_t)bucket;
+                        if (i) near_here[i - 1] = table.value[bucket];
+                    }
                 } else {
                     far = table.value[fb];
                 }
@@ -213,7 +226,9 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
                 }
                 if (to_table) {
                     if (fb < 0) {
-                        add_band(s[i], n0 + 32 * (first + i) - mw - p.start, sums[wave], table.border, p.bk, lane);
+                        // a half's first key and the wave's first query, less 32: 32 (first + i) + ROWS - 32 - 32 wave after lo - 1
+                        if ((uint32_t)(bits >> (32 * (first + i))))
+                            add_band(s[i], bucket_here + 32 * (first + i) + ROWS - 32 - 32 * wave, sums[wave], lane);
                     } else {
                         float a = 0.f;
 #pragma unroll
@@ -512,14 +527,12 @@ int sm_delta(int dtype, const SmParams& p, hipStream_t st) {
 
 int sm_dq(int dtype, const SmParams& p, int waves, hipStream_t st) {
     return sm::dispatch(dtype, p.D, [&](auto t, auto dp) {
-        return waves == 1 ? sm::run_dq<decltype(t), dp.value, 1>(p, st)
-             : waves == 2 ? sm::run_dq<decltype(t), dp.value, 2>(p, st) : sm::run_dq<decltype(t), dp.value, 4>(p, st); });
+        return waves == 2 ? sm::run_dq<decltype(t), dp.value, 2>(p, st) : sm::run_dq<decltype(t), dp.value, 4>(p, st); });
 }
 
 int sm_dkv(int dtype, const SmParams& p, int waves, hipStream_t st) {
     return sm::dispatch(dtype, p.D, [&](auto t, auto dp) {
-        return waves == 1 ? sm::run_dkv<decltype(t), dp.value, 1>(p, st)
-             : waves == 2 ? sm::run_dkv<decltype(t), dp.value, 2>(p, st) : sm::run_dkv<decltype(t), dp.value, 4>(p, st); });
+        return waves == 2 ? sm::run_dkv<decltype(t), dp.value, 2>(p, st) : sm::run_dkv<decltype(t), dp.value, 4>(p, st); });
 }
 
 int sm_sum_parts(int dtype, const float* part, void* out, SmStrides so, float scale, int splits, int B, int heads,

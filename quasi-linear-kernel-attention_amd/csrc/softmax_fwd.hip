@@ -287,10 +287,9 @@ template <class T, int DP> int launch_combine(const SmParams& p, hipStream_t st)
 
 }  // namespace sm
 
-int sm_fwd(int dtype, const SmParams& p, int waves, hipStream_t st) {
+int sm_fwd(int dtype, const SmParams& p, hipStream_t st) {
     return sm::dispatch(dtype, p.D, [&](auto t, auto dp) {
-        return waves == 1 ? sm::launch_fwd<decltype(t), dp.value, 1>(p, st)
-             : waves == 2 ? sm::launch_fwd<decltype(t), dp.value, 2>(p, st) : sm::launch_fwd<decltype(t), dp.value, 4>(p, st); });
+        return sm::launch_fwd<decltype(t), dp.value, FWD_WAVES>(p, st); });
 }
 
 int sm_combine(int dtype, const SmParams& p, hipStream_t st) {

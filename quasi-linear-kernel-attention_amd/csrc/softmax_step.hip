@@ -2,7 +2,7 @@
 // bound by reading k and v once.
 //
 // A key row is read by DP / 8 lanes of a wave, 8 elements each, so a wave reads 512 / DP keys with one 16-byte load a lane (two
-// for float) and keeps four such loads of k and four of v in flight. Scores are formed with fp32 multiply-adds and summed
+// for float) and keeps four such loads of k and four of v in flight, twice. Scores are formed with fp32 multiply-adds and summed
 // over a row's lanes by DPP; every group of lanes runs its own softmax over the keys that pass it, and the groups, then the
 // waves, are joined at the end. The keys are split over workgroups until the GPU is full (softmax_combine joins the
 // splits). A matrix tile would use one of its 32 rows here. Near the diagonal a lane finds the bias of one key of the tile for
@@ -72,72 +72,95 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p
     const int last = p.causal ? p.M - 1 + p.start : p.N - 1;          // the last key that any row sees
     t1 = min(t1, last < 0 ? 0 : last / 64 + 1);
     KeyBits<64> seen(p, b);
-    for (int t = t0 + wave; t < t1; t += NW) {
-        const int n0 = t * 64;
-        uint64_t bits = seen.of(t);
-        if (last - n0 < 63) bits &= (1ull << (last - n0 + 1)) - 1;
+    struct Place { int t, u0; uint64_t bits; };                       // a tile, the first key of U * KEYS of it, its keys
+    const auto next = [&](Place at) {                                 // the next U * KEYS keys of this wave with one to see
+        at.u0 += U * KEYS;
+        while (at.t < t1) {
+            while (at.u0 < 64) {
+                if (at.bits >> at.u0 & (U * KEYS == 64 ? ~0ull : (1ull << U * KEYS % 64) - 1)) return at;
+                at.u0 += U * KEYS;
+            }
+            at.t += NW;
+            at.u0 = 0;
+            if (at.t >= t1) break;
+            at.bits = seen.of(at.t);
+            if (last - at.t * 64 < 63) at.bits &= (1ull << (last - at.t * 64 + 1)) - 1;
+        }
+        return at;
+    };
+    // the keys of one place are on their way while those of the place before are worked on
+    struct Rows { typename Elem<T>::seg k[U], v[U]; };
+    const auto fetch = [&](Place at) {
+        Rows x;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int n = at.u0 + u * KEYS + group;
+            x.k[u] = {};
+            x.v[u] = {};
+            if (at.bits >> n & 1) {
+                x.k[u] = load_seg(k + (at.t * 64 + n) * p.sk.r, d, p.D);
+                x.v[u] = load_seg(v + (at.t * 64 + n) * p.sv.r, d, p.D);
+            }
+        }
+        return x;
+    };
+    Place at = next(Place{t0 + wave - NW, 64, 0});
+    Rows rows_here;
+    if (at.t < t1) rows_here = fetch(at);
+    int near_tile = -1;
+    while (at.t < t1) {
+        const Place after = next(at);
+        Rows rows_next;
+        if (after.t < t1) rows_next = fetch(after);
+        const int n0 = at.t * 64;
         int fb = -1;
         if constexpr (BIAS) {
             fb = far_bucket(p.bk, n0 - (p.M - 1) - p.start, n0 + 63 - p.start);
-            if (fb < 0)
+            if (fb < 0 && near_tile != at.t) {
+                near_tile = at.t;
                 for (int m = 0; m < p.M; ++m) {
                     const int bucket = bucket_of(border, p.bk.n, p.bk.both, n0 + lane - m - p.start);
                     for (int r = m; r < rows; r += p.M) near_bias[wave][r][lane] = table[r][bucket];
                 }
+            }
         }
-#pragma unroll 1
-        for (int u0 = 0; u0 < 64; u0 += U * KEYS) {
-            if (!(bits >> u0 & (U * KEYS == 64 ? ~0ull : (1ull << (U * KEYS % 64)) - 1))) continue;
-            typename Elem<T>::seg ks[U], vs[U];
-            bool in[U];
+        float x[R][U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int n = u0 + u * KEYS + group;
-                in[u] = bits >> n & 1;
-                ks[u] = {};
-                if (in[u]) ks[u] = load_seg(k + (n0 + n) * p.sk.r, d, p.D);
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                vs[u] = {};
-                if (in[u]) vs[u] = load_seg(v + (n0 + u0 + u * KEYS + group) * p.sv.r, d, p.D);
-            }
-            float x[R][U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const f32x8 kf = floats(ks[u]);
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    float a = q[r][0] * kf[0];
-#pragma unroll
-                    for (int i = 1; i < 8; ++i) a = __builtin_fmaf(q[r][i], kf[i], a);
-                    x[r][u] = row_sum<LANES>(a);
-                }
-            }
+        for (int u = 0; u < U; ++u) {
+            const f32x8 kf = floats(rows_here.k[u]);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                if (r >= rows) continue;
-                const int seat = r % p.M + p.start;                    // the query's position
-                float hi = LOW;
+                float a = q[r][0] * kf[0];
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int n = n0 + u0 + u * KEYS + group;
-                    if constexpr (BIAS) x[r][u] += fb >= 0 ? table[r][fb] : near_bias[wave][r][n - n0];
-                    if (!in[u] || (p.causal && n > seat)) x[r][u] = LOW;
-                    hi = fmaxf(hi, x[r][u]);
-                }
-                const float to = fmaxf(top[r], hi), ref = to == LOW ? 0.f : to, f = fexp2(top[r] - ref);
-                top[r] = to;
-                sum[r] *= f;
-                o[r] *= f;
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const float e = fexp2(x[r][u] - ref);
-                    sum[r] += e;
-                    o[r] += floats(vs[u]) * e;
-                }
+                for (int i = 1; i < 8; ++i) a = __builtin_fmaf(q[r][i], kf[i], a);
+                x[r][u] = row_sum<LANES>(a);
             }
         }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (r >= rows) continue;
+            const int seat = r % p.M + p.start;                        // the query's position
+            float hi = LOW;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int n = at.u0 + u * KEYS + group;
+                if constexpr (BIAS) x[r][u] += fb >= 0 ? table[r][fb] : near_bias[wave][r][n];
+                if (!(at.bits >> n & 1) || (p.causal && n0 + n > seat)) x[r][u] = LOW;
+                hi = fmaxf(hi, x[r][u]);
+            }
+            const float to = fmaxf(top[r], hi), ref = to == LOW ? 0.f : to, f = fexp2(top[r] - ref);
+            top[r] = to;
+            sum[r] *= f;
+            o[r] *= f;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float e = fexp2(x[r][u] - ref);
+                sum[r] += e;
+                o[r] += floats(rows_here.v[u]) * e;
+            }
+        }
+        at = after;
+        rows_here = rows_next;
     }
 
 #pragma unroll
