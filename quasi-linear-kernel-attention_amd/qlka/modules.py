@@ -8,7 +8,9 @@ entries, provided here with the same names and arguments:
     fused libqlka call each (qlka.layers); "softmax" is scaled dot-product attention with scale tau**-2
     (attention.py:99-102). TAU holds the default temperatures (kernels.py:13-25).
   * KernelMultiheadAttention(embed_dim, num_heads, kernel, tau, impl) (vision_transformer.py:19-44): self-attention
-    whose state_dict is nn.MultiheadAttention's (in_proj_weight, in_proj_bias, out_proj), so trained weights load.
+    whose state_dict is nn.MultiheadAttention's (in_proj_weight, in_proj_bias, out_proj), so trained weights load. With the
+    "softmax" kernel it also attends to another sequence (context), to earlier positions alone (causal) and with a learned
+    relative position bias (position_bias, a RelativePositionBias), on the kernels of qlka.softmax.
   * use_kernel_attention(model, kernel, tau, impl) and KernelAttention(config, kernel, tau, impl) (nomic.py:9-40):
     kernel attention inside a HF NomicBertModel with its own weights.
 
@@ -25,7 +27,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import layers
+from . import layers, softmax
 
 TAU = {"softmax": 64 ** 0.25, "add_laplace": 0.5, "add_riesz": 1.0, "add_bump": 1.5}   # kernels.py:13-25
 KERNELS = tuple(TAU)
@@ -61,14 +63,38 @@ def _resolve_tau(kernel, tau):
 
 
 # --------------------------------------------------------------------------------------------- vision transformer
-class KernelMultiheadAttention(nn.Module):
-    """x (B, S, E) -> (B, S, E) self-attention with a chosen kernel. Parameters and their initialisation follow
-    nn.MultiheadAttention (packed q/k/v input projection, output projection), so its state_dict loads both ways."""
+class RelativePositionBias(nn.Module):
+    """A learned position bias for each head and bucket of key - query distance: weight (num_buckets, num_heads).
+    forward(M, N, start) is the bias as a map (num_heads, M, N), for M queries from position start on and N keys."""
 
-    def __init__(self, embed_dim, num_heads, kernel="softmax", tau=None, impl="efficient"):
+    def __init__(self, num_heads, num_buckets=32, max_distance=128, bidirectional=True):
+        super().__init__()
+        self.buckets = softmax.RelativeBuckets(num_buckets, max_distance, bidirectional)
+        self.buckets.borders                             # refuses what has no buckets
+        self.weight = nn.Parameter(torch.zeros(num_buckets, num_heads))
+
+    def forward(self, M, N, start=0):
+        return softmax.relative_bias(self.weight, M, N, self.buckets, start=start)
+
+
+class KernelMultiheadAttention(nn.Module):
+    """x (B, S, E) -> (B, S, E) attention with a chosen kernel. Parameters and their initialisation follow
+    nn.MultiheadAttention (packed q/k/v input projection, output projection), so its state_dict loads both ways; a
+    position_bias (RelativePositionBias, "softmax" only) adds its own parameter.
+
+    forward(x, keep): self-attention. With the "softmax" kernel also
+      * forward(x, keep, context): attention to context (B, N, E), a sequence of another length, or to its heads as
+        project_context(context) gives them, which a decoder computes once and passes at every token; keep (B, N) marks
+        context's real positions;
+      * causal=True: the query at position start + m sees the keys up to its own position. For a decoder's next tokens,
+        context holds the heads of all tokens up to them and start is the position of x's first one."""
+
+    def __init__(self, embed_dim, num_heads, kernel="softmax", tau=None, impl="efficient", position_bias=None):
         super().__init__()
         if embed_dim % num_heads:
             raise ValueError(f"embed_dim {embed_dim} is not a multiple of num_heads {num_heads}")
+        if position_bias is not None and kernel != "softmax":
+            raise NotImplementedError(f"a position bias runs on the 'softmax' kernel, not on {kernel!r}")
         self.num_heads = num_heads
         self.kernel, self.tau, self.impl = kernel, _resolve_tau(kernel, tau), impl
         self.in_proj_weight = nn.Parameter(nn.init.xavier_uniform_(torch.empty(3 * embed_dim, embed_dim)))
@@ -76,17 +102,53 @@ class KernelMultiheadAttention(nn.Module):
         self.out_proj = nn.Linear(embed_dim, embed_dim)
         nn.init.xavier_uniform_(self.out_proj.weight)
         nn.init.zeros_(self.out_proj.bias)
+        self.position_bias = position_bias
+
+    def _heads(self, x, first, count):
+        """`count` of the packed projections of x from the first-th on, as (B, H, S, E / H) tensors."""
+        E = self.out_proj.in_features
+        part = slice(first * E, (first + count) * E)
+        packed = F.linear(x, self.in_proj_weight[part], self.in_proj_bias[part])    # [q | k | v] along the last dim
+        per_head = packed.unflatten(-1, (count, self.num_heads, -1))                 # (B, S, count, H, Dh)
+        return per_head.permute(2, 0, 3, 1, 4).unbind(0)
 
     def split_heads(self, x):
         """The packed projection of x as three (B, H, S, E / H) tensors q, k, v."""
-        packed = F.linear(x, self.in_proj_weight, self.in_proj_bias)            # [q | k | v] along the last dim
-        per_head = packed.unflatten(-1, (3, self.num_heads, -1))                 # (B, S, 3, H, Dh)
-        return per_head.permute(2, 0, 3, 1, 4).unbind(0)
+        return self._heads(x, 0, 3)
 
-    def forward(self, x, keep=None):
-        q, k, v = self.split_heads(x)
-        heads = attention(q, k, v, self.kernel, self.tau, keep, self.impl)      # (B, H, S, Dh)
+    def project_context(self, context):
+        """The heads (k, v) of context (B, N, E), each (B, H, N, E / H), as forward takes them."""
+        return self._heads(context, 1, 2)
+
+    def forward(self, x, keep=None, context=None, causal=False, start=0):
+        if context is None:
+            q, k, v = self.split_heads(x)
+            if self.position_bias is None and not causal:
+                heads = attention(q, k, v, self.kernel, self.tau, keep, self.impl)  # (B, H, S, Dh)
+                return self.out_proj(heads.transpose(1, 2).flatten(2))
+        else:
+            q, = self._heads(x, 0, 1)
+            k, v = context if isinstance(context, (tuple, list)) else self.project_context(context)
+        if self.kernel != "softmax":
+            raise NotImplementedError(f"attention to a context, causal order and a position bias run on the 'softmax' kernel, "
+                                      f"not on {self.kernel!r}")
+        heads = _softmax_to(q, k, v, self.tau, keep, self.position_bias, causal, start)
         return self.out_proj(heads.transpose(1, 2).flatten(2))
+
+
+def _softmax_to(q, k, v, tau, keep, position_bias, causal, start):
+    """Softmax attention of q to k, v of another length: qlka.softmax on the GPU, torch's own on the CPU (no bias there)."""
+    table = buckets = None
+    if position_bias is not None:
+        table, buckets = position_bias.weight, position_bias.buckets
+    if q.is_cuda or position_bias is not None:
+        return softmax.softmax_attention(q, k, v, scale=tau ** -2, keep=keep, table=table, buckets=buckets, causal=causal,
+                                         start=start)
+    mask = None if keep is None else keep.bool()[:, None, None, :]
+    if causal:
+        past = (torch.arange(k.shape[2])[None, :] <= torch.arange(q.shape[2])[:, None] + start)
+        mask = past if mask is None else mask & past
+    return F.scaled_dot_product_attention(q, k, v, attn_mask=mask, scale=tau ** -2)
 
 
 # ---------------------------------------------------------------------------------------------------- nomic-bert
