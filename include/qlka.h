@@ -245,7 +245,7 @@ int qlka_layer_fwd_masked(int kind, const float* q, const float* k, const float*
  * and num_borders + 1 buckets. table and g_table are (buckets, H) fp32, contiguous.
  *
  * Forward: writes out and, where not NULL, lse (B, H, M) (log2 of each row's sum, +inf for a row without keys) and out_full
- * (with QLKA_BF16 and a table: (B, H, M, D) fp32, out before it is rounded; the probabilities are then taken to 16 bits).
+ * (with QLKA_BF16 and a table: (B, H, M, D) fp32, out before it is rounded; the probabilities are then taken whole).
  * Backward: reads q, k, v, out, lse, g_out and, where not NULL, out_full, writes g_q (may be NULL), g_k and g_v (both or
  * neither NULL) and g_table (may be NULL; with QLKA_BF16 it needs out_full). No atomics: results do not change from run to run.
  */

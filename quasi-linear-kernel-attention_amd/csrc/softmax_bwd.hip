@@ -6,7 +6,7 @@
 // queries (of all the heads that share a key head) for 32 keys a wave. That is 7 products instead of the 5 of one pass, and no
 // sum between workgroups: no atomics, results that do not change from run to run. Scores stay in registers as in the
 // forward. Rounding P and dS to bf16 for the products with bf16 operands costs what rounding the results does. For the
-// table's gradient, which is fp32, dS is taken as it is, and delta formed from O to 16 bits (softmax_fwd.hip, FINE).
+// table's gradient, which is fp32, dS is taken as it is, and delta formed from an O that nothing was rounded in (softmax_fwd.hip, FINE).
 #include "softmax_tile.h"
 
 #include <limits>
@@ -112,11 +112,12 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
     }
     KeyBits<BN> seen(p, b);
     PairT tile(lds, p.sk.r, p.sv.r, p.D, tid);
-    const auto fetch = [&](int t, int buffer) {
-        tile.fetch(lds, buffer, k + (int64_t)t * BN * p.sk.r, v + (int64_t)t * BN * p.sv.r, seen.of(t), p.D, tid);
+    const auto fetch = [&](int t, uint64_t bits, int buffer) {
+        tile.fetch(lds, buffer, k + (int64_t)t * BN * p.sk.r, v + (int64_t)t * BN * p.sv.r, bits, p.D, tid);
     };
-    int t = seen.next(t0, t1), buffer = 0;
-    if (t < t1) fetch(t, 0);
+    int t = t0, buffer = 0;
+    uint64_t coming = seen.find(t, t1);                // the keys of tile t, which is on its way
+    if (coming) fetch(t, coming, 0);
 
     Frag<NP> qf[DP / 16], gf[DP / 16];
     float delta = 0.f;
@@ -152,9 +153,9 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
     const float c2 = p.scale * LOG2E;
     Acc<NP> dq[ND];
 
-    while (t < t1) {
+    while (coming) {
         const int n0 = t * BN;
-        const uint64_t bits = seen.of(t);
+        const uint64_t bits = coming;
         float far = 0.f;
         int fb = -1;
         float *near_here = near_bias[buffer], *mask = mask_of[buffer];
@@ -178,8 +179,8 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
         const auto& kt = lds.a[buffer];
         const auto& vt = lds.b[buffer];
         buffer ^= BUFFERS - 1;
-        t = seen.next(t + 1, t1);
-        if (t < t1) fetch(t, buffer);
+        coming = seen.find(++t, t1);
+        if (coming) fetch(t, coming, buffer);
         if (mw >= p.M || (p.causal && n0 > mw + 31 + p.start)) continue;
 
         const bool edge = p.causal && n0 + BN - 1 > mw + p.start;

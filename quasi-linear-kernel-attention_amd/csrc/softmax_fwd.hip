@@ -7,7 +7,7 @@
 // issued before the current tile's products. The running maximum is moved only when it grows by more than 2^8, so
 // that the output is hardly ever scaled; probabilities are then at most 2^8. Rounding them to bf16 for the product with bf16
 // values (not for fp32) costs what rounding the result does; the sum they are divided by is then that of the rounded ones. Where
-// the table's gradient will be wanted (FINE) they are taken in two parts of 8 bits: that gradient is fp32 and a sum over rows of
+// the table's gradient will be wanted (FINE) they are taken in three parts of 8 bits: that gradient is fp32 and a sum over rows of
 // dS = P (dP - delta), in which an error of delta, the row sum of dO * O, does not average out.
 //
 // Masked keys are read as zeros (what stands there may be anything) and their tiles, where none is left, are skipped.
@@ -49,11 +49,12 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
     }
     KeyBits<BN> seen(p, b);
     PairT tile(lds, p.sk.r, p.sv.r, p.D, tid);
-    const auto fetch = [&](int t, int buffer) {
-        tile.fetch(lds, buffer, k + (int64_t)t * BN * p.sk.r, v + (int64_t)t * BN * p.sv.r, seen.of(t), p.D, tid);
+    const auto fetch = [&](int t, uint64_t bits, int buffer) {
+        tile.fetch(lds, buffer, k + (int64_t)t * BN * p.sk.r, v + (int64_t)t * BN * p.sv.r, bits, p.D, tid);
     };
-    int t = seen.next(t0, t1), buffer = 0;
-    if (t < t1) fetch(t, 0);
+    int t = t0, buffer = 0;
+    uint64_t coming = seen.find(t, t1);                // the keys of tile t, which is on its way
+    if (coming) fetch(t, coming, 0);
 
     Frag<NP> qf[DP / 16];
 #pragma unroll
@@ -72,9 +73,9 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
     Acc<NP> o[ND];
     float top = -std::numeric_limits<float>::infinity(), ref = 0.f, sum = 0.f;
 
-    while (t < t1) {
+    while (coming) {
         const int n0 = t * BN;
-        const uint64_t bits = seen.of(t);
+        const uint64_t bits = coming;
         float far = 0.f;
         bool near = false;
         float *near_here = near_bias[buffer], *mask = mask_of[buffer];
@@ -95,8 +96,8 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
         const auto& kt = lds.a[buffer];
         const auto& vt = lds.b[buffer];
         buffer ^= BUFFERS - 1;
-        t = seen.next(t + 1, t1);
-        if (t < t1) fetch(t, buffer);
+        coming = seen.find(++t, t1);
+        if (coming) fetch(t, coming, buffer);
         if (mw >= p.M || (p.causal && n0 > mw + 31 + p.start)) continue;
 
         f32x16 s[NS];
@@ -171,18 +172,25 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
 #pragma unroll
                 for (int j = 0; j < 8; ++j) e[j] = fexp2(__builtin_fmaf(e[j], mul, add));
                 const Frag<NP> pf = split<NP>(e);
-                Frag<NP> rest;
-                if constexpr (FINE) rest = split<NP>(e - floats(pf.p[0]));
                 if constexpr (NP == 1 && !FINE) {
                     sum = add_all(pf.p[0], sum);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) sum += e[j];
                 }
+                Frag<NP> rest[2];
+                if constexpr (FINE) {
+                    e -= floats(pf.p[0]);
+                    rest[0] = split<NP>(e);
+                    rest[1] = split<NP>(e - floats(rest[0].p[0]));
+                }
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
                     const Frag<NP> vf = vt.column(32 * i + 16 * c, 32 * d, lane);
-                    if constexpr (FINE) o[d].add(vf, rest);
+                    if constexpr (FINE) {
+                        o[d].add(vf, rest[1]);
+                        o[d].add(vf, rest[0]);
+                    }
                     o[d].add(vf, pf);
                 }
             }

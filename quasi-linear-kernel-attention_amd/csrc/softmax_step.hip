@@ -75,18 +75,18 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p
     struct Place { int t, u0; uint64_t bits; };                       // a tile, the first key of U * KEYS of it, its keys
     const auto next = [&](Place at) {                                 // the next U * KEYS keys of this wave with one to see
         at.u0 += U * KEYS;
-        while (at.t < t1) {
+        while (true) {
             while (at.u0 < 64) {
                 if (at.bits >> at.u0 & (U * KEYS == 64 ? ~0ull : (1ull << U * KEYS % 64) - 1)) return at;
                 at.u0 += U * KEYS;
             }
             at.t += NW;
             at.u0 = 0;
-            if (at.t >= t1) break;
-            at.bits = seen.of(at.t);
+            if (at.t >= t1) return at;
+            int t = at.t;
+            at.bits = seen.find(t, t + 1);
             if (last - at.t * 64 < 63) at.bits &= (1ull << (last - at.t * 64 + 1)) - 1;
         }
-        return at;
     };
     // the keys of one place are on their way while those of the place before are worked on
     struct Rows { typename Elem<T>::seg k[U], v[U]; };

@@ -327,24 +327,22 @@ template <int BN> struct KeyBits {
             bits |= t << j;
         }
     }
-    __device__ __forceinline__ uint64_t of(int t) {
+    // moves t to the first tile from t on, before end, that has a key, and gives its keys; 0 where there is none
+    __device__ __forceinline__ uint64_t find(int& t, int end) {
         if (!keep) {
             const int left = N - t * BN;
-            return left >= BN ? (BN == 64 ? ~0ull : (1ull << BN % 64) - 1) : (1ull << left) - 1;
+            return t >= end ? 0 : left >= BN ? (BN == 64 ? ~0ull : (1ull << BN % 64) - 1) : (1ull << left) - 1;
         }
-        look(t >> 6);
-        return lane_u64(bits, t & 63);
-    }
-    // the first tile from t on that has a key, or end
-    __device__ __forceinline__ int next(int t, int end) {
-        if (!keep) return t < end ? t : end;
         while (t < end) {
             look(t >> 6);
             const uint64_t any = __ballot(bits != 0) >> (t & 63);
-            if (any) { const int f = t + __builtin_ctzll(any); return f < end ? f : end; }
+            if (any) {
+                t += __builtin_ctzll(any);
+                return t < end ? lane_u64(bits, t & 63) : 0;
+            }
             t = (t | 63) + 1;
         }
-        return end;
+        return 0;
     }
 };
 
