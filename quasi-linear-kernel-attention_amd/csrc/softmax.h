@@ -55,6 +55,7 @@ inline int sm_buckets(const SmBuckets& b) { return (b.n + 1) * (b.both ? 2 : 1);
 constexpr int FWD_WAVES = 4;
 int sm_fwd(int dtype, const SmParams& p, hipStream_t st);
 // waves (of 32 rows) a workgroup: 2 or 4
+constexpr int STEP_MOST = 4;              // query rows a key head that sm_step takes
 int sm_step(int dtype, const SmParams& p, hipStream_t st);
 int sm_combine(int dtype, const SmParams& p, hipStream_t st);
 int sm_delta(int dtype, const SmParams& p, hipStream_t st);

@@ -106,8 +106,18 @@ RowPlan row_plan(const qlka_softmax_args* a, int heads, int len, int64_t tiles, 
     return r;
 }
 
-// Few query rows per key head: the kernel without matrix tiles (softmax_step.hip).
-bool steps(const qlka_softmax_args* a) { return (int64_t)a->H / a->G * a->M <= 8; }
+// Few query rows per key head: the kernel without matrix tiles (softmax_step.hip), against the tiles, which read shared keys once
+// for each query head but hardly compute in bf16. Measured (us, step : tiles), B, heads / key heads, M, N of 64 elements:
+//   bf16  8, 12 / 12, 1,  197     6.2 :  7.9       fp32  8, 12 / 12, 4,  197    11.6 :  15.4
+//   bf16  4, 12 / 4,  1,  300    14.2 :  8.8       fp32 16, 12 / 3,  1, 4096    36   : 136
+//   bf16  4, 12 / 4,  1, 4097    19.5 : 19.6       fp32  1,  8 / 1,  1, 4096    21.3 :  15.8
+//   bf16 16, 12 / 3,  1, 8192      50 : 64         bf16 16, 12 / 12, 2, 8192    87   :  74
+bool steps(const qlka_softmax_args* a) {
+    const int64_t rows = (int64_t)a->H / a->G * a->M;
+    if (a->dtype == QLKA_F32) return rows <= STEP_MOST;
+    const double bytes = 4.0 * a->B * a->G * a->N * a->D;                 // of k and v
+    return rows == 1 || (a->M == 1 && rows <= STEP_MOST && bytes > 32e6);
+}
 
 struct FwdPlan { bool step; RowPlan rows; size_t part, part2; };
 FwdPlan fwd_plan(const qlka_softmax_args* a) {

@@ -5,7 +5,7 @@
 // for float) and keeps four such loads of k and four of v in flight, twice. Scores are formed with fp32 multiply-adds and summed
 // over a row's lanes by DPP; every group of lanes runs its own softmax over the keys that pass it, and the groups, then the
 // waves, are joined at the end. The keys are split over workgroups until the GPU is full (softmax_combine joins the
-// splits). A matrix tile would use one of its 32 rows here. Near the diagonal a lane finds the bias of one key of the tile for
+// splits). A matrix tile would use one of its 32 rows here; from a few rows on it is faster all the same (softmax_api.hip). Near the diagonal a lane finds the bias of one key of the tile for
 // every row, which the keys' groups then read from LDS.
 #include "softmax_tile.h"
 
@@ -43,28 +43,6 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p
     const int kvh = w % p.G, b = w / p.G, share = p.H / p.G, rows = share * p.M;
     const T* k = (const T*)p.k + b * p.sk.b + kvh * p.sk.h;
     const T* v = (const T*)p.v + b * p.sv.b + kvh * p.sv.h;
-
-    f32x8 q[R], o[R];
-    float top[R], sum[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        o[r] = f32x8{};
-        q[r] = f32x8{};
-        top[r] = LOW;
-        sum[r] = 0.f;
-        if (r < rows) {
-            const int head = kvh * share + r / p.M, m = r % p.M;
-            q[r] = floats(load_seg((const T*)p.q + b * p.sq.b + head * p.sq.h + m * p.sq.r, d, p.D)) *
-                   (p.q_sign * p.scale * LOG2E);
-            if constexpr (BIAS)
-                for (int i = tid; i < (p.bk.n + 1) * (p.bk.both ? 2 : 1); i += NT)
-                    table[r][i] = p.table[(int64_t)i * p.H + head] * LOG2E;
-        }
-    }
-    if constexpr (BIAS) {
-        for (int i = tid; i < p.bk.n; i += NT) border[i] = p.bk.border[i];
-        __syncthreads();
-    }
 
     const int tiles = (p.N + 63) / 64;
     const int t0 = (int)((int64_t)tiles * split_i / p.splits);
@@ -107,6 +85,29 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p
     Place at = next(Place{t0 + wave - NW, 64, 0});
     Rows rows_here;
     if (at.t < t1) rows_here = fetch(at);
+
+    f32x8 q[R], o[R];
+    float top[R], sum[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        o[r] = f32x8{};
+        q[r] = f32x8{};
+        top[r] = LOW;
+        sum[r] = 0.f;
+        if (r < rows) {
+            const int head = kvh * share + r / p.M, m = r % p.M;
+            q[r] = floats(load_seg((const T*)p.q + b * p.sq.b + head * p.sq.h + m * p.sq.r, d, p.D)) *
+                   (p.q_sign * p.scale * LOG2E);
+            if constexpr (BIAS)
+                for (int i = tid; i < (p.bk.n + 1) * (p.bk.both ? 2 : 1); i += NT)
+                    table[r][i] = p.table[(int64_t)i * p.H + head] * LOG2E;
+        }
+    }
+    if constexpr (BIAS) {
+        for (int i = tid; i < p.bk.n; i += NT) border[i] = p.bk.border[i];
+        __syncthreads();
+    }
+
     int near_tile = -1;
     while (at.t < t1) {
         const Place after = next(at);
@@ -225,8 +226,8 @@ template <class T, int DP, int R> int launch_step(const SmParams& p, hipStream_t
 }
 template <class T, int DP> int pick_step(const SmParams& p, hipStream_t st) {
     const int rows = p.H / p.G * p.M;
-    return rows == 1 ? launch_step<T, DP, 1>(p, st) : rows == 2 ? launch_step<T, DP, 2>(p, st)
-         : rows <= 4 ? launch_step<T, DP, 4>(p, st) : launch_step<T, DP, 8>(p, st);
+    static_assert(STEP_MOST == 4, "the largest number of rows has an instance");
+    return rows == 1 ? launch_step<T, DP, 1>(p, st) : rows == 2 ? launch_step<T, DP, 2>(p, st) : launch_step<T, DP, 4>(p, st);
 }
 }  // namespace sm
 
