@@ -217,7 +217,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c2, add);
                 }
-                if (bits != PairT::ALL) s[i] += rows_of(mask, 32 * (first + i) + 4 * half);
+                if (bits != PairT::ALL) s[i] = masked(s[i], mask, 32 * (first + i) + 4 * half);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[i][r] = fexp2(s[i][r]) * (dp[i][r] - delta);
                 if (edge) {

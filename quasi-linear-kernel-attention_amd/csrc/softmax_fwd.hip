@@ -131,7 +131,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
             }
             if (!all) {
 #pragma unroll
-                for (int i = 0; i < NS; ++i) s[i] += rows_of(mask, 32 * i + 4 * half);
+                for (int i = 0; i < NS; ++i) s[i] = masked(s[i], mask, 32 * i + 4 * half);
             }
             if (edge) {
                 const int lim = m + p.start - n0 - 4 * half;             // the last key seen

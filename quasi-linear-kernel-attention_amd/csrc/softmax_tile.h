@@ -357,9 +357,16 @@ struct BiasLds {
     }
 };
 
-// The masked keys of a tile as scores to add: 0 or -inf for each.
+// The masked keys of a tile: 0 or -inf for each.
 template <int BN> __device__ __forceinline__ void put_mask(float* mask, uint64_t bits, int tid) {
     if (tid < BN) mask[tid] = bits >> tid & 1 ? 0.f : -__builtin_inff();
+}
+// Scores with -inf for masked keys (whatever stood there); first as for rows_of.
+__device__ __forceinline__ f32x16 masked(f32x16 s, const float* mask, int first) {
+    const f32x16 z = rows_of(mask, first);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = z[r] == 0.f ? s[r] : z[r];
+    return s;
 }
 
 // number of borders <= dist
