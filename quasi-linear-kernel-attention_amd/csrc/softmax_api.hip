@@ -60,7 +60,9 @@ int check_sizes(const qlka_softmax_args* a) {
         return refuse("M, N and |start| must be <= 2^28");
     if ((double)a->B * a->H * a->M > (double)MOST_ROWS || (double)a->B * a->G * a->N > (double)MOST_ROWS)
         return refuse("B * H * M and B * G * N must fit int32");
-    if (!std::isfinite(a->scale)) return refuse("scale must be finite");
+    // the gradients hold log sums in units of the scale
+    if (a->scale != 0.f && !(std::fabs(a->scale) >= 0x1p-96f && std::fabs(a->scale) <= 0x1p96f))
+        return refuse("scale must be 0 or of a size in [2^-96, 2^96]");
     return QLKA_OK;
 }
 
@@ -247,7 +249,7 @@ int qlka_softmax_fwd(const qlka_softmax_args* a, void* ws, size_t ws_bytes, void
 }
 
 size_t qlka_softmax_bwd_ws_bytes(const qlka_softmax_args* a) {
-    if (check_sizes(a)) return 0;
+    if (check_sizes(a) || (a->g_table && (a->num_borders < 0 || a->num_borders >= QLKA_MAX_BUCKETS))) return 0;
     const BwdPlan w = bwd_plan(a, a->g_q, a->g_k, a->g_table);
     return w.delta + w.part + w.part2 + w.table;
 }
@@ -336,7 +338,7 @@ int qlka_bias_map_fwd(const float* table, const int* border, int num_borders, in
 }
 
 size_t qlka_bias_map_bwd_ws_bytes(int num_borders, int bidirectional, int H, int M, int N) {
-    if (check_map(H, M, N, 0) || num_borders < 0 || M == 0 || N == 0) return 0;
+    if (check_map(H, M, N, 0) || num_borders < 0 || num_borders >= QLKA_MAX_BUCKETS || M == 0 || N == 0) return 0;
     return (size_t)H * bias_map_blocks(M, N) * (num_borders + 1) * (bidirectional ? 2 : 1) * 4;
 }
 

@@ -87,7 +87,8 @@ WRONG = [
     (dict(dtype=2), "dtype must be"), (dict(B=-1), "B, M and N must be >= 0"), (dict(M=-1), "must be >= 0"),
     (dict(G=0), "H and G >= 1"), (dict(G=3), "H must be a multiple of G"), (dict(D=0), "multiple of 8"),
     (dict(D=60), "multiple of 8"), (dict(D=136), "multiple of 8"), (dict(N=(1 << 28) + 1), "2^28"), (dict(start=-(1 << 28) - 1), "2^28"),
-    (dict(B=1 << 20, M=1 << 20), "must fit int32"), (dict(scale=float("nan")), "scale must be finite"),
+    (dict(B=1 << 20, M=1 << 20), "must fit int32"), (dict(scale=float("nan")), "scale must be 0 or"),
+    (dict(scale=float("inf")), "scale must be 0 or"), (dict(scale=1e-38), "scale must be 0 or"),
     (dict(q=(1 << 12) + 4), "rows of q must be aligned"), (dict(v_stride=(896, 448, 66)), "rows of v must be aligned"),
     (dict(table=1 << 12, border=[3, 2]), "border must be positive"), (dict(table=1 << 12, border=[0]), "border must be positive"),
     (dict(table=1 << 12, border=list(range(1, 257))), "at most 256 buckets"),
