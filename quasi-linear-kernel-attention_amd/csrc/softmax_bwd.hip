@@ -6,7 +6,9 @@
 // queries (of all the heads that share a key head) for 32 keys a wave. That is 7 products instead of the 5 of one pass, and no
 // sum between workgroups: no atomics, results that do not change from run to run. Scores stay in registers as in the
 // forward. Rounding P and dS to bf16 for the products with bf16 operands costs what rounding the results does. For the
-// table's gradient, which is fp32, dS is taken as it is, and delta formed from an O that nothing was rounded in (softmax_fwd.hip, FINE).
+// table's gradient, which is fp32, dS is taken as it is, and delta formed from an O that nothing was rounded in
+// (softmax_fwd.hip, FINE). Bound as the forward is. Measured: 12 x 8192 x 8192 of 64 with the table's gradient, bf16:
+// softmax_dq 577 us (536 TFLOP/s), softmax_dkv 566 us (730); fp32, 32 x 4 heads of 600 to 65: 40 and 43 us.
 #include "softmax_tile.h"
 
 #include <limits>
@@ -121,6 +123,9 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
 
     Frag<NP> qf[DP / 16], gf[DP / 16];
     float delta = 0.f;
+    // dP is formed as -((-dO) V^T) for every other query: the matrix instruction's sums are a little low (softmax_tile.h), and a
+    // bucket adds up millions of dS (12 x 8192 x 8192, four inputs: error of the table's gradient 2 to 12% less)
+    const float turn = BIAS && (col & 1) ? -1.f : 1.f;
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
         const int d = 16 * c + 8 * half;
@@ -134,9 +139,10 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
         }
         s = s * (T)p.q_sign;
         qf[c] = frag_of(s);
-        gf[c] = frag_of(g);
 #pragma unroll
         for (int i = 0; i < 8; ++i) delta = __builtin_fmaf((float)g[i], o[i], delta);
+        g = g * (T)turn;
+        gf[c] = frag_of(g);
     }
     delta += other_half(delta);
     const float lse = m < p.M ? p.lse[row] : HIGH;
@@ -219,7 +225,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
                 }
                 if (bits != PairT::ALL) s[i] = masked(s[i], mask, 32 * (first + i) + 4 * half);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[i][r] = fexp2(s[i][r]) * (dp[i][r] - delta);
+                for (int r = 0; r < 16; ++r) s[i][r] = fexp2(s[i][r]) * __builtin_fmaf(dp[i][r], turn, -delta);
                 if (edge) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
