@@ -224,31 +224,32 @@ int qlka_layer_fwd_masked(int kind, const float* q, const float* k, const float*
                           int P, int D, int N, int M, int C, void* ws, size_t ws_bytes, void* stream);
 
 /*
- * Softmax attention to a sequence of another length, and the learned relative position bias by buckets. No counterpart in
- * the reference's operators: its "softmax" baseline is torch's scaled_dot_product_attention
+ * Softmax attention to a sequence of another length, and the learned relative position bias by buckets. No counterpart
+ * in the reference's operators: its "softmax" baseline is torch's scaled_dot_product_attention
  * (Experiments/kernel_attention/attention.py:99-102), for which it has no position bias.
  *
  *   S[b,h,m,n] = scale <q[b,h,m], k[b,h/(H/G),n]> + table[bucket(n - (m + start))][h]      (table may be NULL: no bias)
  *   out[b,h,m] = sum_n P[m,n] v[b,h/(H/G),n],  P = softmax of S over the keys that the query sees
- * A query sees key n if keep[b][n] is nonzero (keep may be NULL) and, with causal, n <= m + start. A row that sees no key
- * (or only scores of -inf) gives zeros, here and in every gradient. Masked keys' rows are not read. scale: 0 or of a size in
- * [2^-96, 2^96]. The table's values are finite or -inf; other infinities and NaN in what is read make NaN. Sums, the softmax's
- * statistics and every sum of the gradients are fp32; with QLKA_BF16 the probabilities and dS are rounded to bf16 for their
- * matrix products, and each result once at its end.
+ * A query sees key n if keep[b][n] is nonzero (keep may be NULL) and, with causal, n <= m + start. A row that sees no
+ * key (or only scores of -inf) gives zeros, here and in every gradient. Masked keys' rows are not read. scale: 0 or of
+ * a size in [2^-96, 2^96]. The table's values are finite or -inf; other infinities and NaN in what is read make NaN.
+ * Sums, the softmax's statistics and every sum of the gradients are fp32; with QLKA_BF16 the probabilities and dS are
+ * rounded to bf16 for their matrix products, and each result once at its end.
  *
- * q (B, H, M, D), k and v (B, G, N, D) with H a multiple of G; D a multiple of 8 up to 128, its elements contiguous; *_stride are
- * the distances in elements between batches, heads and rows (a dimension of size 1: any value); every row starts at a
- * multiple of 16 bytes. keep is rows of N bytes, keep_stride bytes apart. M and N may be 0.
+ * q (B, H, M, D), k and v (B, G, N, D) with H a multiple of G; D a multiple of 8 up to 128, its elements contiguous;
+ * *_stride are the distances in elements between batches, heads and rows (a dimension of size 1: any value); every row
+ * starts at a multiple of 16 bytes. keep is rows of N bytes, keep_stride bytes apart. M and N may be 0.
  *
- * Buckets: a side's bucket i holds the distances from border[i - 1] up to below border[i] (bucket 0 from 0 on, the last one
- * without end); border is non-decreasing and positive, on the host. bidirectional: distance |d| for d = n - (m + start),
- * keys after the query (d > 0) in buckets num_borders + 1 on, 2 (num_borders + 1) buckets in all. Else distance max(-d, 0)
- * and num_borders + 1 buckets. table and g_table are (buckets, H) fp32, contiguous.
+ * Buckets: a side's bucket i holds the distances from border[i - 1] up to below border[i] (bucket 0 from 0 on, the last
+ * one without end); border is non-decreasing and positive, on the host. bidirectional: distance |d| for d = n - (m +
+ * start), keys after the query (d > 0) in buckets num_borders + 1 on, 2 (num_borders + 1) buckets in all. Else distance
+ * max(-d, 0) and num_borders + 1 buckets. table and g_table are (buckets, H) fp32, contiguous.
  *
- * Forward: writes out and, where not NULL, lse (B, H, M) (log2 of each row's sum, +inf for a row without keys) and out_full
- * (with QLKA_BF16 and a table: (B, H, M, D) fp32, out before it is rounded; the probabilities are then taken whole).
- * Backward: reads q, k, v, out, lse, g_out and, where not NULL, out_full, writes g_q (may be NULL), g_k and g_v (both or
- * neither NULL) and g_table (may be NULL; with QLKA_BF16 it needs out_full). No atomics: results do not change from run to run.
+ * Forward: writes out and, where not NULL, lse (B, H, M) (log2 of each row's sum, +inf for a row without keys) and
+ * out_full (with QLKA_BF16 and a table: (B, H, M, D) fp32, out before it is rounded; the probabilities are then taken
+ * whole). Backward: reads q, k, v, out, lse, g_out and, where not NULL, out_full, writes g_q (may be NULL), g_k and g_v
+ * (both or neither NULL) and g_table (may be NULL; with QLKA_BF16 it needs out_full). No atomics: results do not change
+ * from run to run.
  */
 #define QLKA_F32  0
 #define QLKA_BF16 1

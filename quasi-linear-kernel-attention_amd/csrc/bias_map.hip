@@ -1,6 +1,7 @@
-// The relative position bias by buckets as a map: out[h, m, n] = table[bucket(n - (m + start))][h], and its gradient, the sums
-// of the map's gradient over each bucket. Both are bound by the map's bytes. The map is constant along its diagonals: a
-// workgroup finds the bucket of each diagonal of its tile once, and writes rows as windows of one array in LDS.
+// The relative position bias by buckets as a map: out[h, m, n] = table[bucket(n - (m + start))][h], and its gradient,
+// the sums of the map's gradient over each bucket. Both are bound by the map's bytes. The map is constant along its
+// diagonals: a workgroup finds the bucket of each diagonal of its tile once, and writes rows as windows of one array in
+// LDS.
 #include "softmax_tile.h"
 
 namespace qlka {
@@ -35,11 +36,11 @@ __global__ __launch_bounds__(MAP_T) void map_fwd(const float* table, const SmBuc
     }
 }
 
-// A workgroup sums its rows along 1024 diagonals. A thread takes 4 x 4 values at a time, four loads of four, and goes down
-// and to the right by four, so that it stays on the same seven diagonals; then the diagonals of a bucket are summed, at once
-// where a wave's lie in one. Measured for 12 x 1777 x 2049 (175 MB): 35 us, a plain sum's time, where the last-level cache
-// holds the map, 53 us after as many bytes were written. (64 rows a workgroup 58 us, 8 rows 53; one diagonal a thread, with
-// single loads, 148.)
+// A workgroup sums its rows along 1024 diagonals. A thread takes 4 x 4 values at a time, four loads of four, and goes
+// down and to the right by four, so that it stays on the same seven diagonals; then the diagonals of a bucket are
+// summed, at once where a wave's lie in one. Measured for 12 x 1777 x 2049 (175 MB): 35 us, a plain sum's time, where
+// the last-level cache holds the map, 53 us after as many bytes were written. (64 rows a workgroup 58 us, 8 rows 53;
+// one diagonal a thread, with single loads, 148.)
 __global__ __launch_bounds__(MAP_T) void map_bwd(const float* g, const SmBuckets bk, float* part, int M, int N, int start) {
     constexpr int NW = MAP_T / 64;
     __shared__ int border[QLKA_MAX_BUCKETS];

@@ -71,8 +71,9 @@ int check_sizes(const qlka_softmax_args* a) {
 constexpr int CUS = 256;
 
 // Splits of an axis of `tiles` tiles for `groups` workgroups over the other axes, by an estimate of the time: rounds of
-// workgroups on a CU (one alone on a CU is not twice as fast as two, waits not being filled), each its tiles and what it costs by
-// itself, and the joining of `join` bytes a split. In microseconds, fitted to prompts and gradients of 65 to 8192 keys.
+// workgroups on a CU (one alone on a CU is not twice as fast as two, waits not being filled), each its tiles and what
+// it costs by itself, and the joining of `join` bytes a split. In microseconds, fitted to prompts and gradients of 65
+// to 8192 keys.
 int splits_for(int64_t groups, int64_t tiles, double tile_us, double join_bytes) {
     int best = 1;
     double least = 0;
@@ -87,7 +88,8 @@ int splits_for(int64_t groups, int64_t tiles, double tile_us, double join_bytes)
     }
     return best;
 }
-// The same for the kernel of few rows, which is bound by memory: enough workgroups to fill the GPU, four tiles each or more.
+// The same for the kernel of few rows, which is bound by memory: enough workgroups to fill the GPU, four tiles each or
+// more.
 int step_splits(int64_t groups, int64_t tiles) {
     if (groups >= 1024) return 1;
     return (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(2048, std::max<int64_t>(groups, 1)), tiles / 4, 256}));
@@ -108,8 +110,9 @@ RowPlan row_plan(const qlka_softmax_args* a, int heads, int len, int64_t tiles, 
     return r;
 }
 
-// Few query rows per key head: the kernel without matrix tiles (softmax_step.hip), against the tiles, which read shared keys once
-// for each query head but hardly compute in bf16. Measured (us, step : tiles), B, heads / key heads, M, N of 64 elements:
+// Few query rows per key head: the kernel without matrix tiles (softmax_step.hip), against the tiles, which read shared
+// keys once for each query head but hardly compute in bf16. Measured (us, step : tiles), B, heads / key heads, M, N of
+// 64 elements:
 //   bf16  8, 12 / 12, 1,  197     6.2 :  7.9       fp32  8, 12 / 12, 4,  197    11.6 :  15.4
 //   bf16  4, 12 / 4,  1,  300    14.2 :  8.8       fp32 16, 12 / 3,  1, 4096    36   : 136
 //   bf16  4, 12 / 4,  1, 4097    19.5 : 19.6       fp32  1,  8 / 1,  1, 4096    21.3 :  15.8

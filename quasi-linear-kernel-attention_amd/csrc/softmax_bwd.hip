@@ -2,13 +2,14 @@
 //   dV = P^T dO,  dP = dO V^T,  delta = rowsum(dO * O),  dS = P * (dP - delta),  dQ = scale dS K,  dK = scale dS^T Q,
 // and the gradient of a bias bucket is the sum of dS over its scores.
 //
-// Two kernels, each forming P and dP for itself: softmax_dq goes over the keys for 32 queries a wave, softmax_dkv over the
-// queries (of all the heads that share a key head) for 32 keys a wave. That is 7 products instead of the 5 of one pass, and no
-// sum between workgroups: no atomics, results that do not change from run to run. Scores stay in registers as in the
-// forward. Rounding P and dS to bf16 for the products with bf16 operands costs what rounding the results does. For the
-// table's gradient, which is fp32, dS is taken as it is, and delta formed from an O that nothing was rounded in
-// (softmax_fwd.hip, FINE). Bound as the forward is. Measured: 12 x 8192 x 8192 of 64 with the table's gradient, bf16:
-// softmax_dq 577 us (536 TFLOP/s), softmax_dkv 566 us (730); fp32, 32 x 4 heads of 600 to 65: 40 and 43 us.
+// Two kernels, each forming P and dP for itself: softmax_dq goes over the keys for 32 queries a wave, softmax_dkv over
+// the queries (of all the heads that share a key head) for 32 keys a wave. That is 7 products instead of the 5 of one
+// pass, and no sum between workgroups: no atomics, results that do not change from run to run. Scores stay in registers
+// as in the forward. Rounding P and dS to bf16 for the products with bf16 operands costs what rounding the results
+// does. For the table's gradient, which is fp32, dS is taken as it is, and delta formed from an O that nothing was
+// rounded in (softmax_fwd.hip, FINE). Bound as the forward is. Measured: 12 x 8192 x 8192 of 64 with the table's
+// gradient, bf16: softmax_dq 577 us (536 TFLOP/s), softmax_dkv 566 us (730); fp32, 32 x 4 heads of 600 to 65: 40 and 43
+// us.
 #include "softmax_tile.h"
 
 #include <limits>
@@ -47,10 +48,11 @@ template <int CTRL, int ROWS> __device__ __forceinline__ void scan_step(float& x
     if (c == bucket) x += __int_as_float(y);
 }
 
-// Adds a wave's 32 x 32 scores' gradients to the buckets of their distances. A lane holds one query (lane % 32) and 16 keys;
-// for each register the values of 32 queries are turned in the wave until lane t holds the diagonal (key - query) = t or
-// t - 32, so a diagonal's sum gathers in one lane; lanes of one bucket, which are neighbours, are then summed by a segmented
-// scan. buckets: those of the distances from the tile's first key and first query less 32 on. acc: this wave's own, in LDS.
+// Adds a wave's 32 x 32 scores' gradients to the buckets of their distances. A lane holds one query (lane % 32) and 16
+// keys; for each register the values of 32 queries are turned in the wave until lane t holds the diagonal (key - query)
+// = t or t - 32, so a diagonal's sum gathers in one lane; lanes of one bucket, which are neighbours, are then summed by
+// a segmented scan. buckets: those of the distances from the tile's first key and first query less 32 on. acc: this
+// wave's own, in LDS.
 __device__ __forceinline__ void add_band(f32x16 ds, const uint8_t* buckets, float* acc, int lane) {
     const int t = lane & 31, half = lane >> 5, from = 4 * (4 * half - t);
     float pos = 0.f, neg = 0.f;
@@ -75,8 +77,8 @@ __device__ __forceinline__ void add_band(f32x16 ds, const uint8_t* buckets, floa
     if (lane == 63 || after != bucket) acc[bucket] += x;
 }
 
-// f(first half, halves together): both halves of a tile together where registers reach for it, else one after the other, and
-// the second only where it has something to do
+// f(first half, halves together): both halves of a tile together where registers reach for it, else one after the
+// other, and the second only where it has something to do
 template <int NP, int NS, class F> __device__ __forceinline__ void by_halves(bool one, F f) {
     if constexpr (NP == 1) {
         f(0, std::integral_constant<int, NS>());

@@ -5,19 +5,19 @@
 // the row maximum and sum need one exchange between the halves of the wave, and O^T += v^T P^T takes the probabilities
 // from the registers they are in. A workgroup's waves share the tiles of k and v in LDS; the next tile's loads are
 // issued before the current tile's products. The running maximum is moved only when it grows by more than 2^8, so
-// that the output is hardly ever scaled; probabilities are then at most 2^8. Rounding them to bf16 for the product with bf16
-// values (not for fp32) costs what rounding the result does; the sum they are divided by is then that of the rounded ones. Where
-// the table's gradient will be wanted (FINE) they are taken in three parts of 8 bits: that gradient is fp32 and a sum over rows of
-// dS = P (dP - delta), in which an error of delta, the row sum of dO * O, does not average out. The smaller parts' products then
-// gather in a sum of their own, as in Acc (12 x 8192 x 8192: error of the table's gradient 1.0e-6, 1.8e-6 without; 513 us
-// for 482).
+// that the output is hardly ever scaled; probabilities are then at most 2^8. Rounding them to bf16 for the product with
+// bf16 values (not for fp32) costs what rounding the result does; the sum they are divided by is then that of the
+// rounded ones. Where the table's gradient will be wanted (FINE) they are taken in three parts of 8 bits: that gradient
+// is fp32 and a sum over rows of dS = P (dP - delta), in which an error of delta, the row sum of dO * O, does not
+// average out. The smaller parts' products then gather in a sum of their own, as in Acc (12 x 8192 x 8192: error of the
+// table's gradient 1.0e-6, 1.8e-6 without; 513 us for 482).
 //
 // Masked keys are read as zeros (what stands there may be anything) and their tiles, where none is left, are skipped.
-// Bound by the matrix cores and by the scores' work between them (an exponential, a maximum and two multiply-adds a score),
-// which other waves' products hide only in part. Measured: 12 x 16384 x 16384 of 64 with the bias, bf16, 980 us, 840 TFLOP/s;
-// 4 x 12 x 2048 x 8192, padded, 205 us; fp32, 2 x 12 x 301 x 3111, padded, 54 us with the joining of the splits.
-// When a call has too few queries to fill the GPU, the keys are split: each split leaves its unscaled O with its maximum
-// and sum, and softmax_combine joins them.
+// Bound by the matrix cores and by the scores' work between them (an exponential, a maximum and two multiply-adds a
+// score), which other waves' products hide only in part. Measured: 12 x 16384 x 16384 of 64 with the bias, bf16, 980
+// us, 840 TFLOP/s; 4 x 12 x 2048 x 8192, padded, 205 us; fp32, 2 x 12 x 301 x 3111, padded, 54 us with the joining of
+// the splits. When a call has too few queries to fill the GPU, the keys are split: each split leaves its unscaled O
+// with its maximum and sum, and softmax_combine joins them.
 #include "softmax_tile.h"
 
 #include <limits>
@@ -251,7 +251,8 @@ template <class T, int DP, int NW> int launch_fwd(const SmParams& p, hipStream_t
     return (int)hipGetLastError();
 }
 // Joins the splits of a row, a wave a row: first a lane for each split's maximum and sum, then DP / 4 lanes for each of
-// several splits at a time, four elements a lane. Both steps' loads are issued together: a row costs two memory latencies.
+// several splits at a time, four elements a lane. Both steps' loads are issued together: a row costs two memory
+// latencies.
 constexpr int COMBINE_ROWS = 4, MOST_SPLITS = 256;
 
 template <class T, int DP>
@@ -301,7 +302,8 @@ __global__ __launch_bounds__(64 * COMBINE_ROWS) void softmax_combine(const SmPar
     if (p.lse && d == 0) p.lse[row] = sum == 0.f ? std::numeric_limits<float>::infinity() : ref + __log2f(sum);
 }
 
-// The same for up to FEW_SPLITS splits, DP / 4 lanes a row (12 x 4096 rows of 2 splits: 23 us with a wave a row, 16 us so).
+// The same for up to FEW_SPLITS splits, DP / 4 lanes a row (12 x 4096 rows of 2 splits: 23 us with a wave a row, 16 us
+// so).
 constexpr int FEW_SPLITS = 8;
 
 template <class T, int DP>

@@ -1,13 +1,14 @@
 // Softmax attention for a few query rows per key head (a decoder's single tokens; with shared heads all their queries):
 // bound by reading k and v once.
 //
-// A key row is read by DP / 8 lanes of a wave, 8 elements each, so a wave reads 512 / DP keys with one 16-byte load a lane (two
-// for float) and keeps four such loads of k and four of v in flight, twice. Scores are formed with fp32 multiply-adds and summed
-// over a row's lanes by DPP; every group of lanes runs its own softmax over the keys that pass it, and the groups, then the
-// waves, are joined at the end. The keys are split over workgroups until the GPU is full (softmax_combine joins the
-// splits). A matrix tile would use one of its 32 rows here; from a few rows on it is faster all the same (softmax_api.hip).
-// Near the diagonal a lane finds the bias of one key of the tile for every row, which the keys' groups then read from LDS.
-// Measured: 16 x 12 heads, 8192 padded keys of 64 in bf16 (303 MB read) 52 us, 5.8 TB/s; 8 x 12 heads, 197 keys 6.2 us.
+// A key row is read by DP / 8 lanes of a wave, 8 elements each, so a wave reads 512 / DP keys with one 16-byte load a
+// lane (two for float) and keeps four such loads of k and four of v in flight, twice. Scores are formed with fp32
+// multiply-adds and summed over a row's lanes by DPP; every group of lanes runs its own softmax over the keys that pass
+// it, and the groups, then the waves, are joined at the end. The keys are split over workgroups until the GPU is full
+// (softmax_combine joins the splits). A matrix tile would use one of its 32 rows here; from a few rows on it is faster
+// all the same (softmax_api.hip). Near the diagonal a lane finds the bias of one key of the tile for every row, which
+// the keys' groups then read from LDS. Measured: 16 x 12 heads, 8192 padded keys of 64 in bf16 (303 MB read) 52 us, 5.8
+// TB/s; 8 x 12 heads, 197 keys 6.2 us.
 #include "softmax_tile.h"
 
 #include <limits>

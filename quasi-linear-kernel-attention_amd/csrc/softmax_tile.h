@@ -2,15 +2,15 @@
 //
 // Products run on v_mfma_f32_32x32x16_bf16 (lane l: row or column l % 32, elements 8 (l / 32) + 0..7 of a 16-element
 // chunk; result: column l % 32, rows 8 (r / 4) + 4 (l / 32) + r % 4 for register r). The scores are formed with the
-// other side's rows in the registers, so a lane holds scores of one row (or one key), and eight successive result registers
-// are, as they are, the second operand of the next product: its 16-element chunk is taken in the order
+// other side's rows in the registers, so a lane holds scores of one row (or one key), and eight successive result
+// registers are, as they are, the second operand of the next product: its 16-element chunk is taken in the order
 //   slot (half, j) <- element 8 (j / 4) + 4 half + j % 4,
 // and the first operand is read from LDS in that order, transposed, by ds_read_b64_tr_b16 (four successive rows of one
 // column a lane). No score crosses lanes or goes through LDS.
 //
 // float inputs are split into three bf16 parts of 8 bits each (24 in all), and a product is the six products of parts
-// whose sizes add up to 2^-16 of the largest or more; what is left out is below 2^-26 of it. At 6 bf16 products that is 2.7
-// times the rate of the fp32 matrix instruction. An infinity among the inputs gives NaN this way.
+// whose sizes add up to 2^-16 of the largest or more; what is left out is below 2^-26 of it. At 6 bf16 products that is
+// 2.7 times the rate of the fp32 matrix instruction. An infinity among the inputs gives NaN this way.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -121,8 +121,8 @@ template <class T> __device__ __forceinline__ typename Elem<T>::seg load_seg(con
 }
 
 // A tile of ROWS rows of DP elements in LDS, one plane for each part, without gaps. A row's 16-byte pieces are turned
-// (exclusive or) by bits of the row's number so that the 128 bytes that LDS gives in a cycle, one piece of 8 rows or the two
-// pieces of 4 rows that a transposing read takes, are on different banks.
+// (exclusive or) by bits of the row's number so that the 128 bytes that LDS gives in a cycle, one piece of 8 rows or
+// the two pieces of 4 rows that a transposing read takes, are on different banks.
 template <int NP, int ROWS, int DP> struct Tile {
     static constexpr int PLANE = ROWS * DP, PIECES = DP / 8;
     __bf16 x[NP * PLANE];
@@ -170,9 +170,9 @@ template <class T, int DP> struct Shape {
     static constexpr int WAVES = NP == 3 && DP == 128 ? 1 : 2;
 };
 
-// 16 bytes a lane from memory to LDS, lane l's to `to` + 16 l bytes. Written out because of the waits: before every transposing
-// read the compiler would wait for its own form of this, though that goes to the other buffer. Pair::arrive() waits.
-// The low half of a generic pointer into LDS is the place in LDS.
+// 16 bytes a lane from memory to LDS, lane l's to `to` + 16 l bytes. Written out because of the waits: before every
+// transposing read the compiler would wait for its own form of this, though that goes to the other buffer.
+// Pair::arrive() waits. The low half of a generic pointer into LDS is the place in LDS.
 __device__ __forceinline__ uint32_t lds_place(const void* to) {
     return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)to);
 }
@@ -186,10 +186,10 @@ __device__ __forceinline__ void load_to_lds(const void* from, uint32_t bytes, ui
 
 // Two tiles (k and v, or q and dO) of ROWS rows on their way into LDS, where a workgroup of NW waves then reads them.
 //
-// bf16 goes there directly (global_load_lds, 16 bytes a lane, 1 KB an instruction; the pieces are turned by reading from turned
-// places), into the other one of two buffers while the current one is read: no registers hold a tile, and one barrier a tile is
-// enough. float goes through registers, where it is split into parts, and has one buffer and two barriers. Rows that are not
-// to be read become zeros.
+// bf16 goes there directly (global_load_lds, 16 bytes a lane, 1 KB an instruction; the pieces are turned by reading
+// from turned places), into the other one of two buffers while the current one is read: no registers hold a tile, and
+// one barrier a tile is enough. float goes through registers, where it is split into parts, and has one buffer and two
+// barriers. Rows that are not to be read become zeros.
 template <class T, int DP, int ROWS, int NW> struct Pair {
     static constexpr int NP = Elem<T>::PARTS, NT = 64 * NW, PIECES = DP / 8, BUFFERS = NP == 1 ? 2 : 1;
     static constexpr uint64_t ALL = ROWS == 64 ? ~0ull : (1ull << ROWS % 64) - 1;
@@ -391,9 +391,9 @@ __device__ __forceinline__ int far_bucket(const SmBuckets& bk, int lo, int hi) {
     return lo >= 0 ? 0 : -1;
 }
 
-// The work of a workgroup: `blocks` blocks of each of `pairs` (batch, head) pairs. Workgroups go round the 8 XCDs; all blocks
-// of a pair go to one of them, whose L2 then serves its keys, and successive pairs to different ones, since the heads of a
-// batch with more keys are next to each other. The pairs that are left over are spread over all.
+// The work of a workgroup: `blocks` blocks of each of `pairs` (batch, head) pairs. Workgroups go round the 8 XCDs; all
+// blocks of a pair go to one of them, whose L2 then serves its keys, and successive pairs to different ones, since the
+// heads of a batch with more keys are next to each other. The pairs that are left over are spread over all.
 struct Work { int pair, block; };
 __device__ __forceinline__ Work xcd_work(int wg, int pairs, int blocks) {
     const int full = (pairs >> 3) * blocks, slot = wg >> 3;
