@@ -197,3 +197,11 @@ def test_position_bias_parameters():
         n for n, _ in mod.named_parameters() if not n.startswith("position_bias"))
     with pytest.raises(RuntimeError, match="CUDA"):
         mod(torch.randn(1, 5, 32))
+
+
+@pytest.mark.parametrize("borders", [-5, 256, 1 << 30])
+def test_workspace_of_impossible_buckets_is_none(borders):
+    a = args(table=1 << 12, g_table=1 << 12)
+    a.num_borders = borders
+    assert _lib.load().qlka_softmax_bwd_ws_bytes(ctypes.byref(a)) == 0
+    assert _lib.load().qlka_bias_map_bwd_ws_bytes(borders, 0, 2, 30, 40) == 0
