@@ -164,13 +164,18 @@ BwdPlan bwd_plan(const qlka_softmax_args* a, bool dq, bool dkv, bool table) {
 
 SmStrides strides(const int64_t* s) { return {s[0], s[1], s[2]}; }
 
-// Rows are read and written in pieces of 16 bytes.
+// Rows are read and written in pieces of 16 bytes, those of a tile at unsigned offsets from its first one.
 int check_rows(const qlka_softmax_args* a, const char* name, const void* x, const int64_t* s, int heads, int rows) {
     const int64_t piece = a->dtype == QLKA_F32 ? 4 : 8;
-    if (!x || ((uintptr_t)x % 16 == 0 && (a->B <= 1 || s[0] % piece == 0) && (heads <= 1 || s[1] % piece == 0) &&
-               (rows <= 1 || s[2] % piece == 0)))
-        return QLKA_OK;
-    return refuse("the rows of %s must be aligned to 16 bytes", name);
+    if (!x) return QLKA_OK;
+    const int sizes[3] = {a->B, heads, rows};
+    bool aligned = (uintptr_t)x % 16 == 0;
+    for (int i = 0; i < 3; ++i) {
+        if (sizes[i] <= 1) continue;
+        if (s[i] < 0) return refuse("the strides of %s must not be negative", name);
+        aligned = aligned && s[i] % piece == 0;
+    }
+    return aligned ? QLKA_OK : refuse("the rows of %s must be aligned to 16 bytes", name);
 }
 
 int params(const qlka_softmax_args* a, SmParams* p) {

@@ -205,3 +205,21 @@ def test_workspace_of_impossible_buckets_is_none(borders):
     a.num_borders = borders
     assert _lib.load().qlka_softmax_bwd_ws_bytes(ctypes.byref(a)) == 0
     assert _lib.load().qlka_bias_map_bwd_ws_bytes(borders, 0, 2, 30, 40) == 0
+
+
+# --------------------------------------------------------------------------------------------- strides, sizes, launches
+@pytest.mark.parametrize("name,heads,rows", [("q", 4, 5), ("k", 2, 7), ("v", 2, 7), ("out", 4, 5), ("g_out", 4, 5), ("g_q", 4, 5),
+                                             ("g_k", 2, 7), ("g_v", 2, 7)])
+def test_negative_strides_are_refused(lib, name, heads, rows):
+    # rows of a tile are found by unsigned offsets from its first one
+    good = (heads * rows * 64, rows * 64, 64)
+    for i in range(3):
+        a = args(**{name + "_stride": [-s if i == j else s for j, s in enumerate(good)]})
+        for fn in (lib.qlka_softmax_fwd, lib.qlka_softmax_bwd):
+            assert fn(ctypes.byref(a), 1 << 12, 1 << 40, None) == 1
+            assert f"strides of {name} must not be negative" in lib.qlka_last_error().decode()
+
+
+def test_strides_of_single_rows_may_be_anything(lib):
+    a = args(B=1, H=1, G=1, M=0, N=1, **{n + "_stride": (-8, -8, -8) for n in ("q", "k", "v", "out")})
+    assert lib.qlka_softmax_fwd(ctypes.byref(a), None, 0, None) == 0           # nothing to do, and nothing refused
