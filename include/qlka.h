@@ -239,6 +239,7 @@ int qlka_layer_fwd_masked(int kind, const float* q, const float* k, const float*
  * q (B, H, M, D), k and v (B, G, N, D) with H a multiple of G; D a multiple of 8 up to 128, its elements contiguous;
  * *_stride are the distances in elements between batches, heads and rows, 0 or more (a dimension of size 1: any value);
  * every row starts at a multiple of 16 bytes. keep is rows of N bytes, keep_stride bytes apart. M and N may be 0.
+ * A launch takes less than 2^32 threads: B * heads * ceil(rows / 128) stays below 2^24.
  *
  * Buckets: a side's bucket i holds the distances from border[i - 1] up to below border[i] (bucket 0 from 0 on, the last
  * one without end); border is non-decreasing and positive, on the host. bidirectional: distance |d| for d = n - (m +

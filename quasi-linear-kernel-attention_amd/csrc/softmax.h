@@ -52,7 +52,7 @@ constexpr int sm_tile_rows(int parts, int DP) { return DP == 128 || (parts == 3 
 inline int sm_buckets(const SmBuckets& b) { return (b.n + 1) * (b.both ? 2 : 1); }
 
 // Launchers; each returns a hipError_t value. The dtype is QLKA_F32 or QLKA_BF16.
-constexpr int FWD_WAVES = 4;
+constexpr int FWD_WAVES = 4;              // waves a workgroup of the forward's kernels, of tiles and of single tokens
 int sm_fwd(int dtype, const SmParams& p, hipStream_t st);
 // waves (of 32 rows) a workgroup: 2 or 4
 constexpr int STEP_MOST = 4;              // query rows a key head that sm_step takes

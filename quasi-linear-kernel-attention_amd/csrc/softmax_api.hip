@@ -213,9 +213,13 @@ int need_ws(const void* ws, size_t have, size_t need) {
     return QLKA_OK;
 }
 
-int fits_grid(int64_t groups) {
-    return groups <= INT32_MAX ? QLKA_OK : refuse("too many workgroups: B * heads * blocks of rows must fit int32");
+// A launch takes less than 2^32 threads.
+int fits_grid(int64_t groups, int threads) {
+    if (groups <= (int64_t)UINT32_MAX / threads) return QLKA_OK;
+    return refuse("too many workgroups: %lld of %d threads, a launch takes less than 2^32 threads", (long long)groups, threads);
 }
+// a kernel of workgroups of 256 that takes `lanes` lanes a row
+int fits_rows(int64_t rows, int lanes) { return fits_grid(ceil_div(rows * lanes, 256), 256); }
 
 }  // namespace
 
@@ -237,7 +241,10 @@ int qlka_softmax_fwd(const qlka_softmax_args* a, void* ws, size_t ws_bytes, void
     if (a->out_full && (a->dtype == QLKA_F32 || !a->table)) return refuse("out_full goes with QLKA_BF16 and a table");
     const FwdPlan f = fwd_plan(a);
     if (int e = need_ws(ws, ws_bytes, f.part + f.part2)) return e;
-    if (int e = fits_grid((int64_t)a->B * (f.step ? a->G : a->H) * std::max(f.rows.blocks, 1) * f.rows.splits)) return e;
+    const int64_t heads = (int64_t)a->B * (f.step ? a->G : a->H);
+    if (int e = fits_grid(heads * std::max(f.rows.blocks, 1) * f.rows.splits, 64 * FWD_WAVES)) return e;
+    if (f.rows.splits > 1)
+        if (int e = fits_rows((int64_t)a->B * a->H * a->M, 64)) return e;
     hipStream_t st = (hipStream_t)stream;
     p.splits = f.rows.splits;
     p.blocks = f.rows.blocks;
@@ -276,8 +283,18 @@ int qlka_softmax_bwd(const qlka_softmax_args* a, void* ws, size_t ws_bytes, void
     if (rows && a->g_table && a->dtype == QLKA_BF16 && !a->out_full) return refuse("g_table needs out_full with QLKA_BF16");
     const BwdPlan w = bwd_plan(a, a->g_q, a->g_k, a->g_table);
     if (int e = need_ws(ws, ws_bytes, w.delta + w.part + w.part2 + w.table)) return e;
-    if (int e = fits_grid((int64_t)a->B * a->H * w.dq.blocks * w.dq.splits)) return e;
-    if (int e = fits_grid((int64_t)a->B * a->G * w.dkv.blocks * w.dkv.splits)) return e;
+    const int64_t queries = (int64_t)a->B * a->H * a->M, kept = (int64_t)a->B * a->G * a->N;
+    const int DP = sm_padded(a->D);
+    if (int e = fits_grid((int64_t)a->B * a->H * w.dq.blocks * w.dq.splits, 64 * std::max(w.dq.waves, 1))) return e;
+    if (int e = fits_grid((int64_t)a->B * a->G * w.dkv.blocks * w.dkv.splits, 64 * std::max(w.dkv.waves, 1))) return e;
+    if (!a->g_q && !a->g_table)
+        if (int e = fits_rows(queries, DP / 8)) return e;
+    if (w.dq.splits > 1)
+        if (int e = fits_rows(queries, DP / 4)) return e;
+    if (w.dkv.splits > 1)
+        if (int e = fits_rows(kept, DP / 4)) return e;
+    if (a->g_table)
+        if (int e = fits_grid(a->H, 256)) return e;
     hipStream_t st = (hipStream_t)stream;
     char* at = (char*)ws;
     p.delta = (float*)at; at += w.delta;

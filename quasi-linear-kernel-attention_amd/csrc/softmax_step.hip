@@ -16,7 +16,7 @@
 namespace qlka {
 namespace sm {
 
-constexpr int STEP_WAVES = 4;
+constexpr int STEP_WAVES = FWD_WAVES;
 
 template <int CTRL> __device__ __forceinline__ float dpp(float x) {
     return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, true));

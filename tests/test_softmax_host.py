@@ -223,3 +223,24 @@ def test_negative_strides_are_refused(lib, name, heads, rows):
 def test_strides_of_single_rows_may_be_anything(lib):
     a = args(B=1, H=1, G=1, M=0, N=1, **{n + "_stride": (-8, -8, -8) for n in ("q", "k", "v", "out")})
     assert lib.qlka_softmax_fwd(ctypes.byref(a), None, 0, None) == 0           # nothing to do, and nothing refused
+
+
+def refused(lib, fn, message, **kw):
+    a = args(**kw)
+    assert fn(ctypes.byref(a), 1 << 12, 1 << 44, None) == 1
+    assert message in lib.qlka_last_error().decode()
+
+
+def test_launches_past_2_32_threads_are_refused(lib):
+    """B * G single tokens take a workgroup of 256 threads each, and a launch less than 2^32 threads."""
+    one = dict(H=1, G=1, D=8, table=None)
+    many = "too many workgroups"
+    refused(lib, lib.qlka_softmax_fwd, many, **one, B=1 << 24, M=1, N=1)                        # a workgroup a token
+    refused(lib, lib.qlka_softmax_fwd, many, **one, B=1 << 24, M=5, N=1)                        # a workgroup 128 rows
+    nothing = dict(g_q=None, g_k=None, g_v=None)
+    for wanted in (dict(g_q=1 << 12), dict(g_k=1 << 12, g_v=1 << 12)):                          # two waves a workgroup
+        refused(lib, lib.qlka_softmax_bwd, many, **{**one, **nothing, **wanted}, B=1 << 25, M=1, N=1)
+    wide = {**one, **nothing, "D": 128, "B": 1 << 20, "M": 1 << 9, "N": 0}                       # row sums: 16 lanes a row
+    refused(lib, lib.qlka_softmax_bwd, many, **wide)
+    refused(lib, lib.qlka_softmax_bwd, many, H=1 << 24, G=1, B=1, M=0, N=1, D=8, g_q=None, g_k=None, g_v=None, table=1 << 12,
+            g_table=1 << 12, border=[1])                                                       # a workgroup a head and bucket
