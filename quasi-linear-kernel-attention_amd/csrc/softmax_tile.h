@@ -125,7 +125,7 @@ template <class T> __device__ __forceinline__ typename Elem<T>::seg load_seg(con
 // the two pieces of 4 rows that a transposing read takes, are on different banks.
 template <int NP, int ROWS, int DP> struct Tile {
     static constexpr int PLANE = ROWS * DP, PIECES = DP / 8;
-    __bf16 x[NP * PLANE];
+    alignas(16) __bf16 x[NP * PLANE];
 
     static __device__ __forceinline__ int turn(int row) {
         return DP == 32 ? (row & 2) | (row >> 2 & 1) : (row & 3) << 1 | (row >> 2 & 1);
@@ -195,6 +195,7 @@ template <class T, int DP, int ROWS, int NW> struct Pair {
     static constexpr uint64_t ALL = ROWS == 64 ? ~0ull : (1ull << ROWS % 64) - 1;
     typedef Tile<NP, ROWS, DP> TileT;
     struct Lds { TileT a[BUFFERS], b[BUFFERS]; };
+    static_assert(alignof(Lds) >= 16, "pieces of 16 bytes are read, written and loaded");
     static constexpr int HELD = NP == 1 ? 1 : ROWS * PIECES / NT, STEP = NT / PIECES;
     static_assert(NP == 1 || (HELD * NT == ROWS * PIECES && STEP * PIECES == NT), "a thread takes one column of HELD rows");
 
