@@ -104,6 +104,7 @@ __global__ __launch_bounds__(MAP_T) void map_bwd(const float* g, const SmBuckets
             }
             const int after = __shfl_down(bucket, 1);
             if (lane == 63 || after != bucket) sums[wave][bucket] += y;
+            wave_sync();
         }
     }
     __syncthreads();

@@ -75,6 +75,7 @@ __device__ __forceinline__ void add_band(f32x16 ds, const uint8_t* buckets, floa
     scan_step<0x143, 0xc>(x, bucket);        // row_bcast 31 into rows 2 and 3
     const int after = __shfl_down(bucket, 1);
     if (lane == 63 || after != bucket) acc[bucket] += x;
+    wave_sync();
 }
 
 // f(first half, halves together): both halves of a tile together where registers reach for it, else one after the

@@ -283,6 +283,7 @@ __global__ __launch_bounds__(64 * COMBINE_ROWS) void softmax_combine(const SmPar
         if (lane + 64 * i < p.splits) weight[wave][lane + 64 * i] = f;
         sum += a[i].y * f;
     }
+    wave_sync();
 #pragma unroll
     for (int far = 1; far < 64; far *= 2) sum += __shfl_xor(sum, far);
     const int d = lane % LANES * 4, first = lane / LANES;

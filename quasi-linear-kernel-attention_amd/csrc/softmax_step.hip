@@ -121,10 +121,12 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p
             fb = far_bucket(p.bk, n0 - (p.M - 1) - p.start, n0 + 63 - p.start);
             if (fb < 0 && near_tile != at.t) {
                 near_tile = at.t;
+                wave_sync();
                 for (int m = 0; m < p.M; ++m) {
                     const int bucket = bucket_of(border, p.bk.n, p.bk.both, n0 + lane - m - p.start);
                     for (int r = m; r < rows; r += p.M) near_bias[wave][r][lane] = table[r][bucket];
                 }
+                wave_sync();
             }
         }
         float x[R][U];

@@ -109,6 +109,13 @@ __device__ __forceinline__ float add_all(bf16x8 x, float to) {
     for (int i = 0; i < 4; ++i) to = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{x[2 * i], x[2 * i + 1]}, one, to, false);
     return to;
 }
+// What this wave's lanes wrote to LDS before, its other lanes read after (LDS serves a wave in order: no instruction, only an
+// order for the compiler).
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 __device__ __forceinline__ float fexp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
 __device__ __forceinline__ int reg_row(int r) { return (r >> 2) * 8 + (r & 3); }   // + 4 (lane / 32)
