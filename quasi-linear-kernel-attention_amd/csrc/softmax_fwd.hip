@@ -77,6 +77,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
     const float c2 = p.scale * LOG2E;
     Acc<NP> o[ND];
     float top = -std::numeric_limits<float>::infinity(), ref = 0.f, sum = 0.f;
+    bool wide = false;                                 // a row here has a large ref
 
     while (coming) {
         const int n0 = t * BN;
@@ -161,12 +162,22 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
             const float was = ref;
             top = fmaxf(top, hi);
             ref = top == -std::numeric_limits<float>::infinity() ? 0.f : top;
+            wide = __any(fabsf(ref) > WIDE);
             const float f = first ? 1.f : fexp2(was - ref);               // the first time there is nothing to scale
             sum *= f;
 #pragma unroll
             for (int d = 0; d < ND; ++d) o[d].main *= f;
         }
-        add -= ref;
+        if (__builtin_expect(wide, 0)) {
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], mul, add) - ref;
+            mul = 1.f;
+            add = 0.f;
+        } else {
+            add -= ref;
+        }
         float tile_sum = 0.f;                          // summed by tiles: thousands of terms one by one lose two digits more
         f32x16 small[ND];                              // FINE: the smaller parts apart, as in Acc
 #pragma unroll

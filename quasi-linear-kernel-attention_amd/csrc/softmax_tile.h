@@ -31,6 +31,10 @@ typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 
 constexpr float LOG2E = 1.4426950408889634f;
+// Where a row's reference (its maximum, its log sum) is larger, in log2 units, scores are rounded before it is taken off: it is
+// a rounded score itself, and the exact product in fma(score, scale, bias - reference) would be off from it by up to half its
+// last place, which is 2^-14 here and grows to any factor of the exponential.
+constexpr float WIDE = 1024.f;
 
 template <class T> struct Elem;
 template <> struct Elem<__bf16> { static constexpr int PARTS = 1; typedef bf16x8 seg; };
