@@ -98,8 +98,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p
         sum[r] = 0.f;
         if (r < rows) {
             const int head = kvh * share + r / p.M, m = r % p.M;
-            q[r] = floats(load_seg((const T*)p.q + b * p.sq.b + head * p.sq.h + m * p.sq.r, d, p.D)) *
-                   (p.q_sign * p.scale * LOG2E);
+            q[r] = floats(load_seg((const T*)p.q + b * p.sq.b + head * p.sq.h + m * p.sq.r, d, p.D)) * p.q_sign;
             if constexpr (BIAS)
                 for (int i = tid; i < (p.bk.n + 1) * (p.bk.both ? 2 : 1); i += NT)
                     table[r][i] = p.table[(int64_t)i * p.H + head] * LOG2E;
@@ -110,6 +109,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p
         __syncthreads();
     }
 
+    const float c2 = p.scale * LOG2E;
     int near_tile = -1;
     while (at.t < t1) {
         const Place after = next(at);
@@ -149,7 +149,8 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int n = at.u0 + u * KEYS + group;
-                if constexpr (BIAS) x[r][u] += fb >= 0 ? table[r][fb] : near_bias[wave][r][n];
+                // scaled after the sum, as in the tiles: equal products stay equal however large the scale is
+                x[r][u] = __builtin_fmaf(x[r][u], c2, BIAS ? fb >= 0 ? table[r][fb] : near_bias[wave][r][n] : 0.f);
                 if (!(at.bits >> n & 1) || (p.causal && n0 + n > seat)) x[r][u] = LOW;
                 hi = fmaxf(hi, x[r][u]);
             }

@@ -28,11 +28,11 @@ def equal_scores(t, see, scale):
 
 
 
-def whole(t, seed=0):
+def whole(t, seed=0, most=2):
     """q and k of small whole numbers: every score is exact before it is scaled, and scores are equal or 1 apart at least."""
     gen = torch.Generator().manual_seed(seed)
     for n in "qk":
-        t[n] = torch.randint(-2, 3, t[n].shape, generator=gen).to(t[n].dtype)
+        t[n] = torch.randint(-most, most + 1, t[n].shape, generator=gen).to(t[n].dtype)
     return t
 
 
@@ -44,12 +44,13 @@ def largest(t, see):
 
 
 @TYPES
-@pytest.mark.parametrize("M,N", [(40, 256), (200, 300), (70, 4000)])
-@pytest.mark.parametrize("scale", [2.0 ** 12, 2.0 ** 20, 2.0 ** 30, -2.0 ** 30, 2.0 ** 96])
+@pytest.mark.parametrize("M,N", [(40, 256), (200, 300), (70, 4000), (1, 300), (2, 4100)])
+@pytest.mark.parametrize("scale", [2.0 ** 12, 2.0 ** 20, 2.0 ** 30, -2.0 ** 30, 2.0 ** 96, 1e9])
 @pytest.mark.parametrize("masked", [False, True], ids=["all", "keep"])
 def test_large_scales_forward(dev, scale, M, N, masked, dtype):
-    """The keys of a row's largest score share it, on tiles with and without a mask, split and whole."""
-    t = whole(make(1, 2, 1, M, N, 64, dtype, seed=M, keep="random" if masked else None))
+    """The keys of a row's largest score share it, on tiles with and without a mask and for single tokens,
+    split and whole."""
+    t = whole(make(1, 2, 1, M, N, 64, dtype, seed=M, keep="random" if masked else None), most=2 if M > 4 else 9)
     see = oracle.visible(1, M, N, t["keep"])
     if scale < 0:
         t["q"] = -t["q"]
@@ -73,3 +74,17 @@ def test_large_scales_of_any_values_stay_finite(dev, scale, M, dtype):
     lo, hi = (f(t["v"].float(), 2, keepdim=True) for f in (torch.amin, torch.amax))
     slack = 2 ** -7 if dtype == BF16 else 2 ** -16
     assert (out >= lo - slack * lo.abs()).all() and (out <= hi + slack * hi.abs()).all()
+
+
+@TYPES
+@pytest.mark.parametrize("M", [1, 2, 40])
+def test_equal_products_stay_equal(dev, M, dtype):
+    """Keys of the same elements in another order against a query of equal ones: their sums are exact, so the scores are the
+    same however large the scale is."""
+    t = make(2, 2, 2, M, 200, 64, dtype, seed=4)
+    t["q"] = torch.ones_like(t["q"])
+    gen = torch.Generator().manual_seed(8)
+    row = torch.randint(-9, 20, (64,), generator=gen)
+    t["k"] = row[torch.rand(t["k"].shape, generator=gen).argsort(-1)].to(dtype)
+    want = equal_scores(t, torch.ones(2, M, 200, dtype=torch.bool), 1e9)
+    check(run(dev, t, train=False, scale=1e9), want, ["out"])
