@@ -138,11 +138,16 @@ FwdPlan fwd_plan(const qlka_softmax_args* a) {
     return f;
 }
 
-struct BwdPlan { RowPlan dq, dkv; size_t delta, part, part2, table; };
+struct BwdPlan {
+    RowPlan dq, dkv;
+    size_t delta, large, part, part2, table;
+    size_t bytes() const { return delta + large + part + part2 + table; }
+};
 BwdPlan bwd_plan(const qlka_softmax_args* a, bool dq, bool dkv, bool table) {
     BwdPlan w{};
     const int t = tile_rows(a), DP = sm_padded(a->D);
     w.delta = align256((size_t)a->B * a->H * a->M * 4);
+    w.large = align256((size_t)a->B * a->H * ceil_div(a->M, 32) * 4);
     if (dq || table) {
         w.dq = row_plan(a, a->H, a->M, ceil_div(a->N, t), 3, 0);
         if (w.dq.splits > 1) w.part = align256((size_t)w.dq.splits * a->B * a->H * a->M * DP * 4);
@@ -188,7 +193,7 @@ int params(const qlka_softmax_args* a, SmParams* p) {
     p->sgq = strides(a->g_q_stride); p->sgk = strides(a->g_k_stride); p->sgv = strides(a->g_v_stride);
     p->keep = a->keep; p->keep_stride = a->keep_stride;
     p->table = a->table;
-    p->lse = a->lse;
+    p->lse = a->lse; p->lse_low = a->lse_low;
     p->B = a->B; p->H = a->H; p->G = a->G; p->M = a->M; p->N = a->N; p->D = a->D;
     p->causal = a->causal ? 1 : 0;
     p->start = a->start;
@@ -266,7 +271,7 @@ int qlka_softmax_fwd(const qlka_softmax_args* a, void* ws, size_t ws_bytes, void
 size_t qlka_softmax_bwd_ws_bytes(const qlka_softmax_args* a) {
     if (check_sizes(a) || (a->g_table && (a->num_borders < 0 || a->num_borders >= QLKA_MAX_BUCKETS))) return 0;
     const BwdPlan w = bwd_plan(a, a->g_q, a->g_k, a->g_table);
-    return w.delta + w.part + w.part2 + w.table;
+    return w.bytes();
 }
 
 int qlka_softmax_bwd(const qlka_softmax_args* a, void* ws, size_t ws_bytes, void* stream) {
@@ -282,13 +287,13 @@ int qlka_softmax_bwd(const qlka_softmax_args* a, void* ws, size_t ws_bytes, void
     if (a->out_full && (a->dtype == QLKA_F32 || !a->table)) return refuse("out_full goes with QLKA_BF16 and a table");
     if (rows && a->g_table && a->dtype == QLKA_BF16 && !a->out_full) return refuse("g_table needs out_full with QLKA_BF16");
     const BwdPlan w = bwd_plan(a, a->g_q, a->g_k, a->g_table);
-    if (int e = need_ws(ws, ws_bytes, w.delta + w.part + w.part2 + w.table)) return e;
+    if (int e = need_ws(ws, ws_bytes, w.bytes())) return e;
     const int64_t queries = (int64_t)a->B * a->H * a->M, kept = (int64_t)a->B * a->G * a->N;
     const int DP = sm_padded(a->D);
     if (int e = fits_grid((int64_t)a->B * a->H * w.dq.blocks * w.dq.splits, 64 * std::max(w.dq.waves, 1))) return e;
     if (int e = fits_grid((int64_t)a->B * a->G * w.dkv.blocks * w.dkv.splits, 64 * std::max(w.dkv.waves, 1))) return e;
     if (!a->g_q && !a->g_table)
-        if (int e = fits_rows(queries, DP / 8)) return e;
+        if (int e = fits_rows((int64_t)a->B * a->H * ceil_div(a->M, 32), 64)) return e;
     if (w.dq.splits > 1)
         if (int e = fits_rows(queries, DP / 4)) return e;
     if (w.dkv.splits > 1)
@@ -298,6 +303,7 @@ int qlka_softmax_bwd(const qlka_softmax_args* a, void* ws, size_t ws_bytes, void
     hipStream_t st = (hipStream_t)stream;
     char* at = (char*)ws;
     p.delta = (float*)at; at += w.delta;
+    p.large = (int*)at; at += w.large;
     p.part = (float*)at; at += w.part;
     p.part2 = (float*)at; at += w.part2;
     p.part_table = (float*)at;

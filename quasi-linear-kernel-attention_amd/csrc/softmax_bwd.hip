@@ -19,25 +19,34 @@ namespace sm {
 
 constexpr float HIGH = std::numeric_limits<float>::infinity();
 
-// delta: DP / 8 lanes a row
+// delta, a wave 32 rows of a head, DP / 8 lanes a row; and whether one of the 32 has a large log sum
 template <class T, int DP>
 __global__ __launch_bounds__(256) void softmax_delta(const SmParams p) {
     constexpr int LANES = DP / 8;
-    const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES, rows = (int64_t)p.B * p.H * p.M;
-    const int d = threadIdx.x % LANES * 8;
-    float x = 0.f;
-    if (row < rows) {
-        const int m = (int)(row % p.M), head = (int)(row / p.M % p.H), b = (int)(row / p.M / p.H);
-        const T* out = (const T*)p.out + b * p.so.b + head * p.so.h + m * p.so.r;
-        const auto g = load_seg((const T*)p.g_out + b * p.sg.b + head * p.sg.h + m * p.sg.r, d, p.D);
-        const f32x8 o = p.out_full ? load_seg(p.out_full + row * p.D, d, p.D)
-                                   : floats(load_seg(out, d, p.D));
+    const int groups = (p.M + 31) / 32, lane = threadIdx.x & 63, d = lane % LANES * 8;
+    const int64_t group = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (group >= (int64_t)p.B * p.H * groups) return;
+    const int first = (int)(group % groups) * 32, head = (int)(group / groups % p.H), b = (int)(group / groups / p.H);
+    const int64_t row0 = ((int64_t)b * p.H + head) * p.M;
+    bool large = false;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x = __builtin_fmaf((float)g[i], o[i], x);
+    for (int i = 0; i < 32; i += 64 / LANES) {
+        const int m = first + i + lane / LANES;
+        float x = 0.f;
+        if (m < p.M) {
+            const T* out = (const T*)p.out + b * p.so.b + head * p.so.h + m * p.so.r;
+            const auto g = load_seg((const T*)p.g_out + b * p.sg.b + head * p.sg.h + m * p.sg.r, d, p.D);
+            const f32x8 o = p.out_full ? load_seg(p.out_full + (row0 + m) * p.D, d, p.D) : floats(load_seg(out, d, p.D));
+            large |= large_lse(p.lse[row0 + m]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x = __builtin_fmaf((float)g[j], o[j], x);
+        }
+#pragma unroll
+        for (int far = 1; far < LANES; far *= 2) x += __shfl_xor(x, far);
+        if (m < p.M && d == 0) p.delta[row0 + m] = x;
     }
-#pragma unroll
-    for (int far = 1; far < LANES; far *= 2) x += __shfl_xor(x, far);
-    if (row < rows && d == 0) p.delta[row] = x;
+    large = __any(large);
+    if (lane == 0) p.large[group] = large;
 }
 
 // y of a lane added to x where both lanes' buckets are the same: one step of a segmented scan over a wave (CTRL: a DPP
@@ -87,6 +96,17 @@ template <int NP, int NS, class F> __device__ __forceinline__ void by_halves(boo
 #pragma unroll 1
         for (int i = 0; i < (one ? 1 : NS); ++i) f(i, std::integral_constant<int, 1>());
     }
+}
+
+// Large log sums are taken off in two steps, after the score is rounded. With bf16 operands in a loop of its own, f(true): a
+// test between a tile's products and its exponentials keeps those apart (8% of softmax_dkv's time at 4 x 12 x 1024 x 4096
+// of 64). With fp32 the test is in the loop, by tiles, f(false): there it costs 1% at 32 x 4 heads of 600 to 65, and what a
+// second loop needs before it starts, and its registers, 5%.
+template <int NP, class F> __device__ __forceinline__ void by_size(bool large, F f) {
+    if constexpr (NP == 1) {
+        if (__builtin_expect(large, 0)) return f(std::true_type());
+    }
+    f(std::false_type());
 }
 
 template <class T, int DP, int NW, bool BIAS>
@@ -149,19 +169,27 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
     }
     delta += other_half(delta);
     const float lse = m < p.M ? p.lse[row] : HIGH;
-    if (m < p.M && half == 0 && split_i == 0) p.delta[row] = delta;        // softmax_dkv reads it
+    const bool large = __any(large_lse(lse));
+    if (split_i == 0) {                                // softmax_dkv reads them
+        if (m < p.M && half == 0) p.delta[row] = delta;
+        if (mw < p.M && lane == 0) p.large[((int64_t)b * p.H + head) * ((p.M + 31) / 32) + mw / 32] = large;
+    }
     const int buckets = (p.bk.n + 1) * (p.bk.both ? 2 : 1);
     float left = 0.f, right = 0.f;                     // this lane's sums far below and far above the diagonal
     const bool to_table = BIAS && p.part_table;
     if constexpr (BIAS) {
         table.fill(p, head, tid, NT);
         for (int i = lane; i < buckets; i += 64) sums[wave][i] = 0.f;
-        __syncthreads();
     }
+    bool any_large = false;
+    if constexpr (NP == 1) any_large = __syncthreads_or(large);
+    else if constexpr (BIAS) __syncthreads();
 
     const float c2 = p.scale * LOG2E;
     Acc<NP> dq[ND];
 
+    const auto go = [&](auto all_wide) {
+    const bool wide = NP == 3 ? large : all_wide;
     while (coming) {
         const int n0 = t * BN;
         const uint64_t bits = coming;
@@ -195,7 +223,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
         const bool edge = p.causal && n0 + BN - 1 > mw + p.start;
         const int lim = m + p.start - n0 - 4 * half;                     // at an edge, the last key seen
         const float* nb = &near_here[BIAS ? ROWS - 1 - wave * 32 - col + 4 * half : 0];
-        const float add = far - lse;
+        const float off = wide ? 0.f : lse, add = far - off;
         // `count` halves of the tile together: the products of one are under way while the other's scores are worked on
         const auto halves = [&](auto first, auto count) {
             f32x16 s[count], dp[count];
@@ -221,10 +249,15 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
             for (int i = 0; i < count; ++i) {
                 if (BIAS && fb < 0) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c2, nb[32 * (first + i) + reg_row(r)] - lse);
+                    for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c2, nb[32 * (first + i) + reg_row(r)] - off);
                 } else {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c2, add);
+                }
+                if (wide) {
+                    const float low = m < p.M && p.lse_low ? p.lse_low[row] : 0.f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[i][r] = at_most_0((s[i][r] - lse) - low);
                 }
                 if (bits != PairT::ALL) s[i] = masked(s[i], mask, 32 * (first + i) + 4 * half);
 #pragma unroll
@@ -260,6 +293,8 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
         };
         by_halves<NP, NS>(NS == 1 || !(bits >> 32), halves);
     }
+    };
+    by_size<NP>(any_large, go);
     if (to_table) {
 #pragma unroll
         for (int x = 1; x < 64; x *= 2) {
@@ -300,7 +335,8 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
     typedef Pair<T, DP, BM, NW> PairT;
     constexpr int BUFFERS = PairT::BUFFERS;
     __shared__ typename PairT::Lds lds;
-    __shared__ __attribute__((aligned(16))) float lse_of[BUFFERS][BM], delta_of[BUFFERS][BM];
+    __shared__ __attribute__((aligned(16))) float lse_of[BUFFERS][BM], delta_of[BUFFERS][BM], large_of[BUFFERS][2][BM];
+    __shared__ int wide_of;                            // (fp32, of the one buffer) a row of the tile has a large log sum
     __shared__ BiasLds table;
     __shared__ float near_bias[BUFFERS][BIAS ? KEYS + BM : 1];
 
@@ -351,16 +387,25 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
         vf[c] = frag_of(x);
     }
 
+    const int groups = share * ((p.M + 31) / 32);      // of 32 rows of the heads that share these keys
+    bool any_large = false;
+    if constexpr (NP == 1) {
+        for (int i = tid; i < groups; i += NT) any_large |= p.large[((int64_t)b * p.G + kvh) * groups + i] != 0;
+        any_large = __syncthreads_or(any_large);
+    }
+
     const float c2 = p.scale * LOG2E;
     Acc<NP> dk[ND], dv[ND];
     const float per_c2 = 1.f / c2;
     int filled = -1;                                   // the head whose bias stands in LDS
 
+    const auto go = [&](auto all_wide) {
     while (t < t1) {
         const int m0 = t % tiles * BM, head = kvh * share + t / tiles;
         float far = 0.f;
         bool near = false;
         float *near_here = near_bias[buffer], *lse = lse_of[buffer], *delta = delta_of[buffer];
+        float (*two)[BM] = large_of[buffer];
         if (BIAS && head != filled) {
             __syncthreads();
             table.fill(p, head, tid, NT);
@@ -368,9 +413,15 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
             __syncthreads();
         }
         tile.arrive(lds, tid, [&] {
+            const bool wide = NP == 3 ? __any(large_lse(ls)) : all_wide;      // all rows are in the first wave
+            if (NP == 3 && tid == 0) wide_of = wide;
             if (tid < BM) {
-                lse[tid] = -ls * per_c2;
+                lse[tid] = wide ? 0.f : -ls * per_c2;
                 delta[tid] = -des;
+                if (wide) {
+                    two[0][tid] = ls;
+                    two[1][tid] = p.lse_low && m0 + tid < p.M ? p.lse_low[((int64_t)b * p.H + head) * p.M + m0 + tid] : 0.f;
+                }
             }
             if constexpr (BIAS) {
                 const int lo = n0 - (m0 + BM - 1) - p.start;
@@ -395,14 +446,14 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
         const int lim = edge ? n - p.start - m0 - 4 * half : -1;         // the first query that sees the key
         const float* nb = &near_here[BIAS ? wave * 32 + col + BM - 1 - 4 * half : 0];
         const auto halves = [&](auto first, auto count) {
-            // scores less the row's log sum (in units of the scores), and dP less delta
+            // scores less the row's log sum (in units of the scores; a large one later), and dP less delta
             f32x16 s[count], dp[count];
 #pragma unroll
             for (int i = 0; i < count; ++i) {
                 Acc<NP> a(rows_of(lse, 32 * (first + i) + 4 * half));
                 a.start();
 #pragma unroll
-                for (int c = 0; c < DP / 16; ++c) a.add(qt.row(32 * (first + i) + col, 16 * c + 8 * half), kf[c]);
+                for (int c = 0; c < DP / 16; ++c) a.add_turned(qt.row(32 * (first + i) + col, 16 * c + 8 * half), kf[c]);
                 a.join();
                 s[i] = a.main;
             }
@@ -415,14 +466,23 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
                 a.join();
                 dp[i] = a.main;
             }
+            const bool wide = NP == 3 ? __builtin_amdgcn_readfirstlane(wide_of) : all_wide;
 #pragma unroll
             for (int i = 0; i < count; ++i) {
                 if (BIAS && near) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c2, nb[-32 * (first + i) - reg_row(r)]);
-                } else {
+                } else if (BIAS || !wide) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c2, far);
+                }
+                if (wide) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int row = 32 * (first + i) + 4 * half + reg_row(r);
+                        const float x = BIAS ? s[i][r] : __builtin_fmaf(s[i][r], c2, far);     // apart from the above: fewer spills
+                        s[i][r] = at_most_0((x - two[0][row]) - two[1][row]);
+                    }
                 }
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
@@ -457,6 +517,8 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
         };
         by_halves<NP, NS>(m0 + 32 >= p.M, halves);
     }
+    };
+    by_size<NP>(any_large, go);
     if (n >= p.N) return;
     const float f = p.scale * p.q_sign;
     const int64_t row = ((int64_t)b * p.G + kvh) * p.N + n, all = (int64_t)p.B * p.G * p.N;
@@ -505,8 +567,8 @@ __global__ __launch_bounds__(256) void softmax_table(const float* part, float* g
 }
 
 template <class T, int DP> int run_delta(const SmParams& p, hipStream_t st) {
-    const int64_t threads = (int64_t)p.B * p.H * p.M * (DP / 8);
-    softmax_delta<T, DP><<<dim3((unsigned)((threads + 255) / 256)), 256, 0, st>>>(p);
+    const int64_t groups = (int64_t)p.B * p.H * ((p.M + 31) / 32);
+    softmax_delta<T, DP><<<dim3((unsigned)((groups + 3) / 4)), 256, 0, st>>>(p);
     return (int)hipGetLastError();
 }
 template <class T, int DP, int NW> int run_dq(const SmParams& p, hipStream_t st) {

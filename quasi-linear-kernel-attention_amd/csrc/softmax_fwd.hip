@@ -168,60 +168,64 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
 #pragma unroll
             for (int d = 0; d < ND; ++d) o[d].main *= f;
         }
-        if (__builtin_expect(wide, 0)) {
+        const auto weigh = [&](auto wide) {
+            if constexpr (wide) {
 #pragma unroll
-            for (int i = 0; i < NS; ++i)
+                for (int i = 0; i < NS; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], mul, add) - ref;
-            mul = 1.f;
-            add = 0.f;
-        } else {
-            add -= ref;
-        }
-        float tile_sum = 0.f;                          // summed by tiles: thousands of terms one by one lose two digits more
-        f32x16 small[ND];                              // FINE: the smaller parts apart, as in Acc
+                    for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], mul, add) - ref;
+                mul = 1.f;
+                add = 0.f;
+            } else {
+                add -= ref;
+            }
+            float tile_sum = 0.f;                          // summed by tiles: thousands of terms one by one lose two digits more
+            f32x16 small[ND];                              // FINE: the smaller parts apart, as in Acc
 #pragma unroll
-        for (int d = 0; d < ND; ++d) {
-            o[d].start();
-            if constexpr (FINE) small[d] = f32x16{};
-        }
+            for (int d = 0; d < ND; ++d) {
+                o[d].start();
+                if constexpr (FINE) small[d] = f32x16{};
+            }
 #pragma unroll
-        for (int i = 0; i < NS; ++i) {
+            for (int i = 0; i < NS; ++i) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                f32x8 e = eight(s[i], c);
+                for (int c = 0; c < 2; ++c) {
+                    f32x8 e = eight(s[i], c);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) e[j] = fexp2(__builtin_fmaf(e[j], mul, add));
-                const Frag<NP> pf = split<NP>(e);
-                if constexpr (NP == 1 && !FINE) {
-                    sum = add_all(pf.p[0], sum);
-                } else {
+                    for (int j = 0; j < 8; ++j) e[j] = fexp2(__builtin_fmaf(e[j], mul, add));
+                    const Frag<NP> pf = split<NP>(e);
+                    if constexpr (NP == 1 && !FINE) {
+                        sum = add_all(pf.p[0], sum);
+                    } else {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) tile_sum += e[j];
-                }
-                Frag<NP> rest[2];
-                if constexpr (FINE) {
-                    e -= floats(pf.p[0]);
-                    rest[0] = split<NP>(e);
-                    rest[1] = split<NP>(e - floats(rest[0].p[0]));
-                }
-#pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    const Frag<NP> vf = vt.column(32 * i + 16 * c, 32 * d, lane);
-                    if constexpr (FINE) {
-                        small[d] = mfma(vf.p[0], rest[1].p[0], small[d]);
-                        small[d] = mfma(vf.p[0], rest[0].p[0], small[d]);
+                        for (int j = 0; j < 8; ++j) tile_sum += e[j];
                     }
-                    o[d].add(vf, pf);
+                    Frag<NP> rest[2];
+                    if constexpr (FINE) {
+                        e -= floats(pf.p[0]);
+                        rest[0] = split<NP>(e);
+                        rest[1] = split<NP>(e - floats(rest[0].p[0]));
+                    }
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        const Frag<NP> vf = vt.column(32 * i + 16 * c, 32 * d, lane);
+                        if constexpr (FINE) {
+                            small[d] = mfma(vf.p[0], rest[1].p[0], small[d]);
+                            small[d] = mfma(vf.p[0], rest[0].p[0], small[d]);
+                        }
+                        o[d].add(vf, pf);
+                    }
                 }
             }
-        }
-        sum += tile_sum;
+            sum += tile_sum;
 #pragma unroll
-        for (int d = 0; d < ND; ++d) {
-            o[d].join();
-            if constexpr (FINE) o[d].main += small[d];
-        }
+            for (int d = 0; d < ND; ++d) {
+                o[d].join();
+                if constexpr (FINE) o[d].main += small[d];
+            }
+        };
+        if (__builtin_expect(wide, 0)) weigh(std::true_type());
+        else weigh(std::false_type());
     }
     if (m >= p.M) return;
     sum += other_half(sum);
@@ -250,8 +254,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
             store4(out, 32 * d + 8 * r + 4 * half, p.D, x);
             if constexpr (FINE) store4(p.out_full + row * p.D, 32 * d + 8 * r + 4 * half, p.D, x);
         }
-    if (p.lse && half == 0)
-        p.lse[row] = sum == 0.f ? std::numeric_limits<float>::infinity() : ref + __log2f(sum);
+    if (half == 0) store_lse(p, row, ref, sum);
 }
 
 template <class T, int DP, int NW> int launch_fwd(const SmParams& p, hipStream_t st) {
@@ -311,7 +314,7 @@ __global__ __launch_bounds__(64 * COMBINE_ROWS) void softmax_combine(const SmPar
     const int m = (int)(row % p.M), head = (int)(row / p.M % p.H), b = (int)(row / p.M / p.H);
     store4((T*)p.out + b * p.so.b + head * p.so.h + m * p.so.r, d, p.D, x);
     if (p.out_full) store4(p.out_full + row * p.D, d, p.D, x);
-    if (p.lse && d == 0) p.lse[row] = sum == 0.f ? std::numeric_limits<float>::infinity() : ref + __log2f(sum);
+    if (d == 0) store_lse(p, row, ref, sum);
 }
 
 // The same for up to FEW_SPLITS splits, DP / 4 lanes a row (12 x 4096 rows of 2 splits: 23 us with a wave a row, 16 us
@@ -353,7 +356,7 @@ __global__ __launch_bounds__(256) void softmax_combine_few(const SmParams p) {
     const int m = (int)(row % p.M), head = (int)(row / p.M % p.H), b = (int)(row / p.M / p.H);
     store4((T*)p.out + b * p.so.b + head * p.so.h + m * p.so.r, d, p.D, x);
     if (p.out_full) store4(p.out_full + row * p.D, d, p.D, x);
-    if (p.lse && d == 0) p.lse[row] = sum == 0.f ? std::numeric_limits<float>::infinity() : ref + __log2f(sum);
+    if (d == 0) store_lse(p, row, ref, sum);
 }
 
 template <class T, int DP> int launch_combine(const SmParams& p, hipStream_t st) {

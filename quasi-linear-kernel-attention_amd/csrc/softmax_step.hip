@@ -219,7 +219,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p
             ((T*)p.out)[at] = (T)x;
             if (p.out_full) p.out_full[row * p.D + c] = x;
         }
-        if (p.lse && c == 0) p.lse[row] = s == 0.f ? std::numeric_limits<float>::infinity() : ref + __log2f(s);
+        if (c == 0) store_lse(p, row, ref, s);
     }
 }
 

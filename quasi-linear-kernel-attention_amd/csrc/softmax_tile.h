@@ -79,6 +79,17 @@ template <int NP> struct Acc {
         }
         main = mfma(a.p[0], b.p[0], main);
     }
+    // the same sum, bit for bit, as add(b, a)
+    __device__ __forceinline__ void add_turned(const Frag<NP>& a, const Frag<NP>& b) {
+        if constexpr (NP == 3) {
+            rest = mfma(a.p[2], b.p[0], rest);
+            rest = mfma(a.p[0], b.p[2], rest);
+            rest = mfma(a.p[1], b.p[1], rest);
+            rest = mfma(a.p[1], b.p[0], rest);
+            rest = mfma(a.p[0], b.p[1], rest);
+        }
+        main = mfma(a.p[0], b.p[0], main);
+    }
     __device__ __forceinline__ void join() {
         if constexpr (NP == 3) main = main + rest;
     }
@@ -121,6 +132,17 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 __device__ __forceinline__ float fexp2(float x) { return __builtin_amdgcn_exp2f(x); }
+// A row's log sum, ref + log2(sum), in two floats: the second is what the first one's rounding drops. With a large ref that is
+// all of log2(sum), without which each of n equal keys would have the probability 1.
+__device__ __forceinline__ void store_lse(const SmParams& p, int64_t row, float ref, float sum) {
+    const float l = __log2f(sum), hi = ref + l, back = hi - ref;
+    if (p.lse) p.lse[row] = sum == 0.f ? __builtin_inff() : hi;
+    if (p.lse_low) p.lse_low[row] = sum == 0.f ? 0.f : (ref - (hi - back)) + (l - back);
+}
+// Whether a row's log sum is one to take off in two steps, after the score is rounded (WIDE).
+__device__ __forceinline__ bool large_lse(float lse) { return fabsf(lse) > WIDE && lse != __builtin_inff(); }
+// P of such a row from (score - lse) - lse_low: 1 at most, however the score was rounded here and in the forward
+__device__ __forceinline__ float at_most_0(float x) { return x > 0.f ? 0.f : x; }
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
 __device__ __forceinline__ int reg_row(int r) { return (r >> 2) * 8 + (r & 3); }   // + 4 (lane / 32)
 

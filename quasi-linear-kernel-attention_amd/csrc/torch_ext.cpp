@@ -456,7 +456,12 @@ qlka_softmax_args softmax_args(const SoftmaxCall& c, const std::vector<int>& bor
     return a;
 }
 
-// (out, out before its rounding to bfloat16, the rows' log sums); the last where a gradient will be wanted, the second where
+void set_lse(qlka_softmax_args& a, const Tensor& lse) {
+    a.lse = lse.data_ptr<float>();
+    a.lse_low = a.lse + lse.numel() / 2;
+}
+
+// (out, out before its rounding to bfloat16, the rows' log sums in two floats); the last where a gradient will be wanted, the second where
 // the table's will
 std::tuple<Tensor, Tensor, Tensor> softmax_forward(SoftmaxCall& c, bool train, bool train_table) {
     check_softmax(c);
@@ -471,8 +476,8 @@ std::tuple<Tensor, Tensor, Tensor> softmax_forward(SoftmaxCall& c, bool train, b
     a.out = out.data_ptr();
     set_strides(a.out_stride, out);
     if (train) {
-        lse = at::empty({a.B, a.H, a.M}, c.q.options().dtype(at::kFloat));
-        a.lse = lse.data_ptr<float>();
+        lse = at::empty({2, a.B, a.H, a.M}, c.q.options().dtype(at::kFloat));
+        set_lse(a, lse);
         if (a.dtype == QLKA_BF16 && train_table) {
             full = at::empty({a.B, a.H, a.M, a.D}, lse.options());
             a.out_full = full.data_ptr<float>();
@@ -518,7 +523,7 @@ struct SoftmaxFn : public torch::autograd::Function<SoftmaxFn> {
         a.out = out.data_ptr();
         set_strides(a.out_stride, out);
         if (full.defined()) a.out_full = full.data_ptr<float>();
-        a.lse = lse.data_ptr<float>();
+        set_lse(a, lse);
         a.g_out = g.data_ptr();
         set_strides(a.g_out_stride, g);
         if (ctx->needs_input_grad(0)) {

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from oracle import softmax as oracle
-from test_gpu_softmax import BF16, F32, check, make, run
+from test_gpu_softmax import BF16, BOTH, F32, PAST, check, make, reference, run
 
 pytestmark = pytest.mark.gpu
 
@@ -88,3 +88,87 @@ def test_equal_products_stay_equal(dev, M, dtype):
     t["k"] = row[torch.rand(t["k"].shape, generator=gen).argsort(-1)].to(dtype)
     want = equal_scores(t, torch.ones(2, M, 200, dtype=torch.bool), 1e9)
     check(run(dev, t, train=False, scale=1e9), want, ["out"])
+
+
+@TYPES
+@pytest.mark.parametrize("scale,bias", [(0.125, -1e38), (0.125, -4.5e37), (2.0 ** -96, 1e10), (2.0 ** -96, -1e10), (2.0 ** -90, 1e12)])
+def test_log_sums_far_larger_than_the_scale(dev, scale, bias, dtype):
+    """Rows of one key: its probability is 1 whatever its score."""
+    t = make(2, 4, 2, 40, 1, 64, dtype, seed=1, bias=PAST)
+    t["table"].fill_(bias)
+    want = equal_scores(t, torch.ones(2, 40, 1, dtype=torch.bool), scale)
+    check(run(dev, t, PAST, scale=scale), want, ["out", "gq", "gk", "gv"])
+
+
+@TYPES
+@pytest.mark.parametrize("M,N,causal", [(1, 50, False), (40, 50, False), (70, 300, True), (3, 4100, False), (600, 65, False)])
+@pytest.mark.parametrize("scale,bias", [(0.125, -1e38), (0.125, 2e38), (0.125, -1e30), (2.0 ** -96, 1e10)])
+def test_biases_that_swallow_the_scores(dev, scale, bias, M, N, causal, dtype):
+    """A bias so large that scores next to it are all the same: n keys share a row by 1 / n each, in the gradients too."""
+    t = make(2, 4, 2, M, N, 64, dtype, seed=1, bias=PAST, keep="random")
+    t["table"].fill_(bias)
+    start = N - M if causal else 0
+    want = equal_scores(t, oracle.visible(2, M, N, t["keep"], causal, start), scale)
+    check(run(dev, t, PAST, scale=scale, causal=causal, start=start), want, ["out", "gq", "gk", "gv"])
+
+
+@TYPES
+@pytest.mark.parametrize("M,N", [(40, 256), (200, 300), (1, 300)])
+@pytest.mark.parametrize("scale", [2.0 ** 12, 2.0 ** 22, 2.0 ** 30, 2.0 ** 96])
+@pytest.mark.parametrize("masked", [False, True], ids=["all", "keep"])
+def test_large_scales_gradients(dev, scale, M, N, masked, dtype):
+    t = whole(make(2, 1, 1, M, N, 64, dtype, seed=M, keep="random" if masked else None))
+    t["g"] = t["g"] * 2.0 ** -40                   # so that the largest scale's gradients stay in range
+    top = largest(t, oracle.visible(2, M, N, t["keep"]))
+    check(run(dev, t, scale=scale), equal_scores(t, top[:, 0], scale))
+
+
+@TYPES
+@pytest.mark.parametrize("bias", [None, BOTH], ids=["plain", "bias"])
+@pytest.mark.parametrize("size", [200.0, 3000.0])
+@pytest.mark.parametrize("M,N", [(2, 90), (150, 200)])
+def test_scores_of_thousands(dev, M, N, size, bias, dtype):
+    """Where the log sums begin to be taken off in two steps: all values against the oracle."""
+    t = make(2, 4, 2, M, N, 64, dtype, seed=6, bias=bias)
+    if bias:
+        t["table"] += size
+        check(run(dev, t, bias), reference(t, bias))
+    scale = size / 16
+    t = dict(t, table=None)
+    check(run(dev, t, scale=scale), reference(t, scale=scale))
+
+
+@TYPES
+@pytest.mark.parametrize("M", [1, 3, 70])
+def test_gradients_of_large_scales_stay_finite(dev, M, dtype):
+    """Scores whose roundings are larger than 1, formed once in the forward and again in the backward: no probability is
+    larger than 1, so a value's gradient is at most the sum of its queries'."""
+    t = make(2, 2, 2, M, 700, 64, dtype, seed=3)
+    for scale in (2.0 ** 20, 2.0 ** 24, 2.0 ** 31):
+        got = run(dev, t, scale=scale)
+        for n in got:
+            assert torch.isfinite(got[n]).all(), (n, scale)
+        most = t["g"].double().abs().sum(2, keepdim=True)
+        assert (got["gv"].double().cpu().abs() <= most * (1 + 2 ** -7)).all(), scale
+
+
+def test_backward_without_the_second_part_of_the_log_sums(dev):
+    """The C entries with lse alone: what they gave before lse_low was there, right for log sums of the ordinary size."""
+    import ctypes
+
+    from qlka import _lib
+    lib = _lib.load()
+    t = make(2, 2, 2, 50, 70, 64, F32, seed=2)
+    want = reference(t)
+    x = {n: t[n].to(dev) for n in "qkvg"}
+    r = {n: torch.empty_like(x[m]) for n, m in (("out", "q"), ("g_q", "q"), ("g_k", "k"), ("g_v", "v"))}
+    lse = torch.empty(2, 2, 50, device=dev)
+    a = _lib.SoftmaxArgs(dtype=0, B=2, H=2, G=2, M=50, N=70, D=64, scale=0.125, lse=lse.data_ptr(), g_out=x["g"].data_ptr())
+    for n, y in [(n, x[n]) for n in "qkv"] + [("g_out", x["g"])] + list(r.items()):
+        setattr(a, n, y.data_ptr())
+        setattr(a, n + "_stride", (ctypes.c_int64 * 3)(*y.stride()[:3]))
+    stream = torch.cuda.current_stream().cuda_stream
+    for fn, need in ((lib.qlka_softmax_fwd, lib.qlka_softmax_fwd_ws_bytes), (lib.qlka_softmax_bwd, lib.qlka_softmax_bwd_ws_bytes)):
+        ws = torch.empty(max(need(ctypes.byref(a)), 16), dtype=torch.uint8, device=dev)
+        assert fn(ctypes.byref(a), ws.data_ptr(), ws.numel(), stream) == 0
+    check({"out": r["out"], "gq": r["g_q"], "gk": r["g_k"], "gv": r["g_v"]}, want)

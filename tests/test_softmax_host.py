@@ -240,7 +240,7 @@ def test_launches_past_2_32_threads_are_refused(lib):
     nothing = dict(g_q=None, g_k=None, g_v=None)
     for wanted in (dict(g_q=1 << 12), dict(g_k=1 << 12, g_v=1 << 12)):                          # two waves a workgroup
         refused(lib, lib.qlka_softmax_bwd, many, **{**one, **nothing, **wanted}, B=1 << 25, M=1, N=1)
-    wide = {**one, **nothing, "D": 128, "B": 1 << 20, "M": 1 << 9, "N": 0}                       # row sums: 16 lanes a row
+    wide = {**one, **nothing, "B": 1 << 26, "M": 1, "N": 0}                                     # row sums: a wave 32 rows
     refused(lib, lib.qlka_softmax_bwd, many, **wide)
     refused(lib, lib.qlka_softmax_bwd, many, H=1 << 24, G=1, B=1, M=0, N=1, D=8, g_q=None, g_k=None, g_v=None, table=1 << 12,
             g_table=1 << 12, border=[1])                                                       # a workgroup a head and bucket
