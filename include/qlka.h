@@ -246,7 +246,7 @@ int qlka_layer_fwd_masked(int kind, const float* q, const float* k, const float*
  * start), keys after the query (d > 0) in buckets num_borders + 1 on, 2 (num_borders + 1) buckets in all. Else distance
  * max(-d, 0) and num_borders + 1 buckets. table and g_table are (buckets, H) fp32, contiguous.
  *
- * Forward: writes out and, where not NULL, lse (B, H, M) (log2 of each row's sum, +inf for a row without keys), lse_low
+ * Forward: writes out and, where not NULL, lse (B, H, M) (half the log2 of each row's sum, +inf for a row without keys), lse_low
  * (B, H, M) (what of it lies below lse's last place: where scores are large, the log of the number of keys that share a
  * row) and out_full (with QLKA_BF16 and a table: (B, H, M, D) fp32, out before it is rounded; the probabilities are then taken
  * whole). Backward: reads q, k, v, out, lse, g_out and, where not NULL, lse_low and out_full, writes g_q (may be NULL), g_k and g_v

@@ -19,6 +19,9 @@ namespace sm {
 
 constexpr float HIGH = std::numeric_limits<float>::infinity();
 
+// Twice a bias that a whole tile has, finite where it is above: a row past the last one adds -inf to it
+__device__ __forceinline__ float far_twice(float x) { return fminf(2.f * x, std::numeric_limits<float>::max()); }
+
 // delta, a wave 32 rows of a head, DP / 8 lanes a row; and whether one of the 32 has a large log sum
 template <class T, int DP>
 __global__ __launch_bounds__(256) void softmax_delta(const SmParams p) {
@@ -185,7 +188,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
     if constexpr (NP == 1) any_large = __syncthreads_or(large);
     else if constexpr (BIAS) __syncthreads();
 
-    const float c2 = p.scale * LOG2E;
+    const float c1 = p.scale * UNIT;
     Acc<NP> dq[ND];
 
     const auto go = [&](auto all_wide) {
@@ -223,7 +226,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
         const bool edge = p.causal && n0 + BN - 1 > mw + p.start;
         const int lim = m + p.start - n0 - 4 * half;                     // at an edge, the last key seen
         const float* nb = &near_here[BIAS ? ROWS - 1 - wave * 32 - col + 4 * half : 0];
-        const float off = wide ? 0.f : lse, add = far - off;
+        const float off = wide ? 0.f : lse, add = far_twice(far - off);
         // `count` halves of the tile together: the products of one are under way while the other's scores are worked on
         const auto halves = [&](auto first, auto count) {
             f32x16 s[count], dp[count];
@@ -247,17 +250,25 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
             }
 #pragma unroll
             for (int i = 0; i < count; ++i) {
-                if (BIAS && fb < 0) {
+                // to twice the scores less the row's log sum
+                if (wide || (BIAS && fb < 0)) {
+                    if (BIAS && fb < 0) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c2, nb[32 * (first + i) + reg_row(r)] - off);
+                        for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c1, nb[32 * (first + i) + reg_row(r)] - off);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c1, far);
+                    }
+                    if (wide) {
+                        const float low = m < p.M && p.lse_low ? p.lse_low[row] : 0.f;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[i][r] = at_most_0((s[i][r] - lse) - low);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[i][r] += s[i][r];
                 } else {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c2, add);
-                }
-                if (wide) {
-                    const float low = m < p.M && p.lse_low ? p.lse_low[row] : 0.f;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[i][r] = at_most_0((s[i][r] - lse) - low);
+                    for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], 2.f * c1, add);
                 }
                 if (bits != PairT::ALL) s[i] = masked(s[i], mask, 32 * (first + i) + 4 * half);
 #pragma unroll
@@ -394,9 +405,9 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
         any_large = __syncthreads_or(any_large);
     }
 
-    const float c2 = p.scale * LOG2E;
+    const float c1 = p.scale * UNIT;
     Acc<NP> dk[ND], dv[ND];
-    const float per_c2 = 1.f / c2;
+    const float per_c1 = 1.f / c1;
     int filled = -1;                                   // the head whose bias stands in LDS
 
     const auto go = [&](auto all_wide) {
@@ -416,7 +427,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
             const bool wide = NP == 3 ? __any(large_lse(ls)) : all_wide;      // all rows are in the first wave
             if (NP == 3 && tid == 0) wide_of = wide;
             if (tid < BM) {
-                lse[tid] = wide ? 0.f : -ls * per_c2;
+                lse[tid] = wide ? 0.f : -ls * per_c1;
                 delta[tid] = -des;
                 if (wide) {
                     two[0][tid] = ls;
@@ -445,6 +456,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
         const bool edge = p.causal && m0 + p.start < nw + 31;
         const int lim = edge ? n - p.start - m0 - 4 * half : -1;         // the first query that sees the key
         const float* nb = &near_here[BIAS ? wave * 32 + col + BM - 1 - 4 * half : 0];
+        const float add = far_twice(far);
         const auto halves = [&](auto first, auto count) {
             // scores less the row's log sum (in units of the scores; a large one later), and dP less delta
             f32x16 s[count], dp[count];
@@ -469,20 +481,27 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
             const bool wide = NP == 3 ? __builtin_amdgcn_readfirstlane(wide_of) : all_wide;
 #pragma unroll
             for (int i = 0; i < count; ++i) {
-                if (BIAS && near) {
+                // to twice the scores less the row's log sum
+                if (wide || (BIAS && near)) {
+                    if (BIAS && near) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c2, nb[-32 * (first + i) - reg_row(r)]);
-                } else if (BIAS || !wide) {
+                        for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c1, nb[-32 * (first + i) - reg_row(r)]);
+                    } else {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c2, far);
-                }
-                if (wide) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int row = 32 * (first + i) + 4 * half + reg_row(r);
-                        const float x = BIAS ? s[i][r] : __builtin_fmaf(s[i][r], c2, far);     // apart from the above: fewer spills
-                        s[i][r] = at_most_0((x - two[0][row]) - two[1][row]);
+                        for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c1, far);
                     }
+                    if (wide) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int row = 32 * (first + i) + 4 * half + reg_row(r);
+                            s[i][r] = at_most_0((s[i][r] - two[0][row]) - two[1][row]);
+                        }
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[i][r] += s[i][r];
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], 2.f * c1, add);
                 }
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {

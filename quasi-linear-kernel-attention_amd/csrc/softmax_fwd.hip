@@ -25,7 +25,7 @@
 namespace qlka {
 namespace sm {
 
-constexpr float GROW = 8.f;
+constexpr float GROW = 4.f;          // 2^8 of the exponentials
 
 template <class T, int DP, int NW, bool BIAS, bool FINE>
 __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(const SmParams p) {
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
         __syncthreads();
     }
 
-    const float c2 = p.scale * LOG2E;
+    const float c1 = p.scale * UNIT;
     Acc<NP> o[ND];
     float top = -std::numeric_limits<float>::infinity(), ref = 0.f, sum = 0.f;
     bool wide = false;                                 // a row here has a large ref
@@ -119,8 +119,8 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
             s[i] = a.main;
         }
 
-        // scores in log2 units are fma(s, mul, add) from here on
-        float mul = c2, add = far;
+        // scores are fma(s, mul, add) from here on
+        float mul = c1, add = far;
         const bool edge = p.causal && n0 + BN - 1 > mw + p.start, all = bits == PairT::ALL;
         if (near || edge || !all) {
             const float* nb = &near_here[BIAS ? ROWS - 1 - wave * 32 - col + 4 * half : 0];
@@ -128,12 +128,12 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
 #pragma unroll
                 for (int i = 0; i < NS; ++i)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c2, nb[32 * i + reg_row(r)]);
+                    for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c1, nb[32 * i + reg_row(r)]);
             } else {
 #pragma unroll
                 for (int i = 0; i < NS; ++i)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c2, far);
+                    for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c1, far);
             }
             if (!all) {
 #pragma unroll
@@ -163,7 +163,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
             top = fmaxf(top, hi);
             ref = top == -std::numeric_limits<float>::infinity() ? 0.f : top;
             wide = __any(fabsf(ref) > WIDE);
-            const float f = first ? 1.f : fexp2(was - ref);               // the first time there is nothing to scale
+            const float f = first ? 1.f : exp_of(was - ref);              // the first time there is nothing to scale
             sum *= f;
 #pragma unroll
             for (int d = 0; d < ND; ++d) o[d].main *= f;
@@ -174,10 +174,11 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
                 for (int i = 0; i < NS; ++i)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], mul, add) - ref;
-                mul = 1.f;
+                mul = 2.f;
                 add = 0.f;
             } else {
-                add -= ref;
+                mul *= 2.f;
+                add = 2.f * (add - ref);
             }
             float tile_sum = 0.f;                          // summed by tiles: thousands of terms one by one lose two digits more
             f32x16 small[ND];                              // FINE: the smaller parts apart, as in Acc
@@ -293,7 +294,7 @@ __global__ __launch_bounds__(64 * COMBINE_ROWS) void softmax_combine(const SmPar
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < LOOK; ++i) {
-        const float f = fexp2(a[i].x - ref);
+        const float f = exp_of(a[i].x - ref);
         if (lane + 64 * i < p.splits) weight[wave][lane + 64 * i] = f;
         sum += a[i].y * f;
     }
@@ -348,7 +349,7 @@ __global__ __launch_bounds__(256) void softmax_combine_few(const SmParams p) {
     f32x4 x = {};
 #pragma unroll
     for (int s = 0; s < FEW_SPLITS; ++s) {
-        const float f = fexp2(a[s].x - ref);
+        const float f = exp_of(a[s].x - ref);
         sum += a[s].y * f;
         x = x + y[s] * f;
     }

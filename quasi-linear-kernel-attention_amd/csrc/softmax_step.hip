@@ -101,7 +101,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p
             q[r] = floats(load_seg((const T*)p.q + b * p.sq.b + head * p.sq.h + m * p.sq.r, d, p.D)) * p.q_sign;
             if constexpr (BIAS)
                 for (int i = tid; i < (p.bk.n + 1) * (p.bk.both ? 2 : 1); i += NT)
-                    table[r][i] = p.table[(int64_t)i * p.H + head] * LOG2E;
+                    table[r][i] = p.table[(int64_t)i * p.H + head] * UNIT;
         }
     }
     if constexpr (BIAS) {
@@ -109,7 +109,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p
         __syncthreads();
     }
 
-    const float c2 = p.scale * LOG2E;
+    const float c1 = p.scale * UNIT;
     int near_tile = -1;
     while (at.t < t1) {
         const Place after = next(at);
@@ -150,17 +150,17 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p
             for (int u = 0; u < U; ++u) {
                 const int n = at.u0 + u * KEYS + group;
                 // scaled after the sum, as in the tiles: equal products stay equal however large the scale is
-                x[r][u] = __builtin_fmaf(x[r][u], c2, BIAS ? fb >= 0 ? table[r][fb] : near_bias[wave][r][n] : 0.f);
+                x[r][u] = __builtin_fmaf(x[r][u], c1, BIAS ? fb >= 0 ? table[r][fb] : near_bias[wave][r][n] : 0.f);
                 if (!(at.bits >> n & 1) || (p.causal && n0 + n > seat)) x[r][u] = LOW;
                 hi = fmaxf(hi, x[r][u]);
             }
-            const float to = fmaxf(top[r], hi), ref = to == LOW ? 0.f : to, f = fexp2(top[r] - ref);
+            const float to = fmaxf(top[r], hi), ref = to == LOW ? 0.f : to, f = exp_of(top[r] - ref);
             top[r] = to;
             sum[r] *= f;
             o[r] *= f;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const float e = fexp2(x[r][u] - ref);
+                const float e = exp_of(x[r][u] - ref);
                 sum[r] += e;
                 o[r] += floats(rows_here.v[u]) * e;
             }
@@ -174,7 +174,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p
 #pragma unroll
         for (int far = LANES; far < 64; far *= 2) {
             const float top2 = __shfl_xor(top[r], far), to = fmaxf(top[r], top2), ref = to == LOW ? 0.f : to;
-            const float f = fexp2(top[r] - ref), f2 = fexp2(top2 - ref);
+            const float f = exp_of(top[r] - ref), f2 = exp_of(top2 - ref);
             sum[r] = sum[r] * f + __shfl_xor(sum[r], far) * f2;
 #pragma unroll
             for (int i = 0; i < 8; ++i) o[r][i] = o[r][i] * f + __shfl_xor(o[r][i], far) * f2;
@@ -200,7 +200,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p
         float s = 0.f, x = 0.f;
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
-            const float f = fexp2(join_m[i][r] - ref);
+            const float f = exp_of(join_m[i][r] - ref);
             s += join_s[i][r] * f;
             x += join_o[i][r][c] * f;
         }

@@ -30,11 +30,13 @@ typedef __attribute__((ext_vector_type(8))) float f32x8;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 
-constexpr float LOG2E = 1.4426950408889634f;
-// Where a row's reference (its maximum, its log sum) is larger, in log2 units, scores are rounded before it is taken off: it is
-// a rounded score itself, and the exact product in fma(score, scale, bias - reference) would be off from it by up to half its
-// last place, which is 2^-14 here and grows to any factor of the exponential.
-constexpr float WIDE = 1024.f;
+// Scores, biases and log sums are held in units of 2 ln 2, halves of a power of two: x ln 2 units are larger than x, and the
+// lowest finite bias, with which a bucket is hidden, would become -inf. exp2 of the double is e to the score.
+constexpr float UNIT = 0.72134752044448170f;
+// Where a row's reference (its maximum, its log sum) is larger, scores are rounded before it is taken off: it is a rounded score
+// itself, and the exact product in fma(score, scale, bias - reference) would be off from it by up to half its last place,
+// which is 2^-15 here and grows to any factor of the exponential.
+constexpr float WIDE = 512.f;
 
 template <class T> struct Elem;
 template <> struct Elem<__bf16> { static constexpr int PARTS = 1; typedef bf16x8 seg; };
@@ -132,10 +134,10 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 __device__ __forceinline__ float fexp2(float x) { return __builtin_amdgcn_exp2f(x); }
-// A row's log sum, ref + log2(sum), in two floats: the second is what the first one's rounding drops. With a large ref that is
-// all of log2(sum), without which each of n equal keys would have the probability 1.
+// A row's log sum, ref + log2(sum) / 2, in two floats: the second is what the first one's rounding drops. With a large ref that
+// is all of log2(sum), without which each of n equal keys would have the probability 1.
 __device__ __forceinline__ void store_lse(const SmParams& p, int64_t row, float ref, float sum) {
-    const float l = __log2f(sum), hi = ref + l, back = hi - ref;
+    const float l = 0.5f * __log2f(sum), hi = ref + l, back = hi - ref;
     if (p.lse) p.lse[row] = sum == 0.f ? __builtin_inff() : hi;
     if (p.lse_low) p.lse_low[row] = sum == 0.f ? 0.f : (ref - (hi - back)) + (l - back);
 }
@@ -143,6 +145,8 @@ __device__ __forceinline__ void store_lse(const SmParams& p, int64_t row, float 
 __device__ __forceinline__ bool large_lse(float lse) { return fabsf(lse) > WIDE && lse != __builtin_inff(); }
 // P of such a row from (score - lse) - lse_low: 1 at most, however the score was rounded here and in the forward
 __device__ __forceinline__ float at_most_0(float x) { return x > 0.f ? 0.f : x; }
+// e to a score
+__device__ __forceinline__ float exp_of(float x) { return fexp2(x + x); }
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
 __device__ __forceinline__ int reg_row(int r) { return (r >> 2) * 8 + (r & 3); }   // + 4 (lane / 32)
 
@@ -380,13 +384,13 @@ template <int BN> struct KeyBits {
     }
 };
 
-// The bias of one head in LDS: its column of the table in log2 units, and the borders.
+// The bias of one head in LDS: its column of the table, and the borders.
 struct BiasLds {
     float value[QLKA_MAX_BUCKETS];
     int border[QLKA_MAX_BUCKETS];
     __device__ __forceinline__ void fill(const SmParams& p, int head, int tid, int nt) {
         const int nb = (p.bk.n + 1) * (p.bk.both ? 2 : 1);
-        for (int i = tid; i < nb; i += nt) value[i] = p.table[(int64_t)i * p.H + head] * LOG2E;
+        for (int i = tid; i < nb; i += nt) value[i] = p.table[(int64_t)i * p.H + head] * UNIT;
         for (int i = tid; i < p.bk.n; i += nt) border[i] = p.bk.border[i];
     }
 };

@@ -172,3 +172,38 @@ def test_backward_without_the_second_part_of_the_log_sums(dev):
         ws = torch.empty(max(need(ctypes.byref(a)), 16), dtype=torch.uint8, device=dev)
         assert fn(ctypes.byref(a), ws.data_ptr(), ws.numel(), stream) == 0
     check({"out": r["out"], "gq": r["g_q"], "gk": r["g_k"], "gv": r["g_v"]}, want)
+
+
+def highest(t, see, start, bias):
+    """(B, H, M, N): the keys of the largest bias that a row sees."""
+    B, M, N = see.shape
+    value = t["table"].t()[:, oracle.bucket_map(M, N, start, *bias).flatten()].view(1, -1, M, N).expand(B, -1, M, N)
+    value = value.masked_fill(~see[:, None], float("-inf"))
+    return see[:, None] & (value == value.amax(-1, keepdim=True))
+
+
+LOWEST, LOWEST_BF16 = torch.finfo(F32).min, torch.finfo(BF16).min
+TABLES = {
+    "lowest": lambda n: [LOWEST] * n, "lowest_bf16": lambda n: [LOWEST_BF16] * n, "largest": lambda n: [-LOWEST] * n,
+    # which of two is the larger one has to be seen where both are below -2.36e38
+    "two": lambda n: [LOWEST if i % 3 else LOWEST_BF16 for i in range(n)],
+    "close": lambda n: [-2.5e38 if i % 2 else -2.4e38 for i in range(n)],
+    "both_ends": lambda n: [LOWEST if i % 2 else -LOWEST for i in range(n)],
+    "hidden": lambda n: [0.0] + [LOWEST] * (n - 1),
+}
+
+
+@TYPES
+@pytest.mark.parametrize("M,N,causal", [(1, 50, True), (2, 300, False), (40, 50, False), (130, 300, True), (3, 4100, True), (600, 65, False)])
+@pytest.mark.parametrize("kind", TABLES)
+def test_biases_as_low_and_as_large_as_they_may_be(dev, kind, M, N, causal, dtype):
+    """A bucket of the type's lowest value hides its keys from rows that see others, and not from those that do not: these
+    see equal scores. "hidden" leaves some rows one bucket of ordinary scores (the queries are 0 there, so they are equal)."""
+    t = make(2, 2, 2, M, N, 64, dtype, seed=1, bias=PAST, keep="random")
+    t["table"] = torch.tensor(TABLES[kind](32))[:, None].repeat(1, 2)
+    if kind == "hidden":
+        t["q"] = torch.zeros_like(t["q"])
+    start = N - M if causal else 0
+    see = oracle.visible(2, M, N, t["keep"], causal, start)
+    top = highest(t, see, start, PAST)[:, 0]
+    check(run(dev, t, PAST, scale=0.125, causal=causal, start=start), equal_scores(t, top, 0.125), ["out", "gq", "gk", "gv"])
