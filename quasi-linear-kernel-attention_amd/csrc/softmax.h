@@ -28,6 +28,7 @@ struct SmParams {
     const void *q, *k, *v, *g_out;
     void *out, *g_q, *g_k, *g_v;
     float* out_full;                         // [B][H][M][D], or null
+    int table_kept;                          // the table will have no gradient
     SmStrides sq, sk, sv, so, sg, sgq, sgk, sgv;
     const uint8_t* keep;                     // [B] rows of N bytes, keep_stride apart, or null
     int64_t keep_stride;

@@ -186,7 +186,7 @@ int check_rows(const qlka_softmax_args* a, const char* name, const void* x, cons
 int params(const qlka_softmax_args* a, SmParams* p) {
     *p = SmParams{};
     p->q = a->q; p->k = a->k; p->v = a->v; p->g_out = a->g_out;
-    p->out = a->out; p->out_full = a->out_full;
+    p->out = a->out; p->out_full = a->out_full; p->table_kept = a->table_kept;
     p->g_q = a->g_q; p->g_k = a->g_k; p->g_v = a->g_v;
     p->sq = strides(a->q_stride); p->sk = strides(a->k_stride); p->sv = strides(a->v_stride);
     p->so = strides(a->out_stride); p->sg = strides(a->g_out_stride);
@@ -243,7 +243,7 @@ int qlka_softmax_fwd(const qlka_softmax_args* a, void* ws, size_t ws_bytes, void
     if (int e = params(a, &p)) return e;
     if (a->B == 0 || a->M == 0) return QLKA_OK;
     if (!a->q || !a->out || (a->N > 0 && (!a->k || !a->v))) return refuse("q, k, v and out must be non-null");
-    if (a->out_full && (a->dtype == QLKA_F32 || !a->table)) return refuse("out_full goes with QLKA_BF16 and a table");
+    if (a->out_full && a->dtype == QLKA_F32) return refuse("out_full goes with QLKA_BF16");
     const FwdPlan f = fwd_plan(a);
     if (int e = need_ws(ws, ws_bytes, f.part + f.part2)) return e;
     const int64_t heads = (int64_t)a->B * (f.step ? a->G : a->H);
@@ -284,7 +284,7 @@ int qlka_softmax_bwd(const qlka_softmax_args* a, void* ws, size_t ws_bytes, void
     const bool rows = (int64_t)a->B * a->M > 0, keys = (int64_t)a->B * a->N > 0;
     if (rows && (!a->q || !a->out || !a->lse || !a->g_out)) return refuse("q, out, lse and g_out must be non-null");
     if (keys && (!a->k || !a->v)) return refuse("k and v must be non-null");
-    if (a->out_full && (a->dtype == QLKA_F32 || !a->table)) return refuse("out_full goes with QLKA_BF16 and a table");
+    if (a->out_full && a->dtype == QLKA_F32) return refuse("out_full goes with QLKA_BF16");
     if (rows && a->g_table && a->dtype == QLKA_BF16 && !a->out_full) return refuse("g_table needs out_full with QLKA_BF16");
     const BwdPlan w = bwd_plan(a, a->g_q, a->g_k, a->g_table);
     if (int e = need_ws(ws, ws_bytes, w.bytes())) return e;

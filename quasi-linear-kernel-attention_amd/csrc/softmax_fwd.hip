@@ -253,14 +253,14 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
         for (int r = 0; r < 4; ++r) {
             const f32x4 x = quad(o[d].main, r) * inv;
             store4(out, 32 * d + 8 * r + 4 * half, p.D, x);
-            if constexpr (FINE) store4(p.out_full + row * p.D, 32 * d + 8 * r + 4 * half, p.D, x);
+            if (p.out_full) store4(p.out_full + row * p.D, 32 * d + 8 * r + 4 * half, p.D, x);
         }
     if (half == 0) store_lse(p, row, ref, sum);
 }
 
 template <class T, int DP, int NW> int launch_fwd(const SmParams& p, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)p.B * p.H * p.blocks * p.splits));
-    if (sizeof(T) == 2 && p.out_full) softmax_fwd<T, DP, NW, true, sizeof(T) == 2><<<grid, 64 * NW, 0, st>>>(p);
+    if (sizeof(T) == 2 && p.table && p.out_full && !p.table_kept) softmax_fwd<T, DP, NW, true, sizeof(T) == 2><<<grid, 64 * NW, 0, st>>>(p);
     else if (p.table) softmax_fwd<T, DP, NW, true, false><<<grid, 64 * NW, 0, st>>>(p);
     else softmax_fwd<T, DP, NW, false, false><<<grid, 64 * NW, 0, st>>>(p);
     return (int)hipGetLastError();

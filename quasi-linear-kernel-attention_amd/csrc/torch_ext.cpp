@@ -461,9 +461,9 @@ void set_lse(qlka_softmax_args& a, const Tensor& lse) {
     a.lse_low = a.lse + lse.numel() / 2;
 }
 
-// (out, out before its rounding to bfloat16, the rows' log sums in two floats); the last where a gradient will be wanted, the second where
-// the table's will
-std::tuple<Tensor, Tensor, Tensor> softmax_forward(SoftmaxCall& c, bool train, bool train_table) {
+// (out, out before its rounding to bfloat16, the rows' log sums in two floats); the last where a gradient will be wanted,
+// the second where one through the scores will (v's needs none)
+std::tuple<Tensor, Tensor, Tensor> softmax_forward(SoftmaxCall& c, bool train, bool train_scores, bool train_table) {
     check_softmax(c);
     c10::DeviceGuard guard(c.q.device());
     c.q = packed_rows(c.q);
@@ -478,7 +478,8 @@ std::tuple<Tensor, Tensor, Tensor> softmax_forward(SoftmaxCall& c, bool train, b
     if (train) {
         lse = at::empty({2, a.B, a.H, a.M}, c.q.options().dtype(at::kFloat));
         set_lse(a, lse);
-        if (a.dtype == QLKA_BF16 && train_table) {
+        if (a.dtype == QLKA_BF16 && train_scores) {
+            a.table_kept = !train_table;
             full = at::empty({a.B, a.H, a.M, a.D}, lse.options());
             a.out_full = full.data_ptr<float>();
         }
@@ -497,7 +498,8 @@ struct SoftmaxFn : public torch::autograd::Function<SoftmaxFn> {
         const Tensor table = table_.value_or(Tensor()), keep = keep_.value_or(Tensor());
         SoftmaxCall c{q, k, v, table, keep, scale, causal, start, border, both};
         Tensor out, full, lse;
-        std::tie(out, full, lse) = softmax_forward(c, true, table.defined() && table.requires_grad());
+        const bool train_table = table.defined() && table.requires_grad();
+        std::tie(out, full, lse) = softmax_forward(c, true, q.requires_grad() || k.requires_grad() || train_table, train_table);
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["causal"] = causal;
         ctx->saved_data["start"] = start;
@@ -564,7 +566,7 @@ Tensor softmax_attention(const Tensor& q, const Tensor& k, const Tensor& v, cons
                                        (t.defined() && t.requires_grad())))
         return SoftmaxFn::apply(q, k, v, table, keep, scale, causal, start, border, both);
     SoftmaxCall c{q, k, v, t, m, scale, causal, start, border, both};
-    return std::get<0>(softmax_forward(c, false, false));
+    return std::get<0>(softmax_forward(c, false, false, false));
 }
 
 struct BiasMapFn : public torch::autograd::Function<BiasMapFn> {

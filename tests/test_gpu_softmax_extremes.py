@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from oracle import softmax as oracle
+from qlka.softmax import softmax_attention
 from test_gpu_softmax import BF16, BOTH, F32, PAST, check, make, reference, run
 
 pytestmark = pytest.mark.gpu
@@ -207,3 +208,22 @@ def test_biases_as_low_and_as_large_as_they_may_be(dev, kind, M, N, causal, dtyp
     see = oracle.visible(2, M, N, t["keep"], causal, start)
     top = highest(t, see, start, PAST)[:, 0]
     check(run(dev, t, PAST, scale=0.125, causal=causal, start=start), equal_scores(t, top, 0.125), ["out", "gq", "gk", "gv"])
+
+
+@pytest.mark.parametrize("M,N", [(1, 300), (40, 300), (200, 65), (3, 5000)])
+def test_row_sums_of_unrounded_values(dev, M, N):
+    """The row sums that the gradients take off, rowsum(dO * O), are formed from out before it is rounded to bfloat16. Scores are
+    equal, so that no probability is rounded and out before its rounding is right to fp32; the bounds are then those
+    with a table. Values and keys far from 0 show an error that is common to a row's dS."""
+    t = make(2, 4, 2, M, N, 64, BF16, seed=9)
+    t["q"] = torch.zeros_like(t["q"])
+    t["k"] = (t["k"].float() / 8 + 4).to(BF16)
+    t["v"] = (t["v"].float() / 8 + 8).to(BF16)
+    zeros, none = torch.zeros(1, 4), torch.zeros(M, N, dtype=torch.long)
+    want = oracle.attention(t["q"], t["k"], t["v"], 0.125, oracle.visible(2, M, N), t["g"], zeros, none)
+    check(run(dev, t), want)
+    kept = dict(t, table=torch.zeros(32, 4))                          # with a table that wants no gradient
+    x = {n: kept[n].to(dev).requires_grad_(n in "qkv") for n in ("q", "k", "v", "g", "table")}
+    out = softmax_attention(x["q"], x["k"], x["v"], table=x["table"], buckets=PAST)
+    got = dict(zip(("gq", "gk", "gv"), torch.autograd.grad(out, [x[n] for n in "qkv"], x["g"].detach())), out=out.detach())
+    check(got, want)
