@@ -555,6 +555,9 @@ struct SoftmaxFn : public torch::autograd::Function<SoftmaxFn> {
 
 Tensor softmax_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& table, const OptTensor& keep,
                          double scale, bool causal, int64_t start, const std::vector<int64_t>& border, bool both) {
+    // a call without a gradient goes around the autograd function, which would refuse a tangent
+    for (const Tensor& t : {q, k, v, table.value_or(Tensor())})
+        TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "softmax_attention has no forward-mode derivative");
     if (q.dim() == 4 && k.dim() == 4 && v.dim() == 4 && q.size(3) % 8 && q.size(3) == k.size(3) && q.size(3) == v.size(3)) {
         // zeros up to a multiple of 8 change no product
         const auto padded = [&](const Tensor& t) { return at::constant_pad_nd(t, {0, 8 - t.size(3) % 8}); };

@@ -248,3 +248,17 @@ def test_bfloat16_table_and_numeric_mask(dev):
     table = x["table"].to(BF16).requires_grad_(True)
     out = softmax_attention(x["q"], x["k"], x["v"], keep=keep, table=table, buckets=bias)
     assert torch.autograd.grad(out, table, x["g"])[0].dtype == BF16
+
+
+def test_forward_mode_is_refused(dev):
+    import torch.autograd.forward_ad as fwAD
+    x = leaves(dev, 1, 2, 2, 10, 12, 32, F32, RelativeBuckets())
+    for wants in (False, True):                       # whether another input wants a gradient
+        k = x["k"].clone().requires_grad_(wants)
+        with fwAD.dual_level():
+            q = fwAD.make_dual(x["q"], torch.ones_like(x["q"]))
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                softmax_attention(q, k, x["v"])
+            table = fwAD.make_dual(x["table"], torch.ones_like(x["table"]))
+            with pytest.raises(RuntimeError, match="jvp"):
+                relative_bias(table, 3, 4)

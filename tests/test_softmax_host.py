@@ -244,3 +244,16 @@ def test_launches_past_2_32_threads_are_refused(lib):
     refused(lib, lib.qlka_softmax_bwd, many, **wide)
     refused(lib, lib.qlka_softmax_bwd, many, H=1 << 24, G=1, B=1, M=0, N=1, D=8, g_q=None, g_k=None, g_v=None, table=1 << 12,
             g_table=1 << 12, border=[1])                                                       # a workgroup a head and bucket
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v", "table"])
+@pytest.mark.parametrize("D", [8, 5])
+def test_forward_mode_is_refused(name, D):
+    """Not dropped: a tangent on an input that wants no gradient would be lost without a word."""
+    import torch.autograd.forward_ad as fwAD
+    x = {n: torch.zeros(1, 2, 4, D) for n in "qkv"}
+    x["table"] = torch.zeros(32, 2)
+    with fwAD.dual_level():
+        x[name] = fwAD.make_dual(x[name], torch.ones_like(x[name]))
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            softmax_attention(x["q"], x["k"], x["v"], table=x["table"])
