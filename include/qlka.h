@@ -231,8 +231,11 @@ int qlka_layer_fwd_masked(int kind, const float* q, const float* k, const float*
  *   S[b,h,m,n] = scale <q[b,h,m], k[b,h/(H/G),n]> + table[bucket(n - (m + start))][h]      (table may be NULL: no bias)
  *   out[b,h,m] = sum_n P[m,n] v[b,h/(H/G),n],  P = softmax of S over the keys that the query sees
  * A query sees key n if keep[b][n] is nonzero (keep may be NULL) and, with causal, n <= m + start. A row that sees no
- * key (or only scores of -inf) gives zeros, here and in every gradient. Masked keys' rows are not read. scale: 0 or of
- * a size in [2^-96, 2^96]. The table's values are finite or -inf; other infinities and NaN in what is read make NaN.
+ * key (or only scores of -inf) gives zeros, here and in every gradient. Rows of keys that are masked, or that no query
+ * of the call sees, are not read. scale: 0 or of a size in [2^-96, 2^96]. The table's values are finite, up to the type's
+ * lowest and largest, or -inf. Scores may be as large as fp32 holds (where their roundings pass 1, equal ones share a
+ * row and others may not compare as they would in exact arithmetic); past that, and where other infinities or NaN are
+ * read, a row can be NaN.
  * Sums, the softmax's statistics and every sum of the gradients are fp32; with QLKA_BF16 the probabilities and dS are
  * rounded to bf16 for their matrix products, and each result once at its end.
  *

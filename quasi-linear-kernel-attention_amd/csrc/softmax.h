@@ -41,6 +41,7 @@ struct SmParams {
     float* part2;                            // a second set (dV), or [split][B * H][M][2] (maximum, sum) of the forward
     float* part_table;                       // [H][B * row blocks * splits][buckets]
     int B, H, G, M, N, D;
+    int seen;                                // keys from here on are seen by no query, and not read
     int causal, start;
     int splits, blocks;                      // splits of the long axis; blocks of rows (or keys) per head
     float scale;                             // |scale|; its sign (or 0) is in q_sign

@@ -95,6 +95,9 @@ int step_splits(int64_t groups, int64_t tiles) {
     return (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(2048, std::max<int64_t>(groups, 1)), tiles / 4, 256}));
 }
 
+// Keys that some query may see; in causal order a longer cache's are not read.
+int seen_keys(const qlka_softmax_args* a) { return a->causal ? std::max(0, std::min(a->N, a->M + a->start)) : a->N; }
+
 int tile_rows(const qlka_softmax_args* a) { return sm_tile_rows(a->dtype == QLKA_F32 ? 3 : 1, sm_padded(a->D)); }
 
 struct RowPlan { int waves, blocks, splits; };
@@ -120,7 +123,7 @@ RowPlan row_plan(const qlka_softmax_args* a, int heads, int len, int64_t tiles, 
 bool steps(const qlka_softmax_args* a) {
     const int64_t rows = (int64_t)a->H / a->G * a->M;
     if (a->dtype == QLKA_F32) return rows <= STEP_MOST;
-    const double bytes = 4.0 * a->B * a->G * a->N * a->D;                 // of k and v
+    const double bytes = 4.0 * a->B * a->G * seen_keys(a) * a->D;                 // of k and v
     return rows == 1 || (a->M == 1 && rows <= STEP_MOST && bytes > 32e6);
 }
 
@@ -128,8 +131,8 @@ struct FwdPlan { bool step; RowPlan rows; size_t part, part2; };
 FwdPlan fwd_plan(const qlka_softmax_args* a) {
     FwdPlan f{};
     f.step = steps(a);
-    if (f.step) f.rows = {0, 0, step_splits((int64_t)a->B * a->G, ceil_div(a->N, 64))};
-    else f.rows = row_plan(a, a->H, a->M, ceil_div(a->N, tile_rows(a)), 2, FWD_WAVES);
+    if (f.step) f.rows = {0, 0, step_splits((int64_t)a->B * a->G, ceil_div(seen_keys(a), 64))};
+    else f.rows = row_plan(a, a->H, a->M, ceil_div(seen_keys(a), tile_rows(a)), 2, FWD_WAVES);
     if (f.rows.splits > 1) {
         const size_t rows = (size_t)f.rows.splits * a->B * a->H * a->M;
         f.part = align256(rows * sm_padded(a->D) * 4);
@@ -149,7 +152,7 @@ BwdPlan bwd_plan(const qlka_softmax_args* a, bool dq, bool dkv, bool table) {
     w.delta = align256((size_t)a->B * a->H * a->M * 4);
     w.large = align256((size_t)a->B * a->H * ceil_div(a->M, 32) * 4);
     if (dq || table) {
-        w.dq = row_plan(a, a->H, a->M, ceil_div(a->N, t), 3, 0);
+        w.dq = row_plan(a, a->H, a->M, ceil_div(seen_keys(a), t), 3, 0);
         if (w.dq.splits > 1) w.part = align256((size_t)w.dq.splits * a->B * a->H * a->M * DP * 4);
     }
     if (table)
@@ -195,6 +198,7 @@ int params(const qlka_softmax_args* a, SmParams* p) {
     p->table = a->table;
     p->lse = a->lse; p->lse_low = a->lse_low;
     p->B = a->B; p->H = a->H; p->G = a->G; p->M = a->M; p->N = a->N; p->D = a->D;
+    p->seen = seen_keys(a);
     p->causal = a->causal ? 1 : 0;
     p->start = a->start;
     p->splits = p->blocks = 1;

@@ -132,7 +132,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
     const T* v = (const T*)p.v + b * p.sv.b + kvh * p.sv.h;
     const int64_t row = ((int64_t)b * p.H + head) * p.M + m;
 
-    const int tiles = (p.N + BN - 1) / BN;
+    const int tiles = (p.seen + BN - 1) / BN;
     int t0 = (int)((int64_t)tiles * split_i / p.splits), t1 = (int)((int64_t)tiles * (split_i + 1) / p.splits);
     if (p.causal) {
         const int last = min(m0 + ROWS, p.M) - 1 + p.start;
@@ -356,7 +356,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
     const int block = w.block % p.blocks, split_i = w.block / p.blocks;
     const int kvh = w.pair % p.G, b = w.pair / p.G, share = p.H / p.G;
     const int n0 = block * KEYS, nw = n0 + wave * 32, n = nw + col;
-    const bool shown = n < p.N && (!p.keep || p.keep[b * p.keep_stride + n]);
+    const bool shown = n < p.seen && (!p.keep || p.keep[b * p.keep_stride + n]);
     const bool idle = !__any(shown);
 
     // the tiles of queries of all heads that share these keys, one after the other

@@ -46,7 +46,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
     const T* k = (const T*)p.k + b * p.sk.b + kvh * p.sk.h;
     const T* v = (const T*)p.v + b * p.sv.b + kvh * p.sv.h;
 
-    const int tiles = (p.N + BN - 1) / BN;
+    const int tiles = (p.seen + BN - 1) / BN;
     int t0 = (int)((int64_t)tiles * split_i / p.splits), t1 = (int)((int64_t)tiles * (split_i + 1) / p.splits);
     if (p.causal) {
         const int last = min(m0 + ROWS, p.M) - 1 + p.start;          // the last key that a row here sees

@@ -46,11 +46,9 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p
     const T* k = (const T*)p.k + b * p.sk.b + kvh * p.sk.h;
     const T* v = (const T*)p.v + b * p.sv.b + kvh * p.sv.h;
 
-    const int tiles = (p.N + 63) / 64;
+    const int tiles = (p.seen + 63) / 64;
     const int t0 = (int)((int64_t)tiles * split_i / p.splits);
-    int t1 = (int)((int64_t)tiles * (split_i + 1) / p.splits);
-    const int last = p.causal ? p.M - 1 + p.start : p.N - 1;          // the last key that any row sees
-    t1 = min(t1, last < 0 ? 0 : last / 64 + 1);
+    const int t1 = (int)((int64_t)tiles * (split_i + 1) / p.splits);
     KeyBits<64> seen(p, b);
     struct Place { int t, u0; uint64_t bits; };                       // a tile, the first key of U * KEYS of it, its keys
     const auto next = [&](Place at) {                                 // the next U * KEYS keys of this wave with one to see
@@ -65,7 +63,6 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p
             if (at.t >= t1) return at;
             int t = at.t;
             at.bits = seen.find(t, t + 1);
-            if (last - at.t * 64 < 63) at.bits &= (1ull << (last - at.t * 64 + 1)) - 1;
         }
     };
     // the keys of one place are on their way while those of the place before are worked on

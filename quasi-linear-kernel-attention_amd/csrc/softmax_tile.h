@@ -341,11 +341,11 @@ __device__ __forceinline__ uint64_t lane_u64(uint64_t x, int lane) {
 // The keys of each tile of BN that a batch's mask keeps, one bit a key; 64 tiles are looked at together, one a lane.
 template <int BN> struct KeyBits {
     const uint8_t* keep;       // the batch's row, or null
-    int N, window;
+    int N, window;             // N: keys that are seen
     uint64_t bits;             // of tile 64 * window + lane
 
     __device__ __forceinline__ KeyBits(const SmParams& p, int b)
-        : keep(p.keep ? p.keep + b * p.keep_stride : nullptr), N(p.N), window(-1), bits(0) {}
+        : keep(p.keep ? p.keep + b * p.keep_stride : nullptr), N(p.seen), window(-1), bits(0) {}
 
     __device__ __forceinline__ void look(int w) {
         if (w == window) return;

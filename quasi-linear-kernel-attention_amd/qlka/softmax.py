@@ -63,9 +63,9 @@ def softmax_attention(q, k, v, scale=None, keep=None, table=None, buckets=None, 
     float32 or bfloat16, D up to 128, any strides. scale: D ** -0.5 by default; 0 or of a size in [2^-96, 2^96]. keep (B, N):
     nonzero marks the keys to attend to (others are not read). table (num_buckets, H) with buckets (RelativeBuckets): the
     learned position bias table[bucket(n - (m + start)), h], finite or -inf (a bucket that is not attended to). causal: query
-    m sees the keys n <= m + start; start is the position of the first query among the keys. A row that sees no key gives
-    zeros and has no gradient. Differentiable once in q, k, v and table; results and gradients do not change from run to
-    run."""
+    m sees the keys n <= m + start; start is the position of the first query among the keys, of which those past
+    the last query are not read (a cache may be longer than its tokens). A row that sees no key gives zeros and has no
+    gradient. Differentiable once, backward, in q, k, v and table; results and gradients do not change from run to run."""
     if q.dim() == 4 and scale is None:
         scale = max(q.shape[3], 1) ** -0.5
     border, both = (), False

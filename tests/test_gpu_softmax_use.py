@@ -262,3 +262,38 @@ def test_forward_mode_is_refused(dev):
             table = fwAD.make_dual(x["table"], torch.ones_like(x["table"]))
             with pytest.raises(RuntimeError, match="jvp"):
                 relative_bias(table, 3, 4)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("M", [1, 2, 5, 40, 200])
+@pytest.mark.parametrize("start", [-300, -3, 0, 37, 250])
+@pytest.mark.parametrize("bias", [None, RelativeBuckets(bidirectional=False)], ids=["plain", "bias"])
+def test_a_cache_longer_than_its_tokens(dev, bias, start, M, dtype):
+    """Rows of a cache that no token has reached may hold anything: the same result as without them, and zeros as their
+    gradients."""
+    N, cache = max(0, M + start), 600
+    x = leaves(dev, 2, 4, 2, M, cache, 64, dtype, bias, seed=M)
+    dirty = {n: x[n].clone() for n in "kv"}
+    dirty["k"][:, :, N:], dirty["v"][:, :, N:] = float("nan"), float("inf")
+
+    def call(k, v):
+        y = {"q": x["q"].clone(), "k": k.clone(), "v": v.clone()}
+        if bias:
+            y["table"] = x["table"].clone()
+        for a in y.values():
+            a.requires_grad_(True)
+        out = softmax_attention(y["q"], y["k"], y["v"], table=y.get("table"), buckets=bias, causal=True, start=start)
+        with torch.no_grad():
+            assert torch.equal(softmax_attention(y["q"], y["k"], y["v"], causal=True, start=start), out) or bias
+        return (out.detach(),) + torch.autograd.grad(out, list(y.values()), x["g"])
+
+    want = call(x["k"][:, :, :N], x["v"][:, :, :N])
+    got = call(dirty["k"], dirty["v"])
+    for i, (a, b) in enumerate(zip(got, want)):
+        if i in (2, 3):                               # keys and values
+            assert (a[:, :, N:] == 0).all(), i
+            a = a[:, :, :N]
+        assert torch.isfinite(a).all(), i
+        # the axes may be split otherwise: sums of up to 250 terms of one size, and each result's rounding
+        h = torch.finfo(dtype).eps if a.dtype == BF16 else 2 ** -17
+        assert (a.double() - b.double()).abs().max() <= 2 * h * b.double().abs().max() if b.numel() else True, i
