@@ -87,7 +87,8 @@ class KernelMultiheadAttention(nn.Module):
         project_context(context) gives them, which a decoder computes once and passes at every token; keep (B, N) marks
         context's real positions;
       * causal=True: the query at position start + m sees the keys up to its own position. For a decoder's next tokens,
-        context holds the heads of all tokens up to them and start is the position of x's first one."""
+        context holds the heads of all tokens up to them and start is the position of x's first one (without a context,
+        where the keys are x's own, there is no other position than 0)."""
 
     def __init__(self, embed_dim, num_heads, kernel="softmax", tau=None, impl="efficient", position_bias=None):
         super().__init__()
@@ -122,6 +123,8 @@ class KernelMultiheadAttention(nn.Module):
 
     def forward(self, x, keep=None, context=None, causal=False, start=0):
         if context is None:
+            if start != 0:
+                raise ValueError(f"start {start} without a context: the keys are x's own, whose first position is 0")
             q, k, v = self.split_heads(x)
             if self.position_bias is None and not causal:
                 heads = attention(q, k, v, self.kernel, self.tau, keep, self.impl)  # (B, H, S, Dh)

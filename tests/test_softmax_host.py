@@ -257,3 +257,15 @@ def test_forward_mode_is_refused(name, D):
         x[name] = fwAD.make_dual(x[name], torch.ones_like(x[name]))
         with pytest.raises(RuntimeError, match="no forward-mode derivative"):
             softmax_attention(x["q"], x["k"], x["v"], table=x["table"])
+
+
+def test_start_goes_with_a_context():
+    """Without one the keys are x's own, from position 0 on: queries placed after them would see tokens to come."""
+    x = torch.randn(1, 5, 32)
+    for mod in (modules.KernelMultiheadAttention(32, 4),
+                modules.KernelMultiheadAttention(32, 4, position_bias=modules.RelativePositionBias(4, bidirectional=False))):
+        for causal in (False, True):
+            with pytest.raises(ValueError, match="start 3 without a context"):
+                mod(x, causal=causal, start=3)
+    mod = modules.KernelMultiheadAttention(32, 4)
+    torch.testing.assert_close(mod(x, start=0), mod(x))
