@@ -227,3 +227,19 @@ def test_row_sums_of_unrounded_values(dev, M, N):
     out = softmax_attention(x["q"], x["k"], x["v"], table=x["table"], buckets=PAST)
     got = dict(zip(("gq", "gk", "gv"), torch.autograd.grad(out, [x[n] for n in "qkv"], x["g"].detach())), out=out.detach())
     check(got, want)
+
+
+@TYPES
+@pytest.mark.parametrize("D", [8, 32, 80, 128])
+@pytest.mark.parametrize("M,N,causal", [(50, 90, True), (100, 300, False), (100, 300, True), (1, 700, True), (900, 70, False)])
+def test_extremes_at_other_head_dimensions(dev, M, N, causal, D, dtype):
+    """Every instance of the kernels, two and four waves a workgroup, whole and split: a bias of the lowest value everywhere, and
+    a large scale of whole numbers, the mask's and the causal order's edges inside tiles."""
+    start = N - M if causal else 0
+    t = make(2, 4, 2, M, N, D, dtype, seed=D, bias=PAST, keep="random")
+    see = oracle.visible(2, M, N, t["keep"], causal, start)
+    t["table"].fill_(LOWEST)
+    check(run(dev, t, PAST, scale=0.25, causal=causal, start=start), equal_scores(t, see, 0.25), ["out", "gq", "gk", "gv"])
+    t = whole(make(2, 1, 1, M, N, D, dtype, seed=D, keep="random"))
+    see = oracle.visible(2, M, N, t["keep"], causal, start)
+    check(run(dev, t, scale=2.0 ** 30, causal=causal, start=start), equal_scores(t, largest(t, see)[:, 0], 2.0 ** 30))
