@@ -232,10 +232,10 @@ int qlka_layer_fwd_masked(int kind, const float* q, const float* k, const float*
  *   out[b,h,m] = sum_n P[m,n] v[b,h/(H/G),n],  P = softmax of S over the keys that the query sees
  * A query sees key n if keep[b][n] is nonzero (keep may be NULL) and, with causal, n <= m + start. A row that sees no
  * key (or only scores of -inf) gives zeros, here and in every gradient. Rows of keys that are masked, or that no query
- * of the call sees, are not read. scale: 0 or of a size in [2^-96, 2^96]. The table's values are finite, up to the type's
- * lowest and largest, or -inf. Scores may be as large as fp32 holds (where their roundings pass 1, equal ones share a
- * row and others may not compare as they would in exact arithmetic); past that, and where other infinities or NaN are
- * read, a row can be NaN.
+ * of the call sees, are not read. scale: 0 or of a size in [2^-96, 2^96]. The table's values are finite, up to the
+ * type's lowest and largest, or -inf. Scores may be as large as fp32 holds (where their roundings pass 1, equal ones
+ * share a row and others may not compare as they would in exact arithmetic); past that, and where other infinities or
+ * NaN are read, a row can be NaN.
  * Sums, the softmax's statistics and every sum of the gradients are fp32; with QLKA_BF16 the probabilities and dS are
  * rounded to bf16 for their matrix products, and each result once at its end.
  *
@@ -249,13 +249,14 @@ int qlka_layer_fwd_masked(int kind, const float* q, const float* k, const float*
  * start), keys after the query (d > 0) in buckets num_borders + 1 on, 2 (num_borders + 1) buckets in all. Else distance
  * max(-d, 0) and num_borders + 1 buckets. table and g_table are (buckets, H) fp32, contiguous.
  *
- * Forward: writes out and, where not NULL, lse (B, H, M) (half the log2 of each row's sum, +inf for a row without keys),
- * lse_low (B, H, M) (what of it lies below lse's last place: where scores are large, the log of the number of keys that
- * share a row) and out_full (with QLKA_BF16: (B, H, M, D) fp32, out before it is rounded; for the gradients' row sums,
- * in which an error of out is common to all of a row's dS). With out_full and a table the probabilities are taken whole,
- * for the table's gradient, unless table_kept is nonzero: the table will have none. Backward: reads q, k, v, out, lse,
- * g_out and, where not NULL, lse_low and out_full, writes g_q (may be NULL), g_k and g_v (both or neither NULL) and
- * g_table (may be NULL; with QLKA_BF16 it needs out_full). No atomics: results do not change from run to run.
+ * Forward: writes out and, where not NULL, lse (B, H, M) (half the log2 of each row's sum, +inf for a row without
+ * keys), lse_low (B, H, M) (what of it lies below lse's last place: where scores are large, the log of the number of
+ * keys that share a row) and out_full (with QLKA_BF16: (B, H, M, D) fp32, out before it is rounded; for the gradients'
+ * row sums, in which an error of out is common to all of a row's dS). With out_full and a table the probabilities are
+ * taken whole, for the table's gradient, unless table_kept is nonzero: the table will have none, and out is what the
+ * same call without out_full gives. Backward: reads q, k, v, out, lse, g_out and, where not NULL, lse_low and out_full,
+ * writes g_q (may be NULL), g_k and g_v (both or neither NULL) and g_table (may be NULL; with QLKA_BF16 it needs
+ * out_full). No atomics: results do not change from run to run.
  */
 #define QLKA_F32  0
 #define QLKA_BF16 1
@@ -291,11 +292,11 @@ int qlka_softmax_bwd(const qlka_softmax_args* args, void* ws, size_t ws_bytes, v
  * The bias as a map, out (H, M, N) fp32 with out[h,m,n] = table[bucket(n - (m + start))][h], and its gradient, g_table
  * (buckets, H) = the sums of g (H, M, N) over each bucket.
  */
-int qlka_bias_map_fwd(const float* table, const int* border, int num_borders, int bidirectional, float* out, int H, int M,
-                      int N, int start, void* stream);
+int qlka_bias_map_fwd(const float* table, const int* border, int num_borders, int bidirectional, float* out, int H,
+                      int M, int N, int start, void* stream);
 size_t qlka_bias_map_bwd_ws_bytes(int num_borders, int bidirectional, int H, int M, int N);
-int qlka_bias_map_bwd(const float* g, const int* border, int num_borders, int bidirectional, float* g_table, int H, int M,
-                      int N, int start, void* ws, size_t ws_bytes, void* stream);
+int qlka_bias_map_bwd(const float* g, const int* border, int num_borders, int bidirectional, float* g_table, int H,
+                      int M, int N, int start, void* ws, size_t ws_bytes, void* stream);
 
 /*
  * Test entry: stable ascending sort of num_segs contiguous segments of seg_len fp32 keys; perm[i] is the in-segment

@@ -12,8 +12,8 @@ constexpr int SUM_ROWS = 16, SUM_COLS = 1024;         // of the gradient
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));   // rows start at any float
 
-__global__ __launch_bounds__(MAP_T) void map_fwd(const float* table, const SmBuckets bk, float* out, int H, int M, int N,
-                                                 int start) {
+__global__ __launch_bounds__(MAP_T) void map_fwd(const float* table, const SmBuckets bk, float* out, int H, int M,
+                                                 int N, int start) {
     __shared__ float along[MAP_ROWS + MAP_COLS];
     __shared__ int border[QLKA_MAX_BUCKETS];
     const int n0 = blockIdx.x * MAP_COLS, m0 = blockIdx.y * MAP_ROWS, h = blockIdx.z, tid = threadIdx.x;
@@ -41,7 +41,8 @@ __global__ __launch_bounds__(MAP_T) void map_fwd(const float* table, const SmBuc
 // summed, at once where a wave's lie in one. Measured for 12 x 1777 x 2049 (175 MB): 35 us, a plain sum's time, where
 // the last-level cache holds the map, 53 us after as many bytes were written. (64 rows a workgroup 58 us, 8 rows 53;
 // one diagonal a thread, with single loads, 148.)
-__global__ __launch_bounds__(MAP_T) void map_bwd(const float* g, const SmBuckets bk, float* part, int M, int N, int start) {
+__global__ __launch_bounds__(MAP_T) void map_bwd(const float* g, const SmBuckets bk, float* part, int M, int N,
+                                                 int start) {
     constexpr int NW = MAP_T / 64;
     __shared__ int border[QLKA_MAX_BUCKETS];
     __shared__ float sums[NW][QLKA_MAX_BUCKETS];
@@ -116,7 +117,8 @@ static dim3 map_grid(int M, int N, int H) {
     return dim3((unsigned)((N + MAP_COLS - 1) / MAP_COLS), (unsigned)((M + MAP_ROWS - 1) / MAP_ROWS), (unsigned)H);
 }
 static dim3 sum_grid(int M, int N, int H) {
-    return dim3((unsigned)((M + SUM_ROWS - 1) / SUM_ROWS), (unsigned)((N + SUM_ROWS + SUM_COLS - 1) / SUM_COLS), (unsigned)H);
+    return dim3((unsigned)((M + SUM_ROWS - 1) / SUM_ROWS), (unsigned)((N + SUM_ROWS + SUM_COLS - 1) / SUM_COLS),
+                (unsigned)H);
 }
 
 }  // namespace sm

@@ -33,8 +33,8 @@ struct SmParams {
     const uint8_t* keep;                     // [B] rows of N bytes, keep_stride apart, or null
     int64_t keep_stride;
     const float* table;                      // [buckets][H], or null
-    float *lse, *lse_low;                    // [B][H][M], half the log2 of the row's sum, and what lies below its last place
-                                             // (may be null); +inf and 0 for a row without keys
+    float *lse, *lse_low;                    // [B][H][M], half the log2 of the row's sum, and what lies below its last
+                                             // place (may be null); +inf and 0 for a row without keys
     float* delta;                            // [B][H][M]
     int* large;                              // [B][H][groups of 32 rows]: whether a row has a large log sum
     float* part;                             // partial rows of DP floats: [split][B * heads][rows]

@@ -53,7 +53,8 @@ int check_buckets(const int* border, int n, int both, SmBuckets* bk) {
 int check_sizes(const qlka_softmax_args* a) {
     if (!a) return refuse("args must be non-null");
     if (a->dtype != QLKA_F32 && a->dtype != QLKA_BF16) return refuse("dtype must be QLKA_F32 or QLKA_BF16");
-    if (a->B < 0 || a->M < 0 || a->N < 0 || a->H < 1 || a->G < 1) return refuse("B, M and N must be >= 0, H and G >= 1");
+    if (a->B < 0 || a->M < 0 || a->N < 0 || a->H < 1 || a->G < 1)
+        return refuse("B, M and N must be >= 0, H and G >= 1");
     if (a->H % a->G) return refuse("H must be a multiple of G");
     if (a->D < 8 || a->D > 128 || a->D % 8) return refuse("D must be a multiple of 8 in [8, 128]");
     if (a->M > LONGEST || a->N > LONGEST || a->start > LONGEST || a->start < -LONGEST)
@@ -72,8 +73,10 @@ constexpr int CUS = 256;
 
 // Splits of an axis of `tiles` tiles for `groups` workgroups over the other axes, by an estimate of the time: rounds of
 // workgroups on a CU (one alone on a CU is not twice as fast as two, waits not being filled), each its tiles and what
-// it costs by itself, and the joining of `join` bytes a split. In microseconds, fitted to prompts and gradients of 65
-// to 8192 keys.
+// it costs by itself, and the joining of `join` bytes a split. In microseconds, the constants set by hand until 12
+// shapes (prompts and gradients of 65 to 8192 keys, fp32 and bf16) came near the best of 1 to 16 splits of all their axes:
+// eight of them within 4% of it or faster (1 x 4 heads, 100 x 8000: 14.4 us, 17.2 the best one number, 132 unsplit),
+// the others 7 to 18% slower (1 x 12, 512 x 4096: 26.8 : 23.7, unsplit 70; 4 x 12, 1024 x 4096: 91 : 77, unsplit 88).
 int splits_for(int64_t groups, int64_t tiles, double tile_us, double join_bytes) {
     int best = 1;
     double least = 0;
@@ -117,9 +120,15 @@ RowPlan row_plan(const qlka_softmax_args* a, int heads, int len, int64_t tiles, 
 // keys once for each query head but hardly compute in bf16. Measured (us, step : tiles), B, heads / key heads, M, N of
 // 64 elements:
 //   bf16  8, 12 / 12, 1,  197     6.2 :  7.9       fp32  8, 12 / 12, 4,  197    11.6 :  15.4
-//   bf16  4, 12 / 4,  1,  300    14.2 :  8.8       fp32 16, 12 / 3,  1, 4096    36   : 136
-//   bf16  4, 12 / 4,  1, 4097    19.5 : 19.6       fp32  1,  8 / 1,  1, 4096    21.3 :  15.8
-//   bf16 16, 12 / 3,  1, 8192      50 : 64         bf16 16, 12 / 12, 2, 8192    87   :  74
+//   bf16 16, 12 / 12, 2, 8192      87 :   74       fp32 16, 12 / 3,  1, 4096      36 :  136
+//                                                  fp32  1,  8 / 1,  1, 4096    21.3 :  15.8
+// and bf16 single tokens whose heads share keys, by the bytes of k and v (MB):
+//    4.2   4, 12 / 4, 1024     15.1 : 11.0          50   8, 12 / 6, 4096    20.1 : 22.5
+//   16.8   4, 12 / 4, 4097     18.0 : 17.2          50   8, 12 / 3, 8192    30.0 : 35.7
+//   33.6  64,  8 / 4,  512     16.1 : 14.2          67  32, 12 / 4, 2048    31.1 : 35.9
+//   33.6   8, 12 / 4, 4097     21.7 : 22.6          67 128,  8 / 4,  512    23.5 : 26.8
+//   33.6   4, 12 / 4, 8192     20.4 : 23.1         101  16, 12 / 6, 4096    31.9 : 37.6
+//   33.6   1,  8 / 2, 65536    26.4 : 28.3         102   1,  8 / 2, 200000  49.3 : 65.5
 bool steps(const qlka_softmax_args* a) {
     const int64_t rows = (int64_t)a->H / a->G * a->M;
     if (a->dtype == QLKA_F32) return rows <= STEP_MOST;
@@ -218,14 +227,15 @@ int params(const qlka_softmax_args* a, SmParams* p) {
 
 int need_ws(const void* ws, size_t have, size_t need) {
     if (need == 0) return QLKA_OK;
-    if (!ws || have < need || (uintptr_t)ws % 16) return api_error(QLKA_EWORKSPACE, "workspace too small, null or not aligned to 16 bytes");
-    return QLKA_OK;
+    if (ws && have >= need && (uintptr_t)ws % 16 == 0) return QLKA_OK;
+    return api_error(QLKA_EWORKSPACE, "workspace too small, null or not aligned to 16 bytes");
 }
 
 // A launch takes less than 2^32 threads.
 int fits_grid(int64_t groups, int threads) {
     if (groups <= (int64_t)UINT32_MAX / threads) return QLKA_OK;
-    return refuse("too many workgroups: %lld of %d threads, a launch takes less than 2^32 threads", (long long)groups, threads);
+    return refuse("too many workgroups: %lld of %d threads, a launch takes less than 2^32 threads", (long long)groups,
+                  threads);
 }
 // a kernel of workgroups of 256 that takes `lanes` lanes a row
 int fits_rows(int64_t rows, int lanes) { return fits_grid(ceil_div(rows * lanes, 256), 256); }
@@ -289,7 +299,8 @@ int qlka_softmax_bwd(const qlka_softmax_args* a, void* ws, size_t ws_bytes, void
     if (rows && (!a->q || !a->out || !a->lse || !a->g_out)) return refuse("q, out, lse and g_out must be non-null");
     if (keys && (!a->k || !a->v)) return refuse("k and v must be non-null");
     if (a->out_full && a->dtype == QLKA_F32) return refuse("out_full goes with QLKA_BF16");
-    if (rows && a->g_table && a->dtype == QLKA_BF16 && !a->out_full) return refuse("g_table needs out_full with QLKA_BF16");
+    if (rows && a->g_table && a->dtype == QLKA_BF16 && !a->out_full)
+        return refuse("g_table needs out_full with QLKA_BF16");
     const BwdPlan w = bwd_plan(a, a->g_q, a->g_k, a->g_table);
     if (int e = need_ws(ws, ws_bytes, w.bytes())) return e;
     const int64_t queries = (int64_t)a->B * a->H * a->M, kept = (int64_t)a->B * a->G * a->N;
@@ -360,8 +371,8 @@ static int check_map(int H, int M, int N, int start) {
     return QLKA_OK;
 }
 
-int qlka_bias_map_fwd(const float* table, const int* border, int num_borders, int bidirectional, float* out, int H, int M,
-                      int N, int start, void* stream) {
+int qlka_bias_map_fwd(const float* table, const int* border, int num_borders, int bidirectional, float* out, int H,
+                      int M, int N, int start, void* stream) {
     api_error(QLKA_OK, "");
     if (int e = check_map(H, M, N, start)) return e;
     SmBuckets bk;
@@ -377,8 +388,8 @@ size_t qlka_bias_map_bwd_ws_bytes(int num_borders, int bidirectional, int H, int
     return (size_t)H * bias_map_blocks(M, N) * (num_borders + 1) * (bidirectional ? 2 : 1) * 4;
 }
 
-int qlka_bias_map_bwd(const float* g, const int* border, int num_borders, int bidirectional, float* g_table, int H, int M,
-                      int N, int start, void* ws, size_t ws_bytes, void* stream) {
+int qlka_bias_map_bwd(const float* g, const int* border, int num_borders, int bidirectional, float* g_table, int H,
+                      int M, int N, int start, void* ws, size_t ws_bytes, void* stream) {
     api_error(QLKA_OK, "");
     if (int e = check_map(H, M, N, start)) return e;
     SmBuckets bk;

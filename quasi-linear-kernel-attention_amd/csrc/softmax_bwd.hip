@@ -6,10 +6,12 @@
 // the queries (of all the heads that share a key head) for 32 keys a wave. That is 7 products instead of the 5 of one
 // pass, and no sum between workgroups: no atomics, results that do not change from run to run. Scores stay in registers
 // as in the forward. Rounding P and dS to bf16 for the products with bf16 operands costs what rounding the results
-// does. For the table's gradient, which is fp32, dS is taken as it is, and delta formed from an O that nothing was
-// rounded in (softmax_fwd.hip, FINE). Bound as the forward is. Measured: 12 x 8192 x 8192 of 64 with the table's
-// gradient, bf16: softmax_dq 577 us (536 TFLOP/s), softmax_dkv 566 us (730); fp32, 32 x 4 heads of 600 to 65: 40 and 43
-// us.
+// does. An error of delta is in all of a row's dS alike, so it is formed from O before that is rounded to bf16. For the
+// table's gradient, which is fp32, dS is taken as it is, and O is that of P in three parts (softmax_fwd.hip, FINE).
+// The waves wait for 34 to 50% of their cycles, for the next tile and for each other. Measured: 12 x 8192 x 8192 of 64
+// with the table's gradient, bf16: softmax_dq 527 us (587 TFLOP/s), softmax_dkv 565 us (730); fp32, 32 x 4 heads of 600
+// to 65: 41 and 42 us; bf16 of 128, 2 x 8 x 2048 x 2048: 257 us with the forward. Registers are short: at fp32 of 64
+// elements and more, and at bf16 of 128, some values live in scratch memory.
 #include "softmax_tile.h"
 
 #include <limits>
@@ -39,7 +41,8 @@ __global__ __launch_bounds__(256) void softmax_delta(const SmParams p) {
         if (m < p.M) {
             const T* out = (const T*)p.out + b * p.so.b + head * p.so.h + m * p.so.r;
             const auto g = load_seg((const T*)p.g_out + b * p.sg.b + head * p.sg.h + m * p.sg.r, d, p.D);
-            const f32x8 o = p.out_full ? load_seg(p.out_full + (row0 + m) * p.D, d, p.D) : floats(load_seg(out, d, p.D));
+            const f32x8 o = p.out_full ? load_seg(p.out_full + (row0 + m) * p.D, d, p.D)
+                                       : floats(load_seg(out, d, p.D));
             large |= large_lse(p.lse[row0 + m]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) x = __builtin_fmaf((float)g[j], o[j], x);
@@ -70,7 +73,8 @@ __device__ __forceinline__ void add_band(f32x16 ds, const uint8_t* buckets, floa
     float pos = 0.f, neg = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-        const int x = __builtin_amdgcn_ds_bpermute(((from + 4 * reg_row(r)) & 124) | (lane & 32) << 2, __float_as_int(ds[r]));
+        const int x = __builtin_amdgcn_ds_bpermute(((from + 4 * reg_row(r)) & 124) | (lane & 32) << 2,
+                                                   __float_as_int(ds[r]));
         const bool after = t <= reg_row(r) + 4 * half;
         pos += after ? __int_as_float(x) : 0.f;
         neg += after ? 0.f : __int_as_float(x);
@@ -101,10 +105,10 @@ template <int NP, int NS, class F> __device__ __forceinline__ void by_halves(boo
     }
 }
 
-// Large log sums are taken off in two steps, after the score is rounded. With bf16 operands in a loop of its own, f(true): a
-// test between a tile's products and its exponentials keeps those apart (8% of softmax_dkv's time at 4 x 12 x 1024 x 4096
-// of 64). With fp32 the test is in the loop, by tiles, f(false): there it costs 1% at 32 x 4 heads of 600 to 65, and what a
-// second loop needs before it starts, and its registers, 5%.
+// Large log sums are taken off in two steps, after the score is rounded. With bf16 operands in a loop of its own,
+// f(true): a test between a tile's products and its exponentials keeps those apart (8% of softmax_dkv's time at 4 x 12
+// x 1024 x 4096 of 64). With fp32 the test is in the loop, by tiles, f(false): there it costs 1% at 32 x 4 heads of 600
+// to 65, and what a second loop needs before it starts, and its registers, 5%.
 template <int NP, class F> __device__ __forceinline__ void by_size(bool large, F f) {
     if constexpr (NP == 1) {
         if (__builtin_expect(large, 0)) return f(std::true_type());
@@ -121,7 +125,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
     __shared__ BiasLds table;
     __shared__ __attribute__((aligned(16))) float mask_of[BUFFERS][BN];
     __shared__ float near_bias[BUFFERS][BIAS ? ROWS + BN : 1], sums[BIAS ? NW : 1][QLKA_MAX_BUCKETS];
-    __shared__ uint8_t near_bucket[BUFFERS][BIAS ? ROWS + BN : 1];        // from the distance before near_bias's first on
+    __shared__ uint8_t near_bucket[BUFFERS][BIAS ? ROWS + BN : 1];     // from the distance before near_bias's first on
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
     const Work w = xcd_work(blockIdx.x, p.B * p.H, p.blocks * p.splits);
@@ -149,8 +153,9 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
 
     Frag<NP> qf[DP / 16], gf[DP / 16];
     float delta = 0.f;
-    // dP is formed as -((-dO) V^T) for every other query: the matrix instruction's sums are a little low (softmax_tile.h), and a
-    // bucket adds up millions of dS (12 x 8192 x 8192, four inputs: error of the table's gradient 2 to 12% less)
+    // dP is formed as -((-dO) V^T) for every other query: the matrix instruction's sums are a little low
+    // (softmax_tile.h), and a bucket adds up millions of dS (12 x 8192 x 8192, four inputs: error of the table's
+    // gradient 2 to 12% less)
     const float turn = BIAS && (col & 1) ? -1.f : 1.f;
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
@@ -192,118 +197,122 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
     Acc<NP> dq[ND];
 
     const auto go = [&](auto all_wide) {
-    const bool wide = NP == 3 ? large : all_wide;
-    while (coming) {
-        const int n0 = t * BN;
-        const uint64_t bits = coming;
-        float far = 0.f;
-        int fb = -1;
-        float *near_here = near_bias[buffer], *mask = mask_of[buffer];
-        uint8_t* bucket_here = near_bucket[buffer];
-        tile.arrive(lds, tid, [&] {
-            if (bits != PairT::ALL) put_mask<BN>(mask, bits, tid);
-            if constexpr (BIAS) {
-                const int lo = n0 - (m0 + ROWS - 1) - p.start;
-                fb = far_bucket(p.bk, lo, n0 + BN - 1 - m0 - p.start);
-                if (fb < 0) {
-                    for (int i = tid; i < ROWS + BN; i += NT) {
-                        const int bucket = bucket_of(table.border, p.bk.n, p.bk.both, lo + i - 1);
-                        bucket_here[i] = (uint8_t)bucket;
-                        if (i) near_here[i - 1] = table.value[bucket];
-                    }
-                } else {
-                    far = table.value[fb];
-                }
-            }
-        });
-        const auto& kt = lds.a[buffer];
-        const auto& vt = lds.b[buffer];
-        buffer ^= BUFFERS - 1;
-        coming = seen.find(++t, t1);
-        if (coming) fetch(t, coming, buffer);
-        if (mw >= p.M || (p.causal && n0 > mw + 31 + p.start)) continue;
-
-        const bool edge = p.causal && n0 + BN - 1 > mw + p.start;
-        const int lim = m + p.start - n0 - 4 * half;                     // at an edge, the last key seen
-        const float* nb = &near_here[BIAS ? ROWS - 1 - wave * 32 - col + 4 * half : 0];
-        const float off = wide ? 0.f : lse, add = far_twice(far - off);
-        // `count` halves of the tile together: the products of one are under way while the other's scores are worked on
-        const auto halves = [&](auto first, auto count) {
-            f32x16 s[count], dp[count];
-#pragma unroll
-            for (int i = 0; i < count; ++i) {
-                Acc<NP> a;
-                a.start();
-#pragma unroll
-                for (int c = 0; c < DP / 16; ++c) a.add(kt.row(32 * (first + i) + col, 16 * c + 8 * half), qf[c]);
-                a.join();
-                s[i] = a.main;
-            }
-#pragma unroll
-            for (int i = 0; i < count; ++i) {
-                Acc<NP> a;
-                a.start();
-#pragma unroll
-                for (int c = 0; c < DP / 16; ++c) a.add(vt.row(32 * (first + i) + col, 16 * c + 8 * half), gf[c]);
-                a.join();
-                dp[i] = a.main;
-            }
-#pragma unroll
-            for (int i = 0; i < count; ++i) {
-                // to twice the scores less the row's log sum
-                if (wide || (BIAS && fb < 0)) {
-                    if (BIAS && fb < 0) {
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c1, nb[32 * (first + i) + reg_row(r)] - off);
-                    } else {
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c1, far);
-                    }
-                    if (wide) {
-                        const float low = m < p.M && p.lse_low ? p.lse_low[row] : 0.f;
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) s[i][r] = at_most_0((s[i][r] - lse) - low);
-                    }
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[i][r] += s[i][r];
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], 2.f * c1, add);
-                }
-                if (bits != PairT::ALL) s[i] = masked(s[i], mask, 32 * (first + i) + 4 * half);
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[i][r] = fexp2(s[i][r]) * __builtin_fmaf(dp[i][r], turn, -delta);
-                if (edge) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (32 * (first + i) + reg_row(r) > lim) s[i][r] = 0.f;
-                }
-                if (to_table) {
+        const bool wide = NP == 3 ? large : all_wide;
+        while (coming) {
+            const int n0 = t * BN;
+            const uint64_t bits = coming;
+            float far = 0.f;
+            int fb = -1;
+            float *near_here = near_bias[buffer], *mask = mask_of[buffer];
+            uint8_t* bucket_here = near_bucket[buffer];
+            tile.arrive(lds, tid, [&] {
+                if (bits != PairT::ALL) put_mask<BN>(mask, bits, tid);
+                if constexpr (BIAS) {
+                    const int lo = n0 - (m0 + ROWS - 1) - p.start;
+                    fb = far_bucket(p.bk, lo, n0 + BN - 1 - m0 - p.start);
                     if (fb < 0) {
-                        // a half's first key and the wave's first query, less 32: 32 (first + i) + ROWS - 32 - 32 wave after lo - 1
-                        if ((uint32_t)(bits >> (32 * (first + i))))
-                            add_band(s[i], bucket_here + 32 * (first + i) + ROWS - 32 - 32 * wave, sums[wave], lane);
+                        for (int i = tid; i < ROWS + BN; i += NT) {
+                            const int bucket = bucket_of(table.border, p.bk.n, p.bk.both, lo + i - 1);
+                            bucket_here[i] = (uint8_t)bucket;
+                            if (i) near_here[i - 1] = table.value[bucket];
+                        }
                     } else {
-                        float a = 0.f;
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) a += s[i][r];
-                        if (fb == p.bk.n) left += a; else right += a;
+                        far = table.value[fb];
                     }
                 }
-                Frag<NP> df[2];
+            });
+            const auto& kt = lds.a[buffer];
+            const auto& vt = lds.b[buffer];
+            buffer ^= BUFFERS - 1;
+            coming = seen.find(++t, t1);
+            if (coming) fetch(t, coming, buffer);
+            if (mw >= p.M || (p.causal && n0 > mw + 31 + p.start)) continue;
+
+            const bool edge = p.causal && n0 + BN - 1 > mw + p.start;
+            const int lim = m + p.start - n0 - 4 * half;                     // at an edge, the last key seen
+            const float* nb = &near_here[BIAS ? ROWS - 1 - wave * 32 - col + 4 * half : 0];
+            const float off = wide ? 0.f : lse, add = far_twice(far - off);
+            // `count` halves of the tile together: the products of one are under way while the other's scores are
+            // worked on
+            const auto halves = [&](auto first, auto count) {
+                f32x16 s[count], dp[count];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) df[c] = split<NP>(eight(s[i], c));
+                for (int i = 0; i < count; ++i) {
+                    Acc<NP> a;
+                    a.start();
 #pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    dq[d].start();
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) dq[d].add(kt.column(32 * (first + i) + 16 * c, 32 * d, lane), df[c]);
-                    dq[d].join();
+                    for (int c = 0; c < DP / 16; ++c) a.add(kt.row(32 * (first + i) + col, 16 * c + 8 * half), qf[c]);
+                    a.join();
+                    s[i] = a.main;
                 }
-            }
-        };
-        by_halves<NP, NS>(NS == 1 || !(bits >> 32), halves);
-    }
+#pragma unroll
+                for (int i = 0; i < count; ++i) {
+                    Acc<NP> a;
+                    a.start();
+#pragma unroll
+                    for (int c = 0; c < DP / 16; ++c) a.add(vt.row(32 * (first + i) + col, 16 * c + 8 * half), gf[c]);
+                    a.join();
+                    dp[i] = a.main;
+                }
+#pragma unroll
+                for (int i = 0; i < count; ++i) {
+                    // to twice the scores less the row's log sum
+                    if (wide || (BIAS && fb < 0)) {
+                        if (BIAS && fb < 0) {
+#pragma unroll
+                            for (int r = 0; r < 16; ++r)
+                                s[i][r] = __builtin_fmaf(s[i][r], c1, nb[32 * (first + i) + reg_row(r)] - off);
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c1, far);
+                        }
+                        if (wide) {
+                            const float low = m < p.M && p.lse_low ? p.lse_low[row] : 0.f;
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) s[i][r] = at_most_0((s[i][r] - lse) - low);
+                        }
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[i][r] += s[i][r];
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], 2.f * c1, add);
+                    }
+                    if (bits != PairT::ALL) s[i] = masked(s[i], mask, 32 * (first + i) + 4 * half);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[i][r] = fexp2(s[i][r]) * __builtin_fmaf(dp[i][r], turn, -delta);
+                    if (edge) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            if (32 * (first + i) + reg_row(r) > lim) s[i][r] = 0.f;
+                    }
+                    if (to_table) {
+                        if (fb < 0) {
+                            // a half's first key and the wave's first query, less 32, after lo - 1
+                            const int from = 32 * (first + i) + ROWS - 32 - 32 * wave;
+                            if ((uint32_t)(bits >> (32 * (first + i))))
+                                add_band(s[i], bucket_here + from, sums[wave], lane);
+                        } else {
+                            float a = 0.f;
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) a += s[i][r];
+                            if (fb == p.bk.n) left += a; else right += a;
+                        }
+                    }
+                    Frag<NP> df[2];
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) df[c] = split<NP>(eight(s[i], c));
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        dq[d].start();
+#pragma unroll
+                        for (int c = 0; c < 2; ++c)
+                            dq[d].add(kt.column(32 * (first + i) + 16 * c, 32 * d, lane), df[c]);
+                        dq[d].join();
+                    }
+                }
+            };
+            by_halves<NP, NS>(NS == 1 || !(bits >> 32), halves);
+        }
     };
     by_size<NP>(any_large, go);
     if (to_table) {
@@ -347,7 +356,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
     constexpr int BUFFERS = PairT::BUFFERS;
     __shared__ typename PairT::Lds lds;
     __shared__ __attribute__((aligned(16))) float lse_of[BUFFERS][BM], delta_of[BUFFERS][BM], large_of[BUFFERS][2][BM];
-    __shared__ int wide_of;                            // (fp32, of the one buffer) a row of the tile has a large log sum
+    __shared__ int wide_of;                            // (fp32, one buffer) a row of the tile has a large log sum
     __shared__ BiasLds table;
     __shared__ float near_bias[BUFFERS][BIAS ? KEYS + BM : 1];
 
@@ -372,9 +381,9 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
     float ls = HIGH, des = 0.f;
     const auto fetch = [&](int t, int buffer) {
         const int head = kvh * share + t / tiles, m0 = t % tiles * BM, left = p.M - m0;
+        const uint64_t bits = left >= BM ? PairT::ALL : (1ull << left) - 1;
         tile.fetch(lds, buffer, (const T*)p.q + b * p.sq.b + head * p.sq.h + m0 * p.sq.r,
-                   (const T*)p.g_out + b * p.sg.b + head * p.sg.h + m0 * p.sg.r, left >= BM ? PairT::ALL : (1ull << left) - 1, p.D,
-                   tid);
+                   (const T*)p.g_out + b * p.sg.b + head * p.sg.h + m0 * p.sg.r, bits, p.D, tid);
         ls = HIGH;
         des = 0.f;
         if (tid < BM && tid < left) {
@@ -411,131 +420,134 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
     int filled = -1;                                   // the head whose bias stands in LDS
 
     const auto go = [&](auto all_wide) {
-    while (t < t1) {
-        const int m0 = t % tiles * BM, head = kvh * share + t / tiles;
-        float far = 0.f;
-        bool near = false;
-        float *near_here = near_bias[buffer], *lse = lse_of[buffer], *delta = delta_of[buffer];
-        float (*two)[BM] = large_of[buffer];
-        if (BIAS && head != filled) {
-            __syncthreads();
-            table.fill(p, head, tid, NT);
-            filled = head;
-            __syncthreads();
-        }
-        tile.arrive(lds, tid, [&] {
-            const bool wide = NP == 3 ? __any(large_lse(ls)) : all_wide;      // all rows are in the first wave
-            if (NP == 3 && tid == 0) wide_of = wide;
-            if (tid < BM) {
-                lse[tid] = wide ? 0.f : -ls * per_c1;
-                delta[tid] = -des;
-                if (wide) {
-                    two[0][tid] = ls;
-                    two[1][tid] = p.lse_low && m0 + tid < p.M ? p.lse_low[((int64_t)b * p.H + head) * p.M + m0 + tid] : 0.f;
-                }
+        while (t < t1) {
+            const int m0 = t % tiles * BM, head = kvh * share + t / tiles;
+            float far = 0.f;
+            bool near = false;
+            float *near_here = near_bias[buffer], *lse = lse_of[buffer], *delta = delta_of[buffer];
+            float (*two)[BM] = large_of[buffer];
+            if (BIAS && head != filled) {
+                __syncthreads();
+                table.fill(p, head, tid, NT);
+                filled = head;
+                __syncthreads();
             }
-            if constexpr (BIAS) {
-                const int lo = n0 - (m0 + BM - 1) - p.start;
-                const int fb = far_bucket(p.bk, lo, n0 + KEYS - 1 - m0 - p.start);
-                near = fb < 0;
-                if (near) {
-                    for (int i = tid; i < KEYS + BM - 1; i += NT)
-                        near_here[i] = table.value[bucket_of(table.border, p.bk.n, p.bk.both, lo + i)];
-                } else {
-                    far = table.value[fb];
+            tile.arrive(lds, tid, [&] {
+                const bool wide = NP == 3 ? __any(large_lse(ls)) : all_wide;      // all rows are in the first wave
+                if (NP == 3 && tid == 0) wide_of = wide;
+                if (tid < BM) {
+                    lse[tid] = wide ? 0.f : -ls * per_c1;
+                    delta[tid] = -des;
+                    if (wide) {
+                        two[0][tid] = ls;
+                        const int64_t row = ((int64_t)b * p.H + head) * p.M + m0 + tid;
+                        two[1][tid] = p.lse_low && m0 + tid < p.M ? p.lse_low[row] : 0.f;
+                    }
                 }
-            }
-        });
-        const auto& qt = lds.a[buffer];
-        const auto& gt = lds.b[buffer];
-        buffer ^= BUFFERS - 1;
-        t = next(t + 1);
-        if (t < t1) fetch(t, buffer);
-        if (idle || (p.causal && m0 + BM - 1 + p.start < nw)) continue;
+                if constexpr (BIAS) {
+                    const int lo = n0 - (m0 + BM - 1) - p.start;
+                    const int fb = far_bucket(p.bk, lo, n0 + KEYS - 1 - m0 - p.start);
+                    near = fb < 0;
+                    if (near) {
+                        for (int i = tid; i < KEYS + BM - 1; i += NT)
+                            near_here[i] = table.value[bucket_of(table.border, p.bk.n, p.bk.both, lo + i)];
+                    } else {
+                        far = table.value[fb];
+                    }
+                }
+            });
+            const auto& qt = lds.a[buffer];
+            const auto& gt = lds.b[buffer];
+            buffer ^= BUFFERS - 1;
+            t = next(t + 1);
+            if (t < t1) fetch(t, buffer);
+            if (idle || (p.causal && m0 + BM - 1 + p.start < nw)) continue;
 
-        const bool edge = p.causal && m0 + p.start < nw + 31;
-        const int lim = edge ? n - p.start - m0 - 4 * half : -1;         // the first query that sees the key
-        const float* nb = &near_here[BIAS ? wave * 32 + col + BM - 1 - 4 * half : 0];
-        const float add = far_twice(far);
-        const auto halves = [&](auto first, auto count) {
-            // scores less the row's log sum (in units of the scores; a large one later), and dP less delta
-            f32x16 s[count], dp[count];
+            const bool edge = p.causal && m0 + p.start < nw + 31;
+            const int lim = edge ? n - p.start - m0 - 4 * half : -1;         // the first query that sees the key
+            const float* nb = &near_here[BIAS ? wave * 32 + col + BM - 1 - 4 * half : 0];
+            const float add = far_twice(far);
+            const auto halves = [&](auto first, auto count) {
+                // scores less the row's log sum (in units of the scores; a large one later), and dP less delta
+                f32x16 s[count], dp[count];
 #pragma unroll
-            for (int i = 0; i < count; ++i) {
-                Acc<NP> a(rows_of(lse, 32 * (first + i) + 4 * half));
-                a.start();
+                for (int i = 0; i < count; ++i) {
+                    Acc<NP> a(rows_of(lse, 32 * (first + i) + 4 * half));
+                    a.start();
 #pragma unroll
-                for (int c = 0; c < DP / 16; ++c) a.add_turned(qt.row(32 * (first + i) + col, 16 * c + 8 * half), kf[c]);
-                a.join();
-                s[i] = a.main;
-            }
+                    for (int c = 0; c < DP / 16; ++c)
+                        a.add_turned(qt.row(32 * (first + i) + col, 16 * c + 8 * half), kf[c]);
+                    a.join();
+                    s[i] = a.main;
+                }
 #pragma unroll
-            for (int i = 0; i < count; ++i) {
-                Acc<NP> a(rows_of(delta, 32 * (first + i) + 4 * half));
-                a.start();
+                for (int i = 0; i < count; ++i) {
+                    Acc<NP> a(rows_of(delta, 32 * (first + i) + 4 * half));
+                    a.start();
 #pragma unroll
-                for (int c = 0; c < DP / 16; ++c) a.add(gt.row(32 * (first + i) + col, 16 * c + 8 * half), vf[c]);
-                a.join();
-                dp[i] = a.main;
-            }
-            const bool wide = NP == 3 ? __builtin_amdgcn_readfirstlane(wide_of) : all_wide;
+                    for (int c = 0; c < DP / 16; ++c) a.add(gt.row(32 * (first + i) + col, 16 * c + 8 * half), vf[c]);
+                    a.join();
+                    dp[i] = a.main;
+                }
+                const bool wide = NP == 3 ? __builtin_amdgcn_readfirstlane(wide_of) : all_wide;
 #pragma unroll
-            for (int i = 0; i < count; ++i) {
-                // to twice the scores less the row's log sum
-                if (wide || (BIAS && near)) {
-                    if (BIAS && near) {
+                for (int i = 0; i < count; ++i) {
+                    // to twice the scores less the row's log sum
+                    if (wide || (BIAS && near)) {
+                        if (BIAS && near) {
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c1, nb[-32 * (first + i) - reg_row(r)]);
+                            for (int r = 0; r < 16; ++r)
+                                s[i][r] = __builtin_fmaf(s[i][r], c1, nb[-32 * (first + i) - reg_row(r)]);
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c1, far);
+                        }
+                        if (wide) {
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) {
+                                const int row = 32 * (first + i) + 4 * half + reg_row(r);
+                                s[i][r] = at_most_0((s[i][r] - two[0][row]) - two[1][row]);
+                            }
+                        }
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[i][r] += s[i][r];
                     } else {
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c1, far);
-                    }
-                    if (wide) {
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int row = 32 * (first + i) + 4 * half + reg_row(r);
-                            s[i][r] = at_most_0((s[i][r] - two[0][row]) - two[1][row]);
-                        }
+                        for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], 2.f * c1, add);
                     }
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[i][r] += s[i][r];
-                } else {
+                    for (int r = 0; r < 16; ++r) {
+                        s[i][r] = fexp2(s[i][r]);
+                        dp[i][r] *= s[i][r];
+                    }
+                    if (edge) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], 2.f * c1, add);
+                        for (int r = 0; r < 16; ++r)
+                            if (32 * (first + i) + reg_row(r) < lim) s[i][r] = dp[i][r] = 0.f;
+                    }
+                    Frag<NP> f[2];
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) f[c] = split<NP>(eight(s[i], c));
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        dv[d].start();
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) dv[d].add(gt.column(32 * (first + i) + 16 * c, 32 * d, lane), f[c]);
+                        dv[d].join();
+                    }
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) f[c] = split<NP>(eight(dp[i], c));
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        dk[d].start();
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) dk[d].add(qt.column(32 * (first + i) + 16 * c, 32 * d, lane), f[c]);
+                        dk[d].join();
+                    }
                 }
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    s[i][r] = fexp2(s[i][r]);
-                    dp[i][r] *= s[i][r];
-                }
-                if (edge) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (32 * (first + i) + reg_row(r) < lim) s[i][r] = dp[i][r] = 0.f;
-                }
-                Frag<NP> f[2];
-#pragma unroll
-                for (int c = 0; c < 2; ++c) f[c] = split<NP>(eight(s[i], c));
-#pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    dv[d].start();
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) dv[d].add(gt.column(32 * (first + i) + 16 * c, 32 * d, lane), f[c]);
-                    dv[d].join();
-                }
-#pragma unroll
-                for (int c = 0; c < 2; ++c) f[c] = split<NP>(eight(dp[i], c));
-#pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    dk[d].start();
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) dk[d].add(qt.column(32 * (first + i) + 16 * c, 32 * d, lane), f[c]);
-                    dk[d].join();
-                }
-            }
-        };
-        by_halves<NP, NS>(m0 + 32 >= p.M, halves);
-    }
+            };
+            by_halves<NP, NS>(m0 + 32 >= p.M, halves);
+        }
     };
     by_size<NP>(any_large, go);
     if (n >= p.N) return;
@@ -618,12 +630,14 @@ int sm_delta(int dtype, const SmParams& p, hipStream_t st) {
 
 int sm_dq(int dtype, const SmParams& p, int waves, hipStream_t st) {
     return sm::dispatch(dtype, p.D, [&](auto t, auto dp) {
-        return waves == 2 ? sm::run_dq<decltype(t), dp.value, 2>(p, st) : sm::run_dq<decltype(t), dp.value, 4>(p, st); });
+        return waves == 2 ? sm::run_dq<decltype(t), dp.value, 2>(p, st)
+                          : sm::run_dq<decltype(t), dp.value, 4>(p, st); });
 }
 
 int sm_dkv(int dtype, const SmParams& p, int waves, hipStream_t st) {
     return sm::dispatch(dtype, p.D, [&](auto t, auto dp) {
-        return waves == 2 ? sm::run_dkv<decltype(t), dp.value, 2>(p, st) : sm::run_dkv<decltype(t), dp.value, 4>(p, st); });
+        return waves == 2 ? sm::run_dkv<decltype(t), dp.value, 2>(p, st)
+                          : sm::run_dkv<decltype(t), dp.value, 4>(p, st); });
 }
 
 int sm_sum_parts(int dtype, const float* part, void* out, SmStrides so, float scale, int splits, int B, int heads,

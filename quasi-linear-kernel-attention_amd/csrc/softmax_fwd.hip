@@ -6,18 +6,19 @@
 // from the registers they are in. A workgroup's waves share the tiles of k and v in LDS; the next tile's loads are
 // issued before the current tile's products. The running maximum is moved only when it grows by more than 2^8, so
 // that the output is hardly ever scaled; probabilities are then at most 2^8. Rounding them to bf16 for the product with
-// bf16 values (not for fp32) costs what rounding the result does; the sum they are divided by is then that of the
-// rounded ones. Where the table's gradient will be wanted (FINE) they are taken in three parts of 8 bits: that gradient
-// is fp32 and a sum over rows of dS = P (dP - delta), in which an error of delta, the row sum of dO * O, does not
-// average out. The smaller parts' products then gather in a sum of their own, as in Acc (12 x 8192 x 8192: error of the
-// table's gradient 1.0e-6, 1.8e-6 without; 513 us for 482).
+// bf16 values (not for fp32) costs what rounding the result does (error against float64 0.0023, 0.0017 with P whole;
+// two parts of P: 1337 us for 965 at 12 x 16384 x 16384); the sum they are divided by is then that of the rounded ones.
+// Where the table's gradient will be wanted (FINE) they are taken in three parts of 8 bits: that gradient is fp32 and a
+// sum over rows of dS = P (dP - delta), in which an error of delta, the row sum of dO * O, does not average out. The
+// smaller parts' products then gather in a sum of their own, as in Acc (12 x 8192 x 8192: error of the table's gradient
+// 1.0e-6, 1.8e-6 without; 565 us, 260 with one part).
 //
 // Masked keys are read as zeros (what stands there may be anything) and their tiles, where none is left, are skipped.
 // Bound by the matrix cores and by the scores' work between them (an exponential, a maximum and two multiply-adds a
-// score), which other waves' products hide only in part. Measured: 12 x 16384 x 16384 of 64 with the bias, bf16, 980
-// us, 840 TFLOP/s; 4 x 12 x 2048 x 8192, padded, 205 us; fp32, 2 x 12 x 301 x 3111, padded, 54 us with the joining of
-// the splits. When a call has too few queries to fill the GPU, the keys are split: each split leaves its unscaled O
-// with its maximum and sum, and softmax_combine joins them.
+// score), which other waves' products hide only in part. Measured: 12 x 16384 x 16384 of 64 with the bias, bf16, 977 to
+// 1003 us, 835 TFLOP/s; 4 x 12 x 2048 x 8192, padded, 200 to 220 us; fp32, 2 x 12 x 301 x 3111, padded, 54 us with the
+// joining of the splits; causal order, 12 x 8192 x 8192, 197 us. When a call has too few queries to fill the GPU, the
+// keys are split: each split leaves its unscaled O with its maximum and sum, and softmax_combine joins them.
 #include "softmax_tile.h"
 
 #include <limits>
@@ -180,8 +181,8 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
                 mul *= 2.f;
                 add = 2.f * (add - ref);
             }
-            float tile_sum = 0.f;                          // summed by tiles: thousands of terms one by one lose two digits more
-            f32x16 small[ND];                              // FINE: the smaller parts apart, as in Acc
+            float tile_sum = 0.f;                      // by tiles: thousands of terms one by one lose two digits more
+            f32x16 small[ND];                          // FINE: the smaller parts apart, as in Acc
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
                 o[d].start();
@@ -260,7 +261,8 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(co
 
 template <class T, int DP, int NW> int launch_fwd(const SmParams& p, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)p.B * p.H * p.blocks * p.splits));
-    if (sizeof(T) == 2 && p.table && p.out_full && !p.table_kept) softmax_fwd<T, DP, NW, true, sizeof(T) == 2><<<grid, 64 * NW, 0, st>>>(p);
+    const bool fine = sizeof(T) == 2 && p.table && p.out_full && !p.table_kept;
+    if (fine) softmax_fwd<T, DP, NW, true, sizeof(T) == 2><<<grid, 64 * NW, 0, st>>>(p);
     else if (p.table) softmax_fwd<T, DP, NW, true, false><<<grid, 64 * NW, 0, st>>>(p);
     else softmax_fwd<T, DP, NW, false, false><<<grid, 64 * NW, 0, st>>>(p);
     return (int)hipGetLastError();

@@ -50,8 +50,8 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void softmax_step(const SmParams p
     const int t0 = (int)((int64_t)tiles * split_i / p.splits);
     const int t1 = (int)((int64_t)tiles * (split_i + 1) / p.splits);
     KeyBits<64> seen(p, b);
-    struct Place { int t, u0; uint64_t bits; };                       // a tile, the first key of U * KEYS of it, its keys
-    const auto next = [&](Place at) {                                 // the next U * KEYS keys of this wave with one to see
+    struct Place { int t, u0; uint64_t bits; };        // a tile, the first key of U * KEYS of it, its keys
+    const auto next = [&](Place at) {                  // the next U * KEYS keys of this wave with one to see
         at.u0 += U * KEYS;
         while (true) {
             while (at.u0 < 64) {
@@ -229,7 +229,9 @@ template <class T, int DP, int R> int launch_step(const SmParams& p, hipStream_t
 template <class T, int DP> int pick_step(const SmParams& p, hipStream_t st) {
     const int rows = p.H / p.G * p.M;
     static_assert(STEP_MOST == 4, "the largest number of rows has an instance");
-    return rows == 1 ? launch_step<T, DP, 1>(p, st) : rows == 2 ? launch_step<T, DP, 2>(p, st) : launch_step<T, DP, 4>(p, st);
+    return rows == 1   ? launch_step<T, DP, 1>(p, st)
+           : rows == 2 ? launch_step<T, DP, 2>(p, st)
+                       : launch_step<T, DP, 4>(p, st);
 }
 }  // namespace sm
 

@@ -9,8 +9,9 @@
 // column a lane). No score crosses lanes or goes through LDS.
 //
 // float inputs are split into three bf16 parts of 8 bits each (24 in all), and a product is the six products of parts
-// whose sizes add up to 2^-16 of the largest or more; what is left out is below 2^-26 of it. At 6 bf16 products that is
-// 2.7 times the rate of the fp32 matrix instruction. An infinity among the inputs gives NaN this way.
+// whose sizes add up to 2^-16 of the largest or more; what is left out is below 2^-26 of it. At the rates of large
+// products (bf16 1215 TFLOP/s, fp32 152, measured) six of them are 1.33 times as fast as one in fp32. An infinity among
+// the inputs gives NaN this way.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -30,12 +31,13 @@ typedef __attribute__((ext_vector_type(8))) float f32x8;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 
-// Scores, biases and log sums are held in units of 2 ln 2, halves of a power of two: x ln 2 units are larger than x, and the
-// lowest finite bias, with which a bucket is hidden, would become -inf. exp2 of the double is e to the score.
+// Scores, biases and log sums are held in units of 2 ln 2, halves of a power of two: in units of ln 2 the number of a
+// score is larger than the score, and the lowest finite bias, with which a bucket is hidden, would become -inf. exp2 of
+// twice the number is e to the score.
 constexpr float UNIT = 0.72134752044448170f;
-// Where a row's reference (its maximum, its log sum) is larger, scores are rounded before it is taken off: it is a rounded score
-// itself, and the exact product in fma(score, scale, bias - reference) would be off from it by up to half its last place,
-// which is 2^-15 here and grows to any factor of the exponential.
+// Where a row's reference (its maximum, its log sum) is larger, scores are rounded before it is taken off: it is a
+// rounded score itself, and the exact product in fma(score, scale, bias - reference) would be off from it by up to half
+// its last place, which is 2^-15 here and grows to any factor of the exponential.
 constexpr float WIDE = 512.f;
 
 template <class T> struct Elem;
@@ -100,7 +102,9 @@ template <int NP> struct Acc {
 __device__ __forceinline__ f32x8 floats(bf16x8 x) { return __builtin_convertvector(x, f32x8); }
 __device__ __forceinline__ f32x8 floats(f32x8 x) { return x; }
 // registers 4 r .. 4 r + 3: four successive rows of a result
-__device__ __forceinline__ f32x4 quad(f32x16 x, int r) { return f32x4{x[4 * r], x[4 * r + 1], x[4 * r + 2], x[4 * r + 3]}; }
+__device__ __forceinline__ f32x4 quad(f32x16 x, int r) {
+    return f32x4{x[4 * r], x[4 * r + 1], x[4 * r + 2], x[4 * r + 3]};
+}
 // a result's 16 rows of x from x[first] on (first includes 4 (lane / 32))
 __device__ __forceinline__ f32x16 rows_of(const float* x, int first) {
     f32x16 y;
@@ -126,16 +130,16 @@ __device__ __forceinline__ float add_all(bf16x8 x, float to) {
     for (int i = 0; i < 4; ++i) to = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{x[2 * i], x[2 * i + 1]}, one, to, false);
     return to;
 }
-// What this wave's lanes wrote to LDS before, its other lanes read after (LDS serves a wave in order: no instruction, only an
-// order for the compiler).
+// What this wave's lanes wrote to LDS before, its other lanes read after (LDS serves a wave in order: no instruction,
+// only an order for the compiler).
 __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 __device__ __forceinline__ float fexp2(float x) { return __builtin_amdgcn_exp2f(x); }
-// A row's log sum, ref + log2(sum) / 2, in two floats: the second is what the first one's rounding drops. With a large ref that
-// is all of log2(sum), without which each of n equal keys would have the probability 1.
+// A row's log sum, ref + log2(sum) / 2, in two floats: the second is what the first one's rounding drops. With a large
+// ref that is all of log2(sum), without which each of n equal keys would have the probability 1.
 __device__ __forceinline__ void store_lse(const SmParams& p, int64_t row, float ref, float sum) {
     const float l = 0.5f * __log2f(sum), hi = ref + l, back = hi - ref;
     if (p.lse) p.lse[row] = sum == 0.f ? __builtin_inff() : hi;
@@ -158,8 +162,10 @@ template <class T> __device__ __forceinline__ typename Elem<T>::seg load_seg(con
 }
 
 // A tile of ROWS rows of DP elements in LDS, one plane for each part, without gaps. A row's 16-byte pieces are turned
-// (exclusive or) by bits of the row's number so that the 128 bytes that LDS gives in a cycle, one piece of 8 rows or
-// the two pieces of 4 rows that a transposing read takes, are on different banks.
+// (exclusive or) by bits of the row's number, so that the two pieces of 4 rows that a transposing read takes in a cycle
+// are on different banks: at 64 elements such reads count no conflict. LDS serves 16 lanes' pieces in a cycle, of 16
+// rows when a row is read, among which the turn repeats at 64 elements: each such read takes 8 cycles for 4
+// (SQ_LDS_BANK_CONFLICT is 4 cycles a read in every kernel here).
 template <int NP, int ROWS, int DP> struct Tile {
     static constexpr int PLANE = ROWS * DP, PIECES = DP / 8;
     alignas(16) __bf16 x[NP * PLANE];
@@ -202,8 +208,8 @@ template <int NP, int ROWS, int DP> struct Tile {
 template <class T, int DP> struct Shape {
     static constexpr int NP = Elem<T>::PARTS;
     static constexpr int BN = sm_tile_rows(NP, DP);
-    // Waves a SIMD has room for. From 2 on a wave has 256 registers at most, and the compiler keeps sums in those that vector
-    // instructions can reach; with 1 it puts them in the others and copies every score.
+    // Waves a SIMD has room for. From 2 on a wave has 256 registers at most, and the compiler keeps sums in those that
+    // vector instructions can reach; with 1 it puts them in the others and copies every score.
     static constexpr int WAVES = NP == 3 && DP == 128 ? 1 : 2;
 };
 
@@ -214,9 +220,11 @@ __device__ __forceinline__ uint32_t lds_place(const void* to) {
     return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)to);
 }
 __device__ __forceinline__ void load_to_lds(const void* from, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(to), "v"(from) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 :: "s"(to), "v"(from) : "memory", "m0");
 }
-__device__ __forceinline__ void load_to_lds(const void* from, uint32_t bytes, uint32_t to) {      // from is the same for all lanes
+// from is the same for all lanes
+__device__ __forceinline__ void load_to_lds(const void* from, uint32_t bytes, uint32_t to) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                  :: "s"(to), "v"(bytes), "s"(from) : "memory", "m0");
 }
@@ -234,7 +242,8 @@ template <class T, int DP, int ROWS, int NW> struct Pair {
     struct Lds { TileT a[BUFFERS], b[BUFFERS]; };
     static_assert(alignof(Lds) >= 16, "pieces of 16 bytes are read, written and loaded");
     static constexpr int HELD = NP == 1 ? 1 : ROWS * PIECES / NT, STEP = NT / PIECES;
-    static_assert(NP == 1 || (HELD * NT == ROWS * PIECES && STEP * PIECES == NT), "a thread takes one column of HELD rows");
+    static_assert(NP == 1 || (HELD * NT == ROWS * PIECES && STEP * PIECES == NT),
+                  "a thread takes one column of HELD rows");
 
     // Rows whose pieces a lane takes: the first one, and every APART-th after it.
     static constexpr int RPI = 64 / PIECES, EACH = ROWS / RPI / NW, APART = RPI * NW;
@@ -260,16 +269,19 @@ template <class T, int DP, int ROWS, int NW> struct Pair {
         }
     }
     // tile_a, tile_b: first rows; bits: the rows to read
-    __device__ __forceinline__ void fetch(Lds& lds, int buffer, const T* tile_a, const T* tile_b, uint64_t bits, int D, int tid) {
+    __device__ __forceinline__ void fetch(Lds& lds, int buffer, const T* tile_a, const T* tile_b, uint64_t bits, int D,
+                                          int tid) {
         if (near && bits == ALL) {                         // without a test for each row
             if constexpr (NP == 1) {
                 const uint32_t to_a = lds_place(&lds.a[buffer].x[(tid >> 6) * RPI * DP]);
                 const uint32_t to_b = lds_place(&lds.b[buffer].x[(tid >> 6) * RPI * DP]);
                 if (has) {
 #pragma unroll
-                    for (int j = 0; j < EACH; ++j) load_to_lds(tile_a + j * APART * stride_a, at_a, to_a + j * APART * DP * 2);
+                    for (int j = 0; j < EACH; ++j)
+                        load_to_lds(tile_a + j * APART * stride_a, at_a, to_a + j * APART * DP * 2);
 #pragma unroll
-                    for (int j = 0; j < EACH; ++j) load_to_lds(tile_b + j * APART * stride_b, at_b, to_b + j * APART * DP * 2);
+                    for (int j = 0; j < EACH; ++j)
+                        load_to_lds(tile_b + j * APART * stride_b, at_b, to_b + j * APART * DP * 2);
                 }
             } else {
                 typedef const typename Elem<T>::seg* segs;
@@ -286,7 +298,8 @@ template <class T, int DP, int ROWS, int NW> struct Pair {
             for (int j = 0; j < EACH; ++j) {
                 const int first = (tid >> 6) * RPI + j * APART, row = first + (tid & 63) / PIECES;
                 const int slot = tid % PIECES, piece = slot ^ TileT::turn(row);
-                const uint32_t to_a = lds_place(&lds.a[buffer].x[first * DP]), to_b = lds_place(&lds.b[buffer].x[first * DP]);
+                const uint32_t to_a = lds_place(&lds.a[buffer].x[first * DP]);
+                const uint32_t to_b = lds_place(&lds.b[buffer].x[first * DP]);
                 if (piece * 8 >= D) continue;
                 if (bits >> row & 1) {
                     load_to_lds(tile_a + row * stride_a + piece * 8, to_a);
@@ -307,8 +320,8 @@ template <class T, int DP, int ROWS, int NW> struct Pair {
             }
         }
     }
-    // until here the fetched tile has arrived and nobody reads the buffer that the next fetch goes to; between two calls of it
-    // what `more` writes is read
+    // until here the fetched tile has arrived and nobody reads the buffer that the next fetch goes to; between two
+    // calls of it what `more` writes is read
     template <class F> __device__ __forceinline__ void arrive(Lds& lds, int tid, F more) {
         if constexpr (NP == 1) {
             more();
@@ -444,8 +457,10 @@ __device__ __forceinline__ Work xcd_work(int wg, int pairs, int blocks) {
 template <class F> int dispatch(int dtype, int D, F f) {
     const int DP = sm_padded(D);
     const auto at = [&](auto t) {
-        return DP == 32 ? f(t, std::integral_constant<int, 32>()) : DP == 64 ? f(t, std::integral_constant<int, 64>())
-                                                                            : f(t, std::integral_constant<int, 128>()); };
+        return DP == 32   ? f(t, std::integral_constant<int, 32>())
+               : DP == 64 ? f(t, std::integral_constant<int, 64>())
+                          : f(t, std::integral_constant<int, 128>());
+    };
     return dtype == QLKA_BF16 ? at(__bf16()) : at(float());
 }
 

@@ -358,7 +358,8 @@ std::vector<Tensor> abs_sum_autograd(const Tensor& q, const Tensor& k, const Ten
     return AbsSumFn::apply(q, k, v, path, full, keep);
 }
 
-// ---- softmax attention to a sequence of another length, and the bucketed position bias (qlka_softmax_*, qlka_bias_map_*)
+// ---- softmax attention to a sequence of another length, and the bucketed position bias (qlka_softmax_*,
+// qlka_bias_map_*)
 
 struct SoftmaxCall {
     Tensor q, k, v, table, keep;      // table and keep may be undefined
@@ -369,12 +370,15 @@ struct SoftmaxCall {
     bool both;
 };
 
-int64_t bucket_count(const std::vector<int64_t>& border, bool both) { return ((int64_t)border.size() + 1) * (both ? 2 : 1); }
+int64_t bucket_count(const std::vector<int64_t>& border, bool both) {
+    return ((int64_t)border.size() + 1) * (both ? 2 : 1);
+}
 
 void check_table(const Tensor& table, int64_t heads, const std::vector<int64_t>& border, bool both) {
     TORCH_CHECK(table.scalar_type() == at::kFloat, "table must be float32");
     TORCH_CHECK(table.dim() == 2 && table.size(0) == bucket_count(border, both) && table.size(1) == heads,
-                "table must be (num_buckets, H) = (", bucket_count(border, both), ", ", heads, "), got ", table.sizes());
+                "table must be (num_buckets, H) = (", bucket_count(border, both), ", ", heads, "), got ",
+                table.sizes());
 }
 
 void check_start(int64_t start) { TORCH_CHECK(std::abs(start) <= (1 << 28), "|start| must be <= 2^28"); }
@@ -406,7 +410,8 @@ void check_softmax(const SoftmaxCall& c) {
     }
     if (c.keep.defined()) {
         TORCH_CHECK(c.keep.device() == q.device(), "keep must be on q's device");
-        TORCH_CHECK(c.keep.scalar_type() == at::kBool || c.keep.scalar_type() == at::kByte, "keep must be bool or uint8");
+        TORCH_CHECK(c.keep.scalar_type() == at::kBool || c.keep.scalar_type() == at::kByte,
+                    "keep must be bool or uint8");
         TORCH_CHECK(c.keep.dim() == 2 && c.keep.size(0) == q.size(0) && c.keep.size(1) == k.size(2),
                     "keep must be (B, N) = (", q.size(0), ", ", k.size(2), "), got ", c.keep.sizes());
     }
@@ -461,8 +466,8 @@ void set_lse(qlka_softmax_args& a, const Tensor& lse) {
     a.lse_low = a.lse + lse.numel() / 2;
 }
 
-// (out, out before its rounding to bfloat16, the rows' log sums in two floats); the last where a gradient will be wanted,
-// the second where one through the scores will (v's needs none)
+// (out, out before its rounding to bfloat16, the rows' log sums in two floats); the last where a gradient will be
+// wanted, the second where one through the scores will (v's needs none)
 std::tuple<Tensor, Tensor, Tensor> softmax_forward(SoftmaxCall& c, bool train, bool train_scores, bool train_table) {
     check_softmax(c);
     c10::DeviceGuard guard(c.q.device());
@@ -499,7 +504,8 @@ struct SoftmaxFn : public torch::autograd::Function<SoftmaxFn> {
         SoftmaxCall c{q, k, v, table, keep, scale, causal, start, border, both};
         Tensor out, full, lse;
         const bool train_table = table.defined() && table.requires_grad();
-        std::tie(out, full, lse) = softmax_forward(c, true, q.requires_grad() || k.requires_grad() || train_table, train_table);
+        const bool train_scores = q.requires_grad() || k.requires_grad() || train_table;
+        std::tie(out, full, lse) = softmax_forward(c, true, train_scores, train_table);
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["causal"] = causal;
         ctx->saved_data["start"] = start;
@@ -553,12 +559,14 @@ struct SoftmaxFn : public torch::autograd::Function<SoftmaxFn> {
     }
 };
 
-Tensor softmax_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& table, const OptTensor& keep,
-                         double scale, bool causal, int64_t start, const std::vector<int64_t>& border, bool both) {
+Tensor softmax_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& table,
+                         const OptTensor& keep, double scale, bool causal, int64_t start,
+                         const std::vector<int64_t>& border, bool both) {
     // a call without a gradient goes around the autograd function, which would refuse a tangent
     for (const Tensor& t : {q, k, v, table.value_or(Tensor())})
         TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "softmax_attention has no forward-mode derivative");
-    if (q.dim() == 4 && k.dim() == 4 && v.dim() == 4 && q.size(3) % 8 && q.size(3) == k.size(3) && q.size(3) == v.size(3)) {
+    if (q.dim() == 4 && k.dim() == 4 && v.dim() == 4 && q.size(3) % 8 && q.size(3) == k.size(3) &&
+        q.size(3) == v.size(3)) {
         // zeros up to a multiple of 8 change no product
         const auto padded = [&](const Tensor& t) { return at::constant_pad_nd(t, {0, 8 - t.size(3) % 8}); };
         return softmax_attention(padded(q), padded(k), padded(v), table, keep, scale, causal, start, border, both)
@@ -609,7 +617,8 @@ struct BiasMapFn : public torch::autograd::Function<BiasMapFn> {
     }
 };
 
-Tensor relative_bias(const Tensor& table, int64_t M, int64_t N, int64_t start, const std::vector<int64_t>& border, bool both) {
+Tensor relative_bias(const Tensor& table, int64_t M, int64_t N, int64_t start, const std::vector<int64_t>& border,
+                     bool both) {
     return BiasMapFn::apply(table, M, N, start, border, both);
 }
 
