@@ -249,14 +249,15 @@ int qlka_layer_fwd_masked(int kind, const float* q, const float* k, const float*
  * start), keys after the query (d > 0) in buckets num_borders + 1 on, 2 (num_borders + 1) buckets in all. Else distance
  * max(-d, 0) and num_borders + 1 buckets. table and g_table are (buckets, H) fp32, contiguous.
  *
- * Forward: writes out and, where not NULL, lse (B, H, M) (half the log2 of each row's sum, +inf for a row without
- * keys), lse_low (B, H, M) (what of it lies below lse's last place: where scores are large, the log of the number of
- * keys that share a row) and out_full (with QLKA_BF16: (B, H, M, D) fp32, out before it is rounded; for the gradients'
- * row sums, in which an error of out is common to all of a row's dS). With out_full and a table the probabilities are
- * taken whole, for the table's gradient, unless table_kept is nonzero: the table will have none, and out is what the
- * same call without out_full gives. Backward: reads q, k, v, out, lse, g_out and, where not NULL, lse_low and out_full,
- * writes g_q (may be NULL), g_k and g_v (both or neither NULL) and g_table (may be NULL; with QLKA_BF16 it needs
- * out_full). No atomics: results do not change from run to run.
+ * Forward: writes out and, where not NULL, lse (B, H, M) (log2 of each row's sum, +inf for a row without keys),
+ * log_sums (2, B, H, M) (half of that log2, in two floats: the second is what lies below the first one's last place;
+ * where scores are large, it is the log of the number of keys that share a row) and out_full (with QLKA_BF16: (B, H, M,
+ * D) fp32, out before it is rounded; for the gradients' row sums, in which an error of out is common to all of a row's
+ * dS). With out_full and a table the probabilities are taken whole, for the table's gradient, unless table_kept is
+ * nonzero: the table will have none, and out is what the same call without out_full gives. Backward: reads q, k, v,
+ * out, g_out, log_sums or (for log sums of the ordinary size) lse alone and, where not NULL, out_full, writes g_q (may
+ * be NULL), g_k and g_v (both or neither NULL) and g_table (may be NULL; with QLKA_BF16 it needs out_full). No atomics:
+ * results do not change from run to run.
  */
 #define QLKA_F32  0
 #define QLKA_BF16 1
@@ -281,7 +282,7 @@ typedef struct qlka_softmax_args {
     void *g_q, *g_k, *g_v;
     int64_t g_q_stride[3], g_k_stride[3], g_v_stride[3];
     float* g_table;
-    float* lse_low;
+    float* log_sums;
     int table_kept;
 } qlka_softmax_args;
 size_t qlka_softmax_fwd_ws_bytes(const qlka_softmax_args* args);

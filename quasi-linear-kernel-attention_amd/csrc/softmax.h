@@ -34,7 +34,9 @@ struct SmParams {
     int64_t keep_stride;
     const float* table;                      // [buckets][H], or null
     float *lse, *lse_low;                    // [B][H][M], half the log2 of the row's sum, and what lies below its last
-                                             // place (may be null); +inf and 0 for a row without keys
+                                             // place; +inf and 0 for a row without keys
+    float* log2_sum;                         // [B][H][M], the log2 of the row's sum (each of these may be null)
+    float lse_unit;                          // backward: what lse is multiplied by (lse may be a log2_sum)
     float* delta;                            // [B][H][M]
     int* large;                              // [B][H][groups of 32 rows]: whether a row has a large log sum
     float* part;                             // partial rows of DP floats: [split][B * heads][rows]

@@ -74,8 +74,8 @@ constexpr int CUS = 256;
 // Splits of an axis of `tiles` tiles for `groups` workgroups over the other axes, by an estimate of the time: rounds of
 // workgroups on a CU (one alone on a CU is not twice as fast as two, waits not being filled), each its tiles and what
 // it costs by itself, and the joining of `join` bytes a split. In microseconds, the constants set by hand until 12
-// shapes (prompts and gradients of 65 to 8192 keys, fp32 and bf16) came near the best of 1 to 16 splits of all their axes:
-// eight of them within 4% of it or faster (1 x 4 heads, 100 x 8000: 14.4 us, 17.2 the best one number, 132 unsplit),
+// shapes (prompts and gradients of 65 to 8192 keys, fp32 and bf16) came near the best of 1 to 16 splits of all their
+// axes: eight of them within 4% of it or faster (1 x 4 heads, 100 x 8000: 14.4 us, 17.2 the best one number, 132 unsplit),
 // the others 7 to 18% slower (1 x 12, 512 x 4096: 26.8 : 23.7, unsplit 70; 4 x 12, 1024 x 4096: 91 : 77, unsplit 88).
 int splits_for(int64_t groups, int64_t tiles, double tile_us, double join_bytes) {
     int best = 1;
@@ -205,7 +205,10 @@ int params(const qlka_softmax_args* a, SmParams* p) {
     p->sgq = strides(a->g_q_stride); p->sgk = strides(a->g_k_stride); p->sgv = strides(a->g_v_stride);
     p->keep = a->keep; p->keep_stride = a->keep_stride;
     p->table = a->table;
-    p->lse = a->lse; p->lse_low = a->lse_low;
+    p->log2_sum = a->lse;
+    p->lse = a->log_sums;
+    p->lse_low = a->log_sums ? a->log_sums + (int64_t)a->B * a->H * a->M : nullptr;
+    p->lse_unit = 1.f;
     p->B = a->B; p->H = a->H; p->G = a->G; p->M = a->M; p->N = a->N; p->D = a->D;
     p->seen = seen_keys(a);
     p->causal = a->causal ? 1 : 0;
@@ -296,7 +299,12 @@ int qlka_softmax_bwd(const qlka_softmax_args* a, void* ws, size_t ws_bytes, void
     if (!a->g_k != !a->g_v) return refuse("g_k and g_v: both or neither");
     if (a->g_table && !a->table) return refuse("g_table needs the table");
     const bool rows = (int64_t)a->B * a->M > 0, keys = (int64_t)a->B * a->N > 0;
-    if (rows && (!a->q || !a->out || !a->lse || !a->g_out)) return refuse("q, out, lse and g_out must be non-null");
+    if (rows && (!a->q || !a->out || (!a->lse && !a->log_sums) || !a->g_out))
+        return refuse("q, out, lse or log_sums, and g_out must be non-null");
+    if (!a->log_sums) {                                 // lse alone
+        p.lse = a->lse;
+        p.lse_unit = 0.5f;
+    }
     if (keys && (!a->k || !a->v)) return refuse("k and v must be non-null");
     if (a->out_full && a->dtype == QLKA_F32) return refuse("out_full goes with QLKA_BF16");
     if (rows && a->g_table && a->dtype == QLKA_BF16 && !a->out_full)

@@ -9,7 +9,7 @@
 // does. An error of delta is in all of a row's dS alike, so it is formed from O before that is rounded to bf16. For the
 // table's gradient, which is fp32, dS is taken as it is, and O is that of P in three parts (softmax_fwd.hip, FINE).
 // The waves wait for 34 to 50% of their cycles, for the next tile and for each other. Measured: 12 x 8192 x 8192 of 64
-// with the table's gradient, bf16: softmax_dq 527 us (587 TFLOP/s), softmax_dkv 565 us (730); fp32, 32 x 4 heads of 600
+// with the table's gradient, bf16: softmax_dq 491 us (630 TFLOP/s), softmax_dkv 533 us (773); fp32, 32 x 4 heads of 600
 // to 65: 41 and 42 us; bf16 of 128, 2 x 8 x 2048 x 2048: 257 us with the forward. Registers are short: at fp32 of 64
 // elements and more, and at bf16 of 128, some values live in scratch memory.
 #include "softmax_tile.h"
@@ -43,7 +43,7 @@ __global__ __launch_bounds__(256) void softmax_delta(const SmParams p) {
             const auto g = load_seg((const T*)p.g_out + b * p.sg.b + head * p.sg.h + m * p.sg.r, d, p.D);
             const f32x8 o = p.out_full ? load_seg(p.out_full + (row0 + m) * p.D, d, p.D)
                                        : floats(load_seg(out, d, p.D));
-            large |= large_lse(p.lse[row0 + m]);
+            large |= large_lse(p.lse_unit * p.lse[row0 + m]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) x = __builtin_fmaf((float)g[j], o[j], x);
         }
@@ -176,7 +176,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
         gf[c] = frag_of(g);
     }
     delta += other_half(delta);
-    const float lse = m < p.M ? p.lse[row] : HIGH;
+    const float lse = m < p.M ? p.lse_unit * p.lse[row] : HIGH;
     const bool large = __any(large_lse(lse));
     if (split_i == 0) {                                // softmax_dkv reads them
         if (m < p.M && half == 0) p.delta[row] = delta;
@@ -433,6 +433,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
                 __syncthreads();
             }
             tile.arrive(lds, tid, [&] {
+                ls *= p.lse_unit;                          // (not where it is loaded, which would wait for it)
                 const bool wide = NP == 3 ? __any(large_lse(ls)) : all_wide;      // all rows are in the first wave
                 if (NP == 3 && tid == 0) wide_of = wide;
                 if (tid < BM) {

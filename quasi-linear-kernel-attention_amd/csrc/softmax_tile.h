@@ -142,6 +142,7 @@ __device__ __forceinline__ float fexp2(float x) { return __builtin_amdgcn_exp2f(
 // ref that is all of log2(sum), without which each of n equal keys would have the probability 1.
 __device__ __forceinline__ void store_lse(const SmParams& p, int64_t row, float ref, float sum) {
     const float l = 0.5f * __log2f(sum), hi = ref + l, back = hi - ref;
+    if (p.log2_sum) p.log2_sum[row] = sum == 0.f ? __builtin_inff() : hi + hi;
     if (p.lse) p.lse[row] = sum == 0.f ? __builtin_inff() : hi;
     if (p.lse_low) p.lse_low[row] = sum == 0.f ? 0.f : (ref - (hi - back)) + (l - back);
 }

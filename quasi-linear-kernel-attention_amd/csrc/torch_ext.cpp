@@ -461,11 +461,6 @@ qlka_softmax_args softmax_args(const SoftmaxCall& c, const std::vector<int>& bor
     return a;
 }
 
-void set_lse(qlka_softmax_args& a, const Tensor& lse) {
-    a.lse = lse.data_ptr<float>();
-    a.lse_low = a.lse + lse.numel() / 2;
-}
-
 // (out, out before its rounding to bfloat16, the rows' log sums in two floats); the last where a gradient will be
 // wanted, the second where one through the scores will (v's needs none)
 std::tuple<Tensor, Tensor, Tensor> softmax_forward(SoftmaxCall& c, bool train, bool train_scores, bool train_table) {
@@ -482,7 +477,7 @@ std::tuple<Tensor, Tensor, Tensor> softmax_forward(SoftmaxCall& c, bool train, b
     set_strides(a.out_stride, out);
     if (train) {
         lse = at::empty({2, a.B, a.H, a.M}, c.q.options().dtype(at::kFloat));
-        set_lse(a, lse);
+        a.log_sums = lse.data_ptr<float>();
         if (a.dtype == QLKA_BF16 && train_scores) {
             a.table_kept = !train_table;
             full = at::empty({a.B, a.H, a.M, a.D}, lse.options());
@@ -531,7 +526,7 @@ struct SoftmaxFn : public torch::autograd::Function<SoftmaxFn> {
         a.out = out.data_ptr();
         set_strides(a.out_stride, out);
         if (full.defined()) a.out_full = full.data_ptr<float>();
-        set_lse(a, lse);
+        a.log_sums = lse.data_ptr<float>();
         a.g_out = g.data_ptr();
         set_strides(a.g_out_stride, g);
         if (ctx->needs_input_grad(0)) {

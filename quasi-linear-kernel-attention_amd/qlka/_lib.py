@@ -33,7 +33,7 @@ class SoftmaxArgs(ctypes.Structure):
                    ("out", _c_ptr), ("out_stride", _c_i64x3), ("out_full", _c_ptr), ("lse", _c_ptr),
                    ("g_out", _c_ptr), ("g_out_stride", _c_i64x3), ("g_q", _c_ptr), ("g_k", _c_ptr), ("g_v", _c_ptr)]
                 + [(n, _c_i64x3) for n in ("g_q_stride", "g_k_stride", "g_v_stride")]
-                + [("g_table", _c_ptr), ("lse_low", _c_ptr), ("table_kept", _c_int)])
+                + [("g_table", _c_ptr), ("log_sums", _c_ptr), ("table_kept", _c_int)])
 
 
 _c_softmax = ctypes.POINTER(SoftmaxArgs)

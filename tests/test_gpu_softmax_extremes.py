@@ -5,6 +5,8 @@ A row's probabilities depend on the differences of its scores alone, so cases ar
 (equal scores, or some so much larger than the others that these weigh 0), and the oracle forms the same probabilities from
 scores of the ordinary size."""
 
+import math
+
 import pytest
 import torch
 
@@ -153,26 +155,38 @@ def test_gradients_of_large_scales_stay_finite(dev, M, dtype):
         assert (got["gv"].double().cpu().abs() <= most * (1 + 2 ** -7)).all(), scale
 
 
-def test_backward_without_the_second_part_of_the_log_sums(dev):
-    """The C entries with lse alone: what they gave before lse_low was there, right for log sums of the ordinary size."""
+def test_the_c_entries_with_lse_alone(dev):
+    """lse is the log2 of a row's sum, and enough for the backward where that is of the ordinary size."""
     import ctypes
 
     from qlka import _lib
     lib = _lib.load()
-    t = make(2, 2, 2, 50, 70, 64, F32, seed=2)
+    t = make(2, 2, 2, 50, 70, 64, F32, seed=2, keep="holes")
     want = reference(t)
     x = {n: t[n].to(dev) for n in "qkvg"}
+    keep = t["keep"].to(dev)
     r = {n: torch.empty_like(x[m]) for n, m in (("out", "q"), ("g_q", "q"), ("g_k", "k"), ("g_v", "v"))}
     lse = torch.empty(2, 2, 50, device=dev)
-    a = _lib.SoftmaxArgs(dtype=0, B=2, H=2, G=2, M=50, N=70, D=64, scale=0.125, lse=lse.data_ptr(), g_out=x["g"].data_ptr())
+    a = _lib.SoftmaxArgs(dtype=0, B=2, H=2, G=2, M=50, N=70, D=64, scale=0.125, lse=lse.data_ptr(),
+                         keep=keep.data_ptr(), keep_stride=70)
     for n, y in [(n, x[n]) for n in "qkv"] + [("g_out", x["g"])] + list(r.items()):
         setattr(a, n, y.data_ptr())
         setattr(a, n + "_stride", (ctypes.c_int64 * 3)(*y.stride()[:3]))
     stream = torch.cuda.current_stream().cuda_stream
-    for fn, need in ((lib.qlka_softmax_fwd, lib.qlka_softmax_fwd_ws_bytes), (lib.qlka_softmax_bwd, lib.qlka_softmax_bwd_ws_bytes)):
+    for fn, need in ((lib.qlka_softmax_fwd, lib.qlka_softmax_fwd_ws_bytes),
+                     (lib.qlka_softmax_bwd, lib.qlka_softmax_bwd_ws_bytes)):
         ws = torch.empty(max(need(ctypes.byref(a)), 16), dtype=torch.uint8, device=dev)
         assert fn(ctypes.byref(a), ws.data_ptr(), ws.numel(), stream) == 0
     check({"out": r["out"], "gq": r["g_q"], "gk": r["g_k"], "gv": r["g_v"]}, want)
+    s = torch.matmul(t["q"].double(), t["k"].double().transpose(-1, -2)) * 0.125
+    s = s.masked_fill(~t["keep"][:, None, None, :], float("-inf"))
+    exact = torch.logsumexp(s, -1) / math.log(2)
+    none = torch.isinf(exact)
+    assert (lse.cpu()[none] == float("inf")).all()
+    # 64 products and their sum, the change of units, up to 70 exponentials and their sum, log2 and the sum with the maximum
+    size = 0.125 * torch.matmul(t["q"].double().abs(), t["k"].double().abs().transpose(-1, -2)).amax(-1)
+    bound = oracle.U * ((64 + 16) * size * 1.5 + (2 * 70 + 32) + 4 * exact.abs())
+    assert ((lse.cpu().double() - exact).abs() <= bound)[~none].all()
 
 
 def highest(t, see, start, bias):
