@@ -11,7 +11,7 @@
 // Where the table's gradient will be wanted (FINE) they are taken in three parts of 8 bits: that gradient is fp32 and a
 // sum over rows of dS = P (dP - delta), in which an error of delta, the row sum of dO * O, does not average out. The
 // smaller parts' products then gather in a sum of their own, as in Acc (12 x 8192 x 8192: error of the table's gradient
-// 1.0e-6, 1.8e-6 without; 565 us, 260 with one part).
+// 1.0e-6, 1.8e-6 without; 476 us, 250 with one part).
 //
 // Masked keys are read as zeros (what stands there may be anything) and their tiles, where none is left, are skipped.
 // Bound by the matrix cores and by the scores' work between them (an exponential, a maximum and two multiply-adds a
@@ -28,8 +28,11 @@ namespace sm {
 
 constexpr float GROW = 4.f;          // 2^8 of the exponentials
 
+// Three parts of P leave room for three waves a SIMD (of 64 elements) only if the compiler is held to it: 476 us for 524 at
+// 12 x 8192 x 8192.
 template <class T, int DP, int NW, bool BIAS, bool FINE>
-__global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_fwd(const SmParams p) {
+__global__ __launch_bounds__(64 * NW, (FINE && DP <= 64 ? 3 : Shape<T, DP>::WAVES))
+void softmax_fwd(const SmParams p) {
     constexpr int NP = Elem<T>::PARTS, BN = Shape<T, DP>::BN, NT = 64 * NW, ROWS = 32 * NW, NS = BN / 32, ND = DP / 32;
     typedef Pair<T, DP, BN, NW> PairT;
     constexpr int BUFFERS = PairT::BUFFERS;
