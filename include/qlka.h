@@ -300,6 +300,41 @@ int qlka_bias_map_bwd(const float* g, const int* border, int num_borders, int bi
                       int M, int N, int start, void* ws, size_t ws_bytes, void* stream);
 
 /*
+ * Softmax attention within sequences of different lengths that lie one after the other in T rows (no padding). offsets
+ * (B + 1 numbers on the device, not decreasing, in [0, T]) are where the sequences begin, and where the last one ends: a
+ * row sees the keys of its own sequence, with causal those up to itself. Rows outside every sequence get zeros, here and
+ * in every gradient. No sequence changes another one's results, whatever it holds. No counterpart in the reference.
+ *
+ *   out[h,m] = sum_n P[m,n] v[h/(H/G),n],  P = softmax of scale <q[h,m], k[h/(H/G),n]> over the keys n that m sees
+ *
+ * q (H, T, D), k and v (G, T, D); *_stride are the distances in elements between heads and rows. Types, D, alignment,
+ * scale, roundings, lse, log_sums (2, H, T), out_full (H, T, D) and the gradients are as for qlka_softmax_fwd / _bwd
+ * without a table; offsets that decrease give rows that are not said, but no access outside the tensors. The offsets may
+ * change between the replays of a captured call. A launch takes less than 2^32 threads: heads * (T / 32 + B) stays below
+ * 2^24.
+ */
+typedef struct qlka_packed_args {
+    int dtype, B, H, G, T, D;
+    int causal;
+    float scale;
+    const int* offsets;
+    const void *q, *k, *v;
+    int64_t q_stride[2], k_stride[2], v_stride[2];
+    void* out;
+    int64_t out_stride[2];
+    float* out_full;
+    float* log_sums;
+    const void* g_out;
+    int64_t g_out_stride[2];
+    void *g_q, *g_k, *g_v;
+    int64_t g_q_stride[2], g_k_stride[2], g_v_stride[2];
+} qlka_packed_args;
+size_t qlka_packed_fwd_ws_bytes(const qlka_packed_args* args);
+int qlka_packed_fwd(const qlka_packed_args* args, void* ws, size_t ws_bytes, void* stream);
+size_t qlka_packed_bwd_ws_bytes(const qlka_packed_args* args);
+int qlka_packed_bwd(const qlka_packed_args* args, void* ws, size_t ws_bytes, void* stream);
+
+/*
  * Test entry: stable ascending sort of num_segs contiguous segments of seg_len fp32 keys; perm[i] is the in-segment
  * index of the i-th smallest key (np.argsort(kind="stable"); -0.0 ties +0.0 and is written as +0.0).
  * Replaces launch_iota + launch_cub_sort (Weighted_Abs_Sum/csrc/sort_utils.cu:85-117).

@@ -49,6 +49,8 @@ struct SmParams {
     float scale;                             // |scale|; its sign (or 0) is in q_sign
     float q_sign;
     SmBuckets bk;
+    const int* offsets;                      // packed sequences (softmax_packed_*): segments.h; then B is 1, M and N are
+    int sequences, groups;                   // the rows of all, and `large` has `groups` numbers a head
 };
 
 // Elements of a row in LDS and in the partial rows.
@@ -60,6 +62,8 @@ inline int sm_buckets(const SmBuckets& b) { return (b.n + 1) * (b.both ? 2 : 1);
 // Launchers; each returns a hipError_t value. The dtype is QLKA_F32 or QLKA_BF16.
 constexpr int FWD_WAVES = 4;              // waves a workgroup of the forward's kernels, of tiles and of single tokens
 int sm_fwd(int dtype, const SmParams& p, hipStream_t st);
+// the same for packed sequences (no mask, no bias), waves (of 32 rows) a workgroup: 1 or 4
+int sm_packed_fwd(int dtype, const SmParams& p, int waves, hipStream_t st);
 // waves (of 32 rows) a workgroup: 2 or 4
 constexpr int STEP_MOST = 4;              // query rows a key head that sm_step takes
 int sm_step(int dtype, const SmParams& p, hipStream_t st);
@@ -67,6 +71,8 @@ int sm_combine(int dtype, const SmParams& p, hipStream_t st);
 int sm_delta(int dtype, const SmParams& p, hipStream_t st);
 int sm_dq(int dtype, const SmParams& p, int waves, hipStream_t st);
 int sm_dkv(int dtype, const SmParams& p, int waves, hipStream_t st);
+int sm_packed_dq(int dtype, const SmParams& p, int waves, hipStream_t st);
+int sm_packed_dkv(int dtype, const SmParams& p, int waves, hipStream_t st);
 // out[row] = scale * sum over the splits of part's rows; rows of heads x len per batch
 int sm_sum_parts(int dtype, const float* part, void* out, SmStrides so, float scale, int splits, int B, int heads,
                  int len, int D, hipStream_t st);

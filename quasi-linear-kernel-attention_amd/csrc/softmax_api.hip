@@ -1,39 +1,10 @@
 // The C ABI of softmax attention and of the bias map (include/qlka.h): validation, the choice of kernel and split, the
 // workspace and the launches.
-#include "qlka.h"
-#include "qlka_internal.h"
-#include "softmax.h"
-
-#include <algorithm>
-#include <cmath>
-#include <cstdarg>
-#include <cstdio>
+#include "api_checks.h"
 
 using namespace qlka;
 
 namespace {
-
-constexpr int64_t LONGEST = 1 << 28;      // rows, keys, positions: sums of a few stay in 32 bits
-constexpr int64_t MOST_ROWS = INT32_MAX;
-
-int refuse(const char* fmt, ...) {
-    char buf[256];
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(buf, sizeof(buf), fmt, ap);
-    va_end(ap);
-    return api_error(QLKA_EINVAL, buf);
-}
-
-int status(int e, const char* where) {
-    if (e == 0) return QLKA_OK;
-    char buf[256];
-    snprintf(buf, sizeof(buf), "%s: %s", where, hipGetErrorString((hipError_t)e));
-    return api_error(QLKA_EHIP, buf);
-}
-
-size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 int check_buckets(const int* border, int n, int both, SmBuckets* bk) {
     const int most = both ? QLKA_MAX_BUCKETS / 2 : QLKA_MAX_BUCKETS;
@@ -61,37 +32,12 @@ int check_sizes(const qlka_softmax_args* a) {
         return refuse("M, N and |start| must be <= 2^28");
     if ((double)a->B * a->H * a->M > (double)MOST_ROWS || (double)a->B * a->G * a->N > (double)MOST_ROWS)
         return refuse("B * H * M and B * G * N must fit int32");
-    // the gradients hold log sums in units of the scale
-    if (a->scale != 0.f && !(std::fabs(a->scale) >= 0x1p-96f && std::fabs(a->scale) <= 0x1p96f))
-        return refuse("scale must be 0 or of a size in [2^-96, 2^96]");
-    return QLKA_OK;
+    return check_scale(a->scale);
 }
 
 // ---- how a call runs
 
-constexpr int CUS = 256;
-
-// Splits of an axis of `tiles` tiles for `groups` workgroups over the other axes, by an estimate of the time: rounds of
-// workgroups on a CU (one alone on a CU is not twice as fast as two, waits not being filled), each its tiles and what
-// it costs by itself, and the joining of `join` bytes a split. In microseconds, the constants set by hand until 12
-// shapes (prompts and gradients of 65 to 8192 keys, fp32 and bf16) came near the best of 1 to 16 splits of all their
-// axes: eight of them within 4% of it or faster (1 x 4 heads, 100 x 8000: 14.4 us, 17.2 the best one number, 132 unsplit),
-// the others 7 to 18% slower (1 x 12, 512 x 4096: 26.8 : 23.7, unsplit 70; 4 x 12, 1024 x 4096: 91 : 77, unsplit 88).
-int splits_for(int64_t groups, int64_t tiles, double tile_us, double join_bytes) {
-    int best = 1;
-    double least = 0;
-    for (int s = 1; s <= 64 && (s == 1 || 2 * s <= tiles); ++s) {
-        const double rounds = std::max<double>(1.7, (double)ceil_div(groups * s, CUS));
-        double t = rounds * (2.0 + tile_us * ceil_div(tiles, s));
-        if (s > 1) t += 4.0 + s * join_bytes / 2e6;
-        if (s == 1 || t < 0.95 * least) {
-            best = s;
-            least = t;
-        }
-    }
-    return best;
-}
-// The same for the kernel of few rows, which is bound by memory: enough workgroups to fill the GPU, four tiles each or
+// Splits of the keys for the kernel of few rows, which is bound by memory: enough workgroups to fill the GPU, four tiles each or
 // more.
 int step_splits(int64_t groups, int64_t tiles) {
     if (groups >= 1024) return 1;
@@ -181,18 +127,9 @@ BwdPlan bwd_plan(const qlka_softmax_args* a, bool dq, bool dkv, bool table) {
 
 SmStrides strides(const int64_t* s) { return {s[0], s[1], s[2]}; }
 
-// Rows are read and written in pieces of 16 bytes, those of a tile at unsigned offsets from its first one.
-int check_rows(const qlka_softmax_args* a, const char* name, const void* x, const int64_t* s, int heads, int rows) {
-    const int64_t piece = a->dtype == QLKA_F32 ? 4 : 8;
-    if (!x) return QLKA_OK;
-    const int sizes[3] = {a->B, heads, rows};
-    bool aligned = (uintptr_t)x % 16 == 0;
-    for (int i = 0; i < 3; ++i) {
-        if (sizes[i] <= 1) continue;
-        if (s[i] < 0) return refuse("the strides of %s must not be negative", name);
-        aligned = aligned && s[i] % piece == 0;
-    }
-    return aligned ? QLKA_OK : refuse("the rows of %s must be aligned to 16 bytes", name);
+int rows_of(const qlka_softmax_args* a, const char* name, const void* x, const int64_t* s, int heads, int rows) {
+    const int64_t sizes[3] = {a->B, heads, rows};
+    return check_rows(name, x, s, sizes, 3, a->dtype == QLKA_F32 ? 4 : 2);
 }
 
 int params(const qlka_softmax_args* a, SmParams* p) {
@@ -223,25 +160,10 @@ int params(const qlka_softmax_args* a, SmParams* p) {
         {"g_out", a->g_out, a->g_out_stride, a->H, a->M}, {"g_q", a->g_q, a->g_q_stride, a->H, a->M},
         {"g_k", a->g_k, a->g_k_stride, a->G, a->N},    {"g_v", a->g_v, a->g_v_stride, a->G, a->N}};
     for (const auto& o : all)
-        if (int e = check_rows(a, o.name, o.x, o.s, o.heads, o.rows)) return e;
+        if (int e = rows_of(a, o.name, o.x, o.s, o.heads, o.rows)) return e;
     if ((uintptr_t)a->out_full % 16) return refuse("out_full must be aligned to 16 bytes");
     return a->table ? check_buckets(a->border, a->num_borders, a->bidirectional, &p->bk) : QLKA_OK;
 }
-
-int need_ws(const void* ws, size_t have, size_t need) {
-    if (need == 0) return QLKA_OK;
-    if (ws && have >= need && (uintptr_t)ws % 16 == 0) return QLKA_OK;
-    return api_error(QLKA_EWORKSPACE, "workspace too small, null or not aligned to 16 bytes");
-}
-
-// A launch takes less than 2^32 threads.
-int fits_grid(int64_t groups, int threads) {
-    if (groups <= (int64_t)UINT32_MAX / threads) return QLKA_OK;
-    return refuse("too many workgroups: %lld of %d threads, a launch takes less than 2^32 threads", (long long)groups,
-                  threads);
-}
-// a kernel of workgroups of 256 that takes `lanes` lanes a row
-int fits_rows(int64_t rows, int lanes) { return fits_grid(ceil_div(rows * lanes, 256), 256); }
 
 }  // namespace
 

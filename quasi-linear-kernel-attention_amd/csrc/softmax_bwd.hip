@@ -116,7 +116,7 @@ template <int NP, class F> __device__ __forceinline__ void by_size(bool large, F
     f(std::false_type());
 }
 
-template <class T, int DP, int NW, bool BIAS>
+template <class T, int DP, int NW, bool BIAS, bool PACKED>
 __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(const SmParams p) {
     constexpr int NP = Elem<T>::PARTS, BN = Shape<T, DP>::BN, NT = 64 * NW, ROWS = 32 * NW, NS = BN / 32, ND = DP / 32;
     typedef Pair<T, DP, BN, NW> PairT;
@@ -129,20 +129,23 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
     const Work w = xcd_work(blockIdx.x, p.B * p.H, p.blocks * p.splits);
-    const int block = w.block % p.blocks, split_i = w.block / p.blocks;
+    const int split_i = w.block / p.blocks;
+    const Span<PACKED> span(p, w.block % p.blocks, ROWS);
     const int head = w.pair % p.H, b = w.pair / p.H, kvh = head / (p.H / p.G);
-    const int m0 = block * ROWS, mw = m0 + wave * 32, m = mw + col;
-    const T* k = (const T*)p.k + b * p.sk.b + kvh * p.sk.h;
-    const T* v = (const T*)p.v + b * p.sv.b + kvh * p.sv.h;
-    const int64_t row = ((int64_t)b * p.H + head) * p.M + m;
+    const int m0 = span.block * ROWS, mw = m0 + wave * 32, m = mw + col;
+    if (PACKED && m0 >= span.M()) return;
+    const T* k = span.from((const T*)p.k + b * p.sk.b + kvh * p.sk.h, p.sk.r);
+    const T* v = span.from((const T*)p.v + b * p.sv.b + kvh * p.sv.h, p.sv.r);
+    const auto at_m = span.row(m);
+    const int64_t row = ((int64_t)b * p.H + head) * p.M + at_m;
 
-    const int tiles = (p.seen + BN - 1) / BN;
+    const int tiles = (span.seen() + BN - 1) / BN;
     int t0 = (int)((int64_t)tiles * split_i / p.splits), t1 = (int)((int64_t)tiles * (split_i + 1) / p.splits);
     if (p.causal) {
-        const int last = min(m0 + ROWS, p.M) - 1 + p.start;
+        const int last = min(m0 + ROWS, span.M()) - 1 + p.start;
         t1 = min(t1, last < 0 ? 0 : last / BN + 1);
     }
-    KeyBits<BN> seen(p, b);
+    KeyBits<BN> seen = span.template keys<BN>(b);
     PairT tile(lds, p.sk.r, p.sv.r, p.D, tid);
     const auto fetch = [&](int t, uint64_t bits, int buffer) {
         tile.fetch(lds, buffer, k + (int64_t)t * BN * p.sk.r, v + (int64_t)t * BN * p.sv.r, bits, p.D, tid);
@@ -162,11 +165,11 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
         const int d = 16 * c + 8 * half;
         typename Elem<T>::seg s = {}, g = {};
         f32x8 o = {};
-        if (m < p.M) {
-            s = load_seg((const T*)p.q + b * p.sq.b + head * p.sq.h + m * p.sq.r, d, p.D);
-            g = load_seg((const T*)p.g_out + b * p.sg.b + head * p.sg.h + m * p.sg.r, d, p.D);
+        if (m < span.M()) {
+            s = load_seg((const T*)p.q + b * p.sq.b + head * p.sq.h + at_m * p.sq.r, d, p.D);
+            g = load_seg((const T*)p.g_out + b * p.sg.b + head * p.sg.h + at_m * p.sg.r, d, p.D);
             o = p.out_full ? load_seg(p.out_full + row * p.D, d, p.D)
-                           : floats(load_seg((const T*)p.out + b * p.so.b + head * p.so.h + m * p.so.r, d, p.D));
+                           : floats(load_seg((const T*)p.out + b * p.so.b + head * p.so.h + at_m * p.so.r, d, p.D));
         }
         s = s * (T)p.q_sign;
         qf[c] = frag_of(s);
@@ -176,11 +179,12 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
         gf[c] = frag_of(g);
     }
     delta += other_half(delta);
-    const float lse = m < p.M ? p.lse_unit * p.lse[row] : HIGH;
+    const float lse = m < span.M() ? p.lse_unit * p.lse[row] : HIGH;
     const bool large = __any(large_lse(lse));
     if (split_i == 0) {                                // softmax_dkv reads them
-        if (m < p.M && half == 0) p.delta[row] = delta;
-        if (mw < p.M && lane == 0) p.large[((int64_t)b * p.H + head) * ((p.M + 31) / 32) + mw / 32] = large;
+        if (m < span.M() && half == 0) p.delta[row] = delta;
+        if (mw < span.M() && lane == 0) p.large[PACKED ? (int64_t)head * p.groups + span.group + mw / 32
+                                                : ((int64_t)b * p.H + head) * ((p.M + 31) / 32) + mw / 32] = large;
     }
     const int buckets = (p.bk.n + 1) * (p.bk.both ? 2 : 1);
     float left = 0.f, right = 0.f;                     // this lane's sums far below and far above the diagonal
@@ -226,7 +230,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
             buffer ^= BUFFERS - 1;
             coming = seen.find(++t, t1);
             if (coming) fetch(t, coming, buffer);
-            if (mw >= p.M || (p.causal && n0 > mw + 31 + p.start)) continue;
+            if (mw >= span.M() || (p.causal && n0 > mw + 31 + p.start)) continue;
 
             const bool edge = p.causal && n0 + BN - 1 > mw + p.start;
             const int lim = m + p.start - n0 - 4 * half;                     // at an edge, the last key seen
@@ -267,7 +271,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
                             for (int r = 0; r < 16; ++r) s[i][r] = __builtin_fmaf(s[i][r], c1, far);
                         }
                         if (wide) {
-                            const float low = m < p.M && p.lse_low ? p.lse_low[row] : 0.f;
+                            const float low = m < span.M() && p.lse_low ? p.lse_low[row] : 0.f;
 #pragma unroll
                             for (int r = 0; r < 16; ++r) s[i][r] = at_most_0((s[i][r] - lse) - low);
                         }
@@ -327,14 +331,14 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
         }
         __syncthreads();
         const int64_t count = (int64_t)p.B * p.splits * p.blocks;
-        float* part = p.part_table + (head * count + ((int64_t)b * p.splits + split_i) * p.blocks + block) * buckets;
+        float* part = p.part_table + (head * count + ((int64_t)b * p.splits + split_i) * p.blocks + span.block) * buckets;
         for (int i = tid; i < buckets; i += NT) {
             float a = 0.f;
             for (int j = 0; j < NW; ++j) a += sums[j][i];
             part[i] = a;
         }
     }
-    if (m >= p.M || !p.g_q) return;
+    if (m >= span.M() || !p.g_q) return;
     const float f = p.scale * p.q_sign;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -345,11 +349,11 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
             if (p.splits > 1)
                 *reinterpret_cast<f32x4*>(p.part + ((int64_t)split_i * p.B * p.H * p.M + row) * DP + at) = x;
             else
-                store4((T*)p.g_q + b * p.sgq.b + head * p.sgq.h + m * p.sgq.r, at, p.D, x * f);
+                store4((T*)p.g_q + b * p.sgq.b + head * p.sgq.h + at_m * p.sgq.r, at, p.D, x * f);
         }
 }
 
-template <class T, int DP, int NW, bool BIAS>
+template <class T, int DP, int NW, bool BIAS, bool PACKED>
 __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(const SmParams p) {
     constexpr int NP = Elem<T>::PARTS, BM = Shape<T, DP>::BN, NT = 64 * NW, KEYS = 32 * NW, NS = BM / 32, ND = DP / 32;
     typedef Pair<T, DP, BM, NW> PairT;
@@ -362,14 +366,17 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
     const Work w = xcd_work(blockIdx.x, p.B * p.G, p.blocks * p.splits);
-    const int block = w.block % p.blocks, split_i = w.block / p.blocks;
+    const int split_i = w.block / p.blocks;
+    const Span<PACKED> span(p, w.block % p.blocks, KEYS);
     const int kvh = w.pair % p.G, b = w.pair / p.G, share = p.H / p.G;
-    const int n0 = block * KEYS, nw = n0 + wave * 32, n = nw + col;
-    const bool shown = n < p.seen && (!p.keep || p.keep[b * p.keep_stride + n]);
+    const int n0 = span.block * KEYS, nw = n0 + wave * 32, n = nw + col;
+    if (PACKED && n0 >= span.N()) return;
+    const auto at_n = span.row(n);
+    const bool shown = n < span.seen() && (!p.keep || p.keep[b * p.keep_stride + n]);
     const bool idle = !__any(shown);
 
     // the tiles of queries of all heads that share these keys, one after the other
-    const int tiles = (p.M + BM - 1) / BM;
+    const int M = PACKED ? span.seen() : p.M, tiles = (M + BM - 1) / BM;
     const int64_t work = (int64_t)tiles * share;
     const int t1 = (int)(work * (split_i + 1) / p.splits);
     const auto next = [&](int t) {                     // the first tile from t on with a query that sees a key here
@@ -380,14 +387,14 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
     PairT tile(lds, p.sq.r, p.sg.r, p.D, tid);
     float ls = HIGH, des = 0.f;
     const auto fetch = [&](int t, int buffer) {
-        const int head = kvh * share + t / tiles, m0 = t % tiles * BM, left = p.M - m0;
+        const int head = kvh * share + t / tiles, m0 = t % tiles * BM, left = M - m0;
         const uint64_t bits = left >= BM ? PairT::ALL : (1ull << left) - 1;
-        tile.fetch(lds, buffer, (const T*)p.q + b * p.sq.b + head * p.sq.h + m0 * p.sq.r,
-                   (const T*)p.g_out + b * p.sg.b + head * p.sg.h + m0 * p.sg.r, bits, p.D, tid);
+        tile.fetch(lds, buffer, (const T*)p.q + b * p.sq.b + head * p.sq.h + span.row(m0) * p.sq.r,
+                   (const T*)p.g_out + b * p.sg.b + head * p.sg.h + span.row(m0) * p.sg.r, bits, p.D, tid);
         ls = HIGH;
         des = 0.f;
         if (tid < BM && tid < left) {
-            const int64_t row = ((int64_t)b * p.H + head) * p.M + m0 + tid;
+            const int64_t row = ((int64_t)b * p.H + head) * p.M + span.row(m0) + tid;
             ls = p.lse[row];
             des = p.delta[row];
         }
@@ -399,18 +406,22 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
     for (int c = 0; c < DP / 16; ++c) {
         typename Elem<T>::seg s = {}, x = {};
         if (shown) {
-            s = load_seg((const T*)p.k + b * p.sk.b + kvh * p.sk.h + n * p.sk.r, 16 * c + 8 * half, p.D);
-            x = load_seg((const T*)p.v + b * p.sv.b + kvh * p.sv.h + n * p.sv.r, 16 * c + 8 * half, p.D);
+            s = load_seg((const T*)p.k + b * p.sk.b + kvh * p.sk.h + at_n * p.sk.r, 16 * c + 8 * half, p.D);
+            x = load_seg((const T*)p.v + b * p.sv.b + kvh * p.sv.h + at_n * p.sv.r, 16 * c + 8 * half, p.D);
         }
         s = s * (T)p.q_sign;
         kf[c] = frag_of(s);
         vf[c] = frag_of(x);
     }
 
-    const int groups = share * ((p.M + 31) / 32);      // of 32 rows of the heads that share these keys
+    const int a_head = (M + 31) / 32, groups = share * a_head;       // of 32 rows of the heads that share these keys
     bool any_large = false;
     if constexpr (NP == 1) {
-        for (int i = tid; i < groups; i += NT) any_large |= p.large[((int64_t)b * p.G + kvh) * groups + i] != 0;
+        for (int i = tid; i < groups; i += NT) {
+            const int64_t at = PACKED ? (int64_t)(kvh * share + i / a_head) * p.groups + span.group + i % a_head
+                                      : ((int64_t)b * p.G + kvh) * groups + i;
+            any_large |= p.large[at] != 0;
+        }
         any_large = __syncthreads_or(any_large);
     }
 
@@ -441,8 +452,8 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
                     delta[tid] = -des;
                     if (wide) {
                         two[0][tid] = ls;
-                        const int64_t row = ((int64_t)b * p.H + head) * p.M + m0 + tid;
-                        two[1][tid] = p.lse_low && m0 + tid < p.M ? p.lse_low[row] : 0.f;
+                        const int64_t row = ((int64_t)b * p.H + head) * p.M + span.row(m0) + tid;
+                        two[1][tid] = p.lse_low && m0 + tid < M ? p.lse_low[row] : 0.f;
                     }
                 }
                 if constexpr (BIAS) {
@@ -547,13 +558,13 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
                     }
                 }
             };
-            by_halves<NP, NS>(m0 + 32 >= p.M, halves);
+            by_halves<NP, NS>(m0 + 32 >= M, halves);
         }
     };
     by_size<NP>(any_large, go);
-    if (n >= p.N) return;
+    if (n >= span.N()) return;
     const float f = p.scale * p.q_sign;
-    const int64_t row = ((int64_t)b * p.G + kvh) * p.N + n, all = (int64_t)p.B * p.G * p.N;
+    const int64_t row = ((int64_t)b * p.G + kvh) * p.N + at_n, all = (int64_t)p.B * p.G * p.N;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -565,8 +576,8 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
                 *reinterpret_cast<f32x4*>(p.part + (split_i * all + row) * DP + at) = x;
                 *reinterpret_cast<f32x4*>(p.part2 + (split_i * all + row) * DP + at) = y;
             } else {
-                store4((T*)p.g_k + b * p.sgk.b + kvh * p.sgk.h + n * p.sgk.r, at, p.D, x * f);
-                store4((T*)p.g_v + b * p.sgv.b + kvh * p.sgv.h + n * p.sgv.r, at, p.D, y);
+                store4((T*)p.g_k + b * p.sgk.b + kvh * p.sgk.h + at_n * p.sgk.r, at, p.D, x * f);
+                store4((T*)p.g_v + b * p.sgv.b + kvh * p.sgv.h + at_n * p.sgv.r, at, p.D, y);
             }
         }
 }
@@ -605,14 +616,24 @@ template <class T, int DP> int run_delta(const SmParams& p, hipStream_t st) {
 }
 template <class T, int DP, int NW> int run_dq(const SmParams& p, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)p.B * p.H * p.blocks * p.splits));
-    if (p.table) softmax_dq<T, DP, NW, true><<<grid, 64 * NW, 0, st>>>(p);
-    else softmax_dq<T, DP, NW, false><<<grid, 64 * NW, 0, st>>>(p);
+    if (p.table) softmax_dq<T, DP, NW, true, false><<<grid, 64 * NW, 0, st>>>(p);
+    else softmax_dq<T, DP, NW, false, false><<<grid, 64 * NW, 0, st>>>(p);
     return (int)hipGetLastError();
 }
 template <class T, int DP, int NW> int run_dkv(const SmParams& p, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)p.B * p.G * p.blocks * p.splits));
-    if (p.table) softmax_dkv<T, DP, NW, true><<<grid, 64 * NW, 0, st>>>(p);
-    else softmax_dkv<T, DP, NW, false><<<grid, 64 * NW, 0, st>>>(p);
+    if (p.table) softmax_dkv<T, DP, NW, true, false><<<grid, 64 * NW, 0, st>>>(p);
+    else softmax_dkv<T, DP, NW, false, false><<<grid, 64 * NW, 0, st>>>(p);
+    return (int)hipGetLastError();
+}
+template <class T, int DP, int NW> int run_packed_dq(const SmParams& p, hipStream_t st) {
+    const dim3 grid((unsigned)((int64_t)p.H * p.blocks * p.splits));
+    softmax_dq<T, DP, NW, false, true><<<grid, 64 * NW, 0, st>>>(p);
+    return (int)hipGetLastError();
+}
+template <class T, int DP, int NW> int run_packed_dkv(const SmParams& p, hipStream_t st) {
+    const dim3 grid((unsigned)((int64_t)p.G * p.blocks * p.splits));
+    softmax_dkv<T, DP, NW, false, true><<<grid, 64 * NW, 0, st>>>(p);
     return (int)hipGetLastError();
 }
 template <class T, int DP> int run_sum(const float* part, void* out, SmStrides so, float scale, int splits, int B,
@@ -639,6 +660,18 @@ int sm_dkv(int dtype, const SmParams& p, int waves, hipStream_t st) {
     return sm::dispatch(dtype, p.D, [&](auto t, auto dp) {
         return waves == 2 ? sm::run_dkv<decltype(t), dp.value, 2>(p, st)
                           : sm::run_dkv<decltype(t), dp.value, 4>(p, st); });
+}
+
+int sm_packed_dq(int dtype, const SmParams& p, int waves, hipStream_t st) {
+    return sm::dispatch(dtype, p.D, [&](auto t, auto dp) {
+        return waves == 2 ? sm::run_packed_dq<decltype(t), dp.value, 2>(p, st)
+                          : sm::run_packed_dq<decltype(t), dp.value, 4>(p, st); });
+}
+
+int sm_packed_dkv(int dtype, const SmParams& p, int waves, hipStream_t st) {
+    return sm::dispatch(dtype, p.D, [&](auto t, auto dp) {
+        return waves == 2 ? sm::run_packed_dkv<decltype(t), dp.value, 2>(p, st)
+                          : sm::run_packed_dkv<decltype(t), dp.value, 4>(p, st); });
 }
 
 int sm_sum_parts(int dtype, const float* part, void* out, SmStrides so, float scale, int splits, int B, int heads,

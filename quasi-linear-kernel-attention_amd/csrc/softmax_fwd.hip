@@ -30,7 +30,7 @@ constexpr float GROW = 4.f;          // 2^8 of the exponentials
 
 // Three parts of P leave room for three waves a SIMD (of 64 elements) only if the compiler is held to it: 476 us for 524 at
 // 12 x 8192 x 8192.
-template <class T, int DP, int NW, bool BIAS, bool FINE>
+template <class T, int DP, int NW, bool BIAS, bool FINE, bool PACKED>
 __global__ __launch_bounds__(64 * NW, (FINE && DP <= 64 ? 3 : Shape<T, DP>::WAVES))
 void softmax_fwd(const SmParams p) {
     constexpr int NP = Elem<T>::PARTS, BN = Shape<T, DP>::BN, NT = 64 * NW, ROWS = 32 * NW, NS = BN / 32, ND = DP / 32;
@@ -43,20 +43,22 @@ void softmax_fwd(const SmParams p) {
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
     const Work w = xcd_work(blockIdx.x, p.B * p.H, p.blocks * p.splits);
-    const int block = w.block % p.blocks, split_i = w.block / p.blocks;
+    const int split_i = w.block / p.blocks;
+    const Span<PACKED> span(p, w.block % p.blocks, ROWS);
     const int head = w.pair % p.H, b = w.pair / p.H, kvh = head / (p.H / p.G);
-    const int m0 = block * ROWS, mw = m0 + wave * 32, m = mw + col;
-    const T* q = (const T*)p.q + b * p.sq.b + head * p.sq.h;
-    const T* k = (const T*)p.k + b * p.sk.b + kvh * p.sk.h;
-    const T* v = (const T*)p.v + b * p.sv.b + kvh * p.sv.h;
+    const int m0 = span.block * ROWS, mw = m0 + wave * 32, m = mw + col;
+    if (PACKED && m0 >= span.M()) return;
+    const T* q = span.from((const T*)p.q + b * p.sq.b + head * p.sq.h, p.sq.r);
+    const T* k = span.from((const T*)p.k + b * p.sk.b + kvh * p.sk.h, p.sk.r);
+    const T* v = span.from((const T*)p.v + b * p.sv.b + kvh * p.sv.h, p.sv.r);
 
-    const int tiles = (p.seen + BN - 1) / BN;
+    const int tiles = (span.seen() + BN - 1) / BN;
     int t0 = (int)((int64_t)tiles * split_i / p.splits), t1 = (int)((int64_t)tiles * (split_i + 1) / p.splits);
     if (p.causal) {
-        const int last = min(m0 + ROWS, p.M) - 1 + p.start;          // the last key that a row here sees
+        const int last = min(m0 + ROWS, span.M()) - 1 + p.start;          // the last key that a row here sees
         t1 = min(t1, last < 0 ? 0 : last / BN + 1);
     }
-    KeyBits<BN> seen(p, b);
+    KeyBits<BN> seen = span.template keys<BN>(b);
     PairT tile(lds, p.sk.r, p.sv.r, p.D, tid);
     const auto fetch = [&](int t, uint64_t bits, int buffer) {
         tile.fetch(lds, buffer, k + (int64_t)t * BN * p.sk.r, v + (int64_t)t * BN * p.sv.r, bits, p.D, tid);
@@ -69,7 +71,7 @@ void softmax_fwd(const SmParams p) {
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
         typename Elem<T>::seg s = {};
-        if (m < p.M) s = load_seg(q + m * p.sq.r, 16 * c + 8 * half, p.D);
+        if (m < span.M()) s = load_seg(q + m * p.sq.r, 16 * c + 8 * half, p.D);
         s = s * (T)p.q_sign;
         qf[c] = frag_of(s);
     }
@@ -108,7 +110,7 @@ void softmax_fwd(const SmParams p) {
         buffer ^= BUFFERS - 1;
         coming = seen.find(++t, t1);
         if (coming) fetch(t, coming, buffer);
-        if (mw >= p.M || (p.causal && n0 > mw + 31 + p.start)) continue;
+        if (mw >= span.M() || (p.causal && n0 > mw + 31 + p.start)) continue;
 
         f32x16 s[NS];
 #pragma unroll
@@ -232,9 +234,9 @@ void softmax_fwd(const SmParams p) {
         if (__builtin_expect(wide, 0)) weigh(std::true_type());
         else weigh(std::false_type());
     }
-    if (m >= p.M) return;
+    if (m >= span.M()) return;
     sum += other_half(sum);
-    const int64_t row = ((int64_t)b * p.H + head) * p.M + m;
+    const int64_t row = ((int64_t)b * p.H + head) * p.M + span.row(m);
     if (p.splits > 1) {
         const int64_t at = (int64_t)split_i * p.B * p.H * p.M + row;
 #pragma unroll
@@ -250,7 +252,7 @@ void softmax_fwd(const SmParams p) {
         return;
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    T* out = (T*)p.out + b * p.so.b + head * p.so.h + m * p.so.r;
+    T* out = (T*)p.out + b * p.so.b + head * p.so.h + span.row(m) * p.so.r;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -265,9 +267,14 @@ void softmax_fwd(const SmParams p) {
 template <class T, int DP, int NW> int launch_fwd(const SmParams& p, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)p.B * p.H * p.blocks * p.splits));
     const bool fine = sizeof(T) == 2 && p.table && p.out_full && !p.table_kept;
-    if (fine) softmax_fwd<T, DP, NW, true, sizeof(T) == 2><<<grid, 64 * NW, 0, st>>>(p);
-    else if (p.table) softmax_fwd<T, DP, NW, true, false><<<grid, 64 * NW, 0, st>>>(p);
-    else softmax_fwd<T, DP, NW, false, false><<<grid, 64 * NW, 0, st>>>(p);
+    if (fine) softmax_fwd<T, DP, NW, true, sizeof(T) == 2, false><<<grid, 64 * NW, 0, st>>>(p);
+    else if (p.table) softmax_fwd<T, DP, NW, true, false, false><<<grid, 64 * NW, 0, st>>>(p);
+    else softmax_fwd<T, DP, NW, false, false, false><<<grid, 64 * NW, 0, st>>>(p);
+    return (int)hipGetLastError();
+}
+template <class T, int DP, int NW> int launch_packed(const SmParams& p, hipStream_t st) {
+    const dim3 grid((unsigned)((int64_t)p.H * p.blocks * p.splits));
+    softmax_fwd<T, DP, NW, false, false, true><<<grid, 64 * NW, 0, st>>>(p);
     return (int)hipGetLastError();
 }
 // Joins the splits of a row, a wave a row: first a lane for each split's maximum and sum, then DP / 4 lanes for each of
@@ -380,6 +387,12 @@ template <class T, int DP> int launch_combine(const SmParams& p, hipStream_t st)
 int sm_fwd(int dtype, const SmParams& p, hipStream_t st) {
     return sm::dispatch(dtype, p.D, [&](auto t, auto dp) {
         return sm::launch_fwd<decltype(t), dp.value, FWD_WAVES>(p, st); });
+}
+
+int sm_packed_fwd(int dtype, const SmParams& p, int waves, hipStream_t st) {
+    return sm::dispatch(dtype, p.D, [&](auto t, auto dp) {
+        return waves == 1 ? sm::launch_packed<decltype(t), dp.value, 1>(p, st)
+                          : sm::launch_packed<decltype(t), dp.value, FWD_WAVES>(p, st); });
 }
 
 int sm_combine(int dtype, const SmParams& p, hipStream_t st) {

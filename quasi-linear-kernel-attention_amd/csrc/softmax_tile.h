@@ -18,6 +18,7 @@
 #include <cstdint>
 #include <type_traits>
 
+#include "segments.h"
 #include "softmax.h"
 
 namespace qlka {
@@ -360,6 +361,7 @@ template <int BN> struct KeyBits {
 
     __device__ __forceinline__ KeyBits(const SmParams& p, int b)
         : keep(p.keep ? p.keep + b * p.keep_stride : nullptr), N(p.seen), window(-1), bits(0) {}
+    __device__ __forceinline__ explicit KeyBits(int N) : keep(nullptr), N(N), window(-1), bits(0) {}
 
     __device__ __forceinline__ void look(int w) {
         if (w == window) return;
@@ -453,6 +455,40 @@ __device__ __forceinline__ Work xcd_work(int wg, int pairs, int blocks) {
     const int rest = wg - 8 * full;
     return {(pairs & ~7) + rest / blocks, rest % blocks};
 }
+
+// The rows that a workgroup works on: its block of those of a pair, or, in a packed call, of those of one sequence.
+template <bool PACKED> struct Span;
+template <> struct Span<false> {
+    const SmParams& p;
+    int block;
+    static constexpr int group = 0;
+    __device__ __forceinline__ Span(const SmParams& p, int block, int) : p(p), block(block) {}
+    __device__ __forceinline__ int M() const { return p.M; }
+    __device__ __forceinline__ int N() const { return p.N; }
+    __device__ __forceinline__ int seen() const { return p.seen; }
+    __device__ __forceinline__ int row(int i) const { return i; }          // of the tensors
+    template <class T> __device__ __forceinline__ T* from(T* x, int64_t) const { return x; }
+    template <int BN> __device__ __forceinline__ KeyBits<BN> keys(int b) const { return KeyBits<BN>(p, b); }
+};
+template <> struct Span<true> {
+    int block, rows, inside;
+    int first, group;                        // the first row, and the number of its group of 32
+    // in causal order a sequence's last rows see the most keys: they begin first
+    __device__ __forceinline__ Span(const SmParams& p, int number, int size) {
+        const Segment s = segment_of(p.offsets, p.sequences, p.M, 1, size, p.causal ? p.blocks - 1 - number : number);
+        block = s.block;
+        rows = s.rows;
+        inside = s.index < 0 || s.index >= p.sequences ? 0 : s.rows;
+        first = s.first;
+        group = segment_start(first, s.index + 1, 1, 32);
+    }
+    __device__ __forceinline__ int M() const { return rows; }
+    __device__ __forceinline__ int N() const { return rows; }
+    __device__ __forceinline__ int seen() const { return inside; }
+    __device__ __forceinline__ int64_t row(int i) const { return (int64_t)first + i; }
+    template <class T> __device__ __forceinline__ T* from(T* x, int64_t stride) const { return x + first * stride; }
+    template <int BN> __device__ __forceinline__ KeyBits<BN> keys(int) const { return KeyBits<BN>(inside); }
+};
 
 // f(element, padded row length) for a call's type and row length.
 template <class F> int dispatch(int dtype, int D, F f) {

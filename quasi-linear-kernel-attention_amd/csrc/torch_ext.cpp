@@ -419,9 +419,9 @@ void check_softmax(const SoftmaxCall& c) {
 
 // whether the kernels can read t's rows: their elements next to each other, each row at a multiple of 16 bytes
 bool readable(const Tensor& t) {
-    const int64_t piece = 16 / t.element_size();
-    if (t.stride(3) != 1 || (uintptr_t)t.data_ptr() % 16) return false;
-    for (int i = 0; i < 3; ++i)
+    const int64_t piece = 16 / t.element_size(), last = t.dim() - 1;
+    if (t.stride(last) != 1 || (uintptr_t)t.data_ptr() % 16) return false;
+    for (int i = 0; i < last; ++i)
         if (t.size(i) > 1 && t.stride(i) % piece) return false;
     return true;
 }
@@ -434,7 +434,7 @@ Tensor empty_rows(const Tensor& t) {
     return r.numel() == 0 || readable(r) ? r : at::empty(t.sizes(), t.options());
 }
 void set_strides(int64_t* to, const Tensor& t) {
-    for (int i = 0; i < 3; ++i) to[i] = t.stride(i);
+    for (int i = 0; i < t.dim() - 1; ++i) to[i] = t.stride(i);
 }
 
 // Sizes, inputs and the bias of a call; border has to outlive the arguments.
@@ -617,6 +617,146 @@ Tensor relative_bias(const Tensor& table, int64_t M, int64_t N, int64_t start, c
     return BiasMapFn::apply(table, M, N, start, border, both);
 }
 
+// ---- attention within packed sequences (qlka_packed_*)
+
+struct PackedCall {
+    Tensor q, k, v, offsets;
+    double scale;
+    bool causal;
+};
+
+// (B + 1) numbers on q's device
+void check_offsets(const Tensor& offsets, const Tensor& q) {
+    TORCH_CHECK(offsets.is_cuda() && offsets.device() == q.device(), "offsets must be on q's device");
+    TORCH_CHECK(offsets.scalar_type() == at::kInt, "offsets must be int32");
+    TORCH_CHECK(offsets.dim() == 1 && offsets.size(0) >= 1, "offsets must be (B + 1)");
+    TORCH_CHECK(offsets.size(0) <= (1 << 28), "at most 2^28 sequences");
+    TORCH_CHECK(offsets.is_contiguous(), "offsets must be contiguous");
+}
+
+void check_packed(const PackedCall& c) {
+    const Tensor &q = c.q, &k = c.k, &v = c.v;
+    TORCH_CHECK(q.is_cuda() && k.is_cuda() && v.is_cuda(), "q, k and v must be CUDA tensors");
+    TORCH_CHECK(q.device() == k.device() && q.device() == v.device(), "q, k and v must be on one device");
+    TORCH_CHECK(q.scalar_type() == at::kFloat || q.scalar_type() == at::kBFloat16, "q must be float32 or bfloat16");
+    TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(),
+                "q, k and v must have the same dtype");
+    TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && v.dim() == 3, "q, k and v must be 3D: (heads, rows, D)");
+    TORCH_CHECK(k.sizes() == v.sizes(), "k and v must have the same shape");
+    TORCH_CHECK(q.size(1) == k.size(1), "q and k must have the same number of rows");
+    TORCH_CHECK(q.size(2) == k.size(2), "q and k must have the same head dimension");
+    TORCH_CHECK(q.size(0) >= 1 && k.size(0) >= 1 && q.size(0) % k.size(0) == 0,
+                "the heads of q must be a multiple of those of k and v");
+    TORCH_CHECK(1 <= q.size(2) && q.size(2) <= 128, "the head dimension must be in [1, 128]");
+    TORCH_CHECK(q.size(1) <= (1 << 28) && (double)q.size(0) * q.size(1) <= INT32_MAX,
+                "at most 2^28 rows, and heads * rows must fit int32");
+    check_offsets(c.offsets, q);
+}
+
+qlka_packed_args packed_args(const PackedCall& c) {
+    qlka_packed_args a{};
+    a.dtype = c.q.scalar_type() == at::kFloat ? QLKA_F32 : QLKA_BF16;
+    a.B = (int)c.offsets.size(0) - 1; a.H = (int)c.q.size(0); a.G = (int)c.k.size(0);
+    a.T = (int)c.q.size(1); a.D = (int)c.q.size(2);
+    a.causal = c.causal;
+    a.scale = (float)c.scale;
+    a.offsets = c.offsets.data_ptr<int>();
+    a.q = c.q.data_ptr(); a.k = c.k.data_ptr(); a.v = c.v.data_ptr();
+    set_strides(a.q_stride, c.q); set_strides(a.k_stride, c.k); set_strides(a.v_stride, c.v);
+    return a;
+}
+
+// (out, out before its rounding to bfloat16, the rows' log sums in two floats), as softmax_forward
+std::tuple<Tensor, Tensor, Tensor> packed_forward(PackedCall& c, bool train, bool train_scores) {
+    check_packed(c);
+    c10::DeviceGuard guard(c.q.device());
+    c.q = packed_rows(c.q);
+    c.k = packed_rows(c.k);
+    c.v = packed_rows(c.v);
+    Tensor out = empty_rows(c.q), full, lse;
+    qlka_packed_args a = packed_args(c);
+    a.out = out.data_ptr();
+    set_strides(a.out_stride, out);
+    if (train) {
+        lse = at::empty({2, a.H, a.T}, c.q.options().dtype(at::kFloat));
+        a.log_sums = lse.data_ptr<float>();
+        if (a.dtype == QLKA_BF16 && train_scores) {
+            full = at::empty({a.H, a.T, a.D}, lse.options());
+            a.out_full = full.data_ptr<float>();
+        }
+    }
+    const size_t bytes = qlka_packed_fwd_ws_bytes(&a);
+    Tensor ws;
+    if (bytes) ws = workspace(bytes, c.q);
+    check_rc(qlka_packed_fwd(&a, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(c.q)));
+    return {out, full, lse};
+}
+
+struct PackedFn : public torch::autograd::Function<PackedFn> {
+    static Tensor forward(AutogradContext* ctx, Tensor q, Tensor k, Tensor v, Tensor offsets, double scale, bool causal) {
+        ctx->set_materialize_grads(false);
+        PackedCall c{q, k, v, offsets, scale, causal};
+        Tensor out, full, lse;
+        std::tie(out, full, lse) = packed_forward(c, true, q.requires_grad() || k.requires_grad());
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["causal"] = causal;
+        ctx->save_for_backward({c.q, c.k, c.v, offsets, out, full, lse});
+        return out;
+    }
+
+    static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "packed_attention has no second derivative");
+        tensor_list r(6);
+        if (!grads[0].defined()) return r;
+        const auto s = ctx->get_saved_variables();
+        const PackedCall c{s[0], s[1], s[2], s[3], ctx->saved_data["scale"].toDouble(), ctx->saved_data["causal"].toBool()};
+        const Tensor &out = s[4], &full = s[5], &lse = s[6];
+        c10::DeviceGuard guard(c.q.device());
+        qlka_packed_args a = packed_args(c);
+        const Tensor g = packed_rows(grads[0]);
+        a.out = out.data_ptr();
+        set_strides(a.out_stride, out);
+        if (full.defined()) a.out_full = full.data_ptr<float>();
+        a.log_sums = lse.data_ptr<float>();
+        a.g_out = g.data_ptr();
+        set_strides(a.g_out_stride, g);
+        if (ctx->needs_input_grad(0)) {
+            r[0] = empty_rows(c.q);
+            a.g_q = r[0].data_ptr();
+            set_strides(a.g_q_stride, r[0]);
+        }
+        if (ctx->needs_input_grad(1) || ctx->needs_input_grad(2)) {
+            r[1] = empty_rows(c.k);
+            r[2] = empty_rows(c.v);
+            a.g_k = r[1].data_ptr();
+            a.g_v = r[2].data_ptr();
+            set_strides(a.g_k_stride, r[1]);
+            set_strides(a.g_v_stride, r[2]);
+        }
+        const size_t bytes = qlka_packed_bwd_ws_bytes(&a);
+        Tensor ws;
+        if (bytes) ws = workspace(bytes, c.q);
+        check_rc(qlka_packed_bwd(&a, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(c.q)));
+        return r;
+    }
+};
+
+Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& offsets, double scale,
+                        bool causal) {
+    for (const Tensor& t : {q, k, v})
+        TORCH_CHECK(!t._fw_grad(0).defined(), "packed_attention has no forward-mode derivative");
+    if (q.dim() == 3 && k.dim() == 3 && v.dim() == 3 && q.size(2) % 8 && q.size(2) == k.size(2) &&
+        q.size(2) == v.size(2)) {
+        // zeros up to a multiple of 8 change no product
+        const auto padded = [&](const Tensor& t) { return at::constant_pad_nd(t, {0, 8 - t.size(2) % 8}); };
+        return packed_attention(padded(q), padded(k), padded(v), offsets, scale, causal).narrow(2, 0, q.size(2));
+    }
+    if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
+        return PackedFn::apply(q, k, v, offsets, scale, causal);
+    PackedCall c{q, k, v, offsets, scale, causal};
+    return std::get<0>(packed_forward(c, false, false));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -658,5 +798,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           "differentiable softmax attention (qlka_softmax_fwd / qlka_softmax_bwd)");
     m.def("relative_bias", &relative_bias, py::arg("table"), py::arg("M"), py::arg("N"), py::arg("start"),
           py::arg("border"), py::arg("both"), "differentiable bias map (qlka_bias_map_fwd / qlka_bias_map_bwd)");
+    m.def("packed_attention", &packed_attention, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("offsets"),
+          py::arg("scale"), py::arg("causal"),
+          "differentiable softmax attention within packed sequences (qlka_packed_fwd / qlka_packed_bwd)");
     m.attr("DIRECT") = DIRECT;
 }

@@ -19,6 +19,7 @@ EXT_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_qlka_torch
 _c_int = ctypes.c_int
 _c_size = ctypes.c_size_t
 _c_ptr = ctypes.c_void_p
+_c_i64x2 = ctypes.c_int64 * 2
 _c_i64x3 = ctypes.c_int64 * 3
 
 
@@ -36,7 +37,19 @@ class SoftmaxArgs(ctypes.Structure):
                 + [("g_table", _c_ptr), ("log_sums", _c_ptr), ("table_kept", _c_int)])
 
 
+class PackedArgs(ctypes.Structure):
+    """qlka_packed_args of include/qlka.h."""
+    _fields_ = ([(n, _c_int) for n in ("dtype", "B", "H", "G", "T", "D", "causal")]
+                + [("scale", ctypes.c_float), ("offsets", _c_ptr)]
+                + [(n, _c_ptr) for n in ("q", "k", "v")]
+                + [(n, _c_i64x2) for n in ("q_stride", "k_stride", "v_stride")]
+                + [("out", _c_ptr), ("out_stride", _c_i64x2), ("out_full", _c_ptr), ("log_sums", _c_ptr),
+                   ("g_out", _c_ptr), ("g_out_stride", _c_i64x2), ("g_q", _c_ptr), ("g_k", _c_ptr), ("g_v", _c_ptr)]
+                + [(n, _c_i64x2) for n in ("g_q_stride", "g_k_stride", "g_v_stride")])
+
+
 _c_softmax = ctypes.POINTER(SoftmaxArgs)
+_c_packed = ctypes.POINTER(PackedArgs)
 _c_border = [ctypes.POINTER(_c_int), _c_int, _c_int]       # border, num_borders, bidirectional
 
 # name -> (restype, argtypes)
@@ -69,6 +82,10 @@ _SIGNATURES = {
     "qlka_softmax_fwd": (_c_int, [_c_softmax, _c_ptr, _c_size, _c_ptr]),
     "qlka_softmax_bwd_ws_bytes": (_c_size, [_c_softmax]),
     "qlka_softmax_bwd": (_c_int, [_c_softmax, _c_ptr, _c_size, _c_ptr]),
+    "qlka_packed_fwd_ws_bytes": (_c_size, [_c_packed]),
+    "qlka_packed_fwd": (_c_int, [_c_packed, _c_ptr, _c_size, _c_ptr]),
+    "qlka_packed_bwd_ws_bytes": (_c_size, [_c_packed]),
+    "qlka_packed_bwd": (_c_int, [_c_packed, _c_ptr, _c_size, _c_ptr]),
     "qlka_bias_map_fwd": (_c_int, [_c_ptr] + _c_border + [_c_ptr] + [_c_int] * 4 + [_c_ptr]),
     "qlka_bias_map_bwd_ws_bytes": (_c_size, [_c_int] * 5),
     "qlka_bias_map_bwd": (_c_int, [_c_ptr] + _c_border + [_c_ptr] + [_c_int] * 4 + [_c_ptr, _c_size, _c_ptr]),
