@@ -335,6 +335,59 @@ size_t qlka_packed_bwd_ws_bytes(const qlka_packed_args* args);
 int qlka_packed_bwd(const qlka_packed_args* args, void* ws, size_t ws_bytes, void* stream);
 
 /*
+ * A cache of keys and values in pages. A sequence's token at position i is row i % page_size of page
+ * tables[b][i / page_size]; pages are rows of D elements for each of G key heads, at any strides (elements, between pages,
+ * heads and rows). What is held (held):
+ *   QLKA_F32, QLKA_BF16  the rows as they are; of the type of the call (dtype) only
+ *   QLKA_INT8, QLKA_E4M3 8 bits an element, and for every 32 elements of a row a byte e (k_exp, v_exp: ceil(D / 32) a row,
+ *                        contiguous; strides in bytes between pages, heads and rows): an element stands for
+ *                        code * 2^(e - 127). e is the least of [27, 248] (int8; 246 with e4m3) with which the largest
+ *                        code (127; 448) reaches the largest element, the codes are the nearest ones, ties to the
+ *                        even one. Such values are exact in bf16 and fp32, so nothing is rounded a second time when
+ *                        they are read. e = 255 marks 32 elements of which one was infinite or NaN: all read as NaN.
+ *
+ * tables: B rows of table_len page numbers, table_stride apart; lengths: B numbers of tokens, the new ones included;
+ * offsets (B + 1): the new tokens of the sequences one after the other in T rows, or NULL: one for each, T = B. All on the
+ * device; their contents may change between the replays of a captured call. Row m of sequence b is at position
+ * lengths[b] - (offsets[b + 1] - m). Page numbers outside [0, num_pages), and what a table's row has no place for, are
+ * pages that do not exist: nothing is written there, keys there are not seen, reading gives zeros.
+ *
+ * qlka_paged_write: the new tokens' k and v (G, T, D) go to their positions. Rows outside every sequence, or at negative
+ *   positions, are left out; nothing else in the pages changes. Two rows of one call at one place in a page leave either
+ *   one's values, or parts of both.
+ * qlka_paged_read: out_k and out_v (B, G, N, D) of dtype get the first N positions of each sequence, zeros from lengths[b]
+ *   on.
+ * qlka_paged_attention: out (H, T, D), softmax attention of the new tokens q (H, T, D) to their sequence's held keys up to
+ *   their own position, which have been written before. Rows that see none, and rows outside every sequence, get zeros.
+ *   longest: the most new tokens of a sequence if the caller knows it, else 0. It only decides which kernels run.
+ *
+ * Strides are in elements between heads and rows ((B, heads, rows) for out_k and out_v); D a multiple of 8 up to 128, rows
+ * at multiples of 16 bytes (in pages of 8 bits with D no multiple of 16: of 8 bytes). The scale is as for qlka_softmax_fwd, the probabilities are rounded
+ * to bf16 for their product where q is.
+ */
+#define QLKA_INT8 2
+#define QLKA_E4M3 3
+typedef struct qlka_paged_args {
+    int dtype, held, B, H, G, T, D;
+    int page_size, num_pages, table_len, longest, N;
+    float scale;
+    const int *tables, *lengths, *offsets;
+    int64_t table_stride;
+    void *k_pages, *v_pages;
+    int64_t k_pages_stride[3], v_pages_stride[3];
+    uint8_t *k_exp, *v_exp;
+    int64_t k_exp_stride[3], v_exp_stride[3];
+    const void *q, *k, *v;
+    int64_t q_stride[2], k_stride[2], v_stride[2];
+    void *out, *out_k, *out_v;
+    int64_t out_stride[2], out_k_stride[3], out_v_stride[3];
+} qlka_paged_args;
+int qlka_paged_write(const qlka_paged_args* args, void* stream);
+int qlka_paged_read(const qlka_paged_args* args, void* stream);
+size_t qlka_paged_attention_ws_bytes(const qlka_paged_args* args);
+int qlka_paged_attention(const qlka_paged_args* args, void* ws, size_t ws_bytes, void* stream);
+
+/*
  * Test entry: stable ascending sort of num_segs contiguous segments of seg_len fp32 keys; perm[i] is the in-segment
  * index of the i-th smallest key (np.argsort(kind="stable"); -0.0 ties +0.0 and is written as +0.0).
  * Replaces launch_iota + launch_cub_sort (Weighted_Abs_Sum/csrc/sort_utils.cu:85-117).

@@ -1,0 +1,228 @@
+// The C ABI of the cache in pages and of attention over it (include/qlka.h): validation, the choice of kernels and
+// splits, the workspace and the launches.
+#include "api_checks.h"
+#include "paged.h"
+#include "segments.h"
+
+using namespace qlka;
+
+namespace {
+
+bool coded(const qlka_paged_args* a) { return a->held == QLKA_INT8 || a->held == QLKA_E4M3; }
+int held_size(const qlka_paged_args* a) { return coded(a) ? 1 : a->held == QLKA_F32 ? 4 : 2; }
+
+int check_sizes(const qlka_paged_args* a) {
+    if (!a) return refuse("args must be non-null");
+    if (a->dtype != QLKA_F32 && a->dtype != QLKA_BF16) return refuse("dtype must be QLKA_F32 or QLKA_BF16");
+    if (!coded(a) && a->held != a->dtype) return refuse("held must be dtype, QLKA_INT8 or QLKA_E4M3");
+    if (a->B < 0 || a->T < 0 || a->N < 0 || a->H < 1 || a->G < 1) return refuse("B, T and N must be >= 0, H and G >= 1");
+    if (a->H % a->G) return refuse("H must be a multiple of G");
+    if (a->D < 8 || a->D > 128 || a->D % 8) return refuse("D must be a multiple of 8 in [8, 128]");
+    if (a->T > LONGEST || a->B > LONGEST || a->N > LONGEST) return refuse("B, T and N must be <= 2^28");
+    if (a->page_size < 1 || a->page_size > 1 << 16) return refuse("page_size must be in [1, 65536]");
+    if (a->num_pages < 0 || a->table_len < 0) return refuse("num_pages and table_len must be >= 0");
+    if (a->longest < 0) return refuse("longest must be >= 0");
+    if ((double)a->H * a->T > (double)MOST_ROWS || (double)a->B * a->G * a->N > (double)MOST_ROWS)
+        return refuse("H * T and B * G * N must fit int32");
+    if (!a->offsets && a->T != a->B) return refuse("without offsets every sequence has one token: T must be B");
+    return QLKA_OK;
+}
+
+// ---- how a call runs
+
+// Sequences of up to FEW rows a key head go through the step kernel, 16 rows at a time, others through the tiles.
+constexpr int FEW = 32;
+
+struct Plan {
+    bool step, tiles;
+    int few, step_blocks, tile_blocks, splits;
+    size_t part, part2;
+};
+Plan plan(const qlka_paged_args* a) {
+    Plan r{};
+    const int64_t share = a->H / a->G, sequences = std::max(a->B, 1);
+    const int64_t longest = !a->offsets ? 1 : a->longest ? std::min(a->longest, a->T) : a->T;
+    r.step = r.tiles = true;
+    r.few = FEW;
+    if (!a->offsets || longest * share <= FEW) {
+        r.tiles = false;
+        r.few = INT32_MAX;
+    } else if (a->T * share >= 256 * sequences) {       // chunks, on the average: a token among them takes a tile too
+        r.step = false;
+        r.few = -1;
+    }
+    r.step_blocks = (int)ceil_div(std::min<int64_t>(longest * share, std::max<int64_t>(FEW, share)), PG_STEP_ROWS);
+    r.tile_blocks = (int)segment_blocks(a->T, a->B, (int)share, PG_TILE_ROWS);
+
+    const int64_t places = std::min<int64_t>((int64_t)a->table_len * a->page_size, LONGEST);
+    const int DP = sm_padded(a->D);
+    int64_t splits = 1;
+    if (r.step) {
+        const int64_t groups = a->G * sequences * ceil_div(std::min<int64_t>(longest, ceil_div(a->T, sequences)) * share, PG_STEP_ROWS);
+        splits = std::min<int64_t>({ceil_div(1024, std::max<int64_t>(groups, 1)), places / 512, 256});
+    }
+    if (r.tiles) {
+        const int BN = sm_tile_rows(a->held == QLKA_F32 ? 3 : 1, DP);
+        const double tile_us = 0.6 * DP / 64 * BN / 64 * (a->dtype == QLKA_F32 ? 2 : 1);
+        splits = std::max<int64_t>(splits, splits_for((int64_t)a->G * ceil_div(a->T * share, PG_TILE_ROWS), ceil_div(places, BN),
+                                                      tile_us, (double)a->H * a->T * DP * 8));
+    }
+    r.splits = (int)std::max<int64_t>(splits, 1);
+    if (r.splits > 1) {
+        const size_t rows = (size_t)r.splits * a->H * a->T;
+        r.part = align256(rows * DP * 4);
+        r.part2 = align256(rows * 8);
+    }
+    return r;
+}
+
+// ---- arguments to kernel parameters
+
+PgStrides page_strides(const int64_t* s) { return {s[0], s[1], s[2]}; }
+PgOut strides2(const int64_t* s) { return {0, s[0], s[1]}; }
+PgOut strides3(const int64_t* s) { return {s[0], s[1], s[2]}; }
+
+// The cache and where the sequences are in it.
+int params(const qlka_paged_args* a, PgParams* p) {
+    *p = PgParams{};
+    p->k_pages = (char*)a->k_pages; p->v_pages = (char*)a->v_pages;
+    p->sk = page_strides(a->k_pages_stride); p->sv = page_strides(a->v_pages_stride);
+    p->k_exp = a->k_exp; p->v_exp = a->v_exp;
+    p->ske = page_strides(a->k_exp_stride); p->sve = page_strides(a->v_exp_stride);
+    p->tables = a->tables; p->lengths = a->lengths; p->offsets = a->offsets;
+    p->table_stride = a->table_stride;
+    p->B = a->B; p->H = a->H; p->G = a->G; p->T = a->T; p->D = a->D; p->N = a->N;
+    p->page_size = a->page_size; p->num_pages = a->num_pages; p->table_len = a->table_len;
+    p->places = (int)std::min<int64_t>((int64_t)a->table_len * a->page_size, LONGEST);
+    int log = 0;
+    while (1 << log < a->page_size) ++log;
+    p->shift = 31 + log;
+    p->magic = (uint32_t)(((uint64_t(1) << p->shift) + a->page_size - 1) / a->page_size);
+    p->splits = p->blocks = 1;
+    const int64_t sizes[3] = {a->num_pages, a->G, a->page_size};
+    const struct { const char* name; const void* x; const int64_t* s; } pages[] = {
+        {"k_pages", a->k_pages, a->k_pages_stride}, {"v_pages", a->v_pages, a->v_pages_stride}};
+    const int64_t unit = coded(a) && a->D % 16 ? 8 : 16;
+    for (const auto& o : pages) {
+        if (a->num_pages && !o.x) return refuse("%s must be non-null", o.name);
+        bool aligned = (uintptr_t)o.x % unit == 0;
+        for (int i = 0; i < 3; ++i) {
+            if (sizes[i] <= 1) continue;
+            if (o.s[i] < 0) return refuse("the strides of %s must not be negative", o.name);
+            aligned = aligned && o.s[i] * held_size(a) % unit == 0;
+        }
+        if (!aligned) return refuse("the rows of %s must be aligned to %d bytes", o.name, (int)unit);
+    }
+    if (coded(a) && a->num_pages) {
+        if (!a->k_exp || !a->v_exp) return refuse("k_exp and v_exp must be non-null where 8 bits are held");
+        for (int i = 0; i < 3; ++i)
+            if (sizes[i] > 1 && (a->k_exp_stride[i] < 0 || a->v_exp_stride[i] < 0))
+                return refuse("the strides of k_exp and v_exp must not be negative");
+    }
+    if (a->B > 0 && (!a->lengths || (a->table_len > 0 && !a->tables))) return refuse("tables and lengths must be non-null");
+    if (a->B > 1 && a->table_stride < 0) return refuse("table_stride must not be negative");
+    return QLKA_OK;
+}
+
+int rows_of(const qlka_paged_args* a, const char* name, const void* x, const int64_t* s, int heads) {
+    const int64_t sizes[2] = {heads, a->T};
+    return check_rows(name, x, s, sizes, 2, a->dtype == QLKA_F32 ? 4 : 2);
+}
+
+}  // namespace
+
+extern "C" {
+
+int qlka_paged_write(const qlka_paged_args* a, void* stream) {
+    api_error(QLKA_OK, "");
+    if (int e = check_sizes(a)) return e;
+    PgParams p;
+    if (int e = params(a, &p)) return e;
+    if (int e = rows_of(a, "k", a->k, a->k_stride, a->G)) return e;
+    if (int e = rows_of(a, "v", a->v, a->v_stride, a->G)) return e;
+    if (a->T == 0 || a->B == 0 || p.places == 0 || a->num_pages == 0) return QLKA_OK;
+    if (!a->k || !a->v) return refuse("k and v must be non-null");
+    if (int e = fits_grid(ceil_div(a->T, 4), 256)) return e;
+    p.k = a->k; p.v = a->v;
+    p.snk = strides2(a->k_stride); p.snv = strides2(a->v_stride);
+    hipStream_t st = (hipStream_t)stream;
+    StageTimer timer("paged_write", st);
+    return status(pg_write(a->dtype, a->held, p, st), "writing to pages");
+}
+
+int qlka_paged_read(const qlka_paged_args* a, void* stream) {
+    api_error(QLKA_OK, "");
+    if (int e = check_sizes(a)) return e;
+    PgParams p;
+    if (int e = params(a, &p)) return e;
+    const int64_t sizes[3] = {a->B, a->G, a->N};
+    if (int e = check_rows("out_k", a->out_k, a->out_k_stride, sizes, 3, a->dtype == QLKA_F32 ? 4 : 2)) return e;
+    if (int e = check_rows("out_v", a->out_v, a->out_v_stride, sizes, 3, a->dtype == QLKA_F32 ? 4 : 2)) return e;
+    if (a->B == 0 || a->N == 0) return QLKA_OK;
+    if (!a->out_k || !a->out_v) return refuse("out_k and out_v must be non-null");
+    p.out_k = a->out_k; p.out_v = a->out_v;
+    p.sok = strides3(a->out_k_stride); p.sov = strides3(a->out_v_stride);
+    p.blocks = (int)ceil_div(a->N, 256 / (sm_padded(a->D) / 8) * PG_READ_ROWS);
+    if (int e = fits_grid((int64_t)a->B * a->G * p.blocks, 256)) return e;
+    hipStream_t st = (hipStream_t)stream;
+    StageTimer timer("paged_read", st);
+    return status(pg_read(a->dtype, a->held, p, st), "reading pages");
+}
+
+size_t qlka_paged_attention_ws_bytes(const qlka_paged_args* a) {
+    if (check_sizes(a) || check_scale(a->scale)) return 0;
+    const Plan r = plan(a);
+    return r.part + r.part2;
+}
+
+int qlka_paged_attention(const qlka_paged_args* a, void* ws, size_t ws_bytes, void* stream) {
+    api_error(QLKA_OK, "");
+    if (int e = check_sizes(a)) return e;
+    if (int e = check_scale(a->scale)) return e;
+    PgParams p;
+    if (int e = params(a, &p)) return e;
+    if (int e = rows_of(a, "q", a->q, a->q_stride, a->H)) return e;
+    if (int e = rows_of(a, "out", a->out, a->out_stride, a->H)) return e;
+    if (a->T == 0) return QLKA_OK;
+    if (!a->q || !a->out) return refuse("q and out must be non-null");
+    const Plan r = plan(a);
+    if (int e = need_ws(ws, ws_bytes, r.part + r.part2)) return e;
+    p.outside = a->offsets && r.step && !r.tiles;
+    const int64_t segments = a->B + (p.outside ? 2 : 0);
+    if (r.step)
+        if (int e = fits_grid(segments * r.step_blocks * a->G * r.splits, 256)) return e;
+    if (r.tiles)
+        if (int e = fits_grid((int64_t)a->G * r.tile_blocks * r.splits, 2 * PG_TILE_ROWS)) return e;
+    if (r.splits > 1)
+        if (int e = fits_rows((int64_t)a->H * a->T, 64)) return e;
+    p.q = a->q; p.out = a->out;
+    p.sq = strides2(a->q_stride); p.so = strides2(a->out_stride);
+    p.scale = a->scale == 0.f ? 1.f : std::fabs(a->scale);
+    p.q_sign = a->scale == 0.f ? 0.f : a->scale < 0.f ? -1.f : 1.f;
+    p.few = r.few;
+    p.splits = r.splits;
+    p.part = (float*)ws;
+    p.part2 = (float*)((char*)ws + r.part);
+    hipStream_t st = (hipStream_t)stream;
+    if (r.step && segments) {
+        StageTimer timer("paged_step", st);
+        p.blocks = r.step_blocks;
+        if (int e = pg_step(a->dtype, a->held, p, st)) return status(e, "attention over pages, few rows");
+    }
+    if (r.tiles) {
+        StageTimer timer("paged_tiles", st);
+        p.blocks = r.tile_blocks;
+        if (int e = pg_tiles(a->dtype, a->held, p, st)) return status(e, "attention over pages");
+    }
+    if (r.splits == 1) return QLKA_OK;
+    SmParams c{};
+    c.B = 1; c.H = a->H; c.M = a->T; c.D = a->D;
+    c.out = a->out;
+    c.so = {0, a->out_stride[0], a->out_stride[1]};
+    c.splits = r.splits;
+    c.part = p.part; c.part2 = p.part2;
+    StageTimer timer("softmax_combine", st);
+    return status(sm_combine(a->dtype, c, st), "attention over pages, joining of splits");
+}
+
+}  // extern "C"

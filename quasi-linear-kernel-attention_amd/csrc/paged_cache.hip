@@ -1,0 +1,167 @@
+// A cache of keys and values in pages, written as tokens come and read back (include/qlka.h).
+//
+// With 8 bits held, 32 elements of a row share a power of two: the least one, 2^e, whose multiple by the largest code
+// reaches the largest of them. x / 2^e, the code's rounding (nearest, ties to the even one) and code * 2^e are then exact
+// but for that rounding, in any type that holds x: what is written is what the definition says, to the bit, and products
+// of what is read need no further rounding (int8 and e4m3 values have at most 7 and 4 bits, bf16 has 8). A scale of
+// largest / 127 would use up to one bit more of int8, but every reader would round.
+//
+// Both kernels are bound by memory, and at few rows by the latency of offsets, length, table and row, one after the
+// other. DP / 8 lanes take a row, 8 elements each; 4 lanes find a block's largest element. A wave writes one token's
+// rows of all heads, keys and values, so that the sequence is looked up once for all of them.
+#include "paged_device.h"
+
+namespace qlka {
+namespace pg {
+
+// The exponent (plus 127) of a block whose largest element is `most`: the least of [27, top] with most <= largest * 2^(e -
+// 127), largest = MANT * 2^SHIFT with MANT in [1, 2); 255 if it is not finite.
+template <class C> __device__ __forceinline__ uint32_t exponent_of(float most) {
+    constexpr bool INT = std::is_same<C, Int8>::value;
+    constexpr uint32_t MANT = INT ? 0x7e0000u : 0x600000u;            // of 127 = 1.984375 * 2^6, of 448 = 1.75 * 2^8
+    constexpr int SHIFT = INT ? 6 : 8, TOP = INT ? 248 : 246;
+    const uint32_t bits = __float_as_uint(most);
+    if (bits >= 0x7f800000u) return 255;
+    const int e = (int)(bits >> 23) - SHIFT + ((bits & 0x7fffffu) > MANT ? 1 : 0);
+    return (uint32_t)min(max(e, LEAST_EXP), TOP);
+}
+
+template <class C> __device__ __forceinline__ u32x2 codes_of(f32x8 x, uint32_t e) {
+    const float s = __uint_as_float((254 - min(e, 253u)) << 23);       // 2^(127 - e)
+    u32x2 w;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if constexpr (std::is_same<C, Int8>::value) {
+            uint32_t y = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float c = fminf(fmaxf(__builtin_rintf(x[4 * h + i] * s), -127.f), 127.f);
+                y |= ((uint32_t)(int)c & 255u) << 8 * i;
+            }
+            w[h] = e == 255 ? 0u : y;
+        } else {
+            float c[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[i] = fminf(fmaxf(x[4 * h + i] * s, -448.f), 448.f);
+            int y = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
+            y = __builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], y, true);
+            w[h] = e == 255 ? 0x7f7f7f7fu : (uint32_t)y;
+        }
+    }
+    return w;
+}
+
+// One wave a token: its rows of all heads, keys then values, DP / 8 lanes a row.
+template <class T, class C, int DP> __global__ __launch_bounds__(256) void paged_write(const PgParams p) {
+    constexpr int LANES = DP / 8, AT_ONCE = 64 / LANES;
+    const int lane = threadIdx.x & 63, token = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (token >= p.T) return;
+    int b = token, seat = -1;
+    if (p.offsets) b = last_upto(p.B + 1, token, [&](int i) { return p.offsets[i]; });
+    b = __builtin_amdgcn_readfirstlane(b);
+    if (b < 0 || b >= p.B) return;
+    {
+        const int length = min(max(p.lengths[b], 0), 1 << 28);
+        const int64_t end = p.offsets ? p.offsets[b + 1] : b + 1;
+        // offsets are the caller's: whatever they are, a position without a place is none
+        const int64_t at = length - (end - token);
+        seat = at < 0 || at >= p.places ? -1 : (int)at;
+    }
+    if (seat < 0) return;
+    const int index = page_at(p, seat), page = p.tables[b * p.table_stride + index];
+    if ((uint32_t)page >= (uint32_t)p.num_pages) return;
+    const int row = seat - index * p.page_size, d = lane % LANES * 8;
+#pragma unroll 2
+    for (int i = lane / LANES; i < 2 * p.G; i += AT_ONCE) {
+        const bool key = i < p.G;
+        const int g = key ? i : i - p.G;
+        const PgOut s = key ? p.snk : p.snv;
+        const PgStrides to = key ? p.sk : p.sv;
+        const auto x = sm::load_seg((const T*)(key ? p.k : p.v) + g * s.h + token * s.r, d, p.D);
+        char* pages = key ? p.k_pages : p.v_pages;
+        const int64_t at = page * to.page + g * to.head + row * to.row + d;
+        if constexpr (!coded<C>) {
+            if (d < p.D) *reinterpret_cast<typename sm::Elem<T>::seg*>(pages + at * (int64_t)sizeof(T)) = x;
+        } else {
+            const f32x8 y = sm::floats(x);
+            // the largest of the block's bits: NaN and infinities are above every finite number
+            uint32_t most = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(y[j]) & 0x7fffffffu);
+            most = max(most, (uint32_t)__shfl_xor((int)most, 1));
+            most = max(most, (uint32_t)__shfl_xor((int)most, 2));
+            const uint32_t e = exponent_of<C>(__uint_as_float(most));
+            if (d < p.D) {
+                *reinterpret_cast<u32x2*>(pages + at) = codes_of<C>(y, e);
+                if (d % BLOCK == 0) {
+                    const PgStrides te = key ? p.ske : p.sve;
+                    (key ? p.k_exp : p.v_exp)[page * te.page + g * te.head + row * te.row + d / BLOCK] = (uint8_t)e;
+                }
+            }
+        }
+    }
+}
+
+// Rows of one sequence and head, keys and values, DP / 8 lanes a row and PG_READ_ROWS rows a lane.
+template <class T, class C, int DP> __global__ __launch_bounds__(256) void paged_read(const PgParams p) {
+    constexpr int LANES = DP / 8, ROWS = 256 / LANES;
+    const int d = threadIdx.x % LANES * 8, g = blockIdx.x / p.blocks % p.G, b = blockIdx.x / p.blocks / p.G;
+    const int length = min(max(p.lengths[b], 0), p.places);
+    const int first = blockIdx.x % p.blocks * ROWS * PG_READ_ROWS + threadIdx.x / LANES;
+    if (d >= p.D) return;
+    typedef typename Piece<C, 8>::raw Raw;
+    Raw k[PG_READ_ROWS], v[PG_READ_ROWS];
+    uint32_t ke[PG_READ_ROWS], ve[PG_READ_ROWS];
+#pragma unroll
+    for (int i = 0; i < PG_READ_ROWS; ++i) {
+        const int n = first + i * ROWS;
+        k[i] = v[i] = Raw{};
+        ke[i] = ve[i] = 127;
+        if (n >= length || n >= p.N) continue;
+        const int index = page_at(p, n), page = p.tables[b * p.table_stride + index], row = n - index * p.page_size;
+        if ((uint32_t)page >= (uint32_t)p.num_pages) continue;
+        k[i] = *reinterpret_cast<const Raw*>(
+            p.k_pages + (page * p.sk.page + g * p.sk.head + row * p.sk.row + d) * Piece<C, 8>::SIZE);
+        v[i] = *reinterpret_cast<const Raw*>(
+            p.v_pages + (page * p.sv.page + g * p.sv.head + row * p.sv.row + d) * Piece<C, 8>::SIZE);
+        if constexpr (coded<C>) {
+            ke[i] = p.k_exp[page * p.ske.page + g * p.ske.head + row * p.ske.row + d / BLOCK];
+            ve[i] = p.v_exp[page * p.sve.page + g * p.sve.head + row * p.sve.row + d / BLOCK];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < PG_READ_ROWS; ++i) {
+        const int n = first + i * ROWS;
+        if (n >= p.N) continue;
+        typedef typename sm::Elem<T>::seg Seg;
+        Seg x, y;
+        if constexpr (coded<C>) {
+            x = __builtin_convertvector(eight<C>(k[i], power_of(ke[i])), Seg);
+            y = __builtin_convertvector(eight<C>(v[i], power_of(ve[i])), Seg);
+        } else {
+            x = k[i];
+            y = v[i];
+        }
+        *reinterpret_cast<Seg*>((T*)p.out_k + b * p.sok.b + g * p.sok.h + n * p.sok.r + d) = x;
+        *reinterpret_cast<Seg*>((T*)p.out_v + b * p.sov.b + g * p.sov.h + n * p.sov.r + d) = y;
+    }
+}
+
+}  // namespace pg
+
+int pg_write(int dtype, int held, const PgParams& p, hipStream_t st) {
+    return pg::dispatch_types(dtype, held, [&](auto t, auto c) {
+        return pg::by_width(p.D, [&](auto dp) {
+            pg::paged_write<decltype(t), decltype(c), dp.value><<<dim3((unsigned)((p.T + 3) / 4)), 256, 0, st>>>(p);
+            return (int)hipGetLastError(); }); });
+}
+
+int pg_read(int dtype, int held, const PgParams& p, hipStream_t st) {
+    return pg::dispatch_types(dtype, held, [&](auto t, auto c) {
+        return pg::by_width(p.D, [&](auto dp) {
+            const dim3 grid((unsigned)((int64_t)p.B * p.G * p.blocks));
+            pg::paged_read<decltype(t), decltype(c), dp.value><<<grid, 256, 0, st>>>(p);
+            return (int)hipGetLastError(); }); });
+}
+
+}  // namespace qlka

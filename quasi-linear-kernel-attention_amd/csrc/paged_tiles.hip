@@ -1,0 +1,323 @@
+// Softmax attention of chunks of new tokens over a cache in pages: the tiles of softmax_fwd.hip over rows that are found
+// through the sequence's table.
+//
+// A workgroup takes 128 rows of one sequence and key head, token by token and within a token the query heads that share
+// the key head, so that heads with common keys read (and take apart) them once. Each thread finds the pages of the rows
+// that it brings, one tile ahead of them. bf16 rows go to LDS directly, into the other of two buffers; rows of 8 bits
+// stay in registers until the tile before is done with and become bf16 on their way into the other buffer (exactly, see
+// paged_cache.hip); float rows are split into three parts there, with one buffer.
+#include "paged_device.h"
+
+#include <limits>
+
+namespace qlka {
+namespace pg {
+
+constexpr int TILE_WAVES = PG_TILE_ROWS / 32;
+constexpr float NONE = -std::numeric_limits<float>::infinity();
+constexpr float MOVE = 4.f;                  // 2^8 of the exponentials
+
+// A sum of products of operands in NA and NB parts, the smaller parts' apart (softmax_tile.h, Acc).
+template <int NA, int NB> struct Gather {
+    sm::f32x16 main = {}, rest;
+    __device__ __forceinline__ void start() {
+        if constexpr (NA + NB > 2) rest = sm::f32x16{};
+    }
+    __device__ __forceinline__ void add(const sm::Frag<NA>& a, const sm::Frag<NB>& b) {
+        if constexpr (NB == 3) rest = sm::mfma(a.p[0], b.p[2], rest);
+        if constexpr (NA == 3) {
+            rest = sm::mfma(a.p[2], b.p[0], rest);
+            rest = sm::mfma(a.p[1], b.p[1], rest);
+        }
+        if constexpr (NB == 3) rest = sm::mfma(a.p[0], b.p[1], rest);
+        if constexpr (NA == 3) rest = sm::mfma(a.p[1], b.p[0], rest);
+        main = sm::mfma(a.p[0], b.p[0], main);
+    }
+    __device__ __forceinline__ void join() {
+        if constexpr (NA + NB > 2) main = main + rest;
+    }
+};
+
+// Tiles of keys and values on their way from pages into LDS.
+template <class C, int DP, int BN> struct Bring {
+    typedef Piece<C, 8> P;
+    typedef typename P::raw Raw;
+    static constexpr int NP = P::PARTS, NT = 64 * TILE_WAVES, PIECES = DP / 8, BUFFERS = NP == 1 ? 2 : 1;
+    static constexpr int APART = NT / PIECES, EACH = BN / APART;       // rows of a thread: one in APART, EACH of them
+    static constexpr bool DIRECT = std::is_same<C, __bf16>::value;
+    static_assert(APART * PIECES == NT && EACH * APART == BN, "every thread brings as many pieces");
+    typedef sm::Tile<NP, BN, DP> TileT;
+    struct Lds { TileT k[BUFFERS], v[BUFFERS]; };
+
+    int row, slot;                           // this thread's first row, and its place among the row's pieces
+    int page[EACH];                          // of the tile that is fetched next
+    uint32_t ok;                             // which of the rows being brought are there
+    Raw k[DIRECT ? 1 : EACH], v[DIRECT ? 1 : EACH];
+    uint32_t ke[EACH], ve[EACH];
+
+    __device__ __forceinline__ Bring(Lds& lds, const PgParams& p, int tid) : row(tid / PIECES), slot(tid % PIECES), ok(0) {
+        if (DIRECT && p.D < DP) {            // pieces past D stay as they are
+            bf16x8* x = reinterpret_cast<bf16x8*>(&lds);
+            for (int i = tid; i < (int)(sizeof(Lds) / 16); i += NT) x[i] = bf16x8{};
+            __syncthreads();
+        }
+    }
+    // the pages of tile t; -1 for positions from seen on
+    __device__ __forceinline__ void look(const PgParams& p, const int* table, int t, int seen) {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int n = t * BN + row + i * APART;
+            page[i] = n < seen ? table[page_at(p, n)] : -1;
+        }
+    }
+    // tile t, whose pages have been looked up
+    __device__ __forceinline__ void fetch(Lds& lds, int buffer, const PgParams& p, int kvh, int t, int tid) {
+        ok = 0;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int n = t * BN + row + i * APART, at = n - page_at(p, n) * p.page_size;
+            const bool there = (uint32_t)page[i] < (uint32_t)p.num_pages;
+            ok |= (uint32_t)there << i;
+            // a row's pieces are turned by bits of its number: where they go, or, straight to LDS, where they come from
+            const int piece = DIRECT ? slot ^ TileT::turn(row + i * APART) : slot, d = piece * 8;
+            if constexpr (DIRECT) {
+                const int first = (tid >> 6) * (64 / PIECES) + i * APART;        // of the wave's rows
+                const uint32_t to_k = sm::lds_place(&lds.k[buffer].x[first * DP]);
+                const uint32_t to_v = sm::lds_place(&lds.v[buffer].x[first * DP]);
+                if (d >= p.D) continue;
+                if (there) {
+                    sm::load_to_lds(p.k_pages + (page[i] * p.sk.page + kvh * p.sk.head + at * p.sk.row + d) * P::SIZE, to_k);
+                    sm::load_to_lds(p.v_pages + (page[i] * p.sv.page + kvh * p.sv.head + at * p.sv.row + d) * P::SIZE, to_v);
+                } else {
+                    *reinterpret_cast<bf16x8*>(&lds.k[buffer].x[(row + i * APART) * DP + slot * 8]) = bf16x8{};
+                    *reinterpret_cast<bf16x8*>(&lds.v[buffer].x[(row + i * APART) * DP + slot * 8]) = bf16x8{};
+                }
+            } else {
+                // what is not there is read from a place that is, and dropped in arrive(): no load waits for a test
+                const int64_t from = there ? page[i] : 0, place = there ? at : 0, e = d < p.D ? d : 0;
+                k[i] = *reinterpret_cast<const Raw*>(
+                    p.k_pages + (from * p.sk.page + kvh * p.sk.head + place * p.sk.row + e) * P::SIZE);
+                v[i] = *reinterpret_cast<const Raw*>(
+                    p.v_pages + (from * p.sv.page + kvh * p.sv.head + place * p.sv.row + e) * P::SIZE);
+                if constexpr (coded<C>) {
+                    ke[i] = p.k_exp[from * p.ske.page + kvh * p.ske.head + place * p.ske.row + e / BLOCK];
+                    ve[i] = p.v_exp[from * p.sve.page + kvh * p.sve.head + place * p.sve.row + e / BLOCK];
+                }
+            }
+        }
+    }
+    // the rows that were fetched are in LDS from here on, and nobody reads the buffer that the next fetch goes to; mask:
+    // where not null, 0 or -inf for each of the tile's rows
+    __device__ __forceinline__ void arrive(Lds& lds, int buffer, int D, float* mask) {
+        if constexpr (BUFFERS == 1) __syncthreads();
+        if constexpr (DIRECT) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        } else {
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                if (!(ok >> i & 1) || slot * 8 >= D) {
+                    k[i] = v[i] = Raw{};
+                    ke[i] = ve[i] = 127;
+                }
+                const sm::Frag<NP> x = parts_of(k[i], 0, coded<C> ? power_of(ke[i]) : 1.f, C());
+                const sm::Frag<NP> y = parts_of(v[i], 0, coded<C> ? power_of(ve[i]) : 1.f, C());
+                const int at = TileT::at(row + i * APART, slot);
+#pragma unroll
+                for (int n = 0; n < NP; ++n) {
+                    *reinterpret_cast<bf16x8*>(&lds.k[buffer].x[n * TileT::PLANE + at]) = x.p[n];
+                    *reinterpret_cast<bf16x8*>(&lds.v[buffer].x[n * TileT::PLANE + at]) = y.p[n];
+                }
+            }
+        }
+        if (mask && slot == 0) {
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) mask[row + i * APART] = ok >> i & 1 ? 0.f : NONE;
+        }
+        __syncthreads();
+    }
+};
+
+template <class T, class C, int DP>
+__global__ __launch_bounds__(64 * TILE_WAVES, (sm::Elem<T>::PARTS == 3 && DP == 128 ? 1 : 2))
+void paged_tiles(const PgParams p) {
+    constexpr int NQ = sm::Elem<T>::PARTS, NK = Piece<C, 8>::PARTS, BN = sm_tile_rows(NK, DP), NS = BN / 32, ND = DP / 32;
+    constexpr int ROWS = PG_TILE_ROWS, NT = 64 * TILE_WAVES;
+    typedef Bring<C, DP, BN> BringT;
+    __shared__ __attribute__((aligned(16))) typename BringT::Lds lds;
+    __shared__ __attribute__((aligned(16))) float mask_of[BringT::BUFFERS][BN];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+    const int share = p.H / p.G;
+    const sm::Work w = sm::xcd_work(blockIdx.x, p.G, p.blocks * p.splits);
+    const int kvh = w.pair, split_i = w.block / p.blocks;
+    // a chunk's last rows see the most keys: they begin first
+    const Segment s0 = segment_of(p.offsets, p.B, p.T, share, ROWS, p.blocks - 1 - w.block % p.blocks);
+    const bool inside = s0.index >= 0 && s0.index < p.B;
+    const int rows = s0.rows * share, r0 = s0.block * ROWS, rw = r0 + wave * 32, r = rw + col;
+    if (r0 >= rows || (inside && rows <= p.few)) return;
+    const Tokens seq = inside ? tokens_of(p, s0.index, s0.first, s0.rows) : Tokens{s0.first, s0.rows, -s0.rows};
+
+    const bool real = r < rows;
+    const int head = kvh * share + r % share, t_q = s0.first + r / share;
+    const int last = seq.start + min(r0 + ROWS - 1, rows - 1) / share;              // the workgroup's last position
+    const int wave_first = seq.start + rw / share, wave_last = seq.start + min(rw + 31, rows - 1) / share;
+    const int seat = seq.start + r / share;
+    const int seen = p.num_pages ? min(max(last + 1, 0), p.places) : 0;
+    const int tiles = (seen + BN - 1) / BN;
+    int t = (int)((int64_t)tiles * split_i / p.splits);
+    const int t1 = (int)((int64_t)tiles * (split_i + 1) / p.splits);
+
+    const int* table = inside ? p.tables + s0.index * p.table_stride : nullptr;
+    // whether some page here does not exist
+    bool lacks = false;
+    if (t < t1) {
+        const int end = page_at(p, min(t1 * BN, seen) - 1);
+        for (int i = page_at(p, t * BN) + tid; i <= end; i += NT) lacks |= (uint32_t)table[i] >= (uint32_t)p.num_pages;
+    }
+    lacks = __syncthreads_or(lacks);
+    BringT tile(lds, p, tid);
+    int buffer = 0;
+    if (t < t1) {
+        tile.look(p, table, t, seen);
+        tile.fetch(lds, 0, p, kvh, t, tid);
+        if (t + 1 < t1) tile.look(p, table, t + 1, seen);
+    }
+
+    sm::Frag<NQ> qf[DP / 16];
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+        typename sm::Elem<T>::seg s = {};
+        if (real) s = sm::load_seg((const T*)p.q + head * p.sq.h + t_q * p.sq.r, 16 * c + 8 * half, p.D);
+        s = s * (T)p.q_sign;
+        qf[c] = sm::frag_of(s);
+    }
+
+    const float c1 = p.scale * sm::UNIT;
+    Gather<NK, NQ> o[ND];
+    float top = NONE, ref = 0.f, sum = 0.f;
+    bool wide = false;                                 // a row here has a large ref
+
+    for (; t < t1; ++t) {
+        const int n0 = t * BN;
+        float* mask = mask_of[buffer];
+        tile.arrive(lds, buffer, p.D, lacks ? mask : nullptr);
+        const auto& kt = lds.k[buffer];
+        const auto& vt = lds.v[buffer];
+        buffer ^= BringT::BUFFERS - 1;
+        if (t + 1 < t1) {
+            tile.fetch(lds, buffer, p, kvh, t + 1, tid);
+            if (t + 2 < t1) tile.look(p, table, t + 2, seen);
+        }
+        if (rw >= rows || n0 > wave_last) continue;
+
+        sm::f32x16 s[NS];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            Gather<NK, NQ> a;
+            a.start();
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) a.add(kt.row(32 * i + col, 16 * c + 8 * half), qf[c]);
+            __builtin_amdgcn_s_setprio(0);
+            a.join();
+            s[i] = a.main;
+        }
+        if (lacks) {
+#pragma unroll
+            for (int i = 0; i < NS; ++i) s[i] = sm::masked(s[i], mask, 32 * i + 4 * half);
+        }
+        if (n0 + BN - 1 > min(wave_first, seen - 1)) {
+            const int lim = min(seat, seen - 1) - n0 - 4 * half;         // the last key seen
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (32 * i + sm::reg_row(e) > lim) s[i][e] = NONE;
+        }
+        float hi = s[0][0];
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) hi = fmaxf(hi, s[i][e]);
+        hi = fmaxf(hi, sm::other_half(hi)) * c1;
+        if (__any(hi > top + MOVE)) {                                    // top -inf: any score at all
+            const bool before = top == NONE;
+            const float was = ref;
+            top = fmaxf(top, hi);
+            ref = top == NONE ? 0.f : top;
+            wide = __any(fabsf(ref) > sm::WIDE);
+            const float f = before ? 1.f : sm::exp_of(was - ref);        // the first time there is nothing to scale
+            sum *= f;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[d].main *= f;
+        }
+        float mul = 2.f * c1, add = -2.f * ref;
+        if (__builtin_expect(wide, 0)) {               // scores are rounded before the reference is taken off (WIDE)
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    s[i][e] = __builtin_fmaf(s[i][e], c1, 0.f) - ref;      // (a product would be contracted with it)
+                }
+            mul = 2.f;
+            add = 0.f;
+        }
+        float tile_sum = 0.f;                          // by tiles: thousands of terms one by one lose two digits more
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[d].start();
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                f32x8 e = sm::eight(s[i], c);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) e[j] = sm::fexp2(__builtin_fmaf(e[j], mul, add));
+                const sm::Frag<NQ> pf = sm::split<NQ>(e);
+                if constexpr (NQ == 1) {
+                    sum = sm::add_all(pf.p[0], sum);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) tile_sum += e[j];
+                }
+#pragma unroll
+                for (int d = 0; d < ND; ++d) o[d].add(vt.column(32 * i + 16 * c, 32 * d, lane), pf);
+            }
+        sum += tile_sum;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[d].join();
+    }
+    if (!real) return;
+    sum += sm::other_half(sum);
+    if (p.splits > 1) {
+        const int64_t at = ((int64_t)split_i * p.H + head) * p.T + t_q;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                *reinterpret_cast<f32x4*>(p.part + at * DP + 32 * d + 8 * e + 4 * half) = sm::quad(o[d].main, e);
+        if (half == 0) {
+            p.part2[2 * at] = ref;
+            p.part2[2 * at + 1] = sum;
+        }
+        return;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    T* out = (T*)p.out + head * p.so.h + t_q * p.so.r;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            sm::store4(out, 32 * d + 8 * e + 4 * half, p.D, sm::quad(o[d].main, e) * inv);
+}
+
+}  // namespace pg
+
+int pg_tiles(int dtype, int held, const PgParams& p, hipStream_t st) {
+    return pg::dispatch_types(dtype, held, [&](auto t, auto c) {
+        return pg::by_width(p.D, [&](auto dp) {
+            const dim3 grid((unsigned)((int64_t)p.G * p.blocks * p.splits));
+            pg::paged_tiles<decltype(t), decltype(c), dp.value><<<grid, 64 * pg::TILE_WAVES, 0, st>>>(p);
+            return (int)hipGetLastError(); }); });
+}
+
+}  // namespace qlka

@@ -757,6 +757,168 @@ Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
     return std::get<0>(packed_forward(c, false, false));
 }
 
+// ---- a cache of keys and values in pages (qlka_paged_*)
+
+// The pages, and where the sequences are in them.
+struct PagedCall {
+    Tensor k_pages, v_pages, k_exp, v_exp, tables, lengths, offsets;    // exponents and offsets may be undefined
+};
+
+PagedCall paged_call(const Tensor& k_pages, const Tensor& v_pages, const OptTensor& k_exp, const OptTensor& v_exp,
+                     const Tensor& tables, const Tensor& lengths, const OptTensor& offsets) {
+    return {k_pages, v_pages, k_exp.value_or(Tensor()), v_exp.value_or(Tensor()), tables, lengths, offsets.value_or(Tensor())};
+}
+
+int held_of(const Tensor& pages) {
+    switch (pages.scalar_type()) {
+        case at::kFloat: return QLKA_F32;
+        case at::kBFloat16: return QLKA_BF16;
+        case at::kChar: return QLKA_INT8;
+        case at::kFloat8_e4m3fn: return QLKA_E4M3;
+        default: return -1;
+    }
+}
+
+// Checks the cache alone: (num_pages, G, page_size, D) of one type, exponents (num_pages, G, page_size, ceil(D / 32)).
+void check_pages(const Tensor& k, const Tensor& v, const Tensor& k_exp, const Tensor& v_exp) {
+    TORCH_CHECK(k.is_cuda() && v.is_cuda(), "pages must be CUDA tensors");
+    TORCH_CHECK(held_of(k) >= 0, "pages must be float32, bfloat16, int8 or float8_e4m3fn");
+    TORCH_CHECK(k.scalar_type() == v.scalar_type() && k.sizes() == v.sizes() && k.device() == v.device(),
+                "the pages of k and v must have one dtype, shape and device");
+    TORCH_CHECK(k.dim() == 4, "pages must be 4D: (num_pages, key heads, page_size, D)");
+    TORCH_CHECK(k.size(1) >= 1, "pages must have key heads");
+    TORCH_CHECK(1 <= k.size(2) && k.size(2) <= 65536, "page_size must be in [1, 65536]");
+    TORCH_CHECK(8 <= k.size(3) && k.size(3) <= 128 && k.size(3) % 8 == 0,
+                "the head dimension of pages must be a multiple of 8 in [8, 128]");
+    TORCH_CHECK(k.size(0) <= INT32_MAX, "at most 2^31 - 1 pages");
+    TORCH_CHECK(!at::GradMode::is_enabled() || (!k.requires_grad() && !v.requires_grad()),
+                "attention over pages has no gradient: pages must not require one");
+    TORCH_CHECK(k.stride(3) == 1 && v.stride(3) == 1, "the elements of a row of pages must be next to each other");
+    if (held_of(k) < QLKA_INT8) {
+        TORCH_CHECK(!k_exp.defined() && !v_exp.defined(), "exponents go with pages of 8 bits");
+        return;
+    }
+    TORCH_CHECK(k_exp.defined() && v_exp.defined(), "pages of 8 bits need exponents");
+    for (const Tensor& e : {k_exp, v_exp}) {
+        TORCH_CHECK(e.is_cuda() && e.device() == k.device(), "exponents must be on the pages' device");
+        TORCH_CHECK(e.scalar_type() == at::kByte, "exponents must be uint8");
+        TORCH_CHECK(e.dim() == 4 && e.size(0) == k.size(0) && e.size(1) == k.size(1) && e.size(2) == k.size(2) &&
+                        e.size(3) == (k.size(3) + 31) / 32,
+                    "exponents must be (num_pages, key heads, page_size, ceil(D / 32)), got ", e.sizes());
+        TORCH_CHECK(e.size(3) == 1 || e.stride(3) == 1, "the exponents of a row must be next to each other");
+    }
+}
+
+// The sizes of a call on x's type and device; T rows of `heads` heads.
+qlka_paged_args paged_args(const PagedCall& c, at::ScalarType dtype, int64_t T, int64_t heads) {
+    check_pages(c.k_pages, c.v_pages, c.k_exp, c.v_exp);
+    TORCH_CHECK(dtype == at::kFloat || dtype == at::kBFloat16, "tokens must be float32 or bfloat16");
+    const int held = held_of(c.k_pages), type = dtype == at::kFloat ? QLKA_F32 : QLKA_BF16;
+    TORCH_CHECK(held >= QLKA_INT8 || held == type, "pages must have the tokens' dtype or 8 bits");
+    for (const Tensor& t : {c.tables, c.lengths}) {
+        TORCH_CHECK(t.is_cuda() && t.device() == c.k_pages.device(), "tables and lengths must be on the pages' device");
+        TORCH_CHECK(t.scalar_type() == at::kInt, "tables and lengths must be int32");
+    }
+    TORCH_CHECK(c.tables.dim() == 2 && c.lengths.dim() == 1 && c.tables.size(0) == c.lengths.size(0),
+                "tables must be (B, pages) and lengths (B)");
+    TORCH_CHECK(c.lengths.is_contiguous() && (c.tables.size(1) <= 1 || c.tables.stride(1) == 1),
+                "lengths and the rows of tables must be contiguous");
+    TORCH_CHECK(c.tables.size(0) <= (1 << 28) && c.tables.size(1) <= INT32_MAX, "at most 2^28 sequences");
+    if (c.offsets.defined()) {
+        check_offsets(c.offsets, c.k_pages);
+        TORCH_CHECK(c.offsets.size(0) == c.lengths.size(0) + 1, "offsets must be (B + 1)");
+    }
+    const Tensor& k = c.k_pages;
+    TORCH_CHECK(heads >= 1 && heads % k.size(1) == 0, "the heads of q must be a multiple of those of the pages");
+    TORCH_CHECK(T <= (1 << 28) && (double)T * heads <= INT32_MAX, "at most 2^28 rows, and heads * rows must fit int32");
+    qlka_paged_args a{};
+    a.dtype = type;
+    a.held = held;
+    a.B = (int)c.lengths.size(0); a.H = (int)heads; a.G = (int)k.size(1); a.T = (int)T; a.D = (int)k.size(3);
+    a.page_size = (int)k.size(2); a.num_pages = (int)k.size(0); a.table_len = (int)c.tables.size(1);
+    a.tables = c.tables.data_ptr<int>();
+    a.lengths = c.lengths.data_ptr<int>();
+    a.offsets = c.offsets.defined() ? c.offsets.data_ptr<int>() : nullptr;
+    a.table_stride = c.tables.stride(0);
+    a.k_pages = k.data_ptr(); a.v_pages = c.v_pages.data_ptr();
+    set_strides(a.k_pages_stride, k); set_strides(a.v_pages_stride, c.v_pages);
+    if (c.k_exp.defined()) {
+        a.k_exp = c.k_exp.data_ptr<uint8_t>(); a.v_exp = c.v_exp.data_ptr<uint8_t>();
+        set_strides(a.k_exp_stride, c.k_exp); set_strides(a.v_exp_stride, c.v_exp);
+    }
+    return a;
+}
+
+// New tokens' rows (heads, T, D) next to the pages.
+void check_tokens(const char* name, const Tensor& x, const PagedCall& c) {
+    TORCH_CHECK(x.is_cuda() && x.device() == c.k_pages.device(), name, " must be on the pages' device");
+    TORCH_CHECK(x.dim() == 3 && x.size(2) == c.k_pages.size(3), name, " must be (heads, rows, D) with the pages' D");
+    TORCH_CHECK(c.offsets.defined() || x.size(1) == c.lengths.size(0),
+                "without offsets every sequence has one token: rows must be B");
+    TORCH_CHECK(!x._fw_grad(0).defined(), "attention over pages has no forward-mode derivative");
+    TORCH_CHECK(!at::GradMode::is_enabled() || !x.requires_grad(), "attention over pages has no gradient: ", name,
+                " must not require one");
+}
+
+void paged_write(const Tensor& k_, const Tensor& v_, const Tensor& k_pages, const Tensor& v_pages, const OptTensor& k_exp,
+                 const OptTensor& v_exp, const Tensor& tables, const Tensor& lengths, const OptTensor& offsets) {
+    const PagedCall c = paged_call(k_pages, v_pages, k_exp, v_exp, tables, lengths, offsets);
+    check_pages(c.k_pages, c.v_pages, c.k_exp, c.v_exp);
+    check_tokens("k", k_, c);
+    check_tokens("v", v_, c);
+    TORCH_CHECK(k_.sizes() == v_.sizes() && k_.scalar_type() == v_.scalar_type(), "k and v must have one shape and dtype");
+    TORCH_CHECK(k_.size(0) == k_pages.size(1), "k and v must have the heads of the pages");
+    c10::DeviceGuard guard(k_pages.device());
+    const Tensor k = packed_rows(k_), v = packed_rows(v_);
+    qlka_paged_args a = paged_args(c, k.scalar_type(), k.size(1), k.size(0));
+    a.k = k.data_ptr(); a.v = v.data_ptr();
+    set_strides(a.k_stride, k); set_strides(a.v_stride, v);
+    check_rc(qlka_paged_write(&a, stream_of(k_pages)));
+    for (const Tensor& t : {c.k_pages, c.v_pages, c.k_exp, c.v_exp})
+        if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+std::tuple<Tensor, Tensor> paged_read(const Tensor& k_pages, const Tensor& v_pages, const OptTensor& k_exp,
+                                      const OptTensor& v_exp, const Tensor& tables, const Tensor& lengths, int64_t N,
+                                      at::ScalarType dtype) {
+    const PagedCall c = paged_call(k_pages, v_pages, k_exp, v_exp, tables, lengths, OptTensor());
+    TORCH_CHECK(0 <= N && N <= (1 << 28), "the number of positions must be in [0, 2^28]");
+    qlka_paged_args a = paged_args(c, dtype, lengths.dim() ? lengths.size(0) : 0, k_pages.size(1));
+    TORCH_CHECK((double)a.B * a.G * N <= INT32_MAX, "batch * heads * positions must fit int32");
+    a.N = (int)N;
+    c10::DeviceGuard guard(k_pages.device());
+    const auto options = k_pages.options().dtype(dtype);
+    Tensor k = at::empty({a.B, a.G, N, a.D}, options), v = at::empty({a.B, a.G, N, a.D}, options);
+    a.out_k = k.data_ptr(); a.out_v = v.data_ptr();
+    set_strides(a.out_k_stride, k); set_strides(a.out_v_stride, v);
+    check_rc(qlka_paged_read(&a, stream_of(k_pages)));
+    return {k, v};
+}
+
+Tensor paged_attention(const Tensor& q_, const Tensor& k_pages, const Tensor& v_pages, const OptTensor& k_exp,
+                       const OptTensor& v_exp, const Tensor& tables, const Tensor& lengths, const OptTensor& offsets,
+                       int64_t longest, double scale) {
+    const PagedCall c = paged_call(k_pages, v_pages, k_exp, v_exp, tables, lengths, offsets);
+    check_pages(c.k_pages, c.v_pages, c.k_exp, c.v_exp);
+    check_tokens("q", q_, c);
+    TORCH_CHECK(0 <= longest && longest <= INT32_MAX, "longest must be in [0, 2^31)");
+    c10::DeviceGuard guard(k_pages.device());
+    const Tensor q = packed_rows(q_);
+    qlka_paged_args a = paged_args(c, q.scalar_type(), q.size(1), q.size(0));
+    Tensor out = empty_rows(q);
+    a.longest = (int)longest;
+    a.scale = (float)scale;
+    a.q = q.data_ptr();
+    set_strides(a.q_stride, q);
+    a.out = out.data_ptr();
+    set_strides(a.out_stride, out);
+    const size_t bytes = qlka_paged_attention_ws_bytes(&a);
+    Tensor ws;
+    if (bytes) ws = workspace(bytes, q);
+    check_rc(qlka_paged_attention(&a, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(k_pages)));
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -801,5 +963,19 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("packed_attention", &packed_attention, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("offsets"),
           py::arg("scale"), py::arg("causal"),
           "differentiable softmax attention within packed sequences (qlka_packed_fwd / qlka_packed_bwd)");
+    m.def("check_pages", [](const Tensor& k, const Tensor& v, const OptTensor& ke, const OptTensor& ve) {
+        check_pages(k, v, ke.value_or(Tensor()), ve.value_or(Tensor()));
+    }, py::arg("k_pages"), py::arg("v_pages"), py::arg("k_exp"), py::arg("v_exp"), "refuses what is no cache in pages");
+    m.def("paged_write", &paged_write, py::arg("k"), py::arg("v"), py::arg("k_pages"), py::arg("v_pages"),
+          py::arg("k_exp"), py::arg("v_exp"), py::arg("tables"), py::arg("lengths"), py::arg("offsets"),
+          "new tokens into the pages (qlka_paged_write)");
+    m.def("paged_read", [](const Tensor& k, const Tensor& v, const OptTensor& ke, const OptTensor& ve, const Tensor& tables,
+                           const Tensor& lengths, int64_t N, py::object dtype) {
+        return paged_read(k, v, ke, ve, tables, lengths, N, torch::python::detail::py_object_to_dtype(dtype));
+    }, py::arg("k_pages"), py::arg("v_pages"), py::arg("k_exp"), py::arg("v_exp"), py::arg("tables"), py::arg("lengths"),
+          py::arg("N"), py::arg("dtype"), "the first N positions of each sequence (qlka_paged_read)");
+    m.def("paged_attention", &paged_attention, py::arg("q"), py::arg("k_pages"), py::arg("v_pages"), py::arg("k_exp"),
+          py::arg("v_exp"), py::arg("tables"), py::arg("lengths"), py::arg("offsets"), py::arg("longest"),
+          py::arg("scale"), "attention of new tokens over the pages (qlka_paged_attention)");
     m.attr("DIRECT") = DIRECT;
 }

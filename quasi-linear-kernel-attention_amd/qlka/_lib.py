@@ -48,8 +48,24 @@ class PackedArgs(ctypes.Structure):
                 + [(n, _c_i64x2) for n in ("g_q_stride", "g_k_stride", "g_v_stride")])
 
 
+class PagedArgs(ctypes.Structure):
+    """qlka_paged_args of include/qlka.h."""
+    _fields_ = ([(n, _c_int) for n in ("dtype", "held", "B", "H", "G", "T", "D", "page_size", "num_pages", "table_len",
+                                       "longest", "N")]
+                + [("scale", ctypes.c_float)]
+                + [(n, _c_ptr) for n in ("tables", "lengths", "offsets")]
+                + [("table_stride", ctypes.c_int64), ("k_pages", _c_ptr), ("v_pages", _c_ptr),
+                   ("k_pages_stride", _c_i64x3), ("v_pages_stride", _c_i64x3), ("k_exp", _c_ptr), ("v_exp", _c_ptr),
+                   ("k_exp_stride", _c_i64x3), ("v_exp_stride", _c_i64x3)]
+                + [(n, _c_ptr) for n in ("q", "k", "v")]
+                + [(n, _c_i64x2) for n in ("q_stride", "k_stride", "v_stride")]
+                + [(n, _c_ptr) for n in ("out", "out_k", "out_v")]
+                + [("out_stride", _c_i64x2), ("out_k_stride", _c_i64x3), ("out_v_stride", _c_i64x3)])
+
+
 _c_softmax = ctypes.POINTER(SoftmaxArgs)
 _c_packed = ctypes.POINTER(PackedArgs)
+_c_paged = ctypes.POINTER(PagedArgs)
 _c_border = [ctypes.POINTER(_c_int), _c_int, _c_int]       # border, num_borders, bidirectional
 
 # name -> (restype, argtypes)
@@ -86,6 +102,10 @@ _SIGNATURES = {
     "qlka_packed_fwd": (_c_int, [_c_packed, _c_ptr, _c_size, _c_ptr]),
     "qlka_packed_bwd_ws_bytes": (_c_size, [_c_packed]),
     "qlka_packed_bwd": (_c_int, [_c_packed, _c_ptr, _c_size, _c_ptr]),
+    "qlka_paged_write": (_c_int, [_c_paged, _c_ptr]),
+    "qlka_paged_read": (_c_int, [_c_paged, _c_ptr]),
+    "qlka_paged_attention_ws_bytes": (_c_size, [_c_paged]),
+    "qlka_paged_attention": (_c_int, [_c_paged, _c_ptr, _c_size, _c_ptr]),
     "qlka_bias_map_fwd": (_c_int, [_c_ptr] + _c_border + [_c_ptr] + [_c_int] * 4 + [_c_ptr]),
     "qlka_bias_map_bwd_ws_bytes": (_c_size, [_c_int] * 5),
     "qlka_bias_map_bwd": (_c_int, [_c_ptr] + _c_border + [_c_ptr] + [_c_int] * 4 + [_c_ptr, _c_size, _c_ptr]),
