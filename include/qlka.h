@@ -337,7 +337,7 @@ int qlka_packed_bwd(const qlka_packed_args* args, void* ws, size_t ws_bytes, voi
 /*
  * A cache of keys and values in pages. A sequence's token at position i is row i % page_size of page
  * tables[b][i / page_size]; pages are rows of D elements for each of G key heads, at any strides (elements, between pages,
- * heads and rows). What is held (held):
+ * heads and rows, each below 2^32 bytes). What is held (held):
  *   QLKA_F32, QLKA_BF16  the rows as they are; of the type of the call (dtype) only
  *   QLKA_INT8, QLKA_E4M3 8 bits an element, and for every 32 elements of a row a byte e (k_exp, v_exp: ceil(D / 32) a row,
  *                        contiguous; strides in bytes between pages, heads and rows): an element stands for

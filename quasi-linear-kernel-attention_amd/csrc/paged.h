@@ -10,8 +10,17 @@
 
 namespace qlka {
 
-struct PgStrides { int64_t page, head, row; };                 // of pages, in elements or bytes of exponents
+struct PgStrides { uint32_t page, head, row; };                // of pages, in bytes (one instruction a product)
 struct PgOut { int64_t b, h, r; };
+
+// How a launch's work is cut (paged_device.h): workgroups aimed at for each key head, the least positions of a part, the
+// launch's size, and where the parts' sums go: [unit][rows of a block][padded D], and [unit][rows][2] (reference, sum).
+struct PgUnits {
+    float aim;
+    int least, groups;
+    int64_t room;                            // units that the workspace has places for
+    float *part, *part2;
+};
 
 struct PgParams {
     char *k_pages, *v_pages;
@@ -26,17 +35,16 @@ struct PgParams {
     int B, H, G, T, D, N;
     int page_size, num_pages, table_len;
     int places;                              // positions that a table's row has pages for
-    uint32_t magic, shift;                   // n / page_size = n * magic >> shift for n below 2^31
+    uint32_t magic, shift;                   // n / page_size = high word of 2 n * magic, >> shift, for n below 2^31
     float scale, q_sign;                     // |scale|; its sign (or 0)
-    int splits;                              // of a sequence's keys
-    int few;                                 // sequences of more rows a key head are the tiles' (paged_tiles)
-    int blocks;                              // of rows: of all sequences (paged_tiles), of each
-    int outside;                             // step kernel: it also writes the rows outside every sequence
-    float *part, *part2;                     // [split][H][T][padded D], [split][H][T][2], as softmax.h has them
+    PgUnits step, tiles;                     // few rows (paged_step.h) and chunks (paged_tiles.h); groups 0: not in this call
+    int few;                                 // sequences of more rows a key head are the tiles'
+    int blocks;                              // of rows (paged_read)
 };
 
 constexpr int BLOCK = 32;                    // elements of a row that share an exponent
 constexpr int LEAST_EXP = 27;
+constexpr int PG_ALIGN = 128;                // positions of a part: a multiple
 constexpr int PG_STEP_ROWS = 16;             // rows (of the heads that share a key head) of the step kernel's blocks
 constexpr int PG_READ_ROWS = 2;               // rows of a lane that reads the cache back
 constexpr int PG_TILE_ROWS = 128;            // of the tiles' workgroups
@@ -44,7 +52,8 @@ constexpr int PG_TILE_ROWS = 128;            // of the tiles' workgroups
 // Launchers; each returns a hipError_t value.
 int pg_write(int dtype, int held, const PgParams& p, hipStream_t st);
 int pg_read(int dtype, int held, const PgParams& p, hipStream_t st);
-int pg_step(int dtype, int held, const PgParams& p, hipStream_t st);
-int pg_tiles(int dtype, int held, const PgParams& p, hipStream_t st);
+int pg_attend_bf16(int held, const PgParams& p, hipStream_t st);
+int pg_attend_f32(int held, const PgParams& p, hipStream_t st);
+int pg_join(int dtype, const PgParams& p, hipStream_t st);
 
 }  // namespace qlka

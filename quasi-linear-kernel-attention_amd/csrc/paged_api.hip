@@ -32,11 +32,15 @@ int check_sizes(const qlka_paged_args* a) {
 
 // Sequences of up to FEW rows a key head go through the step kernel, 16 rows at a time, others through the tiles.
 constexpr int FEW = 32;
+// Workgroups of a launch that fill the GPU, and the least positions that one takes.
+constexpr int64_t STEP_LEAST = 256, TILE_GROUPS = 768, TILE_LEAST = 512;
 
 struct Plan {
-    bool step, tiles;
-    int few, step_blocks, tile_blocks, splits;
-    size_t part, part2;
+    bool step, tiles, join;
+    int few;
+    PgUnits units[2];                        // step, tiles
+    size_t part[2], part2[2];
+    size_t bytes() const { return part[0] + part2[0] + part[1] + part2[1]; }
 };
 Plan plan(const qlka_paged_args* a) {
     Plan r{};
@@ -51,34 +55,41 @@ Plan plan(const qlka_paged_args* a) {
         r.step = false;
         r.few = -1;
     }
-    r.step_blocks = (int)ceil_div(std::min<int64_t>(longest * share, std::max<int64_t>(FEW, share)), PG_STEP_ROWS);
-    r.tile_blocks = (int)segment_blocks(a->T, a->B, (int)share, PG_TILE_ROWS);
-
     const int64_t places = std::min<int64_t>((int64_t)a->table_len * a->page_size, LONGEST);
     const int DP = sm_padded(a->D);
-    int64_t splits = 1;
-    if (r.step) {
-        const int64_t groups = a->G * sequences * ceil_div(std::min<int64_t>(longest, ceil_div(a->T, sequences)) * share, PG_STEP_ROWS);
-        splits = std::min<int64_t>({ceil_div(1024, std::max<int64_t>(groups, 1)), places / 512, 256});
-    }
-    if (r.tiles) {
-        const int BN = sm_tile_rows(a->held == QLKA_F32 ? 3 : 1, DP);
-        const double tile_us = 0.6 * DP / 64 * BN / 64 * (a->dtype == QLKA_F32 ? 2 : 1);
-        splits = std::max<int64_t>(splits, splits_for((int64_t)a->G * ceil_div(a->T * share, PG_TILE_ROWS), ceil_div(places, BN),
-                                                      tile_us, (double)a->H * a->T * DP * 8));
-    }
-    r.splits = (int)std::max<int64_t>(splits, 1);
-    if (r.splits > 1) {
-        const size_t rows = (size_t)r.splits * a->H * a->T;
-        r.part = align256(rows * DP * 4);
-        r.part2 = align256(rows * 8);
+    const struct { bool used; int rows; int64_t groups, least; } kernels[2] = {
+        {r.step, PG_STEP_ROWS, coded(a) ? 768 : 1536, STEP_LEAST}, {r.tiles, PG_TILE_ROWS, TILE_GROUPS, TILE_LEAST}};
+    for (int i = 0; i < 2; ++i) {
+        const auto& k = kernels[i];
+        if (!k.used) continue;
+        // blocks of rows a key head: each sequence has one that is not full at most, and more in the step kernel only
+        // where it is alone
+        int64_t blocks = a->T * share / k.rows + a->B;
+        if (i == 0 && r.tiles) blocks = std::min<int64_t>(blocks, (int64_t)a->B * (FEW / PG_STEP_ROWS));
+        // a sequence's last part is shorter than the others: room for those within the round of workgroups
+        const int64_t last = a->G * (i == 0 ? sequences : a->T * share / k.rows + sequences) / 2;
+        const int64_t aim = std::max<int64_t>(std::max(k.groups - last, k.groups / 2) / a->G, 1);
+        const bool parts = places > k.least;
+        const int64_t units = (blocks + (parts ? aim + 1 : 0)) * a->G;          // the sum of parts rounded up
+        PgUnits& u = r.units[i];
+        u.aim = (float)aim;
+        u.least = (int)k.least;
+        u.room = units;
+        u.groups = (int)std::min<int64_t>(ceil_div(units, 8) * 8, INT32_MAX);
+        if (parts) {
+            r.join = true;
+            r.part[i] = align256((size_t)units * k.rows * DP * 4);
+            r.part2[i] = align256((size_t)units * k.rows * 8);
+        }
     }
     return r;
 }
 
 // ---- arguments to kernel parameters
 
-PgStrides page_strides(const int64_t* s) { return {s[0], s[1], s[2]}; }
+PgStrides page_strides(const int64_t* s, int size) {
+    return {(uint32_t)(s[0] * size), (uint32_t)(s[1] * size), (uint32_t)(s[2] * size)};
+}
 PgOut strides2(const int64_t* s) { return {0, s[0], s[1]}; }
 PgOut strides3(const int64_t* s) { return {s[0], s[1], s[2]}; }
 
@@ -86,9 +97,9 @@ PgOut strides3(const int64_t* s) { return {s[0], s[1], s[2]}; }
 int params(const qlka_paged_args* a, PgParams* p) {
     *p = PgParams{};
     p->k_pages = (char*)a->k_pages; p->v_pages = (char*)a->v_pages;
-    p->sk = page_strides(a->k_pages_stride); p->sv = page_strides(a->v_pages_stride);
+    p->sk = page_strides(a->k_pages_stride, held_size(a)); p->sv = page_strides(a->v_pages_stride, held_size(a));
     p->k_exp = a->k_exp; p->v_exp = a->v_exp;
-    p->ske = page_strides(a->k_exp_stride); p->sve = page_strides(a->v_exp_stride);
+    p->ske = page_strides(a->k_exp_stride, 1); p->sve = page_strides(a->v_exp_stride, 1);
     p->tables = a->tables; p->lengths = a->lengths; p->offsets = a->offsets;
     p->table_stride = a->table_stride;
     p->B = a->B; p->H = a->H; p->G = a->G; p->T = a->T; p->D = a->D; p->N = a->N;
@@ -96,9 +107,9 @@ int params(const qlka_paged_args* a, PgParams* p) {
     p->places = (int)std::min<int64_t>((int64_t)a->table_len * a->page_size, LONGEST);
     int log = 0;
     while (1 << log < a->page_size) ++log;
-    p->shift = 31 + log;
-    p->magic = (uint32_t)(((uint64_t(1) << p->shift) + a->page_size - 1) / a->page_size);
-    p->splits = p->blocks = 1;
+    p->shift = log;
+    p->magic = (uint32_t)(((uint64_t(1) << (31 + log)) + a->page_size - 1) / a->page_size);
+    p->blocks = 1;
     const int64_t sizes[3] = {a->num_pages, a->G, a->page_size};
     const struct { const char* name; const void* x; const int64_t* s; } pages[] = {
         {"k_pages", a->k_pages, a->k_pages_stride}, {"v_pages", a->v_pages, a->v_pages_stride}};
@@ -108,7 +119,8 @@ int params(const qlka_paged_args* a, PgParams* p) {
         bool aligned = (uintptr_t)o.x % unit == 0;
         for (int i = 0; i < 3; ++i) {
             if (sizes[i] <= 1) continue;
-            if (o.s[i] < 0) return refuse("the strides of %s must not be negative", o.name);
+            if (o.s[i] < 0 || o.s[i] * held_size(a) > UINT32_MAX)
+                return refuse("the strides of %s must be in [0, 2^32) bytes", o.name);
             aligned = aligned && o.s[i] * held_size(a) % unit == 0;
         }
         if (!aligned) return refuse("the rows of %s must be aligned to %d bytes", o.name, (int)unit);
@@ -116,8 +128,8 @@ int params(const qlka_paged_args* a, PgParams* p) {
     if (coded(a) && a->num_pages) {
         if (!a->k_exp || !a->v_exp) return refuse("k_exp and v_exp must be non-null where 8 bits are held");
         for (int i = 0; i < 3; ++i)
-            if (sizes[i] > 1 && (a->k_exp_stride[i] < 0 || a->v_exp_stride[i] < 0))
-                return refuse("the strides of k_exp and v_exp must not be negative");
+            if (sizes[i] > 1 && ((uint64_t)a->k_exp_stride[i] > UINT32_MAX || (uint64_t)a->v_exp_stride[i] > UINT32_MAX))
+                return refuse("the strides of k_exp and v_exp must be in [0, 2^32)");
     }
     if (a->B > 0 && (!a->lengths || (a->table_len > 0 && !a->tables))) return refuse("tables and lengths must be non-null");
     if (a->B > 1 && a->table_stride < 0) return refuse("table_stride must not be negative");
@@ -172,7 +184,7 @@ int qlka_paged_read(const qlka_paged_args* a, void* stream) {
 size_t qlka_paged_attention_ws_bytes(const qlka_paged_args* a) {
     if (check_sizes(a) || check_scale(a->scale)) return 0;
     const Plan r = plan(a);
-    return r.part + r.part2;
+    return r.bytes();
 }
 
 int qlka_paged_attention(const qlka_paged_args* a, void* ws, size_t ws_bytes, void* stream) {
@@ -186,43 +198,31 @@ int qlka_paged_attention(const qlka_paged_args* a, void* ws, size_t ws_bytes, vo
     if (a->T == 0) return QLKA_OK;
     if (!a->q || !a->out) return refuse("q and out must be non-null");
     const Plan r = plan(a);
-    if (int e = need_ws(ws, ws_bytes, r.part + r.part2)) return e;
-    p.outside = a->offsets && r.step && !r.tiles;
-    const int64_t segments = a->B + (p.outside ? 2 : 0);
-    if (r.step)
-        if (int e = fits_grid(segments * r.step_blocks * a->G * r.splits, 256)) return e;
-    if (r.tiles)
-        if (int e = fits_grid((int64_t)a->G * r.tile_blocks * r.splits, 2 * PG_TILE_ROWS)) return e;
-    if (r.splits > 1)
+    if (int e = need_ws(ws, ws_bytes, r.bytes())) return e;
+    if (int e = fits_grid((int64_t)r.units[0].groups + r.units[1].groups + 16, 256)) return e;
+    if (r.join)
         if (int e = fits_rows((int64_t)a->H * a->T, 64)) return e;
     p.q = a->q; p.out = a->out;
     p.sq = strides2(a->q_stride); p.so = strides2(a->out_stride);
     p.scale = a->scale == 0.f ? 1.f : std::fabs(a->scale);
     p.q_sign = a->scale == 0.f ? 0.f : a->scale < 0.f ? -1.f : 1.f;
     p.few = r.few;
-    p.splits = r.splits;
-    p.part = (float*)ws;
-    p.part2 = (float*)((char*)ws + r.part);
+    p.step = r.units[0];
+    p.tiles = r.units[1];
+    char* at = (char*)ws;
+    p.step.part = (float*)at; at += r.part[0];
+    p.step.part2 = (float*)at; at += r.part2[0];
+    p.tiles.part = (float*)at; at += r.part[1];
+    p.tiles.part2 = (float*)at;
     hipStream_t st = (hipStream_t)stream;
-    if (r.step && segments) {
-        StageTimer timer("paged_step", st);
-        p.blocks = r.step_blocks;
-        if (int e = pg_step(a->dtype, a->held, p, st)) return status(e, "attention over pages, few rows");
+    {
+        StageTimer timer("paged_attend", st);
+        const int e = a->dtype == QLKA_BF16 ? pg_attend_bf16(a->held, p, st) : pg_attend_f32(a->held, p, st);
+        if (e) return status(e, "attention over pages");
     }
-    if (r.tiles) {
-        StageTimer timer("paged_tiles", st);
-        p.blocks = r.tile_blocks;
-        if (int e = pg_tiles(a->dtype, a->held, p, st)) return status(e, "attention over pages");
-    }
-    if (r.splits == 1) return QLKA_OK;
-    SmParams c{};
-    c.B = 1; c.H = a->H; c.M = a->T; c.D = a->D;
-    c.out = a->out;
-    c.so = {0, a->out_stride[0], a->out_stride[1]};
-    c.splits = r.splits;
-    c.part = p.part; c.part2 = p.part2;
-    StageTimer timer("softmax_combine", st);
-    return status(sm_combine(a->dtype, c, st), "attention over pages, joining of splits");
+    if (!r.join) return QLKA_OK;
+    StageTimer timer("paged_join", st);
+    return status(pg_join(a->dtype, p, st), "attention over pages, joining of parts");
 }
 
 }  // extern "C"

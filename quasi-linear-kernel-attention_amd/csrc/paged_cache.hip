@@ -68,9 +68,10 @@ template <class T, class C, int DP> __global__ __launch_bounds__(256) void paged
         seat = at < 0 || at >= p.places ? -1 : (int)at;
     }
     if (seat < 0) return;
-    const int index = page_at(p, seat), page = p.tables[b * p.table_stride + index];
-    if ((uint32_t)page >= (uint32_t)p.num_pages) return;
-    const int row = seat - index * p.page_size, d = lane % LANES * 8;
+    const Place place = place_of(p, seat);
+    const uint32_t page = p.tables[b * p.table_stride + place.index];
+    if (page >= (uint32_t)p.num_pages) return;
+    const int d = lane % LANES * 8;
 #pragma unroll 2
     for (int i = lane / LANES; i < 2 * p.G; i += AT_ONCE) {
         const bool key = i < p.G;
@@ -78,10 +79,10 @@ template <class T, class C, int DP> __global__ __launch_bounds__(256) void paged
         const PgOut s = key ? p.snk : p.snv;
         const PgStrides to = key ? p.sk : p.sv;
         const auto x = sm::load_seg((const T*)(key ? p.k : p.v) + g * s.h + token * s.r, d, p.D);
-        char* pages = key ? p.k_pages : p.v_pages;
-        const int64_t at = page * to.page + g * to.head + row * to.row + d;
+        char* at = (key ? p.k_pages : p.v_pages) + (uint64_t)g * to.head + bytes_to(to, page, place.row) +
+                   d * Piece<C, 8>::SIZE;
         if constexpr (!coded<C>) {
-            if (d < p.D) *reinterpret_cast<typename sm::Elem<T>::seg*>(pages + at * (int64_t)sizeof(T)) = x;
+            if (d < p.D) *reinterpret_cast<typename sm::Elem<T>::seg*>(at) = x;
         } else {
             const f32x8 y = sm::floats(x);
             // the largest of the block's bits: NaN and infinities are above every finite number
@@ -92,10 +93,10 @@ template <class T, class C, int DP> __global__ __launch_bounds__(256) void paged
             most = max(most, (uint32_t)__shfl_xor((int)most, 2));
             const uint32_t e = exponent_of<C>(__uint_as_float(most));
             if (d < p.D) {
-                *reinterpret_cast<u32x2*>(pages + at) = codes_of<C>(y, e);
+                *reinterpret_cast<u32x2*>(at) = codes_of<C>(y, e);
                 if (d % BLOCK == 0) {
                     const PgStrides te = key ? p.ske : p.sve;
-                    (key ? p.k_exp : p.v_exp)[page * te.page + g * te.head + row * te.row + d / BLOCK] = (uint8_t)e;
+                    (key ? p.k_exp : p.v_exp)[(uint64_t)g * te.head + bytes_to(te, page, place.row) + d / BLOCK] = (uint8_t)e;
                 }
             }
         }
@@ -118,15 +119,16 @@ template <class T, class C, int DP> __global__ __launch_bounds__(256) void paged
         k[i] = v[i] = Raw{};
         ke[i] = ve[i] = 127;
         if (n >= length || n >= p.N) continue;
-        const int index = page_at(p, n), page = p.tables[b * p.table_stride + index], row = n - index * p.page_size;
-        if ((uint32_t)page >= (uint32_t)p.num_pages) continue;
-        k[i] = *reinterpret_cast<const Raw*>(
-            p.k_pages + (page * p.sk.page + g * p.sk.head + row * p.sk.row + d) * Piece<C, 8>::SIZE);
-        v[i] = *reinterpret_cast<const Raw*>(
-            p.v_pages + (page * p.sv.page + g * p.sv.head + row * p.sv.row + d) * Piece<C, 8>::SIZE);
+        const Place place = place_of(p, n);
+        const uint32_t page = p.tables[b * p.table_stride + place.index];
+        if (page >= (uint32_t)p.num_pages) continue;
+        k[i] = *reinterpret_cast<const Raw*>(p.k_pages + (uint64_t)g * p.sk.head + bytes_to(p.sk, page, place.row) +
+                                             d * Piece<C, 8>::SIZE);
+        v[i] = *reinterpret_cast<const Raw*>(p.v_pages + (uint64_t)g * p.sv.head + bytes_to(p.sv, page, place.row) +
+                                             d * Piece<C, 8>::SIZE);
         if constexpr (coded<C>) {
-            ke[i] = p.k_exp[page * p.ske.page + g * p.ske.head + row * p.ske.row + d / BLOCK];
-            ve[i] = p.v_exp[page * p.sve.page + g * p.sve.head + row * p.sve.row + d / BLOCK];
+            ke[i] = p.k_exp[(uint64_t)g * p.ske.head + bytes_to(p.ske, page, place.row) + d / BLOCK];
+            ve[i] = p.v_exp[(uint64_t)g * p.sve.head + bytes_to(p.sve, page, place.row) + d / BLOCK];
         }
     }
 #pragma unroll

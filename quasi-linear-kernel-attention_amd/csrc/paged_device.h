@@ -5,8 +5,13 @@
 #include "segments.h"
 #include "softmax_tile.h"
 
+#include <limits>
+
 namespace qlka {
 namespace pg {
+
+constexpr float LOW = -std::numeric_limits<float>::infinity();
+constexpr float GROW = 4.f;                  // of a row's reference: 2^8 of the exponentials
 
 using sm::bf16x2;
 using sm::bf16x4;
@@ -39,6 +44,7 @@ __device__ __forceinline__ float power_of(uint32_t e) {
 template <class C> __device__ __forceinline__ f32x4 four(uint32_t w, float s) {
     f32x4 x;
     if constexpr (std::is_same<C, Int8>::value) {
+        asm("" : "+v"(w));                   // (else the word may be loaded as four bytes)
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)(w >> 8 * i) * s;
     } else {
@@ -56,24 +62,175 @@ template <class C> __device__ __forceinline__ f32x8 eight(u32x2 w, float s) {
 // Eight elements as the parts that matrix products take (i: which eight of the piece).
 __device__ __forceinline__ sm::Frag<1> parts_of(bf16x8 x, int, float, __bf16) { return sm::frag_of(x); }
 __device__ __forceinline__ sm::Frag<3> parts_of(f32x8 x, int, float, float) { return sm::frag_of(x); }
-template <class C> __device__ __forceinline__ sm::Frag<1> parts_of(u32x2 x, int, float s, C) {
-    return sm::frag_of(__builtin_convertvector(eight<C>(x, s), bf16x8));
+__device__ __forceinline__ sm::Frag<1> parts_of(u32x2 x, int, float s, Int8) {
+    return sm::frag_of(__builtin_convertvector(eight<Int8>(x, s), bf16x8));
 }
-template <class C> __device__ __forceinline__ sm::Frag<1> parts_of(u32x4 x, int i, float s, C) {
-    return sm::frag_of(__builtin_convertvector(eight<C>(u32x2{x[2 * i], x[2 * i + 1]}, s), bf16x8));
+__device__ __forceinline__ sm::Frag<1> parts_of(u32x2 x, int, float s, E4m3) {      // an instruction for two
+    bf16x8 y;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[h], s, false);
+        const bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[h], s, true);
+        y[4 * h] = lo[0]; y[4 * h + 1] = lo[1]; y[4 * h + 2] = hi[0]; y[4 * h + 3] = hi[1];
+    }
+    return sm::frag_of(y);
+}
+template <class C> __device__ __forceinline__ sm::Frag<1> parts_of(u32x4 x, int i, float s, C c) {
+    return parts_of(u32x2{x[2 * i], x[2 * i + 1]}, 0, s, c);
 }
 
-// Where a position's page is in the table, and its row in the page.
-__device__ __forceinline__ int page_at(const PgParams& p, int n) {
-    return (int)((uint64_t)(uint32_t)n * p.magic >> p.shift);
+// A position's place: the index of its page in the table, and its row in the page.
+struct Place { int index, row; };
+__device__ __forceinline__ Place place_of(const PgParams& p, int n) {
+    const int index = (int)(__umulhi(2u * (uint32_t)n, p.magic) >> p.shift);
+    return {index, n - index * p.page_size};
+}
+// Where a row of a page is from the first one of its head on.
+__device__ __forceinline__ uint64_t bytes_to(PgStrides s, uint32_t page, uint32_t row) {
+    return (uint64_t)page * s.page + (uint64_t)row * s.row;
 }
 
-// The new tokens of a sequence: `first` of the T rows on, `rows` of them, the first at position `start`.
+// Sums over the lanes up to this one, in registers; the last lane has the sum of all.
+template <int CTRL, int ROWS, class X> __device__ __forceinline__ X moved(X x) {
+    union { X x; int i; } a{x}, y;
+    y.i = __builtin_amdgcn_update_dpp(0, a.i, CTRL, ROWS, 0xf, false);
+    return y.x;
+}
+template <class X> __device__ __forceinline__ X sums_upto(X x) {
+    x += moved<0x111, 0xf>(x);               // row_shr 1, 2, 4, 8
+    x += moved<0x112, 0xf>(x);
+    x += moved<0x114, 0xf>(x);
+    x += moved<0x118, 0xf>(x);
+    x += moved<0x142, 0xa>(x);               // row_bcast 15 into rows 1 and 3
+    x += moved<0x143, 0xc>(x);               // row_bcast 31 into rows 2 and 3
+    return x;
+}
+template <class X> __device__ __forceinline__ X last_lane(X x) {
+    union { X x; int i; } a{x}, y;
+    y.i = __builtin_amdgcn_readlane(a.i, 63);
+    return y.x;
+}
+
+// The new tokens of a sequence: `rows` of them from row `first` on, the first at position `start`.
 struct Tokens { int first, rows, start; };
-__device__ __forceinline__ Tokens tokens_of(const PgParams& p, int b, int first, int rows) {
-    const int length = min(max(p.lengths[b], 0), 1 << 28);
-    return {first, rows, length - rows};
+__device__ __forceinline__ Tokens tokens_of(const PgParams& p, int b) {
+    int first = b, rows = 1;
+    if (p.offsets) {
+        first = segment_edge(p.offsets, p.B, p.T, b + 1);
+        rows = max(segment_edge(p.offsets, p.B, p.T, b + 2) - first, 0);
+    }
+    return {first, rows, min(max(p.lengths[b], 0), 1 << 28) - rows};
 }
+// Positions up to `seat` that have a place.
+__device__ __forceinline__ int seen_from(const PgParams& p, int seat) {
+    return p.num_pages ? min(max(seat + 1, 0), p.places) : 0;
+}
+
+// How the work of a launch is cut into units of about equal time: a block of ROWS rows of one key head over `span` successive
+// positions. The span goes by what the sequences of this launch (STEP: those of few rows) hold together, which only
+// the device knows, so that there are about `aim` units a key head; every workgroup finds it, and its unit, by itself,
+// a lane a sequence. Units of one sequence, part and key head are next to each other, and successive ones on one XCD, whose L2
+// then serves their keys. Where a sequence's positions are one part, its rows are written at once, else each part's sums
+// go to the unit's place in the workspace and paged_join adds them up.
+struct Cut { int blocks, parts; };           // of a sequence: units a key head = blocks * parts
+struct Unit { int b, part, kvh, block, parts, span, at; };
+
+template <bool STEP, int ROWS> struct Units {
+    const PgParams& p;
+    const PgUnits& u;
+    int share, span, all;                    // all: units a key head
+
+    int first, before;                       // of the first 64 sequences, this lane's: units a key head, and up to them
+    Cut cut_here;
+
+    struct Held { int blocks, seen; };
+    __device__ __forceinline__ Held held(int b) const {
+        if (b >= p.B) return {0, 0};
+        const Tokens t = tokens_of(p, b);
+        const int rows = t.rows * share;
+        const bool mine = STEP == (rows <= p.few) && rows > 0;
+        return {mine ? (rows + ROWS - 1) / ROWS : 0, seen_from(p, t.start + t.rows - 1)};
+    }
+    __device__ __forceinline__ Cut cut(Held h) const { return {h.blocks, max(1, (h.seen + span - 1) / span)}; }
+
+    __device__ __forceinline__ Units(const PgParams& p, const PgUnits& u) : p(p), u(u), share(p.H / p.G) {
+        const int lane = threadIdx.x & 63;
+        const Held mine = held(lane);
+        float work = (float)mine.blocks * (float)mine.seen;
+#pragma unroll 1
+        for (int b = 64 + lane; b - lane < p.B; b += 64) {
+            const Held h = held(b);
+            work += (float)h.blocks * (float)h.seen;
+        }
+        work = last_lane(sums_upto(work));
+        span = max((int)fminf(work / u.aim, (float)(1 << 28)) + 1, u.least);
+        span = __builtin_amdgcn_readfirstlane((span + PG_ALIGN - 1) / PG_ALIGN * PG_ALIGN);
+        cut_here = cut(mine);
+        first = cut_here.blocks * cut_here.parts;
+        before = sums_upto(first);
+        all = upto(p.B);
+    }
+    // units of the sequences before `end`
+    __device__ __forceinline__ int upto(int end) const {
+        if (end <= 0) return 0;
+        int n = __builtin_amdgcn_readlane(before, min(end, 64) - 1);
+        if (end <= 64) return n;
+        const int lane = threadIdx.x & 63;
+        int more = 0;
+#pragma unroll 1
+        for (int b = 64 + lane; b - lane < end; b += 64) {
+            const Cut c = cut(held(b));
+            more += b < end ? c.blocks * c.parts : 0;
+        }
+        return n + last_lane(sums_upto(more));
+    }
+    // The unit of a workgroup; b < 0 where it has none.
+    __device__ __forceinline__ Unit of(int wg) const {
+        const int lane = threadIdx.x & 63, units = all * p.G, each = (units + 7) / 8;
+        Unit x{};
+        x.b = -1;
+        x.at = (wg & 7) * each + (wg >> 3);
+        // (offsets that decrease can make more units than a launch and its workspace are made for)
+        if ((wg >> 3) >= each || x.at >= units || x.at >= u.room) return x;
+        Cut c = cut_here;
+        int n = first, to = before, base = 0;          // of this lane's sequence; units a key head of those before the 64
+#pragma unroll 1
+        for (int b0 = 0;;) {
+            const uint64_t past = __ballot((base + to) * p.G > x.at);
+            if (past) {
+                const int l = __builtin_ctzll(past);
+                const int blocks = __builtin_amdgcn_readlane(c.blocks, l);
+                const int rest = x.at - (base + __builtin_amdgcn_readlane(to - n, l)) * p.G;
+                x.b = b0 + l;
+                x.parts = __builtin_amdgcn_readlane(c.parts, l);
+                x.span = span;
+                x.part = rest / (blocks * p.G);
+                x.kvh = rest % (blocks * p.G) / blocks;
+                x.block = rest % blocks;
+                return x;
+            }
+            base += last_lane(to);
+            b0 += 64;
+            if (b0 >= p.B) return x;
+            c = cut(held(b0 + lane));
+            n = c.blocks * c.parts;
+            to = sums_upto(n);
+        }
+    }
+};
+
+// Zeros for the rows outside every sequence, by `count` workgroups of which this is number wg.
+template <class T> __device__ __forceinline__ void write_outside(const PgParams& p, int wg, int count) {
+    const int lo = segment_edge(p.offsets, p.B, p.T, 1), hi = segment_edge(p.offsets, p.B, p.T, p.B + 1);
+    const int64_t rows = (int64_t)p.H * (lo + max(p.T - hi, 0));
+    const int lanes = p.D / 4;
+    for (int64_t i = (int64_t)wg * blockDim.x + threadIdx.x; i < rows * lanes; i += (int64_t)count * blockDim.x) {
+        const int d = (int)(i % lanes) * 4, head = (int)(i / lanes % p.H), n = (int)(i / lanes / p.H);
+        const int t = n < lo ? n : n - lo + hi;
+        sm::store4((T*)p.out + head * p.so.h + t * p.so.r, d, p.D, f32x4{});
+    }
+}
+constexpr int OUTSIDE_GROUPS = 16;
 
 // f(padded row length)
 template <class F> int by_width(int D, F f) {

@@ -1,0 +1,91 @@
+// Attention over pages: the sums of a row's parts (paged_device.h, Units) to the row.
+#include "paged_device.h"
+
+namespace qlka {
+namespace pg {
+
+// Adds up the parts of rows whose positions are more than one. A wave takes a row (MANY: 256 / DP rows of a token, since
+// finding the sequence costs as much as a row): its lanes look at the parts' references and sums, one each, then DP / 4
+// lanes take a part's sums.
+template <class T, int DP, bool MANY> __global__ __launch_bounds__(256) void paged_join(const PgParams p) {
+    constexpr int LANES = DP / 4, GROUPS = 64 / LANES;                 // lanes of a part's row
+    constexpr int LOOK = MANY ? LANES : 64, AT_ONCE = MANY ? 1 : GROUPS;
+    const int lane = threadIdx.x & 63, share = p.H / p.G, i = lane % LANES, group = lane / LANES;
+    const uint32_t w = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    const uint32_t turns = MANY ? (p.H + GROUPS - 1) / GROUPS : p.H;
+    const int t = (int)(w / turns), head0 = (int)(w % turns) * (MANY ? GROUPS : 1);
+    if (t >= p.T) return;
+    int b = t;
+    if (p.offsets) b = __builtin_amdgcn_readfirstlane(last_upto(p.B + 1, t, [&](int j) { return p.offsets[j]; }));
+    if (b < 0 || b >= p.B) return;
+    const Tokens seq = tokens_of(p, b);
+    const bool step = seq.rows * share <= p.few;
+    int span, before, blocks, parts;         // of the sequence: units a key head before it, its blocks and parts
+    const auto find = [&](const auto& units) {
+        const Cut c = units.cut(units.held(b));
+        span = units.span;
+        before = units.upto(b);
+        blocks = c.blocks;
+        parts = c.parts;
+    };
+    if (step) find(Units<true, PG_STEP_ROWS>(p, p.step));
+    else find(Units<false, PG_TILE_ROWS>(p, p.tiles));
+    if (parts == 1) return;
+    const int size = step ? PG_STEP_ROWS : PG_TILE_ROWS;
+    const PgUnits& u = step ? p.step : p.tiles;
+    const int seen = seen_from(p, seq.start + t - seq.first);
+    parts = max(1, (seen + span - 1) / span);                          // that this token sees
+    const int64_t next = (int64_t)p.G * blocks, apart = next * size;   // units and rows from a part to the next
+
+    const int head = MANY ? min(head0 + group, p.H - 1) : head0, kvh = head / share;
+    const int r = (t - seq.first) * share + head % share;
+    const int64_t unit = (int64_t)before * p.G + (int64_t)kvh * blocks + r / size;         // of part 0
+    if (unit < 0 || unit + (parts - 1) * next >= u.room) return;  // offsets that decrease
+    const int64_t row = unit * size + r % size;
+    float ref = LOW, sum = 0.f;
+    f32x4 x = {};
+#pragma unroll 1
+    for (int s0 = 0; s0 < parts; s0 += LOOK) {
+        const int mine = s0 + (MANY ? i : lane), count = min(LOOK, parts - s0);
+        float2 a = {LOW, 0.f};
+        if (mine < parts) a = *reinterpret_cast<const float2*>(u.part2 + 2 * (mine * apart + row));
+        if (a.y == 0.f) a.x = LOW;                                  // no key there
+        float top = a.x;
+#pragma unroll
+        for (int far = 1; far < LOOK; far *= 2) top = fmaxf(top, __shfl_xor(top, far));
+        top = fmaxf(top, ref);
+        const float to = top == LOW ? 0.f : top, was = sm::exp_of(ref - to), f = sm::exp_of(a.x - to);
+        ref = top;
+        sum = sum * was + a.y * f;
+        x = x * was;
+#pragma unroll 8
+        for (int s = MANY ? 0 : group; s < count; s += AT_ONCE)
+            x = x + *reinterpret_cast<const f32x4*>(u.part + ((s0 + s) * apart + row) * DP + 4 * i) *
+                        __shfl(f, MANY ? group * LANES + s : s);
+    }
+#pragma unroll
+    for (int far = 1; far < LOOK; far *= 2) sum += __shfl_xor(sum, far);
+    if constexpr (!MANY) {
+#pragma unroll
+        for (int far = LANES; far < 64; far *= 2)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] += __shfl_xor(x[e], far);
+    }
+    if (MANY ? head0 + group < p.H : group == 0)
+        sm::store4((T*)p.out + head * p.so.h + t * p.so.r, 4 * i, p.D, x * (sum == 0.f ? 0.f : 1.f / sum));
+}
+constexpr int64_t JOIN_MANY = 4096;          // rows
+
+}  // namespace pg
+
+int pg_join(int dtype, const PgParams& p, hipStream_t st) {
+    return sm::dispatch(dtype, p.D, [&](auto t, auto dp) {
+        const int64_t rows = (int64_t)p.T * p.H, at_once = 256 / dp.value, waves = p.T * ((p.H + at_once - 1) / at_once);
+        if (rows >= pg::JOIN_MANY)
+            pg::paged_join<decltype(t), dp.value, true><<<dim3((unsigned)((waves + 3) / 4)), 256, 0, st>>>(p);
+        else
+            pg::paged_join<decltype(t), dp.value, false><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, st>>>(p);
+        return (int)hipGetLastError(); });
+}
+
+}  // namespace qlka

@@ -6,6 +6,8 @@
 // that it brings, one tile ahead of them. bf16 rows go to LDS directly, into the other of two buffers; rows of 8 bits
 // stay in registers until the tile before is done with and become bf16 on their way into the other buffer (exactly, see
 // paged_cache.hip); float rows are split into three parts there, with one buffer.
+#pragma once
+
 #include "paged_device.h"
 
 #include <limits>
@@ -14,8 +16,6 @@ namespace qlka {
 namespace pg {
 
 constexpr int TILE_WAVES = PG_TILE_ROWS / 32;
-constexpr float NONE = -std::numeric_limits<float>::infinity();
-constexpr float MOVE = 4.f;                  // 2^8 of the exponentials
 
 // A sum of products of operands in NA and NB parts, the smaller parts' apart (softmax_tile.h, Acc).
 template <int NA, int NB> struct Gather {
@@ -38,6 +38,9 @@ template <int NA, int NB> struct Gather {
     }
 };
 
+// A key head's first rows of all pages.
+struct Heads { const char *k, *v; const uint8_t *ke, *ve; };
+
 // Tiles of keys and values on their way from pages into LDS.
 template <class C, int DP, int BN> struct Bring {
     typedef Piece<C, 8> P;
@@ -50,7 +53,7 @@ template <class C, int DP, int BN> struct Bring {
     struct Lds { TileT k[BUFFERS], v[BUFFERS]; };
 
     int row, slot;                           // this thread's first row, and its place among the row's pieces
-    int page[EACH];                          // of the tile that is fetched next
+    int page[EACH], at[EACH];                // of the tile that is fetched next: its rows' pages and places in them
     uint32_t ok;                             // which of the rows being brought are there
     Raw k[DIRECT ? 1 : EACH], v[DIRECT ? 1 : EACH];
     uint32_t ke[EACH], ve[EACH];
@@ -62,20 +65,21 @@ template <class C, int DP, int BN> struct Bring {
             __syncthreads();
         }
     }
-    // the pages of tile t; -1 for positions from seen on
+    // the pages of tile t
     __device__ __forceinline__ void look(const PgParams& p, const int* table, int t, int seen) {
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
             const int n = t * BN + row + i * APART;
-            page[i] = n < seen ? table[page_at(p, n)] : -1;
+            const Place place = place_of(p, min(n, seen - 1));
+            page[i] = n < seen ? table[place.index] : -1;
+            at[i] = place.row;
         }
     }
-    // tile t, whose pages have been looked up
-    __device__ __forceinline__ void fetch(Lds& lds, int buffer, const PgParams& p, int kvh, int t, int tid) {
+    // the tile whose pages have been looked up
+    __device__ __forceinline__ void fetch(Lds& lds, int buffer, const PgParams& p, const Heads& heads, int tid) {
         ok = 0;
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
-            const int n = t * BN + row + i * APART, at = n - page_at(p, n) * p.page_size;
             const bool there = (uint32_t)page[i] < (uint32_t)p.num_pages;
             ok |= (uint32_t)there << i;
             // a row's pieces are turned by bits of its number: where they go, or, straight to LDS, where they come from
@@ -86,22 +90,20 @@ template <class C, int DP, int BN> struct Bring {
                 const uint32_t to_v = sm::lds_place(&lds.v[buffer].x[first * DP]);
                 if (d >= p.D) continue;
                 if (there) {
-                    sm::load_to_lds(p.k_pages + (page[i] * p.sk.page + kvh * p.sk.head + at * p.sk.row + d) * P::SIZE, to_k);
-                    sm::load_to_lds(p.v_pages + (page[i] * p.sv.page + kvh * p.sv.head + at * p.sv.row + d) * P::SIZE, to_v);
+                    sm::load_to_lds(heads.k + bytes_to(p.sk, page[i], at[i]) + d * P::SIZE, to_k);
+                    sm::load_to_lds(heads.v + bytes_to(p.sv, page[i], at[i]) + d * P::SIZE, to_v);
                 } else {
                     *reinterpret_cast<bf16x8*>(&lds.k[buffer].x[(row + i * APART) * DP + slot * 8]) = bf16x8{};
                     *reinterpret_cast<bf16x8*>(&lds.v[buffer].x[(row + i * APART) * DP + slot * 8]) = bf16x8{};
                 }
             } else {
                 // what is not there is read from a place that is, and dropped in arrive(): no load waits for a test
-                const int64_t from = there ? page[i] : 0, place = there ? at : 0, e = d < p.D ? d : 0;
-                k[i] = *reinterpret_cast<const Raw*>(
-                    p.k_pages + (from * p.sk.page + kvh * p.sk.head + place * p.sk.row + e) * P::SIZE);
-                v[i] = *reinterpret_cast<const Raw*>(
-                    p.v_pages + (from * p.sv.page + kvh * p.sv.head + place * p.sv.row + e) * P::SIZE);
+                const uint32_t from = there ? page[i] : 0, e = d < p.D ? d : 0;
+                k[i] = *reinterpret_cast<const Raw*>(heads.k + bytes_to(p.sk, from, at[i]) + e * P::SIZE);
+                v[i] = *reinterpret_cast<const Raw*>(heads.v + bytes_to(p.sv, from, at[i]) + e * P::SIZE);
                 if constexpr (coded<C>) {
-                    ke[i] = p.k_exp[from * p.ske.page + kvh * p.ske.head + place * p.ske.row + e / BLOCK];
-                    ve[i] = p.v_exp[from * p.sve.page + kvh * p.sve.head + place * p.sve.row + e / BLOCK];
+                    ke[i] = heads.ke[bytes_to(p.ske, from, at[i]) + e / BLOCK];
+                    ve[i] = heads.ve[bytes_to(p.sve, from, at[i]) + e / BLOCK];
                 }
             }
         }
@@ -131,15 +133,15 @@ template <class C, int DP, int BN> struct Bring {
         }
         if (mask && slot == 0) {
 #pragma unroll
-            for (int i = 0; i < EACH; ++i) mask[row + i * APART] = ok >> i & 1 ? 0.f : NONE;
+            for (int i = 0; i < EACH; ++i) mask[row + i * APART] = ok >> i & 1 ? 0.f : LOW;
         }
         __syncthreads();
     }
 };
 
-template <class T, class C, int DP>
-__global__ __launch_bounds__(64 * TILE_WAVES, (sm::Elem<T>::PARTS == 3 && DP == 128 ? 1 : 2))
-void paged_tiles(const PgParams p) {
+template <class T, class C, int DP> constexpr int tiles_room() { return sm::Elem<T>::PARTS == 3 && DP == 128 ? 1 : 2; }
+
+template <class T, class C, int DP> __device__ __forceinline__ void tiles(const PgParams& p, int wg) {
     constexpr int NQ = sm::Elem<T>::PARTS, NK = Piece<C, 8>::PARTS, BN = sm_tile_rows(NK, DP), NS = BN / 32, ND = DP / 32;
     constexpr int ROWS = PG_TILE_ROWS, NT = 64 * TILE_WAVES;
     typedef Bring<C, DP, BN> BringT;
@@ -148,39 +150,37 @@ void paged_tiles(const PgParams p) {
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
     const int share = p.H / p.G;
-    const sm::Work w = sm::xcd_work(blockIdx.x, p.G, p.blocks * p.splits);
-    const int kvh = w.pair, split_i = w.block / p.blocks;
-    // a chunk's last rows see the most keys: they begin first
-    const Segment s0 = segment_of(p.offsets, p.B, p.T, share, ROWS, p.blocks - 1 - w.block % p.blocks);
-    const bool inside = s0.index >= 0 && s0.index < p.B;
-    const int rows = s0.rows * share, r0 = s0.block * ROWS, rw = r0 + wave * 32, r = rw + col;
-    if (r0 >= rows || (inside && rows <= p.few)) return;
-    const Tokens seq = inside ? tokens_of(p, s0.index, s0.first, s0.rows) : Tokens{s0.first, s0.rows, -s0.rows};
+    const Unit unit = Units<false, ROWS>(p, p.tiles).of(wg);
+    if (unit.b < 0) return;
+    const Tokens seq = tokens_of(p, unit.b);
+    const int kvh = unit.kvh, rows = seq.rows * share, r0 = unit.block * ROWS, rw = r0 + wave * 32, r = rw + col;
 
     const bool real = r < rows;
-    const int head = kvh * share + r % share, t_q = s0.first + r / share;
+    const int head = kvh * share + r % share, t_q = seq.first + r / share;
     const int last = seq.start + min(r0 + ROWS - 1, rows - 1) / share;              // the workgroup's last position
     const int wave_first = seq.start + rw / share, wave_last = seq.start + min(rw + 31, rows - 1) / share;
     const int seat = seq.start + r / share;
-    const int seen = p.num_pages ? min(max(last + 1, 0), p.places) : 0;
-    const int tiles = (seen + BN - 1) / BN;
-    int t = (int)((int64_t)tiles * split_i / p.splits);
-    const int t1 = (int)((int64_t)tiles * (split_i + 1) / p.splits);
+    const int seen = seen_from(p, last);
+    if (unit.part && (int64_t)unit.part * unit.span >= seen) return;   // (the first part leaves zeros all the same)
+    int t = unit.part * (unit.span / BN);
+    const int t1 = min(t + unit.span / BN, (seen + BN - 1) / BN);
 
-    const int* table = inside ? p.tables + s0.index * p.table_stride : nullptr;
+    const int* table = p.tables + unit.b * p.table_stride;
+    const Heads heads = {p.k_pages + (uint64_t)kvh * p.sk.head, p.v_pages + (uint64_t)kvh * p.sv.head,
+                         p.k_exp + (uint64_t)kvh * p.ske.head, p.v_exp + (uint64_t)kvh * p.sve.head};
     // whether some page here does not exist
     bool lacks = false;
     if (t < t1) {
-        const int end = page_at(p, min(t1 * BN, seen) - 1);
-        for (int i = page_at(p, t * BN) + tid; i <= end; i += NT) lacks |= (uint32_t)table[i] >= (uint32_t)p.num_pages;
+        const int end = place_of(p, min(t1 * BN, seen) - 1).index;
+        for (int i = place_of(p, t * BN).index + tid; i <= end; i += NT) lacks |= (uint32_t)table[i] >= (uint32_t)p.num_pages;
     }
     lacks = __syncthreads_or(lacks);
     BringT tile(lds, p, tid);
     int buffer = 0;
     if (t < t1) {
         tile.look(p, table, t, seen);
-        tile.fetch(lds, 0, p, kvh, t, tid);
-        if (t + 1 < t1) tile.look(p, table, t + 1, seen);
+        tile.fetch(lds, 0, p, heads, tid);
+        tile.look(p, table, min(t + 1, t1 - 1), seen);
     }
 
     sm::Frag<NQ> qf[DP / 16];
@@ -194,7 +194,7 @@ void paged_tiles(const PgParams p) {
 
     const float c1 = p.scale * sm::UNIT;
     Gather<NK, NQ> o[ND];
-    float top = NONE, ref = 0.f, sum = 0.f;
+    float top = LOW, ref = 0.f, sum = 0.f;
     bool wide = false;                                 // a row here has a large ref
 
     for (; t < t1; ++t) {
@@ -204,10 +204,10 @@ void paged_tiles(const PgParams p) {
         const auto& kt = lds.k[buffer];
         const auto& vt = lds.v[buffer];
         buffer ^= BringT::BUFFERS - 1;
-        if (t + 1 < t1) {
-            tile.fetch(lds, buffer, p, kvh, t + 1, tid);
-            if (t + 2 < t1) tile.look(p, table, t + 2, seen);
-        }
+        // (into registers the last tile is fetched once more: what is fetched behind a test is waited for where the
+        // paths meet)
+        if (!BringT::DIRECT || t + 1 < t1) tile.fetch(lds, buffer, p, heads, tid);
+        tile.look(p, table, min(t + 2, t1 - 1), seen);
         if (rw >= rows || n0 > wave_last) continue;
 
         sm::f32x16 s[NS];
@@ -232,7 +232,7 @@ void paged_tiles(const PgParams p) {
             for (int i = 0; i < NS; ++i)
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    if (32 * i + sm::reg_row(e) > lim) s[i][e] = NONE;
+                    if (32 * i + sm::reg_row(e) > lim) s[i][e] = LOW;
         }
         float hi = s[0][0];
 #pragma unroll
@@ -240,11 +240,11 @@ void paged_tiles(const PgParams p) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) hi = fmaxf(hi, s[i][e]);
         hi = fmaxf(hi, sm::other_half(hi)) * c1;
-        if (__any(hi > top + MOVE)) {                                    // top -inf: any score at all
-            const bool before = top == NONE;
+        if (__any(hi > top + GROW)) {                                    // top -inf: any score at all
+            const bool before = top == LOW;
             const float was = ref;
             top = fmaxf(top, hi);
-            ref = top == NONE ? 0.f : top;
+            ref = top == LOW ? 0.f : top;
             wide = __any(fabsf(ref) > sm::WIDE);
             const float f = before ? 1.f : sm::exp_of(was - ref);        // the first time there is nothing to scale
             sum *= f;
@@ -288,16 +288,16 @@ void paged_tiles(const PgParams p) {
     }
     if (!real) return;
     sum += sm::other_half(sum);
-    if (p.splits > 1) {
-        const int64_t at = ((int64_t)split_i * p.H + head) * p.T + t_q;
+    if (unit.parts > 1) {
+        const int64_t at = (int64_t)unit.at * ROWS + (r - r0);
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                *reinterpret_cast<f32x4*>(p.part + at * DP + 32 * d + 8 * e + 4 * half) = sm::quad(o[d].main, e);
+                *reinterpret_cast<f32x4*>(p.tiles.part + at * DP + 32 * d + 8 * e + 4 * half) = sm::quad(o[d].main, e);
         if (half == 0) {
-            p.part2[2 * at] = ref;
-            p.part2[2 * at + 1] = sum;
+            p.tiles.part2[2 * at] = ref;
+            p.tiles.part2[2 * at + 1] = sum;
         }
         return;
     }
@@ -311,13 +311,4 @@ void paged_tiles(const PgParams p) {
 }
 
 }  // namespace pg
-
-int pg_tiles(int dtype, int held, const PgParams& p, hipStream_t st) {
-    return pg::dispatch_types(dtype, held, [&](auto t, auto c) {
-        return pg::by_width(p.D, [&](auto dp) {
-            const dim3 grid((unsigned)((int64_t)p.G * p.blocks * p.splits));
-            pg::paged_tiles<decltype(t), decltype(c), dp.value><<<grid, 64 * pg::TILE_WAVES, 0, st>>>(p);
-            return (int)hipGetLastError(); }); });
-}
-
 }  // namespace qlka

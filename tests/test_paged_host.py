@@ -57,16 +57,16 @@ def test_values_that_are_not_finite():
 
 
 def test_division_by_the_page_size():
-    """n / size as n * magic >> shift, for every n below 2^31 (its ends, multiples and their neighbours)."""
+    """n / size as the high word of 2 n * magic, shifted, for n below 2^31 (its ends, multiples and their neighbours)."""
     rng = random.Random(0)
     for size in list(range(1, 300)) + [rng.randint(300, 65536) for _ in range(300)] + [65535, 65536]:
-        shift = 31 + (size - 1).bit_length()
-        magic = -(-(1 << shift) // size)
+        shift = (size - 1).bit_length()
+        magic = -(-(1 << 31 + shift) // size)
         assert magic < 1 << 32
         for n in [0, 1, size - 1, size, size + 1, (1 << 28) - 1, 1 << 28, (1 << 31) - 1] + [
                 rng.randint(0, (1 << 31) // size - 1) * size + d for d in (-1, 0, 1) for _ in range(30)]:
             if n >= 0:
-                assert n * magic >> shift == n // size
+                assert (2 * n * magic >> 32) >> shift == n // size
 
 
 # ------------------------------------------------------------------------------------------------------- refusals
@@ -117,8 +117,9 @@ WRONG = [
     (dict(offsets=None), "T must be B"), (dict(k_pages=None), "k_pages must be non-null"),
     (dict(k_pages=(1 << 12) + 8), "rows of k_pages must be aligned to 16"), (dict(v_pages_stride=(2048, 1024, 72)), "rows of v_pages must be aligned to 16"),
     (dict(D=40, v_pages_stride=(2048, 1024, 36)), "rows of v_pages must be aligned to 8"),
-    (dict(k_pages_stride=(-2048, 1024, 64)), "strides of k_pages must not be negative"),
-    (dict(k_exp=None), "k_exp and v_exp must be non-null"), (dict(v_exp_stride=(64, -1, 2)), "strides of k_exp and v_exp"),
+    (dict(k_pages_stride=(-2048, 1024, 64)), "strides of k_pages must be in"),
+    (dict(v_pages_stride=(1 << 33, 1024, 64)), "strides of v_pages must be in"), (dict(k_exp_stride=(1 << 32, 32, 2)), "strides of k_exp"),
+    (dict(k_exp=None), "k_exp and v_exp must be non-null"), (dict(v_exp_stride=(64, -1, 2)), "strides of k_exp and v_exp must be in"),
     (dict(lengths=None), "tables and lengths must be"), (dict(tables=None), "tables and lengths must be"),
     (dict(table_stride=-4), "table_stride must not"),
 ]
