@@ -139,47 +139,59 @@ template <bool STEP, int ROWS> struct Units {
     const PgParams& p;
     const PgUnits& u;
     int share, span, all;                    // all: units a key head
-
-    int first, before;                       // of the first 64 sequences, this lane's: units a key head, and up to them
-    Cut cut_here;
+    // of the first 64 sequences this lane's: looked up once
+    Tokens mine;
+    Cut cut_mine;
+    int first, before;                       // its units a key head, and those up to it
 
     struct Held { int blocks, seen; };
-    __device__ __forceinline__ Held held(int b) const {
-        if (b >= p.B) return {0, 0};
-        const Tokens t = tokens_of(p, b);
+    __device__ __forceinline__ Held held(int b, Tokens t) const {
         const int rows = t.rows * share;
-        const bool mine = STEP == (rows <= p.few) && rows > 0;
-        return {mine ? (rows + ROWS - 1) / ROWS : 0, seen_from(p, t.start + t.rows - 1)};
+        const bool here = b < p.B && STEP == (rows <= p.few) && rows > 0;
+        return {here ? (rows + ROWS - 1) / ROWS : 0, seen_from(p, t.start + t.rows - 1)};
     }
+    __device__ __forceinline__ Tokens load(int b) const { return b < p.B ? tokens_of(p, b) : Tokens{0, 0, 0}; }
     __device__ __forceinline__ Cut cut(Held h) const { return {h.blocks, max(1, (h.seen + span - 1) / span)}; }
 
-    __device__ __forceinline__ Units(const PgParams& p, const PgUnits& u) : p(p), u(u), share(p.H / p.G) {
+    __device__ __forceinline__ Units(const PgParams& p, const PgUnits& u) : Units(p, u, load_mine(p)) {}
+    static __device__ __forceinline__ Tokens load_mine(const PgParams& p) {
         const int lane = threadIdx.x & 63;
-        const Held mine = held(lane);
-        float work = (float)mine.blocks * (float)mine.seen;
+        return lane < p.B ? tokens_of(p, lane) : Tokens{0, 0, 0};
+    }
+    __device__ __forceinline__ Units(const PgParams& p, const PgUnits& u, Tokens mine)
+        : p(p), u(u), share(p.H / p.G), mine(mine) {
+        const int lane = threadIdx.x & 63;
+        const Held held_mine = held(lane, mine);
+        float work = (float)held_mine.blocks * (float)held_mine.seen;
 #pragma unroll 1
         for (int b = 64 + lane; b - lane < p.B; b += 64) {
-            const Held h = held(b);
+            const Held h = held(b, load(b));
             work += (float)h.blocks * (float)h.seen;
         }
         work = last_lane(sums_upto(work));
         span = max((int)fminf(work / u.aim, (float)(1 << 28)) + 1, u.least);
         span = __builtin_amdgcn_readfirstlane((span + PG_ALIGN - 1) / PG_ALIGN * PG_ALIGN);
-        cut_here = cut(mine);
-        first = cut_here.blocks * cut_here.parts;
+        cut_mine = cut(held_mine);
+        first = cut_mine.blocks * cut_mine.parts;
         before = sums_upto(first);
         all = upto(p.B);
+    }
+    // of a sequence that is the same for all lanes
+    __device__ __forceinline__ Tokens tokens(int b) const {
+        if (b >= 64) return tokens_of(p, b);
+        return {__builtin_amdgcn_readlane(mine.first, b), __builtin_amdgcn_readlane(mine.rows, b),
+                __builtin_amdgcn_readlane(mine.start, b)};
     }
     // units of the sequences before `end`
     __device__ __forceinline__ int upto(int end) const {
         if (end <= 0) return 0;
-        int n = __builtin_amdgcn_readlane(before, min(end, 64) - 1);
+        const int n = __builtin_amdgcn_readlane(before, min(end, 64) - 1);
         if (end <= 64) return n;
         const int lane = threadIdx.x & 63;
         int more = 0;
 #pragma unroll 1
         for (int b = 64 + lane; b - lane < end; b += 64) {
-            const Cut c = cut(held(b));
+            const Cut c = cut(held(b, load(b)));
             more += b < end ? c.blocks * c.parts : 0;
         }
         return n + last_lane(sums_upto(more));
@@ -192,7 +204,7 @@ template <bool STEP, int ROWS> struct Units {
         x.at = (wg & 7) * each + (wg >> 3);
         // (offsets that decrease can make more units than a launch and its workspace are made for)
         if ((wg >> 3) >= each || x.at >= units || x.at >= u.room) return x;
-        Cut c = cut_here;
+        Cut c = cut_mine;
         int n = first, to = before, base = 0;          // of this lane's sequence; units a key head of those before the 64
 #pragma unroll 1
         for (int b0 = 0;;) {
@@ -212,7 +224,7 @@ template <bool STEP, int ROWS> struct Units {
             base += last_lane(to);
             b0 += 64;
             if (b0 >= p.B) return x;
-            c = cut(held(b0 + lane));
+            c = cut(held(b0 + lane, load(b0 + lane)));
             n = c.blocks * c.parts;
             to = sums_upto(n);
         }

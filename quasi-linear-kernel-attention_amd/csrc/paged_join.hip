@@ -9,27 +9,40 @@ namespace pg {
 // lanes take a part's sums.
 template <class T, int DP, bool MANY> __global__ __launch_bounds__(256) void paged_join(const PgParams p) {
     constexpr int LANES = DP / 4, GROUPS = 64 / LANES;                 // lanes of a part's row
-    constexpr int LOOK = MANY ? LANES : 64, AT_ONCE = MANY ? 1 : GROUPS;
+    constexpr int LOOK = MANY ? LANES : 64, AT_ONCE = MANY ? 1 : GROUPS, EARLY = 8;
     const int lane = threadIdx.x & 63, share = p.H / p.G, i = lane % LANES, group = lane / LANES;
     const uint32_t w = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
     const uint32_t turns = MANY ? (p.H + GROUPS - 1) / GROUPS : p.H;
     const int t = (int)(w / turns), head0 = (int)(w % turns) * (MANY ? GROUPS : 1);
     if (t >= p.T) return;
+    // the sequence, looked up together with what its units are found from
+    const Tokens mine = Units<true, PG_STEP_ROWS>::load_mine(p);
     int b = t;
-    if (p.offsets) b = __builtin_amdgcn_readfirstlane(last_upto(p.B + 1, t, [&](int j) { return p.offsets[j]; }));
-    if (b < 0 || b >= p.B) return;
-    const Tokens seq = tokens_of(p, b);
-    const bool step = seq.rows * share <= p.few;
+    if (p.offsets) {
+        const uint64_t begun = __ballot(lane < p.B && mine.first <= t);
+        b = __popcll(begun) - 1;
+        if (b == 63) b = __builtin_amdgcn_readfirstlane(last_upto(p.B + 1, t, [&](int j) { return p.offsets[j]; }));
+        if (b < 0 || b >= p.B) return;
+    }
+    Tokens seq;
     int span, before, blocks, parts;         // of the sequence: units a key head before it, its blocks and parts
+    bool step;
     const auto find = [&](const auto& units) {
-        const Cut c = units.cut(units.held(b));
+        const Cut c = units.cut(units.held(b, seq));
         span = units.span;
         before = units.upto(b);
         blocks = c.blocks;
         parts = c.parts;
     };
-    if (step) find(Units<true, PG_STEP_ROWS>(p, p.step));
-    else find(Units<false, PG_TILE_ROWS>(p, p.tiles));
+    if (b < 64)
+        seq = {__builtin_amdgcn_readlane(mine.first, b), __builtin_amdgcn_readlane(mine.rows, b),
+               __builtin_amdgcn_readlane(mine.start, b)};
+    else
+        seq = tokens_of(p, b);
+    if (t < seq.first || t >= seq.first + seq.rows) return;            // behind the last sequence
+    step = seq.rows * share <= p.few;
+    if (step) find(Units<true, PG_STEP_ROWS>(p, p.step, mine));
+    else find(Units<false, PG_TILE_ROWS>(p, p.tiles, mine));
     if (parts == 1) return;
     const int size = step ? PG_STEP_ROWS : PG_TILE_ROWS;
     const PgUnits& u = step ? p.step : p.tiles;
@@ -46,10 +59,17 @@ template <class T, int DP, bool MANY> __global__ __launch_bounds__(256) void pag
     f32x4 x = {};
 #pragma unroll 1
     for (int s0 = 0; s0 < parts; s0 += LOOK) {
-        const int mine = s0 + (MANY ? i : lane), count = min(LOOK, parts - s0);
+        const int look = s0 + (MANY ? i : lane), count = min(LOOK, parts - s0), first = MANY ? 0 : group;
         float2 a = {LOW, 0.f};
-        if (mine < parts) a = *reinterpret_cast<const float2*>(u.part2 + 2 * (mine * apart + row));
-        if (a.y == 0.f) a.x = LOW;                                  // no key there
+        if (look < parts) a = *reinterpret_cast<const float2*>(u.part2 + 2 * (look * apart + row));
+        // the first parts' sums are on their way before their weights are known
+        f32x4 y[EARLY];
+        const auto from = [&](int s) {
+            return *reinterpret_cast<const f32x4*>(u.part + ((s0 + min(s, count - 1)) * apart + row) * DP + 4 * i);
+        };
+#pragma unroll
+        for (int e = 0; e < EARLY; ++e) y[e] = from(first + e * AT_ONCE);
+        if (a.y == 0.f) a.x = LOW;                                      // no key there
         float top = a.x;
 #pragma unroll
         for (int far = 1; far < LOOK; far *= 2) top = fmaxf(top, __shfl_xor(top, far));
@@ -58,10 +78,15 @@ template <class T, int DP, bool MANY> __global__ __launch_bounds__(256) void pag
         ref = top;
         sum = sum * was + a.y * f;
         x = x * was;
-#pragma unroll 8
-        for (int s = MANY ? 0 : group; s < count; s += AT_ONCE)
-            x = x + *reinterpret_cast<const f32x4*>(u.part + ((s0 + s) * apart + row) * DP + 4 * i) *
-                        __shfl(f, MANY ? group * LANES + s : s);
+        const auto weight = [&](int s) { return __shfl(f, MANY ? group * LANES + s % LANES : s & 63); };
+#pragma unroll
+        for (int e = 0; e < EARLY; ++e) {
+            const int s = first + e * AT_ONCE;
+            const float z = weight(s);
+            if (s < count) x = x + y[e] * z;
+        }
+#pragma unroll 4
+        for (int s = first + EARLY * AT_ONCE; s < count; s += AT_ONCE) x = x + from(s) * weight(s);
     }
 #pragma unroll
     for (int far = 1; far < LOOK; far *= 2) sum += __shfl_xor(sum, far);

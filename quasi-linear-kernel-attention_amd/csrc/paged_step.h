@@ -84,9 +84,10 @@ template <class T, class C, int DP, int EL> __device__ __forceinline__ void step
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
     const int share = p.H / p.G;
-    const Unit unit = Units<true, ROWS>(p, p.step).of(wg);
+    const Units<true, ROWS> units(p, p.step);
+    const Unit unit = units.of(wg);
     if (unit.b < 0) return;
-    const Tokens seq = tokens_of(p, unit.b);
+    const Tokens seq = units.tokens(unit.b);
     const int b = unit.b, kvh = unit.kvh, rows = seq.rows * share, r0 = unit.block * ROWS;
 
     // this lane's row, and the positions that the block's rows see

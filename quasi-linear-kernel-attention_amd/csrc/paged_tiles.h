@@ -150,9 +150,10 @@ template <class T, class C, int DP> __device__ __forceinline__ void tiles(const 
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
     const int share = p.H / p.G;
-    const Unit unit = Units<false, ROWS>(p, p.tiles).of(wg);
+    const Units<false, ROWS> units(p, p.tiles);
+    const Unit unit = units.of(wg);
     if (unit.b < 0) return;
-    const Tokens seq = tokens_of(p, unit.b);
+    const Tokens seq = units.tokens(unit.b);
     const int kvh = unit.kvh, rows = seq.rows * share, r0 = unit.block * ROWS, rw = r0 + wave * 32, r = rw + col;
 
     const bool real = r < rows;

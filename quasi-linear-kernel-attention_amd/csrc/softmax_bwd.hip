@@ -128,7 +128,9 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
     __shared__ uint8_t near_bucket[BUFFERS][BIAS ? ROWS + BN : 1];     // from the distance before near_bias's first on
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
-    const Work w = xcd_work(blockIdx.x, p.B * p.H, p.blocks * p.splits);
+    Work w;
+    if constexpr (PACKED) w = packed_work<false>(p, blockIdx.x);
+    else w = xcd_work(blockIdx.x, p.B * p.H, p.blocks * p.splits);
     const int split_i = w.block / p.blocks;
     const Span<PACKED> span(p, w.block % p.blocks, ROWS);
     const int head = w.pair % p.H, b = w.pair / p.H, kvh = head / (p.H / p.G);
@@ -365,9 +367,11 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dkv(co
     __shared__ float near_bias[BUFFERS][BIAS ? KEYS + BM : 1];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
-    const Work w = xcd_work(blockIdx.x, p.B * p.G, p.blocks * p.splits);
+    Work w;
+    if constexpr (PACKED) w = packed_work<true>(p, blockIdx.x);
+    else w = xcd_work(blockIdx.x, p.B * p.G, p.blocks * p.splits);
     const int split_i = w.block / p.blocks;
-    const Span<PACKED> span(p, w.block % p.blocks, KEYS);
+    const Span<PACKED> span(p, w.block % p.blocks, KEYS, true);
     const int kvh = w.pair % p.G, b = w.pair / p.G, share = p.H / p.G;
     const int n0 = span.block * KEYS, nw = n0 + wave * 32, n = nw + col;
     if (PACKED && n0 >= span.N()) return;

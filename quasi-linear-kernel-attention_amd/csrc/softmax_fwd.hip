@@ -42,7 +42,9 @@ void softmax_fwd(const SmParams p) {
     __shared__ __attribute__((aligned(16))) float mask_of[BUFFERS][BN];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
-    const Work w = xcd_work(blockIdx.x, p.B * p.H, p.blocks * p.splits);
+    Work w;
+    if constexpr (PACKED) w = packed_work<false>(p, blockIdx.x);
+    else w = xcd_work(blockIdx.x, p.B * p.H, p.blocks * p.splits);
     const int split_i = w.block / p.blocks;
     const Span<PACKED> span(p, w.block % p.blocks, ROWS);
     const int head = w.pair % p.H, b = w.pair / p.H, kvh = head / (p.H / p.G);

@@ -462,7 +462,7 @@ template <> struct Span<false> {
     const SmParams& p;
     int block;
     static constexpr int group = 0;
-    __device__ __forceinline__ Span(const SmParams& p, int block, int) : p(p), block(block) {}
+    __device__ __forceinline__ Span(const SmParams& p, int block, int, bool = false) : p(p), block(block) {}
     __device__ __forceinline__ int M() const { return p.M; }
     __device__ __forceinline__ int N() const { return p.N; }
     __device__ __forceinline__ int seen() const { return p.seen; }
@@ -473,14 +473,85 @@ template <> struct Span<false> {
 template <> struct Span<true> {
     int block, rows, inside;
     int first, group;                        // the first row, and the number of its group of 32
-    // in causal order a sequence's last rows see the most keys: they begin first
-    __device__ __forceinline__ Span(const SmParams& p, int number, int size) {
-        const Segment s = segment_of(p.offsets, p.sequences, p.M, 1, size, p.causal ? p.blocks - 1 - number : number);
+    // number: of the block among all; keys: the blocks are of keys (whose queries are those from them on)
+    __device__ __forceinline__ Span(const SmParams& p, int number, int size, bool keys = false) {
+        Segment s;
+        if (p.sequences <= HEAVY_FIRST) {
+            s = p.sequences <= 62 ? heavy_first<1>(p, number, size, keys) : heavy_first<EACH>(p, number, size, keys);
+        } else {
+            // Numbers without a block are at regular places where the sequences are alike (every second one for sequences of
+            // one block), and successive numbers are on different XCDs by turns: eight at a time are moved among
+            // themselves, or half of the XCDs would have nothing to do (128 x 4 heads of 128, fp32: 39 us, 34 so).
+            if ((number | 7) < p.blocks)
+                number = (number & ~7) | ((number + (((uint32_t)number >> 3) * 0x9e3779b1u >> 29)) & 7);
+            s = segment_of(p.offsets, p.sequences, p.M, 1, size, number);
+        }
         block = s.block;
         rows = s.rows;
         inside = s.index < 0 || s.index >= p.sequences ? 0 : s.rows;
         first = s.first;
         group = segment_start(first, s.index + 1, 1, 32);
+    }
+    // The blocks in the order of their work, most first: a call ends with its last workgroups, and a long sequence's take a
+    // hundred times as long as a short one's. A lane holds segments (segments.h) of n blocks each. In causal order a
+    // sequence has a block with 1, 2, .. n blocks to go through, so that sum(max(n - x, 0)) blocks have more than x;
+    // else n with n each, and sum(n where n > x) do. x is found bit by bit. No sequence's blocks leave out numbers.
+    static constexpr int EACH = 4, HEAVY_FIRST = 64 * EACH - 2;       // segments of a lane at most; sequences
+    static __device__ __forceinline__ int sum_of(int x) {
+        x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);           // row_shr 1, 2, 4, 8
+        x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+        x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+        x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+        x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);           // row_bcast 15, 31
+        x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+        return __builtin_amdgcn_readlane(x, 63);
+    }
+    template <int EACH> static __device__ __forceinline__ Segment heavy_first(const SmParams& p, int number, int size,
+                                                                              bool keys) {
+        const int lane = threadIdx.x & 63;
+        int at[EACH], rows[EACH], n[EACH];
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int j = 64 * i + lane;
+            at[i] = rows[i] = 0;
+            if (j < p.sequences + 2) {
+                at[i] = segment_edge(p.offsets, p.sequences, p.M, j);
+                rows[i] = max(segment_edge(p.offsets, p.sequences, p.M, j + 1) - at[i], 0);
+            }
+            n[i] = (rows[i] + size - 1) / size;
+        }
+        const auto above = [&](int x) {
+            int sum = 0;
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) sum += p.causal ? max(n[i] - x, 0) : n[i] > x ? n[i] : 0;
+            return sum_of(sum);
+        };
+        Segment s{-1, 0, 0, 0};
+        if (number >= above(0)) return s;
+        int x = 0;                           // the most with above(x) > number
+        for (int bit = 1 << (31 - __builtin_clz(p.M / size + 1)); bit; bit >>= 1)
+            if (above(x + bit) > number) x += bit;
+        const int rest = number - above(x + 1);
+        // causal: the rest-th segment of more than x blocks; else the rest-th block of those of x + 1 blocks
+        int which = p.causal ? rest : rest / (x + 1);
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const bool mine = p.causal ? n[i] > x : n[i] == x + 1;
+            const uint64_t those = __ballot(mine);
+            const int count = __popcll(those);
+            if (which < count) {
+                const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(those >> 32),
+                                                           __builtin_amdgcn_mbcnt_lo((uint32_t)those, 0u));
+                const int l = __builtin_ctzll(__ballot(mine && rank == which));
+                s.index = 64 * i + l - 1;
+                s.first = __builtin_amdgcn_readlane(at[i], l);
+                s.rows = __builtin_amdgcn_readlane(rows[i], l);
+                s.block = !p.causal ? rest % (x + 1) : keys ? (s.rows + size - 1) / size - 1 - x : x;
+                return s;
+            }
+            which -= count;
+        }
+        return s;
     }
     __device__ __forceinline__ int M() const { return rows; }
     __device__ __forceinline__ int N() const { return rows; }
@@ -489,6 +560,13 @@ template <> struct Span<true> {
     template <class T> __device__ __forceinline__ T* from(T* x, int64_t stride) const { return x + first * stride; }
     template <int BN> __device__ __forceinline__ KeyBits<BN> keys(int) const { return KeyBits<BN>(inside); }
 };
+
+// The work of a workgroup of a packed call: block by block, all heads of a block next to each other, those of one key head
+// on as few XCDs as possible.
+template <bool KEYS> __device__ __forceinline__ Work packed_work(const SmParams& p, int wg) {
+    const int heads = KEYS ? p.G : p.H, i = wg % heads, rest = wg / heads;
+    return {KEYS ? i : i % p.G * (p.H / p.G) + i / p.G, rest % p.splits * p.blocks + rest / p.splits};
+}
 
 // f(element, padded row length) for a call's type and row length.
 template <class F> int dispatch(int dtype, int D, F f) {

@@ -103,7 +103,7 @@ def test_a_sequence_does_not_change_another(dev, lengths, causal, dtype):
 
 
 @TYPES
-@pytest.mark.parametrize("count", [63, 64, 65, 5000])
+@pytest.mark.parametrize("count", [61, 62, 63, 64, 65, 130, 253, 254, 255, 5000])
 def test_many_sequences(dev, count, dtype):
     """More than a wave, and than a wave's square, looks at together."""
     gen = torch.Generator().manual_seed(count)
