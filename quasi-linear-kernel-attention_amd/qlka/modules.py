@@ -10,7 +10,8 @@ entries, provided here with the same names and arguments:
   * KernelMultiheadAttention(embed_dim, num_heads, kernel, tau, impl) (vision_transformer.py:19-44): self-attention
     whose state_dict is nn.MultiheadAttention's (in_proj_weight, in_proj_bias, out_proj), so trained weights load. With the
     "softmax" kernel it also attends to another sequence (context), to earlier positions alone (causal) and with a learned
-    relative position bias (position_bias, a RelativePositionBias), on the kernels of qlka.softmax.
+    relative position bias (position_bias, a RelativePositionBias), on the kernels of qlka.softmax; to sequences of different
+    lengths without padding (offsets), on those of qlka.packed; and to a cache in pages (cache), on those of qlka.paged.
   * use_kernel_attention(model, kernel, tau, impl) and KernelAttention(config, kernel, tau, impl) (nomic.py:9-40):
     kernel attention inside a HF NomicBertModel with its own weights.
 
@@ -27,7 +28,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import layers, softmax
+from . import layers, packed, paged, softmax
 
 TAU = {"softmax": 64 ** 0.25, "add_laplace": 0.5, "add_riesz": 1.0, "add_bump": 1.5}   # kernels.py:13-25
 KERNELS = tuple(TAU)
@@ -88,7 +89,12 @@ class KernelMultiheadAttention(nn.Module):
         context's real positions;
       * causal=True: the query at position start + m sees the keys up to its own position. For a decoder's next tokens,
         context holds the heads of all tokens up to them and start is the position of x's first one (without a context,
-        where the keys are x's own, there is no other position than 0)."""
+        where the keys are x's own, there is no other position than 0);
+      * forward(x, offsets=offsets): x (T, E), sequences one after the other (qlka.packed), each attending to itself (causal
+        or not) -> (T, E);
+      * forward(x, cache=(pages, tables, lengths), offsets=offsets): x (T, E), the new tokens of sequences whose heads a
+        qlka.paged.PagedCache of num_heads key heads holds, one each without offsets. Their own heads are written there,
+        then each attends to its sequence up to itself. No gradient (call it under torch.no_grad())."""
 
     def __init__(self, embed_dim, num_heads, kernel="softmax", tau=None, impl="efficient", position_bias=None):
         super().__init__()
@@ -121,7 +127,26 @@ class KernelMultiheadAttention(nn.Module):
         """The heads (k, v) of context (B, N, E), each (B, H, N, E / H), as forward takes them."""
         return self._heads(context, 1, 2)
 
-    def forward(self, x, keep=None, context=None, causal=False, start=0):
+    def _rows(self, x, offsets, cache, causal):
+        """forward of rows (T, E) without padding."""
+        if self.kernel != "softmax" or self.position_bias is not None:
+            raise NotImplementedError("packed sequences and a cache in pages run on the 'softmax' kernel without a position bias")
+        if x.dim() != 2:
+            raise ValueError(f"packed rows must be (T, E), got {tuple(x.shape)}")
+        q, k, v = (heads[0] for heads in self.split_heads(x[None]))                 # (H, T, Dh)
+        if cache is None:
+            heads = packed.packed_attention(q, k, v, offsets, scale=self.tau ** -2, causal=causal)
+        else:
+            pages, tables, lengths = cache
+            pages.write(k, v, tables, lengths, offsets)
+            heads = paged.paged_attention(q, pages, tables, lengths, offsets, scale=self.tau ** -2)
+        return self.out_proj(heads.transpose(0, 1).flatten(1))
+
+    def forward(self, x, keep=None, context=None, causal=False, start=0, offsets=None, cache=None):
+        if offsets is not None or cache is not None:
+            if keep is not None or context is not None or start != 0:
+                raise ValueError("packed sequences and a cache in pages take no keep, context or start")
+            return self._rows(x, offsets, cache, causal)
         if context is None:
             if start != 0:
                 raise ValueError(f"start {start} without a context: the keys are x's own, whose first position is 0")
