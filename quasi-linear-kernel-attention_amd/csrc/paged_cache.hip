@@ -6,8 +6,8 @@
 // of what is read need no further rounding (int8 and e4m3 values have at most 7 and 4 bits, bf16 has 8). A scale of
 // largest / 127 would use up to one bit more of int8, but every reader would round.
 //
-// Both kernels are bound by memory, and at few rows by the latency of offsets, length, table and row, one after the
-// other. DP / 8 lanes take a row, 8 elements each; 4 lanes find a block's largest element. A wave writes one token's
+// Both kernels are bound by memory, and at few rows by the latency of offsets and lengths, table and store, one after
+// the other (the rows themselves are loaded meanwhile). DP / 8 lanes take a row, 8 elements each; 4 lanes find a block's largest element. A wave writes one token's
 // rows of all heads, keys and values, so that the sequence is looked up once for all of them.
 #include "paged_device.h"
 
@@ -32,17 +32,17 @@ template <class C> __device__ __forceinline__ u32x2 codes_of(f32x8 x, uint32_t e
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         if constexpr (std::is_same<C, Int8>::value) {
-            uint32_t y = 0;
+            // next to 1.5 * 2^23 a float's last place is 1: the sum is rounded as it should be, and its low byte is the code
+            uint32_t y[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float c = fminf(fmaxf(__builtin_rintf(x[4 * h + i] * s), -127.f), 127.f);
-                y |= ((uint32_t)(int)c & 255u) << 8 * i;
-            }
-            w[h] = e == 255 ? 0u : y;
+            for (int i = 0; i < 4; ++i)
+                y[i] = __float_as_uint(__builtin_amdgcn_fmed3f(x[4 * h + i] * s, -127.f, 127.f) + 12582912.f);
+            const uint32_t lo = __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0400), hi = __builtin_amdgcn_perm(y[3], y[2], 0x0c0c0400);
+            w[h] = e == 255 ? 0u : lo | hi << 16;
         } else {
             float c[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) c[i] = fminf(fmaxf(x[4 * h + i] * s, -448.f), 448.f);
+            for (int i = 0; i < 4; ++i) c[i] = __builtin_amdgcn_fmed3f(x[4 * h + i] * s, -448.f, 448.f);
             int y = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
             y = __builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], y, true);
             w[h] = e == 255 ? 0x7f7f7f7fu : (uint32_t)y;
@@ -53,54 +53,61 @@ template <class C> __device__ __forceinline__ u32x2 codes_of(f32x8 x, uint32_t e
 
 // One wave a token: its rows of all heads, keys then values, DP / 8 lanes a row.
 template <class T, class C, int DP> __global__ __launch_bounds__(256) void paged_write(const PgParams p) {
-    constexpr int LANES = DP / 8, AT_ONCE = 64 / LANES;
-    const int lane = threadIdx.x & 63, token = blockIdx.x * 4 + (threadIdx.x >> 6);
+    constexpr int LANES = DP / 8, AT_ONCE = 64 / LANES, AHEAD = 4;
+    const int lane = threadIdx.x & 63;
+    const int token = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), d = lane % LANES * 8;
     if (token >= p.T) return;
-    int b = token, seat = -1;
-    if (p.offsets) b = last_upto(p.B + 1, token, [&](int i) { return p.offsets[i]; });
-    b = __builtin_amdgcn_readfirstlane(b);
-    if (b < 0 || b >= p.B) return;
-    {
-        const int length = min(max(p.lengths[b], 0), 1 << 28);
-        const int64_t end = p.offsets ? p.offsets[b + 1] : b + 1;
-        // offsets are the caller's: whatever they are, a position without a place is none
-        const int64_t at = length - (end - token);
-        seat = at < 0 || at >= p.places ? -1 : (int)at;
-    }
-    if (seat < 0) return;
-    const Place place = place_of(p, seat);
-    const uint32_t page = p.tables[b * p.table_stride + place.index];
-    if (page >= (uint32_t)p.num_pages) return;
-    const int d = lane % LANES * 8;
-#pragma unroll 2
-    for (int i = lane / LANES; i < 2 * p.G; i += AT_ONCE) {
+    typedef typename sm::Elem<T>::seg Seg;
+    const int last = 2 * p.G - 1;
+    // Row i: keys, then values. What all lanes share of an address is found once, for both.
+    const T *k = (const T*)p.k + token * p.snk.r, *v = (const T*)p.v + token * p.snv.r;
+    const auto load = [&](int i) {
         const bool key = i < p.G;
-        const int g = key ? i : i - p.G;
-        const PgOut s = key ? p.snk : p.snv;
-        const PgStrides to = key ? p.sk : p.sv;
-        const auto x = sm::load_seg((const T*)(key ? p.k : p.v) + g * s.h + token * s.r, d, p.D);
-        char* at = (key ? p.k_pages : p.v_pages) + (uint64_t)g * to.head + bytes_to(to, page, place.row) +
-                   d * Piece<C, 8>::SIZE;
+        return sm::load_seg((key ? k : v) + (key ? i : i - p.G) * (key ? p.snk.h : p.snv.h), d, p.D);
+    };
+    // the first rows are on their way while the place is found
+    Seg ahead[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) ahead[j] = load(min(lane / LANES + j * AT_ONCE, last));
+    const Found found = find(p, token, tokens_of_lane(p));
+    if (found.b < 0) return;
+    // offsets and lengths are the caller's: whatever they are, a position without a place is none
+    const int seat = found.tokens.start + token - found.tokens.first;
+    if (seat < 0 || seat >= p.places) return;
+    const Place place = place_of(p, __builtin_amdgcn_readfirstlane(seat));
+    const uint32_t page = __builtin_amdgcn_readfirstlane(p.tables[found.b * p.table_stride + place.index]);
+    if (page >= (uint32_t)p.num_pages) return;
+    char *to_k = p.k_pages + bytes_to(p.sk, page, place.row), *to_v = p.v_pages + bytes_to(p.sv, page, place.row);
+    uint8_t *to_ke = p.k_exp + bytes_to(p.ske, page, place.row), *to_ve = p.v_exp + bytes_to(p.sve, page, place.row);
+    const auto put = [&](int i, Seg x) {
+        const bool key = i < p.G;
+        const uint32_t g = key ? i : i - p.G;
+        char* at = (key ? to_k : to_v) + (uint64_t)g * (key ? p.sk.head : p.sv.head) + d * Piece<C, 8>::SIZE;
         if constexpr (!coded<C>) {
-            if (d < p.D) *reinterpret_cast<typename sm::Elem<T>::seg*>(at) = x;
+            if (d < p.D) *reinterpret_cast<Seg*>(at) = x;
         } else {
             const f32x8 y = sm::floats(x);
             // the largest of the block's bits: NaN and infinities are above every finite number
             uint32_t most = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(y[j]) & 0x7fffffffu);
-            most = max(most, (uint32_t)__shfl_xor((int)most, 1));
-            most = max(most, (uint32_t)__shfl_xor((int)most, 2));
+            most = max(most, (uint32_t)__builtin_amdgcn_mov_dpp((int)most, 0xB1, 0xf, 0xf, true));     // quad: 1 0 3 2
+            most = max(most, (uint32_t)__builtin_amdgcn_mov_dpp((int)most, 0x4E, 0xf, 0xf, true));     // quad: 2 3 0 1
             const uint32_t e = exponent_of<C>(__uint_as_float(most));
             if (d < p.D) {
                 *reinterpret_cast<u32x2*>(at) = codes_of<C>(y, e);
-                if (d % BLOCK == 0) {
-                    const PgStrides te = key ? p.ske : p.sve;
-                    (key ? p.k_exp : p.v_exp)[(uint64_t)g * te.head + bytes_to(te, page, place.row) + d / BLOCK] = (uint8_t)e;
-                }
+                if (d % BLOCK == 0)
+                    ((key ? to_ke : to_ve) + (uint64_t)g * (key ? p.ske.head : p.sve.head))[d / BLOCK] = (uint8_t)e;
             }
         }
+    };
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+        const int i = lane / LANES + j * AT_ONCE;
+        if (i <= last) put(i, ahead[j]);
     }
+#pragma unroll 2
+    for (int i = lane / LANES + AHEAD * AT_ONCE; i <= last; i += AT_ONCE) put(i, load(i));
 }
 
 // Rows of one sequence and head, keys and values, DP / 8 lanes a row and PG_READ_ROWS rows a lane.

@@ -126,6 +126,30 @@ __device__ __forceinline__ int seen_from(const PgParams& p, int seat) {
     return p.num_pages ? min(max(seat + 1, 0), p.places) : 0;
 }
 
+// The tokens of sequence `lane`, the first 64 together.
+__device__ __forceinline__ Tokens tokens_of_lane(const PgParams& p) {
+    const int lane = threadIdx.x & 63;
+    return lane < p.B ? tokens_of(p, lane) : Tokens{0, 0, 0};
+}
+// The sequence of row t (the same for all lanes) and its tokens, from those of every lane; b < 0 outside every sequence.
+struct Found { int b; Tokens tokens; };
+__device__ __forceinline__ Found find(const PgParams& p, int t, Tokens mine) {
+    Found x{t, {}};
+    if (p.offsets) {
+        x.b = __popcll(__ballot((int)(threadIdx.x & 63) < p.B && mine.first <= t)) - 1;
+        if (x.b == 63) x.b = __builtin_amdgcn_readfirstlane(last_upto(p.B + 1, t, [&](int j) { return p.offsets[j]; }));
+        if (x.b >= p.B) x.b = -1;
+        if (x.b < 0) return x;
+    }
+    if (x.b < 64)
+        x.tokens = {__builtin_amdgcn_readlane(mine.first, x.b), __builtin_amdgcn_readlane(mine.rows, x.b),
+                    __builtin_amdgcn_readlane(mine.start, x.b)};
+    else
+        x.tokens = tokens_of(p, x.b);
+    if (t < x.tokens.first || t >= x.tokens.first + x.tokens.rows) x.b = -1;
+    return x;
+}
+
 // How the work of a launch is cut into units of about equal time: a block of ROWS rows of one key head over `span` successive
 // positions. The span goes by what the sequences of this launch (STEP: those of few rows) hold together, which only
 // the device knows, so that there are about `aim` units a key head; every workgroup finds it, and its unit, by itself,
@@ -153,11 +177,7 @@ template <bool STEP, int ROWS> struct Units {
     __device__ __forceinline__ Tokens load(int b) const { return b < p.B ? tokens_of(p, b) : Tokens{0, 0, 0}; }
     __device__ __forceinline__ Cut cut(Held h) const { return {h.blocks, max(1, (h.seen + span - 1) / span)}; }
 
-    __device__ __forceinline__ Units(const PgParams& p, const PgUnits& u) : Units(p, u, load_mine(p)) {}
-    static __device__ __forceinline__ Tokens load_mine(const PgParams& p) {
-        const int lane = threadIdx.x & 63;
-        return lane < p.B ? tokens_of(p, lane) : Tokens{0, 0, 0};
-    }
+    __device__ __forceinline__ Units(const PgParams& p, const PgUnits& u) : Units(p, u, tokens_of_lane(p)) {}
     __device__ __forceinline__ Units(const PgParams& p, const PgUnits& u, Tokens mine)
         : p(p), u(u), share(p.H / p.G), mine(mine) {
         const int lane = threadIdx.x & 63;

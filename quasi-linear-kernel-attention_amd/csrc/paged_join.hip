@@ -16,33 +16,22 @@ template <class T, int DP, bool MANY> __global__ __launch_bounds__(256) void pag
     const int t = (int)(w / turns), head0 = (int)(w % turns) * (MANY ? GROUPS : 1);
     if (t >= p.T) return;
     // the sequence, looked up together with what its units are found from
-    const Tokens mine = Units<true, PG_STEP_ROWS>::load_mine(p);
-    int b = t;
-    if (p.offsets) {
-        const uint64_t begun = __ballot(lane < p.B && mine.first <= t);
-        b = __popcll(begun) - 1;
-        if (b == 63) b = __builtin_amdgcn_readfirstlane(last_upto(p.B + 1, t, [&](int j) { return p.offsets[j]; }));
-        if (b < 0 || b >= p.B) return;
-    }
-    Tokens seq;
+    const Tokens mine = tokens_of_lane(p);
+    const Found found = find(p, t, mine);
+    if (found.b < 0) return;
+    const int b = found.b;
+    const Tokens seq = found.tokens;
     int span, before, blocks, parts;         // of the sequence: units a key head before it, its blocks and parts
-    bool step;
-    const auto find = [&](const auto& units) {
+    const bool step = seq.rows * share <= p.few;
+    const auto look_up = [&](const auto& units) {
         const Cut c = units.cut(units.held(b, seq));
         span = units.span;
         before = units.upto(b);
         blocks = c.blocks;
         parts = c.parts;
     };
-    if (b < 64)
-        seq = {__builtin_amdgcn_readlane(mine.first, b), __builtin_amdgcn_readlane(mine.rows, b),
-               __builtin_amdgcn_readlane(mine.start, b)};
-    else
-        seq = tokens_of(p, b);
-    if (t < seq.first || t >= seq.first + seq.rows) return;            // behind the last sequence
-    step = seq.rows * share <= p.few;
-    if (step) find(Units<true, PG_STEP_ROWS>(p, p.step, mine));
-    else find(Units<false, PG_TILE_ROWS>(p, p.tiles, mine));
+    if (step) look_up(Units<true, PG_STEP_ROWS>(p, p.step, mine));
+    else look_up(Units<false, PG_TILE_ROWS>(p, p.tiles, mine));
     if (parts == 1) return;
     const int size = step ? PG_STEP_ROWS : PG_TILE_ROWS;
     const PgUnits& u = step ? p.step : p.tiles;
