@@ -119,7 +119,7 @@ int params(const qlka_paged_args* a, PgParams* p) {
         bool aligned = (uintptr_t)o.x % unit == 0;
         for (int i = 0; i < 3; ++i) {
             if (sizes[i] <= 1) continue;
-            if (o.s[i] < 0 || o.s[i] * held_size(a) > UINT32_MAX)
+            if (o.s[i] < 0 || o.s[i] > UINT32_MAX / held_size(a))
                 return refuse("the strides of %s must be in [0, 2^32) bytes", o.name);
             aligned = aligned && o.s[i] * held_size(a) % unit == 0;
         }

@@ -29,9 +29,10 @@ namespace sm {
 constexpr float GROW = 4.f;          // 2^8 of the exponentials
 
 // Three parts of P leave room for three waves a SIMD (of 64 elements) only if the compiler is held to it: 476 us for 524 at
-// 12 x 8192 x 8192.
+// 12 x 8192 x 8192. So do packed sequences for four (16 of 100 to 8192, 12 / 4 heads: 571 us for 597).
 template <class T, int DP, int NW, bool BIAS, bool FINE, bool PACKED>
-__global__ __launch_bounds__(64 * NW, (FINE && DP <= 64 ? 3 : Shape<T, DP>::WAVES))
+__global__ __launch_bounds__(64 * NW, (FINE && DP <= 64 ? 3 : PACKED && sizeof(T) == 2 && DP == 64 && NW > 1 ? 4
+                                                                                                          : Shape<T, DP>::WAVES))
 void softmax_fwd(const SmParams p) {
     constexpr int NP = Elem<T>::PARTS, BN = Shape<T, DP>::BN, NT = 64 * NW, ROWS = 32 * NW, NS = BN / 32, ND = DP / 32;
     typedef Pair<T, DP, BN, NW> PairT;

@@ -262,6 +262,71 @@ def test_long_sequences_are_split(dev, new, dtype, held):
 
 
 @KINDS
+@pytest.mark.parametrize("case", ["65_tokens", "130_few", "200_mixed", "129_empty"])
+def test_many_sequences(dev, case, dtype, held):
+    """More than a wave's lanes look up at once."""
+    gen = torch.Generator().manual_seed(13)
+    B = int(case.split("_")[0])
+    draw = lambda lo, hi: torch.randint(lo, hi + 1, (B,), generator=gen).tolist()  # noqa: E731
+    new = [1] * B if "tokens" in case else draw(0, 3) if "few" in case else [0] * B
+    if "mixed" in case:
+        new = [[1, 0, 1, 1, 2][b % 5] for b in range(B)]
+        new[3], new[70], new[199] = 60, 45, 90
+    if "empty" in case:
+        new[64], new[128] = 1, 40
+    lengths = [n + m for n, m in zip(new, draw(0, 40))]
+    lengths[B - 1], lengths[B // 2] = 1200, 900             # some in parts
+    offsets = sums(new, 2)
+    tables, num_pages = tables_of(lengths, 16, gen)
+    cache, cpu = filled(num_pages, 16, 1, 64, dtype, held, gen, dev)
+    q = torch.randn(2, offsets[-1] + 3, 64, generator=gen).to(dtype)
+    want, bound = oracle.attention(q, *cpu, held, tables, lengths, offsets, 0.125)
+    close(attend(dev, q, cache, tables, lengths, offsets), want, bound)
+    k, v = (torch.randn(1, offsets[-1] + 3, 64, generator=gen).to(dtype) for _ in "kv")
+    cache.write(k.to(dev), v.to(dev), tables.to(dev), i32(lengths, dev), i32(offsets, dev))
+    written(cpu, k, v, held, tables, lengths, offsets)
+    for got, want in zip(cache, cpu):
+        assert want is None or torch.equal(as_bytes(got).cpu(), want)
+
+
+@pytest.mark.parametrize("dtype,held", [(F32, F32), (BF16, BF16), (BF16, I8)], ids=["fp32", "bf16", "bf16_int8"])
+@pytest.mark.parametrize("new,length,heads", [([1], 20000, (2, 1, 32)), ([3, 1], 18000, (2, 2, 128)), ([400], 10000, (12, 4, 64)),
+                                              ([700], 5000, (7, 7, 32)), ([600, 1], 4000, (8, 1, 128))], ids=str)
+def test_parts_beyond_what_is_joined_at_once(dev, new, length, heads, dtype, held):
+    """Rows whose parts are more than the lanes that look at them, many rows and few."""
+    H, G, D = heads
+    gen = torch.Generator().manual_seed(length)
+    lengths, offsets = [length] * len(new), sums(new)
+    tables, num_pages = tables_of(lengths, 64, gen)
+    cache, cpu = filled(num_pages, 64, G, D, dtype, held, gen, dev)
+    q = torch.randn(H, offsets[-1], D, generator=gen).to(dtype)
+    want, bound = oracle.attention(q, *cpu, held, tables, lengths, offsets, D ** -0.5)
+    close(attend(dev, q, cache, tables, lengths, offsets), want, bound)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("held", [I8, E4], ids=["int8", "e4m3"])
+@pytest.mark.parametrize("new", [[1, 1], [40, 50]], ids=str)
+def test_blocks_that_were_not_finite(dev, new, held, dtype):
+    """A block marked as such is NaN: in the keys it makes the rows that see it NaN, in the values its 32 elements of them."""
+    gen = torch.Generator().manual_seed(14)
+    lengths = [60, 70]
+    tables, num_pages = tables_of(lengths, 16, gen)
+    cache, _ = filled(num_pages, 16, 1, 64, dtype, held, gen, dev)
+    q = torch.randn(2, sum(new), 64, generator=gen).to(dtype)
+    clean = attend(dev, q, cache, tables, lengths, sums(new))
+    cache.v_exp[int(tables[0, 0]), 0, 3, 1] = 255           # sequence 0, position 3
+    as_bytes(cache.v)[int(tables[0, 0]), 0, 3] = 0          # (whatever its codes are)
+    got = attend(dev, q, cache, tables, lengths, sums(new))
+    assert got[:, :new[0], 32:].isnan().all() and got[:, :new[0], :32].isfinite().all() and got[:, new[0]:].isfinite().all()
+    cache.v_exp[int(tables[0, 0]), 0, 3, 1] = 127
+    cache.k_exp[int(tables[1, 0]), 0, 5, 0] = 255           # sequence 1, position 5
+    got = attend(dev, q, cache, tables, lengths, sums(new))
+    assert got[:, new[0]:].isnan().all() and not got[:, :new[0]].isnan().any()
+    assert clean.isfinite().all()
+
+
+@KINDS
 @pytest.mark.parametrize("new", [[1, 1], [100, 90]], ids=str)
 @pytest.mark.parametrize("scale", [0.0, -0.2, 1e5])
 def test_scales(dev, scale, new, dtype, held):

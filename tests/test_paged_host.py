@@ -119,6 +119,7 @@ WRONG = [
     (dict(D=40, v_pages_stride=(2048, 1024, 36)), "rows of v_pages must be aligned to 8"),
     (dict(k_pages_stride=(-2048, 1024, 64)), "strides of k_pages must be in"),
     (dict(v_pages_stride=(1 << 33, 1024, 64)), "strides of v_pages must be in"), (dict(k_exp_stride=(1 << 32, 32, 2)), "strides of k_exp"),
+    (dict(v_pages_stride=(1 << 62, 1024, 64)), "strides of v_pages must be in"),
     (dict(k_exp=None), "k_exp and v_exp must be non-null"), (dict(v_exp_stride=(64, -1, 2)), "strides of k_exp and v_exp must be in"),
     (dict(lengths=None), "tables and lengths must be"), (dict(tables=None), "tables and lengths must be"),
     (dict(table_stride=-4), "table_stride must not"),
