@@ -28,17 +28,21 @@ int64_t average(const qlka_packed_args* a) { return ceil_div(a->T, std::max(a->B
 int64_t longest(const qlka_packed_args* a) { return std::min<int64_t>(2 * average(a), a->T); }
 
 struct Plan { int waves, blocks, splits; };
-Plan plan(const qlka_packed_args* a, int heads, int64_t tiles, double products, int waves) {
+// Workgroups of `few` waves where sequences have no rows for more, unless they are less than two a compute unit: then waves
+// without rows help to bring the others' (fp32 training, 12 heads of 64 of 8 to 30 rows: 16 sequences 27 us with all
+// waves, 30 with few; 64: 52 and 46; 1000: 641 and 475).
+Plan plan(const qlka_packed_args* a, int heads, int64_t tiles, double products, int few) {
     Plan r;
-    r.waves = waves;
-    r.blocks = (int)segment_blocks(a->T, a->B, 1, 32 * waves);
+    const bool small = average(a) <= 32 * few && heads * segment_blocks(a->T, a->B, 1, 32 * FWD_WAVES) > 512;
+    r.waves = small ? few : FWD_WAVES;
+    r.blocks = (int)segment_blocks(a->T, a->B, 1, 32 * r.waves);
     const int DP = sm_padded(a->D);
     const double tile_us = products * 0.3 * DP / 64 * (a->dtype == QLKA_F32 ? 2 : 1);
     r.splits = splits_for((int64_t)heads * r.blocks, tiles, tile_us, (double)heads * a->T * DP * 8);
     return r;
 }
 Plan fwd_plan(const qlka_packed_args* a) {
-    return plan(a, a->H, ceil_div(longest(a), tile_rows(a)), 2, average(a) <= 32 ? 1 : FWD_WAVES);
+    return plan(a, a->H, ceil_div(longest(a), tile_rows(a)), 2, 1);
 }
 size_t part_bytes(const qlka_packed_args* a, const Plan& p, int heads) {
     return p.splits > 1 ? align256((size_t)p.splits * heads * a->T * sm_padded(a->D) * 4) : 0;
@@ -55,11 +59,11 @@ struct BwdPlan {
 int groups(const qlka_packed_args* a) { return (int)segment_blocks(a->T, a->B, 1, 32); }
 BwdPlan bwd_plan(const qlka_packed_args* a) {
     BwdPlan w{};
-    const int t = tile_rows(a), waves = average(a) <= 64 ? 2 : 4;
+    const int t = tile_rows(a);
     w.delta = align256((size_t)a->H * a->T * 4);
     w.large = align256((size_t)a->H * groups(a) * 4);
-    w.dq = plan(a, a->H, ceil_div(longest(a), t), 3, waves);
-    w.dkv = plan(a, a->G, ceil_div(longest(a), t) * (a->H / a->G), 5, waves);
+    w.dq = plan(a, a->H, ceil_div(longest(a), t), 3, 2);
+    w.dkv = plan(a, a->G, ceil_div(longest(a), t) * (a->H / a->G), 5, 2);
     w.part2 = part_bytes(a, w.dkv, a->G);
     w.part = std::max(part_bytes(a, w.dq, a->H), w.part2);
     return w;

@@ -103,6 +103,18 @@ def test_a_sequence_does_not_change_another(dev, lengths, causal, dtype):
 
 
 @TYPES
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "whole"])
+@pytest.mark.parametrize("longest", [30, 60])
+@pytest.mark.parametrize("D", [32, 40, 64, 128])
+def test_many_short_sequences(dev, D, longest, causal, dtype):
+    """Enough of them for workgroups of one wave and of two."""
+    gen = torch.Generator().manual_seed(longest + D)
+    at = offsets_of([longest, 0] + torch.randint(1, longest + 1, (68,), generator=gen).tolist(), 1)
+    t = make(8, 4, at[-1] + 2, D, dtype, seed=D)
+    check(run(dev, t, at, causal=causal), reference(t, at, causal))
+
+
+@TYPES
 @pytest.mark.parametrize("count", [61, 62, 63, 64, 65, 130, 253, 254, 255, 5000])
 def test_many_sequences(dev, count, dtype):
     """More than a wave, and than a wave's square, looks at together."""
