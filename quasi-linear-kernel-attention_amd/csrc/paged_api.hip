@@ -30,10 +30,23 @@ int check_sizes(const qlka_paged_args* a) {
 
 // ---- how a call runs
 
-// Sequences of up to FEW rows a key head go through the step kernel, 16 rows at a time, others through the tiles.
-constexpr int FEW = 32;
-// Workgroups of a launch that fill the GPU, and the least positions that one takes.
-constexpr int64_t STEP_LEAST = 256, TILE_GROUPS = 768, TILE_LEAST = 512;
+// Sequences of up to so many rows a key head go through the step kernel, 16 at a time, others through the tiles. bf16 rows
+// come as fast to a tile (32 sequences of up to 16384 with 4 to 8 tokens, 12 / 4 heads: 45 us with 16, 57 with 32; 8 to 16
+// tokens: 59 and 55), others have to be taken apart or turned into bf16 (fp32, 4 sequences of up to 8000, 6 to 12 tokens:
+// 24 us with 32, 39 with 16; e4m3, 12 / 12 heads, 12 to 24 tokens: 120 and 128).
+int few_rows(const qlka_paged_args* a) { return a->held == QLKA_BF16 ? 16 : 32; }
+// Workgroups of a launch that fill the GPU, and the least positions that one takes. Tiles alone: three a compute unit (4
+// chunks of 512 at up to 8192, int8, 12 / 4 heads: 68 us; 71 with two, 80 with six), beside tokens two, so that those
+// have a third (32 sequences, two with chunks of 700: 46 us for 50). Tokens over bf16 rows: 1536 (16 sequences of up to 8192, 12
+// heads: 52 us; 56 with 768), over 8 bits 768 (32 of up to 16384, 12 / 4: 33.2 us; 33.8 with 1024, 37.4 with 1536),
+// beside tiles 1024 (64 of up to 8192, 8 with chunks of 512: 164 us; 181 with 768).
+constexpr int64_t TILE_GROUPS = 768, TILE_GROUPS_MIXED = 512;
+constexpr int64_t STEP_GROUPS = 1536, STEP_GROUPS_CODED = 768, STEP_GROUPS_CODED_MIXED = 1024;
+// The least positions of a part: a turn of the step kernel's waves (one sequence of 2000, int8, 12 / 4 heads: 9.3 us; 10.6 with
+// 256, 17.4 as one), a few tiles of the others (300 tokens of it: 20.1 us; 24.4 with 128, 23.2 with 512). A call whose
+// tables have no room for more than so many positions is not cut at all, which saves joining (one sequence of 250: 7.0 us
+// for 9.3; of 500: 9.2 either way).
+constexpr int64_t STEP_LEAST = 128, TILE_LEAST = 256, STEP_WHOLE = 512, TILE_WHOLE = 256;
 
 struct Plan {
     bool step, tiles, join;
@@ -46,9 +59,10 @@ Plan plan(const qlka_paged_args* a) {
     Plan r{};
     const int64_t share = a->H / a->G, sequences = std::max(a->B, 1);
     const int64_t longest = !a->offsets ? 1 : a->longest ? std::min(a->longest, a->T) : a->T;
+    const int few = few_rows(a);
     r.step = r.tiles = true;
-    r.few = FEW;
-    if (!a->offsets || longest * share <= FEW) {
+    r.few = few;
+    if (!a->offsets || longest * share <= few) {
         r.tiles = false;
         r.few = INT32_MAX;
     } else if (a->T * share >= 256 * sequences) {       // chunks, on the average: a token among them takes a tile too
@@ -57,23 +71,25 @@ Plan plan(const qlka_paged_args* a) {
     }
     const int64_t places = std::min<int64_t>((int64_t)a->table_len * a->page_size, LONGEST);
     const int DP = sm_padded(a->D);
-    const struct { bool used; int rows; int64_t groups, least; } kernels[2] = {
-        {r.step, PG_STEP_ROWS, coded(a) ? 768 : 1536, STEP_LEAST}, {r.tiles, PG_TILE_ROWS, TILE_GROUPS, TILE_LEAST}};
+    const struct { bool used; int rows; int64_t groups, least, whole; } kernels[2] = {
+        {r.step, PG_STEP_ROWS, !coded(a) ? STEP_GROUPS : r.tiles ? STEP_GROUPS_CODED_MIXED : STEP_GROUPS_CODED, STEP_LEAST,
+         STEP_WHOLE},
+        {r.tiles, PG_TILE_ROWS, r.step ? TILE_GROUPS_MIXED : TILE_GROUPS, TILE_LEAST, TILE_WHOLE}};
     for (int i = 0; i < 2; ++i) {
         const auto& k = kernels[i];
         if (!k.used) continue;
         // blocks of rows a key head: each sequence has one that is not full at most, and more in the step kernel only
         // where it is alone
         int64_t blocks = a->T * share / k.rows + a->B;
-        if (i == 0 && r.tiles) blocks = std::min<int64_t>(blocks, (int64_t)a->B * (FEW / PG_STEP_ROWS));
+        if (i == 0 && r.tiles) blocks = std::min<int64_t>(blocks, (int64_t)a->B * (few / PG_STEP_ROWS));
         // a sequence's last part is shorter than the others: room for those within the round of workgroups
         const int64_t last = a->G * (i == 0 ? sequences : a->T * share / k.rows + sequences) / 2;
         const int64_t aim = std::max<int64_t>(std::max(k.groups - last, k.groups / 2) / a->G, 1);
-        const bool parts = places > k.least;
+        const bool parts = places > k.whole;
         const int64_t units = (blocks + (parts ? aim + 1 : 0)) * a->G;          // the sum of parts rounded up
         PgUnits& u = r.units[i];
         u.aim = (float)aim;
-        u.least = (int)k.least;
+        u.least = parts ? (int)k.least : (int)LONGEST;
         u.room = units;
         u.groups = (int)std::min<int64_t>(ceil_div(units, 8) * 8, INT32_MAX);
         if (parts) {

@@ -9,7 +9,7 @@ namespace pg {
 // lanes take a part's sums.
 template <class T, int DP, bool MANY> __global__ __launch_bounds__(256) void paged_join(const PgParams p) {
     constexpr int LANES = DP / 4, GROUPS = 64 / LANES;                 // lanes of a part's row
-    constexpr int LOOK = MANY ? LANES : 64, AT_ONCE = MANY ? 1 : GROUPS, EARLY = 8;
+    constexpr int LOOK = MANY ? LANES : 64, AT_ONCE = MANY ? 1 : GROUPS;
     const int lane = threadIdx.x & 63, share = p.H / p.G, i = lane % LANES, group = lane / LANES;
     const uint32_t w = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
     const uint32_t turns = MANY ? (p.H + GROUPS - 1) / GROUPS : p.H;
@@ -46,12 +46,12 @@ template <class T, int DP, bool MANY> __global__ __launch_bounds__(256) void pag
     const int64_t row = unit * size + r % size;
     float ref = LOW, sum = 0.f;
     f32x4 x = {};
-#pragma unroll 1
-    for (int s0 = 0; s0 < parts; s0 += LOOK) {
+    // parts s0 to s0 + LOOK - 1, of which the first `early` of a group of lanes are on their way before their weights are known
+    const auto add = [&](int s0, auto early) {
+        constexpr int EARLY = decltype(early)::value;
         const int look = s0 + (MANY ? i : lane), count = min(LOOK, parts - s0), first = MANY ? 0 : group;
         float2 a = {LOW, 0.f};
         if (look < parts) a = *reinterpret_cast<const float2*>(u.part2 + 2 * (look * apart + row));
-        // the first parts' sums are on their way before their weights are known
         f32x4 y[EARLY];
         const auto from = [&](int s) {
             return *reinterpret_cast<const f32x4*>(u.part + ((s0 + min(s, count - 1)) * apart + row) * DP + 4 * i);
@@ -74,8 +74,14 @@ template <class T, int DP, bool MANY> __global__ __launch_bounds__(256) void pag
             const float z = weight(s);
             if (s < count) x = x + y[e] * z;
         }
-#pragma unroll 4
         for (int s = first + EARLY * AT_ONCE; s < count; s += AT_ONCE) x = x + from(s) * weight(s);
+    };
+#pragma unroll 1
+    for (int s0 = 0; s0 < parts; s0 += LOOK) {
+        const int count = min(LOOK, parts - s0);
+        if (count <= 4 * AT_ONCE) add(s0, std::integral_constant<int, 4>());
+        else if (count <= 8 * AT_ONCE) add(s0, std::integral_constant<int, 8>());
+        else add(s0, std::integral_constant<int, 16 * AT_ONCE <= LOOK ? 16 : LOOK / AT_ONCE>());
     }
 #pragma unroll
     for (int far = 1; far < LOOK; far *= 2) sum += __shfl_xor(sum, far);
