@@ -25,7 +25,7 @@ template <class T, int DP, bool MANY> __global__ __launch_bounds__(256) void pag
     const bool step = seq.rows * share <= p.few;
     const auto look_up = [&](const auto& units) {
         const Cut c = units.cut(units.held(b, seq));
-        span = units.span;
+        span = c.span;
         before = units.upto(b);
         blocks = c.blocks;
         parts = c.parts;

@@ -97,7 +97,7 @@ template <class C, int DP, int BN> struct Bring {
                     *reinterpret_cast<bf16x8*>(&lds.v[buffer].x[(row + i * APART) * DP + slot * 8]) = bf16x8{};
                 }
             } else {
-                // what is not there is read from a place that is, and dropped in arrive(): no load waits for a test
+                // what is not there is read from a place that is, and dropped in put(): no load waits for a test
                 const uint32_t from = there ? page[i] : 0, e = d < p.D ? d : 0;
                 k[i] = *reinterpret_cast<const Raw*>(heads.k + bytes_to(p.sk, from, at[i]) + e * P::SIZE);
                 v[i] = *reinterpret_cast<const Raw*>(heads.v + bytes_to(p.sv, from, at[i]) + e * P::SIZE);
@@ -108,34 +108,30 @@ template <class C, int DP, int BN> struct Bring {
             }
         }
     }
-    // the rows that were fetched are in LDS from here on, and nobody reads the buffer that the next fetch goes to; mask:
-    // where not null, 0 or -inf for each of the tile's rows
-    __device__ __forceinline__ void arrive(Lds& lds, int buffer, int D, float* mask) {
-        if constexpr (BUFFERS == 1) __syncthreads();
-        if constexpr (DIRECT) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        } else {
+    // the rows that were fetched into registers to LDS
+    __device__ __forceinline__ void put(Lds& lds, int buffer, int D) {
 #pragma unroll
-            for (int i = 0; i < EACH; ++i) {
-                if (!(ok >> i & 1) || slot * 8 >= D) {
-                    k[i] = v[i] = Raw{};
-                    ke[i] = ve[i] = 127;
-                }
-                const sm::Frag<NP> x = parts_of(k[i], 0, coded<C> ? power_of(ke[i]) : 1.f, C());
-                const sm::Frag<NP> y = parts_of(v[i], 0, coded<C> ? power_of(ve[i]) : 1.f, C());
-                const int at = TileT::at(row + i * APART, slot);
+        for (int i = 0; i < EACH; ++i) {
+            if (!(ok >> i & 1) || slot * 8 >= D) {
+                k[i] = v[i] = Raw{};
+                ke[i] = ve[i] = 127;
+            }
+            const sm::Frag<NP> x = parts_of(k[i], 0, coded<C> ? power_of(ke[i]) : 1.f, C());
+            const sm::Frag<NP> y = parts_of(v[i], 0, coded<C> ? power_of(ve[i]) : 1.f, C());
+            const int at = TileT::at(row + i * APART, slot);
 #pragma unroll
-                for (int n = 0; n < NP; ++n) {
-                    *reinterpret_cast<bf16x8*>(&lds.k[buffer].x[n * TileT::PLANE + at]) = x.p[n];
-                    *reinterpret_cast<bf16x8*>(&lds.v[buffer].x[n * TileT::PLANE + at]) = y.p[n];
-                }
+            for (int n = 0; n < NP; ++n) {
+                *reinterpret_cast<bf16x8*>(&lds.k[buffer].x[n * TileT::PLANE + at]) = x.p[n];
+                *reinterpret_cast<bf16x8*>(&lds.v[buffer].x[n * TileT::PLANE + at]) = y.p[n];
             }
         }
-        if (mask && slot == 0) {
+    }
+    // 0 or -inf for each of the tile's rows
+    __device__ __forceinline__ void put_mask(float* mask) {
+        if (slot == 0) {
 #pragma unroll
             for (int i = 0; i < EACH; ++i) mask[row + i * APART] = ok >> i & 1 ? 0.f : LOW;
         }
-        __syncthreads();
     }
 };
 
@@ -145,6 +141,7 @@ template <class T, class C, int DP> __device__ __forceinline__ void tiles(const 
     constexpr int NQ = sm::Elem<T>::PARTS, NK = Piece<C, 8>::PARTS, BN = sm_tile_rows(NK, DP), NS = BN / 32, ND = DP / 32;
     constexpr int ROWS = PG_TILE_ROWS, NT = 64 * TILE_WAVES;
     typedef Bring<C, DP, BN> BringT;
+    static_assert(Units<false, ROWS>::ALIGN % BN == 0);
     __shared__ __attribute__((aligned(16))) typename BringT::Lds lds;
     __shared__ __attribute__((aligned(16))) float mask_of[BringT::BUFFERS][BN];
 
@@ -177,11 +174,17 @@ template <class T, class C, int DP> __device__ __forceinline__ void tiles(const 
     }
     lacks = __syncthreads_or(lacks);
     BringT tile(lds, p, tid);
-    int buffer = 0;
+    constexpr bool DIRECT = BringT::DIRECT;
+    int buffer = 0, next = t;                          // next: the tile to be fetched
+    const auto fetch = [&](int to) {
+        tile.fetch(lds, to, p, heads, tid);
+        if (DIRECT && lacks) tile.put_mask(mask_of[to]);
+        ++next;
+        tile.look(p, table, min(next, t1 - 1), seen);
+    };
     if (t < t1) {
         tile.look(p, table, t, seen);
-        tile.fetch(lds, 0, p, heads, tid);
-        tile.look(p, table, min(t + 1, t1 - 1), seen);
+        fetch(0);
     }
 
     sm::Frag<NQ> qf[DP / 16];
@@ -200,15 +203,21 @@ template <class T, class C, int DP> __device__ __forceinline__ void tiles(const 
 
     for (; t < t1; ++t) {
         const int n0 = t * BN;
-        float* mask = mask_of[buffer];
-        tile.arrive(lds, buffer, p.D, lacks ? mask : nullptr);
+        if constexpr (BringT::BUFFERS == 1) __syncthreads();             // nobody reads it any more
+        if constexpr (DIRECT) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        } else {
+            tile.put(lds, buffer, p.D);
+            if (lacks) tile.put_mask(mask_of[buffer]);
+        }
+        __syncthreads();
+        const float* mask = mask_of[buffer];
         const auto& kt = lds.k[buffer];
         const auto& vt = lds.v[buffer];
         buffer ^= BringT::BUFFERS - 1;
         // (into registers the last tile is fetched once more: what is fetched behind a test is waited for where the
         // paths meet)
-        if (!BringT::DIRECT || t + 1 < t1) tile.fetch(lds, buffer, p, heads, tid);
-        tile.look(p, table, min(t + 2, t1 - 1), seen);
+        if (!DIRECT || t + 1 < t1) fetch(buffer);
         if (rw >= rows || n0 > wave_last) continue;
 
         sm::f32x16 s[NS];
