@@ -362,8 +362,9 @@ int qlka_packed_bwd(const qlka_packed_args* args, void* ws, size_t ws_bytes, voi
  *   longest: the most new tokens of a sequence if the caller knows it, else 0. It only decides which kernels run.
  *
  * Strides are in elements between heads and rows ((B, heads, rows) for out_k and out_v); D a multiple of 8 up to 128, rows
- * at multiples of 16 bytes (in pages of 8 bits with D no multiple of 16: of 8 bytes). The scale is as for qlka_softmax_fwd, the probabilities are rounded
- * to bf16 for their product where q is.
+ * at multiples of 16 bytes (in pages of 8 bits with D no multiple of 16: of 8 bytes). The scale is as for
+ * qlka_softmax_fwd, the probabilities are rounded to bf16 for their product where q is. Infinities and NaN that a sequence
+ * holds at its new tokens' positions or before can make any of its new rows NaN, no other sequence's.
  */
 #define QLKA_INT8 2
 #define QLKA_E4M3 3

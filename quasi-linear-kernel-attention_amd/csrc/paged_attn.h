@@ -1,8 +1,7 @@
-// Attention of new tokens over a cache in pages: the kernels. A launch has workgroups for sequences of few rows (paged_step.h),
-// for chunks (paged_tiles.h), or for both: a batch of chunks and tokens is one launch, in which the one kind fills the
-// compute units that the other leaves (32 sequences of 12 / 4 heads, two with chunks: 66 us one after the other,
-// 54 in one launch). The
-// last workgroups write the rows outside every sequence.
+// Attention of new tokens over a cache in pages: the kernels. A launch has workgroups for sequences of few rows
+// (paged_step.h), for chunks (paged_tiles.h), or for both: a batch of chunks and tokens is one launch, in which the one
+// kind fills the compute units that the other leaves (32 sequences of 12 / 4 heads, two with chunks: 66 us one after the
+// other, 54 in one launch). The last workgroups write the rows outside every sequence.
 #pragma once
 
 #include "paged_step.h"

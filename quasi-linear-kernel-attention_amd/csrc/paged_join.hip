@@ -6,7 +6,8 @@ namespace pg {
 
 // Adds up the parts of rows whose positions are more than one. A wave takes a row (MANY: 256 / DP rows of a token, since
 // finding the sequence costs as much as a row): its lanes look at the parts' references and sums, one each, then DP / 4
-// lanes take a part's sums.
+// lanes take a part's sums. Bound by latency: launch, sequence, sums (192 rows: 4.5 us; 19548 rows of 2 to 7 parts:
+// 7.8 us, 20 with a wave a row; of 9 parts 10.2 us, 13.3 where 8 were waited for before the ninth was asked for).
 template <class T, int DP, bool MANY> __global__ __launch_bounds__(256) void paged_join(const PgParams p) {
     constexpr int LANES = DP / 4, GROUPS = 64 / LANES;                 // lanes of a part's row
     constexpr int LOOK = MANY ? LANES : 64, AT_ONCE = MANY ? 1 : GROUPS;

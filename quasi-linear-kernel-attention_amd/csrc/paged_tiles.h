@@ -6,6 +6,10 @@
 // that it brings, one tile ahead of them. bf16 rows go to LDS directly, into the other of two buffers; rows of 8 bits
 // stay in registers until the tile before is done with and become bf16 on their way into the other buffer (exactly, see
 // paged_cache.hip); float rows are split into three parts there, with one buffer.
+//
+// Bound by vector instructions: 4 chunks of 512 new tokens at 1024 to 8192, 12 / 4 heads, int8: 64 us, 378 TFLOP/s (the scores'
+// work; taking 8 bits apart and bringing them 20 us; with bf16 pages 56 us). Two or three waves a SIMD are as fast, with
+// four registers spill (120 us).
 #pragma once
 
 #include "paged_device.h"

@@ -15,8 +15,8 @@ def packed_attention(q, k, v, offsets, scale=None, causal=True):
     rows before the first and behind the last one get zeros and have no gradient. causal: a row sees the keys of its
     sequence up to itself, else all of them. float32 or bfloat16, D up to 128, any strides (rows that do not start at
     multiples of 16 bytes are copied). scale: D ** -0.5 by default; 0 or of a size in [2^-96, 2^96]. What one sequence
-    holds, infinities and NaN too, changes no other one's results. Differentiable once, backward, in q, k and v; results
-    and gradients do not change from run to run. The offsets are read on the device: nothing waits for them, and a captured
+    holds, infinities and NaN too, changes no other one's results (it can make any row of its own NaN, earlier ones too).
+    Differentiable once, backward, in q, k and v; results and gradients do not change from run to run. The offsets are read on the device: nothing waits for them, and a captured
     call may be replayed with others (a backward pass too, with those of its forward)."""
     if q.dim() == 3 and scale is None:
         scale = max(q.shape[2], 1) ** -0.5

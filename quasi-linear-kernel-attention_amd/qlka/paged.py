@@ -79,9 +79,10 @@ def paged_attention(q, cache, tables, lengths, offsets=None, longest=0, scale=No
     cache's key heads.
 
     The tokens' own keys and values have been written before (PagedCache.write with the same tables, lengths and offsets);
-    each sees the keys up to its own position. Rows that see none, and rows outside every sequence, give zeros. float32 or
-    bfloat16 q; the pages hold that type or 8 bits. longest: the most new tokens of a sequence where the caller knows it: it
-    decides which kernels run, and changes no result by more than its rounding. scale: D ** -0.5 by default; 0 or of a size
+    each sees the keys up to its own position. Rows that see none, and rows outside every sequence, give zeros. Infinities
+    and NaN that a sequence holds can make any of its new rows NaN, no other sequence's. float32 or bfloat16 q; the pages
+    hold that type or 8 bits. longest: the most new tokens of a sequence where the caller knows it: it decides which kernels
+    run, and changes no result by more than its rounding. scale: D ** -0.5 by default; 0 or of a size
     in [2^-96, 2^96]. No gradient (a captured graph, several streams and repeated calls give the same results)."""
     if q.dim() == 3 and scale is None:
         scale = max(q.shape[2], 1) ** -0.5
