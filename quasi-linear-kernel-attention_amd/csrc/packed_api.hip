@@ -28,12 +28,14 @@ int64_t average(const qlka_packed_args* a) { return ceil_div(a->T, std::max(a->B
 int64_t longest(const qlka_packed_args* a) { return std::min<int64_t>(2 * average(a), a->T); }
 
 struct Plan { int waves, blocks, splits; };
-// Workgroups of `few` waves where sequences have no rows for more, unless they are less than two a compute unit: then waves
-// without rows help to bring the others' (fp32 training, 12 heads of 64 of 8 to 30 rows: 16 sequences 27 us with all
-// waves, 30 with few; 64: 52 and 46; 1000: 641 and 475).
+// Workgroups of `few` waves where sequences have no rows for more, unless they are less than the GPU has room for at once (two
+// a compute unit, one of fp32 rows of 128): then waves without rows help to bring the others' (fp32 training, 12 heads of
+// 64 of 8 to 30 rows: 16 sequences 27 us with all waves, 30 with few; 64: 52 and 46; 1000: 641 and 475; 12 heads of 80 of 30
+// to 60 rows: 16 sequences 58 and 65, 25 111 and 88).
 Plan plan(const qlka_packed_args* a, int heads, int64_t tiles, double products, int few) {
     Plan r;
-    const bool small = average(a) <= 32 * few && heads * segment_blocks(a->T, a->B, 1, 32 * FWD_WAVES) > 512;
+    const int64_t room = a->dtype == QLKA_F32 && sm_padded(a->D) == 128 ? 256 : 512;
+    const bool small = average(a) <= 32 * few && (int64_t)heads * a->B > room;
     r.waves = small ? few : FWD_WAVES;
     r.blocks = (int)segment_blocks(a->T, a->B, 1, 32 * r.waves);
     const int DP = sm_padded(a->D);

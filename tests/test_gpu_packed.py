@@ -115,6 +115,15 @@ def test_many_short_sequences(dev, D, longest, causal, dtype):
 
 
 @TYPES
+@pytest.mark.parametrize("D", [32, 48, 64, 128])
+def test_many_short_sequences_of_whole_heads(dev, D, dtype):
+    gen = torch.Generator().manual_seed(D)
+    at = offsets_of([60, 0] + torch.randint(20, 61, (68,), generator=gen).tolist())
+    t = make(8, 8, at[-1], D, dtype, seed=D + 1)
+    check(run(dev, t, at, causal=True), reference(t, at, True))
+
+
+@TYPES
 @pytest.mark.parametrize("count", [61, 62, 63, 64, 65, 130, 253, 254, 255, 5000])
 def test_many_sequences(dev, count, dtype):
     """More than a wave, and than a wave's square, looks at together."""
