@@ -20,6 +20,7 @@ struct PgUnits {
     int least, groups;
     int64_t room;                            // units that the workspace has places for
     float *part, *part2;
+    int* table;                              // of many sequences (paged_join.hip, paged_table), else null
 };
 
 struct PgParams {
@@ -45,6 +46,7 @@ struct PgParams {
 constexpr int BLOCK = 32;                    // elements of a row that share an exponent
 constexpr int LEAST_EXP = 27;
 constexpr int PG_ALIGN = 128;                // positions of a part: a multiple
+constexpr int PG_LOOKED_UP = 320;            // sequences that every workgroup looks up by itself: 64, then the others
 constexpr int PG_STEP_ROWS = 16;             // rows (of the heads that share a key head) of the step kernel's blocks
 constexpr int PG_READ_ROWS = 2;               // rows of a lane that reads the cache back
 constexpr int PG_TILE_ROWS = 128;            // of the tiles' workgroups
@@ -54,6 +56,7 @@ int pg_write(int dtype, int held, const PgParams& p, hipStream_t st);
 int pg_read(int dtype, int held, const PgParams& p, hipStream_t st);
 int pg_attend_bf16(int held, const PgParams& p, hipStream_t st);
 int pg_attend_f32(int held, const PgParams& p, hipStream_t st);
+int pg_table(const PgParams& p, hipStream_t st);
 int pg_join(int dtype, const PgParams& p, hipStream_t st);
 
 }  // namespace qlka

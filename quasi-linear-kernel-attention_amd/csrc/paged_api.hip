@@ -48,12 +48,16 @@ constexpr int64_t STEP_GROUPS = 1536, STEP_GROUPS_CODED = 768, STEP_GROUPS_CODED
 // for 9.3; of 500: 9.2 either way).
 constexpr int64_t STEP_LEAST = 128, TILE_LEAST = 256, STEP_WHOLE = 512, TILE_WHOLE = 256;
 
+// The units of more sequences than a workgroup looks up by itself are found once, by a kernel before the others (512 of 100
+// to 1000, 12 / 4 heads, bf16: 52 us for 57; 2000 of 100 to 500, int8: 106 for 278; but 256: 36 for 34).
+bool many(const qlka_paged_args* a) { return a->B > PG_LOOKED_UP; }
+
 struct Plan {
     bool step, tiles, join;
     int few;
     PgUnits units[2];                        // step, tiles
-    size_t part[2], part2[2];
-    size_t bytes() const { return part[0] + part2[0] + part[1] + part2[1]; }
+    size_t part[2], part2[2], table[2];
+    size_t bytes() const { return part[0] + part2[0] + part[1] + part2[1] + table[0] + table[1]; }
 };
 Plan plan(const qlka_paged_args* a) {
     Plan r{};
@@ -92,6 +96,7 @@ Plan plan(const qlka_paged_args* a) {
         u.least = parts ? (int)k.least : (int)LONGEST;
         u.room = units;
         u.groups = (int)std::min<int64_t>(ceil_div(units, 8) * 8, INT32_MAX);
+        if (many(a)) r.table[i] = align256(((size_t)a->B + 2) * 4);
         if (parts) {
             r.join = true;
             r.part[i] = align256((size_t)units * k.rows * DP * 4);
@@ -229,8 +234,15 @@ int qlka_paged_attention(const qlka_paged_args* a, void* ws, size_t ws_bytes, vo
     p.step.part = (float*)at; at += r.part[0];
     p.step.part2 = (float*)at; at += r.part2[0];
     p.tiles.part = (float*)at; at += r.part[1];
-    p.tiles.part2 = (float*)at;
+    p.tiles.part2 = (float*)at; at += r.part2[1];
+    if (r.table[0]) p.step.table = (int*)at;
+    at += r.table[0];
+    if (r.table[1]) p.tiles.table = (int*)at;
     hipStream_t st = (hipStream_t)stream;
+    if (many(a)) {
+        StageTimer timer("paged_table", st);
+        if (int e = pg_table(p, st)) return status(e, "attention over pages, units");
+    }
     {
         StageTimer timer("paged_attend", st);
         const int e = a->dtype == QLKA_BF16 ? pg_attend_bf16(a->held, p, st) : pg_attend_f32(a->held, p, st);

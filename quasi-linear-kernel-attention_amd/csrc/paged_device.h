@@ -156,7 +156,8 @@ __device__ __forceinline__ Found find(const PgParams& p, int t, Tokens mine) {
 // a lane a sequence. The parts of a sequence are of one length (4 chunks of up to 8192: the longest of 19 tiles instead of 20,
 // 65 us instead of 68). Units of one sequence, part and key head are next to each other, and successive ones on one XCD, whose L2
 // then serves their keys. Where a sequence's positions are one part, its rows are written at once, else each part's sums
-// go to the unit's place in the workspace and paged_join adds them up.
+// go to the unit's place in the workspace and paged_join adds them up. Of many sequences a kernel of its own writes the span
+// and the units before each one to the workspace (u.table), where the others look.
 struct Cut { int blocks, parts, span; };     // of a sequence: units a key head = blocks * parts; positions of a part
 struct Unit { int b, part, kvh, block, parts, span, at; };
 
@@ -176,20 +177,20 @@ template <bool STEP, int ROWS> struct Units {
         const bool here = b < p.B && STEP == (rows <= p.few) && rows > 0;
         return {here ? (rows + ROWS - 1) / ROWS : 0, seen_from(p, t.start + t.rows - 1)};
     }
-    // f(the first of 64 sequences, what this lane's is) for those from 64 up to `end`, until it returns true; 256 are looked up
-    // together (512 sequences of 100 to 1000, 12 / 4 heads, bf16: 67 us with 64)
+    // f(the first of 64 sequences, what this lane's is) for those from 64 up to `end`, until it returns true; all are looked up
+    // together (256 of 100 to 1000, 8 with chunks, 12 / 4 heads, bf16: 54 us, 56 one after the other); more of them are in
+    // u.table
     template <class F> __device__ __forceinline__ void others(int end, F f) const {
+        constexpr int EACH = (PG_LOOKED_UP - 64) / 64;
+        if (end <= 64) return;
         const int lane = threadIdx.x & 63;
-#pragma unroll 1
-        for (int from = 64; from < end; from += 256) {
-            Tokens t[4];
+        Tokens t[EACH];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) t[i] = tokens_of(p, min(from + 64 * i + lane, p.B - 1));
+        for (int i = 0; i < EACH; ++i) t[i] = tokens_of(p, min(64 + 64 * i + lane, p.B - 1));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int b = from + 64 * i;
-                if (b >= end || f(b, held(b + lane, t[i]))) return;
-            }
+        for (int i = 0; i < EACH; ++i) {
+            const int b = 64 + 64 * i;
+            if (b >= end || f(b, held(b + lane, t[i]))) return;
         }
     }
     __device__ __forceinline__ Cut cut(Held h) const {
@@ -200,6 +201,11 @@ template <bool STEP, int ROWS> struct Units {
     __device__ __forceinline__ Units(const PgParams& p, const PgUnits& u) : Units(p, u, tokens_of_lane(p)) {}
     __device__ __forceinline__ Units(const PgParams& p, const PgUnits& u, Tokens mine)
         : p(p), u(u), share(p.H / p.G), mine(mine) {
+        if (__builtin_expect(u.table != nullptr, 0)) {
+            all = __builtin_amdgcn_readfirstlane(u.table[p.B]);
+            span = __builtin_amdgcn_readfirstlane(u.table[p.B + 1]);
+            return;
+        }
         const int lane = threadIdx.x & 63;
         const Held held_mine = held(lane, mine);
         float work = (float)held_mine.blocks * (float)held_mine.seen;
@@ -207,23 +213,28 @@ template <bool STEP, int ROWS> struct Units {
             work += (float)h.blocks * (float)h.seen;
             return false;
         });
-        work = last_lane(sums_upto(work));
-        span = max((int)fminf(work / u.aim, (float)(1 << 28)) + 1, u.least);
-        span = __builtin_amdgcn_readfirstlane((span + PG_ALIGN - 1) / PG_ALIGN * PG_ALIGN);
+        set_span(last_lane(sums_upto(work)));
         cut_mine = cut(held_mine);
         first = cut_mine.blocks * cut_mine.parts;
         before = sums_upto(first);
         all = upto(p.B);
     }
+    // for paged_table
+    __device__ __forceinline__ Units(const PgParams& p, const PgUnits& u, int) : p(p), u(u), share(p.H / p.G) {}
+    __device__ __forceinline__ void set_span(float work) {
+        span = max((int)fminf(work / u.aim, (float)(1 << 28)) + 1, u.least);
+        span = __builtin_amdgcn_readfirstlane((span + PG_ALIGN - 1) / PG_ALIGN * PG_ALIGN);
+    }
     // of a sequence that is the same for all lanes
     __device__ __forceinline__ Tokens tokens(int b) const {
-        if (b >= 64) return tokens_of(p, b);
+        if (b >= 64 || u.table) return tokens_of(p, b);
         return {__builtin_amdgcn_readlane(mine.first, b), __builtin_amdgcn_readlane(mine.rows, b),
                 __builtin_amdgcn_readlane(mine.start, b)};
     }
     // units of the sequences before `end`
     __device__ __forceinline__ int upto(int end) const {
         if (end <= 0) return 0;
+        if (__builtin_expect(u.table != nullptr, 0)) return __builtin_amdgcn_readfirstlane(u.table[end]);
         const int n = __builtin_amdgcn_readlane(before, min(end, 64) - 1);
         if (end <= 64) return n;
         const int lane = threadIdx.x & 63;
@@ -235,6 +246,16 @@ template <bool STEP, int ROWS> struct Units {
         });
         return n + last_lane(sums_upto(more));
     }
+    // number `rest` of a sequence's units
+    __device__ __forceinline__ void place(Unit& x, Cut c, int rest) const {
+        const int blocks = max(__builtin_amdgcn_readfirstlane(c.blocks), 1);
+        rest = __builtin_amdgcn_readfirstlane(rest);
+        x.parts = __builtin_amdgcn_readfirstlane(c.parts);
+        x.span = __builtin_amdgcn_readfirstlane(c.span);
+        x.part = rest / (blocks * p.G);
+        x.kvh = rest % (blocks * p.G) / blocks;
+        x.block = rest % blocks;
+    }
     // The unit of a workgroup; b < 0 where it has none.
     __device__ __forceinline__ Unit of(int wg) const {
         const int units = all * p.G, each = (units + 7) / 8;
@@ -243,6 +264,12 @@ template <bool STEP, int ROWS> struct Units {
         x.at = (wg & 7) * each + (wg >> 3);
         // (offsets that decrease can make more units than a launch and its workspace are made for)
         if ((wg >> 3) >= each || x.at >= units || x.at >= u.room) return x;
+        if (__builtin_expect(u.table != nullptr, 0)) {
+            x.b = last_upto(p.B + 1, x.at, [&](int j) { return u.table[j] * p.G; });
+            x.b = min(max(__builtin_amdgcn_readfirstlane(x.b), 0), p.B - 1);
+            place(x, cut(held(x.b, tokens_of(p, x.b))), x.at - u.table[x.b] * p.G);
+            return x;
+        }
         int base = 0;                        // units a key head of the sequences before those that are looked at
         // whether the unit is of one of 64 sequences: this lane's cut, its units a key head, and those up to it
         const auto among = [&](int b0, Cut c, int n, int to) {
@@ -252,14 +279,9 @@ template <bool STEP, int ROWS> struct Units {
                 return false;
             }
             const int l = __builtin_ctzll(past);
-            const int blocks = __builtin_amdgcn_readlane(c.blocks, l);
-            const int rest = x.at - (base + __builtin_amdgcn_readlane(to - n, l)) * p.G;
             x.b = b0 + l;
-            x.parts = __builtin_amdgcn_readlane(c.parts, l);
-            x.span = __builtin_amdgcn_readlane(c.span, l);
-            x.part = rest / (blocks * p.G);
-            x.kvh = rest % (blocks * p.G) / blocks;
-            x.block = rest % blocks;
+            place(x, {__builtin_amdgcn_readlane(c.blocks, l), __builtin_amdgcn_readlane(c.parts, l),
+                      __builtin_amdgcn_readlane(c.span, l)}, x.at - (base + __builtin_amdgcn_readlane(to - n, l)) * p.G);
             return true;
         };
         if (!among(0, cut_mine, first, before))

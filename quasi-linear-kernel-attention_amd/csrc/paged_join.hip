@@ -97,7 +97,57 @@ template <class T, int DP, bool MANY> __global__ __launch_bounds__(256) void pag
 }
 constexpr int64_t JOIN_MANY = 4096;          // rows
 
+// The units before each of the sequences, of all, and the span: B + 2 numbers for each kind of units, of which each has a
+// workgroup.
+constexpr int TABLE_THREADS = 1024;
+template <class U> __device__ __forceinline__ void fill_table(const PgParams& p, const PgUnits& u, U units, int* sums,
+                                                              float* works) {
+    const int tid = threadIdx.x, wave = tid >> 6;
+    double mine = 0;                         // (of a million sequences floats would lose what the span has to spare)
+    for (int b = tid; b < p.B; b += TABLE_THREADS) {
+        const auto h = units.held(b, tokens_of(p, b));
+        mine += (double)h.blocks * h.seen;
+    }
+    float work = last_lane(sums_upto((float)mine));
+    if ((tid & 63) == 0) works[wave] = work;
+    __syncthreads();
+    work = 0.f;
+    for (int w = 0; w < TABLE_THREADS / 64; ++w) work += works[w];
+    units.set_span(work);
+    int base = 0;
+    for (int b0 = 0; b0 < p.B; b0 += TABLE_THREADS) {
+        const int b = b0 + tid;
+        int n = 0;
+        if (b < p.B) {
+            const Cut c = units.cut(units.held(b, tokens_of(p, b)));
+            n = c.blocks * c.parts;
+        }
+        int to = sums_upto(n);
+        if ((tid & 63) == 63) sums[wave] = to;
+        __syncthreads();
+        for (int w = 0; w < wave; ++w) to += sums[w];
+        if (b < p.B) u.table[b] = base + to - n;
+        for (int w = 0; w < TABLE_THREADS / 64; ++w) base += sums[w];
+        __syncthreads();
+    }
+    if (tid == 0) {
+        u.table[p.B] = base;
+        u.table[p.B + 1] = units.span;
+    }
+}
+__global__ __launch_bounds__(TABLE_THREADS) void paged_table(const PgParams p) {
+    __shared__ int sums[TABLE_THREADS / 64];
+    __shared__ float works[TABLE_THREADS / 64];
+    if (blockIdx.x == 0 && p.step.groups) fill_table(p, p.step, Units<true, PG_STEP_ROWS>(p, p.step, 0), sums, works);
+    if (blockIdx.x == 1 && p.tiles.groups) fill_table(p, p.tiles, Units<false, PG_TILE_ROWS>(p, p.tiles, 0), sums, works);
+}
+
 }  // namespace pg
+
+int pg_table(const PgParams& p, hipStream_t st) {
+    pg::paged_table<<<2, pg::TABLE_THREADS, 0, st>>>(p);
+    return (int)hipGetLastError();
+}
 
 int pg_join(int dtype, const PgParams& p, hipStream_t st) {
     return sm::dispatch(dtype, p.D, [&](auto t, auto dp) {

@@ -289,6 +289,27 @@ def test_many_sequences(dev, case, dtype, held):
         assert want is None or torch.equal(as_bytes(got).cpu(), want)
 
 
+@pytest.mark.parametrize("dtype,held", [(F32, F32), (BF16, BF16), (BF16, E4)], ids=["fp32", "bf16", "bf16_e4m3"])
+@pytest.mark.parametrize("B", [255, 256, 1024, 1025, 2100])
+@pytest.mark.parametrize("kind", ["tokens", "mixed", "sparse"])
+def test_hundreds_of_sequences(dev, kind, B, dtype, held):
+    gen = torch.Generator().manual_seed(B)
+    new = [1] * B
+    if kind != "tokens":
+        new = torch.randint(0, 3, (B,), generator=gen).tolist() if kind == "mixed" else [0] * B
+        new[0], new[B // 2], new[B - 1] = 0, 70, 40
+    lengths = [n + m for n, m in zip(new, torch.randint(0, 20, (B,), generator=gen).tolist())]
+    lengths[B - 1], lengths[B // 3] = 1500, 700
+    offsets = sums(new, 1)
+    tables, num_pages = tables_of(lengths, 16, gen)
+    cache, cpu = filled(num_pages, 16, 2, 32, dtype, held, gen, dev)
+    q = torch.randn(4, offsets[-1] + 2, 32, generator=gen).to(dtype)
+    want, bound = oracle.attention(q, *cpu, held, tables, lengths, offsets, 0.2)
+    got = attend(dev, q, cache, tables, lengths, offsets, scale=0.2)
+    close(got, want, bound)
+    assert (got[:, :1] == 0).all() and (got[:, offsets[-1]:] == 0).all()
+
+
 @pytest.mark.parametrize("dtype,held", [(F32, F32), (BF16, BF16), (BF16, I8)], ids=["fp32", "bf16", "bf16_int8"])
 @pytest.mark.parametrize("new,length,heads", [([1], 20000, (2, 1, 32)), ([3, 1], 18000, (2, 2, 128)), ([400], 10000, (12, 4, 64)),
                                               ([700], 5000, (7, 7, 32)), ([600, 1], 4000, (8, 1, 128))], ids=str)
