@@ -35,13 +35,22 @@ int check_sizes(const qlka_paged_args* a) {
 // tokens: 59 and 55), others have to be taken apart or turned into bf16 (fp32, 4 sequences of up to 8000, 6 to 12 tokens:
 // 24 us with 32, 39 with 16; e4m3, 12 / 12 heads, 12 to 24 tokens: 120 and 128).
 int few_rows(const qlka_paged_args* a) { return a->held == QLKA_BF16 ? 16 : 32; }
-// Workgroups of a launch that fill the GPU, and the least positions that one takes. Tiles alone: three a compute unit (4
-// chunks of 512 at up to 8192, int8, 12 / 4 heads: 68 us; 71 with two, 80 with six), beside tokens two, so that those
-// have a third (32 sequences, two with chunks of 700: 46 us for 50). Tokens over bf16 rows: 1536 (16 sequences of up to 8192, 12
-// heads: 52 us; 56 with 768), over 8 bits 768 (32 of up to 16384, 12 / 4: 33.2 us; 33.8 with 1024, 37.4 with 1536),
-// beside tiles 1024 (64 of up to 8192, 8 with chunks of 512: 164 us; 181 with 768).
-constexpr int64_t TILE_GROUPS = 768, TILE_GROUPS_MIXED = 512;
-constexpr int64_t STEP_GROUPS = 1536, STEP_GROUPS_CODED = 768, STEP_GROUPS_CODED_MIXED = 1024;
+// Workgroups of a launch that fill the GPU. Where registers leave room for two a compute unit (fp32, and rows of 128): those, one
+// round (tokens of 16 sequences of 2000 to 8192: 8 heads of 128, int8 41 us, 50 with 768, 47 with 1024; bf16 54, 57 with
+// 1536; fp32, 12 heads of 64, 97, 107 with 768 or 1536; chunks of 512, 8 / 2 heads of 128, int8: 83, 91 with 768).
+// Beside tiles three (24 of 500 to 5000, three with chunks of 500, fp32: 57 us, 60 with six).
+bool two(const qlka_paged_args* a) { return a->dtype == QLKA_F32 || sm_padded(a->D) == 128; }
+// Rows of 64 in bf16: six a compute unit (16 of 2000 to 8192, 12 heads: 52 us, 56 with three), in 8 bits three (32 of up to
+// 16384, 12 / 4: 33.2 us; 33.8 with four, 37.4 with six), beside tiles four (64 of up to 8192, 8 with chunks of 512: 164
+// us; 181 with three). Rows of 32: four (12 heads, bf16 25.3 us, 27.4 with six; int8 23.7, 25.4 with three).
+int64_t step_groups(const qlka_paged_args* a, bool tiles) {
+    if (two(a)) return tiles ? 768 : 512;
+    if (sm_padded(a->D) == 32) return 1024;
+    return !coded(a) ? 1536 : tiles ? 1024 : 768;
+}
+// Tiles alone: three a compute unit (4 chunks of 512 at up to 8192, int8, 12 / 4 heads: 68 us; 71 with two, 80 with six), beside
+// tokens two, so that those have a third (32 sequences, two with chunks of 700: 46 us for 50).
+int64_t tile_groups(const qlka_paged_args* a, bool step) { return two(a) || step ? 512 : 768; }
 // The least positions of a part: a turn of the step kernel's waves (one sequence of 2000, int8, 12 / 4 heads: 9.3 us; 10.6 with
 // 256, 17.4 as one), a few tiles of the others (300 tokens of it: 20.1 us; 24.4 with 128, 23.2 with 512). A call whose
 // tables have no room for more than so many positions is not cut at all, which saves joining (one sequence of 250: 7.0 us
@@ -76,9 +85,8 @@ Plan plan(const qlka_paged_args* a) {
     const int64_t places = std::min<int64_t>((int64_t)a->table_len * a->page_size, LONGEST);
     const int DP = sm_padded(a->D);
     const struct { bool used; int rows; int64_t groups, least, whole; } kernels[2] = {
-        {r.step, PG_STEP_ROWS, !coded(a) ? STEP_GROUPS : r.tiles ? STEP_GROUPS_CODED_MIXED : STEP_GROUPS_CODED, STEP_LEAST,
-         STEP_WHOLE},
-        {r.tiles, PG_TILE_ROWS, r.step ? TILE_GROUPS_MIXED : TILE_GROUPS, TILE_LEAST, TILE_WHOLE}};
+        {r.step, PG_STEP_ROWS, step_groups(a, r.tiles), STEP_LEAST, STEP_WHOLE},
+        {r.tiles, PG_TILE_ROWS, tile_groups(a, r.step), TILE_LEAST, TILE_WHOLE}};
     for (int i = 0; i < 2; ++i) {
         const auto& k = kernels[i];
         if (!k.used) continue;
