@@ -35,18 +35,17 @@ int check_sizes(const qlka_paged_args* a) {
 // tokens: 59 and 55), others have to be taken apart or turned into bf16 (fp32, 4 sequences of up to 8000, 6 to 12 tokens:
 // 24 us with 32, 39 with 16; e4m3, 12 / 12 heads, 12 to 24 tokens: 120 and 128).
 int few_rows(const qlka_paged_args* a) { return a->held == QLKA_BF16 ? 16 : 32; }
-// Workgroups of a launch that fill the GPU. Where registers leave room for two a compute unit (fp32, and rows of 128): those, one
-// round (tokens of 16 sequences of 2000 to 8192: 8 heads of 128, int8 41 us, 50 with 768, 47 with 1024; bf16 54, 57 with
-// 1536; fp32, 12 heads of 64, 97, 107 with 768 or 1536; chunks of 512, 8 / 2 heads of 128, int8: 83, 91 with 768).
-// Beside tiles three (24 of 500 to 5000, three with chunks of 500, fp32: 57 us, 60 with six).
+// Workgroups of a launch: one round of those that registers leave room for. Two a compute unit of fp32 and of rows of 128
+// (tokens of 16 sequences of 2000 to 8192: 8 heads of 128, int8 41 us, 50 with 768, 47 with 1024; bf16 54, 57 with 1536;
+// fp32, 12 heads of 64, 97, 107 with 768 or 1536; chunks of 512, 8 / 2 heads of 128, int8: 83, 91 with 768); three of bf16
+// rows of 64 (12 / 4 heads 20.7 us, 24.5 with 1536; 12 heads, cold pages, 50.4 and 51.5); four of 8 bits and of rows of 32 (12
+// heads of 64, int8: 31.1 us, 33.2 with 768). Beside tiles more and smaller ones fill what those leave (64 of up to 8192, 8
+// with chunks of 512, 12 heads of 64: bf16 162 us, 178 with one round; int8 146 and 160; 24 of 500 to 5000, fp32: 57, 60
+// with three rounds).
 bool two(const qlka_paged_args* a) { return a->dtype == QLKA_F32 || sm_padded(a->D) == 128; }
-// Rows of 64 in bf16: six a compute unit (16 of 2000 to 8192, 12 heads: 52 us, 56 with three), in 8 bits three (32 of up to
-// 16384, 12 / 4: 33.2 us; 33.8 with four, 37.4 with six), beside tiles four (64 of up to 8192, 8 with chunks of 512: 164
-// us; 181 with three). Rows of 32: four (12 heads, bf16 25.3 us, 27.4 with six; int8 23.7, 25.4 with three).
 int64_t step_groups(const qlka_paged_args* a, bool tiles) {
     if (two(a)) return tiles ? 768 : 512;
-    if (sm_padded(a->D) == 32) return 1024;
-    return !coded(a) ? 1536 : tiles ? 1024 : 768;
+    return tiles ? 1536 : coded(a) || sm_padded(a->D) == 32 ? 1024 : 768;
 }
 // Tiles alone: three a compute unit (4 chunks of 512 at up to 8192, int8, 12 / 4 heads: 68 us; 71 with two, 80 with six), beside
 // tokens two, so that those have a third (32 sequences, two with chunks of 700: 46 us for 50).
