@@ -9,8 +9,8 @@
 // this wave uses. A row's reference for the exponentials is moved when some lane's score passes it by 2^8, so nothing
 // crosses lanes in most turns. Waves are joined at the end, the parts of long sequences by paged_join.
 //
-// Measured: 16 sequences of 2000 to 8192, 12 heads of 64, bf16: 38 us under way for 211 MB, of which the card's last-level
-// cache serves a part, 51 with the joining and cold pages (shuffled pages are read at 5.1 TB/s at most); 32 of 1000 to
+// Measured: 16 sequences of 2000 to 8192, 12 heads of 64, bf16: 37 us under way for 211 MB, of which the card's last-level
+// cache serves a part, 50 with the joining and cold pages (shuffled pages are read at 5.1 TB/s at most); 32 of 1000 to
 // 16384, 12 / 4 heads, e4m3: 22 us, 32 with all; 8 of 33 to 197: 6.5 us, latency of lengths, table and rows in turn.
 //
 // Elements of 8 bits become bf16 exactly (paged_cache.hip), so products are those of what is held.
