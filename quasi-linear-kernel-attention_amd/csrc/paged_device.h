@@ -249,7 +249,7 @@ template <bool STEP, int ROWS> struct Units {
     // number `rest` of a sequence's units
     __device__ __forceinline__ void place(Unit& x, Cut c, int rest) const {
         const int blocks = max(__builtin_amdgcn_readfirstlane(c.blocks), 1);
-        rest = __builtin_amdgcn_readfirstlane(rest);
+        rest = max(__builtin_amdgcn_readfirstlane(rest), 0);       // (sums of offsets that decrease can pass 32 bits)
         x.parts = __builtin_amdgcn_readfirstlane(c.parts);
         x.span = __builtin_amdgcn_readfirstlane(c.span);
         x.part = rest / (blocks * p.G);
