@@ -69,7 +69,7 @@ struct Plan {
 };
 Plan plan(const qlka_paged_args* a) {
     Plan r{};
-    const int64_t share = a->H / a->G, sequences = std::max(a->B, 1);
+    const int64_t share = a->H / a->G;
     const int64_t longest = !a->offsets ? 1 : a->longest ? std::min(a->longest, a->T) : a->T;
     const int few = few_rows(a);
     r.step = r.tiles = true;
@@ -77,7 +77,7 @@ Plan plan(const qlka_paged_args* a) {
     if (!a->offsets || longest * share <= few) {
         r.tiles = false;
         r.few = INT32_MAX;
-    } else if (a->T * share >= 256 * sequences) {       // chunks, on the average: a token among them takes a tile too
+    } else if (a->T * share >= 256 * std::max<int64_t>(a->B, 1)) {       // chunks, on the average: a token among them takes a tile too
         r.step = false;
         r.few = -1;
     }
@@ -89,12 +89,17 @@ Plan plan(const qlka_paged_args* a) {
     for (int i = 0; i < 2; ++i) {
         const auto& k = kernels[i];
         if (!k.used) continue;
-        // blocks of rows a key head: each sequence has one that is not full at most, and more in the step kernel only
+        // Sequences that have rows here, at most: of the tiles' beside the step kernel's each has more than `few` rows.
+        // (A chunk of 512 among 1999 tokens, 12 heads of 64: 173 MiB of workspace, 889 with a block for each of them;
+        // among 999: 360 us for 371.)
+        const int64_t tokens = i == 1 && r.step ? few / share + 1 : 1;
+        const int64_t sequences = std::min<int64_t>(a->B, a->T / tokens);
+        // blocks of rows a key head: each of them has one that is not full at most, and more in the step kernel only
         // where it is alone
-        int64_t blocks = a->T * share / k.rows + a->B;
-        if (i == 0 && r.tiles) blocks = std::min<int64_t>(blocks, (int64_t)a->B * (few / PG_STEP_ROWS));
+        int64_t blocks = a->T * share / k.rows + sequences;
+        if (i == 0 && r.tiles) blocks = std::min<int64_t>(blocks, sequences * (few / PG_STEP_ROWS));
         // a sequence's last part is shorter than the others: room for those within the round of workgroups
-        const int64_t last = a->G * (i == 0 ? sequences : a->T * share / k.rows + sequences) / 2;
+        const int64_t last = a->G * (i == 0 ? sequences : blocks) / 2;
         const int64_t aim = std::max<int64_t>(std::max(k.groups - last, k.groups / 2) / a->G, 1);
         const bool parts = places > k.whole;
         const int64_t units = (blocks + (parts ? aim + 1 : 0)) * a->G;          // the sum of parts rounded up

@@ -156,6 +156,19 @@ def test_workspaces(lib):
     assert lib.qlka_paged_attention_ws_bytes(ctypes.byref(args(table_len=2))) == 0           # nothing to split
 
 
+@pytest.mark.parametrize("H,G,D", [(12, 12, 64), (12, 4, 64), (32, 32, 128)])
+def test_workspace_of_a_chunk_among_many_tokens(lib, H, G, D):
+    """Parts' places go by the sequences that can have them: a chunk among single tokens takes no more than both apart and
+    a block of 128 rows for each sequence long enough for the tiles; sequences without a token take none."""
+    def need(**kw):
+        return lib.qlka_paged_attention_ws_bytes(ctypes.byref(args(H=H, G=G, D=D, held=1, page_size=64, table_len=128, **kw)))
+    apart = need(B=2000, T=2000, offsets=None) + need(B=1, T=512)
+    share, few = H // G, 16
+    long_enough = 2511 // (few // share + 1)
+    assert need(B=2000, T=2511) <= apart + 2 * long_enough * G * 128 * (D + 2) * 4
+    assert need(B=2000, T=20) <= need(B=20, T=20) + (1 << 20)
+
+
 def test_nothing_to_do(lib):
     a = args(B=0, T=0, N=0, offsets=None, tables=None, lengths=None, q=None, k=None, v=None, out=None, out_k=None, out_v=None)
     for name, call in calls(lib, ctypes.byref(a)).items():
