@@ -6,6 +6,7 @@
 #include <cstddef>
 #include <cstdint>
 
+#include "paged_cut.h"
 #include "qlka.h"
 
 namespace qlka {
@@ -36,7 +37,7 @@ struct PgParams {
     int B, H, G, T, D, N;
     int page_size, num_pages, table_len;
     int places;                              // positions that a table's row has pages for
-    uint32_t magic, shift;                   // n / page_size = high word of 2 n * magic, >> shift, for n below 2^31
+    pg::Division page_division;
     float scale, q_sign;                     // |scale|; its sign (or 0)
     PgUnits step, tiles;                     // few rows (paged_step.h) and chunks (paged_tiles.h); groups 0: not in this call
     int few;                                 // sequences of more rows a key head are the tiles'

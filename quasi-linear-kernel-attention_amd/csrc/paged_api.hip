@@ -138,10 +138,7 @@ int params(const qlka_paged_args* a, PgParams* p) {
     p->B = a->B; p->H = a->H; p->G = a->G; p->T = a->T; p->D = a->D; p->N = a->N;
     p->page_size = a->page_size; p->num_pages = a->num_pages; p->table_len = a->table_len;
     p->places = (int)std::min<int64_t>((int64_t)a->table_len * a->page_size, LONGEST);
-    int log = 0;
-    while (1 << log < a->page_size) ++log;
-    p->shift = log;
-    p->magic = (uint32_t)(((uint64_t(1) << (31 + log)) + a->page_size - 1) / a->page_size);
+    p->page_division = pg::division_by(a->page_size);
     p->blocks = 1;
     const int64_t sizes[3] = {a->num_pages, a->G, a->page_size};
     const struct { const char* name; const void* x; const int64_t* s; } pages[] = {

@@ -2,6 +2,7 @@
 #pragma once
 
 #include "paged.h"
+#include "paged_cut.h"
 #include "segments.h"
 #include "softmax_tile.h"
 
@@ -82,7 +83,7 @@ template <class C> __device__ __forceinline__ sm::Frag<1> parts_of(u32x4 x, int 
 // A position's place: the index of its page in the table, and its row in the page.
 struct Place { int index, row; };
 __device__ __forceinline__ Place place_of(const PgParams& p, int n) {
-    const int index = (int)(__umulhi(2u * (uint32_t)n, p.magic) >> p.shift);
+    const int index = divided(n, p.page_division);
     return {index, n - index * p.page_size};
 }
 // Where a row of a page is from the first one of its head on.
@@ -111,15 +112,13 @@ template <class X> __device__ __forceinline__ X last_lane(X x) {
     return y.x;
 }
 
-// The new tokens of a sequence: `rows` of them from row `first` on, the first at position `start`.
-struct Tokens { int first, rows, start; };
 __device__ __forceinline__ Tokens tokens_of(const PgParams& p, int b) {
     int first = b, rows = 1;
     if (p.offsets) {
         first = segment_edge(p.offsets, p.B, p.T, b + 1);
-        rows = max(segment_edge(p.offsets, p.B, p.T, b + 2) - first, 0);
+        rows = rows_between(first, segment_edge(p.offsets, p.B, p.T, b + 2));
     }
-    return {first, rows, min(max(p.lengths[b], 0), 1 << 28) - rows};
+    return tokens_at(first, rows, p.lengths[b]);
 }
 // Positions up to `seat` that have a place.
 __device__ __forceinline__ int seen_from(const PgParams& p, int seat) {
@@ -158,7 +157,6 @@ __device__ __forceinline__ Found find(const PgParams& p, int t, Tokens mine) {
 // then serves their keys. Where a sequence's positions are one part, its rows are written at once, else each part's sums
 // go to the unit's place in the workspace and paged_join adds them up. Of many sequences a kernel of its own writes the span
 // and the units before each one to the workspace (u.table), where the others look.
-struct Cut { int blocks, parts, span; };     // of a sequence: units a key head = blocks * parts; positions of a part
 struct Unit { int b, part, kvh, block, parts, span, at; };
 
 template <bool STEP, int ROWS> struct Units {
@@ -171,8 +169,7 @@ template <bool STEP, int ROWS> struct Units {
     Cut cut_mine;
     int first, before;                       // its units a key head, and those up to it
 
-    struct Held { int blocks, seen; };
-    __device__ __forceinline__ Held held(int b, Tokens t) const {
+    __device__ __forceinline__ Extent held(int b, Tokens t) const {
         const int rows = t.rows * share;
         const bool here = b < p.B && STEP == (rows <= p.few) && rows > 0;
         return {here ? (rows + ROWS - 1) / ROWS : 0, seen_from(p, t.start + t.rows - 1)};
@@ -193,10 +190,7 @@ template <bool STEP, int ROWS> struct Units {
             if (b >= end || f(b, held(b + lane, t[i]))) return;
         }
     }
-    __device__ __forceinline__ Cut cut(Held h) const {
-        const uint32_t parts = max(1, (h.seen + span - 1) / span), each = ((uint32_t)h.seen + parts - 1) / parts;
-        return {h.blocks, (int)parts, max((int)(each + ALIGN - 1) / ALIGN, 1) * ALIGN};
-    }
+    __device__ __forceinline__ Cut cut(Extent h) const { return cut_of(h, span, ALIGN); }
 
     __device__ __forceinline__ Units(const PgParams& p, const PgUnits& u) : Units(p, u, tokens_of_lane(p)) {}
     __device__ __forceinline__ Units(const PgParams& p, const PgUnits& u, Tokens mine)
@@ -207,10 +201,10 @@ template <bool STEP, int ROWS> struct Units {
             return;
         }
         const int lane = threadIdx.x & 63;
-        const Held held_mine = held(lane, mine);
-        float work = (float)held_mine.blocks * (float)held_mine.seen;
-        others(p.B, [&](int, Held h) {
-            work += (float)h.blocks * (float)h.seen;
+        const Extent held_mine = held(lane, mine);
+        float work = more_work(0.f, held_mine);
+        others(p.B, [&](int, Extent h) {
+            work = more_work(work, h);
             return false;
         });
         set_span(last_lane(sums_upto(work)));
@@ -222,8 +216,7 @@ template <bool STEP, int ROWS> struct Units {
     // for paged_table
     __device__ __forceinline__ Units(const PgParams& p, const PgUnits& u, int) : p(p), u(u), share(p.H / p.G) {}
     __device__ __forceinline__ void set_span(float work) {
-        span = max((int)fminf(work / u.aim, (float)(1 << 28)) + 1, u.least);
-        span = __builtin_amdgcn_readfirstlane((span + PG_ALIGN - 1) / PG_ALIGN * PG_ALIGN);
+        span = __builtin_amdgcn_readfirstlane(span_of(work, u.aim, u.least, PG_ALIGN));
     }
     // of a sequence that is the same for all lanes
     __device__ __forceinline__ Tokens tokens(int b) const {
@@ -239,7 +232,7 @@ template <bool STEP, int ROWS> struct Units {
         if (end <= 64) return n;
         const int lane = threadIdx.x & 63;
         int more = 0;
-        others(end, [&](int b, Held h) {
+        others(end, [&](int b, Extent h) {
             const Cut c = cut(h);
             more += b + lane < end ? c.blocks * c.parts : 0;
             return false;
@@ -248,13 +241,12 @@ template <bool STEP, int ROWS> struct Units {
     }
     // number `rest` of a sequence's units
     __device__ __forceinline__ void place(Unit& x, Cut c, int rest) const {
-        const int blocks = max(__builtin_amdgcn_readfirstlane(c.blocks), 1);
-        rest = max(__builtin_amdgcn_readfirstlane(rest), 0);       // (sums of offsets that decrease can pass 32 bits)
+        const InSequence at = place_in(__builtin_amdgcn_readfirstlane(c.blocks), __builtin_amdgcn_readfirstlane(rest), p.G);
         x.parts = __builtin_amdgcn_readfirstlane(c.parts);
         x.span = __builtin_amdgcn_readfirstlane(c.span);
-        x.part = rest / (blocks * p.G);
-        x.kvh = rest % (blocks * p.G) / blocks;
-        x.block = rest % blocks;
+        x.part = at.part;
+        x.kvh = at.kvh;
+        x.block = at.block;
     }
     // The unit of a workgroup; b < 0 where it has none.
     __device__ __forceinline__ Unit of(int wg) const {
@@ -285,7 +277,7 @@ template <bool STEP, int ROWS> struct Units {
             return true;
         };
         if (!among(0, cut_mine, first, before))
-            others(p.B, [&](int b0, Held h) {
+            others(p.B, [&](int b0, Extent h) {
                 const Cut c = cut(h);
                 const int n = c.blocks * c.parts;
                 return among(b0, c, n, sums_upto(n));
