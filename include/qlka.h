@@ -309,9 +309,11 @@ int qlka_bias_map_bwd(const float* g, const int* border, int num_borders, int bi
  *
  * q (H, T, D), k and v (G, T, D); *_stride are the distances in elements between heads and rows. Types, D, alignment,
  * scale, roundings, lse, log_sums (2, H, T), out_full (H, T, D) and the gradients are as for qlka_softmax_fwd / _bwd
- * without a table; offsets that decrease give rows that are not said, but no access outside the tensors. The offsets may
- * change between the replays of a captured call. A launch takes less than 2^32 threads: heads * (T / 32 + B) stays below
- * 2^24.
+ * without a table, but that log_sums are those of the exponentials before their rounding to bf16: no other error than its
+ * own rounding is in a probability of the gradients (where keys are split, out can then differ in its last place from
+ * that of a call without log_sums). Offsets that decrease give rows that are not said, but no access
+ * outside the tensors. The offsets may change between the replays of a captured call. A launch takes less than 2^32
+ * threads: heads * (T / 32 + B) stays below 2^24.
  */
 typedef struct qlka_packed_args {
     int dtype, B, H, G, T, D;

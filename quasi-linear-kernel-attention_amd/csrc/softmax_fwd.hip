@@ -11,7 +11,9 @@
 // Where the table's gradient will be wanted (FINE) they are taken in three parts of 8 bits: that gradient is fp32 and a
 // sum over rows of dS = P (dP - delta), in which an error of delta, the row sum of dO * O, does not average out. The
 // smaller parts' products then gather in a sum of their own, as in Acc (12 x 8192 x 8192: error of the table's gradient
-// 1.0e-6, 1.8e-6 without; 476 us, 250 with one part).
+// 1.0e-6, 1.8e-6 without; 476 us, 250 with one part). The gradients form P whole, so the log sums that they divide by are
+// of the whole exponentials for packed sequences (SUMS): with the rounded ones' all of a short row's P is off by up to 2^-8
+// (12 of 256 to 8192, 12 heads, with the gradients: 1448 us, 1415 with the rounded sums).
 //
 // Masked keys are read as zeros (what stands there may be anything) and their tiles, where none is left, are skipped.
 // Bound by the matrix cores and by the scores' work between them (an exponential, a maximum and two multiply-adds a
@@ -31,9 +33,10 @@ namespace sm {
 constexpr float GROW = 4.f;          // 2^8 of the exponentials
 
 // Three parts of P leave room for three waves a SIMD (of 64 elements) only if the compiler is held to it: 476 us for 524 at
-// 12 x 8192 x 8192. So do packed sequences for four (16 of 100 to 8192, 12 / 4 heads: 571 us for 597).
-template <class T, int DP, int NW, bool BIAS, bool FINE, bool PACKED>
-__global__ __launch_bounds__(64 * NW, (FINE && DP <= 64 ? 3 : PACKED && sizeof(T) == 2 && DP == 64 && NW > 1 ? 4
+// 12 x 8192 x 8192. So do packed sequences for four (16 of 100 to 8192, 12 / 4 heads: 571 us for 597), but not with two
+// sums a row (SUMS: 12 of 256 to 8192, 12 heads, with the gradients 1448 us, 1454 with four).
+template <class T, int DP, int NW, bool BIAS, bool FINE, bool PACKED, bool SUMS = false>
+__global__ __launch_bounds__(64 * NW, (FINE && DP <= 64 ? 3 : PACKED && !SUMS && sizeof(T) == 2 && DP == 64 && NW > 1 ? 4
                                                                                                           : Shape<T, DP>::WAVES))
 void softmax_fwd(const SmParams p) {
     constexpr int NP = Elem<T>::PARTS, BN = Shape<T, DP>::BN, NT = 64 * NW, ROWS = 32 * NW, NS = BN / 32, ND = DP / 32;
@@ -88,6 +91,7 @@ void softmax_fwd(const SmParams p) {
     const float c1 = p.scale * UNIT;
     Acc<NP> o[ND];
     float top = -std::numeric_limits<float>::infinity(), ref = 0.f, sum = 0.f;
+    float whole = 0.f;                                 // SUMS: the sum before the rounding
     bool wide = false;                                 // a row here has a large ref
 
     while (coming) {
@@ -176,6 +180,7 @@ void softmax_fwd(const SmParams p) {
             wide = __any(fabsf(ref) > WIDE);
             const float f = first ? 1.f : exp_of(was - ref);              // the first time there is nothing to scale
             sum *= f;
+            if constexpr (SUMS) whole *= f;
 #pragma unroll
             for (int d = 0; d < ND; ++d) o[d].main *= f;
         }
@@ -206,9 +211,8 @@ void softmax_fwd(const SmParams p) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) e[j] = fexp2(__builtin_fmaf(e[j], mul, add));
                     const Frag<NP> pf = split<NP>(e);
-                    if constexpr (NP == 1 && !FINE) {
-                        sum = add_all(pf.p[0], sum);
-                    } else {
+                    if constexpr (NP == 1 && !FINE) sum = add_all(pf.p[0], sum);
+                    if constexpr (NP == 3 || FINE || SUMS) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j) tile_sum += e[j];
                     }
@@ -229,7 +233,7 @@ void softmax_fwd(const SmParams p) {
                     }
                 }
             }
-            sum += tile_sum;
+            (SUMS ? whole : sum) += tile_sum;
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
                 o[d].join();
@@ -241,9 +245,16 @@ void softmax_fwd(const SmParams p) {
     }
     if (m >= span.M()) return;
     sum += other_half(sum);
+    if constexpr (SUMS) whole += other_half(whole);
+    else whole = sum;
     const int64_t row = ((int64_t)b * p.H + head) * p.M + span.row(m);
     if (p.splits > 1) {
         const int64_t at = (int64_t)split_i * p.B * p.H * p.M + row;
+        if constexpr (SUMS) {                          // splits are joined by the sums that they leave
+            const float f = sum == 0.f ? 1.f : whole / sum;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[d].main *= f;
+        }
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -252,7 +263,7 @@ void softmax_fwd(const SmParams p) {
                     quad(o[d].main, r);
         if (half == 0) {
             p.part2[2 * at] = ref;
-            p.part2[2 * at + 1] = sum;
+            p.part2[2 * at + 1] = whole;
         }
         return;
     }
@@ -266,7 +277,7 @@ void softmax_fwd(const SmParams p) {
             store4(out, 32 * d + 8 * r + 4 * half, p.D, x);
             if (p.out_full) store4(p.out_full + row * p.D, 32 * d + 8 * r + 4 * half, p.D, x);
         }
-    if (half == 0) store_lse(p, row, ref, sum);
+    if (half == 0) store_lse(p, row, ref, whole);
 }
 
 template <class T, int DP, int NW> int launch_fwd(const SmParams& p, hipStream_t st) {
@@ -279,7 +290,8 @@ template <class T, int DP, int NW> int launch_fwd(const SmParams& p, hipStream_t
 }
 template <class T, int DP, int NW> int launch_packed(const SmParams& p, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)p.H * p.blocks * p.splits));
-    softmax_fwd<T, DP, NW, false, false, true><<<grid, 64 * NW, 0, st>>>(p);
+    if (sizeof(T) == 2 && p.lse) softmax_fwd<T, DP, NW, false, false, true, sizeof(T) == 2><<<grid, 64 * NW, 0, st>>>(p);
+    else softmax_fwd<T, DP, NW, false, false, true><<<grid, 64 * NW, 0, st>>>(p);
     return (int)hipGetLastError();
 }
 // Joins the splits of a row, a wave a row: first a lane for each split's maximum and sum, then DP / 4 lanes for each of

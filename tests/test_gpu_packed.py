@@ -2,6 +2,8 @@
 bounds that oracle/softmax.py derives; lengths from none to several tiles, rows outside, strides, shared heads, what one
 sequence may hold without another one's noticing, graph replays with other offsets."""
 
+import math
+
 import pytest
 import torch
 
@@ -285,3 +287,22 @@ def test_far_rows(dev, dtype):
         far[n].copy_(t[n])
     out = packed_attention(far["q"], far["k"], far["v"], torch.tensor(at, dtype=torch.int32, device=dev))
     check({"out": out}, reference(t, at, True))
+
+
+@pytest.mark.parametrize("lengths", [[14, 25, 29], [2524]], ids=["short", "split"])
+def test_gradients_divide_by_the_sum_of_whole_exponentials(dev, lengths):
+    """bf16, one key in 29 of score 0 and others whose exponentials all lie just below the middle between 1/2 and the next
+    bf16 number, so that rounding takes nearly 2^-8 of a row's sum; lengths at which P and the gradient of v round the same
+    way as that would. A row's P is off by its own rounding alone, not by the sum's too."""
+    at = offsets_of(lengths)
+    score = torch.tensor(-math.log(2) + 2.0 ** -8 * 0.99, dtype=torch.float64)
+    gen = torch.Generator().manual_seed(0)
+    t = {n: torch.zeros(1, at[-1], 64, dtype=BF16) for n in "qk"}
+    t["q"][..., :2] = 1
+    t["k"][..., 0] = score.to(BF16)
+    t["k"][..., 1] = (score - score.to(BF16).double()).to(BF16)
+    for lo, hi in zip(at, at[1:]):
+        t["k"][:, lo:hi:29] = 0
+    t["v"] = torch.randn(1, at[-1], 64, generator=gen).to(BF16)
+    t["g"] = torch.randn(1, 1, 64, generator=gen).to(BF16).expand(1, at[-1], 64).contiguous()
+    check(run(dev, t, at, causal=False, scale=1.0), reference(t, at, False, 1.0))
