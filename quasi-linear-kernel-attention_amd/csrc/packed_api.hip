@@ -37,7 +37,7 @@ Plan plan(const qlka_packed_args* a, int heads, int64_t tiles, double products, 
     const int64_t room = a->dtype == QLKA_F32 && sm_padded(a->D) == 128 ? 256 : 512;
     const bool small = average(a) <= 32 * few && (int64_t)heads * a->B > room;
     r.waves = small ? few : FWD_WAVES;
-    r.blocks = (int)segment_blocks(a->T, a->B, 1, 32 * r.waves);
+    r.blocks = (int)segment_blocks(a->T, a->B, 32 * r.waves);
     const int DP = sm_padded(a->D);
     const double tile_us = products * 0.3 * DP / 64 * (a->dtype == QLKA_F32 ? 2 : 1);
     r.splits = splits_for((int64_t)heads * r.blocks, tiles, tile_us, (double)heads * a->T * DP * 8);
@@ -58,7 +58,7 @@ struct BwdPlan {
     size_t delta, large, part, part2;
     size_t bytes() const { return delta + large + part + part2; }
 };
-int groups(const qlka_packed_args* a) { return (int)segment_blocks(a->T, a->B, 1, 32); }
+int groups(const qlka_packed_args* a) { return (int)segment_blocks(a->T, a->B, 32); }
 BwdPlan bwd_plan(const qlka_packed_args* a) {
     BwdPlan w{};
     const int t = tile_rows(a);

@@ -33,6 +33,10 @@ __host__ __device__ __forceinline__ int rows_between(int first, int end) { retur
 __host__ __device__ __forceinline__ Tokens tokens_at(int first, int rows, int length) {
     return {first, rows, std::min(std::max(length, 0), MOST_POSITIONS) - rows};
 }
+// Positions up to `seat` that have a place.
+__host__ __device__ __forceinline__ int seen_upto(int seat, int num_pages, int places) {
+    return num_pages ? std::min(std::max(seat + 1, 0), places) : 0;
+}
 
 // ---- units
 

@@ -120,9 +120,8 @@ __device__ __forceinline__ Tokens tokens_of(const PgParams& p, int b) {
     }
     return tokens_at(first, rows, p.lengths[b]);
 }
-// Positions up to `seat` that have a place.
 __device__ __forceinline__ int seen_from(const PgParams& p, int seat) {
-    return p.num_pages ? min(max(seat + 1, 0), p.places) : 0;
+    return seen_upto(seat, p.num_pages, p.places);
 }
 
 // The tokens of sequence `lane`, the first 64 together.

@@ -3,59 +3,71 @@
 // offsets (B + 1 numbers on the device, not decreasing) are where the sequences begin, and where the last one ends. The
 // host does not know them: a launch has room for every way of cutting T rows, and a workgroup finds its sequence here.
 // The rows are cut into B + 2 segments: what lies before the first sequence, the sequences, what lies behind the last
-// one. Segment j begins at row e(j); its blocks of `rows` rows (of `share` rows a token) have the numbers from
-//   e(j) share / rows (rounded down) + j
+// one. Segment j begins at row e(j); its blocks of `rows` rows have the numbers from
+//   e(j) / rows (rounded down) + j
 // on. That grows by at least one with j and by enough for the segment's blocks, since rounding down loses less than
-// one; so no sum over the segments before is needed, and T share / rows + B + 2 numbers are enough. Numbers between a
+// one; so no sum over the segments before is needed, and T / rows + B + 2 numbers are enough. Numbers between a
 // segment's last block and the next one's first have nothing to do. Rows are held to [0, T] whatever the offsets are.
 #pragma once
 
 #include <hip/hip_runtime.h>
+#include <algorithm>
 #include <cstdint>
 
 namespace qlka {
 
 struct Segment {
     int index;             // of its sequence; -1 and B for the rows outside
-    int first, rows;       // tokens: the first one, and how many
+    int first, rows;       // the first row, and how many
     int block;             // of the segment's rows
 };
 
-inline int64_t segment_blocks(int64_t T, int B, int share, int rows) { return T * share / rows + B + 2; }
+inline int64_t segment_blocks(int64_t T, int B, int rows) { return T / rows + B + 2; }
 
-__device__ __forceinline__ int segment_edge(const int* offsets, int B, int T, int j) {
-    return j <= 0 ? 0 : j <= B + 1 ? min(max(offsets[j - 1], 0), T) : T;
+__host__ __device__ __forceinline__ int segment_edge(const int* offsets, int B, int T, int j) {
+    return j <= 0 ? 0 : j <= B + 1 ? std::min(std::max(offsets[j - 1], 0), T) : T;
 }
 
 // The number of the first block of segment j.
-__device__ __forceinline__ int segment_start(int edge, int j, int share, int rows) {
-    return (int)((int64_t)edge * share / rows) + j;
-}
+__host__ __device__ __forceinline__ int segment_start(int edge, int j, int rows) { return edge / rows + j; }
+
+// A wave's lanes: how many f(lane) holds for, and what is the same in all of them.
+struct Lanes {
+    template <class F> __device__ __forceinline__ int count(F f) const {
+        return __popcll(__ballot(f((int)(threadIdx.x & 63))));
+    }
+    __device__ __forceinline__ int same(int x) const { return __builtin_amdgcn_readfirstlane(x); }
+};
 
 // The last j of [0, count) with at(j) <= x, which holds for j = 0 (at: not decreasing, x the same for all lanes), by a
-// wave that looks at 64 places at a time.
-template <class F> __device__ __forceinline__ int last_upto(int count, int x, F at) {
-    const int lane = threadIdx.x & 63;
+// wave that looks at 64 places at a time. Whatever at is, the result is in [-1, count) and at is asked for [0, count).
+template <class F, class L> __host__ __device__ __forceinline__ int last_upto(int count, int x, F at, L lanes) {
     int lo = 0, n = count;                             // the answer is in [lo - 1, lo + n)
     while (n > 64) {
-        const int step = (n + 63) / 64, i = lo + (lane + 1) * step - 1;
-        const int below = __popcll(__ballot(i < lo + n && at(i) <= x));
+        const int step = (n + 63) / 64;
+        const int below = lanes.count([&](int lane) {
+            const int i = lo + (lane + 1) * step - 1;
+            return i < lo + n && at(i) <= x;
+        });
         const int from = lo + below * step;
-        n = min(step - 1, lo + n - from);
+        n = std::min(step - 1, lo + n - from);
         lo = from;
     }
-    return lo + __popcll(__ballot(lane < n && at(lo + lane) <= x)) - 1;
+    return lo + lanes.count([&](int lane) { return lane < n && at(lo + lane) <= x; }) - 1;
+}
+template <class F> __device__ __forceinline__ int last_upto(int count, int x, F at) {
+    return last_upto(count, x, at, Lanes());
 }
 
-__device__ __forceinline__ Segment segment_of(const int* offsets, int B, int T, int share, int rows, int number) {
-    int j = last_upto(B + 2, number, [&](int i) {
-        return segment_start(segment_edge(offsets, B, T, i), i, share, rows); });
-    j = max(__builtin_amdgcn_readfirstlane(j), 0);
+template <class L>
+__host__ __device__ __forceinline__ Segment segment_of(const int* offsets, int B, int T, int rows, int number, L lanes) {
+    int j = last_upto(B + 2, number, [&](int i) { return segment_start(segment_edge(offsets, B, T, i), i, rows); }, lanes);
+    j = std::max(lanes.same(j), 0);
     Segment s;
     s.index = j - 1;
     s.first = segment_edge(offsets, B, T, j);
-    s.rows = max(segment_edge(offsets, B, T, j + 1) - s.first, 0);
-    s.block = number - segment_start(s.first, j, share, rows);
+    s.rows = std::max(segment_edge(offsets, B, T, j + 1) - s.first, 0);
+    s.block = number - segment_start(s.first, j, rows);
     return s;
 }
 

@@ -484,13 +484,13 @@ template <> struct Span<true> {
             // themselves, or half of the XCDs would have nothing to do (128 x 4 heads of 128, fp32: 39 us, 34 so).
             if ((number | 7) < p.blocks)
                 number = (number & ~7) | ((number + (((uint32_t)number >> 3) * 0x9e3779b1u >> 29)) & 7);
-            s = segment_of(p.offsets, p.sequences, p.M, 1, size, number);
+            s = segment_of(p.offsets, p.sequences, p.M, size, number, Lanes());
         }
         block = s.block;
         rows = s.rows;
         inside = s.index < 0 || s.index >= p.sequences ? 0 : s.rows;
         first = s.first;
-        group = segment_start(first, s.index + 1, 1, 32);
+        group = segment_start(first, s.index + 1, 32);
     }
     // The blocks in the order of their work, most first: a call ends with its last workgroups, and a long sequence's take a
     // hundred times as long as a short one's. A lane holds segments (segments.h) of n blocks each. In causal order a

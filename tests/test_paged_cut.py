@@ -47,7 +47,9 @@ def run(tmp_path, source, name, *flags):
     src, exe = tmp_path / f"{name}.hip", tmp_path / name
     src.write_text(source)
     subprocess.run([HIPCC, "--offload-host-only", "-std=c++17", "-O2", *flags, f"-I{CSRC}", str(src), "-o", str(exe)], check=True)
-    return subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()
+    done = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert done.returncode == 0, done.stdout + done.stderr
+    return done.stdout.split()
 
 
 def test_spans_do_not_go_by_what_the_compiler_fuses(tmp_path):
