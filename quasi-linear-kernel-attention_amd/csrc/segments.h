@@ -68,6 +68,7 @@ __host__ __device__ __forceinline__ Segment segment_of(const int* offsets, int B
     s.first = segment_edge(offsets, B, T, j);
     s.rows = std::max(segment_edge(offsets, B, T, j + 1) - s.first, 0);
     s.block = number - segment_start(s.first, j, rows);
+    if (s.block < 0) s.rows = s.block = 0;             // offsets that decrease: a vote of lanes is not the last of them
     return s;
 }
 

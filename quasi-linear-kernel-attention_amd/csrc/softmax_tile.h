@@ -486,9 +486,9 @@ template <> struct Span<true> {
                 number = (number & ~7) | ((number + (((uint32_t)number >> 3) * 0x9e3779b1u >> 29)) & 7);
             s = segment_of(p.offsets, p.sequences, p.M, size, number, Lanes());
         }
-        block = s.block;
-        rows = s.rows;
-        inside = s.index < 0 || s.index >= p.sequences ? 0 : s.rows;
+        block = max(s.block, 0);
+        rows = s.block < 0 ? 0 : s.rows;               // (sums of offsets that decrease can pass 32 bits)
+        inside = s.index < 0 || s.index >= p.sequences ? 0 : rows;
         first = s.first;
         group = segment_start(first, s.index + 1, 32);
     }
