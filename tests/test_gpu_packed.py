@@ -306,3 +306,15 @@ def test_gradients_divide_by_the_sum_of_whole_exponentials(dev, lengths):
     t["v"] = torch.randn(1, at[-1], 64, generator=gen).to(BF16)
     t["g"] = torch.randn(1, 1, 64, generator=gen).to(BF16).expand(1, at[-1], 64).contiguous()
     check(run(dev, t, at, causal=False, scale=1.0), reference(t, at, False, 1.0))
+
+
+@TYPES
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "whole"])
+@pytest.mark.parametrize("count", [200, 300])
+def test_one_long_sequence_among_short_ones(dev, count, causal, dtype):
+    """Workgroups of few waves, which the average length asks for, go through a sequence of many tiles; in the order of work,
+    and by number."""
+    lengths = [10, 0] * (count // 4) + [1300] + [9] * (count // 2)
+    at = offsets_of(lengths, 2)
+    t = make(4, 2, at[-1] + 3, 64, dtype, seed=count)
+    check(run(dev, t, at, causal=causal), reference(t, at, causal))

@@ -509,3 +509,39 @@ def test_nothing_to_do(dev, dtype, held):
     assert (paged_attention(x, bare, full, i32([1, 2, 3], dev)) == 0).all()
     assert (paged_attention(torch.ones(2, 90, 32, dtype=dtype, device=dev), bare, full[:1], i32([90], dev), i32([0, 90], dev)) == 0).all()
     assert (bare.read(full, i32([1, 2, 3], dev), 4)[0] == 0).all()
+
+
+@pytest.mark.parametrize("dtype,held", [(F32, F32), (BF16, BF16), (BF16, I8)], ids=["fp32", "bf16", "bf16_int8"])
+@pytest.mark.parametrize("B", [193, 256, 257, 319, 320, 321])
+@pytest.mark.parametrize("kind", ["tokens", "mixed"])
+def test_as_many_sequences_as_are_looked_up_at_once(dev, kind, B, dtype, held):
+    """The last ones that every workgroup looks up by itself (320), and the first that a kernel does before the others."""
+    gen = torch.Generator().manual_seed(B)
+    new = [1] * B
+    if kind == "mixed":
+        new[0], new[255 % B], new[B - 2], new[B - 1] = 0, 50, 70, 30
+    lengths = [n + m for n, m in zip(new, torch.randint(0, 20, (B,), generator=gen).tolist())]
+    lengths[B - 1], lengths[192] = 1500, 900                # in parts
+    offsets = sums(new, 1)
+    tables, num_pages = tables_of(lengths, 16, gen)
+    cache, cpu = filled(num_pages, 16, 2, 64, dtype, held, gen, dev)
+    q = torch.randn(4, offsets[-1] + 2, 64, generator=gen).to(dtype)
+    want, bound = oracle.attention(q, *cpu, held, tables, lengths, offsets, 0.125)
+    got = attend(dev, q, cache, tables, lengths, offsets)
+    close(got, want, bound)
+    assert (got[:, :1] == 0).all() and (got[:, offsets[-1]:] == 0).all()
+
+
+@KINDS
+@pytest.mark.parametrize("chunk", [500, 520])
+def test_tokens_beside_one_chunk(dev, chunk, dtype, held):
+    """A chunk that takes its tokens to the tiles (12 / 4 heads, six sequences: from 512 on), and one that does not."""
+    gen = torch.Generator().manual_seed(chunk)
+    new = [1, 1, chunk - 5, 1, 1, 1]
+    lengths = [1, 700, 900, 33, 400, 64]
+    offsets = sums(new)
+    tables, num_pages = tables_of(lengths, 32, gen)
+    cache, cpu = filled(num_pages, 32, 4, 64, dtype, held, gen, dev)
+    q = torch.randn(12, offsets[-1], 64, generator=gen).to(dtype)
+    want, bound = oracle.attention(q, *cpu, held, tables, lengths, offsets, 0.125)
+    close(attend(dev, q, cache, tables, lengths, offsets), want, bound)
