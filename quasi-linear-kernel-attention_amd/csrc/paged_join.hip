@@ -75,7 +75,12 @@ template <class T, int DP, bool MANY> __global__ __launch_bounds__(256) void pag
             const float z = weight(s);
             if (s < count) x = x + y[e] * z;
         }
-        for (int s = first + EARLY * AT_ONCE; s < count; s += AT_ONCE) x = x + from(s) * weight(s);
+        // (all lanes go on to the last part: the one that holds its weight may have none left itself)
+        for (int e = EARLY; e * AT_ONCE < count; ++e) {
+            const int s = first + e * AT_ONCE;
+            const float z = weight(s);
+            if (s < count) x = x + from(s) * z;
+        }
     };
 #pragma unroll 1
     for (int s0 = 0; s0 < parts; s0 += LOOK) {

@@ -545,3 +545,20 @@ def test_tokens_beside_one_chunk(dev, chunk, dtype, held):
     q = torch.randn(12, offsets[-1], 64, generator=gen).to(dtype)
     want, bound = oracle.attention(q, *cpu, held, tables, lengths, offsets, 0.125)
     close(attend(dev, q, cache, tables, lengths, offsets), want, bound)
+
+
+@pytest.mark.parametrize("dtype,held", [(F32, F32), (BF16, BF16), (BF16, I8)], ids=["fp32", "bf16", "bf16_int8"])
+@pytest.mark.parametrize("parts,new,heads", [(n, [1], (1, 1, 128)) for n in (3, 17, 31, 33, 34, 47, 63, 64, 65, 99, 127)]
+                         + [(n, [2], (2, 1, 80)) for n in (33, 49)] + [(n, [1], (2, 1, 64)) for n in (33, 65)]
+                         + [(n, [1], (1, 1, 32)) for n in (9, 71)] + [(n, [40], (1, 1, 128)) for n in (33, 35)], ids=str)
+def test_every_number_of_parts(dev, parts, new, heads, dtype, held):
+    """Parts of 128 positions (256 with chunks), odd numbers of them too, which the lanes that add them up share unevenly."""
+    H, G, D = heads
+    gen = torch.Generator().manual_seed(parts)
+    lengths = [(128 if new[0] < 16 else 256) * parts - 5]
+    offsets = sums(new)
+    tables, num_pages = tables_of(lengths, 64, gen)
+    cache, cpu = filled(num_pages, 64, G, D, dtype, held, gen, dev)
+    q = torch.randn(H, offsets[-1], D, generator=gen).to(dtype)
+    want, bound = oracle.attention(q, *cpu, held, tables, lengths, offsets, D ** -0.5)
+    close(attend(dev, q, cache, tables, lengths, offsets), want, bound)
