@@ -35,21 +35,28 @@ int check_sizes(const qlka_paged_args* a) {
 // tokens: 59 and 55), others have to be taken apart or turned into bf16 (fp32, 4 sequences of up to 8000, 6 to 12 tokens:
 // 24 us with 32, 39 with 16; e4m3, 12 / 12 heads, 12 to 24 tokens: 120 and 128).
 int few_rows(const qlka_paged_args* a) { return a->held == QLKA_BF16 ? 16 : 32; }
-// Workgroups of a launch: one round of those that registers leave room for. Two a compute unit of fp32 and of rows of 128
-// (tokens of 16 sequences of 2000 to 8192: 8 heads of 128, int8 41 us, 50 with 768, 47 with 1024; bf16 54, 57 with 1536;
-// fp32, 12 heads of 64, 97, 107 with 768 or 1536; chunks of 512, 8 / 2 heads of 128, int8: 83, 91 with 768); three of bf16
-// rows of 64 (12 / 4 heads 20.7 us, 24.5 with 1536; 12 heads, cold pages, 50.4 and 51.5); four of 8 bits and of rows of 32 (12
-// heads of 64, int8: 31.1 us, 33.2 with 768). Beside tiles more and smaller ones fill what those leave (64 of up to 8192, 8
-// with chunks of 512, 12 heads of 64: bf16 162 us, 178 with one round; int8 146 and 160; 24 of 500 to 5000, fp32: 57, 60
-// with three rounds).
+// Workgroups of a launch: one round of those that registers and LDS leave room for.
+// One a compute unit for fp32 rows of 128 where they are held so (96 KB of LDS) or go through tiles (372 to 388 registers;
+// tokens of 16 sequences of 2000 to 8192, 8 / 2 heads: 45 us, 65 with two; 8 heads 145 either way; 4 chunks of 256, 8 / 2 heads,
+// fp32 115 and 119, int8 79 and 85; two of 200 among 16, fp32 86 and 100, int8 58 and 70).
+bool one(const qlka_paged_args* a, bool tiles) {
+    return a->dtype == QLKA_F32 && sm_padded(a->D) == 128 && (tiles || !coded(a));
+}
+// Two of other fp32 and of rows of 128 (tokens of 16 sequences of 2000 to 8192: 8 heads of 128, int8 41 us, 50 with 768, 47 with
+// 1024; bf16 54, 57 with 1536; fp32, 12 heads of 64, 97, 107 with 768 or 1536; chunks of 512, 8 / 2 heads of 128, int8:
+// 83, 91 with 768); three of bf16 rows of 64 (12 / 4 heads 20.7 us, 24.5 with 1536; 12 heads, cold pages, 50.4 and 51.5);
+// four of 8 bits and of rows of 32 (12 heads of 64, int8: 31.1 us, 33.2 with 768). Beside tiles more and smaller ones fill
+// what those leave (64 of up to 8192, 8 with chunks of 512, 12 heads of 64: bf16 162 us, 178 with one round; int8 146 and
+// 160; 24 of 500 to 5000, fp32: 57, 60 with three rounds).
 bool two(const qlka_paged_args* a) { return a->dtype == QLKA_F32 || sm_padded(a->D) == 128; }
 int64_t step_groups(const qlka_paged_args* a, bool tiles) {
+    if (one(a, tiles)) return 256;
     if (two(a)) return tiles ? 768 : 512;
     return tiles ? 1536 : coded(a) || sm_padded(a->D) == 32 ? 1024 : 768;
 }
 // Tiles alone: three a compute unit (4 chunks of 512 at up to 8192, int8, 12 / 4 heads: 68 us; 71 with two, 80 with six), beside
 // tokens two, so that those have a third (32 sequences, two with chunks of 700: 46 us for 50).
-int64_t tile_groups(const qlka_paged_args* a, bool step) { return two(a) || step ? 512 : 768; }
+int64_t tile_groups(const qlka_paged_args* a, bool step) { return one(a, true) ? 256 : two(a) || step ? 512 : 768; }
 // The least positions of a part: a turn of the step kernel's waves (one sequence of 2000, int8, 12 / 4 heads: 9.3 us; 10.6 with
 // 256, 17.4 as one), a few tiles of the others (300 tokens of it: 20.1 us; 24.4 with 128, 23.2 with 512). A call whose
 // tables have no room for more than so many positions is not cut at all, which saves joining (one sequence of 250: 7.0 us

@@ -169,6 +169,17 @@ def test_workspace_of_a_chunk_among_many_tokens(lib, H, G, D):
     assert need(B=2000, T=20) <= need(B=20, T=20) + (1 << 20)
 
 
+def test_one_round_of_workgroups(lib):
+    """fp32 rows of 128: a compute unit has room for one workgroup (96 KB of LDS, or more than 256 registers), so parts are
+    cut, and have places, for 256 of them."""
+    sizes = dict(dtype=0, H=8, G=8, D=128, T=1, B=1, offsets=None, table_len=4096)
+    pages = {n + "_stride": (16 * 8 * 128, 16 * 128, 128) for n in ("k_pages", "v_pages")}
+    place = 16 * (128 + 2) * 4
+    need = lambda held: lib.qlka_paged_attention_ws_bytes(ctypes.byref(args(held=held, **sizes, **pages)))  # noqa: E731
+    assert 250 * place < need(0) <= (256 + 2 * 8) * place + 512
+    assert need(2) > 500 * place                            # of 8 bits: two
+
+
 def test_nothing_to_do(lib):
     a = args(B=0, T=0, N=0, offsets=None, tables=None, lengths=None, q=None, k=None, v=None, out=None, out_k=None, out_v=None)
     for name, call in calls(lib, ctypes.byref(a)).items():
