@@ -486,16 +486,17 @@ template <> struct Span<true> {
                 number = (number & ~7) | ((number + (((uint32_t)number >> 3) * 0x9e3779b1u >> 29)) & 7);
             s = segment_of(p.offsets, p.sequences, p.M, size, number, Lanes());
         }
-        block = max(s.block, 0);
-        rows = s.block < 0 ? 0 : s.rows;               // (sums of offsets that decrease can pass 32 bits)
-        inside = s.index < 0 || s.index >= p.sequences ? 0 : rows;
+        block = s.block;
+        rows = s.rows;
+        inside = s.index < 0 || s.index >= p.sequences ? 0 : s.rows;
         first = s.first;
         group = segment_start(first, s.index + 1, 32);
     }
     // The blocks in the order of their work, most first: a call ends with its last workgroups, and a long sequence's take a
     // hundred times as long as a short one's. A lane holds segments (segments.h) of n blocks each. In causal order a
     // sequence has a block with 1, 2, .. n blocks to go through, so that sum(max(n - x, 0)) blocks have more than x;
-    // else n with n each, and sum(n where n > x) do. x is found bit by bit. No sequence's blocks leave out numbers.
+    // else n with n each, and sum(n where n > x) do. x is found bit by bit. No sequence's blocks leave out numbers. Offsets
+    // that decrease count rows twice, but every second segment is then empty: sums of n stay below 2^31 all the same.
     static constexpr int EACH = 4, HEAVY_FIRST = 64 * EACH - 2;       // segments of a lane at most; sequences
     static __device__ __forceinline__ int sum_of(int x) {
         x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);           // row_shr 1, 2, 4, 8
