@@ -301,19 +301,19 @@ int qlka_bias_map_bwd(const float* g, const int* border, int num_borders, int bi
 
 /*
  * Softmax attention within sequences of different lengths that lie one after the other in T rows (no padding). offsets
- * (B + 1 numbers on the device, not decreasing, in [0, T]) are where the sequences begin, and where the last one ends: a
- * row sees the keys of its own sequence, with causal those up to itself. Rows outside every sequence get zeros, here and
- * in every gradient. No sequence changes another one's results, whatever it holds. No counterpart in the reference.
+ * (B + 1 numbers on the device, not decreasing, in [0, T]) are where the sequences begin, and where the last one ends:
+ * a row sees the keys of its own sequence, with causal those up to itself. Rows outside every sequence get zeros, here
+ * and in every gradient. No sequence changes another one's results, whatever it holds. No counterpart in the reference.
  *
  *   out[h,m] = sum_n P[m,n] v[h/(H/G),n],  P = softmax of scale <q[h,m], k[h/(H/G),n]> over the keys n that m sees
  *
  * q (H, T, D), k and v (G, T, D); *_stride are the distances in elements between heads and rows. Types, D, alignment,
  * scale, roundings, lse, log_sums (2, H, T), out_full (H, T, D) and the gradients are as for qlka_softmax_fwd / _bwd
- * without a table, but that log_sums are those of the exponentials before their rounding to bf16: no other error than its
- * own rounding is in a probability of the gradients (where keys are split, out can then differ in its last place from
- * that of a call without log_sums). Offsets that decrease give rows that are not said, but no access
- * outside the tensors. The offsets may change between the replays of a captured call. A launch takes less than 2^32
- * threads: heads * (T / 32 + B) stays below 2^24.
+ * without a table, but that log_sums are those of the exponentials before their rounding to bf16: a probability of the
+ * gradients has no other error than its own rounding (where keys are split, out can then differ in its last place from
+ * that of a call without log_sums). Offsets that decrease give rows that are not said, but no access outside the
+ * tensors. The offsets may change between the replays of a captured call. A launch takes less than 2^32 threads, so
+ * heads * (T / 32 + B) stays below 2^24.
  */
 typedef struct qlka_packed_args {
     int dtype, B, H, G, T, D;
@@ -338,35 +338,36 @@ int qlka_packed_bwd(const qlka_packed_args* args, void* ws, size_t ws_bytes, voi
 
 /*
  * A cache of keys and values in pages. A sequence's token at position i is row i % page_size of page
- * tables[b][i / page_size]; pages are rows of D elements for each of G key heads, at any strides (elements, between pages,
- * heads and rows, each below 2^32 bytes). What is held (held):
+ * tables[b][i / page_size]; pages are rows of D elements for each of G key heads, at any strides (elements, between
+ * pages, heads and rows, each below 2^32 bytes). What is held (held):
  *   QLKA_F32, QLKA_BF16  the rows as they are; of the type of the call (dtype) only
- *   QLKA_INT8, QLKA_E4M3 8 bits an element, and for every 32 elements of a row a byte e (k_exp, v_exp: ceil(D / 32) a row,
- *                        contiguous; strides in bytes between pages, heads and rows): an element stands for
+ *   QLKA_INT8, QLKA_E4M3 8 bits an element, and for every 32 elements of a row a byte e (k_exp, v_exp: ceil(D / 32) a
+ *                        row, contiguous; strides in bytes between pages, heads and rows): an element stands for
  *                        code * 2^(e - 127). e is the least of [27, 248] (int8; 246 with e4m3) with which the largest
  *                        code (127; 448) reaches the largest element, the codes are the nearest ones, ties to the
  *                        even one. Such values are exact in bf16 and fp32, so nothing is rounded a second time when
  *                        they are read. e = 255 marks 32 elements of which one was infinite or NaN: all read as NaN.
  *
  * tables: B rows of table_len page numbers, table_stride apart; lengths: B numbers of tokens, the new ones included;
- * offsets (B + 1): the new tokens of the sequences one after the other in T rows, or NULL: one for each, T = B. All on the
- * device; their contents may change between the replays of a captured call. Row m of sequence b is at position
+ * offsets (B + 1): the new tokens of the sequences one after the other in T rows, or NULL: one for each, T = B. All on
+ * the device; their contents may change between the replays of a captured call. Row m of sequence b is at position
  * lengths[b] - (offsets[b + 1] - m). Page numbers outside [0, num_pages), and what a table's row has no place for, are
  * pages that do not exist: nothing is written there, keys there are not seen, reading gives zeros.
  *
- * qlka_paged_write: the new tokens' k and v (G, T, D) go to their positions. Rows outside every sequence, or at negative
- *   positions, are left out; nothing else in the pages changes. Two rows of one call at one place in a page leave either
- *   one's values, or parts of both.
- * qlka_paged_read: out_k and out_v (B, G, N, D) of dtype get the first N positions of each sequence, zeros from lengths[b]
- *   on.
- * qlka_paged_attention: out (H, T, D), softmax attention of the new tokens q (H, T, D) to their sequence's held keys up to
- *   their own position, which have been written before. Rows that see none, and rows outside every sequence, get zeros.
+ * qlka_paged_write: the new tokens' k and v (G, T, D) go to their positions. Rows outside every sequence, or at
+ *   negative positions, are left out; nothing else in the pages changes. Two rows of one call at one place in a page
+ *   leave either one's values, or parts of both.
+ * qlka_paged_read: out_k and out_v (B, G, N, D) of dtype get the first N positions of each sequence, zeros from
+ *   lengths[b] on.
+ * qlka_paged_attention: out (H, T, D), softmax attention of the new tokens q (H, T, D) to their sequence's held keys up
+ *   to their own position, which have been written before. Rows that see none, and rows outside every sequence, get
+ *   zeros.
  *   longest: the most new tokens of a sequence if the caller knows it, else 0. It only decides which kernels run.
  *
- * Strides are in elements between heads and rows ((B, heads, rows) for out_k and out_v); D a multiple of 8 up to 128, rows
- * at multiples of 16 bytes (in pages of 8 bits with D no multiple of 16: of 8 bytes). The scale is as for
- * qlka_softmax_fwd, the probabilities are rounded to bf16 for their product where q is. Infinities and NaN that a sequence
- * holds at its new tokens' positions or before can make any of its new rows NaN, no other sequence's.
+ * Strides are in elements between heads and rows ((B, heads, rows) for out_k and out_v); D a multiple of 8 up to 128,
+ * rows at multiples of 16 bytes (in pages of 8 bits with D no multiple of 16: of 8 bytes). The scale is as for
+ * qlka_softmax_fwd, the probabilities are rounded to bf16 for their product where q is. Infinities and NaN that a
+ * sequence holds at its new tokens' positions or before can make any of its new rows NaN, no other sequence's.
  */
 #define QLKA_INT8 2
 #define QLKA_E4M3 3

@@ -1,4 +1,5 @@
-"""Softmax attention within packed sequences in float64, with its gradients and bounds: oracle/softmax.py sequence by sequence.
+"""Softmax attention within packed sequences in float64, with its gradients and bounds: oracle/softmax.py, sequence by
+sequence.
 TEST INFRASTRUCTURE ONLY.
 """
 
@@ -8,8 +9,8 @@ from . import softmax
 
 
 def attention(q, k, v, offsets, scale, causal, g=None):
-    """q (H, T, D), k and v (G, T, D), offsets a list: {"out", "gq", "gk", "gv"} and their "bound"; rows outside the sequences are
-    zeros with the bound 0."""
+    """q (H, T, D), k and v (G, T, D), offsets a list: {"out", "gq", "gk", "gv"} and their "bound"; rows outside the
+    sequences are zeros with the bound 0."""
     names = ("out",) if g is None else ("out", "gq", "gk", "gv")
     like = {"out": q, "gq": q, "gk": k, "gv": v}
     r = {n: torch.zeros(like[n].shape, dtype=torch.float64) for n in names}

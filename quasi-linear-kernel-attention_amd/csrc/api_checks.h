@@ -1,4 +1,5 @@
-// What the host sides of the softmax kernels share: refusals, workspaces, grids and splits. Not part of the public interface.
+// What the host sides of the softmax kernels share: refusals, workspaces, grids and splits. Not part of the public
+// interface.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -40,8 +41,9 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // workgroups on a CU (one alone on a CU is not twice as fast as two, waits not being filled), each its tiles and what
 // it costs by itself, and the joining of `join` bytes a split. In microseconds, the constants set by hand until 12
 // shapes (prompts and gradients of 65 to 8192 keys, fp32 and bf16) came near the best of 1 to 16 splits of all their
-// axes: eight of them within 4% of it or faster (1 x 4 heads, 100 x 8000: 14.4 us, 17.2 the best one number, 132 unsplit),
-// the others 7 to 18% slower (1 x 12, 512 x 4096: 26.8 : 23.7, unsplit 70; 4 x 12, 1024 x 4096: 91 : 77, unsplit 88).
+// axes: eight of them within 4% of it or faster (1 x 4 heads, 100 x 8000: 14.4 us, 17.2 the best one number, 132
+// unsplit), the others 7 to 18% slower (1 x 12, 512 x 4096: 26.8 : 23.7, unsplit 70; 4 x 12, 1024 x 4096: 91 : 77,
+// unsplit 88).
 inline int splits_for(int64_t groups, int64_t tiles, double tile_us, double join_bytes) {
     int best = 1;
     double least = 0;

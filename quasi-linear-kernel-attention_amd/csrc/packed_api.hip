@@ -21,17 +21,20 @@ int check_sizes(const qlka_packed_args* a) {
 // ---- how a call runs
 
 int tile_rows(const qlka_packed_args* a) { return sm_tile_rows(a->dtype == QLKA_F32 ? 3 : 1, sm_padded(a->D)); }
-// The host does not know the lengths: waves go by the average one, and splits by twice that, since the longest sequence's
-// workgroups are what a call waits for (64 sequences of 65 to 600, fp32 training: 313 us by the average, 273 by twice or
-// three times that; calls of many workgroups are not split either way).
+// The host does not know the lengths: waves go by the average one, and splits by twice that, since the longest
+// sequence's workgroups are what a call waits for (64 sequences of 65 to 600, fp32 training: 313 us by the average, 273
+// by twice or three times that; calls of many workgroups are not split either way). Lengths far from the average are
+// not served well (12 heads of 64, causal, bf16 / fp32): one of 4096 among 300 of 10 takes 136 / 519 us, 381 / 1729
+// with the gradients (alone 70 / 271, 265 / 970), since its blocks are of one wave or two and not in the order of their
+// work; four of 2048 with 300 empty sequences 111 / 400 and 291 / 1290 (without those 46 / 167, 181 / 849).
 int64_t average(const qlka_packed_args* a) { return ceil_div(a->T, std::max(a->B, 1)); }
 int64_t longest(const qlka_packed_args* a) { return std::min<int64_t>(2 * average(a), a->T); }
 
 struct Plan { int waves, blocks, splits; };
-// Workgroups of `few` waves where sequences have no rows for more, unless they are less than the GPU has room for at once (two
-// a compute unit, one of fp32 rows of 128): then waves without rows help to bring the others' (fp32 training, 12 heads of
-// 64 of 8 to 30 rows: 16 sequences 27 us with all waves, 30 with few; 64: 52 and 46; 1000: 641 and 475; 12 heads of 80 of 30
-// to 60 rows: 16 sequences 58 and 65, 25 111 and 88).
+// Workgroups of `few` waves where sequences have no rows for more, unless they are less than the GPU has room for at
+// once (two a compute unit, one of fp32 rows of 128): then waves without rows help to bring the others' (fp32 training,
+// 12 heads of 64 of 8 to 30 rows: 16 sequences 27 us with all waves, 30 with few; 64: 52 and 46; 1000: 641 and 475; 12
+// heads of 80 of 30 to 60 rows: 16 sequences 58 and 65, 25 111 and 88).
 Plan plan(const qlka_packed_args* a, int heads, int64_t tiles, double products, int few) {
     Plan r;
     const int64_t room = a->dtype == QLKA_F32 && sm_padded(a->D) == 128 ? 256 : 512;

@@ -1,5 +1,5 @@
-// A cache of keys and values in pages and the attention that reads it: what the host side (paged_api.hip) and the kernel
-// files share. Not part of the public interface.
+// A cache of keys and values in pages and the attention that reads it: what the host side (paged_api.hip) and the
+// kernel files share. Not part of the public interface.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -14,8 +14,9 @@ namespace qlka {
 struct PgStrides { uint32_t page, head, row; };                // of pages, in bytes (one instruction a product)
 struct PgOut { int64_t b, h, r; };
 
-// How a launch's work is cut (paged_device.h): workgroups aimed at for each key head, the least positions of a part, the
-// launch's size, and where the parts' sums go: [unit][rows of a block][padded D], and [unit][rows][2] (reference, sum).
+// How a launch's work is cut (paged_device.h): workgroups aimed at for each key head, the least positions of a part,
+// the launch's size, and where the parts' sums go: [unit][rows of a block][padded D], and [unit][rows][2] (reference,
+// sum).
 struct PgUnits {
     float aim;
     int least, groups;
@@ -39,7 +40,7 @@ struct PgParams {
     int places;                              // positions that a table's row has pages for
     pg::Division page_division;
     float scale, q_sign;                     // |scale|; its sign (or 0)
-    PgUnits step, tiles;                     // few rows (paged_step.h) and chunks (paged_tiles.h); groups 0: not in this call
+    PgUnits step, tiles;                     // few rows (paged_step.h), chunks (paged_tiles.h); groups 0: not in a call
     int few;                                 // sequences of more rows a key head are the tiles'
     int blocks;                              // of rows (paged_read)
 };

@@ -15,7 +15,8 @@ int check_sizes(const qlka_paged_args* a) {
     if (!a) return refuse("args must be non-null");
     if (a->dtype != QLKA_F32 && a->dtype != QLKA_BF16) return refuse("dtype must be QLKA_F32 or QLKA_BF16");
     if (!coded(a) && a->held != a->dtype) return refuse("held must be dtype, QLKA_INT8 or QLKA_E4M3");
-    if (a->B < 0 || a->T < 0 || a->N < 0 || a->H < 1 || a->G < 1) return refuse("B, T and N must be >= 0, H and G >= 1");
+    if (a->B < 0 || a->T < 0 || a->N < 0 || a->H < 1 || a->G < 1)
+        return refuse("B, T and N must be >= 0, H and G >= 1");
     if (a->H % a->G) return refuse("H must be a multiple of G");
     if (a->D < 8 || a->D > 128 || a->D % 8) return refuse("D must be a multiple of 8 in [8, 128]");
     if (a->T > LONGEST || a->B > LONGEST || a->N > LONGEST) return refuse("B, T and N must be <= 2^28");
@@ -30,41 +31,41 @@ int check_sizes(const qlka_paged_args* a) {
 
 // ---- how a call runs
 
-// Sequences of up to so many rows a key head go through the step kernel, 16 at a time, others through the tiles. bf16 rows
-// come as fast to a tile (32 sequences of up to 16384 with 4 to 8 tokens, 12 / 4 heads: 45 us with 16, 57 with 32; 8 to 16
-// tokens: 59 and 55), others have to be taken apart or turned into bf16 (fp32, 4 sequences of up to 8000, 6 to 12 tokens:
-// 24 us with 32, 39 with 16; e4m3, 12 / 12 heads, 12 to 24 tokens: 120 and 128).
+// Sequences of up to so many rows a key head go through the step kernel, 16 at a time, others through the tiles. bf16
+// rows come as fast to a tile (32 sequences of up to 16384 with 4 to 8 tokens, 12 / 4 heads: 45 us with 16, 57 with 32;
+// 8 to 16 tokens: 59 and 55), others have to be taken apart or turned into bf16 (fp32, 4 sequences of up to 8000, 6 to
+// 12 tokens: 24 us with 32, 39 with 16; e4m3, 12 / 12 heads, 12 to 24 tokens: 120 and 128).
 int few_rows(const qlka_paged_args* a) { return a->held == QLKA_BF16 ? 16 : 32; }
 // Workgroups of a launch: one round of those that registers and LDS leave room for.
-// One a compute unit for fp32 rows of 128 where they are held so (96 KB of LDS) or go through tiles (372 to 388 registers;
-// tokens of 16 sequences of 2000 to 8192, 8 / 2 heads: 45 us, 65 with two; 8 heads 145 either way; 4 chunks of 256, 8 / 2 heads,
-// fp32 115 and 119, int8 79 and 85; two of 200 among 16, fp32 86 and 100, int8 58 and 70).
+// One a compute unit for fp32 rows of 128 where they are held so (96 KB of LDS) or go through tiles (372 to 388
+// registers; tokens of 16 sequences of 2000 to 8192, 8 / 2 heads: 45 us, 65 with two; 8 heads 145 either way; 4 chunks
+// of 256, 8 / 2 heads, fp32 115 and 119, int8 79 and 85; two of 200 among 16, fp32 86 and 100, int8 58 and 70).
 bool one(const qlka_paged_args* a, bool tiles) {
     return a->dtype == QLKA_F32 && sm_padded(a->D) == 128 && (tiles || !coded(a));
 }
-// Two of other fp32 and of rows of 128 (tokens of 16 sequences of 2000 to 8192: 8 heads of 128, int8 41 us, 50 with 768, 47 with
-// 1024; bf16 54, 57 with 1536; fp32, 12 heads of 64, 97, 107 with 768 or 1536; chunks of 512, 8 / 2 heads of 128, int8:
-// 83, 91 with 768); three of bf16 rows of 64 (12 / 4 heads 20.7 us, 24.5 with 1536; 12 heads, cold pages, 50.4 and 51.5);
-// four of 8 bits and of rows of 32 (12 heads of 64, int8: 31.1 us, 33.2 with 768). Beside tiles more and smaller ones fill
-// what those leave (64 of up to 8192, 8 with chunks of 512, 12 heads of 64: bf16 162 us, 178 with one round; int8 146 and
-// 160; 24 of 500 to 5000, fp32: 57, 60 with three rounds).
+// Two of other fp32 and of rows of 128 (tokens of 16 sequences of 2000 to 8192: 8 heads of 128, int8 41 us, 50 with
+// 768, 47 with 1024; bf16 54, 57 with 1536; fp32, 12 heads of 64, 97, 107 with 768 or 1536; chunks of 512, 8 / 2 heads
+// of 128, int8: 83, 91 with 768); three of bf16 rows of 64 (12 / 4 heads 20.7 us, 24.5 with 1536; 12 heads, cold pages,
+// 50.4 and 51.5); four of 8 bits and of rows of 32 (12 heads of 64, int8: 31.1 us, 33.2 with 768). Beside tiles more
+// and smaller ones fill what those leave (64 of up to 8192, 8 with chunks of 512, 12 heads of 64: bf16 162 us, 178 with
+// one round; int8 146 and 160; 24 of 500 to 5000, fp32: 57, 60 with three rounds).
 bool two(const qlka_paged_args* a) { return a->dtype == QLKA_F32 || sm_padded(a->D) == 128; }
 int64_t step_groups(const qlka_paged_args* a, bool tiles) {
     if (one(a, tiles)) return 256;
     if (two(a)) return tiles ? 768 : 512;
     return tiles ? 1536 : coded(a) || sm_padded(a->D) == 32 ? 1024 : 768;
 }
-// Tiles alone: three a compute unit (4 chunks of 512 at up to 8192, int8, 12 / 4 heads: 68 us; 71 with two, 80 with six), beside
-// tokens two, so that those have a third (32 sequences, two with chunks of 700: 46 us for 50).
+// Tiles alone: three a compute unit (4 chunks of 512 at up to 8192, int8, 12 / 4 heads: 68 us; 71 with two, 80 with
+// six), beside tokens two, so that those have a third (32 sequences, two with chunks of 700: 46 us for 50).
 int64_t tile_groups(const qlka_paged_args* a, bool step) { return one(a, true) ? 256 : two(a) || step ? 512 : 768; }
-// The least positions of a part: a turn of the step kernel's waves (one sequence of 2000, int8, 12 / 4 heads: 9.3 us; 10.6 with
-// 256, 17.4 as one), a few tiles of the others (300 tokens of it: 20.1 us; 24.4 with 128, 23.2 with 512). A call whose
-// tables have no room for more than so many positions is not cut at all, which saves joining (one sequence of 250: 7.0 us
-// for 9.3; of 500: 9.2 either way).
+// The least positions of a part: a turn of the step kernel's waves (one sequence of 2000, int8, 12 / 4 heads: 9.3 us;
+// 10.6 with 256, 17.4 as one), a few tiles of the others (300 tokens of it: 20.1 us; 24.4 with 128, 23.2 with 512). A
+// call whose tables have no room for more than so many positions is not cut at all, which saves joining (one sequence
+// of 250: 7.0 us for 9.3; of 500: 9.2 either way).
 constexpr int64_t STEP_LEAST = 128, TILE_LEAST = 256, STEP_WHOLE = 512, TILE_WHOLE = 256;
 
-// The units of more sequences than a workgroup looks up by itself are found once, by a kernel before the others (512 of 100
-// to 1000, 12 / 4 heads, bf16: 52 us for 57; 2000 of 100 to 500, int8: 106 for 278; but 256: 36 for 34).
+// The units of more sequences than a workgroup looks up by itself are found once, by a kernel before the others (512 of
+// 100 to 1000, 12 / 4 heads, bf16: 52 us for 57; 2000 of 100 to 500, int8: 106 for 278; but 256: 36 for 34).
 bool many(const qlka_paged_args* a) { return a->B > PG_LOOKED_UP; }
 
 struct Plan {
@@ -84,7 +85,12 @@ Plan plan(const qlka_paged_args* a) {
     if (!a->offsets || longest * share <= few) {
         r.tiles = false;
         r.few = INT32_MAX;
-    } else if (a->T * share >= 256 * std::max<int64_t>(a->B, 1)) {       // chunks, on the average: a token among them takes a tile too
+    } else if (a->T * share >= 256 * std::max<int64_t>(a->B, 1)) {
+        // Chunks, on the average: tiles alone, for tokens among them too. Measured both ways, bf16, one chunk among
+        // tokens at up to 8192, tiles alone and both kinds: the average is not what tells which is faster. 12 / 4
+        // heads, 2800 and 31 tokens: 90 and 60 us; 700 and 7: 55 and 51; 2048 and 7: 38 and 42; 4096 and 15: 82 and
+        // 102; 12 heads, 2048 and 7: 133 and 108; 4096 and 15: 130 and 106. (int8: 106 and 65, 65 and 55, 45 and 48, 98
+        // and 122, 155 and 133, 165 and 131.)
         r.step = false;
         r.few = -1;
     }
@@ -165,10 +171,12 @@ int params(const qlka_paged_args* a, PgParams* p) {
     if (coded(a) && a->num_pages) {
         if (!a->k_exp || !a->v_exp) return refuse("k_exp and v_exp must be non-null where 8 bits are held");
         for (int i = 0; i < 3; ++i)
-            if (sizes[i] > 1 && ((uint64_t)a->k_exp_stride[i] > UINT32_MAX || (uint64_t)a->v_exp_stride[i] > UINT32_MAX))
+            if (sizes[i] > 1 &&
+                ((uint64_t)a->k_exp_stride[i] > UINT32_MAX || (uint64_t)a->v_exp_stride[i] > UINT32_MAX))
                 return refuse("the strides of k_exp and v_exp must be in [0, 2^32)");
     }
-    if (a->B > 0 && (!a->lengths || (a->table_len > 0 && !a->tables))) return refuse("tables and lengths must be non-null");
+    if (a->B > 0 && (!a->lengths || (a->table_len > 0 && !a->tables)))
+        return refuse("tables and lengths must be non-null");
     if (a->B > 1 && a->table_stride < 0) return refuse("table_stride must not be negative");
     return QLKA_OK;
 }

@@ -1,7 +1,7 @@
 // Attention of new tokens over a cache in pages: the kernels. A launch has workgroups for sequences of few rows
 // (paged_step.h), for chunks (paged_tiles.h), or for both: a batch of chunks and tokens is one launch, in which the one
-// kind fills the compute units that the other leaves (32 sequences of 12 / 4 heads, two with chunks: 66 us one after the
-// other, 54 in one launch). The last workgroups write the rows outside every sequence.
+// kind fills the compute units that the other leaves (32 sequences of 12 / 4 heads, two with chunks: 66 us one after
+// the other, 54 in one launch). The last workgroups write the rows outside every sequence.
 #pragma once
 
 #include "paged_step.h"
@@ -11,9 +11,8 @@ namespace qlka {
 namespace pg {
 
 template <class T, class C, int DP, int EL, bool STEP, bool TILES> constexpr int room() {
-    return STEP && TILES ? (step_room<T, C, DP>() < tiles_room<T, C, DP>() ? step_room<T, C, DP>() : tiles_room<T, C, DP>())
-           : STEP        ? step_room<T, C, DP>()
-                         : tiles_room<T, C, DP>();
+    constexpr int AS_STEP = step_room<T, C, DP>(), AS_TILES = tiles_room<T, C, DP>();
+    return STEP && TILES ? (AS_STEP < AS_TILES ? AS_STEP : AS_TILES) : STEP ? AS_STEP : AS_TILES;
 }
 
 template <class T, class C, int DP, int EL, bool STEP, bool TILES>

@@ -1,4 +1,5 @@
-// Attention of new tokens over a cache in pages, bf16 (fp32: paged_attn_f32.hip; two files, which compile at the same time).
+// Attention of new tokens over a cache in pages, bf16 (fp32: paged_attn_f32.hip; two files, which compile at the same
+// time).
 #include "paged_attn.h"
 
 namespace qlka {

@@ -1,23 +1,23 @@
 // A cache of keys and values in pages, written as tokens come and read back (include/qlka.h).
 //
 // With 8 bits held, 32 elements of a row share a power of two: the least one, 2^e, whose multiple by the largest code
-// reaches the largest of them. x / 2^e, the code's rounding (nearest, ties to the even one) and code * 2^e are then exact
-// but for that rounding, in any type that holds x: what is written is what the definition says, to the bit, and products
-// of what is read need no further rounding (int8 and e4m3 values have at most 7 and 4 bits, bf16 has 8). A scale of
-// largest / 127 would use up to one bit more of int8, but every reader would round.
+// reaches the largest of them. x / 2^e, the code's rounding (nearest, ties to the even one) and code * 2^e are then
+// exact but for that rounding, in any type that holds x: what is written is what the definition says, to the bit, and
+// products of what is read need no further rounding (int8 and e4m3 values have at most 7 and 4 bits, bf16 has 8). A
+// scale of largest / 127 would use up to one bit more of int8, but every reader would round.
 //
 // Both kernels are bound by memory, and at few rows by the latency of offsets and lengths, table and store, one after
-// the other (the rows themselves are loaded meanwhile). DP / 8 lanes take a row, 8 elements each; 4 lanes find a block's
-// largest element. A wave writes one token's rows of all heads, keys and values, so that the sequence is looked up once
-// for all of them. 8 prompts of 200 to 4096 (10211 tokens of 12 heads of 64, bf16 to int8): 14 us for 49 MB; read back
-// padded: 17.5 us for 117 MB; 64 tokens: 3.6 us.
+// the other (the rows themselves are loaded meanwhile). DP / 8 lanes take a row, 8 elements each; 4 lanes find a
+// block's largest element. A wave writes one token's rows of all heads, keys and values, so that the sequence is looked
+// up once for all of them. 8 prompts of 200 to 4096 (10211 tokens of 12 heads of 64, bf16 to int8): 14 us for 49 MB;
+// read back padded: 17.5 us for 117 MB; 64 tokens: 3.6 us.
 #include "paged_device.h"
 
 namespace qlka {
 namespace pg {
 
-// The exponent (plus 127) of a block whose largest element is `most`: the least of [27, top] with most <= largest * 2^(e -
-// 127), largest = MANT * 2^SHIFT with MANT in [1, 2); 255 if it is not finite.
+// The exponent (plus 127) of a block whose largest element is `most`: the least of [27, top] with most <= largest *
+// 2^(e - 127), largest = MANT * 2^SHIFT with MANT in [1, 2); 255 if it is not finite.
 template <class C> __device__ __forceinline__ uint32_t exponent_of(float most) {
     constexpr bool INT = std::is_same<C, Int8>::value;
     constexpr uint32_t MANT = INT ? 0x7e0000u : 0x600000u;            // of 127 = 1.984375 * 2^6, of 448 = 1.75 * 2^8
@@ -34,12 +34,14 @@ template <class C> __device__ __forceinline__ u32x2 codes_of(f32x8 x, uint32_t e
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         if constexpr (std::is_same<C, Int8>::value) {
-            // next to 1.5 * 2^23 a float's last place is 1: the sum is rounded as it should be, and its low byte is the code
+            // next to 1.5 * 2^23 a float's last place is 1: the sum is rounded as it should be, and its low byte is the
+            // code
             uint32_t y[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 y[i] = __float_as_uint(__builtin_amdgcn_fmed3f(x[4 * h + i] * s, -127.f, 127.f) + 12582912.f);
-            const uint32_t lo = __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0400), hi = __builtin_amdgcn_perm(y[3], y[2], 0x0c0c0400);
+            const uint32_t lo = __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0400);
+            const uint32_t hi = __builtin_amdgcn_perm(y[3], y[2], 0x0c0c0400);
             w[h] = e == 255 ? 0u : lo | hi << 16;
         } else {
             float c[4];

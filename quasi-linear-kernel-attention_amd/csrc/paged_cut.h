@@ -1,5 +1,5 @@
-// How pages are found and how the work of attention over them is cut (paged_device.h): the arithmetic, on the host and on
-// the device.
+// How pages are found and how the work of attention over them is cut (paged_device.h): the arithmetic, on the host and
+// on the device.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -43,14 +43,14 @@ __host__ __device__ __forceinline__ int seen_upto(int seat, int num_pages, int p
 struct Extent { int blocks, seen; };           // of a sequence: blocks of rows, positions that its last row sees
 struct Cut { int blocks, parts, span; };     // of a sequence: units a key head = blocks * parts; positions of a part
 
-// The work of the sequences so far and one more. The kernel that joins parts finds the same span as the one that left them
-// only if both round alike, and products of thousands of blocks and positions are rounded: one fused operation, which no
-// compiler can take apart or fuse with another one.
+// The work of the sequences so far and one more. The kernel that joins parts finds the same span as the one that left
+// them only if both round alike, and products of thousands of blocks and positions are rounded: one fused operation,
+// which no compiler can take apart or fuse with another one.
 __host__ __device__ __forceinline__ float more_work(float work, Extent h) {
     return __builtin_fmaf((float)h.blocks, (float)h.seen, work);
 }
-// Positions of a part: what leaves about `aim` units of `work`, `least` at the least, a multiple of `align`. More than work /
-// aim, so that the units are at most as many as the blocks and aim + 1.
+// Positions of a part: what leaves about `aim` units of `work`, `least` at the least, a multiple of `align`. More than
+// work / aim, so that the units are at most as many as the blocks and aim + 1.
 __host__ __device__ __forceinline__ int span_of(float work, float aim, int least, int align) {
     const int span = std::max((int)std::fmin(work / aim, (float)MOST_POSITIONS) + 1, least);
     return (span + align - 1) / align * align;

@@ -50,7 +50,8 @@ template <class C> __device__ __forceinline__ f32x4 four(uint32_t w, float s) {
         for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)(w >> 8 * i) * s;
     } else {
         typedef __attribute__((ext_vector_type(2))) float f32x2;
-        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+        const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
         x = f32x4{lo[0] * s, lo[1] * s, hi[0] * s, hi[1] * s};
     }
     return x;
@@ -129,7 +130,8 @@ __device__ __forceinline__ Tokens tokens_of_lane(const PgParams& p) {
     const int lane = threadIdx.x & 63;
     return lane < p.B ? tokens_of(p, lane) : Tokens{0, 0, 0};
 }
-// The sequence of row t (the same for all lanes) and its tokens, from those of every lane; b < 0 outside every sequence.
+// The sequence of row t (the same for all lanes) and its tokens, from those of every lane; b < 0 outside every
+// sequence.
 struct Found { int b; Tokens tokens; };
 __device__ __forceinline__ Found find(const PgParams& p, int t, Tokens mine) {
     Found x{t, {}};
@@ -148,14 +150,15 @@ __device__ __forceinline__ Found find(const PgParams& p, int t, Tokens mine) {
     return x;
 }
 
-// How the work of a launch is cut into units of about equal time: a block of ROWS rows of one key head over `span` successive
-// positions. The span goes by what the sequences of this launch (STEP: those of few rows) hold together, which only
-// the device knows, so that there are about `aim` units a key head; every workgroup finds it, and its unit, by itself,
-// a lane a sequence. The parts of a sequence are of one length (4 chunks of up to 8192: the longest of 19 tiles instead of 20,
-// 65 us instead of 68). Units of one sequence, part and key head are next to each other, and successive ones on one XCD, whose L2
-// then serves their keys. Where a sequence's positions are one part, its rows are written at once, else each part's sums
-// go to the unit's place in the workspace and paged_join adds them up. Of many sequences a kernel of its own writes the span
-// and the units before each one to the workspace (u.table), where the others look.
+// How the work of a launch is cut into units of about equal time: a block of ROWS rows of one key head over `span`
+// successive positions. The span goes by what the sequences of this launch (STEP: those of few rows) hold together,
+// which only the device knows, so that there are about `aim` units a key head; every workgroup finds it, and its unit,
+// by itself, a lane a sequence. The parts of a sequence are of one length (4 chunks of up to 8192: the longest of 19
+// tiles instead of 20, 65 us instead of 68). Units of one sequence, part and key head are next to each other, and
+// successive ones on one XCD, whose L2 then serves their keys. Where a sequence's positions are one part, its rows are
+// written at once, else each part's sums go to the unit's place in the workspace and paged_join adds them up. Of many
+// sequences a kernel of its own writes the span and the units before each one to the workspace (u.table), where the
+// others look.
 struct Unit { int b, part, kvh, block, parts, span, at; };
 
 template <bool STEP, int ROWS> struct Units {
@@ -173,9 +176,9 @@ template <bool STEP, int ROWS> struct Units {
         const bool here = b < p.B && STEP == (rows <= p.few) && rows > 0;
         return {here ? (rows + ROWS - 1) / ROWS : 0, seen_from(p, t.start + t.rows - 1)};
     }
-    // f(the first of 64 sequences, what this lane's is) for those from 64 up to `end`, until it returns true; all are looked up
-    // together (256 of 100 to 1000, 8 with chunks, 12 / 4 heads, bf16: 54 us, 56 one after the other); more of them are in
-    // u.table
+    // f(the first of 64 sequences, what this lane's is) for those from 64 up to `end`, until it returns true; all are
+    // looked up together (256 of 100 to 1000, 8 with chunks, 12 / 4 heads, bf16: 54 us, 56 one after the other); more
+    // of them are in u.table
     template <class F> __device__ __forceinline__ void others(int end, F f) const {
         constexpr int EACH = (PG_LOOKED_UP - 64) / 64;
         if (end <= 64) return;
@@ -240,7 +243,8 @@ template <bool STEP, int ROWS> struct Units {
     }
     // number `rest` of a sequence's units
     __device__ __forceinline__ void place(Unit& x, Cut c, int rest) const {
-        const InSequence at = place_in(__builtin_amdgcn_readfirstlane(c.blocks), __builtin_amdgcn_readfirstlane(rest), p.G);
+        const InSequence at =
+            place_in(__builtin_amdgcn_readfirstlane(c.blocks), __builtin_amdgcn_readfirstlane(rest), p.G);
         x.parts = __builtin_amdgcn_readfirstlane(c.parts);
         x.span = __builtin_amdgcn_readfirstlane(c.span);
         x.part = at.part;
@@ -271,8 +275,9 @@ template <bool STEP, int ROWS> struct Units {
             }
             const int l = __builtin_ctzll(past);
             x.b = b0 + l;
-            place(x, {__builtin_amdgcn_readlane(c.blocks, l), __builtin_amdgcn_readlane(c.parts, l),
-                      __builtin_amdgcn_readlane(c.span, l)}, x.at - (base + __builtin_amdgcn_readlane(to - n, l)) * p.G);
+            const Cut its = {__builtin_amdgcn_readlane(c.blocks, l), __builtin_amdgcn_readlane(c.parts, l),
+                             __builtin_amdgcn_readlane(c.span, l)};
+            place(x, its, x.at - (base + __builtin_amdgcn_readlane(to - n, l)) * p.G);
             return true;
         };
         if (!among(0, cut_mine, first, before))

@@ -4,10 +4,11 @@
 namespace qlka {
 namespace pg {
 
-// Adds up the parts of rows whose positions are more than one. A wave takes a row (MANY: 256 / DP rows of a token, since
-// finding the sequence costs as much as a row): its lanes look at the parts' references and sums, one each, then DP / 4
-// lanes take a part's sums. Bound by latency: launch, sequence, sums (192 rows: 4.5 us; 19548 rows of 2 to 7 parts:
-// 7.8 us, 20 with a wave a row; of 9 parts 10.2 us, 13.3 where 8 were waited for before the ninth was asked for).
+// Adds up the parts of rows whose positions are more than one. A wave takes a row (MANY: 256 / DP rows of a token,
+// since finding the sequence costs as much as a row): its lanes look at the parts' references and sums, one each, then
+// DP / 4 lanes take a part's sums. Bound by latency: launch, sequence, sums (192 rows: 4.5 us; 19548 rows of 2 to 7
+// parts: 7.8 us, 20 with a wave a row; of 9 parts 10.2 us, 13.3 where 8 were waited for before the ninth was asked
+// for).
 template <class T, int DP, bool MANY> __global__ __launch_bounds__(256) void paged_join(const PgParams p) {
     constexpr int LANES = DP / 4, GROUPS = 64 / LANES;                 // lanes of a part's row
     constexpr int LOOK = MANY ? LANES : 64, AT_ONCE = MANY ? 1 : GROUPS;
@@ -47,7 +48,8 @@ template <class T, int DP, bool MANY> __global__ __launch_bounds__(256) void pag
     const int64_t row = unit * size + r % size;
     float ref = LOW, sum = 0.f;
     f32x4 x = {};
-    // parts s0 to s0 + LOOK - 1, of which the first `early` of a group of lanes are on their way before their weights are known
+    // parts s0 to s0 + LOOK - 1, of which the first `early` of a group of lanes are on their way before their weights
+    // are known
     const auto add = [&](int s0, auto early) {
         constexpr int EARLY = decltype(early)::value;
         const int look = s0 + (MANY ? i : lane), count = min(LOOK, parts - s0), first = MANY ? 0 : group;
@@ -102,8 +104,8 @@ template <class T, int DP, bool MANY> __global__ __launch_bounds__(256) void pag
 }
 constexpr int64_t JOIN_MANY = 4096;          // rows
 
-// The units before each of the sequences, of all, and the span: B + 2 numbers for each kind of units, of which each has a
-// workgroup.
+// The units before each of the sequences, of all, and the span: B + 2 numbers for each kind of units, of which each has
+// a workgroup.
 constexpr int TABLE_THREADS = 1024;
 template <class U> __device__ __forceinline__ void fill_table(const PgParams& p, const PgUnits& u, U units, int* sums,
                                                               float* works) {
@@ -143,8 +145,10 @@ template <class U> __device__ __forceinline__ void fill_table(const PgParams& p,
 __global__ __launch_bounds__(TABLE_THREADS) void paged_table(const PgParams p) {
     __shared__ int sums[TABLE_THREADS / 64];
     __shared__ float works[TABLE_THREADS / 64];
-    if (blockIdx.x == 0 && p.step.groups) fill_table(p, p.step, Units<true, PG_STEP_ROWS>(p, p.step, 0), sums, works);
-    if (blockIdx.x == 1 && p.tiles.groups) fill_table(p, p.tiles, Units<false, PG_TILE_ROWS>(p, p.tiles, 0), sums, works);
+    if (blockIdx.x == 0 && p.step.groups)
+        fill_table(p, p.step, Units<true, PG_STEP_ROWS>(p, p.step, 0), sums, works);
+    if (blockIdx.x == 1 && p.tiles.groups)
+        fill_table(p, p.tiles, Units<false, PG_TILE_ROWS>(p, p.tiles, 0), sums, works);
 }
 
 }  // namespace pg
@@ -156,7 +160,8 @@ int pg_table(const PgParams& p, hipStream_t st) {
 
 int pg_join(int dtype, const PgParams& p, hipStream_t st) {
     return sm::dispatch(dtype, p.D, [&](auto t, auto dp) {
-        const int64_t rows = (int64_t)p.T * p.H, at_once = 256 / dp.value, waves = p.T * ((p.H + at_once - 1) / at_once);
+        const int64_t rows = (int64_t)p.T * p.H, at_once = 256 / dp.value;
+        const int64_t waves = p.T * ((p.H + at_once - 1) / at_once);
         if (rows >= pg::JOIN_MANY)
             pg::paged_join<decltype(t), dp.value, true><<<dim3((unsigned)((waves + 3) / 4)), 256, 0, st>>>(p);
         else

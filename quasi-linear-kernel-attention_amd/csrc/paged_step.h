@@ -1,17 +1,18 @@
-// Softmax attention of a few new tokens over a cache in pages (a decoder's single tokens): bound by reading the held keys
-// and values once.
+// Softmax attention of a few new tokens over a cache in pages (a decoder's single tokens): bound by reading the held
+// keys and values once.
 //
 // A workgroup takes 16 rows, the query heads of one key head's new tokens, and a part of the sequence's positions; its
 // waves take 32 positions each in turn and go through them by themselves (no barrier): pages found, keys and values
 // loaded into registers one turn ahead, S^T = k q^T by v_mfma_f32_16x16x32_bf16 with the keys as they lie in memory as
-// the first operand (a lane holds 8 elements of a key; which 8 goes by the load's width, and q is held to match), O^T +=
-// v^T P^T with the probabilities from the registers that they are in and the values turned by a tile in LDS that only
-// this wave uses. A row's reference for the exponentials is moved when some lane's score passes it by 2^8, so nothing
-// crosses lanes in most turns. Waves are joined at the end, the parts of long sequences by paged_join.
+// the first operand (a lane holds 8 elements of a key; which 8 goes by the load's width, and q is held to match), O^T
+// += v^T P^T with the probabilities from the registers that they are in and the values turned by a tile in LDS that
+// only this wave uses. A row's reference for the exponentials is moved when some lane's score passes it by 2^8, so
+// nothing crosses lanes in most turns. Waves are joined at the end, the parts of long sequences by paged_join.
 //
-// Measured: 16 sequences of 2000 to 8192, 12 heads of 64, bf16: 37 us under way for 211 MB, of which the card's last-level
-// cache serves a part, 50 with the joining and cold pages (shuffled pages are read at 5.1 TB/s at most); 32 of 1000 to
-// 16384, 12 / 4 heads, e4m3: 22 us, 32 with all; 8 of 33 to 197: 6.5 us, latency of lengths, table and rows in turn.
+// Measured: 16 sequences of 2000 to 8192, 12 heads of 64, bf16: 37 us under way for 211 MB, of which the card's
+// last-level cache serves a part, 50 with the joining and cold pages (shuffled pages are read at 5.1 TB/s at most); 32
+// of 1000 to 16384, 12 / 4 heads, e4m3: 22 us, 32 with all; 8 of 33 to 197: 6.5 us, latency of lengths, table and rows
+// in turn.
 //
 // Elements of 8 bits become bf16 exactly (paged_cache.hip), so products are those of what is held.
 #pragma once
@@ -49,9 +50,10 @@ template <int NA, int NB> struct Sum {
     }
 };
 
-// Column d0 + lane % 16 of a tile's 32 rows in the order that scores stand in registers: lane group g (of 16) has rows 4 g
-// .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3.
-template <int NP, int DP> __device__ __forceinline__ sm::Frag<NP> column16(const sm::Tile<NP, 32, DP>& t, int d0, int lane) {
+// Column d0 + lane % 16 of a tile's 32 rows in the order that scores stand in registers: lane group g (of 16) has rows
+// 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3.
+template <int NP, int DP>
+__device__ __forceinline__ sm::Frag<NP> column16(const sm::Tile<NP, 32, DP>& t, int d0, int lane) {
     const int row = 4 * (lane >> 4) + ((lane & 15) >> 2), piece = (d0 >> 3) + ((lane & 3) >> 1);
     const int lo = t.at(row, piece) + (lane & 1) * 4, hi = t.at(row + 16, piece) + (lane & 1) * 4;
     sm::Frag<NP> f;
@@ -66,8 +68,9 @@ template <int NP, int DP> __device__ __forceinline__ sm::Frag<NP> column16(const
     return f;
 }
 
-// Waves that a SIMD has room for: what waits for memory is other waves' time. With 4 waves bf16 rows of 64 would spill in the
-// loop (16 x 12 heads of up to 8192: 70 us, 52 with 3, 59 with 2); 8 bits do not (32 x 12 / 4: 33 us, 41 with 2).
+// Waves that a SIMD has room for: what waits for memory is other waves' time. With 4 waves bf16 rows of 64 would spill
+// in the loop (16 x 12 heads of up to 8192: 70 us, 52 with 3, 59 with 2); 8 bits spill 3 registers, loaded 8 at a time
+// 6 to 14, and are faster so (32 x 12 / 4: 33 us, 41 with 2).
 template <class T, class C, int DP> constexpr int step_room() {
     return sm::Elem<T>::PARTS == 3 || DP == 128 ? 2 : coded<C> || DP == 32 ? 4 : 3;
 }
@@ -134,7 +137,7 @@ template <class T, class C, int DP, int EL> __device__ __forceinline__ void step
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             ok[i] = (uint32_t)pages.page[i] < (uint32_t)p.num_pages;
-            const uint32_t page = ok[i] ? pages.page[i] : 0, row = pages.row[i];   // what is not there: some row, not used
+            const uint32_t page = ok[i] ? pages.page[i] : 0, row = pages.row[i];       // not there: some row, not used
             const char* k = k_head + bytes_to(p.sk, page, row);
             const char* v = v_head + bytes_to(p.sv, page, row);
 #pragma unroll
@@ -258,7 +261,7 @@ template <class T, class C, int DP, int EL> __device__ __forceinline__ void step
         for (int i = 0; i < 8; ++i) e[i] = sm::exp_of(s[i / 4][i % 4] - ref);
         const sm::Frag<NQ> pf = sm::split<NQ>(e);
         if constexpr (NQ == 1) {
-            sum = sm::add_all(pf.p[0], sum);                            // of the rounded ones, which are what is added up
+            sum = sm::add_all(pf.p[0], sum);                            // of the rounded ones: what is added up
         } else {
             float part = 0.f;
 #pragma unroll
@@ -273,7 +276,8 @@ template <class T, class C, int DP, int EL> __device__ __forceinline__ void step
         }
     };
     if constexpr (AHEAD) {
-        // in two sets of registers by turns, so that one turn's rows are waited for while the next ones are on their way
+        // in two sets of registers by turns, so that one turn's rows are waited for while the next ones are on their
+        // way
         while (turn < end) {
             Held odd;
             if (turn + NW < end) odd = fetch(pages);

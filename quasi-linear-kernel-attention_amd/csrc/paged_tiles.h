@@ -1,5 +1,5 @@
-// Softmax attention of chunks of new tokens over a cache in pages: the tiles of softmax_fwd.hip over rows that are found
-// through the sequence's table.
+// Softmax attention of chunks of new tokens over a cache in pages: the tiles of softmax_fwd.hip over rows that are
+// found through the sequence's table.
 //
 // A workgroup takes 128 rows of one sequence and key head, token by token and within a token the query heads that share
 // the key head, so that heads with common keys read (and take apart) them once. Each thread finds the pages of the rows
@@ -7,9 +7,9 @@
 // stay in registers until the tile before is done with and become bf16 on their way into the other buffer (exactly, see
 // paged_cache.hip); float rows are split into three parts there, with one buffer.
 //
-// Bound by vector instructions: 4 chunks of 512 new tokens at 1024 to 8192, 12 / 4 heads, int8: 64 us, 378 TFLOP/s (the scores'
-// work; taking 8 bits apart and bringing them 20 us; with bf16 pages 56 us). Two or three waves a SIMD are as fast, with
-// four registers spill (120 us).
+// Bound by vector instructions: 4 chunks of 512 new tokens at 1024 to 8192, 12 / 4 heads, int8: 64 us, 378 TFLOP/s (the
+// scores' work; taking 8 bits apart and bringing them 20 us; with bf16 pages 56 us). Two or three waves a SIMD are as
+// fast, with four registers spill (120 us).
 #pragma once
 
 #include "paged_device.h"
@@ -62,7 +62,8 @@ template <class C, int DP, int BN> struct Bring {
     Raw k[DIRECT ? 1 : EACH], v[DIRECT ? 1 : EACH];
     uint32_t ke[EACH], ve[EACH];
 
-    __device__ __forceinline__ Bring(Lds& lds, const PgParams& p, int tid) : row(tid / PIECES), slot(tid % PIECES), ok(0) {
+    __device__ __forceinline__ Bring(Lds& lds, const PgParams& p, int tid)
+        : row(tid / PIECES), slot(tid % PIECES), ok(0) {
         if (DIRECT && p.D < DP) {            // pieces past D stay as they are
             bf16x8* x = reinterpret_cast<bf16x8*>(&lds);
             for (int i = tid; i < (int)(sizeof(Lds) / 16); i += NT) x[i] = bf16x8{};
@@ -142,7 +143,8 @@ template <class C, int DP, int BN> struct Bring {
 template <class T, class C, int DP> constexpr int tiles_room() { return sm::Elem<T>::PARTS == 3 && DP == 128 ? 1 : 2; }
 
 template <class T, class C, int DP> __device__ __forceinline__ void tiles(const PgParams& p, int wg) {
-    constexpr int NQ = sm::Elem<T>::PARTS, NK = Piece<C, 8>::PARTS, BN = sm_tile_rows(NK, DP), NS = BN / 32, ND = DP / 32;
+    constexpr int NQ = sm::Elem<T>::PARTS, NK = Piece<C, 8>::PARTS;
+    constexpr int BN = sm_tile_rows(NK, DP), NS = BN / 32, ND = DP / 32;
     constexpr int ROWS = PG_TILE_ROWS, NT = 64 * TILE_WAVES;
     typedef Bring<C, DP, BN> BringT;
     static_assert(Units<false, ROWS>::ALIGN % BN == 0);
@@ -174,7 +176,8 @@ template <class T, class C, int DP> __device__ __forceinline__ void tiles(const 
     bool lacks = false;
     if (t < t1) {
         const int end = place_of(p, min(t1 * BN, seen) - 1).index;
-        for (int i = place_of(p, t * BN).index + tid; i <= end; i += NT) lacks |= (uint32_t)table[i] >= (uint32_t)p.num_pages;
+        for (int i = place_of(p, t * BN).index + tid; i <= end; i += NT)
+            lacks |= (uint32_t)table[i] >= (uint32_t)p.num_pages;
     }
     lacks = __syncthreads_or(lacks);
     BringT tile(lds, p, tid);

@@ -60,9 +60,10 @@ template <class F> __device__ __forceinline__ int last_upto(int count, int x, F 
 }
 
 template <class L>
-__host__ __device__ __forceinline__ Segment segment_of(const int* offsets, int B, int T, int rows, int number, L lanes) {
-    int j = last_upto(B + 2, number, [&](int i) { return segment_start(segment_edge(offsets, B, T, i), i, rows); }, lanes);
-    j = std::max(lanes.same(j), 0);
+__host__ __device__ __forceinline__
+Segment segment_of(const int* offsets, int B, int T, int rows, int number, L lanes) {
+    const auto start = [&](int i) { return segment_start(segment_edge(offsets, B, T, i), i, rows); };
+    const int j = std::max(lanes.same(last_upto(B + 2, number, start, lanes)), 0);
     Segment s;
     s.index = j - 1;
     s.first = segment_edge(offsets, B, T, j);

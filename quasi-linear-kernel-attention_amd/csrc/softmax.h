@@ -49,8 +49,8 @@ struct SmParams {
     float scale;                             // |scale|; its sign (or 0) is in q_sign
     float q_sign;
     SmBuckets bk;
-    const int* offsets;                      // packed sequences (softmax_packed_*): segments.h; then B is 1, M and N are
-    int sequences, groups;                   // the rows of all, and `large` has `groups` numbers a head
+    const int* offsets;                      // packed sequences (sm_packed_*): segments.h; then B is 1, M and N are the
+    int sequences, groups;                   // rows of all, and `large` has `groups` numbers a head
 };
 
 // Elements of a row in LDS and in the partial rows.

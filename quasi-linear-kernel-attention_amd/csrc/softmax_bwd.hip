@@ -10,8 +10,8 @@
 // table's gradient, which is fp32, dS is taken as it is, and O is that of P in three parts (softmax_fwd.hip, FINE).
 // The waves wait for 34 to 50% of their cycles, for the next tile and for each other. Measured: 12 x 8192 x 8192 of 64
 // with the table's gradient, bf16: softmax_dq 491 us (630 TFLOP/s), softmax_dkv 533 us (773); fp32, 32 x 4 heads of 600
-// to 65: 41 and 42 us; bf16 of 128, 2 x 8 x 2048 x 2048: 257 us with the forward; packed sequences, 12 of 256 to 8192, 12 heads,
-// causal, bf16: 520 and 703 us (786 and 775 TFLOP/s of what is visible). Registers are short: at fp32 of 64
+// to 65: 41 and 42 us; bf16 of 128, 2 x 8 x 2048 x 2048: 257 us with the forward; packed sequences, 12 of 256 to 8192,
+// 12 heads, causal, bf16: 520 and 703 us (786 and 775 TFLOP/s of what is visible). Registers are short: at fp32 of 64
 // elements and more, and at bf16 of 128, some values live in scratch memory.
 #include "softmax_tile.h"
 
@@ -334,7 +334,8 @@ __global__ __launch_bounds__(64 * NW, (Shape<T, DP>::WAVES)) void softmax_dq(con
         }
         __syncthreads();
         const int64_t count = (int64_t)p.B * p.splits * p.blocks;
-        float* part = p.part_table + (head * count + ((int64_t)b * p.splits + split_i) * p.blocks + span.block) * buckets;
+        const int64_t before = ((int64_t)b * p.splits + split_i) * p.blocks + span.block;
+        float* part = p.part_table + (head * count + before) * buckets;
         for (int i = tid; i < buckets; i += NT) {
             float a = 0.f;
             for (int j = 0; j < NW; ++j) a += sums[j][i];

@@ -11,17 +11,17 @@
 // Where the table's gradient will be wanted (FINE) they are taken in three parts of 8 bits: that gradient is fp32 and a
 // sum over rows of dS = P (dP - delta), in which an error of delta, the row sum of dO * O, does not average out. The
 // smaller parts' products then gather in a sum of their own, as in Acc (12 x 8192 x 8192: error of the table's gradient
-// 1.0e-6, 1.8e-6 without; 476 us, 250 with one part). The gradients form P whole, so the log sums that they divide by are
-// of the whole exponentials for packed sequences (SUMS): with the rounded ones' all of a short row's P is off by up to 2^-8
-// (12 of 256 to 8192, 12 heads, with the gradients: 1448 us, 1415 with the rounded sums).
+// 1.0e-6, 1.8e-6 without; 476 us, 250 with one part). The gradients form P whole, so the log sums that they divide by
+// are of the whole exponentials for packed sequences (SUMS): with the rounded ones' all of a short row's P is off by up
+// to 2^-8 (12 of 256 to 8192, 12 heads, with the gradients: 1448 us, 1415 with the rounded sums).
 //
 // Masked keys are read as zeros (what stands there may be anything) and their tiles, where none is left, are skipped.
 // Bound by the matrix cores and by the scores' work between them (an exponential, a maximum and two multiply-adds a
 // score), which other waves' products hide only in part. Measured: 12 x 16384 x 16384 of 64 with the bias, bf16, 977 to
 // 1003 us, 835 TFLOP/s; 4 x 12 x 2048 x 8192, padded, 200 to 220 us; fp32, 2 x 12 x 301 x 3111, padded, 54 us with the
 // joining of the splits; causal order, 12 x 8192 x 8192, 197 us; packed sequences (PACKED: a workgroup finds its own,
-// softmax_tile.h), 16 of 100 to 8192, 12 / 4 heads, causal, bf16, 571 to 593 us, 830 TFLOP/s; 24 of 50 to 2048, 12 heads,
-// fp32, 372 us. When a call has too few queries to fill the GPU, the
+// softmax_tile.h), 16 of 100 to 8192, 12 / 4 heads, causal, bf16, 571 to 593 us, 830 TFLOP/s; 24 of 50 to 2048, 12
+// heads, fp32, 372 us. When a call has too few queries to fill the GPU, the
 // keys are split: each split leaves its unscaled O with its maximum and sum, and softmax_combine joins them.
 #include "softmax_tile.h"
 
@@ -32,12 +32,14 @@ namespace sm {
 
 constexpr float GROW = 4.f;          // 2^8 of the exponentials
 
-// Three parts of P leave room for three waves a SIMD (of 64 elements) only if the compiler is held to it: 476 us for 524 at
-// 12 x 8192 x 8192. So do packed sequences for four (16 of 100 to 8192, 12 / 4 heads: 571 us for 597), but not with two
-// sums a row (SUMS: 12 of 256 to 8192, 12 heads, with the gradients 1448 us, 1454 with four).
+// Three parts of P leave room for three waves a SIMD (of 64 elements) only if the compiler is held to it: 476 us for
+// 524 at 12 x 8192 x 8192. So do packed sequences for four (16 of 100 to 8192, 12 / 4 heads: 571 us for 597), but not
+// with two sums a row (SUMS: 12 of 256 to 8192, 12 heads, with the gradients 1448 us, 1454 with four).
+template <class T, int DP, int NW, bool FINE, bool PACKED, bool SUMS> constexpr int fwd_waves() {
+    return FINE && DP <= 64 ? 3 : PACKED && !SUMS && sizeof(T) == 2 && DP == 64 && NW > 1 ? 4 : Shape<T, DP>::WAVES;
+}
 template <class T, int DP, int NW, bool BIAS, bool FINE, bool PACKED, bool SUMS = false>
-__global__ __launch_bounds__(64 * NW, (FINE && DP <= 64 ? 3 : PACKED && !SUMS && sizeof(T) == 2 && DP == 64 && NW > 1 ? 4
-                                                                                                          : Shape<T, DP>::WAVES))
+__global__ __launch_bounds__(64 * NW, (fwd_waves<T, DP, NW, FINE, PACKED, SUMS>()))
 void softmax_fwd(const SmParams p) {
     constexpr int NP = Elem<T>::PARTS, BN = Shape<T, DP>::BN, NT = 64 * NW, ROWS = 32 * NW, NS = BN / 32, ND = DP / 32;
     typedef Pair<T, DP, BN, NW> PairT;
@@ -290,7 +292,8 @@ template <class T, int DP, int NW> int launch_fwd(const SmParams& p, hipStream_t
 }
 template <class T, int DP, int NW> int launch_packed(const SmParams& p, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)p.H * p.blocks * p.splits));
-    if (sizeof(T) == 2 && p.lse) softmax_fwd<T, DP, NW, false, false, true, sizeof(T) == 2><<<grid, 64 * NW, 0, st>>>(p);
+    constexpr bool ROUNDED = sizeof(T) == 2;
+    if (ROUNDED && p.lse) softmax_fwd<T, DP, NW, false, false, true, ROUNDED><<<grid, 64 * NW, 0, st>>>(p);
     else softmax_fwd<T, DP, NW, false, false, true><<<grid, 64 * NW, 0, st>>>(p);
     return (int)hipGetLastError();
 }

@@ -479,9 +479,10 @@ template <> struct Span<true> {
         if (p.sequences <= HEAVY_FIRST) {
             s = p.sequences <= 62 ? heavy_first<1>(p, number, size, keys) : heavy_first<EACH>(p, number, size, keys);
         } else {
-            // Numbers without a block are at regular places where the sequences are alike (every second one for sequences of
-            // one block), and successive numbers are on different XCDs by turns: eight at a time are moved among
-            // themselves, or half of the XCDs would have nothing to do (128 x 4 heads of 128, fp32: 39 us, 34 so).
+            // Numbers without a block are at regular places where the sequences are alike (every second one for
+            // sequences of one block), and successive numbers are on different XCDs by turns: eight at a time are moved
+            // among themselves, or half of the XCDs would have nothing to do (128 x 4 heads of 128, fp32: 39 us, 34
+            // so).
             if ((number | 7) < p.blocks)
                 number = (number & ~7) | ((number + (((uint32_t)number >> 3) * 0x9e3779b1u >> 29)) & 7);
             s = segment_of(p.offsets, p.sequences, p.M, size, number, Lanes());
@@ -492,11 +493,12 @@ template <> struct Span<true> {
         first = s.first;
         group = segment_start(first, s.index + 1, 32);
     }
-    // The blocks in the order of their work, most first: a call ends with its last workgroups, and a long sequence's take a
-    // hundred times as long as a short one's. A lane holds segments (segments.h) of n blocks each. In causal order a
-    // sequence has a block with 1, 2, .. n blocks to go through, so that sum(max(n - x, 0)) blocks have more than x;
-    // else n with n each, and sum(n where n > x) do. x is found bit by bit. No sequence's blocks leave out numbers. Offsets
-    // that decrease count rows twice, but every second segment is then empty: sums of n stay below 2^31 all the same.
+    // The blocks in the order of their work, most first: a call ends with its last workgroups, and a long sequence's
+    // take a hundred times as long as a short one's. A lane holds segments (segments.h) of n blocks each. In causal
+    // order a sequence has a block with 1, 2, .. n blocks to go through, so that sum(max(n - x, 0)) blocks have more
+    // than x; else n with n each, and sum(n where n > x) do. x is found bit by bit. No sequence's blocks leave out
+    // numbers. Offsets that decrease count rows twice, but every second segment is then empty: sums of n stay below
+    // 2^31 all the same.
     static constexpr int EACH = 4, HEAVY_FIRST = 64 * EACH - 2;       // segments of a lane at most; sequences
     static __device__ __forceinline__ int sum_of(int x) {
         x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);           // row_shr 1, 2, 4, 8
@@ -562,8 +564,8 @@ template <> struct Span<true> {
     template <int BN> __device__ __forceinline__ KeyBits<BN> keys(int) const { return KeyBits<BN>(inside); }
 };
 
-// The work of a workgroup of a packed call: block by block, all heads of a block next to each other, those of one key head
-// on as few XCDs as possible.
+// The work of a workgroup of a packed call: block by block, all heads of a block next to each other, those of one key
+// head on as few XCDs as possible.
 template <bool KEYS> __device__ __forceinline__ Work packed_work(const SmParams& p, int wg) {
     const int heads = KEYS ? p.G : p.H, i = wg % heads, rest = wg / heads;
     return {KEYS ? i : i % p.G * (p.H / p.G) + i / p.G, rest % p.splits * p.blocks + rest / p.splits};

@@ -693,7 +693,8 @@ std::tuple<Tensor, Tensor, Tensor> packed_forward(PackedCall& c, bool train, boo
 }
 
 struct PackedFn : public torch::autograd::Function<PackedFn> {
-    static Tensor forward(AutogradContext* ctx, Tensor q, Tensor k, Tensor v, Tensor offsets, double scale, bool causal) {
+    static Tensor forward(AutogradContext* ctx, Tensor q, Tensor k, Tensor v, Tensor offsets, double scale,
+                          bool causal) {
         ctx->set_materialize_grads(false);
         PackedCall c{q, k, v, offsets, scale, causal};
         Tensor out, full, lse;
@@ -709,7 +710,8 @@ struct PackedFn : public torch::autograd::Function<PackedFn> {
         tensor_list r(6);
         if (!grads[0].defined()) return r;
         const auto s = ctx->get_saved_variables();
-        const PackedCall c{s[0], s[1], s[2], s[3], ctx->saved_data["scale"].toDouble(), ctx->saved_data["causal"].toBool()};
+        const PackedCall c{s[0], s[1], s[2], s[3], ctx->saved_data["scale"].toDouble(),
+                           ctx->saved_data["causal"].toBool()};
         const Tensor &out = s[4], &full = s[5], &lse = s[6];
         c10::DeviceGuard guard(c.q.device());
         qlka_packed_args a = packed_args(c);
@@ -766,7 +768,8 @@ struct PagedCall {
 
 PagedCall paged_call(const Tensor& k_pages, const Tensor& v_pages, const OptTensor& k_exp, const OptTensor& v_exp,
                      const Tensor& tables, const Tensor& lengths, const OptTensor& offsets) {
-    return {k_pages, v_pages, k_exp.value_or(Tensor()), v_exp.value_or(Tensor()), tables, lengths, offsets.value_or(Tensor())};
+    return {k_pages, v_pages, k_exp.value_or(Tensor()), v_exp.value_or(Tensor()), tables, lengths,
+            offsets.value_or(Tensor())};
 }
 
 int held_of(const Tensor& pages) {
@@ -860,13 +863,15 @@ void check_tokens(const char* name, const Tensor& x, const PagedCall& c) {
                 " must not require one");
 }
 
-void paged_write(const Tensor& k_, const Tensor& v_, const Tensor& k_pages, const Tensor& v_pages, const OptTensor& k_exp,
-                 const OptTensor& v_exp, const Tensor& tables, const Tensor& lengths, const OptTensor& offsets) {
+void paged_write(const Tensor& k_, const Tensor& v_, const Tensor& k_pages, const Tensor& v_pages,
+                 const OptTensor& k_exp, const OptTensor& v_exp, const Tensor& tables, const Tensor& lengths,
+                 const OptTensor& offsets) {
     const PagedCall c = paged_call(k_pages, v_pages, k_exp, v_exp, tables, lengths, offsets);
     check_pages(c.k_pages, c.v_pages, c.k_exp, c.v_exp);
     check_tokens("k", k_, c);
     check_tokens("v", v_, c);
-    TORCH_CHECK(k_.sizes() == v_.sizes() && k_.scalar_type() == v_.scalar_type(), "k and v must have one shape and dtype");
+    TORCH_CHECK(k_.sizes() == v_.sizes() && k_.scalar_type() == v_.scalar_type(),
+                "k and v must have one shape and dtype");
     TORCH_CHECK(k_.size(0) == k_pages.size(1), "k and v must have the heads of the pages");
     c10::DeviceGuard guard(k_pages.device());
     const Tensor k = packed_rows(k_), v = packed_rows(v_);
@@ -969,11 +974,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("paged_write", &paged_write, py::arg("k"), py::arg("v"), py::arg("k_pages"), py::arg("v_pages"),
           py::arg("k_exp"), py::arg("v_exp"), py::arg("tables"), py::arg("lengths"), py::arg("offsets"),
           "new tokens into the pages (qlka_paged_write)");
-    m.def("paged_read", [](const Tensor& k, const Tensor& v, const OptTensor& ke, const OptTensor& ve, const Tensor& tables,
-                           const Tensor& lengths, int64_t N, py::object dtype) {
+    m.def("paged_read", [](const Tensor& k, const Tensor& v, const OptTensor& ke, const OptTensor& ve,
+                           const Tensor& tables, const Tensor& lengths, int64_t N, py::object dtype) {
         return paged_read(k, v, ke, ve, tables, lengths, N, torch::python::detail::py_object_to_dtype(dtype));
-    }, py::arg("k_pages"), py::arg("v_pages"), py::arg("k_exp"), py::arg("v_exp"), py::arg("tables"), py::arg("lengths"),
-          py::arg("N"), py::arg("dtype"), "the first N positions of each sequence (qlka_paged_read)");
+    }, py::arg("k_pages"), py::arg("v_pages"), py::arg("k_exp"), py::arg("v_exp"), py::arg("tables"),
+          py::arg("lengths"), py::arg("N"), py::arg("dtype"),
+          "the first N positions of each sequence (qlka_paged_read)");
     m.def("paged_attention", &paged_attention, py::arg("q"), py::arg("k_pages"), py::arg("v_pages"), py::arg("k_exp"),
           py::arg("v_exp"), py::arg("tables"), py::arg("lengths"), py::arg("offsets"), py::arg("longest"),
           py::arg("scale"), "attention of new tokens over the pages (qlka_paged_attention)");

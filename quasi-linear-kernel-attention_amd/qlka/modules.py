@@ -8,10 +8,11 @@ entries, provided here with the same names and arguments:
     fused libqlka call each (qlka.layers); "softmax" is scaled dot-product attention with scale tau**-2
     (attention.py:99-102). TAU holds the default temperatures (kernels.py:13-25).
   * KernelMultiheadAttention(embed_dim, num_heads, kernel, tau, impl) (vision_transformer.py:19-44): self-attention
-    whose state_dict is nn.MultiheadAttention's (in_proj_weight, in_proj_bias, out_proj), so trained weights load. With the
-    "softmax" kernel it also attends to another sequence (context), to earlier positions alone (causal) and with a learned
-    relative position bias (position_bias, a RelativePositionBias), on the kernels of qlka.softmax; to sequences of different
-    lengths without padding (offsets), on those of qlka.packed; and to a cache in pages (cache), on those of qlka.paged.
+    whose state_dict is nn.MultiheadAttention's (in_proj_weight, in_proj_bias, out_proj), so trained weights load. With
+    the "softmax" kernel it also attends to another sequence (context), to earlier positions alone (causal) and with a
+    learned relative position bias (position_bias, a RelativePositionBias), on the kernels of qlka.softmax; to sequences
+    of different lengths without padding (offsets), on those of qlka.packed; and to a cache in pages (cache), on those
+    of qlka.paged. The last two, like the bias, run on the GPU alone; the others fall back to torch on the CPU.
   * use_kernel_attention(model, kernel, tau, impl) and KernelAttention(config, kernel, tau, impl) (nomic.py:9-40):
     kernel attention inside a HF NomicBertModel with its own weights.
 
@@ -90,8 +91,8 @@ class KernelMultiheadAttention(nn.Module):
       * causal=True: the query at position start + m sees the keys up to its own position. For a decoder's next tokens,
         context holds the heads of all tokens up to them and start is the position of x's first one (without a context,
         where the keys are x's own, there is no other position than 0);
-      * forward(x, offsets=offsets): x (T, E), sequences one after the other (qlka.packed), each attending to itself (causal
-        or not) -> (T, E);
+      * forward(x, offsets=offsets): x (T, E) on the GPU, sequences one after the other (qlka.packed), each attending to
+        itself (causal or not) -> (T, E);
       * forward(x, cache=(pages, tables, lengths), offsets=offsets): x (T, E), the new tokens of sequences whose heads a
         qlka.paged.PagedCache of num_heads key heads holds, one each without offsets. Their own heads are written there,
         then each attends to its sequence up to itself. No gradient (call it under torch.no_grad())."""
@@ -130,7 +131,8 @@ class KernelMultiheadAttention(nn.Module):
     def _rows(self, x, offsets, cache, causal):
         """forward of rows (T, E) without padding."""
         if self.kernel != "softmax" or self.position_bias is not None:
-            raise NotImplementedError("packed sequences and a cache in pages run on the 'softmax' kernel without a position bias")
+            raise NotImplementedError("packed sequences and a cache in pages run on the 'softmax' kernel without a "
+                                      "position bias")
         if x.dim() != 2:
             raise ValueError(f"packed rows must be (T, E), got {tuple(x.shape)}")
         q, k, v = (heads[0] for heads in self.split_heads(x[None]))                 # (H, T, Dh)

@@ -1,4 +1,4 @@
-"""CPU checks of csrc/paged_cut.h, by which kernels find pages and cut the work of attention over them, each for itself."""
+"""CPU checks of csrc/paged_cut.h, by which kernels find pages and cut the work of attention over them."""
 
 import os
 import subprocess
@@ -46,7 +46,8 @@ int main() {
 def run(tmp_path, source, name, *flags):
     src, exe = tmp_path / f"{name}.hip", tmp_path / name
     src.write_text(source)
-    subprocess.run([HIPCC, "--offload-host-only", "-std=c++17", "-O2", *flags, f"-I{CSRC}", str(src), "-o", str(exe)], check=True)
+    subprocess.run([HIPCC, "--offload-host-only", "-std=c++17", "-O2", *flags, f"-I{CSRC}", str(src), "-o", str(exe)],
+                   check=True)
     done = subprocess.run([str(exe)], capture_output=True, text=True)
     assert done.returncode == 0, done.stdout + done.stderr
     return done.stdout.split()

@@ -1,5 +1,6 @@
-"""CPU checks of how workgroups find their sequences and rows (csrc/segments.h, csrc/paged_cut.h): every row of a valid call in
-one block, positions in their pages, and no row, group, page or place outside the call's, whatever offsets and lengths are."""
+"""CPU checks of how workgroups find their sequences and rows (csrc/segments.h, csrc/paged_cut.h): every row of a valid
+call in one block, positions in their pages, and no row, group, page or place outside the call's, whatever offsets and
+lengths are."""
 
 from test_paged_cut import run
 
@@ -41,7 +42,8 @@ int main() {
             for (int r = s.block * rows; r < s.rows && r < (s.block + 1) * rows; ++r) {
                 ++seen[s.first + r];
                 if (r % 32 == 0) ++groups.at(group + r / 32);
-                if (s.index >= 0 && s.index < B) CHECK(s.first == at[s.index] && s.rows == at[s.index + 1] - at[s.index]);
+                if (s.index >= 0 && s.index < B)
+                    CHECK(s.first == at[s.index] && s.rows == at[s.index + 1] - at[s.index]);
             }
         }
         for (int n : seen) CHECK(n == 1);
@@ -55,7 +57,8 @@ int main() {
             const int x = below(at[count - 1] + 3);
             int want = 0;
             for (int j = 0; j < count; ++j) if (at[j] <= x) want = j;
-            CHECK(last_upto(count, x, [&](int j) { if (j < 0 || j >= count) std::abort(); return at[j]; }, OnHost()) == want);
+            const auto get = [&](int j) { if (j < 0 || j >= count) std::abort(); return at[j]; };
+            CHECK(last_upto(count, x, get, OnHost()) == want);
         }
     std::puts("ok");
     return 0;
