@@ -11,8 +11,9 @@
 // The waves wait for 34 to 50% of their cycles, for the next tile and for each other. Measured: 12 x 8192 x 8192 of 64
 // with the table's gradient, bf16: softmax_dq 491 us (630 TFLOP/s), softmax_dkv 533 us (773); fp32, 32 x 4 heads of 600
 // to 65: 41 and 42 us; bf16 of 128, 2 x 8 x 2048 x 2048: 257 us with the forward; packed sequences, 12 of 256 to 8192,
-// 12 heads, causal, bf16: 520 and 703 us (786 and 775 TFLOP/s of what is visible). Registers are short: at fp32 of 64
-// elements and more, and at bf16 of 128, some values live in scratch memory.
+// 12 heads, causal, bf16: 485 to 520 and 673 to 703 us (786 to 843 and 775 to 810 TFLOP/s of what is visible). Registers
+// are short: at fp32 of 64 elements and more, and at bf16 of 128, some values live in scratch memory (softmax_dkv of
+// packed bf16 rows of 128: 320 to 348 bytes a lane).
 #include "softmax_tile.h"
 
 #include <limits>
